@@ -139,7 +139,7 @@ psgd_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           const uint64_t a_desc = A_MN ? make_smem_desc(a_addr + kk * 2048, kABytes / 2, 1024)
                                        : make_smem_desc(a_addr + kk * 32, 16, 1024);
           const uint64_t b_desc = make_smem_desc(b_addr + kk * 32, 16, 1024);
-          umma_bf16(tmem_base, a_desc, b_desc, idesc, (i > 0 || kk > 0) ? 1u : 0u);
+          umma_f16(tmem_base, a_desc, b_desc, idesc, (i > 0 || kk > 0) ? 1u : 0u);
         }
         umma_commit(&empty[s]);  // frees the stage once these MMAs have read it
       }

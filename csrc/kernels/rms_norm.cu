@@ -1,0 +1,544 @@
+// RMS norm of rows, with the residual's addition before it, with its gradients, and with an output in 8 bits.
+//
+//   h = x + r (rounded to the rows' type, as a sum of its own would be),   rstd = (mean(h^2) + eps)^-1/2,   y = h rstd w
+//   8 bits: f = h rstd w in fp32; scale = max |f| / 448 over the row or over 128 columns; q = e4m3(f / scale)
+//   xhat = h rstd;   dx = dr = dh + rstd (dy w - xhat mean(dy w xhat));   dw = sum over rows of dy xhat
+//
+// All of it is bound by HBM: every value is read once and written once, and a row stays in the registers of the threads that read it
+// between the sums and the results. A row belongs to a warp, or to a CTA of 128 or 512 threads where it is too long for one. Sums and rstd
+// are fp32 and added up in an order that only the sizes determine. The gradient of the weight is summed in registers by CTAs
+// that walk over the rows, and a second kernel adds up the CTAs' parts in order: no atomics.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <type_traits>
+
+#include "follow.cuh"
+#include "launch_util.cuh"
+#include "nangila_kernels.h"
+#include "nangila_model_kernels.h"
+#include "quant.cuh"
+
+namespace nangila {
+namespace {
+
+constexpr float kE4m3Max = 448.0f;
+constexpr float kMinAmax = 1e-12f;  // a row of zeros gets a scale that can be divided by
+
+template <typename T>
+struct Raw8;  // eight values as they lie in memory
+template <> struct Raw8<float> { uint4 a, b; };
+template <> struct Raw8<__nv_bfloat16> { uint4 a; };
+template <> struct Raw8<__half> { uint4 a; };
+
+__device__ __forceinline__ uint4 load_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void fetch(const T* p, Raw8<T>& r) {
+  r.a = load_stream(p);
+  if constexpr (sizeof(T) == 4) r.b = load_stream(reinterpret_cast<const uint4*>(p) + 1);
+}
+__device__ __forceinline__ void unpack(const Raw8<float>& r, float (&v)[8]) {
+  const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+}
+__device__ __forceinline__ void unpack(const Raw8<__nv_bfloat16>& r, float (&v)[8]) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack(const Raw8<__half>& r, float (&v)[8]) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void pack(const float (&v)[8], Raw8<float>& r) {
+  r.a = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  r.b = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+}
+__device__ __forceinline__ void pack(const float (&v)[8], Raw8<__nv_bfloat16>& r) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  r.a = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void pack(const float (&v)[8], Raw8<__half>& r) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  r.a = make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T>
+__device__ __forceinline__ void put(T* p, const Raw8<T>& r) {
+  *reinterpret_cast<uint4*>(p) = r.a;
+  if constexpr (sizeof(T) == 4) reinterpret_cast<uint4*>(p)[1] = r.b;
+}
+
+// Which columns a thread holds. VEC: runs of eight adjacent ones, 16-byte loads; else one by one, neighbours in neighbouring threads, for
+// rows that start anywhere and end anywhere.
+template <int TPR, bool VEC>
+__device__ __forceinline__ int column(int v, int k, int t) {
+  return VEC ? (v * TPR + t) * 8 + k : (v * 8 + k) * TPR + t;
+}
+template <typename T, int TPR, bool VEC>
+__device__ __forceinline__ void load_row8(const T* row, int v, int t, int d, Raw8<T>& raw) {
+  if constexpr (VEC) {
+    if (column<TPR, VEC>(v, 0, t) < d) fetch(row + column<TPR, VEC>(v, 0, t), raw);
+    else raw = Raw8<T>{};
+  } else {
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int c = column<TPR, VEC>(v, k, t);
+      f[k] = c < d ? dev::Vec16<T>::to_float(row[c]) : 0.0f;
+    }
+    pack(f, raw);
+  }
+}
+template <typename T, int TPR, bool VEC>
+__device__ __forceinline__ void store_row8(T* row, int v, int t, int d, const float (&f)[8]) {
+  if constexpr (VEC) {
+    Raw8<T> raw;
+    pack(f, raw);
+    if (column<TPR, VEC>(v, 0, t) < d) put(row + column<TPR, VEC>(v, 0, t), raw);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int c = column<TPR, VEC>(v, k, t);
+      if (c < d) row[c] = dev::Vec16<T>::from_float(f[k]);
+    }
+  }
+}
+template <int TPR, bool VEC>
+__device__ __forceinline__ void load_weight8(const void* w, int dtype, int v, int t, int d, float (&f)[8]) {
+  if constexpr (VEC) {
+    const int c = column<TPR, VEC>(v, 0, t);
+    if (c >= d) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = 0.0f;
+    } else if (dtype == NANGILA_BF16) {
+      Raw8<__nv_bfloat16> r;
+      r.a = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(w) + c));
+      unpack(r, f);
+    } else if (dtype == NANGILA_F16) {
+      Raw8<__half> r;
+      r.a = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(w) + c));
+      unpack(r, f);
+    } else {
+      Raw8<float> r;
+      r.a = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(w) + c));
+      r.b = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(w) + c) + 1);
+      unpack(r, f);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int c = column<TPR, VEC>(v, k, t);
+      f[k] = c >= d                  ? 0.0f
+             : dtype == NANGILA_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(w)[c])
+             : dtype == NANGILA_F16  ? __half2float(static_cast<const __half*>(w)[c])
+                                     : static_cast<const float*>(w)[c];
+    }
+  }
+}
+
+// The sum over the threads of a row, in all of them. `s`: TPR / 32 floats that nobody else uses, given again only after the row's threads
+// have met in between (the sums of a kernel take turns with two of them).
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (TPR > 32) {
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < TPR / 32; ++i) v += s[i];
+  }
+  return v;
+}
+// The larger of two magnitudes, and not a number where either is not one.
+__device__ __forceinline__ float larger(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+template <int TPR>
+__device__ __forceinline__ float row_max(float v, float* s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = larger(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if constexpr (TPR > 32) {
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = s[0];
+#pragma unroll
+    for (int i = 1; i < TPR / 32; ++i) v = larger(v, s[i]);
+  }
+  return v;
+}
+
+// Threads of a CTA: four rows of a warp each, or one row.
+template <int TPR>
+constexpr int kThreads = TPR < 128 ? 128 : TPR;
+
+template <typename T, int TPR, int NV, bool VEC, bool FP8>
+__global__ void __launch_bounds__(kThreads<TPR>) norm_forward_kernel(const __grid_constant__ NangilaNormParams p) {
+  constexpr int kRows = kThreads<TPR> / TPR;
+  __shared__ float s_sum[TPR > 32 ? TPR / 32 : 1], s_max[TPR > 32 ? TPR / 32 : 1];
+  const int t = threadIdx.x % TPR;
+  const int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / TPR;
+  if (row >= p.rows) return;  // whole warps, or a whole CTA
+  const int d = p.d;
+  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+  Raw8<T> raw[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) load_row8<T, TPR, VEC>(x, v, t, d, raw[v]);
+  if (p.residual != nullptr) {
+    const T* r = static_cast<const T*>(p.residual) + row * p.residual_stride;
+    Raw8<T> more[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) load_row8<T, TPR, VEC>(r, v, t, d, more[v]);
+    T* h = static_cast<T*>(p.h) + row * d;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float a[8], b[8];
+      unpack(raw[v], a);
+      unpack(more[v], b);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) a[k] += b[k];
+      store_row8<T, TPR, VEC>(h, v, t, d, a);
+      pack(a, raw[v]);  // what is normalised is the sum as it is kept
+    }
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    float a[8];
+    unpack(raw[v], a);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum = __fmaf_rn(a[k], a[k], sum);
+  }
+  sum = row_sum<TPR>(sum, s_sum);
+  const float rstd = rsqrtf(__fdiv_rn(sum, float(d)) + p.eps);
+  if (p.rstd != nullptr && t == 0) p.rstd[row] = rstd;
+  if constexpr (!FP8) {
+    T* y = static_cast<T*>(p.y) + row * d;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float a[8], w[8];
+      unpack(raw[v], a);
+      load_weight8<TPR, VEC>(p.weight, p.weight_dtype, v, t, d, w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) a[k] = a[k] * rstd * w[k];
+      store_row8<T, TPR, VEC>(y, v, t, d, a);
+    }
+  } else {
+    uint8_t* q = p.q + row * d;
+    float amax = 0.0f;  // of the row; with groups each run of 16 threads has one of its own below
+    if (p.group == 0) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        float a[8], w[8];
+        unpack(raw[v], a);
+        load_weight8<TPR, VEC>(p.weight, p.weight_dtype, v, t, d, w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) amax = larger(amax, fabsf(a[k] * rstd * w[k]));
+      }
+      amax = row_max<TPR>(amax, s_max);
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float a[8], w[8];
+      unpack(raw[v], a);
+      load_weight8<TPR, VEC>(p.weight, p.weight_dtype, v, t, d, w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) a[k] = a[k] * rstd * w[k];
+      if (p.group != 0) {
+        amax = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) amax = larger(amax, fabsf(a[k]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) amax = larger(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      }
+      // a row or group with a value that is not finite has no scale: all of it is not a number
+      const float scale = amax <= 3.4028234e38f ? __fdiv_rn(fmaxf(amax, kMinAmax), kE4m3Max) : __uint_as_float(0x7fc00000u);
+      const int c0 = column<TPR, VEC>(v, 0, t);
+      if (p.group != 0) {
+        if ((t & 15) == 0 && c0 < d) p.scale[row * (d / 128) + c0 / 128] = scale;
+      } else if (v == 0 && t == 0) {
+        p.scale[row] = scale;
+      }
+      uint32_t word[2] = {0u, 0u};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t byte = scale == scale ? uint32_t(__nv_cvt_float_to_fp8(__fdiv_rn(a[k], scale), __NV_SATFINITE, __NV_E4M3)) : 0x7fu;
+        word[k / 4] |= byte << (8 * (k % 4));
+      }
+      if constexpr (VEC) {
+        if (c0 < d) *reinterpret_cast<uint2*>(q + c0) = make_uint2(word[0], word[1]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int c = column<TPR, VEC>(v, k, t);
+          if (c < d) q[c] = uint8_t(word[k / 4] >> (8 * (k % 4)));
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int TPR, int NV, bool VEC>
+__global__ void __launch_bounds__(kThreads<TPR>) norm_backward_kernel(const __grid_constant__ NangilaNormGradParams p) {
+  constexpr int kRows = kThreads<TPR> / TPR;
+  __shared__ float s_sum[2][TPR > 32 ? TPR / 32 : 1];
+  extern __shared__ float s_dw[];  // d, where a CTA has several rows at a time
+  const int t = threadIdx.x % TPR, mine = threadIdx.x / TPR;
+  const int d = p.d;
+  float acc[NV][8];
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[v][k] = 0.0f;
+  may_follow();
+  int turn = 0;
+  for (int64_t row = int64_t(blockIdx.x) * kRows + mine; row < p.rows; row += int64_t(gridDim.x) * kRows) {
+    Raw8<T> h[NV], g[NV], more[NV];
+    float mean = 0.0f, rstd = 0.0f;
+    if (p.dy != nullptr) {
+      const T* hr = static_cast<const T*>(p.h) + row * p.h_stride;
+      const T* gr = static_cast<const T*>(p.dy) + row * p.dy_stride;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        load_row8<T, TPR, VEC>(hr, v, t, d, h[v]);
+        load_row8<T, TPR, VEC>(gr, v, t, d, g[v]);
+      }
+      rstd = p.rstd[row];
+    }
+    if (p.dh != nullptr && p.dx != nullptr) {
+      const T* dr = static_cast<const T*>(p.dh) + row * p.dh_stride;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) load_row8<T, TPR, VEC>(dr, v, t, d, more[v]);
+    }
+    if (p.dy != nullptr) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        float a[8], b[8], w[8];
+        unpack(h[v], a);
+        unpack(g[v], b);
+        load_weight8<TPR, VEC>(p.weight, p.weight_dtype, v, t, d, w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float unit = a[k] * rstd;
+          acc[v][k] = __fmaf_rn(b[k], unit, acc[v][k]);
+          sum = __fmaf_rn(b[k] * w[k], unit, sum);
+        }
+      }
+      mean = __fdiv_rn(row_sum<TPR>(sum, s_sum[turn]), float(d));
+      turn ^= 1;
+    }
+    if (p.dx != nullptr) {
+      T* dx = static_cast<T*>(p.dx) + row * d;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        float o[8];
+        if (p.dh != nullptr) {
+          unpack(more[v], o);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) o[k] = 0.0f;
+        }
+        if (p.dy != nullptr) {
+          float a[8], b[8], w[8];
+          unpack(h[v], a);
+          unpack(g[v], b);
+          load_weight8<TPR, VEC>(p.weight, p.weight_dtype, v, t, d, w);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) o[k] += rstd * (b[k] * w[k] - a[k] * rstd * mean);
+        }
+        store_row8<T, TPR, VEC>(dx, v, t, d, o);
+      }
+    }
+  }
+  if (p.dw == nullptr) return;
+  // the CTA's part: its rows' sums added up one after the other
+  float* part = p.partial + int64_t(blockIdx.x) * d;
+  if constexpr (kRows == 1) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int c = column<TPR, VEC>(v, k, t);
+        if (c < d) part[c] = acc[v][k];
+      }
+  } else {
+    for (int r = 0; r < kRows; ++r) {
+      if (mine == r) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int c = column<TPR, VEC>(v, k, t);
+            if (c < d) s_dw[c] = r == 0 ? acc[v][k] : s_dw[c] + acc[v][k];
+          }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < d; c += kThreads<TPR>) part[c] = s_dw[c];
+  }
+}
+
+// dw: 32 columns of a CTA, 16 threads for each add up every sixteenth part in order, then the sixteen in order.
+constexpr int kDwY = 16;
+__global__ void __launch_bounds__(32 * kDwY) norm_dw_kernel(const float* partial, int parts, int d, void* dw, int dtype) {
+  __shared__ float s[kDwY][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + x;
+  follow();
+  float sum = 0.0f;
+  if (c < d) {
+#pragma unroll 8
+    for (int i = y; i < parts; i += kDwY) sum += partial[int64_t(i) * d + c];
+  }
+  s[y][x] = sum;
+  __syncthreads();
+  if (y == 0 && c < d) {
+#pragma unroll
+    for (int i = 1; i < kDwY; ++i) sum += s[i][x];
+    if (dtype == NANGILA_BF16) static_cast<__nv_bfloat16*>(dw)[c] = __float2bfloat16_rn(sum);
+    else if (dtype == NANGILA_F16) static_cast<__half*>(dw)[c] = __float2half_rn(sum);
+    else static_cast<float*>(dw)[c] = sum;
+  }
+}
+
+template <typename F>
+int by_type(int dtype, const F& f) {
+  switch (dtype) {
+    case NANGILA_F32: return f(float{});
+    case NANGILA_F16: return f(__half{});
+    case NANGILA_BF16: return f(__nv_bfloat16{});
+    default: return int(cudaErrorInvalidValue);
+  }
+}
+template <int A, int B>
+struct Shape {
+  static constexpr int tpr = A, nv = B;
+};
+// Threads for a row, and runs of eight columns for a thread: the fewest threads that hold the row in 8 runs each.
+template <typename F>
+int by_width(int d, const F& f) {
+  const int units = (d + 7) / 8;
+  if (units <= 64) return f(Shape<32, 2>{});
+  if (units <= 128) return f(Shape<32, 4>{});
+  if (units <= 256) return f(Shape<32, 8>{});
+  if (units <= 512) return f(Shape<128, 4>{});
+  if (units <= 1024) return f(Shape<128, 8>{});
+  if (units <= 2048) return f(Shape<512, 4>{});
+  return f(Shape<512, 8>{});
+}
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <typename T, int TPR, int NV, bool VEC>
+int backward_ctas(int64_t rows, int d, int* ctas, size_t* smem) {
+  constexpr int kRows = kThreads<TPR> / TPR;
+  *smem = kRows > 1 ? size_t(d) * 4 : 0;
+  int resident = 0;
+  // (asked for the longest row of this shape, so that the answer depends on the kernel alone)
+  const cudaError_t e = resident_ctas(reinterpret_cast<const void*>(norm_backward_kernel<T, TPR, NV, VEC>), kThreads<TPR>,
+                                      kRows > 1 ? size_t(TPR) * NV * 8 * 4 : 0, &resident);
+  if (e != cudaSuccess) return int(e);
+  *ctas = int(std::max<int64_t>(1, std::min<int64_t>((rows + kRows - 1) / kRows, resident)));
+  return 0;
+}
+
+}  // namespace
+}  // namespace nangila
+
+extern "C" int nangila_rms_norm_forward(const NangilaNormParams* p, cudaStream_t stream) {
+  using namespace nangila;
+  if (!p || !p->x || !p->weight || p->rows < 1 || p->d < 1 || p->d > NANGILA_NORM_MAX_D || (p->residual != nullptr && p->h == nullptr) ||
+      (p->q == nullptr ? p->y == nullptr : p->scale == nullptr) || (p->group != 0 && (p->group != 128 || p->d % 128 != 0)) || p->weight_dtype < 0 ||
+      p->weight_dtype > 2)
+    return int(cudaErrorInvalidValue);
+  const bool vec = p->d % 8 == 0 && p->x_stride % 8 == 0 && p->residual_stride % 8 == 0 && aligned(p->x) && aligned(p->residual) && aligned(p->weight) &&
+                   aligned(p->h) && aligned(p->y) && aligned(p->q);
+  if (p->group != 0 && !vec) return int(cudaErrorMisalignedAddress);
+  return by_type(p->dtype, [&](auto type) {
+    using T = decltype(type);
+    return by_width(p->d, [&](auto shape) {
+      using S = decltype(shape);
+      constexpr int kT = kThreads<S::tpr>, kRows = kT / S::tpr;
+      const int64_t ctas = (p->rows + kRows - 1) / kRows;
+      if (ctas > 0x7fffffff) return int(cudaErrorInvalidValue);
+      auto* kernel = p->q != nullptr ? (vec ? norm_forward_kernel<T, S::tpr, S::nv, true, true> : norm_forward_kernel<T, S::tpr, S::nv, false, true>)
+                                     : (vec ? norm_forward_kernel<T, S::tpr, S::nv, true, false> : norm_forward_kernel<T, S::tpr, S::nv, false, false>);
+      kernel<<<unsigned(ctas), kT, 0, stream>>>(*p);
+      return int(cudaGetLastError());
+    });
+  });
+}
+
+extern "C" int nangila_rms_norm_partials(int64_t rows, int32_t d, int32_t dtype, int32_t* count) {
+  using namespace nangila;
+  if (!count || rows < 1 || d < 1 || d > NANGILA_NORM_MAX_D) return int(cudaErrorInvalidValue);
+  return by_type(dtype, [&](auto type) {
+    using T = decltype(type);
+    return by_width(d, [&](auto shape) {
+      using S = decltype(shape);
+      int a = 0, b = 0;
+      size_t smem = 0;
+      int e = backward_ctas<T, S::tpr, S::nv, true>(rows, d, &a, &smem);
+      if (e == 0) e = backward_ctas<T, S::tpr, S::nv, false>(rows, d, &b, &smem);
+      *count = std::max(a, b);
+      return e;
+    });
+  });
+}
+
+extern "C" int nangila_rms_norm_backward(const NangilaNormGradParams* p, cudaStream_t stream) {
+  using namespace nangila;
+  if (!p || !p->weight || p->rows < 1 || p->d < 1 || p->d > NANGILA_NORM_MAX_D || (p->dy != nullptr && (!p->h || !p->rstd)) || (p->dw != nullptr && !p->partial) ||
+      p->weight_dtype < 0 || p->weight_dtype > 2)
+    return int(cudaErrorInvalidValue);
+  const bool vec = p->d % 8 == 0 && p->h_stride % 8 == 0 && p->dy_stride % 8 == 0 && p->dh_stride % 8 == 0 && aligned(p->h) && aligned(p->dy) && aligned(p->dh) &&
+                   aligned(p->weight) && aligned(p->dx);
+  return by_type(p->dtype, [&](auto type) {
+    using T = decltype(type);
+    return by_width(p->d, [&](auto shape) {
+      using S = decltype(shape);
+      constexpr int kT = kThreads<S::tpr>;
+      auto run = [&](auto how) {
+        constexpr bool VEC = decltype(how)::value;
+        int ctas = 0;
+        size_t smem = 0;
+        if (const int e = backward_ctas<T, S::tpr, S::nv, VEC>(p->rows, p->d, &ctas, &smem)) return e;
+        norm_backward_kernel<T, S::tpr, S::nv, VEC><<<unsigned(ctas), kT, smem, stream>>>(*p);
+        if (const cudaError_t e = cudaGetLastError()) return int(e);
+        if (p->dw == nullptr) return 0;
+        return int(launch_following(norm_dw_kernel, dim3(unsigned((p->d + 31) / 32)), 32 * kDwY, 0, stream, static_cast<const float*>(p->partial), ctas, int(p->d),
+                                    static_cast<void*>(p->dw), int(p->weight_dtype)));
+      };
+      return vec ? run(std::true_type{}) : run(std::false_type{});
+    });
+  });
+}

@@ -1,7 +1,10 @@
 """Device operations of the framework as plain functions over torch tensors.
 
-Each function is a thin wrapper over one hand-written sm_100a kernel (``nangila._cuda``); the fused
+Each function is a thin wrapper over hand-written sm_100a kernels (``nangila._cuda``); the fused
 exchange kernels are driven through the engines in ``nangila.parallel`` instead.
 """
+from .muon import muon_step, orthogonalize  # noqa: F401
 from .reductions import absmax_percentile, crc32, quantizer_gamma, state_hash  # noqa: F401
+from .norm import add_rms_norm, rms_norm, rms_norm_fp8  # noqa: F401
+from .positions import rotary, rotary_table  # noqa: F401
 from .sculptor_stats import DeviceSculptor  # noqa: F401

@@ -1,0 +1,162 @@
+"""Updates made orthogonal by Newton-Schulz steps, and the Muon step on them (``csrc/kernels/orthogonalize.cu``).
+
+With ``X = U / max(|U|, eps)`` (Frobenius norm), each step takes ``A = X X^T`` on the shorter side and ``X <- a X + (b A + c A^2) X``, which moves
+every singular value towards one. The products' operands are float16, accumulated in float32, and X is kept to 22 bits between the steps: with
+the default coefficients the result is within about 1e-3 (relative, 2-norm) of the formula in exact arithmetic. CPU tensors take the
+formula in float32.
+"""
+from __future__ import annotations
+
+import math
+from typing import Dict, List, Sequence, Tuple, Union
+
+import torch
+
+from .reductions import _glue
+
+#: Moves singular values from 1e-3 to 1 into about 0.7 to 1.2 within five steps.
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+MAX_STEPS = 32
+SCALES = ("spectral", "rms", None)
+_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+_Coefficients = Union[Tuple[float, float, float], Sequence[Tuple[float, float, float]]]
+
+
+def _schedule(steps: int, coefficients: _Coefficients) -> List[float]:
+    if not 1 <= steps <= MAX_STEPS:
+        raise ValueError(f"nangila: steps must be 1 to {MAX_STEPS}, got {steps}")
+    rows = list(coefficients)
+    if len(rows) == 3 and all(isinstance(v, (int, float)) for v in rows):
+        rows = [tuple(rows)] * steps
+    if len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise ValueError(f"nangila: coefficients must be three numbers, or three for each of the {steps} steps")
+    flat = [float(v) for r in rows for v in r]
+    if not all(math.isfinite(v) for v in flat):
+        raise ValueError("nangila: coefficients must be finite")
+    return flat
+
+
+def _check_matrix(t: torch.Tensor, name: str) -> None:
+    if not isinstance(t, torch.Tensor) or type(t).__name__ == "DTensor":
+        raise TypeError(f"nangila: {name} must be plain tensors (a sharded matrix has to be gathered first), got {type(t).__name__}")
+    if t.dtype not in _TYPES or t.layout != torch.strided or t.device.type not in ("cuda", "cpu"):
+        raise TypeError(f"nangila: {name} must be dense float32, float16 or bfloat16 CUDA or CPU tensors, got {t.dtype} on {t.device}")
+    if t.dim() != 2 or not 1 <= t.size(0) <= 65536 or not 1 <= t.size(1) <= 65536:
+        raise ValueError(f"nangila: {name} must be matrices of 1 x 1 to 65536 x 65536, got shape {tuple(t.shape)}")
+
+
+def _check_eps(eps: float) -> None:
+    if not (math.isfinite(eps) and eps > 0):
+        raise ValueError(f"nangila: eps must be positive, got {eps}")
+
+
+def _plain(u: torch.Tensor, flat: List[float], eps: float) -> torch.Tensor:
+    """The formula in float32."""
+    x = u.float()
+    x = x / torch.linalg.vector_norm(x).clamp(min=eps)
+    tall = x.size(0) > x.size(1)
+    x = x.mT if tall else x
+    for i in range(0, len(flat), 3):
+        gram = x @ x.mT
+        x = flat[i] * x + (flat[i + 1] * gram + flat[i + 2] * (gram @ gram)) @ x
+    return x.mT if tall else x
+
+
+@torch.no_grad()
+def orthogonalize(update: Union[torch.Tensor, Sequence[torch.Tensor]], steps: int = 5, coefficients: _Coefficients = COEFFICIENTS,
+                  eps: float = 1e-7) -> Union[torch.Tensor, List[torch.Tensor]]:
+    """``update`` with its singular values moved towards one, in bfloat16 (the accuracy of the steps warrants no more). A matrix, a stack
+    ``[count, rows, cols]``, or a list of matrices of any shapes, types and devices: those that agree go through the kernels together, and
+    their results share one allocation. ``coefficients``: ``(a, b, c)``, or one such triple for each step; they have to keep the singular values
+    below about two. No gradient flows through it."""
+    flat = _schedule(steps, coefficients)
+    _check_eps(eps)
+    if isinstance(update, torch.Tensor):
+        if update.dim() == 3 and update.size(0) == 0:
+            _check_matrix(update.new_empty(update.shape[1:]), "updates")
+            return update.new_empty(update.shape, dtype=torch.bfloat16)
+        many = list(update.unbind(0)) if update.dim() == 3 else [update]
+        for t in many:
+            _check_matrix(t, "updates")
+        if update.is_cuda:
+            out = _glue().orth([t.contiguous() for t in many], [], [], flat, eps)
+        else:
+            out = torch.stack([_plain(t, flat, eps).to(torch.bfloat16) for t in many])
+        return out if update.dim() == 3 else out[0]
+    many = list(update)
+    for t in many:
+        _check_matrix(t, "updates")
+    groups: Dict[tuple, List[int]] = {}
+    for i, t in enumerate(many):
+        groups.setdefault((t.shape, t.dtype, t.device), []).append(i)
+    results: List[torch.Tensor] = [None] * len(many)  # type: ignore[list-item]
+    for (_, _, device), members in groups.items():
+        if device.type == "cuda":
+            stack = _glue().orth([many[i].contiguous() for i in members], [], [], flat, eps).unbind(0)
+        else:
+            stack = [_plain(many[i], flat, eps).to(torch.bfloat16) for i in members]
+        for i, t in zip(members, stack):
+            results[i] = t
+    return results
+
+
+def update_scale(rows: int, cols: int, scale: Union[str, None]) -> float:
+    """What a ``rows x cols`` update is multiplied by: ``"spectral"``: ``sqrt(max(1, rows / cols))``; ``"rms"``: ``0.2 sqrt(max(rows, cols))``, the size of
+    an AdamW update, so that its learning rate and weight decay carry over; None: 1."""
+    if scale == "spectral":
+        return math.sqrt(max(1.0, rows / cols))
+    if scale == "rms":
+        return 0.2 * math.sqrt(max(rows, cols))
+    if scale is None:
+        return 1.0
+    raise ValueError(f"nangila: scale must be one of {SCALES}, got {scale!r}")
+
+
+@torch.no_grad()
+def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor], lr: float, momentum: float = 0.95,
+              nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5, coefficients: _Coefficients = COEFFICIENTS, eps: float = 1e-7,
+              scale: Union[str, None] = "rms") -> None:
+    """One Muon step in place, for matrices of any shapes::
+
+        momenta <- momentum * momenta + grads
+        update   = orthogonalize(grads + momentum * momenta)      (momenta alone without nesterov)
+        params  <- params * (1 - lr * weight_decay) - lr * update_scale * update
+
+    ``momenta`` are float32 (zeros before the first step). Everything is packed; no two of ``params`` and ``momenta`` share memory, with one another
+    or with ``grads``. Matrices of one shape and type go through the kernels together; the parameters are updated in the last product's epilogue.
+    ``lr`` and the others are plain numbers: a captured CUDA graph keeps the ones that it was captured with."""
+    flat = _schedule(steps, coefficients)
+    _check_eps(eps)
+    for name, v in (("lr", lr), ("momentum", momentum), ("weight_decay", weight_decay)):
+        if not (math.isfinite(v) and v >= 0):
+            raise ValueError(f"nangila: {name} must be finite and not negative, got {v}")
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    if not len(params) == len(grads) == len(momenta):
+        raise ValueError(f"nangila: {len(params)} parameters, {len(grads)} gradients and {len(momenta)} momenta")
+    groups: Dict[tuple, List[int]] = {}
+    for i, (p, g, m) in enumerate(zip(params, grads, momenta)):
+        for t, name in ((p, "parameters"), (g, "gradients"), (m, "momenta")):
+            _check_matrix(t, name)
+        if not p.shape == g.shape == m.shape or not p.device == g.device == m.device:
+            raise ValueError(f"nangila: parameter {i} is {tuple(p.shape)} on {p.device}, its gradient {tuple(g.shape)} on {g.device}, "
+                             f"its momentum {tuple(m.shape)} on {m.device}")
+        if m.dtype != torch.float32:
+            raise TypeError(f"nangila: momenta must be float32, got {m.dtype}")
+        if not p.is_contiguous() or not m.is_contiguous():
+            raise ValueError(f"nangila: parameter {i} and its momentum must be packed (contiguous)")
+        groups.setdefault((p.shape, p.dtype, g.dtype, p.device), []).append(i)
+    update_scale(1, 1, scale)
+    if _glue().overlapping(params + momenta, grads):
+        raise ValueError("nangila: parameters and momenta must not share memory with one another or with the gradients")
+    for (shape, _, _, device), members in groups.items():
+        rate, decay = lr * update_scale(shape[0], shape[1], scale), 1.0 - lr * weight_decay
+        if device.type == "cuda":
+            _glue().orth([grads[i].contiguous() for i in members], [momenta[i] for i in members], [params[i] for i in members], flat, eps, momentum, nesterov,
+                         decay, rate)
+            # the kernels write where autograd does not look: what was saved for a backward pass is not what it was
+            torch.autograd.graph.increment_version([t for i in members for t in (params[i], momenta[i]) if not t.is_inference()])
+            continue
+        for i in members:
+            momenta[i].mul_(momentum).add_(grads[i])
+            u = momenta[i] * momentum + grads[i] if nesterov else momenta[i]
+            params[i].copy_(params[i].float() * decay - rate * _plain(u, flat, eps))
