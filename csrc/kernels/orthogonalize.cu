@@ -36,65 +36,61 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kTileM = 128;
+constexpr int kTileM = 128;                      // rows of a CTA
 constexpr int kSlabK = 64;                       // one 128-byte swizzle row of fp16
-constexpr int kABytes = kTileM * kSlabK * 2;
-constexpr int kGemmThreads = 192;                // warp 0: TMA, warp 1: products, warps 2 to 5: epilogue
+constexpr int kOperandBytes = 128 * kSlabK * 2;  // what a CTA holds of an operand's slab
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kStages = 5;
+constexpr int kChunk = 64;                       // columns that a warp of the epilogue takes at a time
+constexpr int kBoxBytes = 32 * kChunk * 2;       // 32 rows of them in fp16
+constexpr int kSlotBytes = 2 * kBoxBytes;        // what comes in and goes out at a time, in place
+constexpr int kEpilogueWarps = 4;
+constexpr int kEpilogueBytes = kEpilogueWarps * 2 * kSlotBytes;
+constexpr int kSmem = kStages * kStageBytes + kEpilogueBytes + 1024 + 256;
+constexpr int kGemmThreads = 64 + 32 * kEpilogueWarps;  // warp 0: TMA, warp 1: products, the others: epilogue
 constexpr uint64_t kTimeoutNs = 10ull * 1000 * 1000 * 1000;
 constexpr float kLoScale = 2048.0f;
-template <int TN>
-struct Tile {
-  static constexpr int kBBytes = TN * kSlabK * 2;
-  static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = 196608 / kStageBytes;         // 4 or 6
-  static constexpr int kSmem = kStages * kStageBytes + 1024 + 256;
-};
 
 enum Kind { kGram, kPoly, kUpdate, kFinal };
 
 struct Product {
   int M, N, K;             // D is M x N
-  int tiles_m, tiles_n, per, total;  // tiles of one matrix, of all
+  int tiles_m, per, total; // tiles along M; tiles of one matrix, of all
   int lower;               // only tiles that reach the lower triangle
   float alpha, beta;       // gram: D alpha;  poly: alpha A + beta D;  update: alpha X + D
   float unscale;           // final: result = (alpha X + D) unscale
-  const __half* in;        // poly: A;  update: hi
-  __half* lo;              // update: read and written in place
-  __half* out;             // gram, poly, update
-  int64_t ld, matrix;      // of `in`, `lo` and `out`, in elements
   __nv_bfloat16* result;   // final: packed M x N, or NULL
-  int param_dtype, vector; // final: the parameters' type; runs of eight elements can be written
+  int param_dtype, vector; // final: the parameters' type; runs of four elements can be read and written
   float decay, rate;
   void* param[NANGILA_ORTH_MAX_COUNT];
+};
+struct Maps {
+  CUtensorMap a, b;        // the operands
+  CUtensorMap in, lo;      // poly: A;  update and final: hi and lo
+  CUtensorMap out, mirror; // gram, poly: the result and its other half;  update: hi (lo goes back where it came from)
 };
 
 struct TileAt {
   int batch, m0, n0;
 };
-template <int TN>
+// Square tiles of SIDE x SIDE.
+template <int SIDE>
 __device__ __forceinline__ TileAt tile_at(const Product& p, int i) {
   TileAt t;
   t.batch = i / p.per;
-  int r = i - t.batch * p.per;
+  const int r = i - t.batch * p.per;
   int rb, cb;
   if (!p.lower) {
     cb = r / p.tiles_m;  // neighbours share the columns of the wide operand
     rb = r - cb * p.tiles_m;
-  } else if (TN == 128) {
+  } else {
     rb = int((sqrtf(8.0f * r + 1.0f) - 1.0f) * 0.5f);
     while (rb * (rb + 1) / 2 > r) --rb;
     while ((rb + 1) * (rb + 2) / 2 <= r) ++rb;
     cb = r - rb * (rb + 1) / 2;
-  } else {  // two rows of tiles at a time, with h + 1 tiles each
-    int h = int((sqrtf(4.0f * r + 1.0f) - 1.0f) * 0.5f);
-    while (h * (h + 1) > r) --h;
-    while ((h + 1) * (h + 2) <= r) ++h;
-    r -= h * (h + 1);
-    rb = 2 * h + (r > h ? 1 : 0);
-    cb = r > h ? r - h - 1 : r;
   }
-  t.m0 = rb * kTileM;
-  t.n0 = cb * TN;
+  t.m0 = rb * SIDE;
+  t.n0 = cb * SIDE;
   return t;
 }
 
@@ -125,121 +121,177 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4& hi, uint4& lo
   for (int k = 0; k < 8; ++k) l[k] = (x[k] - h[k]) * kLoScale;
   lo = pack8(l);
 }
-template <typename T>
-__device__ __forceinline__ void update_param(T* p, int n, bool vector, const float (&r)[8], float decay, float rate) {
-  if (vector) {
-    float v[8];
-    dev::Vec8<T>::load(p, v);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = v[k] * decay - rate * r[k];
-    dev::Vec8<T>::store(p, v);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < n) p[k] = dev::Vec16<T>::from_float(dev::Vec16<T>::to_float(p[k]) * decay - rate * r[k]);
-  }
-}
+// Sixteen bytes `j` of a lane's row in a box of 32 rows of 128 bytes, as TMA swizzles them (the box starts on 1024 bytes).
+__device__ __forceinline__ uint4* box_at(uint8_t* box, int row, int j) { return reinterpret_cast<uint4*>(box + row * 128 + ((j ^ (row & 7)) << 4)); }
 
-// Eight results of one row, D[row][col .. col + 7], taken to where they belong. The row is inside the matrix, col < N.
-template <int KIND>
-__device__ __forceinline__ void finish8(const Product& p, int batch, int row, int col, float (&v)[8]) {
-  const int64_t at = batch * p.matrix + int64_t(row) * p.ld + col;
-  if constexpr (KIND == kGram || KIND == kPoly) {
-    if (col > row) return;  // the other half is written from below the diagonal
-    if constexpr (KIND == kGram) {
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float (&v)[4]);
+template <>
+__device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
+  const float4 a = *reinterpret_cast<const float4*>(p);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+}
+template <>
+__device__ __forceinline__ void load4(const __half* p, float (&v)[4]) {
+  const uint2 a = *reinterpret_cast<const uint2*>(p);
+  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a.x)), y = __half22float2(*reinterpret_cast<const __half2*>(&a.y));
+  v[0] = x.x; v[1] = x.y; v[2] = y.x; v[3] = y.y;
+}
+template <>
+__device__ __forceinline__ void load4(const __nv_bfloat16* p, float (&v)[4]) {
+  const uint2 a = *reinterpret_cast<const uint2*>(p);
+  v[0] = __uint_as_float(a.x << 16); v[1] = __uint_as_float(a.x & 0xffff0000u); v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
+}
+__device__ __forceinline__ void store4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store4(__half* p, const float (&v)[4]) {
+  const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&v)[4]) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+// A warp's 32 rows of results in a slot, fp32, taken to the parameters (T) or, with `fresh`, out. Two rows at a time, four columns a lane; the loads of
+// sixteen rows are on their way before the first store.
+template <typename T, bool fresh>
+__device__ __forceinline__ void put_results(const Product& p, T* base, uint8_t* slot, int lane, int row0, int col0) {
+  const int x = lane & 15, col = col0 + 4 * x, left = p.N - col;
+  if (left <= 0) return;
+  // four columns 4 x: group x / 4 of sixteen, its quarter x % 4
+  uint8_t* box = slot + ((x & 2) ? kBoxBytes : 0);
+  const int j = 2 * (x >> 2) + (x & 1);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= p.alpha;
-    } else {
-      float a[8];
-      unpack8(*reinterpret_cast<const uint4*>(p.in + at), a);
+  for (int half = 0; half < 32; half += 16) {
+    float v[8][4];
+    if (!fresh) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = __fmaf_rn(p.alpha, a[k], p.beta * v[k]);
-    }
-    __half* mirror = p.out + batch * p.matrix + int64_t(col) * p.ld + row;
-    if (col + 7 <= row) {
-      *reinterpret_cast<uint4*>(p.out + at) = pack8(v);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (col + k <= row) p.out[at + k] = __float2half_rn(v[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (col + k < row) mirror[k * p.ld] = __float2half_rn(v[k]);
-  } else {
-    float hi[8], lo[8];
-    unpack8(*reinterpret_cast<const uint4*>(p.in + at), hi);
-    unpack8(*reinterpret_cast<const uint4*>(p.lo + at), lo);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = __fmaf_rn(p.alpha, __fmaf_rn(lo[k], 1.0f / kLoScale, hi[k]), v[k]);
-    if constexpr (KIND == kUpdate) {
-      uint4 h, l;
-      split8(v, h, l);
-      *reinterpret_cast<uint4*>(p.out + at) = h;
-      *reinterpret_cast<uint4*>(p.lo + at) = l;
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= p.unscale;
-      const int left = p.N - col;
-      const int64_t to = int64_t(row) * p.N + col;
-      if (p.result != nullptr) {
-        __nv_bfloat16* o = p.result + int64_t(batch) * p.M * p.N + to;
+      for (int i = 0; i < 8; ++i) {
+        const int row = row0 + half + 2 * i + (lane >> 4);
+        if (row >= p.M) continue;
+        const T* from = base + int64_t(row) * p.N + col;
         if (p.vector) {
-          dev::Vec8<__nv_bfloat16>::store(o, v);
+          load4<T>(from, v[i]);
         } else {
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (k < left) o[k] = __float2bfloat16_rn(v[k]);
+          for (int k = 0; k < 4; ++k) v[i][k] = k < left ? dev::Vec16<T>::to_float(from[k]) : 0.0f;
         }
-      } else if (p.param_dtype == NANGILA_F32) {
-        update_param(static_cast<float*>(p.param[batch]) + to, left, p.vector != 0, v, p.decay, p.rate);
-      } else if (p.param_dtype == NANGILA_BF16) {
-        update_param(static_cast<__nv_bfloat16*>(p.param[batch]) + to, left, p.vector != 0, v, p.decay, p.rate);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int at = half + 2 * i + (lane >> 4);
+      if (row0 + at >= p.M) continue;
+      const uint4 raw = *box_at(box, at, j);
+      const float r[4] = {__uint_as_float(raw.x), __uint_as_float(raw.y), __uint_as_float(raw.z), __uint_as_float(raw.w)};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[i][k] = fresh ? r[k] : v[i][k] * p.decay - p.rate * r[k];
+      T* to = base + int64_t(row0 + at) * p.N + col;
+      if (p.vector) {
+        store4(to, v[i]);
       } else {
-        update_param(static_cast<__half*>(p.param[batch]) + to, left, p.vector != 0, v, p.decay, p.rate);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < left) to[k] = dev::Vec16<T>::from_float(v[i][k]);
       }
     }
   }
 }
 
-// D = A B for tiles of kTileM x TN of all matrices, walked over by CTAs that stay. A_MN / B_MN: the operand lies with its rows (columns of B)
-// adjacent in memory, not its K. The accumulators of two tiles share tensor memory: the epilogue of one runs under the products of the next.
+// Sixteen accumulators of a lane's row, columns 16 g to 16 g + 15 of the chunk in the slot, taken into the slot as what goes out.
+template <int KIND>
+__device__ __forceinline__ void into_slot(const Product& p, uint8_t* slot, int lane, int g, float (&v)[16]) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int j = 2 * g + e;
+    float w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = v[8 * e + k];
+    uint4* first = box_at(slot, lane, j);
+    uint4* second = box_at(slot + kBoxBytes, lane, j);
+    if constexpr (KIND == kGram || KIND == kPoly) {
+      if constexpr (KIND == kGram) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] *= p.alpha;
+      } else {
+        float a[8];
+        unpack8(*first, a);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = __fmaf_rn(p.alpha, a[k], p.beta * w[k]);
+      }
+      *first = pack8(w);
+      // the mirror: 64 rows of 32 values, one from each lane
+      __half* t = reinterpret_cast<__half*>(slot + kBoxBytes) + lane;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t[(8 * j + k) * 32] = __float2half_rn(w[k]);
+    } else {
+      float hi[8], lo[8];
+      unpack8(*first, hi);
+      unpack8(*second, lo);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = __fmaf_rn(p.alpha, __fmaf_rn(lo[k], 1.0f / kLoScale, hi[k]), w[k]);
+      if constexpr (KIND == kUpdate) {
+        uint4 h, l;
+        split8(w, h, l);
+        *first = h;
+        *second = l;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[8 * e + k] = w[k] * p.unscale;
+      }
+    }
+  }
+}
+
+// D = A B for square tiles of all matrices, walked over by CTAs that stay (PAIR: pairs of CTAs that share the tensor cores' work on 256 x 256, each
+// with its 128 rows of A, half of B's columns, and 128 rows of the result; else one CTA and 128 x 128). A_MN / B_MN: the operand lies with its rows
+// (columns of B) adjacent in memory, not its K. The accumulators of two tiles share tensor memory: the epilogue of one runs under the
+// products of the next, and what it needs of X or A is on its way before they end. Each of its warps has two slots of shared memory of its own,
+// filled and emptied by TMA, and meets no other warp.
 // A wait that runs out makes every result of this CTA from there on not a number.
-template <int KIND, bool A_MN, bool B_MN, int TN>
-__global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                                                                      const __grid_constant__ Product p) {
-  using T = Tile<TN>;
+template <int KIND, bool A_MN, bool B_MN, bool PAIR>
+__global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p) {
+  constexpr int kSide = PAIR ? 256 : 128;
+  constexpr int kChunks = kSide / kChunk;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + T::kStages * T::kStageBytes);
-  uint64_t* empty = full + T::kStages;
-  uint64_t* acc_full = empty + T::kStages;  // [2]
-  uint64_t* acc_empty = acc_full + 2;       // [2]
-  uint64_t* drained = acc_empty + 2;
+  uint8_t* slots = smem + kStages * kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(slots + kEpilogueBytes);
+  uint64_t* empty = full + kStages;
+  uint64_t* acc_full = empty + kStages;   // [2]
+  uint64_t* acc_empty = acc_full + 2;     // [2]
+  uint64_t* loaded = acc_empty + 2;       // [kEpilogueWarps][2]
+  uint64_t* drained = loaded + 2 * kEpilogueWarps;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile uint32_t* failed = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slabs = (p.K + kSlabK - 1) / kSlabK;
+  const uint32_t rank = PAIR ? cluster_rank() : 0u;   // 0: the CTA that issues the pair's products
+  const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, step = PAIR ? gridDim.x / 2 : gridDim.x;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < T::kStages; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&acc_full[s], 1);
-      mbar_init(&acc_empty[s], 4);
+      mbar_init(&acc_empty[s], kEpilogueWarps * (PAIR ? 2 : 1));
     }
+    for (int s = 0; s < 2 * kEpilogueWarps; ++s) mbar_init(&loaded[s], 1);
     mbar_init(drained, 1);
     *failed = 0;
     fence_barrier_init();
-    prefetch_tensormap(&tmA);
-    prefetch_tensormap(&tmB);
+    prefetch_tensormap(&maps.a);
+    prefetch_tensormap(&maps.b);
   }
-  if (warp == 1) tmem_alloc(tmem_slot, 2 * TN);
+  if (warp == 1) {
+    if (PAIR) tmem_alloc_pair(tmem_slot, 2 * kSide);
+    else tmem_alloc(tmem_slot, 2 * kSide);
+  }
   tc_fence_before_sync();
   __syncthreads();
+  if (PAIR) cluster_sync();  // the other CTA's barriers exist from here on
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   may_follow();
@@ -247,127 +299,188 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __g
 
   if (warp == 0) {
     if (lane == 0) {
-      // ---------------- TMA ----------------
+      // ---------------- TMA: both CTAs of a pair, each its own halves; the bytes are counted where the products are issued ----------------
       int i = 0;  // slabs so far
       bool ok = true;
-      for (int tile = blockIdx.x; tile < p.total && ok; tile += gridDim.x) {
-        const TileAt at = tile_at<TN>(p, tile);
+      for (int tile = first; tile < p.total && ok; tile += step) {
+        const TileAt at = tile_at<kSide>(p, tile);
+        const int row = at.m0 + int(rank) * kTileM, col = at.n0 + int(rank) * 128;
         for (int k = 0; k < slabs; ++k, ++i) {
-          const int s = i % T::kStages;
-          if (i >= T::kStages && !mbar_wait(&empty[s], uint32_t((i / T::kStages - 1) & 1), kTimeoutNs)) {
+          const int s = i % kStages;
+          if (i >= kStages && !mbar_wait(&empty[s], uint32_t((i / kStages - 1) & 1), kTimeoutNs)) {
             *failed = 1;
             ok = false;
             break;
           }
-          uint8_t* a = smem + s * T::kStageBytes;
-          uint8_t* b = a + kABytes;
+          uint8_t* a = smem + s * kStageBytes;
+          uint8_t* b = a + kOperandBytes;
           const int k0 = k * kSlabK;
-          mbar_arrive_expect_tx(&full[s], T::kStageBytes);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], kStageBytes * (PAIR ? 2 : 1));
+          const uint32_t bar = PAIR ? rank0_address(&full[s]) : smem_u32(&full[s]);
           if (A_MN) {
-#pragma unroll
-            for (int g = 0; g < kTileM / 64; ++g) tma_load_3d(a + g * 8192, &tmA, at.m0 + g * 64, k0, at.batch, &full[s]);
+            tma_operand<PAIR>(a, &maps.a, row, k0, at.batch, bar);
+            tma_operand<PAIR>(a + 8192, &maps.a, row + 64, k0, at.batch, bar);
           } else {
-            tma_load_3d(a, &tmA, k0, at.m0, at.batch, &full[s]);
+            tma_operand<PAIR>(a, &maps.a, k0, row, at.batch, bar);
           }
           if (B_MN) {
-#pragma unroll
-            for (int g = 0; g < TN / 64; ++g) tma_load_3d(b + g * 8192, &tmB, at.n0 + g * 64, k0, at.batch, &full[s]);
+            tma_operand<PAIR>(b, &maps.b, col, k0, at.batch, bar);
+            tma_operand<PAIR>(b + 8192, &maps.b, col + 64, k0, at.batch, bar);
           } else {
-            tma_load_3d(b, &tmB, k0, at.n0, at.batch, &full[s]);
+            tma_operand<PAIR>(b, &maps.b, k0, col, at.batch, bar);
           }
         }
       }
-      // the copies that are still under way, if somebody has given up on them
-      if (*failed != 0)
-        for (int j = max(0, i - T::kStages); j < i; ++j) mbar_wait(&full[j % T::kStages], uint32_t((j / T::kStages) & 1), kTimeoutNs);
+      // the copies that are still under way: all have arrived when the products that read them are done; if somebody has given up, as
+      // much as can be waited for (the bytes of a pair are counted by rank 0, the stages of rank 1 are given back by its products)
+      for (int j = max(0, i - kStages); j < i; ++j) {
+        if (*failed == 0 || rank != 0) mbar_wait(&empty[j % kStages], uint32_t((j / kStages) & 1), kTimeoutNs);
+        else mbar_wait(&full[j % kStages], uint32_t((j / kStages) & 1), kTimeoutNs);
+      }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       // ---------------- products ----------------
-      constexpr uint32_t idesc = (1u << 4) | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(TN >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
+      constexpr uint32_t idesc = (1u << 4) | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(kSide >> 3) << 17) | (uint32_t(kSide >> 4) << 24);
       int i = 0, n = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < p.total && ok; tile += gridDim.x, ++n) {
+      for (int tile = first; tile < p.total && ok; tile += step, ++n) {
         const int acc = n & 1;
         if (n >= 2 && !mbar_wait(&acc_empty[acc], uint32_t((n / 2 - 1) & 1), kTimeoutNs)) {
           ok = false;
           break;
         }
         tc_fence_after_sync();
-        const uint32_t d = tmem + uint32_t(acc * TN);
+        const uint32_t d = tmem + uint32_t(acc * kSide);
         for (int k = 0; k < slabs; ++k, ++i) {
-          const int s = i % T::kStages;
-          if (!mbar_wait(&full[s], uint32_t((i / T::kStages) & 1), kTimeoutNs)) {
+          const int s = i % kStages;
+          if (!mbar_wait(&full[s], uint32_t((i / kStages) & 1), kTimeoutNs)) {
             ok = false;
             break;
           }
           tc_fence_after_sync();
-          const uint32_t a = smem_u32(smem + s * T::kStageBytes), b = a + kABytes;
+          const uint32_t a = smem_u32(smem + s * kStageBytes), b = a + kOperandBytes;
 #pragma unroll
           for (int kk = 0; kk < kSlabK / 16; ++kk) {
             // K-major: 16 elements along K are 32 bytes of a swizzle row; MN-major: 16 K-rows are two groups of eight rows of 128 bytes
             const uint64_t ad = A_MN ? make_smem_desc(a + kk * 2048, 8192, 1024) : make_smem_desc(a + kk * 32, 16, 1024);
             const uint64_t bd = B_MN ? make_smem_desc(b + kk * 2048, 8192, 1024) : make_smem_desc(b + kk * 32, 16, 1024);
-            umma_f16(d, ad, bd, idesc, (k > 0 || kk > 0) ? 1u : 0u);
+            if (PAIR) umma_f16_pair(d, ad, bd, idesc, (k > 0 || kk > 0) ? 1u : 0u);
+            else umma_f16(d, ad, bd, idesc, (k > 0 || kk > 0) ? 1u : 0u);
           }
-          umma_commit(&empty[s]);
+          if (PAIR) umma_commit_pair(&empty[s]);
+          else umma_commit(&empty[s]);
         }
-        if (ok) umma_commit(&acc_full[acc]);
+        if (ok) {
+          if (PAIR) umma_commit_pair(&acc_full[acc]);
+          else umma_commit(&acc_full[acc]);
+        }
       }
       if (!ok) {
         *failed = 1;
-        umma_commit(drained);
+        if (PAIR) umma_commit_pair(drained);
+        else umma_commit(drained);
         mbar_wait(drained, 0, kTimeoutNs);
       }
     }
   } else {
     // ---------------- epilogue ----------------
     const int quad = warp & 3;  // the lanes of tensor memory that this warp may read
+    uint8_t* my_slots = slots + (warp - 2) * 2 * kSlotBytes;
+    uint64_t* my_loaded = loaded + (warp - 2) * 2;
+    const uint32_t acc_empty_at = PAIR ? rank0_address(&acc_empty[0]) : smem_u32(&acc_empty[0]);
+    constexpr bool kLoads = KIND != kGram;
+    constexpr uint32_t kLoadBytes = KIND == kPoly ? kBoxBytes : kSlotBytes;
     int n = 0;
-    for (int tile = blockIdx.x; tile < p.total; tile += gridDim.x, ++n) {
-      const TileAt at = tile_at<TN>(p, tile);
+    uint32_t chunks = 0;  // so far
+    for (int tile = first; tile < p.total; tile += step, ++n) {
+      const TileAt at = tile_at<kSide>(p, tile);
       const int acc = n & 1;
+      const int row0 = at.m0 + int(rank) * kTileM + quad * 32;
+      const int mine = row0 < p.M ? min(kChunks, (p.N - at.n0 + kChunk - 1) / kChunk) : 0;
+      auto fetch = [&](int c, uint32_t turn) {  // lane 0: chunk c into the slot whose turn it is, once nothing goes out of it any more
+        uint8_t* slot = my_slots + (turn & 1) * kSlotBytes;
+        bulk_wait_read();
+        mbar_arrive_expect_tx(&my_loaded[turn & 1], kLoadBytes);
+        tma_load_3d(slot, &maps.in, at.n0 + c * kChunk, row0, at.batch, &my_loaded[turn & 1]);
+        if (KIND != kPoly) tma_load_3d(slot + kBoxBytes, &maps.lo, at.n0 + c * kChunk, row0, at.batch, &my_loaded[turn & 1]);
+      };
+      if (kLoads && mine > 0 && lane == 0) fetch(0, chunks);
       bool ok = *failed == 0 && mbar_wait(&acc_full[acc], uint32_t((n / 2) & 1), kTimeoutNs);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) *failed = 1;
       tc_fence_after_sync();
-      const int row = at.m0 + quad * 32 + lane;
 #pragma unroll 1
-      for (int c = 0; c < TN; c += 16) {
-        if (at.n0 + c >= p.N) break;
-        __syncwarp();  // the reads of tensor memory are the whole warp's
-        float v[16];
-        if (ok) {
-          tmem_ld_32x32b_x16(tmem + (uint32_t(quad * 32) << 16) + uint32_t(acc * TN + c), v);
+      for (int c = 0; c < mine; ++c, ++chunks) {
+        uint8_t* slot = my_slots + (chunks & 1) * kSlotBytes;
+        if (kLoads) {
+          if (c + 1 < mine && lane == 0) fetch(c + 1, chunks + 1);
+          const bool here = mbar_wait(&my_loaded[chunks & 1], (chunks >> 1) & 1, kTimeoutNs);
+          if (!__all_sync(0xffffffffu, here)) ok = false;
+          if (!ok) *failed = 1;
         } else {
-#pragma unroll
-          for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(0x7fc00000u);
+          if (lane == 0) bulk_wait_read_but_one();  // this slot's stores; the other's may be under way
+          __syncwarp();
         }
-        if (row < p.M) {
 #pragma unroll
-          for (int g = 0; g < 16; g += 8) {
-            float w[8];
+        for (int g = 0; g < kChunk / 16; ++g) {
+          float v[16];
+          tmem_ld_32x32b_x16(tmem + (uint32_t(quad * 32) << 16) + uint32_t(acc * kSide + c * kChunk + g * 16), v);
+          if (!ok) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = v[g + k];
-            if (at.n0 + c + g < p.N) finish8<KIND>(p, at.batch, row, at.n0 + c + g, w);
+            for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(0x7fc00000u);
+          }
+          into_slot<KIND>(p, slot, lane, g, v);
+          if constexpr (KIND == kFinal) {
+            // columns 16 g and on are 32 bytes of each of the boxes that came in; they are 64 bytes of results, which stay in this lane's rows of both
+            *box_at(slot, lane, 2 * g) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+            *box_at(slot, lane, 2 * g + 1) = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+            *box_at(slot + kBoxBytes, lane, 2 * g) = make_uint4(__float_as_uint(v[8]), __float_as_uint(v[9]), __float_as_uint(v[10]), __float_as_uint(v[11]));
+            *box_at(slot + kBoxBytes, lane, 2 * g + 1) = make_uint4(__float_as_uint(v[12]), __float_as_uint(v[13]), __float_as_uint(v[14]), __float_as_uint(v[15]));
+          }
+        }
+        if constexpr (KIND == kFinal) {
+          __syncwarp();
+          const int col0 = at.n0 + c * kChunk;
+          if (p.result != nullptr) put_results<__nv_bfloat16, true>(p, p.result + int64_t(at.batch) * p.M * p.N, slot, lane, row0, col0);
+          else if (p.param_dtype == NANGILA_F32) put_results<float, false>(p, static_cast<float*>(p.param[at.batch]), slot, lane, row0, col0);
+          else if (p.param_dtype == NANGILA_BF16) put_results<__nv_bfloat16, false>(p, static_cast<__nv_bfloat16*>(p.param[at.batch]), slot, lane, row0, col0);
+          else put_results<__half, false>(p, static_cast<__half*>(p.param[at.batch]), slot, lane, row0, col0);
+          // the slot is filled by TMA again: what was read and written here comes first
+          fence_async_proxy();
+          __syncwarp();
+        } else {
+          fence_async_proxy();
+          __syncwarp();
+          if (lane == 0) {
+            const int col = at.n0 + c * kChunk;
+            tma_store_3d(&maps.out, slot, col, row0, at.batch);
+            if (KIND == kUpdate) tma_store_3d(&maps.lo, slot + kBoxBytes, col, row0, at.batch);
+            else if (at.m0 != at.n0) tma_store_3d(&maps.mirror, slot + kBoxBytes, row0, col, at.batch);
+            bulk_commit();
           }
         }
       }
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[acc]);
+      if (lane == 0) mbar_arrive_at(acc_empty_at + uint32_t(acc) * 8);
     }
+    if (lane == 0) bulk_wait_read();  // the stores have left shared memory; the end of the kernel is what others wait for
   }
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, 2 * TN);
+  if (PAIR) cluster_sync();  // neither CTA's barriers and tensor memory go while the other may still use them
+  if (warp == 1) {
+    if (PAIR) tmem_dealloc_pair(tmem, 2 * kSide);
+    else tmem_dealloc(tmem, 2 * kSide);
+  }
 }
 
 // ---- from the gradients to X -------------------------------------------------------------------------------------------------
 // Two passes over the gradients, which are small next to the products: the sum of squares, in 64 bits and in an order that the sizes determine,
 // then X. With momentum the first pass also advances it: M <- mu M + G, U = G + mu M (Nesterov) or M.
 constexpr int kPrepT = 256;
-constexpr int kMaxChunks = 512;
+constexpr int kMaxChunks = 1024;
 struct Prep {
   const void* grad[NANGILA_ORTH_MAX_COUNT];
   float* momentum[NANGILA_ORTH_MAX_COUNT];
@@ -410,8 +523,16 @@ __global__ void __launch_bounds__(kPrepT) orth_norm_kernel(const __grid_constant
       }
       dev::Vec8<float>::store(m + i * 8, v);
     }
+    // eight squares in fp32 where they fit into its range, else in 64 bits
+    float q = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum = fma(double(u[k]), double(u[k]), sum);
+    for (int k = 0; k < 8; ++k) q = __fmaf_rn(u[k], u[k], q);
+    if (q > 1e-28f && q < 1e38f) {
+      sum += double(q);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum = fma(double(u[k]), double(u[k]), sum);
+    }
   }
   for (int64_t i = runs * 8 + first; i < p.numel; i += stride) {
     float u = dev::Vec16<T>::to_float(g[i]);
@@ -482,21 +603,20 @@ EncodeFn encode_fn() {
   }();
   return fn;
 }
-// count matrices of outer x inner, rows `ld` elements apart, copied in boxes of 64 x box_outer; what lies outside reads as zero
-bool make_map(CUtensorMap* map, const __half* base, int64_t inner, int64_t outer, int64_t ld, int64_t matrix, int count, uint32_t box_outer) {
-  EncodeFn fn = encode_fn();
-  if (!fn) return false;
-  const cuuint64_t dims[3] = {cuuint64_t(inner), cuuint64_t(outer), cuuint64_t(count)};
-  const cuuint64_t strides[2] = {cuuint64_t(ld) * 2, cuuint64_t(matrix) * 2};
-  const cuuint32_t box[3] = {64, box_outer, 1}, step[3] = {1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-struct Matrix {  // an operand as it lies in memory
+struct Matrix {  // `count` matrices as they lie in memory
   const __half* base;
   int64_t rows, cols, ld, matrix;
 };
+// copied in boxes of box_inner x box_outer; what lies outside reads as zero and is not written
+bool make_map(CUtensorMap* map, const Matrix& m, int count, uint32_t box_inner, uint32_t box_outer, bool swizzle = true) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {cuuint64_t(m.cols), cuuint64_t(m.rows), cuuint64_t(count)};
+  const cuuint64_t strides[2] = {cuuint64_t(m.ld) * 2, cuuint64_t(m.matrix) * 2};
+  const cuuint32_t box[3] = {box_inner, box_outer, 1}, step[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(m.base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 int sm_count() {
   static int sms[64] = {};
@@ -505,21 +625,20 @@ int sm_count() {
   if (sms[dev] == 0) cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
   return sms[dev];
 }
+int64_t tiles_of(const Product& p, int side, int count) {
+  const int64_t tm = (p.M + side - 1) / side, tn = (p.N + side - 1) / side;
+  return (p.lower ? tm * (tm + 1) / 2 : tm * tn) * count;
+}
 
-template <int KIND, bool A_MN, bool B_MN, int TN>
-int launch_product(const Matrix& a, const Matrix& b, Product p, int count, cudaStream_t stream) {
-  CUtensorMap ta, tb;
-  if (!make_map(&ta, a.base, a.cols, a.rows, a.ld, a.matrix, count, A_MN ? 64 : kTileM) || !make_map(&tb, b.base, b.cols, b.rows, b.ld, b.matrix, count, B_MN ? 64 : TN))
-    return int(cudaErrorNotSupported);
-  p.tiles_m = (p.M + kTileM - 1) / kTileM;
-  p.tiles_n = (p.N + TN - 1) / TN;
-  p.per = p.tiles_m * p.tiles_n;
-  if (p.lower) {
-    p.per = 0;
-    for (int r = 0; r < p.tiles_m; ++r) p.per += r * kTileM / TN + 1;
-  }
-  p.total = p.per * count;
-  auto* kernel = orth_product_kernel<KIND, A_MN, B_MN, TN>;
+template <int KIND, bool A_MN, bool B_MN, bool PAIR>
+int launch_product(const Maps& maps, Product p, int count, cudaStream_t stream) {
+  constexpr int kSide = PAIR ? 256 : 128;
+  const int64_t total = tiles_of(p, kSide, count);
+  if (total > 0x7fffffff) return int(cudaErrorInvalidValue);
+  p.tiles_m = (p.M + kSide - 1) / kSide;
+  p.total = int(total);
+  p.per = int(total / count);
+  auto* kernel = orth_product_kernel<KIND, A_MN, B_MN, PAIR>;
   static std::mutex mu;
   static uint64_t opted_in = 0;  // by device
   {
@@ -527,21 +646,40 @@ int launch_product(const Matrix& a, const Matrix& b, Product p, int count, cudaS
     if (const cudaError_t e = cudaGetDevice(&dev)) return int(e);
     std::lock_guard<std::mutex> lock(mu);
     if (dev >= 64 || !((opted_in >> dev) & 1)) {
-      if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<TN>::kSmem)) return int(e);
+      if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) return int(e);
       if (dev < 64) opted_in |= uint64_t(1) << dev;
     }
   }
-  return int(launch_following(kernel, dim3(unsigned(std::min(p.total, sm_count()))), kGemmThreads, size_t(Tile<TN>::kSmem), stream, ta, tb, p));
-}
-// 256 columns a tile, or 128 where the wider tiles would leave SMs idle
-template <int KIND, bool A_MN, bool B_MN>
-int product(const Matrix& a, const Matrix& b, const Product& p, int count, cudaStream_t stream) {
-  const int64_t tm = (p.M + kTileM - 1) / kTileM, n128 = (p.N + 127) / 128, n256 = (p.N + 255) / 256;
-  const int64_t narrow = (p.lower ? tm * (tm + 1) / 2 : tm * n128) * count, wide = (p.lower ? (tm / 2) * (tm / 2 + 1) + (tm % 2) * (tm / 2 + 1) : tm * n256) * count;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = PAIR ? 2 : 1;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
   const int sms = sm_count();
-  // a wide tile takes about 1.7 times as long as a narrow one
-  const double cost_narrow = double((narrow + sms - 1) / sms), cost_wide = 1.7 * double((wide + sms - 1) / sms);
-  return cost_wide < cost_narrow ? launch_product<KIND, A_MN, B_MN, 256>(a, b, p, count, stream) : launch_product<KIND, A_MN, B_MN, 128>(a, b, p, count, stream);
+  cfg.gridDim = dim3(unsigned(PAIR ? 2 * std::min(p.total, sms / 2) : std::min(p.total, sms)));
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return int(cudaLaunchKernelEx(&cfg, kernel, maps, p));
+}
+// D of the operands a and b; `in` and `lo` are what the epilogue reads, `out` what it writes.
+template <int KIND, bool A_MN, bool B_MN>
+int product(const Matrix& a, const Matrix& b, const Matrix* in, const Matrix* lo, const Matrix* out, const Product& p, int count, cudaStream_t stream) {
+  Maps maps;
+  bool ok = make_map(&maps.a, a, count, 64, A_MN ? 64 : 128) && make_map(&maps.b, b, count, 64, B_MN ? 64 : 128);
+  ok = ok && make_map(&maps.in, in != nullptr ? *in : a, count, kChunk, 32) && make_map(&maps.lo, lo != nullptr ? *lo : a, count, kChunk, 32);
+  ok = ok && make_map(&maps.out, out != nullptr ? *out : a, count, kChunk, 32) && make_map(&maps.mirror, out != nullptr ? *out : a, count, 32, kChunk, false);
+  if (!ok) return int(cudaErrorNotSupported);
+  // A tile of a pair takes hardly longer than a small one, which is bound by what L2 delivers to an SM (twice the bytes for each product); only its
+  // epilogue is longer. So it is the number of rounds that decides.
+  const int sms = sm_count();
+  const int64_t small = tiles_of(p, 128, count), large = tiles_of(p, 256, count);
+  const double cost_small = double((small + sms - 1) / sms), cost_large = 1.2 * double((large + sms / 2 - 1) / (sms / 2));
+  return cost_large <= cost_small ? launch_product<KIND, A_MN, B_MN, true>(maps, p, count, stream) : launch_product<KIND, A_MN, B_MN, false>(maps, p, count, stream);
 }
 
 struct Layout {
@@ -632,41 +770,31 @@ extern "C" int nangila_orth(const NangilaOrthParams* p, cudaStream_t stream) {
     case NANGILA_BF16: e = start<__nv_bfloat16>(prep, p->count, stream); break;
     default: return int(cudaErrorInvalidValue);
   }
-  const Matrix A{gram, l.m, l.m, l.ldm, l.s}, B{poly, l.m, l.m, l.ldm, l.s};
+  const Matrix A{gram, l.m, l.m, l.ldm, l.s}, B{poly, l.m, l.m, l.ldm, l.s}, Lo{lo, p->rows, p->cols, l.ld, l.x};
   for (int step = 0; step < p->steps && e == 0; ++step) {
     const float* c = p->coefficients[step];
     const bool last = step == p->steps - 1;
-    const Matrix X{hi[step & 1], p->rows, p->cols, l.ld, l.x};
+    const Matrix X{hi[step & 1], p->rows, p->cols, l.ld, l.x}, Next{hi[(step & 1) ^ 1], p->rows, p->cols, l.ld, l.x};
     Product q;
     std::memset(&q, 0, sizeof q);
     q.M = q.N = int(l.m);
     q.lower = 1;
-    q.ld = l.ldm;
-    q.matrix = l.s;
     q.K = int(l.n);
     q.alpha = 1.0f / (scale * scale);
-    q.out = gram;
-    e = tall ? product<kGram, true, true>(X, X, q, p->count, stream) : product<kGram, false, false>(X, X, q, p->count, stream);
+    e = tall ? product<kGram, true, true>(X, X, nullptr, nullptr, &A, q, p->count, stream) : product<kGram, false, false>(X, X, nullptr, nullptr, &A, q, p->count, stream);
     if (e != 0) break;
     q.K = int(l.m);
     q.alpha = c[1];
     q.beta = c[2];
-    q.in = gram;
-    q.out = poly;
-    e = product<kPoly, false, false>(A, A, q, p->count, stream);
+    e = product<kPoly, false, false>(A, A, &A, nullptr, &B, q, p->count, stream);
     if (e != 0) break;
     q.lower = 0;
     q.M = p->rows;
     q.N = p->cols;
-    q.ld = l.ld;
-    q.matrix = l.x;
     q.alpha = c[0];
-    q.in = hi[step & 1];
-    q.lo = lo;
-    q.out = hi[(step & 1) ^ 1];
     if (last) {
       q.unscale = 1.0f / scale;
-      q.vector = p->cols % 8 == 0;
+      q.vector = p->cols % 4 == 0;
       if (p->param[0] != nullptr) {
         for (int i = 0; i < p->count; ++i) {
           q.param[i] = p->param[i];
@@ -679,9 +807,9 @@ extern "C" int nangila_orth(const NangilaOrthParams* p, cudaStream_t stream) {
         q.result = static_cast<__nv_bfloat16*>(p->out);
         if (!aligned(p->out)) q.vector = 0;
       }
-      e = tall ? product<kFinal, false, false>(X, B, q, p->count, stream) : product<kFinal, false, true>(B, X, q, p->count, stream);
+      e = tall ? product<kFinal, false, false>(X, B, &X, &Lo, nullptr, q, p->count, stream) : product<kFinal, false, true>(B, X, &X, &Lo, nullptr, q, p->count, stream);
     } else {
-      e = tall ? product<kUpdate, false, false>(X, B, q, p->count, stream) : product<kUpdate, false, true>(B, X, q, p->count, stream);
+      e = tall ? product<kUpdate, false, false>(X, B, &X, &Lo, &Next, q, p->count, stream) : product<kUpdate, false, true>(B, X, &X, &Lo, &Next, q, p->count, stream);
     }
   }
   return e;

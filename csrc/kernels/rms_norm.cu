@@ -18,10 +18,10 @@
 #include <type_traits>
 
 #include "follow.cuh"
-#include "launch_util.cuh"
 #include "nangila_kernels.h"
 #include "nangila_model_kernels.h"
 #include "quant.cuh"
+#include "raw8.cuh"
 
 namespace nangila {
 namespace {
@@ -29,71 +29,11 @@ namespace {
 constexpr float kE4m3Max = 448.0f;
 constexpr float kMinAmax = 1e-12f;  // a row of zeros gets a scale that can be divided by
 
-template <typename T>
-struct Raw8;  // eight values as they lie in memory
-template <> struct Raw8<float> { uint4 a, b; };
-template <> struct Raw8<__nv_bfloat16> { uint4 a; };
-template <> struct Raw8<__half> { uint4 a; };
-
-__device__ __forceinline__ uint4 load_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-template <typename T>
-__device__ __forceinline__ void fetch(const T* p, Raw8<T>& r) {
-  r.a = load_stream(p);
-  if constexpr (sizeof(T) == 4) r.b = load_stream(reinterpret_cast<const uint4*>(p) + 1);
-}
-__device__ __forceinline__ void unpack(const Raw8<float>& r, float (&v)[8]) {
-  const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
-}
-__device__ __forceinline__ void unpack(const Raw8<__nv_bfloat16>& r, float (&v)[8]) {
-  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-}
-__device__ __forceinline__ void unpack(const Raw8<__half>& r, float (&v)[8]) {
-  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
-}
-__device__ __forceinline__ void pack(const float (&v)[8], Raw8<float>& r) {
-  r.a = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-  r.b = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
-}
-__device__ __forceinline__ void pack(const float (&v)[8], Raw8<__nv_bfloat16>& r) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&h);
-  }
-  r.a = make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ void pack(const float (&v)[8], Raw8<__half>& r) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&h);
-  }
-  r.a = make_uint4(w[0], w[1], w[2], w[3]);
-}
-template <typename T>
-__device__ __forceinline__ void put(T* p, const Raw8<T>& r) {
-  *reinterpret_cast<uint4*>(p) = r.a;
-  if constexpr (sizeof(T) == 4) reinterpret_cast<uint4*>(p)[1] = r.b;
-}
+using dev::Raw8;
+using dev::fetch;
+using dev::pack;
+using dev::put;
+using dev::unpack;
 
 // Which columns a thread holds. VEC: runs of eight adjacent ones, 16-byte loads; else one by one, neighbours in neighbouring threads, for
 // rows that start anywhere and end anywhere.
@@ -101,6 +41,9 @@ template <int TPR, bool VEC>
 __device__ __forceinline__ int column(int v, int k, int t) {
   return VEC ? (v * TPR + t) * 8 + k : (v * 8 + k) * TPR + t;
 }
+// Whether a warp has nothing in its run `v` (rows that fill fewer runs than the threads have).
+template <int TPR, bool VEC>
+__device__ __forceinline__ bool beyond(int v, int t, int d) { return column<TPR, VEC>(v, 0, t & ~31) >= d; }
 template <typename T, int TPR, bool VEC>
 __device__ __forceinline__ void load_row8(const T* row, int v, int t, int d, Raw8<T>& raw) {
   if constexpr (VEC) {
@@ -163,15 +106,20 @@ __device__ __forceinline__ void load_weight8(const void* w, int dtype, int v, in
   }
 }
 
-// The sum over the threads of a row, in all of them. `s`: TPR / 32 floats that nobody else uses, given again only after the row's threads
+// The threads of a row meet. Rows of a CTA have barriers of their own: one may have a row more to do than the others.
+template <int TPR>
+__device__ __forceinline__ void meet() {
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + int(threadIdx.x) / TPR), "n"(TPR) : "memory");
+}
+// The sum over the threads of a row, in all of them. `s`: TPR / 32 floats of this row, given again only after the row's threads
 // have met in between (the sums of a kernel take turns with two of them).
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* s) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if constexpr (TPR > 32) {
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s[(threadIdx.x % TPR) >> 5] = v;
+    meet<TPR>();
     v = 0.0f;
 #pragma unroll
     for (int i = 0; i < TPR / 32; ++i) v += s[i];
@@ -189,8 +137,8 @@ __device__ __forceinline__ float row_max(float v, float* s) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = larger(v, __shfl_xor_sync(0xffffffffu, v, o));
   if constexpr (TPR > 32) {
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s[(threadIdx.x % TPR) >> 5] = v;
+    meet<TPR>();
     v = s[0];
 #pragma unroll
     for (int i = 1; i < TPR / 32; ++i) v = larger(v, s[i]);
@@ -198,9 +146,12 @@ __device__ __forceinline__ float row_max(float v, float* s) {
   return v;
 }
 
-// Threads of a CTA: four rows of a warp each, or one row.
+// Threads of a CTA, forward: four rows of a warp each, or one row. Backward: 256, three CTAs an SM (two in fp32), which keeps
+// enough loads on their way and leaves few parts of the weight's gradient to add up.
 template <int TPR>
 constexpr int kThreads = TPR < 128 ? 128 : TPR;
+template <int TPR>
+constexpr int kThreadsBackward = TPR < 256 ? 256 : TPR;
 
 template <typename T, int TPR, int NV, bool VEC, bool FP8>
 __global__ void __launch_bounds__(kThreads<TPR>) norm_forward_kernel(const __grid_constant__ NangilaNormParams p) {
@@ -222,6 +173,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) norm_forward_kernel(const __gri
     T* h = static_cast<T*>(p.h) + row * d;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
+      if (beyond<TPR, VEC>(v, t, d)) continue;
       float a[8], b[8];
       unpack(raw[v], a);
       unpack(more[v], b);
@@ -234,6 +186,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) norm_forward_kernel(const __gri
   float sum = 0.0f;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
+    if (beyond<TPR, VEC>(v, t, d)) continue;
     float a[8];
     unpack(raw[v], a);
 #pragma unroll
@@ -246,6 +199,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) norm_forward_kernel(const __gri
     T* y = static_cast<T*>(p.y) + row * d;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
+      if (beyond<TPR, VEC>(v, t, d)) continue;
       float a[8], w[8];
       unpack(raw[v], a);
       load_weight8<TPR, VEC>(p.weight, p.weight_dtype, v, t, d, w);
@@ -259,6 +213,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) norm_forward_kernel(const __gri
     if (p.group == 0) {
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
+        if (beyond<TPR, VEC>(v, t, d)) continue;
         float a[8], w[8];
         unpack(raw[v], a);
         load_weight8<TPR, VEC>(p.weight, p.weight_dtype, v, t, d, w);
@@ -269,6 +224,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) norm_forward_kernel(const __gri
     }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
+      if (beyond<TPR, VEC>(v, t, d)) continue;
       float a[8], w[8];
       unpack(raw[v], a);
       load_weight8<TPR, VEC>(p.weight, p.weight_dtype, v, t, d, w);
@@ -283,17 +239,19 @@ __global__ void __launch_bounds__(kThreads<TPR>) norm_forward_kernel(const __gri
       }
       // a row or group with a value that is not finite has no scale: all of it is not a number
       const float scale = amax <= 3.4028234e38f ? __fdiv_rn(fmaxf(amax, kMinAmax), kE4m3Max) : __uint_as_float(0x7fc00000u);
+      const float inverse = __frcp_rn(scale);
       const int c0 = column<TPR, VEC>(v, 0, t);
       if (p.group != 0) {
         if ((t & 15) == 0 && c0 < d) p.scale[row * (d / 128) + c0 / 128] = scale;
       } else if (v == 0 && t == 0) {
         p.scale[row] = scale;
       }
-      uint32_t word[2] = {0u, 0u};
+      uint32_t word[2];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t byte = scale == scale ? uint32_t(__nv_cvt_float_to_fp8(__fdiv_rn(a[k], scale), __NV_SATFINITE, __NV_E4M3)) : 0x7fu;
-        word[k / 4] |= byte << (8 * (k % 4));
+      for (int k = 0; k < 2; ++k) {  // (not a number times anything is not one, and stays so in e4m3)
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a[4 * k] * inverse, a[4 * k + 1] * inverse), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(a[4 * k + 2] * inverse, a[4 * k + 3] * inverse), __NV_SATFINITE, __NV_E4M3);
+        word[k] = lo | hi << 16;
       }
       if constexpr (VEC) {
         if (c0 < d) *reinterpret_cast<uint2*>(q + c0) = make_uint2(word[0], word[1]);
@@ -309,9 +267,9 @@ __global__ void __launch_bounds__(kThreads<TPR>) norm_forward_kernel(const __gri
 }
 
 template <typename T, int TPR, int NV, bool VEC>
-__global__ void __launch_bounds__(kThreads<TPR>) norm_backward_kernel(const __grid_constant__ NangilaNormGradParams p) {
-  constexpr int kRows = kThreads<TPR> / TPR;
-  __shared__ float s_sum[2][TPR > 32 ? TPR / 32 : 1];
+__global__ void __launch_bounds__(kThreadsBackward<TPR>, TPR > 256 ? 1 : sizeof(T) == 2 ? 3 : 2) norm_backward_kernel(const __grid_constant__ NangilaNormGradParams p) {
+  constexpr int kRows = kThreadsBackward<TPR> / TPR;
+  __shared__ float s_sum[2][kThreadsBackward<TPR> / 32];
   extern __shared__ float s_dw[];  // d, where a CTA has several rows at a time
   const int t = threadIdx.x % TPR, mine = threadIdx.x / TPR;
   const int d = p.d;
@@ -344,6 +302,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) norm_backward_kernel(const __gr
       float sum = 0.0f;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
+        if (beyond<TPR, VEC>(v, t, d)) continue;
         float a[8], b[8], w[8];
         unpack(h[v], a);
         unpack(g[v], b);
@@ -355,13 +314,14 @@ __global__ void __launch_bounds__(kThreads<TPR>) norm_backward_kernel(const __gr
           sum = __fmaf_rn(b[k] * w[k], unit, sum);
         }
       }
-      mean = __fdiv_rn(row_sum<TPR>(sum, s_sum[turn]), float(d));
+      mean = __fdiv_rn(row_sum<TPR>(sum, s_sum[turn] + mine * (TPR / 32)), float(d));
       turn ^= 1;
     }
     if (p.dx != nullptr) {
       T* dx = static_cast<T*>(p.dx) + row * d;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
+        if (beyond<TPR, VEC>(v, t, d)) continue;
         float o[8];
         if (p.dh != nullptr) {
           unpack(more[v], o);
@@ -405,12 +365,12 @@ __global__ void __launch_bounds__(kThreads<TPR>) norm_backward_kernel(const __gr
       }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < d; c += kThreads<TPR>) part[c] = s_dw[c];
+    for (int c = threadIdx.x; c < d; c += kThreadsBackward<TPR>) part[c] = s_dw[c];
   }
 }
 
-// dw: 32 columns of a CTA, 16 threads for each add up every sixteenth part in order, then the sixteen in order.
-constexpr int kDwY = 16;
+// dw: 32 columns of a CTA, 32 threads for each add up every 32nd part in order, then the 32 in order.
+constexpr int kDwY = 32;
 __global__ void __launch_bounds__(32 * kDwY) norm_dw_kernel(const float* partial, int parts, int d, void* dw, int dtype) {
   __shared__ float s[kDwY][33];
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + x;
@@ -444,7 +404,7 @@ template <int A, int B>
 struct Shape {
   static constexpr int tpr = A, nv = B;
 };
-// Threads for a row, and runs of eight columns for a thread: the fewest threads that hold the row in 8 runs each.
+// Threads for a row, and runs of eight columns for a thread. Forward: a warp up to 2048 columns, then the fewest threads that hold the row in four runs.
 template <typename F>
 int by_width(int d, const F& f) {
   const int units = (d + 7) / 8;
@@ -452,23 +412,39 @@ int by_width(int d, const F& f) {
   if (units <= 128) return f(Shape<32, 4>{});
   if (units <= 256) return f(Shape<32, 8>{});
   if (units <= 512) return f(Shape<128, 4>{});
-  if (units <= 1024) return f(Shape<128, 8>{});
+  if (units <= 1024) return f(Shape<256, 4>{});
   if (units <= 2048) return f(Shape<512, 4>{});
-  return f(Shape<512, 8>{});
+  return f(Shape<1024, 4>{});
+}
+// Backward: two runs, for a thread also holds its columns of the weight's gradient.
+template <typename F>
+int by_width_backward(int d, const F& f) {
+  const int units = (d + 7) / 8;
+  if (units <= 32) return f(Shape<32, 1>{});
+  if (units <= 64) return f(Shape<32, 2>{});
+  if (units <= 128) return f(Shape<64, 2>{});
+  if (units <= 256) return f(Shape<128, 2>{});
+  if (units <= 512) return f(Shape<256, 2>{});
+  if (units <= 1024) return f(Shape<512, 2>{});
+  if (units <= 2048) return f(Shape<1024, 2>{});
+  return f(Shape<1024, 4>{});
 }
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <typename T, int TPR, int NV, bool VEC>
-int backward_ctas(int64_t rows, int d, int* ctas, size_t* smem) {
-  constexpr int kRows = kThreads<TPR> / TPR;
-  *smem = kRows > 1 ? size_t(d) * 4 : 0;
-  int resident = 0;
-  // (asked for the longest row of this shape, so that the answer depends on the kernel alone)
-  const cudaError_t e = resident_ctas(reinterpret_cast<const void*>(norm_backward_kernel<T, TPR, NV, VEC>), kThreads<TPR>,
-                                      kRows > 1 ? size_t(TPR) * NV * 8 * 4 : 0, &resident);
-  if (e != cudaSuccess) return int(e);
-  *ctas = int(std::max<int64_t>(1, std::min<int64_t>((rows + kRows - 1) / kRows, resident)));
-  return 0;
+// CTAs an SM, backward
+template <typename T, int TPR>
+constexpr int kPerSm = TPR > 256 ? 1 : sizeof(T) == 2 ? 3 : 2;
+int sm_count() {
+  static int sms[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (sms[dev] == 0) cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
+  return sms[dev];
+}
+template <typename T, int TPR>
+int backward_ctas(int64_t rows) {
+  constexpr int kRows = kThreadsBackward<TPR> / TPR;
+  return int(std::max<int64_t>(1, std::min<int64_t>((rows + kRows - 1) / kRows, int64_t(sm_count()) * kPerSm<T, TPR>)));
 }
 
 }  // namespace
@@ -503,14 +479,10 @@ extern "C" int nangila_rms_norm_partials(int64_t rows, int32_t d, int32_t dtype,
   if (!count || rows < 1 || d < 1 || d > NANGILA_NORM_MAX_D) return int(cudaErrorInvalidValue);
   return by_type(dtype, [&](auto type) {
     using T = decltype(type);
-    return by_width(d, [&](auto shape) {
+    return by_width_backward(d, [&](auto shape) {
       using S = decltype(shape);
-      int a = 0, b = 0;
-      size_t smem = 0;
-      int e = backward_ctas<T, S::tpr, S::nv, true>(rows, d, &a, &smem);
-      if (e == 0) e = backward_ctas<T, S::tpr, S::nv, false>(rows, d, &b, &smem);
-      *count = std::max(a, b);
-      return e;
+      *count = backward_ctas<T, S::tpr>(rows);
+      return 0;
     });
   });
 }
@@ -524,14 +496,13 @@ extern "C" int nangila_rms_norm_backward(const NangilaNormGradParams* p, cudaStr
                    aligned(p->weight) && aligned(p->dx);
   return by_type(p->dtype, [&](auto type) {
     using T = decltype(type);
-    return by_width(p->d, [&](auto shape) {
+    return by_width_backward(p->d, [&](auto shape) {
       using S = decltype(shape);
-      constexpr int kT = kThreads<S::tpr>;
+      constexpr int kT = kThreadsBackward<S::tpr>;
       auto run = [&](auto how) {
         constexpr bool VEC = decltype(how)::value;
-        int ctas = 0;
-        size_t smem = 0;
-        if (const int e = backward_ctas<T, S::tpr, S::nv, VEC>(p->rows, p->d, &ctas, &smem)) return e;
+        const int ctas = backward_ctas<T, S::tpr>(p->rows);
+        const size_t smem = kT > S::tpr ? size_t(p->d) * 4 : 0;  // below the default limit: such rows are short
         norm_backward_kernel<T, S::tpr, S::nv, VEC><<<unsigned(ctas), kT, smem, stream>>>(*p);
         if (const cudaError_t e = cudaGetLastError()) return int(e);
         if (p->dw == nullptr) return 0;

@@ -12,7 +12,7 @@ from typing import Dict, List, Sequence, Tuple, Union
 
 import torch
 
-from .reductions import _glue
+from ._native import glue
 
 #: Moves singular values from 1e-3 to 1 into about 0.7 to 1.2 within five steps.
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
@@ -79,7 +79,7 @@ def orthogonalize(update: Union[torch.Tensor, Sequence[torch.Tensor]], steps: in
         for t in many:
             _check_matrix(t, "updates")
         if update.is_cuda:
-            out = _glue().orth([t.contiguous() for t in many], [], [], flat, eps)
+            out = glue().orth([t.contiguous() for t in many], [], [], flat, eps)
         else:
             out = torch.stack([_plain(t, flat, eps).to(torch.bfloat16) for t in many])
         return out if update.dim() == 3 else out[0]
@@ -92,7 +92,7 @@ def orthogonalize(update: Union[torch.Tensor, Sequence[torch.Tensor]], steps: in
     results: List[torch.Tensor] = [None] * len(many)  # type: ignore[list-item]
     for (_, _, device), members in groups.items():
         if device.type == "cuda":
-            stack = _glue().orth([many[i].contiguous() for i in members], [], [], flat, eps).unbind(0)
+            stack = glue().orth([many[i].contiguous() for i in members], [], [], flat, eps).unbind(0)
         else:
             stack = [_plain(many[i], flat, eps).to(torch.bfloat16) for i in members]
         for i, t in zip(members, stack):
@@ -146,12 +146,12 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
             raise ValueError(f"nangila: parameter {i} and its momentum must be packed (contiguous)")
         groups.setdefault((p.shape, p.dtype, g.dtype, p.device), []).append(i)
     update_scale(1, 1, scale)
-    if _glue().overlapping(params + momenta, grads):
+    if glue().overlapping(params + momenta, grads):
         raise ValueError("nangila: parameters and momenta must not share memory with one another or with the gradients")
     for (shape, _, _, device), members in groups.items():
         rate, decay = lr * update_scale(shape[0], shape[1], scale), 1.0 - lr * weight_decay
         if device.type == "cuda":
-            _glue().orth([grads[i].contiguous() for i in members], [momenta[i] for i in members], [params[i] for i in members], flat, eps, momentum, nesterov,
+            glue().orth([grads[i].contiguous() for i in members], [momenta[i] for i in members], [params[i] for i in members], flat, eps, momentum, nesterov,
                          decay, rate)
             # the kernels write where autograd does not look: what was saved for a backward pass is not what it was
             torch.autograd.graph.increment_version([t for i in members for t in (params[i], momenta[i]) if not t.is_inference()])

@@ -10,18 +10,18 @@ from typing import Optional, Tuple
 
 import torch
 
-from .reductions import _glue
+from ._native import glue
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5) -> torch.Tensor:
     """``x / sqrt(mean(x^2) + eps) * weight`` over the last dimension, in the type of ``x``. Differentiable once in ``x`` and ``weight``."""
-    return _glue().rms_norm(x, weight, eps)
+    return glue().rms_norm(x, weight, eps)
 
 
 def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(y, h)`` with ``h = x + residual``, rounded to their type, and ``y = rms_norm(h)``: a block's norm in one pass. The gradients of both
     outputs meet in one kernel; ``x`` and ``residual`` get the same one."""
-    return _glue().add_rms_norm(x, residual, weight, eps)
+    return glue().add_rms_norm(x, residual, weight, eps)
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: Optional[torch.Tensor] = None,
@@ -30,5 +30,5 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, resid
     ``max(|y|, 1e-12) / 448`` over the row, or over each ``group`` of 128 columns; it has the shape of ``x`` without its last dimension, or with
     one value for each group there. A row or group that is not all finite is not a number throughout. No gradient: inputs that require
     one are refused unless gradients are off."""
-    q, scale, h = _glue().rms_norm_fp8(x, weight, eps, residual, 0 if group is None else group)
+    q, scale, h = glue().rms_norm_fp8(x, weight, eps, residual, 0 if group is None else group)
     return (q, scale) if h is None else (q, scale, h)

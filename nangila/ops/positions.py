@@ -6,7 +6,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 
-from .reductions import _glue
+from ._native import glue
 
 LAYOUTS = ("interleaved", "half")
 SCALINGS = (None, "linear", "ntk", "yarn")
@@ -70,5 +70,5 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, posi
     token not a number. Differentiable once in ``q`` and ``k``; computed in float32 and rounded once."""
     if layout not in LAYOUTS:
         raise ValueError(f"nangila: layout must be one of {LAYOUTS}, got {layout!r}")
-    out = _glue().rotary(q, k, table, positions, layout == "half")
+    out = glue().rotary(q, k, table, positions, layout == "half")
     return out[0] if k is None else out
