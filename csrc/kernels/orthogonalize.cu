@@ -44,8 +44,8 @@ constexpr int kStages = 5;
 constexpr int kChunk = 64;                       // columns that a warp of the epilogue takes at a time
 constexpr int kBoxBytes = 32 * kChunk * 2;       // 32 rows of them in fp16
 constexpr int kSlotBytes = 2 * kBoxBytes;        // what comes in and goes out at a time, in place
-constexpr int kEpilogueWarps = 4;
-constexpr int kEpilogueBytes = kEpilogueWarps * 2 * kSlotBytes;
+constexpr int kEpilogueWarps = 8;                // two for each quarter of tensor memory, taking turns with the chunks
+constexpr int kEpilogueBytes = kEpilogueWarps * kSlotBytes;
 constexpr int kSmem = kStages * kStageBytes + kEpilogueBytes + 1024 + 256;
 constexpr int kGemmThreads = 64 + 32 * kEpilogueWarps;  // warp 0: TMA, warp 1: products, the others: epilogue
 constexpr uint64_t kTimeoutNs = 10ull * 1000 * 1000 * 1000;
@@ -245,7 +245,7 @@ __device__ __forceinline__ void into_slot(const Product& p, uint8_t* slot, int l
 // D = A B for square tiles of all matrices, walked over by CTAs that stay (PAIR: pairs of CTAs that share the tensor cores' work on 256 x 256, each
 // with its 128 rows of A, half of B's columns, and 128 rows of the result; else one CTA and 128 x 128). A_MN / B_MN: the operand lies with its rows
 // (columns of B) adjacent in memory, not its K. The accumulators of two tiles share tensor memory: the epilogue of one runs under the
-// products of the next, and what it needs of X or A is on its way before they end. Each of its warps has two slots of shared memory of its own,
+// products of the next, and what it needs of X or A is on its way before they end. Each of its warps has a slot of shared memory of its own,
 // filled and emptied by TMA, and meets no other warp.
 // A wait that runs out makes every result of this CTA from there on not a number.
 template <int KIND, bool A_MN, bool B_MN, bool PAIR>
@@ -259,8 +259,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __g
   uint64_t* empty = full + kStages;
   uint64_t* acc_full = empty + kStages;   // [2]
   uint64_t* acc_empty = acc_full + 2;     // [2]
-  uint64_t* loaded = acc_empty + 2;       // [kEpilogueWarps][2]
-  uint64_t* drained = loaded + 2 * kEpilogueWarps;
+  uint64_t* loaded = acc_empty + 2;       // [kEpilogueWarps]
+  uint64_t* drained = loaded + kEpilogueWarps;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile uint32_t* failed = tmem_slot + 1;
 
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __g
       mbar_init(&acc_full[s], 1);
       mbar_init(&acc_empty[s], kEpilogueWarps * (PAIR ? 2 : 1));
     }
-    for (int s = 0; s < 2 * kEpilogueWarps; ++s) mbar_init(&loaded[s], 1);
+    for (int s = 0; s < kEpilogueWarps; ++s) mbar_init(&loaded[s], 1);
     mbar_init(drained, 1);
     *failed = 0;
     fence_barrier_init();
@@ -386,8 +386,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __g
   } else {
     // ---------------- epilogue ----------------
     const int quad = warp & 3;  // the lanes of tensor memory that this warp may read
-    uint8_t* my_slots = slots + (warp - 2) * 2 * kSlotBytes;
-    uint64_t* my_loaded = loaded + (warp - 2) * 2;
+    const int turn = (warp - 2) >> 2;
+    uint8_t* slot = slots + (warp - 2) * kSlotBytes;
+    uint64_t* my_loaded = loaded + (warp - 2);
     const uint32_t acc_empty_at = PAIR ? rank0_address(&acc_empty[0]) : smem_u32(&acc_empty[0]);
     constexpr bool kLoads = KIND != kGram;
     constexpr uint32_t kLoadBytes = KIND == kPoly ? kBoxBytes : kSlotBytes;
@@ -398,28 +399,26 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __g
       const int acc = n & 1;
       const int row0 = at.m0 + int(rank) * kTileM + quad * 32;
       const int mine = row0 < p.M ? min(kChunks, (p.N - at.n0 + kChunk - 1) / kChunk) : 0;
-      auto fetch = [&](int c, uint32_t turn) {  // lane 0: chunk c into the slot whose turn it is, once nothing goes out of it any more
-        uint8_t* slot = my_slots + (turn & 1) * kSlotBytes;
+      auto fetch = [&](int c) {  // lane 0: chunk c into the slot, once nothing goes out of it any more
         bulk_wait_read();
-        mbar_arrive_expect_tx(&my_loaded[turn & 1], kLoadBytes);
-        tma_load_3d(slot, &maps.in, at.n0 + c * kChunk, row0, at.batch, &my_loaded[turn & 1]);
-        if (KIND != kPoly) tma_load_3d(slot + kBoxBytes, &maps.lo, at.n0 + c * kChunk, row0, at.batch, &my_loaded[turn & 1]);
+        mbar_arrive_expect_tx(my_loaded, kLoadBytes);
+        tma_load_3d(slot, &maps.in, at.n0 + c * kChunk, row0, at.batch, my_loaded);
+        if (KIND != kPoly) tma_load_3d(slot + kBoxBytes, &maps.lo, at.n0 + c * kChunk, row0, at.batch, my_loaded);
       };
-      if (kLoads && mine > 0 && lane == 0) fetch(0, chunks);
+      if (kLoads && turn < mine && lane == 0) fetch(turn);
       bool ok = *failed == 0 && mbar_wait(&acc_full[acc], uint32_t((n / 2) & 1), kTimeoutNs);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) *failed = 1;
       tc_fence_after_sync();
 #pragma unroll 1
-      for (int c = 0; c < mine; ++c, ++chunks) {
-        uint8_t* slot = my_slots + (chunks & 1) * kSlotBytes;
+      for (int c = turn; c < mine; c += 2, ++chunks) {
         if (kLoads) {
-          if (c + 1 < mine && lane == 0) fetch(c + 1, chunks + 1);
-          const bool here = mbar_wait(&my_loaded[chunks & 1], (chunks >> 1) & 1, kTimeoutNs);
+          if (c != turn && lane == 0) fetch(c);
+          const bool here = mbar_wait(my_loaded, chunks & 1, kTimeoutNs);
           if (!__all_sync(0xffffffffu, here)) ok = false;
           if (!ok) *failed = 1;
         } else {
-          if (lane == 0) bulk_wait_read_but_one();  // this slot's stores; the other's may be under way
+          if (lane == 0) bulk_wait_read();  // the slot's last stores
           __syncwarp();
         }
 #pragma unroll

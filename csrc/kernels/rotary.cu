@@ -111,10 +111,24 @@ __global__ void __launch_bounds__(kT) rotary_vec_kernel(const __grid_constant__ 
   }
   constexpr int kPairs = HALF ? 8 : 4;
   float cs[2 * kPairs];
+  // Positions are read a group ahead: the table's values, which depend on them, would otherwise arrive two trips to memory after the group's data.
+  auto row_of = [&](uint32_t token) {
+    const uint32_t b = divide(token, plan.seq), t = token - b * plan.seq.by;
+    if (p.positions == nullptr) return int32_t(t);
+    const int64_t at = int64_t(b) * p.pos_stride_b + int64_t(t) * p.pos_stride_t;
+    const int64_t row = p.positions_64 ? static_cast<const int64_t*>(p.positions)[at] : int64_t(static_cast<const int32_t*>(p.positions)[at]);
+    return row < 0 || row >= p.table_rows ? -1 : int32_t(row);
+  };
+  int32_t next[kAtOnce];
+#pragma unroll
+  for (int j = 0; j < kAtOnce; ++j) {
+    const uint32_t token = blockIdx.x * uint32_t(plan.tokens) + uint32_t(ahead[j]);
+    next[j] = turns && token < plan.all_tokens ? row_of(token) : -1;
+  }
   for (uint32_t group = blockIdx.x; group < plan.groups; group += gridDim.x) {
     const uint32_t first = group * uint32_t(plan.tokens);
-    int64_t have = -2;  // the row of the table in `cs`; -1: none
-    int64_t row[kAtOnce];
+    int32_t have = -2;  // the row of the table in `cs`; -1: none
+    int32_t row[kAtOnce];
     dev::Raw8<T> raw[kAtOnce], partner[HALF ? kAtOnce : 1];
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
@@ -124,12 +138,12 @@ __global__ void __launch_bounds__(kT) rotary_vec_kernel(const __grid_constant__ 
       const T* from = in[j] + int64_t(b) * p.stride_b[which[j]] + int64_t(t) * p.stride_t[which[j]];
       dev::fetch(from, raw[j]);
       if (HALF && turns) dev::fetch(from + half, partner[j]);
-      row[j] = t;
-      if (p.positions != nullptr) {
-        const int64_t at = int64_t(b) * p.pos_stride_b + int64_t(t) * p.pos_stride_t;
-        row[j] = p.positions_64 ? static_cast<const int64_t*>(p.positions)[at] : int64_t(static_cast<const int32_t*>(p.positions)[at]);
-        if (row[j] < 0 || row[j] >= p.table_rows) row[j] = -1;
-      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      row[j] = next[j];
+      const uint64_t token = uint64_t(first) + uint64_t(gridDim.x) * uint32_t(plan.tokens) + uint32_t(ahead[j]);
+      if (turns && token < plan.all_tokens) next[j] = row_of(uint32_t(token));
     }
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
@@ -139,7 +153,7 @@ __global__ void __launch_bounds__(kT) rotary_vec_kernel(const __grid_constant__ 
       if (turns) {
         if (row[j] != have) {
           have = row[j];
-          const float4* values = reinterpret_cast<const float4*>(p.table + (have < 0 ? 0 : have) * p.rot + (HALF ? 2 * col : col));
+          const float4* values = reinterpret_cast<const float4*>(p.table + int64_t(have < 0 ? 0 : have) * p.rot + (HALF ? 2 * col : col));
 #pragma unroll
           for (int i = 0; i < kPairs / 2; ++i) {
             const float4 f = __ldg(values + i);
@@ -202,7 +216,7 @@ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0
 template <typename T>
 int launch(const NangilaRotaryParams& p, cudaStream_t stream) {
   const int64_t pairs = p.batch * p.seq * (p.heads[0] + p.heads[1]);
-  bool vec = p.batch * p.seq < (int64_t(1) << 31) && p.d % 8 == 0 && p.d / 8 <= kT && p.rot % (p.half ? 16 : 8) == 0 && aligned(p.table);
+  bool vec = p.batch * p.seq < (int64_t(1) << 31) && p.table_rows < (int64_t(1) << 31) && p.d % 8 == 0 && p.d / 8 <= kT && p.rot % (p.half ? 16 : 8) == 0 && aligned(p.table);
   for (int i = 0; i < 2; ++i)
     if (p.in[i] != nullptr)
       vec = vec && aligned(p.in[i]) && aligned(p.out[i]) && p.stride_b[i] % 8 == 0 && p.stride_t[i] % 8 == 0 && p.stride_h[i] % 8 == 0;
