@@ -457,6 +457,54 @@ bool overlapping(const std::vector<Tensor>& written, const std::vector<Tensor>& 
   return false;
 }
 
+void check_matrix(const Tensor& t, const char* name) {
+  check_tensor(t, name);
+  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) >= 1 && t.size(1) >= 1 && t.size(0) <= 65536 && t.size(1) <= 65536, "nangila: ", name,
+                    " must be matrices of 1 x 1 to 65536 x 65536, got shape ", t.sizes());
+}
+// Indices of tensors of one shape, type and device, in the order of their first.
+std::vector<std::vector<int64_t>> group_matrices(const std::vector<Tensor>& ts) {
+  std::vector<std::vector<int64_t>> groups;
+  for (size_t i = 0; i < ts.size(); ++i) {
+    check_matrix(ts[i], "updates");
+    auto same = [&](const std::vector<int64_t>& g) {
+      const Tensor& o = ts[g[0]];
+      return o.sizes() == ts[i].sizes() && o.scalar_type() == ts[i].scalar_type() && o.device() == ts[i].device();
+    };
+    auto it = std::find_if(groups.begin(), groups.end(), same);
+    if (it == groups.end()) groups.push_back({int64_t(i)});
+    else it->push_back(int64_t(i));
+  }
+  return groups;
+}
+// The same for a Muon step, with its checks of what belongs together.
+std::vector<std::vector<int64_t>> group_muon(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& momenta) {
+  TORCH_CHECK_VALUE(params.size() == grads.size() && params.size() == momenta.size(), "nangila: ", params.size(), " parameters, ", grads.size(), " gradients and ",
+                    momenta.size(), " momenta");
+  std::vector<std::vector<int64_t>> groups;
+  for (size_t i = 0; i < params.size(); ++i) {
+    const Tensor &p = params[i], &g = grads[i], &m = momenta[i];
+    check_matrix(p, "parameters");
+    check_matrix(g, "gradients");
+    check_matrix(m, "momenta");
+    TORCH_CHECK_VALUE(p.sizes() == g.sizes() && p.sizes() == m.sizes() && p.device() == g.device() && p.device() == m.device(), "nangila: parameter ", i, " is ", p.sizes(), " on ",
+                      p.device(), ", its gradient ", g.sizes(), " on ", g.device(), ", its momentum ", m.sizes(), " on ", m.device());
+    TORCH_CHECK_TYPE(m.scalar_type() == at::kFloat, "nangila: momenta must be float32, got ", m.scalar_type());
+    TORCH_CHECK_VALUE(p.is_contiguous() && m.is_contiguous(), "nangila: parameter ", i, " and its momentum must be packed (contiguous)");
+    auto same = [&](const std::vector<int64_t>& other) {
+      const Tensor &op = params[other[0]], &og = grads[other[0]];
+      return op.sizes() == p.sizes() && op.scalar_type() == p.scalar_type() && og.scalar_type() == g.scalar_type() && op.device() == p.device();
+    };
+    auto it = std::find_if(groups.begin(), groups.end(), same);
+    if (it == groups.end()) groups.push_back({int64_t(i)});
+    else it->push_back(int64_t(i));
+  }
+  std::vector<Tensor> written = params;
+  written.insert(written.end(), momenta.begin(), momenta.end());
+  TORCH_CHECK_VALUE(!overlapping(written, grads), "nangila: parameters and momenta must not share memory with one another or with the gradients");
+  return groups;
+}
+
 }  // namespace
 
 void register_model(py::module_& m) {
@@ -466,5 +514,6 @@ void register_model(py::module_& m) {
   m.def("rotary", &rotary, py::arg("q"), py::arg("k"), py::arg("table"), py::arg("positions"), py::arg("half"));
   m.def("orth", &orth, py::arg("grads"), py::arg("momenta"), py::arg("params"), py::arg("coefficients"), py::arg("eps"), py::arg("mu") = 0.0, py::arg("nesterov") = false,
         py::arg("decay") = 1.0, py::arg("rate") = 0.0);
-  m.def("overlapping", &overlapping, py::arg("written"), py::arg("read"));
+  m.def("group_matrices", &group_matrices, py::arg("matrices"));
+  m.def("group_muon", &group_muon, py::arg("params"), py::arg("grads"), py::arg("momenta"));
 }

@@ -24,6 +24,9 @@
 #include <cstdint>
 #include <cstring>
 #include <mutex>
+#include <set>
+#include <type_traits>
+#include <utility>
 
 #include "follow.cuh"
 #include "nangila_kernels.h"
@@ -58,10 +61,12 @@ struct Product {
   int tiles_m, per, total; // tiles along M; tiles of one matrix, of all
   int lower;               // only tiles that reach the lower triangle
   float alpha, beta;       // gram: D alpha;  poly: alpha A + beta D;  update: alpha X + D
-  float unscale;           // final: result = (alpha X + D) unscale
-  __nv_bfloat16* result;   // final: packed M x N, or NULL
-  int param_dtype, vector; // final: the parameters' type; runs of four elements can be read and written
-  float decay, rate;
+};
+// Where the last update goes: result = (alpha X + D) unscale.
+struct Target {
+  __nv_bfloat16* result;   // packed, one matrix behind the other, or NULL
+  int param_dtype, vector; // the parameters' type; runs of four elements can be read and written
+  float unscale, decay, rate;
   void* param[NANGILA_ORTH_MAX_COUNT];
 };
 struct Maps {
@@ -154,7 +159,7 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&v)[4]) {
 // A warp's 32 rows of results in a slot, fp32, taken to the parameters (T) or, with `fresh`, out. Two rows at a time, four columns a lane; the loads of
 // sixteen rows are on their way before the first store.
 template <typename T, bool fresh>
-__device__ __forceinline__ void put_results(const Product& p, T* base, uint8_t* slot, int lane, int row0, int col0) {
+__device__ __forceinline__ void put_results(const Product& p, const Target& to_where, T* base, uint8_t* slot, int lane, int row0, int col0) {
   const int x = lane & 15, col = col0 + 4 * x, left = p.N - col;
   if (left <= 0) return;
   // four columns 4 x: group x / 4 of sixteen, its quarter x % 4
@@ -169,7 +174,7 @@ __device__ __forceinline__ void put_results(const Product& p, T* base, uint8_t* 
         const int row = row0 + half + 2 * i + (lane >> 4);
         if (row >= p.M) continue;
         const T* from = base + int64_t(row) * p.N + col;
-        if (p.vector) {
+        if (to_where.vector) {
           load4<T>(from, v[i]);
         } else {
 #pragma unroll
@@ -184,9 +189,9 @@ __device__ __forceinline__ void put_results(const Product& p, T* base, uint8_t* 
       const uint4 raw = *box_at(box, at, j);
       const float r[4] = {__uint_as_float(raw.x), __uint_as_float(raw.y), __uint_as_float(raw.z), __uint_as_float(raw.w)};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[i][k] = fresh ? r[k] : v[i][k] * p.decay - p.rate * r[k];
+      for (int k = 0; k < 4; ++k) v[i][k] = fresh ? r[k] : v[i][k] * to_where.decay - to_where.rate * r[k];
       T* to = base + int64_t(row0 + at) * p.N + col;
-      if (p.vector) {
+      if (to_where.vector) {
         store4(to, v[i]);
       } else {
 #pragma unroll
@@ -199,7 +204,7 @@ __device__ __forceinline__ void put_results(const Product& p, T* base, uint8_t* 
 
 // Sixteen accumulators of a lane's row, columns 16 g to 16 g + 15 of the chunk in the slot, taken into the slot as what goes out.
 template <int KIND>
-__device__ __forceinline__ void into_slot(const Product& p, uint8_t* slot, int lane, int g, float (&v)[16]) {
+__device__ __forceinline__ void into_slot(const Product& p, float unscale, uint8_t* slot, int lane, int g, float (&v)[16]) {
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int j = 2 * g + e;
@@ -236,10 +241,207 @@ __device__ __forceinline__ void into_slot(const Product& p, uint8_t* slot, int l
         *second = l;
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[8 * e + k] = w[k] * p.unscale;
+        for (int k = 0; k < 8; ++k) v[8 * e + k] = w[k] * unscale;
       }
     }
   }
+}
+
+// What a CTA's roles share, in shared memory.
+struct Shared {
+  uint8_t *stages, *slots;
+  uint64_t *full, *empty;          // [kStages]
+  uint64_t *acc_full, *acc_empty;  // [2]
+  uint64_t *loaded;                // [kEpilogueWarps]
+  uint64_t *drained;
+  uint32_t* tmem_slot;
+  volatile uint32_t* failed;       // a wait has run out
+};
+__device__ __forceinline__ Shared shared_parts(uint8_t* raw) {
+  Shared s;
+  s.stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  s.slots = s.stages + kStages * kStageBytes;
+  s.full = reinterpret_cast<uint64_t*>(s.slots + kEpilogueBytes);
+  s.empty = s.full + kStages;
+  s.acc_full = s.empty + kStages;
+  s.acc_empty = s.acc_full + 2;
+  s.loaded = s.acc_empty + 2;
+  s.drained = s.loaded + kEpilogueWarps;
+  s.tmem_slot = reinterpret_cast<uint32_t*>(s.drained + 1);
+  s.failed = s.tmem_slot + 1;
+  return s;
+}
+template <bool PAIR>
+__device__ __forceinline__ void init_barriers(const Shared& s) {
+  for (int i = 0; i < kStages; ++i) {
+    mbar_init(&s.full[i], 1);
+    mbar_init(&s.empty[i], 1);
+  }
+  for (int i = 0; i < 2; ++i) {
+    mbar_init(&s.acc_full[i], 1);
+    mbar_init(&s.acc_empty[i], kEpilogueWarps * (PAIR ? 2 : 1));
+  }
+  for (int i = 0; i < kEpilogueWarps; ++i) mbar_init(&s.loaded[i], 1);
+  mbar_init(s.drained, 1);
+  *s.failed = 0;
+  fence_barrier_init();
+}
+
+// TMA of a tile's slabs, `i` of which have gone before: both CTAs of a pair, each its own halves; the bytes are counted where the products are issued.
+// False when a wait has run out.
+template <bool PAIR>
+__device__ __forceinline__ bool load_tile(const Shared& s, const CUtensorMap* a_map, const CUtensorMap* b_map, bool a_mn, bool b_mn, const TileAt& at, uint32_t rank, int slabs, int& i) {
+  const int row = at.m0 + int(rank) * kTileM, col = at.n0 + int(rank) * 128;
+  for (int k = 0; k < slabs; ++k, ++i) {
+    const int st = i % kStages;
+    if (i >= kStages && !mbar_wait(&s.empty[st], uint32_t((i / kStages - 1) & 1), kTimeoutNs)) {
+      *s.failed = 1;
+      return false;
+    }
+    uint8_t* a = s.stages + st * kStageBytes;
+    uint8_t* b = a + kOperandBytes;
+    const int k0 = k * kSlabK;
+    if (rank == 0) mbar_arrive_expect_tx(&s.full[st], kStageBytes * (PAIR ? 2 : 1));
+    const uint32_t bar = PAIR ? rank0_address(&s.full[st]) : smem_u32(&s.full[st]);
+    if (a_mn) {
+      tma_operand<PAIR>(a, a_map, row, k0, at.batch, bar);
+      tma_operand<PAIR>(a + 8192, a_map, row + 64, k0, at.batch, bar);
+    } else {
+      tma_operand<PAIR>(a, a_map, k0, row, at.batch, bar);
+    }
+    if (b_mn) {
+      tma_operand<PAIR>(b, b_map, col, k0, at.batch, bar);
+      tma_operand<PAIR>(b + 8192, b_map, col + 64, k0, at.batch, bar);
+    } else {
+      tma_operand<PAIR>(b, b_map, k0, col, at.batch, bar);
+    }
+  }
+  return true;
+}
+// The copies that are still under way when the loads end: all have arrived when the products that read them are done; if somebody has given up, as
+// much as can be waited for (the bytes of a pair are counted by rank 0, the stages of rank 1 are given back by its products).
+__device__ __forceinline__ void drain_loads(const Shared& s, uint32_t rank, int i) {
+  for (int j = max(0, i - kStages); j < i; ++j) {
+    if (*s.failed == 0 || rank != 0) mbar_wait(&s.empty[j % kStages], uint32_t((j / kStages) & 1), kTimeoutNs);
+    else mbar_wait(&s.full[j % kStages], uint32_t((j / kStages) & 1), kTimeoutNs);
+  }
+}
+// The products of a tile, the n-th, into its accumulator. False when a wait has run out.
+template <bool PAIR>
+__device__ __forceinline__ bool multiply_tile(const Shared& s, uint32_t tmem, bool a_mn, bool b_mn, int slabs, int n, int& i) {
+  constexpr int kSide = PAIR ? 256 : 128;
+  const uint32_t idesc = (1u << 4) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | (uint32_t(kSide >> 3) << 17) | (uint32_t(kSide >> 4) << 24);
+  const int acc = n & 1;
+  if (n >= 2 && !mbar_wait(&s.acc_empty[acc], uint32_t((n / 2 - 1) & 1), kTimeoutNs)) return false;
+  tc_fence_after_sync();
+  const uint32_t d = tmem + uint32_t(acc * kSide);
+  for (int k = 0; k < slabs; ++k, ++i) {
+    const int st = i % kStages;
+    if (!mbar_wait(&s.full[st], uint32_t((i / kStages) & 1), kTimeoutNs)) return false;
+    tc_fence_after_sync();
+    const uint32_t a = smem_u32(s.stages + st * kStageBytes), b = a + kOperandBytes;
+#pragma unroll
+    for (int kk = 0; kk < kSlabK / 16; ++kk) {
+      // K-major: 16 elements along K are 32 bytes of a swizzle row; MN-major: 16 K-rows are two groups of eight rows of 128 bytes
+      const uint64_t ad = a_mn ? make_smem_desc(a + kk * 2048, 8192, 1024) : make_smem_desc(a + kk * 32, 16, 1024);
+      const uint64_t bd = b_mn ? make_smem_desc(b + kk * 2048, 8192, 1024) : make_smem_desc(b + kk * 32, 16, 1024);
+      if (PAIR) umma_f16_pair(d, ad, bd, idesc, (k > 0 || kk > 0) ? 1u : 0u);
+      else umma_f16(d, ad, bd, idesc, (k > 0 || kk > 0) ? 1u : 0u);
+    }
+    if (PAIR) umma_commit_pair(&s.empty[st]);
+    else umma_commit(&s.empty[st]);
+  }
+  if (PAIR) umma_commit_pair(&s.acc_full[acc]);
+  else umma_commit(&s.acc_full[acc]);
+  return true;
+}
+template <bool PAIR>
+__device__ __forceinline__ void drain_products(const Shared& s) {
+  *s.failed = 1;
+  if (PAIR) umma_commit_pair(s.drained);
+  else umma_commit(s.drained);
+  mbar_wait(s.drained, 0, kTimeoutNs);
+}
+// The n-th tile's accumulator taken to where it belongs, by one of the epilogue's warps; `chunks`: how many it has loaded so far.
+template <int KIND, bool PAIR>
+__device__ __forceinline__ void finish_tile(const Shared& s, uint32_t tmem, const Product& p, const Target& target, const CUtensorMap* in, const CUtensorMap* lo, const CUtensorMap* out,
+                                            const CUtensorMap* mirror, const TileAt& at, uint32_t rank, int n, uint32_t& chunks) {
+  constexpr int kSide = PAIR ? 256 : 128;
+  constexpr int kChunks = kSide / kChunk;
+  constexpr bool kLoads = KIND != kGram;
+  constexpr uint32_t kLoadBytes = KIND == kPoly ? kBoxBytes : kSlotBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int quad = warp & 3;  // the lanes of tensor memory that this warp may read
+  const int turn = (warp - 2) >> 2;
+  uint8_t* slot = s.slots + (warp - 2) * kSlotBytes;
+  uint64_t* my_loaded = s.loaded + (warp - 2);
+  const int acc = n & 1;
+  const int row0 = at.m0 + int(rank) * kTileM + quad * 32;
+  const int mine = row0 < p.M ? min(kChunks, (p.N - at.n0 + kChunk - 1) / kChunk) : 0;
+  auto fetch = [&](int c) {  // lane 0: chunk c into the slot, once nothing goes out of it any more
+    bulk_wait_read();
+    mbar_arrive_expect_tx(my_loaded, kLoadBytes);
+    tma_load_3d(slot, in, at.n0 + c * kChunk, row0, at.batch, my_loaded);
+    if (KIND != kPoly) tma_load_3d(slot + kBoxBytes, lo, at.n0 + c * kChunk, row0, at.batch, my_loaded);
+  };
+  if (kLoads && turn < mine && lane == 0) fetch(turn);
+  bool ok = *s.failed == 0 && mbar_wait(&s.acc_full[acc], uint32_t((n / 2) & 1), kTimeoutNs);
+  ok = __all_sync(0xffffffffu, ok);
+  if (!ok) *s.failed = 1;
+  tc_fence_after_sync();
+#pragma unroll 1
+  for (int c = turn; c < mine; c += 2) {
+    if (kLoads) {
+      if (c != turn && lane == 0) fetch(c);
+      const bool here = mbar_wait(my_loaded, chunks & 1, kTimeoutNs);
+      ++chunks;
+      if (!__all_sync(0xffffffffu, here)) ok = false;
+      if (!ok) *s.failed = 1;
+    } else {
+      if (lane == 0) bulk_wait_read();  // the slot's last stores
+      __syncwarp();
+    }
+#pragma unroll
+    for (int g = 0; g < kChunk / 16; ++g) {
+      float v[16];
+      tmem_ld_32x32b_x16(tmem + (uint32_t(quad * 32) << 16) + uint32_t(acc * kSide + c * kChunk + g * 16), v);
+      if (!ok) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(0x7fc00000u);
+      }
+      into_slot<KIND>(p, target.unscale, slot, lane, g, v);
+      if constexpr (KIND == kFinal) {
+        // columns 16 g and on are 32 bytes of each of the boxes that came in; they are 64 bytes of results, which stay in this lane's rows of both
+        *box_at(slot, lane, 2 * g) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        *box_at(slot, lane, 2 * g + 1) = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+        *box_at(slot + kBoxBytes, lane, 2 * g) = make_uint4(__float_as_uint(v[8]), __float_as_uint(v[9]), __float_as_uint(v[10]), __float_as_uint(v[11]));
+        *box_at(slot + kBoxBytes, lane, 2 * g + 1) = make_uint4(__float_as_uint(v[12]), __float_as_uint(v[13]), __float_as_uint(v[14]), __float_as_uint(v[15]));
+      }
+    }
+    const int col0 = at.n0 + c * kChunk;
+    if constexpr (KIND == kFinal) {
+      __syncwarp();
+      if (target.result != nullptr) put_results<__nv_bfloat16, true>(p, target, target.result + int64_t(at.batch) * p.M * p.N, slot, lane, row0, col0);
+      else if (target.param_dtype == NANGILA_F32) put_results<float, false>(p, target, static_cast<float*>(target.param[at.batch]), slot, lane, row0, col0);
+      else if (target.param_dtype == NANGILA_BF16) put_results<__nv_bfloat16, false>(p, target, static_cast<__nv_bfloat16*>(target.param[at.batch]), slot, lane, row0, col0);
+      else put_results<__half, false>(p, target, static_cast<__half*>(target.param[at.batch]), slot, lane, row0, col0);
+      // the slot is filled by TMA again: what was read and written here comes first
+      fence_async_proxy();
+      __syncwarp();
+    } else {
+      fence_async_proxy();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d(out, slot, col0, row0, at.batch);
+        if (KIND == kUpdate) tma_store_3d(lo, slot + kBoxBytes, col0, row0, at.batch);
+        else if (at.m0 != at.n0) tma_store_3d(mirror, slot + kBoxBytes, row0, col0, at.batch);
+        bulk_commit();
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncwarp();
+  if (lane == 0) mbar_arrive_at((PAIR ? rank0_address(&s.acc_empty[0]) : smem_u32(&s.acc_empty[0])) + uint32_t(acc) * 8);
 }
 
 // D = A B for square tiles of all matrices, walked over by CTAs that stay (PAIR: pairs of CTAs that share the tensor cores' work on 256 x 256, each
@@ -249,221 +451,51 @@ __device__ __forceinline__ void into_slot(const Product& p, uint8_t* slot, int l
 // filled and emptied by TMA, and meets no other warp.
 // A wait that runs out makes every result of this CTA from there on not a number.
 template <int KIND, bool A_MN, bool B_MN, bool PAIR>
-__global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p) {
+__global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, const __grid_constant__ Target target) {
   constexpr int kSide = PAIR ? 256 : 128;
-  constexpr int kChunks = kSide / kChunk;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* slots = smem + kStages * kStageBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(slots + kEpilogueBytes);
-  uint64_t* empty = full + kStages;
-  uint64_t* acc_full = empty + kStages;   // [2]
-  uint64_t* acc_empty = acc_full + 2;     // [2]
-  uint64_t* loaded = acc_empty + 2;       // [kEpilogueWarps]
-  uint64_t* drained = loaded + kEpilogueWarps;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
-  volatile uint32_t* failed = tmem_slot + 1;
-
+  const Shared s = shared_parts(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slabs = (p.K + kSlabK - 1) / kSlabK;
   const uint32_t rank = PAIR ? cluster_rank() : 0u;   // 0: the CTA that issues the pair's products
   const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, step = PAIR ? gridDim.x / 2 : gridDim.x;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&acc_full[s], 1);
-      mbar_init(&acc_empty[s], kEpilogueWarps * (PAIR ? 2 : 1));
-    }
-    for (int s = 0; s < kEpilogueWarps; ++s) mbar_init(&loaded[s], 1);
-    mbar_init(drained, 1);
-    *failed = 0;
-    fence_barrier_init();
+    init_barriers<PAIR>(s);
     prefetch_tensormap(&maps.a);
     prefetch_tensormap(&maps.b);
   }
   if (warp == 1) {
-    if (PAIR) tmem_alloc_pair(tmem_slot, 2 * kSide);
-    else tmem_alloc(tmem_slot, 2 * kSide);
+    if (PAIR) tmem_alloc_pair(s.tmem_slot, 2 * kSide);
+    else tmem_alloc(s.tmem_slot, 2 * kSide);
   }
   tc_fence_before_sync();
   __syncthreads();
   if (PAIR) cluster_sync();  // the other CTA's barriers exist from here on
   tc_fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = *s.tmem_slot;
   may_follow();
   follow();
 
   if (warp == 0) {
     if (lane == 0) {
-      // ---------------- TMA: both CTAs of a pair, each its own halves; the bytes are counted where the products are issued ----------------
-      int i = 0;  // slabs so far
-      bool ok = true;
-      for (int tile = first; tile < p.total && ok; tile += step) {
-        const TileAt at = tile_at<kSide>(p, tile);
-        const int row = at.m0 + int(rank) * kTileM, col = at.n0 + int(rank) * 128;
-        for (int k = 0; k < slabs; ++k, ++i) {
-          const int s = i % kStages;
-          if (i >= kStages && !mbar_wait(&empty[s], uint32_t((i / kStages - 1) & 1), kTimeoutNs)) {
-            *failed = 1;
-            ok = false;
-            break;
-          }
-          uint8_t* a = smem + s * kStageBytes;
-          uint8_t* b = a + kOperandBytes;
-          const int k0 = k * kSlabK;
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], kStageBytes * (PAIR ? 2 : 1));
-          const uint32_t bar = PAIR ? rank0_address(&full[s]) : smem_u32(&full[s]);
-          if (A_MN) {
-            tma_operand<PAIR>(a, &maps.a, row, k0, at.batch, bar);
-            tma_operand<PAIR>(a + 8192, &maps.a, row + 64, k0, at.batch, bar);
-          } else {
-            tma_operand<PAIR>(a, &maps.a, k0, row, at.batch, bar);
-          }
-          if (B_MN) {
-            tma_operand<PAIR>(b, &maps.b, col, k0, at.batch, bar);
-            tma_operand<PAIR>(b + 8192, &maps.b, col + 64, k0, at.batch, bar);
-          } else {
-            tma_operand<PAIR>(b, &maps.b, k0, col, at.batch, bar);
-          }
-        }
-      }
-      // the copies that are still under way: all have arrived when the products that read them are done; if somebody has given up, as
-      // much as can be waited for (the bytes of a pair are counted by rank 0, the stages of rank 1 are given back by its products)
-      for (int j = max(0, i - kStages); j < i; ++j) {
-        if (*failed == 0 || rank != 0) mbar_wait(&empty[j % kStages], uint32_t((j / kStages) & 1), kTimeoutNs);
-        else mbar_wait(&full[j % kStages], uint32_t((j / kStages) & 1), kTimeoutNs);
-      }
+      int i = 0;
+      for (int tile = first; tile < p.total; tile += step)
+        if (!load_tile<PAIR>(s, &maps.a, &maps.b, A_MN, B_MN, tile_at<kSide>(p, tile), rank, slabs, i)) break;
+      drain_loads(s, rank, i);
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      // ---------------- products ----------------
-      constexpr uint32_t idesc = (1u << 4) | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(kSide >> 3) << 17) | (uint32_t(kSide >> 4) << 24);
       int i = 0, n = 0;
       bool ok = true;
-      for (int tile = first; tile < p.total && ok; tile += step, ++n) {
-        const int acc = n & 1;
-        if (n >= 2 && !mbar_wait(&acc_empty[acc], uint32_t((n / 2 - 1) & 1), kTimeoutNs)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after_sync();
-        const uint32_t d = tmem + uint32_t(acc * kSide);
-        for (int k = 0; k < slabs; ++k, ++i) {
-          const int s = i % kStages;
-          if (!mbar_wait(&full[s], uint32_t((i / kStages) & 1), kTimeoutNs)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after_sync();
-          const uint32_t a = smem_u32(smem + s * kStageBytes), b = a + kOperandBytes;
-#pragma unroll
-          for (int kk = 0; kk < kSlabK / 16; ++kk) {
-            // K-major: 16 elements along K are 32 bytes of a swizzle row; MN-major: 16 K-rows are two groups of eight rows of 128 bytes
-            const uint64_t ad = A_MN ? make_smem_desc(a + kk * 2048, 8192, 1024) : make_smem_desc(a + kk * 32, 16, 1024);
-            const uint64_t bd = B_MN ? make_smem_desc(b + kk * 2048, 8192, 1024) : make_smem_desc(b + kk * 32, 16, 1024);
-            if (PAIR) umma_f16_pair(d, ad, bd, idesc, (k > 0 || kk > 0) ? 1u : 0u);
-            else umma_f16(d, ad, bd, idesc, (k > 0 || kk > 0) ? 1u : 0u);
-          }
-          if (PAIR) umma_commit_pair(&empty[s]);
-          else umma_commit(&empty[s]);
-        }
-        if (ok) {
-          if (PAIR) umma_commit_pair(&acc_full[acc]);
-          else umma_commit(&acc_full[acc]);
-        }
-      }
-      if (!ok) {
-        *failed = 1;
-        if (PAIR) umma_commit_pair(drained);
-        else umma_commit(drained);
-        mbar_wait(drained, 0, kTimeoutNs);
-      }
+      for (int tile = first; tile < p.total && ok; tile += step, ++n) ok = multiply_tile<PAIR>(s, tmem, A_MN, B_MN, slabs, n, i);
+      if (!ok) drain_products<PAIR>(s);
     }
   } else {
-    // ---------------- epilogue ----------------
-    const int quad = warp & 3;  // the lanes of tensor memory that this warp may read
-    const int turn = (warp - 2) >> 2;
-    uint8_t* slot = slots + (warp - 2) * kSlotBytes;
-    uint64_t* my_loaded = loaded + (warp - 2);
-    const uint32_t acc_empty_at = PAIR ? rank0_address(&acc_empty[0]) : smem_u32(&acc_empty[0]);
-    constexpr bool kLoads = KIND != kGram;
-    constexpr uint32_t kLoadBytes = KIND == kPoly ? kBoxBytes : kSlotBytes;
     int n = 0;
-    uint32_t chunks = 0;  // so far
-    for (int tile = first; tile < p.total; tile += step, ++n) {
-      const TileAt at = tile_at<kSide>(p, tile);
-      const int acc = n & 1;
-      const int row0 = at.m0 + int(rank) * kTileM + quad * 32;
-      const int mine = row0 < p.M ? min(kChunks, (p.N - at.n0 + kChunk - 1) / kChunk) : 0;
-      auto fetch = [&](int c) {  // lane 0: chunk c into the slot, once nothing goes out of it any more
-        bulk_wait_read();
-        mbar_arrive_expect_tx(my_loaded, kLoadBytes);
-        tma_load_3d(slot, &maps.in, at.n0 + c * kChunk, row0, at.batch, my_loaded);
-        if (KIND != kPoly) tma_load_3d(slot + kBoxBytes, &maps.lo, at.n0 + c * kChunk, row0, at.batch, my_loaded);
-      };
-      if (kLoads && turn < mine && lane == 0) fetch(turn);
-      bool ok = *failed == 0 && mbar_wait(&acc_full[acc], uint32_t((n / 2) & 1), kTimeoutNs);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) *failed = 1;
-      tc_fence_after_sync();
-#pragma unroll 1
-      for (int c = turn; c < mine; c += 2, ++chunks) {
-        if (kLoads) {
-          if (c != turn && lane == 0) fetch(c);
-          const bool here = mbar_wait(my_loaded, chunks & 1, kTimeoutNs);
-          if (!__all_sync(0xffffffffu, here)) ok = false;
-          if (!ok) *failed = 1;
-        } else {
-          if (lane == 0) bulk_wait_read();  // the slot's last stores
-          __syncwarp();
-        }
-#pragma unroll
-        for (int g = 0; g < kChunk / 16; ++g) {
-          float v[16];
-          tmem_ld_32x32b_x16(tmem + (uint32_t(quad * 32) << 16) + uint32_t(acc * kSide + c * kChunk + g * 16), v);
-          if (!ok) {
-#pragma unroll
-            for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(0x7fc00000u);
-          }
-          into_slot<KIND>(p, slot, lane, g, v);
-          if constexpr (KIND == kFinal) {
-            // columns 16 g and on are 32 bytes of each of the boxes that came in; they are 64 bytes of results, which stay in this lane's rows of both
-            *box_at(slot, lane, 2 * g) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-            *box_at(slot, lane, 2 * g + 1) = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
-            *box_at(slot + kBoxBytes, lane, 2 * g) = make_uint4(__float_as_uint(v[8]), __float_as_uint(v[9]), __float_as_uint(v[10]), __float_as_uint(v[11]));
-            *box_at(slot + kBoxBytes, lane, 2 * g + 1) = make_uint4(__float_as_uint(v[12]), __float_as_uint(v[13]), __float_as_uint(v[14]), __float_as_uint(v[15]));
-          }
-        }
-        if constexpr (KIND == kFinal) {
-          __syncwarp();
-          const int col0 = at.n0 + c * kChunk;
-          if (p.result != nullptr) put_results<__nv_bfloat16, true>(p, p.result + int64_t(at.batch) * p.M * p.N, slot, lane, row0, col0);
-          else if (p.param_dtype == NANGILA_F32) put_results<float, false>(p, static_cast<float*>(p.param[at.batch]), slot, lane, row0, col0);
-          else if (p.param_dtype == NANGILA_BF16) put_results<__nv_bfloat16, false>(p, static_cast<__nv_bfloat16*>(p.param[at.batch]), slot, lane, row0, col0);
-          else put_results<__half, false>(p, static_cast<__half*>(p.param[at.batch]), slot, lane, row0, col0);
-          // the slot is filled by TMA again: what was read and written here comes first
-          fence_async_proxy();
-          __syncwarp();
-        } else {
-          fence_async_proxy();
-          __syncwarp();
-          if (lane == 0) {
-            const int col = at.n0 + c * kChunk;
-            tma_store_3d(&maps.out, slot, col, row0, at.batch);
-            if (KIND == kUpdate) tma_store_3d(&maps.lo, slot + kBoxBytes, col, row0, at.batch);
-            else if (at.m0 != at.n0) tma_store_3d(&maps.mirror, slot + kBoxBytes, row0, col, at.batch);
-            bulk_commit();
-          }
-        }
-      }
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_at(acc_empty_at + uint32_t(acc) * 8);
-    }
+    uint32_t chunks = 0;
+    for (int tile = first; tile < p.total; tile += step, ++n)
+      finish_tile<KIND, PAIR>(s, tmem, p, target, &maps.in, &maps.lo, &maps.out, &maps.mirror, tile_at<kSide>(p, tile), rank, n, chunks);
     if (lane == 0) bulk_wait_read();  // the stores have left shared memory; the end of the kernel is what others wait for
   }
   tc_fence_before_sync();
@@ -590,6 +622,358 @@ __global__ void __launch_bounds__(kPrepT) orth_start_kernel(const __grid_constan
   }
 }
 
+// ---- matrices with a side of at most 128 ---------------------------------------------------------------------------------------------------
+// Such a matrix stays on the SMs from the gradient to the parameter, in one launch: a CTA keeps up to 384 of its rows (of the longer side) in
+// fp32 in tensor memory, and rounded to fp16 in shared memory as the products' operand; longer ones are shared out over a cluster, whose
+// CTAs add up their parts of the Gram matrix through one another's shared memory, in the order of their ranks. Every product is a few instructions of
+// 128 x 128, so what bounds this is the way from one to the next: two thirds of a step are waits for a product and the pass over its results.
+//   D = X^T X (n long, from X by rows of n: MN-major),  A = D;   D = A A,  B = b A + c D;   X <- a X + X B, accumulated onto a X in tensor memory.
+constexpr int kSmallT = 256;
+constexpr int kBlocks = 3;                       // of 128 rows in a CTA
+constexpr int kBlockBytes = 32768;               // 128 x 128 in fp16, two swizzled halves of 64 columns
+constexpr int kHalfBytes = 16384;
+constexpr int kSmallSmem = (kBlocks + 2) * kBlockBytes + 65536 + 1024 + 256;
+constexpr int kMaxCluster = 8;
+struct Small {
+  const void* grad[NANGILA_ORTH_MAX_COUNT];
+  float* momentum[NANGILA_ORTH_MAX_COUNT];
+  float coefficients[NANGILA_ORTH_MAX_STEPS][3];
+  int steps, m, n, tall, nesterov, blocks, per; // blocks of 128 along n, of a CTA
+  int vector, vector_out; // runs of four elements can be read, and written
+  float mu, eps, scale;
+};
+// Four fp32 of row r in the staging area, columns 4 c to 4 c + 3.
+__device__ __forceinline__ float4* stage_at(uint8_t* stage, int r, int c) { return reinterpret_cast<float4*>(stage + r * 512 + ((c ^ (r & 31)) << 4)); }
+__device__ __forceinline__ float* stage_one(uint8_t* stage, int r, int i) { return reinterpret_cast<float*>(stage_at(stage, r, i >> 2)) + (i & 3); }
+__device__ __forceinline__ void products_128(uint32_t d, uint32_t a, uint32_t b, bool mn, uint32_t first_accumulates) {
+  const uint32_t idesc = (1u << 4) | (uint32_t(mn) << 15) | (uint32_t(mn) << 16) | (uint32_t(128 >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) {
+    const uint32_t off = mn ? kk * 2048 : (kk >> 2) * kHalfBytes + (kk & 3) * 32;
+    const uint64_t ad = make_smem_desc(a + off, mn ? kHalfBytes : 16, 1024), bd = make_smem_desc(b + off, mn ? kHalfBytes : 16, 1024);
+    umma_f16(d, ad, bd, idesc, kk > 0 ? 1u : first_accumulates);
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(kSmallT, 1) orth_small_kernel(const __grid_constant__ Small p, const __grid_constant__ Target target) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* hi = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* a_mat = hi + kBlocks * kBlockBytes;
+  uint8_t* b_mat = a_mat + kBlockBytes;
+  uint8_t* stage = b_mat + kBlockBytes;
+  uint64_t* done = reinterpret_cast<uint64_t*>(stage + 65536);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile uint32_t* failed = tmem_slot + 1;
+  double* sums = reinterpret_cast<double*>(done + 2);            // [kMaxCluster], then a warp's each
+  double* warp_sums = sums + kMaxCluster;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int quad = warp & 3, half = warp >> 2;                   // of tensor memory's lanes; of 128 columns
+  const int row = quad * 32 + lane;                              // this thread's, wherever results are passed over
+  const uint32_t lanes = uint32_t(quad * 32) << 16;
+  const uint32_t rank = cluster_rank(), ranks = cluster_size();
+  const int batch = int(blockIdx.x / ranks);
+  const int block0 = int(rank) * p.per, mine = max(0, min(p.per, p.blocks - block0));
+
+  if (threadIdx.x == 0) {
+    mbar_init(done, 1);
+    *failed = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0) tmem_alloc(tmem_slot, 512);
+  tc_fence_before_sync();
+  cluster_sync();  // all CTAs of the cluster have started
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  uint32_t phase = 0;
+  // All wait for the products that thread 0 has just issued.
+  auto finish = [&]() {
+    if (!mbar_wait(done, phase & 1, kTimeoutNs)) *failed = 1;
+    ++phase;
+    __syncwarp();
+    tc_fence_after_sync();
+  };
+  // What the threads have written to shared and tensor memory is there for thread 0's products.
+  auto ready = [&]() {
+    fence_async_proxy();
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+  };
+  // A block's elements are passed over in runs of four, neighbours in memory (V = 4), or one by one. Run e of a block: its first row (along n), its first
+  // column, and whether it exists. (The quotient is below 128 and at least 1 / 256 away from a whole number: fp32 finds it.)
+  const float inverse_m = 1.0f / float(p.m);
+  auto place = [&](auto run, int e, int base, int& r, int& i) {
+    constexpr int V = decltype(run)::value;
+    if (p.tall) {
+      r = int((float(e * V) + 0.5f) * inverse_m);
+      i = e * V - r * p.m;
+    } else {
+      i = e / (128 / V);
+      r = e % (128 / V) * V;
+    }
+    return e < 128 / V * p.m && base + r < p.n;
+  };
+  auto address = [&](int base, int r, int i) { return p.tall ? int64_t(base + r) * p.m + i : int64_t(i) * p.n + base + r; };
+
+  // ---- the gradient, with its momentum: into tensor memory as it is, and its norm ----
+  const T* g = static_cast<const T*>(p.grad[batch]);
+  float* mom = p.momentum[batch];
+  double sum = 0.0;
+  for (int b = 0; b < mine; ++b) {
+    const int base = (block0 + b) * 128;
+    for (int c = threadIdx.x; c < 128 * 32; c += kSmallT) *stage_at(stage, c >> 5, c & 31) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    __syncthreads();
+    auto take = [&](auto run) {
+      constexpr int V = decltype(run)::value, kAhead = 8;
+      for (int e0 = threadIdx.x; e0 < 128 / V * p.m; e0 += kAhead * kSmallT) {
+        float u[kAhead][V], v[kAhead][V];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          int r, i;
+          if (!place(run, e0 + k * kSmallT, base, r, i)) continue;
+          const int64_t at = address(base, r, i);
+          if constexpr (V == 4) {
+            load4<T>(g + at, u[k]);
+            if (mom != nullptr) load4<float>(mom + at, v[k]);
+          } else {
+            u[k][0] = dev::Vec16<T>::to_float(g[at]);
+            if (mom != nullptr) v[k][0] = mom[at];
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          int r, i;
+          if (!place(run, e0 + k * kSmallT, base, r, i)) continue;
+          if (mom != nullptr) {
+#pragma unroll
+            for (int x = 0; x < V; ++x) {
+              v[k][x] = __fmaf_rn(p.mu, v[k][x], u[k][x]);
+              u[k][x] = p.nesterov ? __fmaf_rn(p.mu, v[k][x], u[k][x]) : v[k][x];
+            }
+            const int64_t at = address(base, r, i);
+            if constexpr (V == 4) store4(mom + at, v[k]);
+            else mom[at] = v[k][0];
+          }
+          if constexpr (V == 4) {
+            if (p.tall) {
+              *stage_at(stage, r, i >> 2) = make_float4(u[k][0], u[k][1], u[k][2], u[k][3]);
+            } else {
+#pragma unroll
+              for (int x = 0; x < 4; ++x) *stage_one(stage, r + x, i) = u[k][x];
+            }
+          } else {
+            *stage_one(stage, r, i) = u[k][0];
+          }
+#pragma unroll
+          for (int x = 0; x < V; ++x) sum = fma(double(u[k][x]), double(u[k][x]), sum);
+        }
+      }
+    };
+    if (p.vector) take(std::integral_constant<int, 4>{});
+    else take(std::integral_constant<int, 1>{});
+    __syncthreads();
+#pragma unroll 1
+    for (int c = 0; c < 64; c += 16) {
+      float v[16];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 f = *stage_at(stage, row, (half * 64 + c) / 4 + q);
+        v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
+      }
+      tmem_st_32x32b_x16(tmem + lanes + uint32_t(128 * (1 + b) + half * 64 + c), v);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) warp_sums[warp] = sum;
+  __syncthreads();
+  if (threadIdx.x < ranks) {
+    sum = 0.0;
+    for (int i = 0; i < kSmallT / 32; ++i) sum += warp_sums[i];
+    store_cluster(cluster_address(sums + rank, threadIdx.x), sum);  // to every CTA of the cluster
+  }
+  cluster_sync();
+  sum = 0.0;
+  for (uint32_t i = 0; i < ranks; ++i) sum += sums[i];
+  sum = sqrt(sum);
+  const float norm = float(double(p.scale) / (sum < double(p.eps) ? double(p.eps) : sum));
+
+  // X (times `f`) from tensor memory: rounded into shared memory, and a X back
+  auto round_x = [&](float f, float a) {
+    for (int b = 0; b < mine; ++b) {
+#pragma unroll 1
+      for (int c = 0; c < 64; c += 16) {
+        const uint32_t at = tmem + lanes + uint32_t(128 * (1 + b) + half * 64 + c);
+        float v[16];
+        tmem_ld_32x32b_x16(at, v);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float w[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) w[k] = v[8 * e + k] *= f;
+          *box_at(hi + b * kBlockBytes + half * kHalfBytes, row, c / 8 + e) = pack8(w);
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] *= a;
+        tmem_st_32x32b_x16(at, v);
+      }
+    }
+  };
+  round_x(norm, p.coefficients[0][0]);
+  const float unscale2 = 1.0f / (p.scale * p.scale);
+
+  for (int step = 0; step < p.steps; ++step) {
+    ready();
+    // ---- A ----
+    if (threadIdx.x == 0) {
+      for (int b = 0; b < mine; ++b) products_128(tmem, smem_u32(hi + b * kBlockBytes), smem_u32(hi + b * kBlockBytes), true, b > 0 ? 1u : 0u);
+      umma_commit(done);
+    }
+    finish();
+    if (ranks == 1) {
+#pragma unroll 1
+      for (int c = 0; c < 64; c += 16) {
+        float v[16];
+        tmem_ld_32x32b_x16(tmem + lanes + uint32_t(half * 64 + c), v);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float w[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) w[k] = v[8 * e + k] * unscale2;
+          *box_at(a_mat + half * kHalfBytes, row, c / 8 + e) = pack8(w);
+        }
+      }
+    } else {
+      // this CTA's part for the others to read; a CTA without rows has none, and its accumulator holds nothing
+      const float mul = *failed != 0 ? __uint_as_float(0x7fc00000u) : unscale2;
+#pragma unroll 1
+      for (int c = 0; c < 64; c += 16) {
+        float v[16];
+        tmem_ld_32x32b_x16(tmem + lanes + uint32_t(half * 64 + c), v);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *stage_at(stage, row, (half * 64 + c) / 4 + q) = make_float4(v[4 * q] * mul, v[4 * q + 1] * mul, v[4 * q + 2] * mul, v[4 * q + 3] * mul);
+      }
+      tc_fence_before_sync();
+      cluster_sync();
+      // 128 / ranks rows are this CTA's to add up, eight columns a thread, for all
+      const int rows = 128 / int(ranks);
+      const int parts = (p.blocks + p.per - 1) / p.per;  // CTAs with rows
+      for (int e = threadIdx.x; e < rows * 16; e += kSmallT) {
+        const int r = int(rank) * rows + (e >> 4), c = e & 15;
+        float v[8] = {};
+#pragma unroll
+        for (int i = 0; i < kMaxCluster; ++i) {
+          if (i < parts) {
+            const float4 x = load_cluster(cluster_address(stage_at(stage, r, 2 * c), uint32_t(i))), y = load_cluster(cluster_address(stage_at(stage, r, 2 * c + 1), uint32_t(i)));
+            v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+          }
+        }
+        const uint4 packed = pack8(v);
+        for (uint32_t i = 0; i < ranks; ++i) store_cluster(cluster_address(box_at(a_mat + (c >> 3) * kHalfBytes, r, c & 7), i), packed);
+      }
+      cluster_sync();
+    }
+    ready();
+    // ---- B ----
+    if (threadIdx.x == 0) {
+      products_128(tmem, smem_u32(a_mat), smem_u32(a_mat), false, 0u);
+      umma_commit(done);
+    }
+    finish();
+    const float fb = p.coefficients[step][1], fc = p.coefficients[step][2];
+#pragma unroll 1
+    for (int c = 0; c < 64; c += 16) {
+      float v[16];
+      tmem_ld_32x32b_x16(tmem + lanes + uint32_t(half * 64 + c), v);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float a[8], w[8];
+        unpack8(*box_at(a_mat + half * kHalfBytes, row, c / 8 + e), a);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = __fmaf_rn(fb, a[k], fc * v[8 * e + k]);
+        *box_at(b_mat + half * kHalfBytes, row, c / 8 + e) = pack8(w);
+      }
+    }
+    ready();
+    // ---- X ----
+    if (threadIdx.x == 0) {
+      for (int b = 0; b < mine; ++b) products_128(tmem + uint32_t(128 * (1 + b)), smem_u32(hi + b * kBlockBytes), smem_u32(b_mat), false, 1u);
+      umma_commit(done);
+    }
+    finish();
+    if (step + 1 < p.steps) round_x(1.0f, p.coefficients[step + 1][0]);
+  }
+
+  // ---- out ----
+  const bool bad = *failed != 0;
+  for (int b = 0; b < mine; ++b) {
+    const int base = (block0 + b) * 128;
+    __syncthreads();
+#pragma unroll 1
+    for (int c = 0; c < 64; c += 16) {
+      float v[16];
+      tmem_ld_32x32b_x16(tmem + lanes + uint32_t(128 * (1 + b) + half * 64 + c), v);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[k] = bad ? __uint_as_float(0x7fc00000u) : v[k] * target.unscale;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) *stage_at(stage, row, (half * 64 + c) / 4 + q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    }
+    __syncthreads();
+    auto write_runs = [&](auto* to, bool fresh, auto run) {
+      using P = std::remove_pointer_t<decltype(to)>;
+      constexpr int V = decltype(run)::value, kAhead = 8;
+      for (int e0 = threadIdx.x; e0 < 128 / V * p.m; e0 += kAhead * kSmallT) {
+        float v[kAhead][V];
+        if (!fresh) {
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) {
+            int r, i;
+            if (!place(run, e0 + k * kSmallT, base, r, i)) continue;
+            if constexpr (V == 4) load4<P>(to + address(base, r, i), v[k]);
+            else v[k][0] = dev::Vec16<P>::to_float(to[address(base, r, i)]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          int r, i;
+          if (!place(run, e0 + k * kSmallT, base, r, i)) continue;
+          float x[V];
+          if constexpr (V == 4) {
+            if (p.tall) {
+              const float4 f = *stage_at(stage, r, i >> 2);
+              x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
+            } else {
+#pragma unroll
+              for (int y = 0; y < 4; ++y) x[y] = *stage_one(stage, r + y, i);
+            }
+          } else {
+            x[0] = *stage_one(stage, r, i);
+          }
+          if (!fresh) {
+#pragma unroll
+            for (int y = 0; y < V; ++y) x[y] = v[k][y] * target.decay - target.rate * x[y];
+          }
+          if constexpr (V == 4) store4(to + address(base, r, i), x);
+          else to[address(base, r, i)] = dev::Vec16<P>::from_float(x[0]);
+        }
+      }
+    };
+    auto write = [&](auto* to, bool fresh) {
+      if (p.vector_out) write_runs(to, fresh, std::integral_constant<int, 4>{});
+      else write_runs(to, fresh, std::integral_constant<int, 1>{});
+    };
+    if (target.result != nullptr) write(target.result + int64_t(batch) * p.m * p.n, true);
+    else if (target.param_dtype == NANGILA_F32) write(static_cast<float*>(target.param[batch]), false);
+    else if (target.param_dtype == NANGILA_BF16) write(static_cast<__nv_bfloat16*>(target.param[batch]), false);
+    else write(static_cast<__half*>(target.param[batch]), false);
+  }
+  tc_fence_before_sync();
+  cluster_sync();  // nobody's shared memory goes while another may read it
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
 // ---- host ----------------------------------------------------------------------------------------------------------------------
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                               CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -629,8 +1013,21 @@ int64_t tiles_of(const Product& p, int side, int count) {
   return (p.lower ? tm * (tm + 1) / 2 : tm * tn) * count;
 }
 
+// Shared memory above the default limit, asked for once for each kernel and device.
+int allow_smem(const void* kernel, int bytes) {
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> asked;
+  int dev = 0;
+  if (const cudaError_t e = cudaGetDevice(&dev)) return int(e);
+  std::lock_guard<std::mutex> lock(mu);
+  if (asked.count({kernel, dev})) return 0;
+  if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return int(e);
+  asked.insert({kernel, dev});
+  return 0;
+}
+
 template <int KIND, bool A_MN, bool B_MN, bool PAIR>
-int launch_product(const Maps& maps, Product p, int count, cudaStream_t stream) {
+int launch_product(const Maps& maps, Product p, const Target& target, int count, cudaStream_t stream) {
   constexpr int kSide = PAIR ? 256 : 128;
   const int64_t total = tiles_of(p, kSide, count);
   if (total > 0x7fffffff) return int(cudaErrorInvalidValue);
@@ -638,17 +1035,7 @@ int launch_product(const Maps& maps, Product p, int count, cudaStream_t stream) 
   p.total = int(total);
   p.per = int(total / count);
   auto* kernel = orth_product_kernel<KIND, A_MN, B_MN, PAIR>;
-  static std::mutex mu;
-  static uint64_t opted_in = 0;  // by device
-  {
-    int dev = 0;
-    if (const cudaError_t e = cudaGetDevice(&dev)) return int(e);
-    std::lock_guard<std::mutex> lock(mu);
-    if (dev >= 64 || !((opted_in >> dev) & 1)) {
-      if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) return int(e);
-      if (dev < 64) opted_in |= uint64_t(1) << dev;
-    }
-  }
+  if (const int e = allow_smem(reinterpret_cast<const void*>(kernel), kSmem)) return e;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -663,11 +1050,11 @@ int launch_product(const Maps& maps, Product p, int count, cudaStream_t stream) 
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return int(cudaLaunchKernelEx(&cfg, kernel, maps, p));
+  return int(cudaLaunchKernelEx(&cfg, kernel, maps, p, target));
 }
 // D of the operands a and b; `in` and `lo` are what the epilogue reads, `out` what it writes.
 template <int KIND, bool A_MN, bool B_MN>
-int product(const Matrix& a, const Matrix& b, const Matrix* in, const Matrix* lo, const Matrix* out, const Product& p, int count, cudaStream_t stream) {
+int product(const Matrix& a, const Matrix& b, const Matrix* in, const Matrix* lo, const Matrix* out, const Product& p, const Target& target, int count, cudaStream_t stream) {
   Maps maps;
   bool ok = make_map(&maps.a, a, count, 64, A_MN ? 64 : 128) && make_map(&maps.b, b, count, 64, B_MN ? 64 : 128);
   ok = ok && make_map(&maps.in, in != nullptr ? *in : a, count, kChunk, 32) && make_map(&maps.lo, lo != nullptr ? *lo : a, count, kChunk, 32);
@@ -678,7 +1065,7 @@ int product(const Matrix& a, const Matrix& b, const Matrix* in, const Matrix* lo
   const int sms = sm_count();
   const int64_t small = tiles_of(p, 128, count), large = tiles_of(p, 256, count);
   const double cost_small = double((small + sms - 1) / sms), cost_large = 1.2 * double((large + sms / 2 - 1) / (sms / 2));
-  return cost_large <= cost_small ? launch_product<KIND, A_MN, B_MN, true>(maps, p, count, stream) : launch_product<KIND, A_MN, B_MN, false>(maps, p, count, stream);
+  return cost_large <= cost_small ? launch_product<KIND, A_MN, B_MN, true>(maps, p, target, count, stream) : launch_product<KIND, A_MN, B_MN, false>(maps, p, target, count, stream);
 }
 
 struct Layout {
@@ -712,6 +1099,32 @@ Layout layout(int64_t count, int64_t rows, int64_t cols) {
 }
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether a matrix stays on the SMs for all its steps, and how many CTAs it takes.
+int small_cluster(int64_t m, int64_t n) {
+  if (m > 128 || n > 128 * kBlocks * kMaxCluster) return 0;
+  const int64_t blocks = (n + 127) / 128;
+  int ctas = 1;
+  while (ctas * kBlocks < blocks) ctas *= 2;
+  return ctas;
+}
+template <typename T>
+int launch_small(const Small& p, const Target& target, int count, int cluster, cudaStream_t stream) {
+  auto* kernel = orth_small_kernel<T>;
+  if (const int e = allow_smem(reinterpret_cast<const void*>(kernel), kSmallSmem)) return e;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(cluster);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(cluster * count));
+  cfg.blockDim = dim3(kSmallT);
+  cfg.dynamicSmemBytes = kSmallSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return int(cudaLaunchKernelEx(&cfg, kernel, p, target));
+}
+
 template <typename T>
 int start(const Prep& p, int count, cudaStream_t stream) {
   const dim3 grid(unsigned(p.chunks), unsigned(count));
@@ -723,7 +1136,10 @@ int start(const Prep& p, int count, cudaStream_t stream) {
 }  // namespace
 }  // namespace nangila
 
-extern "C" int64_t nangila_orth_workspace(int32_t count, int32_t rows, int32_t cols) { return nangila::layout(count, rows, cols).total; }
+extern "C" int64_t nangila_orth_workspace(int32_t count, int32_t rows, int32_t cols) {
+  using namespace nangila;
+  return small_cluster(std::min(rows, cols), std::max(rows, cols)) != 0 ? 256 : layout(count, rows, cols).total;
+}
 
 extern "C" int nangila_orth(const NangilaOrthParams* p, cudaStream_t stream) {
   using namespace nangila;
@@ -741,6 +1157,49 @@ extern "C" int nangila_orth(const NangilaOrthParams* p, cudaStream_t stream) {
   const bool tall = p->rows > p->cols;
   float scale = 1.0f;
   while (scale * scale < float(l.n)) scale *= 2.0f;
+
+  Target target;
+  std::memset(&target, 0, sizeof target);
+  target.unscale = 1.0f / scale;
+  target.vector = p->cols % 4 == 0;
+  if (p->param[0] != nullptr) {
+    for (int i = 0; i < p->count; ++i) {
+      target.param[i] = p->param[i];
+      if (!aligned(p->param[i])) target.vector = 0;
+    }
+    target.param_dtype = p->param_dtype;
+    target.decay = p->decay;
+    target.rate = p->rate;
+  } else {
+    target.result = static_cast<__nv_bfloat16*>(p->out);
+    if (!aligned(p->out)) target.vector = 0;
+  }
+  if (p->grad_dtype < 0 || p->grad_dtype > 2 || (p->param[0] != nullptr && (p->param_dtype < 0 || p->param_dtype > 2))) return int(cudaErrorInvalidValue);
+  if (const int cluster = small_cluster(l.m, l.n)) {
+    Small s;
+    std::memset(&s, 0, sizeof s);
+    s.vector = p->cols % 4 == 0;
+    s.vector_out = target.vector;
+    for (int i = 0; i < p->count; ++i) {
+      s.grad[i] = p->grad[i];
+      s.momentum[i] = p->momentum[0] != nullptr ? p->momentum[i] : nullptr;
+      if (!aligned(p->grad[i]) || !aligned(s.momentum[i])) s.vector = 0;
+    }
+    std::memcpy(s.coefficients, p->coefficients, sizeof s.coefficients);
+    s.steps = p->steps;
+    s.m = int(l.m);
+    s.n = int(l.n);
+    s.tall = tall ? 1 : 0;
+    s.nesterov = p->nesterov;
+    s.blocks = int((l.n + 127) / 128);
+    s.per = (s.blocks + cluster - 1) / cluster;
+    s.mu = p->mu;
+    s.eps = p->eps;
+    s.scale = scale;
+    return p->grad_dtype == NANGILA_F32   ? launch_small<float>(s, target, p->count, cluster, stream)
+           : p->grad_dtype == NANGILA_F16 ? launch_small<__half>(s, target, p->count, cluster, stream)
+                                          : launch_small<__nv_bfloat16>(s, target, p->count, cluster, stream);
+  }
 
   Prep prep;
   std::memset(&prep, 0, sizeof prep);
@@ -769,6 +1228,7 @@ extern "C" int nangila_orth(const NangilaOrthParams* p, cudaStream_t stream) {
     case NANGILA_BF16: e = start<__nv_bfloat16>(prep, p->count, stream); break;
     default: return int(cudaErrorInvalidValue);
   }
+  if (e != 0) return e;
   const Matrix A{gram, l.m, l.m, l.ldm, l.s}, B{poly, l.m, l.m, l.ldm, l.s}, Lo{lo, p->rows, p->cols, l.ld, l.x};
   for (int step = 0; step < p->steps && e == 0; ++step) {
     const float* c = p->coefficients[step];
@@ -780,35 +1240,21 @@ extern "C" int nangila_orth(const NangilaOrthParams* p, cudaStream_t stream) {
     q.lower = 1;
     q.K = int(l.n);
     q.alpha = 1.0f / (scale * scale);
-    e = tall ? product<kGram, true, true>(X, X, nullptr, nullptr, &A, q, p->count, stream) : product<kGram, false, false>(X, X, nullptr, nullptr, &A, q, p->count, stream);
+    e = tall ? product<kGram, true, true>(X, X, nullptr, nullptr, &A, q, target, p->count, stream) : product<kGram, false, false>(X, X, nullptr, nullptr, &A, q, target, p->count, stream);
     if (e != 0) break;
     q.K = int(l.m);
     q.alpha = c[1];
     q.beta = c[2];
-    e = product<kPoly, false, false>(A, A, &A, nullptr, &B, q, p->count, stream);
+    e = product<kPoly, false, false>(A, A, &A, nullptr, &B, q, target, p->count, stream);
     if (e != 0) break;
     q.lower = 0;
     q.M = p->rows;
     q.N = p->cols;
     q.alpha = c[0];
     if (last) {
-      q.unscale = 1.0f / scale;
-      q.vector = p->cols % 4 == 0;
-      if (p->param[0] != nullptr) {
-        for (int i = 0; i < p->count; ++i) {
-          q.param[i] = p->param[i];
-          if (!aligned(p->param[i])) q.vector = 0;
-        }
-        q.param_dtype = p->param_dtype;
-        q.decay = p->decay;
-        q.rate = p->rate;
-      } else {
-        q.result = static_cast<__nv_bfloat16*>(p->out);
-        if (!aligned(p->out)) q.vector = 0;
-      }
-      e = tall ? product<kFinal, false, false>(X, B, &X, &Lo, nullptr, q, p->count, stream) : product<kFinal, false, true>(B, X, &X, &Lo, nullptr, q, p->count, stream);
+      e = tall ? product<kFinal, false, false>(X, B, &X, &Lo, nullptr, q, target, p->count, stream) : product<kFinal, false, true>(B, X, &X, &Lo, nullptr, q, target, p->count, stream);
     } else {
-      e = tall ? product<kUpdate, false, false>(X, B, &X, &Lo, &Next, q, p->count, stream) : product<kUpdate, false, true>(B, X, &X, &Lo, &Next, q, p->count, stream);
+      e = tall ? product<kUpdate, false, false>(X, B, &X, &Lo, &Next, q, target, p->count, stream) : product<kUpdate, false, true>(B, X, &X, &Lo, &Next, q, target, p->count, stream);
     }
   }
   return e;

@@ -8,7 +8,7 @@ formula in float32.
 from __future__ import annotations
 
 import math
-from typing import Dict, List, Sequence, Tuple, Union
+from typing import List, Sequence, Tuple, Union
 
 import torch
 
@@ -18,7 +18,6 @@ from ._native import glue
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 MAX_STEPS = 32
 SCALES = ("spectral", "rms", None)
-_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 _Coefficients = Union[Tuple[float, float, float], Sequence[Tuple[float, float, float]]]
 
 
@@ -36,13 +35,10 @@ def _schedule(steps: int, coefficients: _Coefficients) -> List[float]:
     return flat
 
 
-def _check_matrix(t: torch.Tensor, name: str) -> None:
-    if not isinstance(t, torch.Tensor) or type(t).__name__ == "DTensor":
-        raise TypeError(f"nangila: {name} must be plain tensors (a sharded matrix has to be gathered first), got {type(t).__name__}")
-    if t.dtype not in _TYPES or t.layout != torch.strided or t.device.type not in ("cuda", "cpu"):
-        raise TypeError(f"nangila: {name} must be dense float32, float16 or bfloat16 CUDA or CPU tensors, got {t.dtype} on {t.device}")
-    if t.dim() != 2 or not 1 <= t.size(0) <= 65536 or not 1 <= t.size(1) <= 65536:
-        raise ValueError(f"nangila: {name} must be matrices of 1 x 1 to 65536 x 65536, got shape {tuple(t.shape)}")
+def _plain_tensors(ts: Sequence[torch.Tensor], name: str) -> None:
+    for t in ts:
+        if not isinstance(t, torch.Tensor) or type(t).__name__ == "DTensor":
+            raise TypeError(f"nangila: {name} must be plain tensors (a sharded matrix has to be gathered first), got {type(t).__name__}")
 
 
 def _check_eps(eps: float) -> None:
@@ -72,30 +68,26 @@ def orthogonalize(update: Union[torch.Tensor, Sequence[torch.Tensor]], steps: in
     flat = _schedule(steps, coefficients)
     _check_eps(eps)
     if isinstance(update, torch.Tensor):
-        if update.dim() == 3 and update.size(0) == 0:
-            _check_matrix(update.new_empty(update.shape[1:]), "updates")
+        _plain_tensors([update], "updates")
+        stack = update.dim() == 3
+        many = list(update.unbind(0)) if stack else [update]
+        glue().group_matrices(many or [update.new_empty(update.shape[1:])])
+        if not many:
             return update.new_empty(update.shape, dtype=torch.bfloat16)
-        many = list(update.unbind(0)) if update.dim() == 3 else [update]
-        for t in many:
-            _check_matrix(t, "updates")
         if update.is_cuda:
             out = glue().orth([t.contiguous() for t in many], [], [], flat, eps)
         else:
             out = torch.stack([_plain(t, flat, eps).to(torch.bfloat16) for t in many])
-        return out if update.dim() == 3 else out[0]
+        return out if stack else out[0]
     many = list(update)
-    for t in many:
-        _check_matrix(t, "updates")
-    groups: Dict[tuple, List[int]] = {}
-    for i, t in enumerate(many):
-        groups.setdefault((t.shape, t.dtype, t.device), []).append(i)
+    _plain_tensors(many, "updates")
     results: List[torch.Tensor] = [None] * len(many)  # type: ignore[list-item]
-    for (_, _, device), members in groups.items():
-        if device.type == "cuda":
-            stack = glue().orth([many[i].contiguous() for i in members], [], [], flat, eps).unbind(0)
+    for members in glue().group_matrices(many):
+        if many[members[0]].is_cuda:
+            parts = glue().orth([many[i].contiguous() for i in members], [], [], flat, eps).unbind(0)
         else:
-            stack = [_plain(many[i], flat, eps).to(torch.bfloat16) for i in members]
-        for i, t in zip(members, stack):
+            parts = [_plain(many[i], flat, eps).to(torch.bfloat16) for i in members]
+        for i, t in zip(members, parts):
             results[i] = t
     return results
 
@@ -131,32 +123,19 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
         if not (math.isfinite(v) and v >= 0):
             raise ValueError(f"nangila: {name} must be finite and not negative, got {v}")
     params, grads, momenta = list(params), list(grads), list(momenta)
-    if not len(params) == len(grads) == len(momenta):
-        raise ValueError(f"nangila: {len(params)} parameters, {len(grads)} gradients and {len(momenta)} momenta")
-    groups: Dict[tuple, List[int]] = {}
-    for i, (p, g, m) in enumerate(zip(params, grads, momenta)):
-        for t, name in ((p, "parameters"), (g, "gradients"), (m, "momenta")):
-            _check_matrix(t, name)
-        if not p.shape == g.shape == m.shape or not p.device == g.device == m.device:
-            raise ValueError(f"nangila: parameter {i} is {tuple(p.shape)} on {p.device}, its gradient {tuple(g.shape)} on {g.device}, "
-                             f"its momentum {tuple(m.shape)} on {m.device}")
-        if m.dtype != torch.float32:
-            raise TypeError(f"nangila: momenta must be float32, got {m.dtype}")
-        if not p.is_contiguous() or not m.is_contiguous():
-            raise ValueError(f"nangila: parameter {i} and its momentum must be packed (contiguous)")
-        groups.setdefault((p.shape, p.dtype, g.dtype, p.device), []).append(i)
+    for name, ts in (("parameters", params), ("gradients", grads), ("momenta", momenta)):
+        _plain_tensors(ts, name)
     update_scale(1, 1, scale)
-    if glue().overlapping(params + momenta, grads):
-        raise ValueError("nangila: parameters and momenta must not share memory with one another or with the gradients")
-    for (shape, _, _, device), members in groups.items():
-        rate, decay = lr * update_scale(shape[0], shape[1], scale), 1.0 - lr * weight_decay
-        if device.type == "cuda":
-            glue().orth([grads[i].contiguous() for i in members], [momenta[i] for i in members], [params[i] for i in members], flat, eps, momentum, nesterov,
-                         decay, rate)
+    for members in glue().group_muon(params, grads, momenta):
+        first = params[members[0]]
+        rate, decay = lr * update_scale(first.size(0), first.size(1), scale), 1.0 - lr * weight_decay
+        ps, gs, ms = [params[i] for i in members], [grads[i] for i in members], [momenta[i] for i in members]
+        if first.is_cuda:
+            glue().orth([g.contiguous() for g in gs], ms, ps, flat, eps, momentum, nesterov, decay, rate)
             # the kernels write where autograd does not look: what was saved for a backward pass is not what it was
-            torch.autograd.graph.increment_version([t for i in members for t in (params[i], momenta[i]) if not t.is_inference()])
+            torch.autograd.graph.increment_version([t for t in ps + ms if not t.is_inference()])
             continue
-        for i in members:
-            momenta[i].mul_(momentum).add_(grads[i])
-            u = momenta[i] * momentum + grads[i] if nesterov else momenta[i]
-            params[i].copy_(params[i].float() * decay - rate * _plain(u, flat, eps))
+        for p, g, m in zip(ps, gs, ms):
+            m.mul_(momentum).add_(g)
+            u = m * momentum + g if nesterov else m
+            p.copy_(p.float() * decay - rate * _plain(u, flat, eps))
