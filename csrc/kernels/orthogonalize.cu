@@ -53,6 +53,7 @@ constexpr int kSmem = kStages * kStageBytes + kEpilogueBytes + 1024 + 256;
 constexpr int kGemmThreads = 64 + 32 * kEpilogueWarps;  // warp 0: TMA, warp 1: products, the others: epilogue
 constexpr uint64_t kTimeoutNs = 10ull * 1000 * 1000 * 1000;
 constexpr float kLoScale = 2048.0f;
+constexpr int kMaxCluster = 8;
 
 enum Kind { kGram, kPoly, kUpdate, kFinal };
 
@@ -290,7 +291,7 @@ __device__ __forceinline__ void init_barriers(const Shared& s) {
 // TMA of a tile's slabs, `i` of which have gone before: both CTAs of a pair, each its own halves; the bytes are counted where the products are issued.
 // False when a wait has run out.
 template <bool PAIR>
-__device__ __forceinline__ bool load_tile(const Shared& s, const CUtensorMap* a_map, const CUtensorMap* b_map, bool a_mn, bool b_mn, const TileAt& at, uint32_t rank, int slabs, int& i) {
+__device__ __forceinline__ bool load_tile(const Shared& s, const CUtensorMap* a_map, const CUtensorMap* b_map, bool a_mn, bool b_mn, const TileAt& at, uint32_t rank, int slabs, int& i, int slab0 = 0) {
   const int row = at.m0 + int(rank) * kTileM, col = at.n0 + int(rank) * 128;
   for (int k = 0; k < slabs; ++k, ++i) {
     const int st = i % kStages;
@@ -300,7 +301,7 @@ __device__ __forceinline__ bool load_tile(const Shared& s, const CUtensorMap* a_
     }
     uint8_t* a = s.stages + st * kStageBytes;
     uint8_t* b = a + kOperandBytes;
-    const int k0 = k * kSlabK;
+    const int k0 = (slab0 + k) * kSlabK;
     if (rank == 0) mbar_arrive_expect_tx(&s.full[st], kStageBytes * (PAIR ? 2 : 1));
     const uint32_t bar = PAIR ? rank0_address(&s.full[st]) : smem_u32(&s.full[st]);
     if (a_mn) {
@@ -465,6 +466,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __g
     prefetch_tensormap(&maps.a);
     prefetch_tensormap(&maps.b);
   }
+  if (threadIdx.x == 64) {
+    if (KIND != kGram) prefetch_tensormap(&maps.in);
+    if (KIND == kUpdate || KIND == kFinal) prefetch_tensormap(&maps.lo);
+    if (KIND != kFinal) prefetch_tensormap(&maps.out);
+    if (KIND == kGram || KIND == kPoly) prefetch_tensormap(&maps.mirror);
+  }
   if (warp == 1) {
     if (PAIR) tmem_alloc_pair(s.tmem_slot, 2 * kSide);
     else tmem_alloc(s.tmem_slot, 2 * kSide);
@@ -505,6 +512,107 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __g
     if (PAIR) tmem_dealloc_pair(tmem, 2 * kSide);
     else tmem_dealloc(tmem, 2 * kSide);
   }
+}
+
+// The Gram matrix where few tiles share a long K: a cluster takes a tile, each CTA a part of K and, in the end, 128 / S columns of the result. The parts
+// meet through shared memory, in the order of the ranks.
+template <bool MN>
+__global__ void __launch_bounds__(kGemmThreads, 1) orth_gram_split_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, __half* __restrict__ out, int64_t ld, int64_t matrix) {
+  extern __shared__ uint8_t smem_raw[];
+  const Shared s = shared_parts(smem_raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank(), ranks = cluster_size();
+  const int slabs = (p.K + kSlabK - 1) / kSlabK;
+  const int slab0 = int(rank) * slabs / int(ranks), mine = (int(rank) + 1) * slabs / int(ranks) - slab0;  // one at least
+  const TileAt at = tile_at<128>(p, int(blockIdx.x / ranks));
+  const int width = 128 / int(ranks), pitch = width * 4;   // columns of a CTA; bytes of a row of theirs, fp32
+  auto part_at = [&](uint32_t from, int row, int j) {      // sixteen bytes `j` of what rank `from` sends, in the slots of the CTA whose columns they are
+    return s.slots + from * uint32_t(128 * pitch) + row * pitch + ((j ^ (row & (pitch / 16 - 1))) << 4);
+  };
+
+  if (threadIdx.x == 0) {
+    init_barriers<false>(s);
+    prefetch_tensormap(&maps.a);
+    prefetch_tensormap(&maps.b);
+  }
+  if (warp == 1) tmem_alloc(s.tmem_slot, 256);
+  tc_fence_before_sync();
+  cluster_sync();
+  tc_fence_after_sync();
+  const uint32_t tmem = *s.tmem_slot;
+  may_follow();
+  follow();
+
+  const int quad = warp & 3, turn = (warp - 2) >> 2, row = quad * 32 + lane;
+  if (warp == 0) {
+    if (lane == 0) {
+      int i = 0;
+      load_tile<false>(s, &maps.a, &maps.b, MN, MN, at, 0, mine, i, slab0);
+      drain_loads(s, 0, i);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int i = 0;
+      if (!multiply_tile<false>(s, tmem, MN, MN, mine, 0, i)) drain_products<false>(s);
+    }
+  } else {
+    bool ok = mbar_wait(&s.acc_full[0], 0, kTimeoutNs);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) *s.failed = 1;
+    tc_fence_after_sync();
+    // sixteen columns at a time: to whom they belong, the groups shared out between the two warps of a quarter
+    for (int g = turn; g < 8; g += 2) {
+      const uint32_t owner = uint32_t(g * 16 / width);
+      if (owner == rank) continue;
+      float v[16];
+      tmem_ld_32x32b_x16(tmem + (uint32_t(quad * 32) << 16) + uint32_t(g * 16), v);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float4 f = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        if (!ok) f.x = f.y = f.z = f.w = __uint_as_float(0x7fc00000u);
+        store_cluster(cluster_address(part_at(rank, row, (g * 16 % width) / 4 + q), owner), *reinterpret_cast<const uint4*>(&f));
+      }
+    }
+  }
+  __syncwarp();
+  cluster_sync();
+  if (warp >= 2) {
+    const bool ok = *s.failed == 0;
+    // this CTA's columns, eight at a time
+    for (int c = turn * 8; c < width; c += 16) {
+      float v[8], own[8];
+      tmem_ld_32x32b_x8(tmem + (uint32_t(quad * 32) << 16) + uint32_t(int(rank) * width + c), own);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+      for (uint32_t from = 0; from < ranks; ++from) {
+        float4 x, y;
+        if (from == rank) {
+          x = make_float4(own[0], own[1], own[2], own[3]);
+          y = make_float4(own[4], own[5], own[6], own[7]);
+        } else {
+          x = *reinterpret_cast<const float4*>(part_at(from, row, c / 4));
+          y = *reinterpret_cast<const float4*>(part_at(from, row, c / 4 + 1));
+        }
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = ok ? v[k] * p.alpha : __uint_as_float(0x7fc00000u);
+      const int r = at.m0 + row, col = at.n0 + int(rank) * width + c;
+      if (r < p.M && col < p.N) {  // rows of `out` are padded to eight
+        __half* to = out + at.batch * matrix;
+        *reinterpret_cast<uint4*>(to + int64_t(r) * ld + col) = pack8(v);
+        if (at.m0 != at.n0) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (col + k < p.N) to[int64_t(col + k) * ld + r] = __float2half_rn(v[k]);
+        }
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 256);
 }
 
 // ---- from the gradients to X -------------------------------------------------------------------------------------------------
@@ -633,7 +741,6 @@ constexpr int kBlocks = 3;                       // of 128 rows in a CTA
 constexpr int kBlockBytes = 32768;               // 128 x 128 in fp16, two swizzled halves of 64 columns
 constexpr int kHalfBytes = 16384;
 constexpr int kSmallSmem = (kBlocks + 2) * kBlockBytes + 65536 + 1024 + 256;
-constexpr int kMaxCluster = 8;
 struct Small {
   const void* grad[NANGILA_ORTH_MAX_COUNT];
   float* momentum[NANGILA_ORTH_MAX_COUNT];
@@ -862,12 +969,19 @@ __global__ void __launch_bounds__(kSmallT, 1) orth_small_kernel(const __grid_con
       const int parts = (p.blocks + p.per - 1) / p.per;  // CTAs with rows
       for (int e = threadIdx.x; e < rows * 16; e += kSmallT) {
         const int r = int(rank) * rows + (e >> 4), c = e & 15;
+        float4 x[kMaxCluster], y[kMaxCluster];
+#pragma unroll
+        for (int i = 0; i < kMaxCluster; ++i) {
+          if (i < parts) {
+            x[i] = load_cluster(cluster_address(stage_at(stage, r, 2 * c), uint32_t(i)));
+            y[i] = load_cluster(cluster_address(stage_at(stage, r, 2 * c + 1), uint32_t(i)));
+          }
+        }
         float v[8] = {};
 #pragma unroll
         for (int i = 0; i < kMaxCluster; ++i) {
           if (i < parts) {
-            const float4 x = load_cluster(cluster_address(stage_at(stage, r, 2 * c), uint32_t(i))), y = load_cluster(cluster_address(stage_at(stage, r, 2 * c + 1), uint32_t(i)));
-            v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+            v[0] += x[i].x; v[1] += x[i].y; v[2] += x[i].z; v[3] += x[i].w; v[4] += y[i].x; v[5] += y[i].y; v[6] += y[i].z; v[7] += y[i].w;
           }
         }
         const uint4 packed = pack8(v);
@@ -1049,8 +1163,30 @@ int launch_product(const Maps& maps, Product p, const Target& target, int count,
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = PAIR ? 2 : 1;
   return int(cudaLaunchKernelEx(&cfg, kernel, maps, p, target));
+}
+template <bool MN>
+int launch_gram_split(const Maps& maps, Product p, const Matrix& out, int total, int per, int split, cudaStream_t stream) {
+  auto* kernel = orth_gram_split_kernel<MN>;
+  if (const int e = allow_smem(reinterpret_cast<const void*>(kernel), kSmem)) return e;
+  p.tiles_m = (p.M + 127) / 128;
+  p.total = total;
+  p.per = per;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(split);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(total * split));
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return int(cudaLaunchKernelEx(&cfg, kernel, maps, p, const_cast<__half*>(out.base), out.ld, out.matrix));
 }
 // D of the operands a and b; `in` and `lo` are what the epilogue reads, `out` what it writes.
 template <int KIND, bool A_MN, bool B_MN>
@@ -1064,6 +1200,13 @@ int product(const Matrix& a, const Matrix& b, const Matrix* in, const Matrix* lo
   // epilogue is longer. So it is the number of rounds that decides.
   const int sms = sm_count();
   const int64_t small = tiles_of(p, 128, count), large = tiles_of(p, 256, count);
+  if constexpr (KIND == kGram) {
+    // A CTA's share of K is 8 slabs (2 us) at least: what the meeting costs. Three quarters of the SMs: clusters of eight do not fit into all of them.
+    const int64_t slabs = (p.K + kSlabK - 1) / kSlabK;
+    int split = 1;
+    while (split < kMaxCluster && small * split * 2 <= sms * 3 / 4 && slabs >= split * 2 * 8) split *= 2;
+    if (split > 1) return launch_gram_split<A_MN>(maps, p, *out, int(small), int(small / count), split, stream);
+  }
   const double cost_small = double((small + sms - 1) / sms), cost_large = 1.2 * double((large + sms / 2 - 1) / (sms / 2));
   return cost_large <= cost_small ? launch_product<KIND, A_MN, B_MN, true>(maps, p, target, count, stream) : launch_product<KIND, A_MN, B_MN, false>(maps, p, target, count, stream);
 }
