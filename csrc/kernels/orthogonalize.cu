@@ -445,6 +445,19 @@ __device__ __forceinline__ void finish_tile(const Shared& s, uint32_t tmem, cons
   if (lane == 0) mbar_arrive_at((PAIR ? rank0_address(&s.acc_empty[0]) : smem_u32(&s.acc_empty[0])) + uint32_t(acc) * 8);
 }
 
+// The sum of a few squares: in fp32 where they fit into its range, else in 64 bits.
+template <int N>
+__device__ __forceinline__ double square_sum(const float (&u)[N]) {
+  float q = 0.0f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) q = __fmaf_rn(u[k], u[k], q);
+  if (q > 1e-28f && q < 1e38f) return double(q);
+  double d = 0.0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) d = fma(double(u[k]), double(u[k]), d);
+  return d;
+}
+
 // D = A B for square tiles of all matrices, walked over by CTAs that stay (PAIR: pairs of CTAs that share the tensor cores' work on 256 x 256, each
 // with its 128 rows of A, half of B's columns, and 128 rows of the result; else one CTA and 128 x 128). A_MN / B_MN: the operand lies with its rows
 // (columns of B) adjacent in memory, not its K. The accumulators of two tiles share tensor memory: the epilogue of one runs under the
@@ -662,16 +675,7 @@ __global__ void __launch_bounds__(kPrepT) orth_norm_kernel(const __grid_constant
       }
       dev::Vec8<float>::store(m + i * 8, v);
     }
-    // eight squares in fp32 where they fit into its range, else in 64 bits
-    float q = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) q = __fmaf_rn(u[k], u[k], q);
-    if (q > 1e-28f && q < 1e38f) {
-      sum += double(q);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sum = fma(double(u[k]), double(u[k]), sum);
-    }
+    sum += square_sum(u);
   }
   for (int64_t i = runs * 8 + first; i < p.numel; i += stride) {
     float u = dev::Vec16<T>::to_float(g[i]);
@@ -749,8 +753,8 @@ struct Small {
   int vector, vector_out; // runs of four elements can be read, and written
   float mu, eps, scale;
 };
-// Four fp32 of row r in the staging area, columns 4 c to 4 c + 3.
-__device__ __forceinline__ float4* stage_at(uint8_t* stage, int r, int c) { return reinterpret_cast<float4*>(stage + r * 512 + ((c ^ (r & 31)) << 4)); }
+// Four fp32 of row r in the staging area, columns 4 c to 4 c + 3: neighbouring rows, and every fourth, in different banks.
+__device__ __forceinline__ float4* stage_at(uint8_t* stage, int r, int c) { return reinterpret_cast<float4*>(stage + r * 512 + ((c ^ ((r ^ (r >> 2)) & 31)) << 4)); }
 __device__ __forceinline__ float* stage_one(uint8_t* stage, int r, int i) { return reinterpret_cast<float*>(stage_at(stage, r, i >> 2)) + (i & 3); }
 __device__ __forceinline__ void products_128(uint32_t d, uint32_t a, uint32_t b, bool mn, uint32_t first_accumulates) {
   const uint32_t idesc = (1u << 4) | (uint32_t(mn) << 15) | (uint32_t(mn) << 16) | (uint32_t(128 >> 3) << 17) | (uint32_t(128 >> 4) << 24);
@@ -829,8 +833,10 @@ __global__ void __launch_bounds__(kSmallT, 1) orth_small_kernel(const __grid_con
   double sum = 0.0;
   for (int b = 0; b < mine; ++b) {
     const int base = (block0 + b) * 128;
-    for (int c = threadIdx.x; c < 128 * 32; c += kSmallT) *stage_at(stage, c >> 5, c & 31) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    __syncthreads();
+    if (p.m < 128 || base + 128 > p.n) {  // what lies outside of the matrix
+      for (int c = threadIdx.x; c < 128 * 32; c += kSmallT) *stage_at(stage, c >> 5, c & 31) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      __syncthreads();
+    }
     auto take = [&](auto run) {
       constexpr int V = decltype(run)::value, kAhead = 8;
       for (int e0 = threadIdx.x; e0 < 128 / V * p.m; e0 += kAhead * kSmallT) {
@@ -872,8 +878,7 @@ __global__ void __launch_bounds__(kSmallT, 1) orth_small_kernel(const __grid_con
           } else {
             *stage_one(stage, r, i) = u[k][0];
           }
-#pragma unroll
-          for (int x = 0; x < V; ++x) sum = fma(double(u[k][x]), double(u[k][x]), sum);
+          sum += square_sum(u[k]);
         }
       }
     };
@@ -953,35 +958,34 @@ __global__ void __launch_bounds__(kSmallT, 1) orth_small_kernel(const __grid_con
         }
       }
     } else {
-      // this CTA's part for the others to read; a CTA without rows has none, and its accumulator holds nothing
-      const float mul = *failed != 0 ? __uint_as_float(0x7fc00000u) : unscale2;
+      // 128 / ranks rows are each CTA's to add up, for all: the others' parts of them go into its staging area, [rank][row]. (A CTA without rows has none to
+      // send, and its accumulator holds nothing.)
+      const int rows = 128 / int(ranks), parts = (p.blocks + p.per - 1) / p.per;  // CTAs with rows
+      if (int(rank) < parts) {
+        const float mul = *failed != 0 ? __uint_as_float(0x7fc00000u) : unscale2;
+        const uint32_t owner = uint32_t(row / rows);
+        const int at = int(rank) * rows + row % rows;
 #pragma unroll 1
-      for (int c = 0; c < 64; c += 16) {
-        float v[16];
-        tmem_ld_32x32b_x16(tmem + lanes + uint32_t(half * 64 + c), v);
+        for (int c = 0; c < 64; c += 16) {
+          float v[16];
+          tmem_ld_32x32b_x16(tmem + lanes + uint32_t(half * 64 + c), v);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) *stage_at(stage, row, (half * 64 + c) / 4 + q) = make_float4(v[4 * q] * mul, v[4 * q + 1] * mul, v[4 * q + 2] * mul, v[4 * q + 3] * mul);
+          for (int q = 0; q < 4; ++q) {
+            const float4 f = make_float4(v[4 * q] * mul, v[4 * q + 1] * mul, v[4 * q + 2] * mul, v[4 * q + 3] * mul);
+            store_cluster(cluster_address(stage_at(stage, at, (half * 64 + c) / 4 + q), owner), *reinterpret_cast<const uint4*>(&f));
+          }
+        }
       }
       tc_fence_before_sync();
       cluster_sync();
-      // 128 / ranks rows are this CTA's to add up, eight columns a thread, for all
-      const int rows = 128 / int(ranks);
-      const int parts = (p.blocks + p.per - 1) / p.per;  // CTAs with rows
       for (int e = threadIdx.x; e < rows * 16; e += kSmallT) {
-        const int r = int(rank) * rows + (e >> 4), c = e & 15;
-        float4 x[kMaxCluster], y[kMaxCluster];
-#pragma unroll
-        for (int i = 0; i < kMaxCluster; ++i) {
-          if (i < parts) {
-            x[i] = load_cluster(cluster_address(stage_at(stage, r, 2 * c), uint32_t(i)));
-            y[i] = load_cluster(cluster_address(stage_at(stage, r, 2 * c + 1), uint32_t(i)));
-          }
-        }
+        const int own = e >> 4, r = int(rank) * rows + own, c = e & 15;  // eight columns
         float v[8] = {};
 #pragma unroll
         for (int i = 0; i < kMaxCluster; ++i) {
           if (i < parts) {
-            v[0] += x[i].x; v[1] += x[i].y; v[2] += x[i].z; v[3] += x[i].w; v[4] += y[i].x; v[5] += y[i].y; v[6] += y[i].z; v[7] += y[i].w;
+            const float4 x = *stage_at(stage, i * rows + own, 2 * c), y = *stage_at(stage, i * rows + own, 2 * c + 1);
+            v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
           }
         }
         const uint4 packed = pack8(v);
