@@ -111,6 +111,7 @@ def build_llama(args, dev, world):
     from nangila.models.llama import Llama, LlamaConfig
 
     cfg = LlamaConfig.tiny() if args.small else LlamaConfig.llama_1_3b()
+    cfg.fused = args.fused
     model = Llama(cfg).to(dev)
     mp = MixedPrecisionPolicy(param_dtype=torch.bfloat16, reduce_dtype=torch.bfloat16)
     for blk in model.blocks:
@@ -168,6 +169,7 @@ def main() -> int:
     ap.add_argument("--warmup", type=int, default=4)
     ap.add_argument("--small", action="store_true")
     ap.add_argument("--no-e2e", action="store_true")
+    ap.add_argument("--fused", action="store_true", help="Llama configuration: norms and rotary positions through nangila.ops (either arm)")
     ap.add_argument("--bucket-mb", type=int, default=25, help="DDP bucket size of the BERT configuration")
     args = ap.parse_args()
     args.warmup = max(args.warmup, 3)

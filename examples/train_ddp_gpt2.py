@@ -21,6 +21,7 @@ from torch.nn.parallel import DistributedDataParallel as DDP  # noqa: E402
 from nangila import CompressorType  # noqa: E402
 from nangila.ddp import register_nangila_hook  # noqa: E402
 from nangila.models.gpt2 import GPT2, GPT2Config  # noqa: E402
+from nangila.optim import Muon  # noqa: E402
 from nangila.utils import init_distributed, seed_everything  # noqa: E402
 
 COMPRESSORS = {"predres": CompressorType.PredictionResidual, "dgc": CompressorType.DGC, "powersgd": CompressorType.PowerSGD}
@@ -33,6 +34,8 @@ def main() -> int:
     ap.add_argument("--compressor", default="predres", choices=sorted(COMPRESSORS))
     ap.add_argument("--tiny", action="store_true")
     ap.add_argument("--micro-batch", type=int, default=8)
+    ap.add_argument("--optimizer", default="adamw", choices=["adamw", "muon"],
+                    help="muon: the blocks' matrices take Muon steps, everything else stays with AdamW")
     ap.add_argument("--checkpoint", default="")
     ap.add_argument("--save-every", type=int, default=50)
     ap.add_argument("--liveness-timeout", type=float, default=0.0,
@@ -49,13 +52,18 @@ def main() -> int:
                                  compressor_type=int(COMPRESSORS[args.compressor]), dgc_sparsity=0.999, power_sgd_rank=4,
                                  liveness_timeout=args.liveness_timeout or None)
     hook.enable_safe_mode()  # falls back to exact averaging if the validation loss diverges
-    opt = torch.optim.AdamW(ddp.parameters(), lr=3e-4, weight_decay=0.01)
+    matrices = [p for p in model.blocks.parameters() if p.dim() == 2] if args.optimizer == "muon" else []
+    held = {id(p) for p in matrices}
+    opt = torch.optim.AdamW([p for p in ddp.parameters() if id(p) not in held], lr=3e-4, weight_decay=0.01)
+    muon = Muon(matrices, lr=3e-4, weight_decay=0.01) if matrices else None
     start = 0
     path = f"{args.checkpoint}.rank{rank}" if args.checkpoint else ""
     if path and os.path.exists(path):
         ck = torch.load(path, map_location=dev, weights_only=False)
         model.load_state_dict(ck["model"])
         opt.load_state_dict(ck["opt"])
+        if muon is not None:
+            muon.load_state_dict(ck["muon"])
         hook.load_state_dict(ck["hook"])
         start = ck["step"]
     gen = torch.Generator().manual_seed(1234 + rank)
@@ -65,8 +73,10 @@ def main() -> int:
         try:
             loss = ddp(tok[:, :-1], tok[:, 1:])
             loss.backward()
-            opt.step()
-            opt.zero_grad(set_to_none=True)
+            for o in (opt, muon):
+                if o is not None:
+                    o.step()
+                    o.zero_grad(set_to_none=True)
             hook.step()   # with heartbeats on, raises RankFailure when a peer has left
         except RuntimeError:
             hook.check_peers(wait=2.0 * args.liveness_timeout)   # a failed collective: say which rank it was, if one is gone
@@ -78,7 +88,8 @@ def main() -> int:
                 print(f"step {step:5d}  loss {float(loss):.4f}  compressing {st['compression_enabled']}  "
                       f"ratio {st.get('overall_compression_ratio', 1.0):.2f}")
         if path and (step + 1) % args.save_every == 0:
-            torch.save({"model": model.state_dict(), "opt": opt.state_dict(), "hook": hook.state_dict(), "step": step + 1}, path)
+            torch.save({"model": model.state_dict(), "opt": opt.state_dict(), "hook": hook.state_dict(), "step": step + 1,
+                        **({"muon": muon.state_dict()} if muon is not None else {})}, path)
     dist.barrier()
     dist.destroy_process_group()
     return 0

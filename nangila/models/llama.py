@@ -5,14 +5,21 @@ model of the fully-sharded benchmark: 24 layers, d_model 2048, 16 heads, SwiGLU 
 The reference's FSDP examples wrap Hugging Face Llama checkpoints (examples/train_fsdp_llm.py); here
 the architecture is defined directly and initialised randomly. Each :class:`DecoderBlock` is the unit
 ``fully_shard`` wraps.
+
+``LlamaConfig(fused=True)`` takes the norms (with the residual's addition inside a block) and the rotary positions through
+``nangila.ops``: one kernel each, forward and backward, where PyTorch's operations make several passes. Results agree with the other
+path up to the last rounding. It also opens the positions' options: the half layout, part of the head, scaling for long contexts.
 """
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import Optional, Union
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from .. import ops
 
 
 @dataclass
@@ -26,6 +33,16 @@ class LlamaConfig:
     max_seq: int = 2048
     rope_theta: float = 10000.0
     eps: float = 1e-5
+    fused: bool = False                      # nangila.ops for norms and positions; what follows needs it
+    rope_layout: str = "interleaved"         # or "half"
+    rope_dim: Optional[int] = None           # turned columns of a head; None: all
+    rope_scaling: Optional[str] = None       # "linear", "ntk" or "yarn" (nangila.ops.rotary_table)
+    rope_factor: float = 1.0
+    rope_original_seq: Optional[int] = None
+
+    def __post_init__(self):
+        if not self.fused and (self.rope_layout, self.rope_dim, self.rope_scaling) != ("interleaved", None, None):
+            raise ValueError("nangila: rope_layout, rope_dim and rope_scaling need fused=True")
 
     @staticmethod
     def llama_1_3b() -> "LlamaConfig":
@@ -61,11 +78,19 @@ def apply_rope(x: torch.Tensor, table: torch.Tensor) -> torch.Tensor:
     return out.view(b, t, h, d).to(x.dtype)
 
 
+class Angles:
+    """The table of the fused path, float32: not a tensor among a block's inputs, which FSDP's mixed precision takes to the parameters' type."""
+
+    def __init__(self, table: torch.Tensor):
+        self.table = table
+
+
 class DecoderBlock(nn.Module):
     def __init__(self, cfg: LlamaConfig):
         super().__init__()
         self.h, self.kv = cfg.n_head, cfg.n_kv_head
         self.hd = cfg.d_model // cfg.n_head
+        self.fused, self.layout = cfg.fused, cfg.rope_layout
         self.norm1 = RMSNorm(cfg.d_model, cfg.eps)
         self.wq = nn.Linear(cfg.d_model, self.h * self.hd, bias=False)
         self.wk = nn.Linear(cfg.d_model, self.kv * self.hd, bias=False)
@@ -76,7 +101,9 @@ class DecoderBlock(nn.Module):
         self.up = nn.Linear(cfg.d_model, cfg.d_mlp, bias=False)
         self.down = nn.Linear(cfg.d_mlp, cfg.d_model, bias=False)
 
-    def forward(self, x: torch.Tensor, rope: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, rope: Union[torch.Tensor, Angles]) -> torch.Tensor:
+        if self.fused:
+            return self._fused(x, rope)
         b, t, _ = x.shape
         y = self.norm1(x)
         q = apply_rope(self.wq(y).view(b, t, self.h, self.hd), rope).transpose(1, 2)
@@ -85,6 +112,17 @@ class DecoderBlock(nn.Module):
         a = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=self.kv != self.h)
         x = x + self.wo(a.transpose(1, 2).reshape(b, t, self.h * self.hd))
         y = self.norm2(x)
+        return x + self.down(F.silu(self.gate(y)) * self.up(y))
+
+    def _fused(self, x: torch.Tensor, rope: Angles) -> torch.Tensor:
+        b, t, _ = x.shape
+        y = ops.rms_norm(x, self.norm1.weight, eps=self.norm1.eps)
+        q, k = ops.rotary(self.wq(y).view(b, t, self.h, self.hd), self.wk(y).view(b, t, self.kv, self.hd), rope.table, layout=self.layout)
+        v = self.wv(y).view(b, t, self.kv, self.hd).transpose(1, 2)
+        a = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v, is_causal=True, enable_gqa=self.kv != self.h)
+        a = self.wo(a.transpose(1, 2).reshape(b, t, self.h * self.hd))
+        # (under autocast the projection has another type than the residual stream)
+        y, x = ops.add_rms_norm(a.to(x.dtype), x, self.norm2.weight, eps=self.norm2.eps)
         return x + self.down(F.silu(self.gate(y)) * self.up(y))
 
 
@@ -104,16 +142,25 @@ class Llama(nn.Module):
     def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None):
         t = idx.size(1)
         if self._rope is None or self._rope.device != idx.device or self._rope.size(0) < t:
-            self._rope = rope_table(max(t, self.cfg.max_seq), self.cfg.d_model // self.cfg.n_head, self.cfg.rope_theta, idx.device)
+            self._rope = self._table(max(t, self.cfg.max_seq), idx.device)
         x = self.embed(idx)
+        rope = Angles(self._rope) if self.cfg.fused else self._rope
         for blk in self.blocks:
-            x = blk(x, self._rope)
-        logits = self.head(self.norm(x))
+            x = blk(x, rope)
+        logits = self.head(ops.rms_norm(x, self.norm.weight, eps=self.norm.eps) if self.cfg.fused else self.norm(x))
         if targets is None:
             return logits
         from ..ops.fused_ce import fused_cross_entropy  # fused kernels for bf16 logits on a GPU, PyTorch's path otherwise
 
         return fused_cross_entropy(logits.view(-1, logits.size(-1)), targets.reshape(-1))
+
+    def _table(self, seq: int, device) -> torch.Tensor:
+        cfg = self.cfg
+        head_dim = cfg.d_model // cfg.n_head
+        if not cfg.fused:
+            return rope_table(seq, head_dim, cfg.rope_theta, device)
+        return ops.rotary_table(seq, cfg.rope_dim or head_dim, cfg.rope_theta, device, scaling=cfg.rope_scaling, factor=cfg.rope_factor,
+                                original_seq=cfg.rope_original_seq)
 
     def num_params(self) -> int:
         return sum(p.numel() for p in self.parameters())
