@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "launch_util.cuh"
 #include "nangila_kernels.h"
@@ -77,22 +78,82 @@ Divisor divisor(uint32_t by) {
 }
 __device__ __forceinline__ uint32_t divide(uint32_t n, const Divisor& d) { return (__umulhi(d.magic, n) + n) >> d.shift; }
 
-// How the work is shared out. Items of a head are runs of eight columns (HALF: first those of the first half of the turned columns, each with its
-// partner, then the rest). A thread keeps its item, and its kAtOnce pairs of (token of a group, head): where they lie is worked out once, and per
-// group of tokens only the group's place is added.
+// A run of V adjacent columns, as it lies in memory: 4 to 32 bytes in one or two loads.
+template <typename T, int V>
+struct Run {
+  static constexpr int kWords = V * int(sizeof(T)) / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kWords == 1) w[0] = *reinterpret_cast<const uint32_t*>(p);
+    if constexpr (kWords == 2) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      w[0] = u.x; w[1] = u.y;
+    }
+    if constexpr (kWords >= 4) {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 u = dev::load_stream(reinterpret_cast<const uint32_t*>(p) + i);
+        w[i] = u.x; w[i + 1] = u.y; w[i + 2] = u.z; w[i + 3] = u.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (kWords == 1) *reinterpret_cast<uint32_t*>(p) = w[0];
+    if constexpr (kWords == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    if constexpr (kWords >= 4) {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4) *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(p) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[V]) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        f[i] = __uint_as_float(w[i]);
+      } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        f[2 * i] = v.x;
+        f[2 * i + 1] = v.y;
+      }
+    }
+  }
+  __device__ __forceinline__ void set(const float (&f)[V]) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        w[i] = __float_as_uint(f[i]);
+      } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&v);
+      } else {
+        const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+    }
+  }
+};
+
+// How the work is shared out. An item is a run of a head's columns, or with HALF two of them: a run of the first half of the turned columns with its
+// partner, or two runs of the columns that are copied. A thread keeps its item, and its kAtOnce pairs of (token of a group, head): where they lie is
+// worked out once, and per group of tokens only the group's place is added.
 struct Plan {
   int items, slots, tokens;  // slots: threads with the same item; tokens of a group
   uint32_t all_tokens, groups;
   Divisor seq;
 };
-template <typename T, bool HALF>
+template <typename T, bool HALF, int V>
 __global__ void __launch_bounds__(kT) rotary_vec_kernel(const __grid_constant__ NangilaRotaryParams p, const __grid_constant__ Plan plan) {
   const int item = threadIdx.x % plan.items, slot = threadIdx.x / plan.items;
   if (slot >= plan.slots) return;
   const int half = p.rot / 2;
-  const int turned = HALF ? half / 8 : p.rot / 8;   // items that are turned
+  const int turned = HALF ? half / V : p.rot / V;   // items that are turned
   const bool turns = item < turned;
-  const int col = HALF && !turns ? p.rot + (item - turned) * 8 : item * 8;
+  const int col = HALF && !turns ? p.rot + (item - turned) * 2 * V : item * V;
+  const int second = turns ? half : V;              // HALF: how far on the other run is
+  const bool two = HALF && col + second < p.d;
   const float sign = p.inverse ? -1.0f : 1.0f;
   const int all = p.heads[0] + p.heads[1], pairs = plan.tokens * all;
   const T* in[kAtOnce];
@@ -109,7 +170,7 @@ __global__ void __launch_bounds__(kT) rotary_vec_kernel(const __grid_constant__ 
     out[j] = static_cast<T*>(p.out[which[j]]) + int64_t(head) * p.d + col;
     if (g >= pairs) ahead[j] = 0x7fffffff;
   }
-  constexpr int kPairs = HALF ? 8 : 4;
+  constexpr int kPairs = HALF ? V : V / 2;
   float cs[2 * kPairs];
   // Positions are read a group ahead: the table's values, which depend on them, would otherwise arrive two trips to memory after the group's data.
   auto row_of = [&](uint32_t token) {
@@ -129,15 +190,15 @@ __global__ void __launch_bounds__(kT) rotary_vec_kernel(const __grid_constant__ 
     const uint32_t first = group * uint32_t(plan.tokens);
     int32_t have = -2;  // the row of the table in `cs`; -1: none
     int32_t row[kAtOnce];
-    dev::Raw8<T> raw[kAtOnce], partner[HALF ? kAtOnce : 1];
+    Run<T, V> run[kAtOnce], other[HALF ? kAtOnce : 1];
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
       const uint32_t token = first + uint32_t(ahead[j]);  // below 2^32
       if (token >= plan.all_tokens) continue;
       const uint32_t b = divide(token, plan.seq), t = token - b * plan.seq.by;
       const T* from = in[j] + int64_t(b) * p.stride_b[which[j]] + int64_t(t) * p.stride_t[which[j]];
-      dev::fetch(from, raw[j]);
-      if (HALF && turns) dev::fetch(from + half, partner[j]);
+      run[j].load(from);
+      if (HALF && two) other[j].load(from + second);
     }
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
@@ -153,33 +214,38 @@ __global__ void __launch_bounds__(kT) rotary_vec_kernel(const __grid_constant__ 
       if (turns) {
         if (row[j] != have) {
           have = row[j];
-          const float4* values = reinterpret_cast<const float4*>(p.table + int64_t(have < 0 ? 0 : have) * p.rot + (HALF ? 2 * col : col));
+          const float* values = p.table + int64_t(have < 0 ? 0 : have) * p.rot + (HALF ? 2 * col : col);
+          if constexpr (kPairs >= 2) {
 #pragma unroll
-          for (int i = 0; i < kPairs / 2; ++i) {
-            const float4 f = __ldg(values + i);
-            cs[4 * i] = f.x; cs[4 * i + 1] = sign * f.y; cs[4 * i + 2] = f.z; cs[4 * i + 3] = sign * f.w;
+            for (int i = 0; i < kPairs; i += 2) {
+              const float4 f = __ldg(reinterpret_cast<const float4*>(values) + i / 2);
+              cs[2 * i] = f.x; cs[2 * i + 1] = sign * f.y; cs[2 * i + 2] = f.z; cs[2 * i + 3] = sign * f.w;
+            }
+          } else {
+            const float2 f = __ldg(reinterpret_cast<const float2*>(values));
+            cs[0] = f.x; cs[1] = sign * f.y;
           }
           if (have < 0) {  // no such position: not a number, and not another position's angles
 #pragma unroll
             for (int i = 0; i < 2 * kPairs; ++i) cs[i] = __uint_as_float(0x7fc00000u);
           }
         }
-        float a[8];
-        dev::unpack(raw[j], a);
+        float a[V];
+        run[j].get(a);
         if constexpr (HALF) {
-          float b[8];
-          dev::unpack(partner[j], b);
+          float b[V];
+          other[j].get(b);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) turn(a[i], b[i], cs[2 * i], cs[2 * i + 1]);
-          dev::pack(b, partner[j]);
-          dev::put(to + half, partner[j]);
+          for (int i = 0; i < V; ++i) turn(a[i], b[i], cs[2 * i], cs[2 * i + 1]);
+          other[j].set(b);
         } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) turn(a[2 * i], a[2 * i + 1], cs[2 * i], cs[2 * i + 1]);
+          for (int i = 0; i < V / 2; ++i) turn(a[2 * i], a[2 * i + 1], cs[2 * i], cs[2 * i + 1]);
         }
-        dev::pack(a, raw[j]);
+        run[j].set(a);
       }
-      dev::put(to, raw[j]);
+      run[j].store(to);
+      if (HALF && two) other[j].store(to + second);
     }
   }
 }
@@ -213,37 +279,60 @@ __global__ void __launch_bounds__(kT) rotary_any_kernel(const __grid_constant__ 
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether runs of V columns fit the head and the tensors' places.
 template <typename T>
-int launch(const NangilaRotaryParams& p, cudaStream_t stream) {
-  const int64_t pairs = p.batch * p.seq * (p.heads[0] + p.heads[1]);
-  bool vec = p.batch * p.seq < (int64_t(1) << 31) && p.table_rows < (int64_t(1) << 31) && p.d % 8 == 0 && p.d / 8 <= kT && p.rot % (p.half ? 16 : 8) == 0 && aligned(p.table);
+bool runs_of(const NangilaRotaryParams& p, int v) {
+  const uintptr_t bytes = std::min<uintptr_t>(16, uintptr_t(v) * sizeof(T));
+  bool ok = p.d % v == 0 && p.rot % (p.half ? 2 * v : v) == 0;
   for (int i = 0; i < 2; ++i)
     if (p.in[i] != nullptr)
-      vec = vec && aligned(p.in[i]) && aligned(p.out[i]) && p.stride_b[i] % 8 == 0 && p.stride_t[i] % 8 == 0 && p.stride_h[i] % 8 == 0;
-  const int64_t limit = 0x7fffffff;
-  if (vec) {
-    const int items = p.half ? p.rot / 16 + (p.d - p.rot) / 8 : p.d / 8;
-    const int all = p.heads[0] + p.heads[1], slots = kT / items;
-    Plan plan;
-    plan.items = items;
-    plan.slots = slots;
-    plan.tokens = std::max(1, slots * kAtOnce / all);
-    plan.all_tokens = uint32_t(p.batch * p.seq);
-    plan.groups = (plan.all_tokens + uint32_t(plan.tokens) - 1) / uint32_t(plan.tokens);
-    plan.seq = divisor(uint32_t(p.seq));
-    auto* kernel = p.half ? rotary_vec_kernel<T, true> : rotary_vec_kernel<T, false>;
-    int resident = 0;
-    if (const cudaError_t e = resident_ctas(reinterpret_cast<const void*>(kernel), kT, 0, &resident)) return int(e);
-    const unsigned heads = unsigned((plan.tokens * all + slots * kAtOnce - 1) / (slots * kAtOnce));  // rounds that the heads of a token take
-    const unsigned ctas = std::min(plan.groups, std::max(1u, unsigned(resident) / heads));
-    if (heads > 65535) return int(cudaErrorInvalidValue);
-    kernel<<<dim3(ctas, heads), kT, 0, stream>>>(p, plan);
-  } else {
-    const int items = p.rot / 2 + (p.d - p.rot);
-    const int64_t total = pairs * items, ctas = (total + kT - 1) / kT;
-    if (ctas > limit) return int(cudaErrorInvalidValue);
-    rotary_any_kernel<T><<<unsigned(ctas), kT, 0, stream>>>(p, items, total);
+      ok = ok && reinterpret_cast<uintptr_t>(p.in[i]) % bytes == 0 && reinterpret_cast<uintptr_t>(p.out[i]) % bytes == 0 && p.stride_b[i] % v == 0 && p.stride_t[i] % v == 0 &&
+           p.stride_h[i] % v == 0;
+  const int items = p.half ? p.rot / 2 / v + ((p.d - p.rot) / v + 1) / 2 : p.d / v;
+  return ok && items <= kT && aligned(p.table) && (p.rot % 4 == 0 || v == 2);
+}
+template <typename T, bool HALF, int V>
+int launch_runs(const NangilaRotaryParams& p, cudaStream_t stream) {
+  const int all = p.heads[0] + p.heads[1];
+  Plan plan;
+  plan.items = HALF ? p.rot / 2 / V + ((p.d - p.rot) / V + 1) / 2 : p.d / V;
+  plan.slots = kT / plan.items;
+  // as many tokens together as leave the fewest threads without a pair
+  const int at_once = plan.slots * kAtOnce;
+  plan.tokens = 1;
+  double best = 0.0;
+  for (int tokens = 1; tokens <= std::max(4, at_once / all); ++tokens) {
+    const double used = double(tokens * all) / double((tokens * all + at_once - 1) / at_once * at_once);
+    if (used > best * 1.02) {
+      best = used;
+      plan.tokens = tokens;
+    }
   }
+  plan.all_tokens = uint32_t(p.batch * p.seq);
+  plan.groups = (plan.all_tokens + uint32_t(plan.tokens) - 1) / uint32_t(plan.tokens);
+  plan.seq = divisor(uint32_t(p.seq));
+  auto* kernel = rotary_vec_kernel<T, HALF, V>;
+  int resident = 0;
+  if (const cudaError_t e = resident_ctas(reinterpret_cast<const void*>(kernel), kT, 0, &resident)) return int(e);
+  const unsigned rounds = unsigned((plan.tokens * all + at_once - 1) / at_once);  // that the heads of a group take
+  if (rounds > 65535) return int(cudaErrorInvalidValue);
+  kernel<<<dim3(std::min(plan.groups, std::max(1u, unsigned(resident) / rounds)), rounds), kT, 0, stream>>>(p, plan);
+  return int(cudaGetLastError());
+}
+template <typename T>
+int launch(const NangilaRotaryParams& p, cudaStream_t stream) {
+  // (numbers of tokens, rows and pairs that 32 bits hold)
+  const int64_t limit = 0x7fffffff;
+  if (p.batch * p.seq <= limit && p.table_rows <= limit && int64_t(p.heads[0]) + p.heads[1] <= 65536) {
+    if (runs_of<T>(p, 8)) return p.half ? launch_runs<T, true, 8>(p, stream) : launch_runs<T, false, 8>(p, stream);
+    if (runs_of<T>(p, 4)) return p.half ? launch_runs<T, true, 4>(p, stream) : launch_runs<T, false, 4>(p, stream);
+    if (runs_of<T>(p, 2)) return p.half ? launch_runs<T, true, 2>(p, stream) : launch_runs<T, false, 2>(p, stream);
+  }
+  const int64_t pairs = p.batch * p.seq * (int64_t(p.heads[0]) + p.heads[1]);
+  const int items = p.rot / 2 + (p.d - p.rot);
+  const int64_t total = pairs * items, ctas = (total + kT - 1) / kT;
+  if (ctas > limit) return int(cudaErrorInvalidValue);
+  rotary_any_kernel<T><<<unsigned(ctas), kT, 0, stream>>>(p, items, total);
   return int(cudaGetLastError());
 }
 
