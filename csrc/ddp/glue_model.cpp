@@ -27,6 +27,7 @@ int dtype_code(const Tensor& t) { return t.scalar_type() == at::kFloat ? NANGILA
 void check_launch(int err, const char* what) { TORCH_CHECK(err == 0, "nangila: ", what, " failed: ", cudaGetErrorString(static_cast<cudaError_t>(err))); }
 void check_tensor(const Tensor& t, const char* name) {
   TORCH_CHECK_TYPE(known(t.scalar_type()), "nangila: ", name, " must be float32, float16 or bfloat16, not ", t.scalar_type());
+  TORCH_CHECK_TYPE(!t.unsafeGetTensorImpl()->is_python_dispatch(), "nangila: ", name, " must be plain tensors (a sharded tensor has to be gathered first)");
   TORCH_CHECK_TYPE(t.layout() == at::kStrided, "nangila: ", name, " must be a dense tensor");
   TORCH_CHECK_TYPE(t.is_cuda() || t.is_cpu(), "nangila: ", name, " must be a CUDA or CPU tensor");
 }
@@ -370,31 +371,22 @@ std::tuple<Tensor, c10::optional<Tensor>> rotary(const Tensor& q, const c10::opt
 }
 
 // ---- orthogonalised updates ----------------------------------------------------------------------------------------
-// Matrices of one shape, type and device, packed. With params: param = param * decay - rate * result and nothing is returned; else the
-// results, bf16, one behind the other. The caller has checked the arguments.
-Tensor orth(const std::vector<Tensor>& grads, const std::vector<Tensor>& momenta, const std::vector<Tensor>& params, const std::vector<double>& coefficients, double eps,
-            double mu, bool nesterov, double decay, double rate) {
-  const int64_t total = int64_t(grads.size());
-  TORCH_CHECK_VALUE(total >= 1 && (momenta.empty() || int64_t(momenta.size()) == total) && (params.empty() || int64_t(params.size()) == total), "nangila: lists of one length");
+struct OrthArgs {
+  std::vector<double> coefficients;  // three for each step
+  double eps, mu, decay, rate;
+  bool nesterov;
+};
+void check_schedule(const std::vector<double>& coefficients) {
   TORCH_CHECK_VALUE(!coefficients.empty() && coefficients.size() % 3 == 0 && coefficients.size() / 3 <= NANGILA_ORTH_MAX_STEPS, "nangila: three coefficients for each of 1 to ",
                     NANGILA_ORTH_MAX_STEPS, " steps");
+}
+// Packed CUDA matrices of one shape, type and device, which the callers below have checked. With params: param = param * decay - rate * result
+// and nothing is returned; else the results, bf16, one behind the other.
+Tensor orth_group(const std::vector<Tensor>& grads, const std::vector<Tensor>& momenta, const std::vector<Tensor>& params, const OrthArgs& args) {
+  const int64_t total = int64_t(grads.size());
   const Tensor& first = grads[0];
-  TORCH_CHECK_VALUE(first.dim() == 2, "nangila: matrices");
   const int64_t rows = first.size(0), cols = first.size(1);
-  TORCH_CHECK_VALUE(rows >= 1 && cols >= 1 && rows <= 65536 && cols <= 65536, "nangila: matrices of 1 x 1 to 65536 x 65536, got ", first.sizes());
-  auto check = [&](const Tensor& t, const Tensor& like, const char* name) {
-    TORCH_CHECK_VALUE(t.is_cuda() && t.device() == first.device() && t.dim() == 2 && t.size(0) == rows && t.size(1) == cols && t.is_contiguous() && known(t.scalar_type()) &&
-                          t.scalar_type() == like.scalar_type(),
-                      "nangila: ", name, " must be packed CUDA matrices of one shape, type and device");
-  };
-  for (int64_t i = 0; i < total; ++i) {
-    check(grads[i], first, "gradients");
-    if (!params.empty()) check(params[i], params[0], "parameters");
-    if (!momenta.empty()) {
-      check(momenta[i], momenta[0], "momenta");
-      TORCH_CHECK_VALUE(momenta[i].scalar_type() == at::kFloat, "nangila: momenta must be float32");
-    }
-  }
+  const std::vector<double>& coefficients = args.coefficients;
   c10::cuda::CUDAGuard guard(first.device());
   Tensor out;
   if (params.empty()) out = at::empty({total, rows, cols}, first.options().dtype(at::kBFloat16));
@@ -419,11 +411,11 @@ Tensor orth(const std::vector<Tensor>& grads, const std::vector<Tensor>& momenta
     p.param_dtype = params.empty() ? 0 : dtype_code(params[0]);
     p.steps = int32_t(coefficients.size() / 3);
     for (size_t i = 0; i < coefficients.size(); ++i) p.coefficients[i / 3][i % 3] = float(coefficients[i]);
-    p.nesterov = nesterov ? 1 : 0;
-    p.eps = float(eps);
-    p.mu = float(mu);
-    p.decay = float(decay);
-    p.rate = float(rate);
+    p.nesterov = args.nesterov ? 1 : 0;
+    p.eps = float(args.eps);
+    p.mu = float(args.mu);
+    p.decay = float(args.decay);
+    p.rate = float(args.rate);
     p.workspace = workspace.data_ptr();
     check_launch(nangila_orth(&p, at::cuda::getCurrentCUDAStream()), "orthogonalize");
   }
@@ -462,26 +454,45 @@ void check_matrix(const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) >= 1 && t.size(1) >= 1 && t.size(0) <= 65536 && t.size(1) <= 65536, "nangila: ", name,
                     " must be matrices of 1 x 1 to 65536 x 65536, got shape ", t.sizes());
 }
-// Indices of tensors of one shape, type and device, in the order of their first.
-std::vector<std::vector<int64_t>> group_matrices(const std::vector<Tensor>& ts) {
+template <typename Same>
+std::vector<std::vector<int64_t>> grouped(size_t n, const Same& same) {
   std::vector<std::vector<int64_t>> groups;
-  for (size_t i = 0; i < ts.size(); ++i) {
-    check_matrix(ts[i], "updates");
-    auto same = [&](const std::vector<int64_t>& g) {
-      const Tensor& o = ts[g[0]];
-      return o.sizes() == ts[i].sizes() && o.scalar_type() == ts[i].scalar_type() && o.device() == ts[i].device();
-    };
-    auto it = std::find_if(groups.begin(), groups.end(), same);
+  for (size_t i = 0; i < n; ++i) {
+    auto it = std::find_if(groups.begin(), groups.end(), [&](const std::vector<int64_t>& g) { return same(size_t(g[0]), i); });
     if (it == groups.end()) groups.push_back({int64_t(i)});
     else it->push_back(int64_t(i));
   }
   return groups;
 }
-// The same for a Muon step, with its checks of what belongs together.
-std::vector<std::vector<int64_t>> group_muon(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& momenta) {
+std::vector<Tensor> chosen(const std::vector<Tensor>& ts, const std::vector<int64_t>& which, bool packed = false) {
+  std::vector<Tensor> out;
+  out.reserve(which.size());
+  for (const int64_t i : which) out.push_back(packed ? ts[i].contiguous() : ts[i]);
+  return out;
+}
+// Results for the CUDA matrices among the updates; nothing (None) in the place of the others.
+std::vector<c10::optional<Tensor>> orthogonalize(const std::vector<Tensor>& updates, const std::vector<double>& coefficients, double eps) {
+  at::NoGradGuard no_grad;
+  check_schedule(coefficients);
+  for (const Tensor& t : updates) check_matrix(t, "updates");
+  std::vector<c10::optional<Tensor>> out(updates.size());
+  for (const auto& g : grouped(updates.size(), [&](size_t i, size_t j) {
+         return updates[i].sizes() == updates[j].sizes() && updates[i].scalar_type() == updates[j].scalar_type() && updates[i].device() == updates[j].device();
+       })) {
+    if (!updates[g[0]].is_cuda()) continue;
+    const Tensor stack = orth_group(chosen(updates, g, true), {}, {}, OrthArgs{coefficients, eps, 0.0, 1.0, 0.0, false});
+    for (size_t k = 0; k < g.size(); ++k) out[g[k]] = stack.select(0, int64_t(k));
+  }
+  return out;
+}
+// The step of the CUDA parameters among them; returns the indices of the others. scale: 0 sqrt(max(1, rows / cols)), 1 0.2 sqrt(max(rows, cols)), 2 one.
+// Everything is checked before anything changes.
+std::vector<int64_t> muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& momenta, const std::vector<double>& coefficients, double eps,
+                               double mu, bool nesterov, double lr, double weight_decay, int64_t scale) {
+  at::NoGradGuard no_grad;
+  check_schedule(coefficients);
   TORCH_CHECK_VALUE(params.size() == grads.size() && params.size() == momenta.size(), "nangila: ", params.size(), " parameters, ", grads.size(), " gradients and ",
                     momenta.size(), " momenta");
-  std::vector<std::vector<int64_t>> groups;
   for (size_t i = 0; i < params.size(); ++i) {
     const Tensor &p = params[i], &g = grads[i], &m = momenta[i];
     check_matrix(p, "parameters");
@@ -491,18 +502,29 @@ std::vector<std::vector<int64_t>> group_muon(const std::vector<Tensor>& params, 
                       p.device(), ", its gradient ", g.sizes(), " on ", g.device(), ", its momentum ", m.sizes(), " on ", m.device());
     TORCH_CHECK_TYPE(m.scalar_type() == at::kFloat, "nangila: momenta must be float32, got ", m.scalar_type());
     TORCH_CHECK_VALUE(p.is_contiguous() && m.is_contiguous(), "nangila: parameter ", i, " and its momentum must be packed (contiguous)");
-    auto same = [&](const std::vector<int64_t>& other) {
-      const Tensor &op = params[other[0]], &og = grads[other[0]];
-      return op.sizes() == p.sizes() && op.scalar_type() == p.scalar_type() && og.scalar_type() == g.scalar_type() && op.device() == p.device();
-    };
-    auto it = std::find_if(groups.begin(), groups.end(), same);
-    if (it == groups.end()) groups.push_back({int64_t(i)});
-    else it->push_back(int64_t(i));
   }
   std::vector<Tensor> written = params;
   written.insert(written.end(), momenta.begin(), momenta.end());
   TORCH_CHECK_VALUE(!overlapping(written, grads), "nangila: parameters and momenta must not share memory with one another or with the gradients");
-  return groups;
+  std::vector<int64_t> others;
+  for (const auto& g : grouped(params.size(), [&](size_t i, size_t j) {
+         return params[i].sizes() == params[j].sizes() && params[i].scalar_type() == params[j].scalar_type() && grads[i].scalar_type() == grads[j].scalar_type() &&
+                params[i].device() == params[j].device();
+       })) {
+    const Tensor& first = params[g[0]];
+    if (!first.is_cuda()) {
+      others.insert(others.end(), g.begin(), g.end());
+      continue;
+    }
+    const double rows = double(first.size(0)), cols = double(first.size(1));
+    const double size = scale == 0 ? std::sqrt(std::max(1.0, rows / cols)) : scale == 1 ? 0.2 * std::sqrt(std::max(rows, cols)) : 1.0;
+    orth_group(chosen(grads, g, true), chosen(momenta, g), chosen(params, g), OrthArgs{coefficients, eps, mu, 1.0 - lr * weight_decay, lr * size, nesterov});
+    // the kernels write where autograd does not look: what was saved for a backward pass is not what it was
+    for (const int64_t i : g)
+      for (const Tensor* t : {&params[i], &momenta[i]})
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  }
+  return others;
 }
 
 }  // namespace
@@ -512,8 +534,7 @@ void register_model(py::module_& m) {
   m.def("add_rms_norm", &add_rms_norm, py::arg("x"), py::arg("residual"), py::arg("weight"), py::arg("eps"));
   m.def("rms_norm_fp8", &rms_norm_fp8, py::arg("x"), py::arg("weight"), py::arg("eps"), py::arg("residual") = py::none(), py::arg("group") = 0);
   m.def("rotary", &rotary, py::arg("q"), py::arg("k"), py::arg("table"), py::arg("positions"), py::arg("half"));
-  m.def("orth", &orth, py::arg("grads"), py::arg("momenta"), py::arg("params"), py::arg("coefficients"), py::arg("eps"), py::arg("mu") = 0.0, py::arg("nesterov") = false,
-        py::arg("decay") = 1.0, py::arg("rate") = 0.0);
-  m.def("group_matrices", &group_matrices, py::arg("matrices"));
-  m.def("group_muon", &group_muon, py::arg("params"), py::arg("grads"), py::arg("momenta"));
+  m.def("orthogonalize", &orthogonalize, py::arg("updates"), py::arg("coefficients"), py::arg("eps"));
+  m.def("muon_step", &muon_step, py::arg("params"), py::arg("grads"), py::arg("momenta"), py::arg("coefficients"), py::arg("eps"), py::arg("mu"), py::arg("nesterov"), py::arg("lr"),
+        py::arg("weight_decay"), py::arg("scale"));
 }

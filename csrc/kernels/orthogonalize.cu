@@ -33,6 +33,7 @@
 #include "nangila_model_kernels.h"
 #include "ptx_sm100.cuh"
 #include "quant.cuh"
+#include "raw8.cuh"
 
 namespace nangila {
 namespace {
@@ -640,7 +641,7 @@ struct Prep {
   __half* hi;
   __half* lo;
   int64_t numel, ld, matrix;
-  int cols, chunks, nesterov, vector;
+  int cols, chunks, nesterov, vector, flat; // vector: runs of eight that X has too; flat: of the gradient alone
   float mu, eps, scale;
 };
 __device__ __forceinline__ double block_sum(double v, double* s) {
@@ -661,21 +662,37 @@ __global__ void __launch_bounds__(kPrepT) orth_norm_kernel(const __grid_constant
   const int64_t stride = int64_t(gridDim.x) * kPrepT, first = int64_t(blockIdx.x) * kPrepT + threadIdx.x;
   double sum = 0.0;
   may_follow();
-  const int64_t runs = p.vector ? p.numel / 8 : 0;
-  for (int64_t i = first; i < runs; i += stride) {
-    float u[8];
-    dev::Vec8<T>::load(g + i * 8, u);
-    if (m != nullptr) {
-      float v[8];
-      dev::Vec8<float>::load(m + i * 8, v);
+  const int64_t runs = p.flat ? p.numel / 8 : 0;
+  constexpr int kAhead = 4;  // runs of eight on their way
+  for (int64_t i0 = first; i0 < runs; i0 += kAhead * stride) {
+    dev::Raw8<T> raw[kAhead];
+    dev::Raw8<float> old[kAhead];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        v[k] = __fmaf_rn(p.mu, v[k], u[k]);
-        u[k] = p.nesterov ? __fmaf_rn(p.mu, v[k], u[k]) : v[k];
-      }
-      dev::Vec8<float>::store(m + i * 8, v);
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t i = i0 + k * stride;
+      if (i >= runs) break;
+      dev::fetch(g + i * 8, raw[k]);
+      if (m != nullptr) dev::fetch(m + i * 8, old[k]);
     }
-    sum += square_sum(u);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t i = i0 + k * stride;
+      if (i >= runs) break;
+      float u[8];
+      dev::unpack(raw[k], u);
+      if (m != nullptr) {
+        float v[8];
+        dev::unpack(old[k], v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[j] = __fmaf_rn(p.mu, v[j], u[j]);
+          u[j] = p.nesterov ? __fmaf_rn(p.mu, v[j], u[j]) : v[j];
+        }
+        dev::pack(v, old[k]);
+        dev::put(m + i * 8, old[k]);
+      }
+      sum += square_sum(u);
+    }
   }
   for (int64_t i = runs * 8 + first; i < p.numel; i += stride) {
     float u = dev::Vec16<T>::to_float(g[i]);
@@ -721,15 +738,30 @@ __global__ void __launch_bounds__(kPrepT) orth_start_kernel(const __grid_constan
       *reinterpret_cast<uint4*>(hi + i * 8) = h;
       *reinterpret_cast<uint4*>(lo + i * 8) = l;
     }
-  } else {
-    for (int64_t i = first; i < p.numel; i += stride) {
-      float u = dev::Vec16<T>::to_float(g[i]);
-      if (m != nullptr) u = p.nesterov ? __fmaf_rn(p.mu, m[i], u) : m[i];
-      u *= f;
-      const int64_t row = i / p.cols, at = row * p.ld + (i - row * p.cols);
-      const __half h = __float2half_rn(u);
-      hi[at] = h;
-      lo[at] = __float2half_rn((u - __half2float(h)) * kLoScale);
+  } else {  // a warp takes a row, 128 columns at a time
+    const int lane = threadIdx.x & 31;
+    const int64_t rows = p.numel / p.cols;
+    for (int64_t row = (int64_t(blockIdx.x) * kPrepT + threadIdx.x) >> 5; row < rows; row += stride >> 5) {
+      for (int c0 = lane; c0 < p.cols; c0 += 128) {
+        float u[4], v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (c0 + 32 * k >= p.cols) break;
+          const int64_t i = row * p.cols + c0 + 32 * k;
+          u[k] = dev::Vec16<T>::to_float(g[i]);
+          if (m != nullptr) v[k] = m[i];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (c0 + 32 * k >= p.cols) break;
+          if (m != nullptr) u[k] = p.nesterov ? __fmaf_rn(p.mu, v[k], u[k]) : v[k];
+          u[k] *= f;
+          const int64_t at = row * p.ld + c0 + 32 * k;
+          const __half h = __float2half_rn(u[k]);
+          hi[at] = h;
+          lo[at] = __float2half_rn((u[k] - __half2float(h)) * kLoScale);
+        }
+      }
     }
   }
 }
@@ -1350,12 +1382,13 @@ extern "C" int nangila_orth(const NangilaOrthParams* p, cudaStream_t stream) {
 
   Prep prep;
   std::memset(&prep, 0, sizeof prep);
-  prep.vector = p->cols % 8 == 0;
+  prep.flat = 1;
   for (int i = 0; i < p->count; ++i) {
     prep.grad[i] = p->grad[i];
     prep.momentum[i] = p->momentum[0] != nullptr ? p->momentum[i] : nullptr;
-    if (!aligned(p->grad[i]) || !aligned(prep.momentum[i])) prep.vector = 0;
+    if (!aligned(p->grad[i]) || !aligned(prep.momentum[i])) prep.flat = 0;
   }
+  prep.vector = prep.flat != 0 && p->cols % 8 == 0;
   prep.partial = reinterpret_cast<double*>(ws + l.partial);
   prep.hi = hi[0];
   prep.lo = lo;

@@ -35,12 +35,6 @@ def _schedule(steps: int, coefficients: _Coefficients) -> List[float]:
     return flat
 
 
-def _plain_tensors(ts: Sequence[torch.Tensor], name: str) -> None:
-    for t in ts:
-        if not isinstance(t, torch.Tensor) or type(t).__name__ == "DTensor":
-            raise TypeError(f"nangila: {name} must be plain tensors (a sharded matrix has to be gathered first), got {type(t).__name__}")
-
-
 def _check_eps(eps: float) -> None:
     if not (math.isfinite(eps) and eps > 0):
         raise ValueError(f"nangila: eps must be positive, got {eps}")
@@ -67,29 +61,23 @@ def orthogonalize(update: Union[torch.Tensor, Sequence[torch.Tensor]], steps: in
     below about two. No gradient flows through it."""
     flat = _schedule(steps, coefficients)
     _check_eps(eps)
-    if isinstance(update, torch.Tensor):
-        _plain_tensors([update], "updates")
-        stack = update.dim() == 3
-        many = list(update.unbind(0)) if stack else [update]
-        glue().group_matrices(many or [update.new_empty(update.shape[1:])])
-        if not many:
-            return update.new_empty(update.shape, dtype=torch.bfloat16)
-        if update.is_cuda:
-            out = glue().orth([t.contiguous() for t in many], [], [], flat, eps)
-        else:
-            out = torch.stack([_plain(t, flat, eps).to(torch.bfloat16) for t in many])
-        return out if stack else out[0]
-    many = list(update)
-    _plain_tensors(many, "updates")
-    results: List[torch.Tensor] = [None] * len(many)  # type: ignore[list-item]
-    for members in glue().group_matrices(many):
-        if many[members[0]].is_cuda:
-            parts = glue().orth([many[i].contiguous() for i in members], [], [], flat, eps).unbind(0)
-        else:
-            parts = [_plain(many[i], flat, eps).to(torch.bfloat16) for i in members]
-        for i, t in zip(members, parts):
-            results[i] = t
-    return results
+    if isinstance(update, torch.Tensor) and update.dim() != 3:
+        many = [update]
+    elif isinstance(update, torch.Tensor) and update.size(0) == 0:
+        glue().orthogonalize([update.new_empty(update.shape[1:], device="cpu")], flat, eps)  # its checks
+        return update.new_empty(update.shape, dtype=torch.bfloat16)
+    else:
+        many = list(update)
+    if not all(isinstance(t, torch.Tensor) for t in many):
+        raise TypeError("nangila: updates must be tensors")
+    results = glue().orthogonalize(many, flat, eps)
+    results = [_plain(t, flat, eps).to(torch.bfloat16) if r is None else r for t, r in zip(many, results)]
+    if not isinstance(update, torch.Tensor):
+        return results
+    if update.dim() != 3:
+        return results[0]
+    # (the results of a stack on a GPU lie one behind the other)
+    return torch.stack(results) if not update.is_cuda else results[0].as_strided(update.shape, (update.size(1) * update.size(2), update.size(2), 1))
 
 
 def update_scale(rows: int, cols: int, scale: Union[str, None]) -> float:
@@ -122,20 +110,10 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
     for name, v in (("lr", lr), ("momentum", momentum), ("weight_decay", weight_decay)):
         if not (math.isfinite(v) and v >= 0):
             raise ValueError(f"nangila: {name} must be finite and not negative, got {v}")
-    params, grads, momenta = list(params), list(grads), list(momenta)
-    for name, ts in (("parameters", params), ("gradients", grads), ("momenta", momenta)):
-        _plain_tensors(ts, name)
     update_scale(1, 1, scale)
-    for members in glue().group_muon(params, grads, momenta):
-        first = params[members[0]]
-        rate, decay = lr * update_scale(first.size(0), first.size(1), scale), 1.0 - lr * weight_decay
-        ps, gs, ms = [params[i] for i in members], [grads[i] for i in members], [momenta[i] for i in members]
-        if first.is_cuda:
-            glue().orth([g.contiguous() for g in gs], ms, ps, flat, eps, momentum, nesterov, decay, rate)
-            # the kernels write where autograd does not look: what was saved for a backward pass is not what it was
-            torch.autograd.graph.increment_version([t for t in ps + ms if not t.is_inference()])
-            continue
-        for p, g, m in zip(ps, gs, ms):
-            m.mul_(momentum).add_(g)
-            u = m * momentum + g if nesterov else m
-            p.copy_(p.float() * decay - rate * _plain(u, flat, eps))
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    for i in glue().muon_step(params, grads, momenta, flat, eps, momentum, nesterov, lr, weight_decay, SCALES.index(scale)):
+        p, g, m = params[i], grads[i], momenta[i]
+        m.mul_(momentum).add_(g)
+        u = m * momentum + g if nesterov else m
+        p.copy_(p.float() * (1.0 - lr * weight_decay) - lr * update_scale(p.size(0), p.size(1), scale) * _plain(u, flat, eps))
