@@ -773,6 +773,7 @@ __global__ void __launch_bounds__(kPrepT) orth_start_kernel(const __grid_constan
 // 128 x 128, so what bounds this is the way from one to the next: two thirds of a step are waits for a product and the pass over its results.
 //   D = X^T X (n long, from X by rows of n: MN-major),  A = D;   D = A A,  B = b A + c D;   X <- a X + X B, accumulated onto a X in tensor memory.
 constexpr int kSmallT = 256;
+constexpr int kRuns = 8;                         // of elements that a thread has on their way, to and from memory
 constexpr int kBlocks = 3;                       // of 128 rows in a CTA
 constexpr int kBlockBytes = 32768;               // 128 x 128 in fp16, two swizzled halves of 64 columns
 constexpr int kHalfBytes = 16384;
@@ -781,7 +782,7 @@ struct Small {
   const void* grad[NANGILA_ORTH_MAX_COUNT];
   float* momentum[NANGILA_ORTH_MAX_COUNT];
   float coefficients[NANGILA_ORTH_MAX_STEPS][3];
-  int steps, m, n, tall, nesterov, blocks, per; // blocks of 128 along n, of a CTA
+  int steps, m, n, nesterov, blocks, per; // blocks of 128 along n, of a CTA
   int vector, vector_out; // runs of four elements can be read, and written
   float mu, eps, scale;
 };
@@ -797,7 +798,7 @@ __device__ __forceinline__ void products_128(uint32_t d, uint32_t a, uint32_t b,
     umma_f16(d, ad, bd, idesc, kk > 0 ? 1u : first_accumulates);
   }
 }
-template <typename T>
+template <typename T, bool TALL>
 __global__ void __launch_bounds__(kSmallT, 1) orth_small_kernel(const __grid_constant__ Small p, const __grid_constant__ Target target) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* hi = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -843,92 +844,147 @@ __global__ void __launch_bounds__(kSmallT, 1) orth_small_kernel(const __grid_con
     __syncthreads();
     tc_fence_after_sync();
   };
-  // A block's elements are passed over in runs of four, neighbours in memory (V = 4), or one by one. Run e of a block: its first row (along n), its first
-  // column, and whether it exists. (The quotient is below 128 and at least 1 / 256 away from a whole number: fp32 finds it.)
-  const float inverse_m = 1.0f / float(p.m);
-  auto place = [&](auto run, int e, int base, int& r, int& i) {
-    constexpr int V = decltype(run)::value;
-    if (p.tall) {
-      r = int((float(e * V) + 0.5f) * inverse_m);
-      i = e * V - r * p.m;
-    } else {
-      i = e / (128 / V);
-      r = e % (128 / V) * V;
-    }
-    return e < 128 / V * p.m && base + r < p.n;
+  // A block's elements are passed over in runs of V = 4, neighbours in memory, or one by one; the threads take turns with the runs, kRuns of a thread
+  // being a round. With the longer side outermost (TALL) a block is one stretch of memory; else a thread keeps its rows and goes down the columns.
+  // All of this is a chain of waits in a kernel that runs once, so there are no divisions in it and no branches around a run.
+  struct Walk {
+    int r, i;  // row (along n) and column of a thread's run in a block
   };
-  auto address = [&](int base, int r, int i) { return p.tall ? int64_t(base + r) * p.m + i : int64_t(i) * p.n + base + r; };
+  auto first_of = [&](auto run) {
+    constexpr int V = decltype(run)::value;
+    const int e = int(threadIdx.x) * V;
+    if (TALL) return Walk{e / p.m, e % p.m};
+    return Walk{e & 127, e >> 7};
+  };
+  auto advance = [&](auto run, Walk& w, int dr, int di) {  // dr, di: kSmallT runs further on
+    constexpr int V = decltype(run)::value;
+    if (TALL) {
+      w.i += di;
+      w.r += dr + (w.i >= p.m ? 1 : 0);
+      w.i -= w.i >= p.m ? p.m : 0;
+    } else {
+      w.i += kSmallT * V / 128;
+    }
+  };
+  auto runs_of = [&](auto run, int b, const Walk& first) {  // that a thread has in block b
+    constexpr int V = decltype(run)::value;
+    const int rows = min(128, p.n - (block0 + b) * 128);
+    if (TALL) return max(0, (rows * p.m / V - int(threadIdx.x) + kSmallT - 1) / kSmallT);
+    return first.r < rows ? max(0, (p.m - first.i + 2 * V - 1) / (2 * V)) : 0;
+  };
+  auto start_of = [&](auto run, int b, const Walk& first) {  // where the first of them lies
+    constexpr int V = decltype(run)::value;
+    const int base = (block0 + b) * 128;
+    return TALL ? int64_t(base) * p.m + int64_t(threadIdx.x) * V : int64_t(first.i) * p.n + base + first.r;
+  };
+  auto step_of = [&](auto run) {
+    constexpr int V = decltype(run)::value;
+    return TALL ? int64_t(kSmallT * V) : int64_t(2 * V) * p.n;
+  };
 
-  // ---- the gradient, with its momentum: into tensor memory as it is, and its norm ----
+  // ---- the gradient, with its momentum: into tensor memory as it is, and its norm. A round is on its way while the one before it is worked on. ----
   const T* g = static_cast<const T*>(p.grad[batch]);
   float* mom = p.momentum[batch];
   double sum = 0.0;
-  for (int b = 0; b < mine; ++b) {
-    const int base = (block0 + b) * 128;
-    if (p.m < 128 || base + 128 > p.n) {  // what lies outside of the matrix
-      for (int c = threadIdx.x; c < 128 * 32; c += kSmallT) *stage_at(stage, c >> 5, c & 31) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      __syncthreads();
-    }
-    auto take = [&](auto run) {
-      constexpr int V = decltype(run)::value, kAhead = 8;
-      for (int e0 = threadIdx.x; e0 < 128 / V * p.m; e0 += kAhead * kSmallT) {
-        float u[kAhead][V], v[kAhead][V];
+  auto take = [&](auto run) {
+    constexpr int V = decltype(run)::value;
+    const int last = (128 * p.m / V + kSmallT - 1) / kSmallT;  // runs of a thread in a whole block
+    const int64_t step = step_of(run);
+    const Walk first = first_of(run);
+    const int dr = TALL ? kSmallT * V / p.m : 0, di = TALL ? kSmallT * V - dr * p.m : 0;
+    float u[kRuns][V], v[kRuns][V], next_u[kRuns][V], next_v[kRuns][V];
+    auto fetch = [&](int b, int k0) {
+      const int runs = runs_of(run, b, first);
+      const int64_t at = start_of(run, b, first) + k0 * step;
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-          int r, i;
-          if (!place(run, e0 + k * kSmallT, base, r, i)) continue;
-          const int64_t at = address(base, r, i);
-          if constexpr (V == 4) {
-            load4<T>(g + at, u[k]);
-            if (mom != nullptr) load4<float>(mom + at, v[k]);
-          } else {
-            u[k][0] = dev::Vec16<T>::to_float(g[at]);
-            if (mom != nullptr) v[k][0] = mom[at];
-          }
+      for (int k = 0; k < kRuns; ++k) {
+        if (k0 + k < runs) {
+          if constexpr (V == 4) load4<T>(g + at + k * step, next_u[k]);
+          else next_u[k][0] = dev::Vec16<T>::to_float(g[at + k * step]);
         }
+      }
+      if (mom == nullptr) return;
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-          int r, i;
-          if (!place(run, e0 + k * kSmallT, base, r, i)) continue;
-          if (mom != nullptr) {
-#pragma unroll
-            for (int x = 0; x < V; ++x) {
-              v[k][x] = __fmaf_rn(p.mu, v[k][x], u[k][x]);
-              u[k][x] = p.nesterov ? __fmaf_rn(p.mu, v[k][x], u[k][x]) : v[k][x];
-            }
-            const int64_t at = address(base, r, i);
-            if constexpr (V == 4) store4(mom + at, v[k]);
-            else mom[at] = v[k][0];
-          }
-          if constexpr (V == 4) {
-            if (p.tall) {
-              *stage_at(stage, r, i >> 2) = make_float4(u[k][0], u[k][1], u[k][2], u[k][3]);
-            } else {
-#pragma unroll
-              for (int x = 0; x < 4; ++x) *stage_one(stage, r + x, i) = u[k][x];
-            }
-          } else {
-            *stage_one(stage, r, i) = u[k][0];
-          }
-          sum += square_sum(u[k]);
+      for (int k = 0; k < kRuns; ++k) {
+        if (k0 + k < runs) {
+          if constexpr (V == 4) load4<float>(mom + at + k * step, next_v[k]);
+          else next_v[k][0] = mom[at + k * step];
         }
       }
     };
-    if (p.vector) take(std::integral_constant<int, 4>{});
-    else take(std::integral_constant<int, 1>{});
-    __syncthreads();
-#pragma unroll 1
-    for (int c = 0; c < 64; c += 16) {
-      float v[16];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4 f = *stage_at(stage, row, (half * 64 + c) / 4 + q);
-        v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
+    if (mine > 0) fetch(0, 0);
+    for (int b = 0; b < mine; ++b) {
+      const int runs = runs_of(run, b, first);
+      const int64_t start = start_of(run, b, first);
+      Walk w = first;
+      if (p.m < 128 || (block0 + b + 1) * 128 > p.n) {  // what lies outside of the matrix
+        for (int c = threadIdx.x; c < 128 * 32; c += kSmallT) *stage_at(stage, c >> 5, c & 31) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        __syncthreads();
       }
-      tmem_st_32x32b_x16(tmem + lanes + uint32_t(128 * (1 + b) + half * 64 + c), v);
+      for (int k0 = 0; k0 < last; k0 += kRuns) {
+#pragma unroll
+        for (int k = 0; k < kRuns; ++k)
+#pragma unroll
+          for (int x = 0; x < V; ++x) {
+            u[k][x] = k0 + k < runs ? next_u[k][x] : 0.0f;
+            v[k][x] = next_v[k][x];
+          }
+        if (k0 + kRuns < last) fetch(b, k0 + kRuns);
+        else if (b + 1 < mine) fetch(b + 1, 0);
+        if (mom != nullptr) {
+#pragma unroll
+          for (int k = 0; k < kRuns; ++k) {
+#pragma unroll
+            for (int x = 0; x < V; ++x) {
+              v[k][x] = __fmaf_rn(p.mu, v[k][x], u[k][x]);
+              u[k][x] = k0 + k >= runs ? 0.0f : p.nesterov ? __fmaf_rn(p.mu, v[k][x], u[k][x]) : v[k][x];
+            }
+            if (k0 + k < runs) {
+              if constexpr (V == 4) store4(mom + start + (k0 + k) * step, v[k]);
+              else mom[start + (k0 + k) * step] = v[k][0];
+            }
+          }
+        }
+        float squares = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kRuns; ++k) {
+          if (k0 + k < runs) {
+            if constexpr (V == 4 && TALL) {
+              *stage_at(stage, w.r, w.i >> 2) = make_float4(u[k][0], u[k][1], u[k][2], u[k][3]);
+            } else {
+#pragma unroll
+              for (int x = 0; x < V; ++x) *stage_one(stage, w.r + x, w.i) = u[k][x];
+            }
+          }
+          advance(run, w, dr, di);
+#pragma unroll
+          for (int x = 0; x < V; ++x) squares = __fmaf_rn(u[k][x], u[k][x], squares);
+        }
+        if (squares > 1e-28f && squares < 1e38f) {
+          sum += double(squares);
+        } else {  // where fp32's range does not hold them
+#pragma unroll
+          for (int k = 0; k < kRuns; ++k)
+#pragma unroll
+            for (int x = 0; x < V; ++x) sum = fma(double(u[k][x]), double(u[k][x]), sum);
+        }
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int c = 0; c < 64; c += 16) {
+        float f16[16];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float4 f = *stage_at(stage, row, (half * 64 + c) / 4 + x);
+          f16[4 * x] = f.x; f16[4 * x + 1] = f.y; f16[4 * x + 2] = f.z; f16[4 * x + 3] = f.w;
+        }
+        tmem_st_32x32b_x16(tmem + lanes + uint32_t(128 * (1 + b) + half * 64 + c), f16);
+      }
+      __syncthreads();
     }
-    __syncthreads();
-  }
+  };
+  if (p.vector) take(std::integral_constant<int, 4>{});
+  else take(std::integral_constant<int, 1>{});
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) warp_sums[warp] = sum;
@@ -1056,69 +1112,88 @@ __global__ void __launch_bounds__(kSmallT, 1) orth_small_kernel(const __grid_con
     if (step + 1 < p.steps) round_x(1.0f, p.coefficients[step + 1][0]);
   }
 
-  // ---- out ----
-  const bool bad = *failed != 0;
-  for (int b = 0; b < mine; ++b) {
-    const int base = (block0 + b) * 128;
-    __syncthreads();
-#pragma unroll 1
-    for (int c = 0; c < 64; c += 16) {
-      float v[16];
-      tmem_ld_32x32b_x16(tmem + lanes + uint32_t(128 * (1 + b) + half * 64 + c), v);
+  // ---- out, the parameters read a round ahead ----
+  const float unscale = *failed != 0 ? __uint_as_float(0x7fc00000u) : target.unscale;
+  auto write = [&](auto* to, auto fresh, auto run) {
+    using P = std::remove_pointer_t<decltype(to)>;
+    constexpr int V = decltype(run)::value;
+    constexpr bool kFresh = decltype(fresh)::value;
+    const int last = (128 * p.m / V + kSmallT - 1) / kSmallT;
+    const int64_t step = step_of(run);
+    const Walk first = first_of(run);
+    const int dr = TALL ? kSmallT * V / p.m : 0, di = TALL ? kSmallT * V - dr * p.m : 0;
+    float v[kRuns][V], next[kRuns][V];
+    auto fetch = [&](int b, int k0) {
+      const int runs = runs_of(run, b, first);
+      const int64_t at = start_of(run, b, first) + k0 * step;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) v[k] = bad ? __uint_as_float(0x7fc00000u) : v[k] * target.unscale;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) *stage_at(stage, row, (half * 64 + c) / 4 + q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-    }
-    __syncthreads();
-    auto write_runs = [&](auto* to, bool fresh, auto run) {
-      using P = std::remove_pointer_t<decltype(to)>;
-      constexpr int V = decltype(run)::value, kAhead = 8;
-      for (int e0 = threadIdx.x; e0 < 128 / V * p.m; e0 += kAhead * kSmallT) {
-        float v[kAhead][V];
-        if (!fresh) {
-#pragma unroll
-          for (int k = 0; k < kAhead; ++k) {
-            int r, i;
-            if (!place(run, e0 + k * kSmallT, base, r, i)) continue;
-            if constexpr (V == 4) load4<P>(to + address(base, r, i), v[k]);
-            else v[k][0] = dev::Vec16<P>::to_float(to[address(base, r, i)]);
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-          int r, i;
-          if (!place(run, e0 + k * kSmallT, base, r, i)) continue;
-          float x[V];
-          if constexpr (V == 4) {
-            if (p.tall) {
-              const float4 f = *stage_at(stage, r, i >> 2);
-              x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
-            } else {
-#pragma unroll
-              for (int y = 0; y < 4; ++y) x[y] = *stage_one(stage, r + y, i);
-            }
-          } else {
-            x[0] = *stage_one(stage, r, i);
-          }
-          if (!fresh) {
-#pragma unroll
-            for (int y = 0; y < V; ++y) x[y] = v[k][y] * target.decay - target.rate * x[y];
-          }
-          if constexpr (V == 4) store4(to + address(base, r, i), x);
-          else to[address(base, r, i)] = dev::Vec16<P>::from_float(x[0]);
+      for (int k = 0; k < kRuns; ++k) {
+        if (k0 + k < runs) {
+          if constexpr (V == 4) load4<P>(to + at + k * step, next[k]);
+          else next[k][0] = dev::Vec16<P>::to_float(to[at + k * step]);
         }
       }
     };
-    auto write = [&](auto* to, bool fresh) {
-      if (p.vector_out) write_runs(to, fresh, std::integral_constant<int, 4>{});
-      else write_runs(to, fresh, std::integral_constant<int, 1>{});
-    };
-    if (target.result != nullptr) write(target.result + int64_t(batch) * p.m * p.n, true);
-    else if (target.param_dtype == NANGILA_F32) write(static_cast<float*>(target.param[batch]), false);
-    else if (target.param_dtype == NANGILA_BF16) write(static_cast<__nv_bfloat16*>(target.param[batch]), false);
-    else write(static_cast<__half*>(target.param[batch]), false);
-  }
+    if (!kFresh && mine > 0) fetch(0, 0);
+    for (int b = 0; b < mine; ++b) {
+      const int runs = runs_of(run, b, first);
+      const int64_t start = start_of(run, b, first);
+      Walk w = first;
+      __syncthreads();
+#pragma unroll 1
+      for (int c = 0; c < 64; c += 16) {
+        float f16[16];
+        tmem_ld_32x32b_x16(tmem + lanes + uint32_t(128 * (1 + b) + half * 64 + c), f16);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          *stage_at(stage, row, (half * 64 + c) / 4 + x) = make_float4(f16[4 * x] * unscale, f16[4 * x + 1] * unscale, f16[4 * x + 2] * unscale, f16[4 * x + 3] * unscale);
+      }
+      __syncthreads();
+      for (int k0 = 0; k0 < last; k0 += kRuns) {
+        if constexpr (!kFresh) {
+#pragma unroll
+          for (int k = 0; k < kRuns; ++k)
+#pragma unroll
+            for (int x = 0; x < V; ++x) v[k][x] = next[k][x];
+          if (k0 + kRuns < last) fetch(b, k0 + kRuns);
+          else if (b + 1 < mine) fetch(b + 1, 0);
+        }
+        float x[kRuns][V];
+#pragma unroll
+        for (int k = 0; k < kRuns; ++k) {
+          if (k0 + k < runs) {
+            if constexpr (V == 4 && TALL) {
+              const float4 f = *stage_at(stage, w.r, w.i >> 2);
+              x[k][0] = f.x; x[k][1] = f.y; x[k][2] = f.z; x[k][3] = f.w;
+            } else {
+#pragma unroll
+              for (int y = 0; y < V; ++y) x[k][y] = *stage_one(stage, w.r + y, w.i);
+            }
+          }
+          advance(run, w, dr, di);
+        }
+#pragma unroll
+        for (int k = 0; k < kRuns; ++k) {
+          if constexpr (!kFresh) {
+#pragma unroll
+            for (int y = 0; y < V; ++y) x[k][y] = v[k][y] * target.decay - target.rate * x[k][y];
+          }
+          if (k0 + k < runs) {
+            if constexpr (V == 4) store4(to + start + (k0 + k) * step, x[k]);
+            else to[start + (k0 + k) * step] = dev::Vec16<P>::from_float(x[k][0]);
+          }
+        }
+      }
+    }
+  };
+  auto write_all = [&](auto* to, auto fresh) {
+    if (p.vector_out) write(to, fresh, std::integral_constant<int, 4>{});
+    else write(to, fresh, std::integral_constant<int, 1>{});
+  };
+  if (target.result != nullptr) write_all(target.result + int64_t(batch) * p.m * p.n, std::true_type{});
+  else if (target.param_dtype == NANGILA_F32) write_all(static_cast<float*>(target.param[batch]), std::false_type{});
+  else if (target.param_dtype == NANGILA_BF16) write_all(static_cast<__nv_bfloat16*>(target.param[batch]), std::false_type{});
+  else write_all(static_cast<__half*>(target.param[batch]), std::false_type{});
   tc_fence_before_sync();
   cluster_sync();  // nobody's shared memory goes while another may read it
   if (warp == 0) tmem_dealloc(tmem, 512);
@@ -1287,8 +1362,8 @@ int small_cluster(int64_t m, int64_t n) {
   return ctas;
 }
 template <typename T>
-int launch_small(const Small& p, const Target& target, int count, int cluster, cudaStream_t stream) {
-  auto* kernel = orth_small_kernel<T>;
+int launch_small(const Small& p, const Target& target, bool tall, int count, int cluster, cudaStream_t stream) {
+  auto* kernel = tall ? orth_small_kernel<T, true> : orth_small_kernel<T, false>;
   if (const int e = allow_smem(reinterpret_cast<const void*>(kernel), kSmallSmem)) return e;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1368,16 +1443,15 @@ extern "C" int nangila_orth(const NangilaOrthParams* p, cudaStream_t stream) {
     s.steps = p->steps;
     s.m = int(l.m);
     s.n = int(l.n);
-    s.tall = tall ? 1 : 0;
     s.nesterov = p->nesterov;
     s.blocks = int((l.n + 127) / 128);
     s.per = (s.blocks + cluster - 1) / cluster;
     s.mu = p->mu;
     s.eps = p->eps;
     s.scale = scale;
-    return p->grad_dtype == NANGILA_F32   ? launch_small<float>(s, target, p->count, cluster, stream)
-           : p->grad_dtype == NANGILA_F16 ? launch_small<__half>(s, target, p->count, cluster, stream)
-                                          : launch_small<__nv_bfloat16>(s, target, p->count, cluster, stream);
+    return p->grad_dtype == NANGILA_F32   ? launch_small<float>(s, target, tall, p->count, cluster, stream)
+           : p->grad_dtype == NANGILA_F16 ? launch_small<__half>(s, target, tall, p->count, cluster, stream)
+                                          : launch_small<__nv_bfloat16>(s, target, tall, p->count, cluster, stream);
   }
 
   Prep prep;
