@@ -1046,39 +1046,43 @@ __global__ void __launch_bounds__(kSmallT, 1) orth_small_kernel(const __grid_con
         }
       }
     } else {
-      // 128 / ranks rows are each CTA's to add up, for all: the others' parts of them go into its staging area, [rank][row]. (A CTA without rows has none to
-      // send, and its accumulator holds nothing.)
-      const int rows = 128 / int(ranks), parts = (p.blocks + p.per - 1) / p.per;  // CTAs with rows
-      if (int(rank) < parts) {
-        const float mul = *failed != 0 ? __uint_as_float(0x7fc00000u) : unscale2;
-        const uint32_t owner = uint32_t(row / rows);
-        const int at = int(rank) * rows + row % rows;
-#pragma unroll 1
+      // 128 / ranks rows are each CTA's to add up, for all: the others' parts of them go into its staging area, [rank][row]. A CTA without rows sends zeros.
+      auto add_up = [&](auto of) {
+        constexpr int R = decltype(of)::value, kRows = 128 / R;
+        const float mul = *failed != 0 ? __uint_as_float(0x7fc00000u) : mine > 0 ? unscale2 : 0.0f;
+        const uint32_t owner = uint32_t(row / kRows);
+        const int at = int(rank) * kRows + row % kRows;
+#pragma unroll
         for (int c = 0; c < 64; c += 16) {
           float v[16];
           tmem_ld_32x32b_x16(tmem + lanes + uint32_t(half * 64 + c), v);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const float4 f = make_float4(v[4 * q] * mul, v[4 * q + 1] * mul, v[4 * q + 2] * mul, v[4 * q + 3] * mul);
+            float4 f = make_float4(v[4 * q] * mul, v[4 * q + 1] * mul, v[4 * q + 2] * mul, v[4 * q + 3] * mul);
+            if (mine == 0) f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // (its accumulator holds nothing, not even numbers)
             store_cluster(cluster_address(stage_at(stage, at, (half * 64 + c) / 4 + q), owner), *reinterpret_cast<const uint4*>(&f));
           }
         }
-      }
-      tc_fence_before_sync();
-      cluster_sync();
-      for (int e = threadIdx.x; e < rows * 16; e += kSmallT) {
-        const int own = e >> 4, r = int(rank) * rows + own, c = e & 15;  // eight columns
-        float v[8] = {};
+        tc_fence_before_sync();
+        cluster_sync();
 #pragma unroll
-        for (int i = 0; i < kMaxCluster; ++i) {
-          if (i < parts) {
-            const float4 x = *stage_at(stage, i * rows + own, 2 * c), y = *stage_at(stage, i * rows + own, 2 * c + 1);
+        for (int e = 0; e < kRows * 16 / kSmallT; ++e) {  // eight columns at a time
+          const int own = (int(threadIdx.x) >> 4) + e * (kSmallT / 16), r = int(rank) * kRows + own, c = threadIdx.x & 15;
+          float v[8] = {};
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            const float4 x = *stage_at(stage, i * kRows + own, 2 * c), y = *stage_at(stage, i * kRows + own, 2 * c + 1);
             v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
           }
+          const uint4 packed = pack8(v);
+          const void* to = box_at(a_mat + (c >> 3) * kHalfBytes, r, c & 7);
+#pragma unroll
+          for (int i = 0; i < R; ++i) store_cluster(cluster_address(to, uint32_t(i)), packed);
         }
-        const uint4 packed = pack8(v);
-        for (uint32_t i = 0; i < ranks; ++i) store_cluster(cluster_address(box_at(a_mat + (c >> 3) * kHalfBytes, r, c & 7), i), packed);
-      }
+      };
+      if (ranks == 2) add_up(std::integral_constant<int, 2>{});
+      else if (ranks == 4) add_up(std::integral_constant<int, 4>{});
+      else add_up(std::integral_constant<int, 8>{});
       cluster_sync();
     }
     ready();
