@@ -92,8 +92,7 @@ NormOut norm_forward(const Tensor& x_in, const Tensor& residual_in, const Tensor
   if (fp8) {
     o.q = at::empty(x_in.sizes(), x_in.options().dtype(at::kFloat8_e4m3fn));
     std::vector<int64_t> shape = x_in.sizes().vec();
-    if (group) shape.back() = d / group;
-    else shape.pop_back();
+    shape.back() = group ? d / group : 1;
     o.scale = at::empty(shape, x_in.options().dtype(at::kFloat));
   } else {
     o.y = at::empty(x_in.sizes(), x_in.options());
@@ -230,7 +229,7 @@ std::tuple<Tensor, Tensor, c10::optional<Tensor>> rms_norm_fp8(const Tensor& x, 
     const Tensor h = residual.defined() ? x + residual : x;
     Tensor f = cpu_unit(h, weight, eps);
     const std::vector<int64_t> shape = f.sizes().vec();
-    if (group) f = f.unflatten(-1, {a.d / group, group});
+    f = f.unflatten(-1, {group ? a.d / group : 1, group ? group : a.d});
     Tensor amax = f.abs().amax(-1);
     Tensor scale = at::where(at::isfinite(amax), amax.clamp_min(1e-12) / 448.0, at::full_like(amax, NAN));
     Tensor q = (f / scale.unsqueeze(-1)).clamp(-448.0, 448.0).to(at::kFloat8_e4m3fn).reshape(shape);

@@ -345,10 +345,14 @@ extern "C" int nangila_rotary(const NangilaRotaryParams* p, cudaStream_t stream)
       p->batch < 1 || p->seq < 1 || p->d < 2 || p->rot < 2 || p->rot % 2 != 0 || p->rot > p->d || !p->table || p->table_rows < 1 ||
       (p->positions == nullptr && p->seq > p->table_rows))
     return int(cudaErrorInvalidValue);
-  switch (p->dtype) {
-    case NANGILA_F32: return launch<float>(*p, stream);
-    case NANGILA_F16: return launch<__half>(*p, stream);
-    case NANGILA_BF16: return launch<__nv_bfloat16>(*p, stream);
-    default: return int(cudaErrorInvalidValue);
+  try {
+    switch (p->dtype) {
+      case NANGILA_F32: return launch<float>(*p, stream);
+      case NANGILA_F16: return launch<__half>(*p, stream);
+      case NANGILA_BF16: return launch<__nv_bfloat16>(*p, stream);
+      default: return int(cudaErrorInvalidValue);
+    }
+  } catch (...) {  // (the host's table of occupancies allocates)
+    return int(cudaErrorMemoryAllocation);
   }
 }

@@ -40,6 +40,7 @@ def test_eight_bits_is_the_formula(group):
     x[1] = 0
     x[2, 200] = float("nan")
     q, scale = ops.rms_norm_fp8(x, w, group=group)
+    assert q.shape == x.shape and scale.shape == (6, 2 if group else 1)
     keep = [0, 1, 3, 4, 5]
     f = plain.norm(x[keep], w, 1e-5).view(5, -1, group or 256)
     s = scale[keep].double().view(5, -1)

@@ -140,7 +140,7 @@ def test_eight_bits(rows, d, group, dtype, with_residual):
         h = out[2]
         assert torch.equal(h, (x.float() + r.float()).to(dtype))
     f = plain.norm(h, w, EPS).view(rows, -1, group or d)
-    assert q.dtype == torch.float8_e4m3fn and q.shape == x.shape and scale.shape == ((rows, d // group) if group else (rows,))
+    assert q.dtype == torch.float8_e4m3fn and q.shape == x.shape and scale.shape == (rows, d // group if group else 1)
     s = f.abs().amax(-1).clamp(min=1e-12) / 448
     sc = scale.view(s.shape)
     assert_near(sc, s, s * 2 * F32)

@@ -102,8 +102,9 @@ def test_many_matrices_at_once_are_what_each_is_alone():
     assert torch.equal(mixed[0], together[0]) and mixed[2].device.type == "cpu" and rel(mixed[2].cuda(), together[0].double()) < 2 * TOL
 
 
-def test_a_matrix_that_is_not_finite_spoils_no_other():
-    many = [gradient(96, 130, seed=i) for i in range(5)]
+@pytest.mark.parametrize("m,n", [(96, 130), (500, 100), (300, 200), (200, 2500)])
+def test_a_matrix_that_is_not_finite_spoils_no_other(m, n):
+    many = [gradient(m, n, seed=i) for i in range(5)]
     clean = ops().orthogonalize(many)
     many[1][3, 4] = float("nan")
     many[3][0, 0] = float("inf")
@@ -149,7 +150,7 @@ def muon_plain(p, g, m, lr, mu, nesterov, wd, scale):
 
 @pytest.mark.parametrize("nesterov,scale", [(True, "rms"), (False, "spectral"), (True, None)])
 @pytest.mark.parametrize("ptype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("m,n", [(96, 160), (161, 97), (128, 256)])
+@pytest.mark.parametrize("m,n", [(96, 160), (161, 97), (128, 256), (256, 384), (301, 203), (130, 1029), (600, 152)])
 def test_muon_step(m, n, ptype, nesterov, scale):
     g = torch.Generator(device="cuda").manual_seed(m)
     ps = [0.1 * torch.randn(m, n, device="cuda", generator=g).to(ptype) for _ in range(3)]
@@ -165,9 +166,10 @@ def test_muon_step(m, n, ptype, nesterov, scale):
             assert rel(mo, wm) < 2.0 ** -22
 
 
-def test_muon_step_of_unaligned_tensors_and_captured():
-    hold = [torch.randn(96 * 160 + 1, device="cuda") for _ in range(3)]
-    p, g, m = (h[1:].view(96, 160) for h in hold)
+@pytest.mark.parametrize("rows,cols", [(96, 160), (160, 96), (1000, 104), (264, 200), (200, 2000)])
+def test_muon_step_of_unaligned_tensors_and_captured(rows, cols):
+    hold = [torch.randn(rows * cols + 1, device="cuda") for _ in range(3)]
+    p, g, m = (h[1:].view(rows, cols) for h in hold)
     want, wm, size = muon_plain(p, g, m, 0.02, 0.95, True, 0.0, "rms")
     keep = p.clone(), m.clone()
     ops().muon_step([p], [g], [m], lr=0.02)
@@ -182,6 +184,35 @@ def test_muon_step_of_unaligned_tensors_and_captured():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(p, once[0]) and torch.equal(m, once[1])
+
+
+def test_two_captured_graphs_and_a_call_between_them():
+    """Graphs have workspaces of their own: replays in any order, on streams of their own, give what a call gives."""
+    us = [gradient(264, 320, seed=i) for i in range(2)] + [gradient(100, 600, seed=2)]
+    want = [ops().orthogonalize(u) for u in us]
+    graphs, held = [], []
+    for u in us:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held.append(ops().orthogonalize(u))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        between = ops().orthogonalize(us[0])
+    torch.cuda.synchronize()
+    for h, w in zip(held, want):
+        assert torch.equal(h, w)
+    assert torch.equal(between, want[0])
+
+
+def test_orthogonal_update_of_a_step_by_differences():
+    """The update does not depend on the gradient's size: its difference quotient along the gradient itself vanishes."""
+    u = gradient(160, 200)
+    a, b = ops().orthogonalize(u).double(), ops().orthogonalize(u * 1.5).double()
+    assert rel(a, b) < 2 * TOL
 
 
 def test_an_updated_parameter_is_seen_as_changed():
