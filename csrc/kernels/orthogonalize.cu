@@ -166,14 +166,15 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&v)[4]) {
 }
 // A warp's 32 rows of results in a slot, fp32, taken to the parameters (T) or, with `fresh`, out. Two rows at a time, four columns a lane; the loads of
 // sixteen rows are on their way before the first store.
-template <typename T, bool fresh>
+template <typename T, bool fresh, bool copies>
 __device__ __forceinline__ void put_results(const Product& p, const Target& to_where, T* base, uint8_t* slot, int lane, int row0, int col0) {
   const int x = lane & 15, col = col0 + 4 * x, left = p.N - col;
   if (left <= 0) return;
   // four columns 4 x: group x / 4 of sixteen, its quarter x % 4
   uint8_t* box = slot + ((x & 2) ? kBoxBytes : 0);
   const int j = 2 * (x >> 2) + (x & 1);
-#pragma unroll 1
+  constexpr int kCopies = copies ? 2 : 1;
+#pragma unroll kCopies
   for (int half = 0; half < 32; half += 16) {
     float v[8][4];
     if (!fresh) {
@@ -410,8 +411,10 @@ __device__ __forceinline__ void finish_tile(const Shared& s, uint32_t tmem, cons
       if (lane == 0) bulk_wait_read();  // the slot's last stores
       __syncwarp();
     }
-    // (a loop, not four copies of it: the first tile of a launch is bound by fetching this code. 128 x 128 tiles: 2.2 us unrolled, for 1.6 us)
-#pragma unroll 1
+    // (In small tiles a loop, not four copies of it: the only tile of a launch is bound by fetching this code. 256 x 256 in all: 97 us unrolled, 91 so. Where CTAs
+    // take many tiles the copies are faster: update of sixteen 2048 x 2048 204 us, 218 as a loop.)
+    constexpr int kCopies = PAIR ? kChunk / 16 : 1;
+#pragma unroll kCopies
     for (int g = 0; g < kChunk / 16; ++g) {
       float v[16];
       tmem_ld_32x32b_x16(tmem + (uint32_t(quad * 32) << 16) + uint32_t(acc * kSide + c * kChunk + g * 16), v);
@@ -431,10 +434,10 @@ __device__ __forceinline__ void finish_tile(const Shared& s, uint32_t tmem, cons
     const int col0 = at.n0 + c * kChunk;
     if constexpr (KIND == kFinal) {
       __syncwarp();
-      if (target.result != nullptr) put_results<__nv_bfloat16, true>(p, target, target.result + int64_t(at.batch) * p.M * p.N, slot, lane, row0, col0);
-      else if (target.param_dtype == NANGILA_F32) put_results<float, false>(p, target, static_cast<float*>(target.param[at.batch]), slot, lane, row0, col0);
-      else if (target.param_dtype == NANGILA_BF16) put_results<__nv_bfloat16, false>(p, target, static_cast<__nv_bfloat16*>(target.param[at.batch]), slot, lane, row0, col0);
-      else put_results<__half, false>(p, target, static_cast<__half*>(target.param[at.batch]), slot, lane, row0, col0);
+      if (target.result != nullptr) put_results<__nv_bfloat16, true, PAIR>(p, target, target.result + int64_t(at.batch) * p.M * p.N, slot, lane, row0, col0);
+      else if (target.param_dtype == NANGILA_F32) put_results<float, false, PAIR>(p, target, static_cast<float*>(target.param[at.batch]), slot, lane, row0, col0);
+      else if (target.param_dtype == NANGILA_BF16) put_results<__nv_bfloat16, false, PAIR>(p, target, static_cast<__nv_bfloat16*>(target.param[at.batch]), slot, lane, row0, col0);
+      else put_results<__half, false, PAIR>(p, target, static_cast<__half*>(target.param[at.batch]), slot, lane, row0, col0);
       // the slot is filled by TMA again: what was read and written here comes first
       fence_async_proxy();
       __syncwarp();
@@ -473,6 +476,10 @@ __device__ __forceinline__ double square_sum(const float (&u)[N]) {
 // products of the next, and what it needs of X or A is on its way before they end. Each of its warps has a slot of shared memory of its own,
 // filled and emptied by TMA, and meets no other warp.
 // A wait that runs out makes every result of this CTA from there on not a number.
+// Bound: large ones by the tensor cores, and by power in a long run (update of 4096 x 16384: 376 us, 1.46 PFLOP/s on its own; five steps of it 4.0 ms at the 1000 W limit, where
+// a library's fp16 product of this shape runs at 1.27). Alone, a CTA's 128 x 128 tile is bound by the 64 bytes a cycle that L2 delivers to an SM (32 KB a slab,
+// 0.27 us); with 128 x 256 tiles of one CTA the update took 469 us. Small ones by the way from launch to launch: 768 x 768 about 8 us for each of 15 products, of which
+// 3.2 are the 12 slabs, 1.4 the first load, 1.2 the results, 1.9 the end of a kernel until the next one sees its data.
 template <int KIND, bool A_MN, bool B_MN, bool PAIR>
 __global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, const __grid_constant__ Target target) {
   constexpr int kSide = PAIR ? 256 : 128;
@@ -542,7 +549,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __g
 }
 
 // The Gram matrix where few tiles share a long K: a cluster takes a tile, each CTA a part of K and, in the end, 128 / S columns of the result. The parts
-// meet through shared memory, in the order of the ranks.
+// meet through shared memory, in the order of the ranks. Three of 2051 x 517 (45 tiles, 33 slabs, two CTAs a tile): five steps 243 -> 219 us.
 template <bool MN>
 __global__ void __launch_bounds__(kGemmThreads, 1) orth_gram_split_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, __half* __restrict__ out, int64_t ld, int64_t matrix) {
   extern __shared__ uint8_t smem_raw[];
@@ -643,7 +650,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gram_split_kernel(const 
 }
 
 // ---- from the gradients to X -------------------------------------------------------------------------------------------------
-// Two passes over the gradients, which are small next to the products: the sum of squares, in 64 bits and in an order that the sizes determine,
+// Two passes over the gradients, which are small next to the products (16 of 2048 x 2048, momentum and all: 98 us each, 6.8 TB/s): the sum of squares, in 64 bits and in an order that the sizes determine,
 // then X. With momentum the first pass also advances it: M <- mu M + G, U = G + mu M (Nesterov) or M.
 constexpr int kPrepT = 256;
 constexpr int kMaxChunks = 1024;
@@ -667,7 +674,7 @@ __device__ __forceinline__ double block_sum(double v, double* s) {
   for (int i = 0; i < kPrepT / 32; ++i) v += s[i];
   return v;
 }
-template <typename T>
+template <typename T, bool MOM>
 __global__ void __launch_bounds__(kPrepT) orth_norm_kernel(const __grid_constant__ Prep p) {
   __shared__ double s[kPrepT / 32];
   const T* g = static_cast<const T*>(p.grad[blockIdx.y]);
@@ -676,16 +683,16 @@ __global__ void __launch_bounds__(kPrepT) orth_norm_kernel(const __grid_constant
   double sum = 0.0;
   may_follow();
   const int64_t runs = p.flat ? p.numel / 8 : 0;
-  constexpr int kAhead = 4;  // runs of eight on their way
+  constexpr int kAhead = MOM ? 1 : 4;  // runs of eight on their way (with momentum, 16 of 2048 x 2048: one 98 us, four 121: fewer threads fit)
   for (int64_t i0 = first; i0 < runs; i0 += kAhead * stride) {
     dev::Raw8<T> raw[kAhead];
-    dev::Raw8<float> old[kAhead];
+    dev::Raw8<float> old[MOM ? kAhead : 1];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int64_t i = i0 + k * stride;
       if (i >= runs) break;
       dev::fetch(g + i * 8, raw[k]);
-      if (m != nullptr) dev::fetch(m + i * 8, old[k]);
+      if constexpr (MOM) dev::fetch(m + i * 8, old[k]);
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
@@ -693,7 +700,7 @@ __global__ void __launch_bounds__(kPrepT) orth_norm_kernel(const __grid_constant
       if (i >= runs) break;
       float u[8];
       dev::unpack(raw[k], u);
-      if (m != nullptr) {
+      if constexpr (MOM) {
         float v[8];
         dev::unpack(old[k], v);
 #pragma unroll
@@ -709,7 +716,7 @@ __global__ void __launch_bounds__(kPrepT) orth_norm_kernel(const __grid_constant
   }
   for (int64_t i = runs * 8 + first; i < p.numel; i += stride) {
     float u = dev::Vec16<T>::to_float(g[i]);
-    if (m != nullptr) {
+    if (MOM) {
       const float v = __fmaf_rn(p.mu, m[i], u);
       u = p.nesterov ? __fmaf_rn(p.mu, v, u) : v;
       m[i] = v;
@@ -784,6 +791,7 @@ __global__ void __launch_bounds__(kPrepT) orth_start_kernel(const __grid_constan
 // fp32 in tensor memory, and rounded to fp16 in shared memory as the products' operand; longer ones are shared out over a cluster, whose
 // CTAs add up their parts of the Gram matrix through one another's shared memory, in the order of their ranks. Every product is a few instructions of
 // 128 x 128, so what bounds this is the way from one to the next: two thirds of a step are waits for a product and the pass over its results.
+// 128 x 128: 25 us in all, 2.6 a step; 352 x 128, 24 of them: 39 us (product by product 117); 1024 x 128 in a cluster of four: 52 us (95).
 //   D = X^T X (n long, from X by rows of n: MN-major),  A = D;   D = A A,  B = b A + c D;   X <- a X + X B, accumulated onto a X in tensor memory.
 constexpr int kSmallT = 256;
 constexpr int kRuns = 8;                         // of elements that a thread has on their way, to and from memory
@@ -1400,7 +1408,8 @@ int launch_small(const Small& p, const Target& target, bool tall, int count, int
 template <typename T>
 int start(const Prep& p, int count, cudaStream_t stream) {
   const dim3 grid(unsigned(p.chunks), unsigned(count));
-  orth_norm_kernel<T><<<grid, kPrepT, 0, stream>>>(p);
+  if (p.momentum[0] != nullptr) orth_norm_kernel<T, true><<<grid, kPrepT, 0, stream>>>(p);
+  else orth_norm_kernel<T, false><<<grid, kPrepT, 0, stream>>>(p);
   if (const cudaError_t e = cudaGetLastError()) return int(e);
   return int(launch_following(orth_start_kernel<T>, grid, kPrepT, 0, stream, p));
 }
