@@ -53,15 +53,22 @@ constexpr int kStages = 5;
 constexpr int kChunk = 64;                       // columns that a warp of the epilogue takes at a time
 constexpr int kBoxBytes = 32 * kChunk * 2;       // 32 rows of them in fp16
 constexpr int kSlotBytes = 2 * kBoxBytes;        // what comes in and goes out at a time, in place
-constexpr int kEpilogueWarps = 8;                // two for each quarter of tensor memory, taking turns with the chunks
-constexpr int kEpilogueBytes = kEpilogueWarps * kSlotBytes;
+constexpr int kEpilogueSlots = 8;
+constexpr int kEpilogueBytes = kEpilogueSlots * kSlotBytes;
 constexpr int kSmem = kStages * kStageBytes + kEpilogueBytes + 1024 + 256;
-constexpr int kGemmThreads = 64 + 32 * kEpilogueWarps;  // warp 0: TMA, warp 1: products, the others: epilogue
 constexpr uint64_t kTimeoutNs = 10ull * 1000 * 1000 * 1000;
 constexpr float kLoScale = 2048.0f;
 constexpr int kMaxCluster = 8;
 
 enum Kind { kGram, kPoly, kUpdate, kFinal };
+
+// Warps of the epilogue for each quarter of tensor memory, and slots of each. Two warps with a slot each take turns with a tile's chunks, which ends small tiles
+// sooner; where the results go under the next tile's products anyhow, one warp with two slots disturbs those less (update of 4096 x 16384 376 us, for 397; of sixteen
+// 2048 x 2048 204 us, for 219), but for the last one, which reads and writes parameters (sixteen 2048 x 2048: 409 us with one warp, 250 with two).
+template <int KIND, bool PAIR>
+constexpr int kTurns = PAIR && KIND != kFinal ? 1 : 2;
+template <int KIND, bool PAIR>
+constexpr int kGemmThreads = 64 + 32 * 4 * kTurns<KIND, PAIR>;  // warp 0: TMA, warp 1: products, the others: epilogue
 
 struct Product {
   int M, N, K;             // D is M x N
@@ -262,7 +269,7 @@ struct Shared {
   uint8_t *stages, *slots;
   uint64_t *full, *empty;          // [kStages]
   uint64_t *acc_full, *acc_empty;  // [2]
-  uint64_t *loaded;                // [kEpilogueWarps]
+  uint64_t *loaded;                // [kEpilogueSlots]
   uint64_t *drained;
   uint32_t* tmem_slot;
   volatile uint32_t* failed;       // a wait has run out
@@ -276,12 +283,12 @@ __device__ __forceinline__ Shared shared_parts(uint8_t* raw) {
   s.acc_full = s.empty + kStages;
   s.acc_empty = s.acc_full + 2;
   s.loaded = s.acc_empty + 2;
-  s.drained = s.loaded + kEpilogueWarps;
+  s.drained = s.loaded + kEpilogueSlots;
   s.tmem_slot = reinterpret_cast<uint32_t*>(s.drained + 1);
   s.failed = s.tmem_slot + 1;
   return s;
 }
-template <bool PAIR>
+template <int KIND, bool PAIR>
 __device__ __forceinline__ void init_barriers(const Shared& s) {
   for (int i = 0; i < kStages; ++i) {
     mbar_init(&s.full[i], 1);
@@ -289,9 +296,9 @@ __device__ __forceinline__ void init_barriers(const Shared& s) {
   }
   for (int i = 0; i < 2; ++i) {
     mbar_init(&s.acc_full[i], 1);
-    mbar_init(&s.acc_empty[i], kEpilogueWarps * (PAIR ? 2 : 1));
+    mbar_init(&s.acc_empty[i], 4 * kTurns<KIND, PAIR> * (PAIR ? 2 : 1));
   }
-  for (int i = 0; i < kEpilogueWarps; ++i) mbar_init(&s.loaded[i], 1);
+  for (int i = 0; i < kEpilogueSlots; ++i) mbar_init(&s.loaded[i], 1);
   mbar_init(s.drained, 1);
   *s.failed = 0;
   fence_barrier_init();
@@ -372,7 +379,7 @@ __device__ __forceinline__ void drain_products(const Shared& s) {
   else umma_commit(s.drained);
   mbar_wait(s.drained, 0, kTimeoutNs);
 }
-// The n-th tile's accumulator taken to where it belongs, by one of the epilogue's warps; `chunks`: how many it has loaded so far.
+// The n-th tile's accumulator taken to where it belongs, by one of the epilogue's warps; `chunks`: how many it has done so far.
 template <int KIND, bool PAIR>
 __device__ __forceinline__ void finish_tile(const Shared& s, uint32_t tmem, const Product& p, const Target& target, const CUtensorMap* in, const CUtensorMap* lo, const CUtensorMap* out,
                                             const CUtensorMap* mirror, const TileAt& at, uint32_t rank, int n, uint32_t& chunks) {
@@ -383,36 +390,45 @@ __device__ __forceinline__ void finish_tile(const Shared& s, uint32_t tmem, cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quad = warp & 3;  // the lanes of tensor memory that this warp may read
   const int turn = (warp - 2) >> 2;
-  uint8_t* slot = s.slots + (warp - 2) * kSlotBytes;
-  uint64_t* my_loaded = s.loaded + (warp - 2);
+  constexpr int kWarps = kTurns<KIND, PAIR>, kSlots = 2 / kWarps;
   const int acc = n & 1;
   const int row0 = at.m0 + int(rank) * kTileM + quad * 32;
   const int mine = row0 < p.M ? min(kChunks, (p.N - at.n0 + kChunk - 1) / kChunk) : 0;
-  auto fetch = [&](int c) {  // lane 0: chunk c into the slot, once nothing goes out of it any more
+  auto slot_of = [&](uint32_t turn_no) { return s.slots + ((warp - 2) * kSlots + turn_no % kSlots) * kSlotBytes; };
+  auto loaded_of = [&](uint32_t turn_no) { return s.loaded + (warp - 2) * kSlots + turn_no % kSlots; };
+  auto fetch = [&](int c, uint32_t turn_no) {  // lane 0: chunk c into the slot whose turn it is, once nothing goes out any more
+    uint8_t* to = slot_of(turn_no);
+    uint64_t* bar = loaded_of(turn_no);
     bulk_wait_read();
-    mbar_arrive_expect_tx(my_loaded, kLoadBytes);
-    tma_load_3d(slot, in, at.n0 + c * kChunk, row0, at.batch, my_loaded);
-    if (KIND != kPoly) tma_load_3d(slot + kBoxBytes, lo, at.n0 + c * kChunk, row0, at.batch, my_loaded);
+    mbar_arrive_expect_tx(bar, kLoadBytes);
+    tma_load_3d(to, in, at.n0 + c * kChunk, row0, at.batch, bar);
+    if (KIND != kPoly) tma_load_3d(to + kBoxBytes, lo, at.n0 + c * kChunk, row0, at.batch, bar);
   };
-  if (kLoads && turn < mine && lane == 0) fetch(turn);
+  if (kLoads && turn < mine && lane == 0) fetch(turn, chunks);
   bool ok = *s.failed == 0 && mbar_wait(&s.acc_full[acc], uint32_t((n / 2) & 1), kTimeoutNs);
   ok = __all_sync(0xffffffffu, ok);
   if (!ok) *s.failed = 1;
   tc_fence_after_sync();
 #pragma unroll 1
-  for (int c = turn; c < mine; c += 2) {
+  for (int c = turn; c < mine; c += kWarps, ++chunks) {
+    uint8_t* slot = slot_of(chunks);
     if (kLoads) {
-      if (c != turn && lane == 0) fetch(c);
-      const bool here = mbar_wait(my_loaded, chunks & 1, kTimeoutNs);
-      ++chunks;
+      if (kSlots > 1) {
+        if (c + kWarps < mine && lane == 0) fetch(c + kWarps, chunks + 1);
+      } else {
+        if (c != turn && lane == 0) fetch(c, chunks);
+      }
+      const bool here = mbar_wait(loaded_of(chunks), (chunks / kSlots) & 1, kTimeoutNs);
       if (!__all_sync(0xffffffffu, here)) ok = false;
       if (!ok) *s.failed = 1;
     } else {
-      if (lane == 0) bulk_wait_read();  // the slot's last stores
+      if (lane == 0) {  // the slot's last stores
+        if (kSlots > 1) bulk_wait_read_but_one();
+        else bulk_wait_read();
+      }
       __syncwarp();
     }
-    // (In small tiles a loop, not four copies of it: the only tile of a launch is bound by fetching this code. 256 x 256 in all: 97 us unrolled, 91 so. Where CTAs
-    // take many tiles the copies are faster: update of sixteen 2048 x 2048 204 us, 218 as a loop.)
+    // (In small tiles a loop, not four copies of it: the only tile of a launch is bound by fetching this code. 256 x 256 in all: 97 us unrolled, 91 so.)
     constexpr int kCopies = PAIR ? kChunk / 16 : 1;
 #pragma unroll kCopies
     for (int g = 0; g < kChunk / 16; ++g) {
@@ -473,7 +489,7 @@ __device__ __forceinline__ double square_sum(const float (&u)[N]) {
 // D = A B for square tiles of all matrices, walked over by CTAs that stay (PAIR: pairs of CTAs that share the tensor cores' work on 256 x 256, each
 // with its 128 rows of A, half of B's columns, and 128 rows of the result; else one CTA and 128 x 128). A_MN / B_MN: the operand lies with its rows
 // (columns of B) adjacent in memory, not its K. The accumulators of two tiles share tensor memory: the epilogue of one runs under the
-// products of the next, and what it needs of X or A is on its way before they end. Each of its warps has a slot of shared memory of its own,
+// products of the next, and what it needs of X or A is on its way before they end. Each of its warps has one or two slots of shared memory of its own,
 // filled and emptied by TMA, and meets no other warp.
 // A wait that runs out makes every result of this CTA from there on not a number.
 // Bound: large ones by the tensor cores, and by power in a long run (update of 4096 x 16384: 376 us, 1.46 PFLOP/s on its own; five steps of it 4.0 ms at the 1000 W limit, where
@@ -481,7 +497,7 @@ __device__ __forceinline__ double square_sum(const float (&u)[N]) {
 // 0.27 us); with 128 x 256 tiles of one CTA the update took 469 us. Small ones by the way from launch to launch: 768 x 768 about 8 us for each of 15 products, of which
 // 3.2 are the 12 slabs, 1.4 the first load, 1.2 the results, 1.9 the end of a kernel until the next one sees its data.
 template <int KIND, bool A_MN, bool B_MN, bool PAIR>
-__global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, const __grid_constant__ Target target) {
+__global__ void __launch_bounds__(kGemmThreads<KIND, PAIR>, 1) orth_product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, const __grid_constant__ Target target) {
   constexpr int kSide = PAIR ? 256 : 128;
   extern __shared__ uint8_t smem_raw[];
   const Shared s = shared_parts(smem_raw);
@@ -491,7 +507,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __g
   const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, step = PAIR ? gridDim.x / 2 : gridDim.x;
 
   if (threadIdx.x == 0) {
-    init_barriers<PAIR>(s);
+    init_barriers<KIND, PAIR>(s);
     prefetch_tensormap(&maps.a);
     prefetch_tensormap(&maps.b);
   }
@@ -551,7 +567,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_product_kernel(const __g
 // The Gram matrix where few tiles share a long K: a cluster takes a tile, each CTA a part of K and, in the end, 128 / S columns of the result. The parts
 // meet through shared memory, in the order of the ranks. Three of 2051 x 517 (45 tiles, 33 slabs, two CTAs a tile): five steps 243 -> 219 us.
 template <bool MN>
-__global__ void __launch_bounds__(kGemmThreads, 1) orth_gram_split_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, __half* __restrict__ out, int64_t ld, int64_t matrix) {
+__global__ void __launch_bounds__(kGemmThreads<kGram, false>, 1) orth_gram_split_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, __half* __restrict__ out, int64_t ld, int64_t matrix) {
   extern __shared__ uint8_t smem_raw[];
   const Shared s = shared_parts(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -565,7 +581,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gram_split_kernel(const 
   };
 
   if (threadIdx.x == 0) {
-    init_barriers<false>(s);
+    init_barriers<kGram, false>(s);
     prefetch_tensormap(&maps.a);
     prefetch_tensormap(&maps.b);
   }
@@ -1296,7 +1312,7 @@ int launch_product(const Maps& maps, Product p, const Target& target, int count,
   cudaLaunchConfig_t cfg = {};
   const int sms = sm_count();
   cfg.gridDim = dim3(unsigned(PAIR ? 2 * std::min(p.total, sms / 2) : std::min(p.total, sms)));
-  cfg.blockDim = dim3(kGemmThreads);
+  cfg.blockDim = dim3(kGemmThreads<KIND, PAIR>);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
@@ -1318,7 +1334,7 @@ int launch_gram_split(const Maps& maps, Product p, const Matrix& out, int total,
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(total * split));
-  cfg.blockDim = dim3(kGemmThreads);
+  cfg.blockDim = dim3(kGemmThreads<kGram, false>);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
