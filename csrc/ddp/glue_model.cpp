@@ -25,11 +25,14 @@ using torch::autograd::variable_list;
 bool known(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
 int dtype_code(const Tensor& t) { return t.scalar_type() == at::kFloat ? NANGILA_F32 : t.scalar_type() == at::kHalf ? NANGILA_F16 : NANGILA_BF16; }
 void check_launch(int err, const char* what) { TORCH_CHECK(err == 0, "nangila: ", what, " failed: ", cudaGetErrorString(static_cast<cudaError_t>(err))); }
+void check_plain(const Tensor& t, const char* name) {
+  TORCH_CHECK_TYPE(!t.unsafeGetTensorImpl()->is_python_dispatch(), "nangila: ", name, " must be a plain tensor (a sharded one has to be gathered first)");
+  TORCH_CHECK_TYPE(t.layout() == at::kStrided, "nangila: ", name, " must be dense");
+  TORCH_CHECK_TYPE(t.is_cuda() || t.is_cpu(), "nangila: ", name, " must be on a CUDA device or the CPU");
+}
 void check_tensor(const Tensor& t, const char* name) {
+  check_plain(t, name);
   TORCH_CHECK_TYPE(known(t.scalar_type()), "nangila: ", name, " must be float32, float16 or bfloat16, not ", t.scalar_type());
-  TORCH_CHECK_TYPE(!t.unsafeGetTensorImpl()->is_python_dispatch(), "nangila: ", name, " must be plain tensors (a sharded tensor has to be gathered first)");
-  TORCH_CHECK_TYPE(t.layout() == at::kStrided, "nangila: ", name, " must be a dense tensor");
-  TORCH_CHECK_TYPE(t.is_cuda() || t.is_cpu(), "nangila: ", name, " must be a CUDA or CPU tensor");
 }
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
@@ -250,12 +253,14 @@ void check_rotary(const Tensor& q, const Tensor& k, const Tensor& table, const T
     TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type(), "nangila: k is ", k.scalar_type(), ", q ", q.scalar_type());
     TORCH_CHECK_VALUE(k.device() == q.device(), "nangila: k is on ", k.device(), ", q on ", q.device());
   }
+  check_plain(table, "the table");
   TORCH_CHECK_VALUE(table.dim() == 3 && table.size(2) == 2 && table.scalar_type() == at::kFloat && table.size(0) >= 1 && table.size(1) >= 1,
                     "nangila: the table must be float32 of shape [positions, rot / 2, 2], got ", table.scalar_type(), " ", table.sizes());
   TORCH_CHECK_VALUE(2 * table.size(1) <= q.size(3), "nangila: the table turns ", 2 * table.size(1), " columns, a head has ", q.size(3));
   TORCH_CHECK_VALUE(table.device() == q.device(), "nangila: the table is on ", table.device(), ", q on ", q.device());
   TORCH_CHECK_VALUE(!table.requires_grad(), "nangila: the table has no gradient");
   if (positions.defined()) {
+    check_plain(positions, "positions");
     TORCH_CHECK_TYPE(positions.scalar_type() == at::kLong || positions.scalar_type() == at::kInt, "nangila: positions must be int64 or int32, not ", positions.scalar_type());
     TORCH_CHECK_VALUE(positions.device() == q.device(), "nangila: positions are on ", positions.device(), ", q on ", q.device());
     TORCH_CHECK_VALUE((positions.dim() == 1 && positions.size(0) == q.size(1)) ||

@@ -4,8 +4,8 @@
 //
 // X has m rows and n >= m columns; a matrix that is taller than wide is kept as it lies, and its transpose is what the formulas speak of.
 // The three products are one tcgen05 kernel with different operands and epilogues: operands come through TMA (128-byte swizzle, K-major or
-// MN-major, so that nothing is transposed in memory), one thread issues the products with the accumulator in tensor memory, four warps read
-// it back and write results. Of the symmetric A and A^2 only the tiles that reach the lower triangle are computed; their epilogue writes both halves.
+// MN-major, so that nothing is transposed in memory), one thread issues the products with the accumulator in tensor memory, four or eight warps
+// read it back and write results. Of the symmetric A and A^2 only the tiles that reach the lower triangle are computed; their epilogue writes both halves.
 //
 // Roundings. The products' operands are rounded to fp16 (11 bits; the values are bounded, so that bf16's range is not needed and its 8 bits
 // would cost a factor of eight), the accumulator is fp32. A and B multiply X: their errors, and those of X inside the products, come out as relative
@@ -449,14 +449,14 @@ __device__ __forceinline__ void finish_tile(const Shared& s, uint32_t tmem, cons
     }
     const int col0 = at.n0 + c * kChunk;
     if constexpr (KIND == kFinal) {
+      // the slot is filled by TMA again: what was written here comes first (a fence after the stores to memory below would wait for them)
+      fence_async_proxy();
       __syncwarp();
       if (target.result != nullptr) put_results<__nv_bfloat16, true, PAIR>(p, target, target.result + int64_t(at.batch) * p.M * p.N, slot, lane, row0, col0);
       else if (target.param_dtype == NANGILA_F32) put_results<float, false, PAIR>(p, target, static_cast<float*>(target.param[at.batch]), slot, lane, row0, col0);
       else if (target.param_dtype == NANGILA_BF16) put_results<__nv_bfloat16, false, PAIR>(p, target, static_cast<__nv_bfloat16*>(target.param[at.batch]), slot, lane, row0, col0);
       else put_results<__half, false, PAIR>(p, target, static_cast<__half*>(target.param[at.batch]), slot, lane, row0, col0);
-      // the slot is filled by TMA again: what was read and written here comes first
-      fence_async_proxy();
-      __syncwarp();
+      __syncwarp();  // all have read the slot
     } else {
       fence_async_proxy();
       __syncwarp();

@@ -27,33 +27,20 @@ namespace {
 constexpr int kT = 128;
 constexpr int kAtOnce = 4;  // (token, head) pairs of a thread whose loads are on their way together
 
-// A pair of (token, head), counted from the CTA's first token; the heads of both tensors follow one another.
+// Where pair `g` of (token, head) lies; the heads of both tensors follow one another.
 struct Where {
   int which;       // q or k
   int64_t in, out; // first column of the head
   int64_t row;     // of the table; -1: outside of it
 };
-struct First {
-  int64_t token, b, t;
-};
-__device__ __forceinline__ First first_token(const NangilaRotaryParams& p, int64_t token) {
-  const int64_t b = token / p.seq;
-  return {token, b, token - b * p.seq};
-}
-__device__ __forceinline__ Where locate(const NangilaRotaryParams& p, const First& f, uint32_t pair) {
-  const uint32_t all = uint32_t(p.heads[0] + p.heads[1]);
-  const uint32_t ahead = pair / all;
-  int head = int(pair - ahead * all);
-  int64_t b = f.b, t = f.t + ahead;
-  while (t >= p.seq) {  // a CTA's tokens are few
-    t -= p.seq;
-    ++b;
-  }
+__device__ __forceinline__ Where locate(const NangilaRotaryParams& p, int64_t g) {
+  const int64_t all = int64_t(p.heads[0]) + p.heads[1], token = g / all, b = token / p.seq, t = token - b * p.seq;
+  int64_t head = g - token * all;
   Where w;
   w.which = head >= p.heads[0] ? 1 : 0;
   if (w.which) head -= p.heads[0];
   w.in = b * p.stride_b[w.which] + t * p.stride_t[w.which] + head * p.stride_h[w.which];
-  w.out = ((f.token + ahead) * p.heads[w.which] + head) * p.d;
+  w.out = (token * p.heads[w.which] + head) * p.d;
   int64_t pos = t;
   if (p.positions != nullptr) {
     const int64_t at = b * p.pos_stride_b + t * p.pos_stride_t;
@@ -168,7 +155,7 @@ __global__ void __launch_bounds__(kT) rotary_vec_kernel(const __grid_constant__ 
     int head = g - ahead[j] * all;
     which[j] = head >= p.heads[0] ? 1 : 0;
     if (which[j]) head -= p.heads[0];
-    in[j] = static_cast<const T*>(p.in[which[j]]) + head * p.stride_h[which[j]] + col;
+    in[j] = static_cast<const T*>(p.in[which[j]]) + int64_t(head) * p.stride_h[which[j]] + col;
     out[j] = static_cast<T*>(p.out[which[j]]) + int64_t(head) * p.d + col;
     if (g >= pairs) ahead[j] = 0x7fffffff;
   }
@@ -257,9 +244,9 @@ template <typename T>
 __global__ void __launch_bounds__(kT) rotary_any_kernel(const __grid_constant__ NangilaRotaryParams p, int items, int64_t total) {
   const int64_t i = int64_t(blockIdx.x) * kT + threadIdx.x;
   if (i >= total) return;
-  const int64_t g = i / items, token = g / (p.heads[0] + p.heads[1]);
+  const int64_t g = i / items;
   const int item = int(i - g * items), half = p.rot / 2;
-  const Where w = locate(p, first_token(p, token), uint32_t(g - token * (p.heads[0] + p.heads[1])));
+  const Where w = locate(p, g);
   const T* in = static_cast<const T*>(p.in[w.which]) + w.in;
   T* out = static_cast<T*>(p.out[w.which]) + w.out;
   if (item >= half) {

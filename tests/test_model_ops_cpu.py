@@ -261,6 +261,27 @@ def test_muon_optimizer_keeps_its_momentum_in_float32():
     assert len(opt.param_groups) == 1
 
 
+def test_sharded_tensors_are_refused():
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import DeviceMesh
+    from torch.distributed.tensor import DTensor, Replicate
+
+    own = not dist.is_initialized()
+    if own:
+        dist.init_process_group("gloo", rank=0, world_size=1, store=dist.HashStore())
+    try:
+        d = DTensor.from_local(torch.randn(4, 6), DeviceMesh("cpu", [0]), [Replicate()])
+        table = ops.rotary_table(4, 4)
+        for call in (lambda: ops.rms_norm(d, torch.ones(6)), lambda: ops.rotary(d.to_local().view(1, 4, 1, 6), None, DTensor.from_local(table, DeviceMesh("cpu", [0]), [Replicate()])),
+                     lambda: ops.orthogonalize(d), lambda: ops.orthogonalize([d]), lambda: ops.muon_step([d], [torch.randn(4, 6)], [torch.zeros(4, 6)], lr=0.1),
+                     lambda: Muon([torch.nn.Parameter(d)])):
+            with pytest.raises(TypeError, match="nangila"):
+                call()
+    finally:
+        if own:
+            dist.destroy_process_group()
+
+
 # ---- where they are used -------------------------------------------------------------------------------------------------
 
 def test_the_decoder_gives_the_same_with_them():
