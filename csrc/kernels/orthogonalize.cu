@@ -64,7 +64,8 @@ enum Kind { kGram, kPoly, kUpdate, kFinal };
 
 // Warps of the epilogue for each quarter of tensor memory, and slots of each. Two warps with a slot each take turns with a tile's chunks, which ends small tiles
 // sooner; where the results go under the next tile's products anyhow, one warp with two slots disturbs those less (update of 4096 x 16384 376 us, for 397; of sixteen
-// 2048 x 2048 204 us, for 219), but for the last one, which reads and writes parameters (sixteen 2048 x 2048: 409 us with one warp, 250 with two).
+// 2048 x 2048 204 us, for 219), but for the last one, which reads and writes parameters (sixteen 2048 x 2048: 409 us with one warp, 228 with two
+// and the parameters fetched ahead).
 template <int KIND, bool PAIR>
 constexpr int kTurns = PAIR && KIND != kFinal ? 1 : 2;
 template <int KIND, bool PAIR>
@@ -173,15 +174,14 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&v)[4]) {
 }
 // A warp's 32 rows of results in a slot, fp32, taken to the parameters (T) or, with `fresh`, out. Two rows at a time, four columns a lane; the loads of
 // sixteen rows are on their way before the first store.
-template <typename T, bool fresh, bool copies>
+template <typename T, bool fresh>
 __device__ __forceinline__ void put_results(const Product& p, const Target& to_where, T* base, uint8_t* slot, int lane, int row0, int col0) {
   const int x = lane & 15, col = col0 + 4 * x, left = p.N - col;
   if (left <= 0) return;
   // four columns 4 x: group x / 4 of sixteen, its quarter x % 4
   uint8_t* box = slot + ((x & 2) ? kBoxBytes : 0);
   const int j = 2 * (x >> 2) + (x & 1);
-  constexpr int kCopies = copies ? 2 : 1;
-#pragma unroll kCopies
+#pragma unroll 1
   for (int half = 0; half < 32; half += 16) {
     float v[8][4];
     if (!fresh) {
@@ -405,6 +405,15 @@ __device__ __forceinline__ void finish_tile(const Shared& s, uint32_t tmem, cons
     if (KIND != kPoly) tma_load_3d(to + kBoxBytes, lo, at.n0 + c * kChunk, row0, at.batch, bar);
   };
   if (kLoads && turn < mine && lane == 0) fetch(turn, chunks);
+  if constexpr (KIND == kFinal) {
+    // the parameters that this tile is going to change: on their way from memory while its products are made
+    if (target.result == nullptr && row0 + lane < p.M) {
+      const int size = target.param_dtype == NANGILA_F32 ? 4 : 2;
+      const char* at_row = static_cast<const char*>(target.param[at.batch]) + (int64_t(row0 + lane) * p.N + at.n0) * size;
+      for (int c = turn; c < mine; c += kWarps)
+        for (int x = c * kChunk; x < min((c + 1) * kChunk, p.N - at.n0); x += 128 / size) asm volatile("prefetch.global.L2 [%0];" ::"l"(at_row + int64_t(x) * size));
+    }
+  }
   bool ok = *s.failed == 0 && mbar_wait(&s.acc_full[acc], uint32_t((n / 2) & 1), kTimeoutNs);
   ok = __all_sync(0xffffffffu, ok);
   if (!ok) *s.failed = 1;
@@ -452,10 +461,10 @@ __device__ __forceinline__ void finish_tile(const Shared& s, uint32_t tmem, cons
       // the slot is filled by TMA again: what was written here comes first (a fence after the stores to memory below would wait for them)
       fence_async_proxy();
       __syncwarp();
-      if (target.result != nullptr) put_results<__nv_bfloat16, true, PAIR>(p, target, target.result + int64_t(at.batch) * p.M * p.N, slot, lane, row0, col0);
-      else if (target.param_dtype == NANGILA_F32) put_results<float, false, PAIR>(p, target, static_cast<float*>(target.param[at.batch]), slot, lane, row0, col0);
-      else if (target.param_dtype == NANGILA_BF16) put_results<__nv_bfloat16, false, PAIR>(p, target, static_cast<__nv_bfloat16*>(target.param[at.batch]), slot, lane, row0, col0);
-      else put_results<__half, false, PAIR>(p, target, static_cast<__half*>(target.param[at.batch]), slot, lane, row0, col0);
+      if (target.result != nullptr) put_results<__nv_bfloat16, true>(p, target, target.result + int64_t(at.batch) * p.M * p.N, slot, lane, row0, col0);
+      else if (target.param_dtype == NANGILA_F32) put_results<float, false>(p, target, static_cast<float*>(target.param[at.batch]), slot, lane, row0, col0);
+      else if (target.param_dtype == NANGILA_BF16) put_results<__nv_bfloat16, false>(p, target, static_cast<__nv_bfloat16*>(target.param[at.batch]), slot, lane, row0, col0);
+      else put_results<__half, false>(p, target, static_cast<__half*>(target.param[at.batch]), slot, lane, row0, col0);
       __syncwarp();  // all have read the slot
     } else {
       fence_async_proxy();
