@@ -51,7 +51,8 @@ def check_all(x, r, w, dy, dh, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,d", [(1, 1), (1, 8), (3, 7), (5, 33), (1, 2048), (257, 128), (130, 520), (17, 1000), (9, 1001), (1500, 2048), (33, 4096), (6, 5632), (3, 8200),
-                                    (2, 16384), (2, 20000), (1, 32768), (2, 32767)])
+                                    (2, 16384), (2, 20000), (1, 32768), (2, 32767), (3, 6),
+                                    (5, 66), (11, 1004), (7, 1002), (300, 250), (3, 4100), (3, 3001), (2, 6002), (2, 16388), (2, 9999)])
 def test_add_norm_and_gradients(rows, d, dtype):
     x, r, w, g = make(rows, d, dtype)
     dy = torch.randn(rows, d, device="cuda", generator=g).to(dtype)
@@ -127,7 +128,8 @@ def test_only_what_is_wanted_gets_a_gradient():
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,d,group", [(1, 128, 128), (5, 384, 128), (300, 2048, 128), (3, 5632, 128), (2, 32768, 128), (1, 1, None), (7, 33, None), (40, 1000, None),
-                                          (2, 1001, None), (64, 2048, None), (3, 16385, None)])
+                                          (2, 1001, None), (64, 2048, None), (3, 16385, None), (9, 1004, None), (5, 1002, None), (4, 250, None),
+                                          (3, 4099, None), (2, 6002, None)])
 @pytest.mark.parametrize("with_residual", [False, True])
 def test_eight_bits(rows, d, group, dtype, with_residual):
     # q: half a step of e4m3 is 2^-4 of the value, or 2^-10 of the scale among the subnormals; the scale and the value carry fp32's error
