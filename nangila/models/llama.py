@@ -8,7 +8,7 @@ the architecture is defined directly and initialised randomly. Each :class:`Deco
 
 ``LlamaConfig(fused=True)`` takes the norms (with the residual's addition inside a block) and the rotary positions through
 ``nangila.ops``: one kernel each, forward and backward, where PyTorch's operations make several passes. Results agree with the other
-path up to the last rounding. It also opens the positions' options: the half layout, part of the head, scaling for long contexts.
+path up to the last rounding (the benchmark's step on one GPU: 126 -> 90 ms). It also opens the positions' options: the half layout, part of the head, scaling for long contexts.
 """
 from __future__ import annotations
 
