@@ -213,6 +213,17 @@ def test_a_broadcast_input_gets_the_sum_of_its_gradients():
     assert_near(row.grad[0], wx.sum(0), sx.sum(0) * 2 * F32)
 
 
+def test_the_same_tensor_twice():
+    x, _, w, g = make(20, 264, torch.float32)
+    x.requires_grad_()
+    dy = torch.randn(20, 264, device="cuda", generator=g)
+    y, h = ops().add_rms_norm(x, x, w, eps=EPS)
+    assert torch.equal(h, x.detach() * 2)
+    dx, = torch.autograd.grad((y, h), x, (dy, dy))
+    wx, _, sx, _ = plain.norm_grads(h.detach(), w, EPS, dy, dy)
+    assert_near(dx, 2 * wx, rounding(2 * wx, torch.float32) + 2 * sx * F32)
+
+
 def test_nothing_to_do():
     w = torch.ones(16, device="cuda", requires_grad=True)
     x = torch.empty(0, 16, device="cuda", requires_grad=True)

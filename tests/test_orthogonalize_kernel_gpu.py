@@ -35,7 +35,8 @@ def gradient(m, n, seed=0, dtype=torch.float32, fall=0.5):
 
 SIZES = [(1, 1), (1, 7), (7, 1), (2, 3), (8, 8), (16, 64), (63, 65), (65, 63), (64, 64), (128, 128), (129, 127), (100, 1000), (1000, 100), (255, 257), (257, 255), (384, 256), (130, 515),
          (517, 259), (768, 768), (352, 128), (768, 2304), (1024, 640), (200, 4000), (4001, 136), (129, 2100), (128, 384), (385, 128), (40, 3001),
-         (2900, 128), (128, 3073), (17, 769)]
+         (2900, 128), (128, 3073), (17, 769), (1, 65536), (65536, 1), (130, 30000), (30000, 136),
+         (65536, 72)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
