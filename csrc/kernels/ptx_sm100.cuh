@@ -1,7 +1,10 @@
-// Thin inline-PTX wrappers for the Blackwell (sm_100a) data path used by the PowerSGD GEMM kernel:
-// mbarrier, TMA tile loads (cp.async.bulk.tensor, never with cluster multicast), tensor memory
-// allocation, tcgen05.mma / commit / ld, and the shared-memory / instruction descriptors.
+// Thin inline-PTX wrappers for the Blackwell (sm_100a) data path used by the products of PowerSGD and of the orthogonalised updates:
+// mbarrier, TMA tile loads and stores (cp.async.bulk.tensor, never with cluster multicast), pairs and clusters of CTAs, tensor memory
+// allocation, tcgen05.mma / commit / ld / st, and the shared-memory / instruction descriptors.
 // Every wait takes a time limit and reports failure instead of spinning forever.
+//
+// Instructions marked .aligned need all lanes of a warp at once. After a branch that one lane took, nothing but a warp barrier promises that: the cluster's
+// barrier and the tensor memory's allocation, which callers reach from such branches, bring theirs along; tcgen05.ld and st are called behind one.
 #pragma once
 #include <cuda.h>
 #include <cstdint>
@@ -94,6 +97,7 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   return r;
 }
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Where rank 0 of the cluster has what lies at `p` in this CTA.
@@ -136,19 +140,23 @@ __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
 // ---- tensor memory ------------------------------------------------------------------------------------
 // One full warp executes these. `ncols` is a power of two >= 32.
 __device__ __forceinline__ void tmem_alloc(uint32_t* smem_result, uint32_t ncols) {
+  __syncwarp();
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_result)), "r"(ncols)
                : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+  __syncwarp();
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
 // The same for both CTAs of a pair: one warp of each.
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_result, uint32_t ncols) {
+  __syncwarp();
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_result)), "r"(ncols) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  __syncwarp();
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }

@@ -157,9 +157,11 @@ __device__ __forceinline__ void load_weight8(const void* w, int dtype, int v, in
   else load_weight_as<float, TPR, G>(static_cast<const float*>(w), v, t, d, f);
 }
 
-// The threads of a row meet. Rows of a CTA have barriers of their own: one may have a row more to do than the others.
+// The threads of a row meet. Rows of a CTA have barriers of their own: one may have a row more to do than the others. The instruction needs whole warps, and
+// its callers come from a branch that one lane took.
 template <int TPR>
 __device__ __forceinline__ void meet() {
+  __syncwarp();
   asm volatile("bar.sync %0, %1;" ::"r"(1 + int(threadIdx.x) / TPR), "n"(TPR) : "memory");
 }
 // The sum over the threads of a row, in all of them. `s`: TPR / 32 floats of this row, given again only after the row's threads
