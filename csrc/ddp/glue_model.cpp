@@ -1,8 +1,10 @@
 // Bindings of the model and update operators: RMS norm, rotary positions, orthogonalised updates. The checks of arguments are here, for
 // tensors of either device; CPU tensors take the formulas in ATen operations, CUDA tensors the kernels, on the current stream of their device.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -26,13 +28,30 @@ bool known(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == 
 int dtype_code(const Tensor& t) { return t.scalar_type() == at::kFloat ? NANGILA_F32 : t.scalar_type() == at::kHalf ? NANGILA_F16 : NANGILA_BF16; }
 void check_launch(int err, const char* what) { TORCH_CHECK(err == 0, "nangila: ", what, " failed: ", cudaGetErrorString(static_cast<cudaError_t>(err))); }
 void check_plain(const Tensor& t, const char* name) {
-  TORCH_CHECK_TYPE(!t.unsafeGetTensorImpl()->is_python_dispatch(), "nangila: ", name, " must be a plain tensor (a sharded one has to be gathered first)");
+  TORCH_CHECK_TYPE(!t.unsafeGetTensorImpl()->is_python_dispatch(), "nangila: ", name, " must be a plain tensor, not one that wraps another (a sharded one has to be gathered first)");
   TORCH_CHECK_TYPE(t.layout() == at::kStrided, "nangila: ", name, " must be dense");
   TORCH_CHECK_TYPE(t.is_cuda() || t.is_cpu(), "nangila: ", name, " must be on a CUDA device or the CPU");
 }
 void check_tensor(const Tensor& t, const char* name) {
   check_plain(t, name);
   TORCH_CHECK_TYPE(known(t.scalar_type()), "nangila: ", name, " must be float32, float16 or bfloat16, not ", t.scalar_type());
+}
+// The kernels write into fresh memory behind the dispatcher's back. What follows the operations of PyTorch from there (forward-mode derivatives, tracers,
+// tensors that stand for others) would not see them, and go on as if the results were constants: such calls are refused.
+void check_followed(const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(),
+                              "nangila: the kernels have no forward-mode derivative; give them tensors without a tangent (forward_ad.unpack_dual(..).primal), or CPU tensors");
+}
+void check_no_tracer() {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "nangila: the kernels cannot be traced (torch.jit.trace)");
+  for (const TorchDispatchModeKey key : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+    TORCH_CHECK_NOT_IMPLEMENTED(!TorchDispatchModeTLS::get_mode(key).has_value(), "nangila: the kernels cannot be traced (make_fx, export or fake tensors)");
+}
+void check_unseen(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts) check_followed(*t);
+  check_no_tracer();
 }
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
@@ -154,6 +173,7 @@ class RmsNorm : public torch::autograd::Function<RmsNorm> {
     Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
     variable_list out(4);
     if (!dy.defined() && !dh.defined()) return out;
+    check_unseen({&dy, &dh});
     // (asked for by the place among the tensors that were given)
     const bool two = ctx->saved_data["residual"].toBool(), for_x = ctx->needs_input_grad(0), for_residual = two && ctx->needs_input_grad(1);
     const bool want_x = for_x || for_residual, want_w = ctx->needs_input_grad(two ? 2 : 1) && dy.defined();
@@ -206,6 +226,7 @@ Tensor cpu_unit(const Tensor& h, const Tensor& weight, double eps) {
 Tensor rms_norm(const Tensor& x, const Tensor& weight, double eps) {
   check_norm(x, Tensor(), weight, eps);
   if (x.is_cpu()) return cpu_unit(x, weight, eps).to(x.scalar_type());
+  check_unseen({&x, &weight});
   if (!wants_grad({&x, &weight})) return norm_forward(x, Tensor(), weight, eps, false, false, 0).y;
   return RmsNorm::apply(x, c10::optional<Tensor>(), weight, eps)[0];
 }
@@ -215,6 +236,7 @@ std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& residual,
     const Tensor h = x + residual;
     return {cpu_unit(h, weight, eps).to(x.scalar_type()), h};
   }
+  check_unseen({&x, &residual, &weight});
   if (!wants_grad({&x, &residual, &weight})) {
     NormOut o = norm_forward(x, residual, weight, eps, false, false, 0);
     return {o.y, o.h};
@@ -238,6 +260,7 @@ std::tuple<Tensor, Tensor, c10::optional<Tensor>> rms_norm_fp8(const Tensor& x, 
     Tensor q = (f / scale.unsqueeze(-1)).clamp(-448.0, 448.0).to(at::kFloat8_e4m3fn).reshape(shape);
     return {q, scale, residual.defined() ? c10::optional<Tensor>(h) : c10::nullopt};
   }
+  check_unseen({&x, &residual, &weight});
   NormOut o = norm_forward(x, residual, weight, eps, false, true, group);
   return {o.q, o.scale, residual.defined() ? c10::optional<Tensor>(o.h) : c10::nullopt};
 }
@@ -331,6 +354,7 @@ class Rotary : public torch::autograd::Function<Rotary> {
     variable_list out(5);
     Tensor gq = ctx->needs_input_grad(0) ? grads[0] : Tensor(), gk = grads.size() > 1 && ctx->needs_input_grad(1) ? grads[1] : Tensor();
     if (!gq.defined() && !gk.defined()) return out;
+    check_unseen({&gq, &gk});
     std::tie(out[0], out[1]) = rotary_launch(gq, gk, saved[0], saved[1], ctx->saved_data["half"].toBool(), true);
     return out;
   }
@@ -364,7 +388,10 @@ std::tuple<Tensor, c10::optional<Tensor>> rotary(const Tensor& q, const c10::opt
     angles = angles.unsqueeze(-3);
     oq = cpu_turn(q, angles, half);
     if (k.defined()) ok = cpu_turn(k, angles, half);
-  } else if (wants_grad({&q, &k})) {
+    return {oq, k.defined() ? c10::optional<Tensor>(ok) : c10::nullopt};
+  }
+  check_unseen({&q, &k, &table});
+  if (wants_grad({&q, &k})) {
     variable_list o = Rotary::apply(q, k_in, table, positions_in, half);
     oq = o[0];
     if (k.defined()) ok = o[1];
@@ -478,7 +505,14 @@ std::vector<Tensor> chosen(const std::vector<Tensor>& ts, const std::vector<int6
 std::vector<c10::optional<Tensor>> orthogonalize(const std::vector<Tensor>& updates, const std::vector<double>& coefficients, double eps) {
   at::NoGradGuard no_grad;
   check_schedule(coefficients);
-  for (const Tensor& t : updates) check_matrix(t, "updates");
+  bool cuda = false;
+  for (const Tensor& t : updates) {
+    check_matrix(t, "updates");
+    if (!t.is_cuda()) continue;
+    check_followed(t);
+    cuda = true;
+  }
+  if (cuda) check_no_tracer();
   std::vector<c10::optional<Tensor>> out(updates.size());
   for (const auto& g : grouped(updates.size(), [&](size_t i, size_t j) {
          return updates[i].sizes() == updates[j].sizes() && updates[i].scalar_type() == updates[j].scalar_type() && updates[i].device() == updates[j].device();
@@ -497,6 +531,7 @@ std::vector<int64_t> muon_step(const std::vector<Tensor>& params, const std::vec
   check_schedule(coefficients);
   TORCH_CHECK_VALUE(params.size() == grads.size() && params.size() == momenta.size(), "nangila: ", params.size(), " parameters, ", grads.size(), " gradients and ",
                     momenta.size(), " momenta");
+  bool cuda = false;
   for (size_t i = 0; i < params.size(); ++i) {
     const Tensor &p = params[i], &g = grads[i], &m = momenta[i];
     check_matrix(p, "parameters");
@@ -506,7 +541,11 @@ std::vector<int64_t> muon_step(const std::vector<Tensor>& params, const std::vec
                       p.device(), ", its gradient ", g.sizes(), " on ", g.device(), ", its momentum ", m.sizes(), " on ", m.device());
     TORCH_CHECK_TYPE(m.scalar_type() == at::kFloat, "nangila: momenta must be float32, got ", m.scalar_type());
     TORCH_CHECK_VALUE(p.is_contiguous() && m.is_contiguous(), "nangila: parameter ", i, " and its momentum must be packed (contiguous)");
+    if (!p.is_cuda()) continue;
+    for (const Tensor* t : {&p, &g, &m}) check_followed(*t);
+    cuda = true;
   }
+  if (cuda) check_no_tracer();
   std::vector<Tensor> written = params;
   written.insert(written.end(), momenta.begin(), momenta.end());
   TORCH_CHECK_VALUE(!overlapping(written, grads), "nangila: parameters and momenta must not share memory with one another or with the gradients");
