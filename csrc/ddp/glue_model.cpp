@@ -63,9 +63,16 @@ void once_only() {
   TORCH_CHECK(!at::GradMode::is_enabled(), "nangila: this gradient cannot be differentiated again (create_graph=True)");
 }
 
+// The tensor with its values in memory: a view that is negated only when it is read has others there, zeros that nobody has read yet have none.
+Tensor in_memory(const Tensor& t) {
+  if (t._is_zerotensor()) return at::zeros(t.sizes(), t.options());
+  return t.is_neg() ? t.resolve_neg() : t;
+}
+
 // ---- RMS norm --------------------------------------------------------------------------------------------------
 // `t` as rows of d adjacent values, `stride` apart: the tensor itself where its strides allow that, else a packed copy.
-Tensor as_rows(const Tensor& t, int64_t d, int64_t* stride) {
+Tensor as_rows(const Tensor& given, int64_t d, int64_t* stride) {
+  const Tensor t = in_memory(given);
   *stride = d;
   if (t.is_contiguous()) return t;
   if (t.dim() >= 2 && t.stride(-1) == 1) {
@@ -123,7 +130,7 @@ NormOut norm_forward(const Tensor& x_in, const Tensor& residual_in, const Tensor
   if (rows == 0) return o;
   NangilaNormParams p;
   std::memset(&p, 0, sizeof p);
-  Tensor x = as_rows(x_in, d, &p.x_stride), residual = residual_in, weight = weight_in.contiguous();
+  Tensor x = as_rows(x_in, d, &p.x_stride), residual = residual_in, weight = in_memory(weight_in).contiguous();
   if (residual.defined()) residual = as_rows(residual, d, &p.residual_stride);
   if (group) {  // a group's columns are read sixteen bytes at a time
     auto packed = [&](Tensor& t, int64_t* stride) {
@@ -168,7 +175,7 @@ class RmsNorm : public torch::autograd::Function<RmsNorm> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once_only();
     const variable_list saved = ctx->get_saved_variables();
-    Tensor h = saved[0], weight = saved[1].contiguous();
+    Tensor h = saved[0], weight = in_memory(saved[1]).contiguous();
     const Tensor& rstd = saved[2];
     Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
     variable_list out(4);
@@ -294,10 +301,10 @@ void check_rotary(const Tensor& q, const Tensor& k, const Tensor& table, const T
   }
 }
 // one or two tensors turned; an undefined one is left out
-std::tuple<Tensor, Tensor> rotary_launch(const Tensor& q, const Tensor& k, const Tensor& table_in, const Tensor& positions, bool half, bool inverse) {
+std::tuple<Tensor, Tensor> rotary_launch(const Tensor& q, const Tensor& k, const Tensor& table_in, const Tensor& positions_in, bool half, bool inverse) {
   const Tensor& some = q.defined() ? q : k;
   c10::cuda::CUDAGuard guard(some.device());
-  const Tensor table = table_in.contiguous();
+  const Tensor table = in_memory(table_in).contiguous(), positions = positions_in.defined() ? in_memory(positions_in) : positions_in;
   NangilaRotaryParams p;
   std::memset(&p, 0, sizeof p);
   Tensor out[2], in[2];
@@ -307,7 +314,8 @@ std::tuple<Tensor, Tensor> rotary_launch(const Tensor& q, const Tensor& k, const
     if (!t->defined()) continue;
     o = at::empty(t->sizes(), t->options());
     if (t->numel() == 0) continue;
-    in[n] = t->stride(3) == 1 ? *t : t->contiguous();
+    in[n] = in_memory(*t);
+    if (in[n].stride(3) != 1) in[n] = in[n].contiguous();
     p.in[n] = in[n].data_ptr();
     p.out[n] = o.data_ptr();
     p.stride_b[n] = in[n].stride(0);
@@ -498,7 +506,7 @@ std::vector<std::vector<int64_t>> grouped(size_t n, const Same& same) {
 std::vector<Tensor> chosen(const std::vector<Tensor>& ts, const std::vector<int64_t>& which, bool packed = false) {
   std::vector<Tensor> out;
   out.reserve(which.size());
-  for (const int64_t i : which) out.push_back(packed ? ts[i].contiguous() : ts[i]);
+  for (const int64_t i : which) out.push_back(packed ? in_memory(ts[i]).contiguous() : ts[i]);
   return out;
 }
 // Results for the CUDA matrices among the updates; nothing (None) in the place of the others.
@@ -542,6 +550,7 @@ std::vector<int64_t> muon_step(const std::vector<Tensor>& params, const std::vec
     TORCH_CHECK_TYPE(m.scalar_type() == at::kFloat, "nangila: momenta must be float32, got ", m.scalar_type());
     TORCH_CHECK_VALUE(p.is_contiguous() && m.is_contiguous(), "nangila: parameter ", i, " and its momentum must be packed (contiguous)");
     if (!p.is_cuda()) continue;
+    TORCH_CHECK_VALUE(!p.is_neg() && !m.is_neg() && !p._is_zerotensor() && !m._is_zerotensor(), "nangila: parameter ", i, " or its momentum is a view whose values are not in memory");
     for (const Tensor* t : {&p, &g, &m}) check_followed(*t);
     cuda = true;
   }
