@@ -32,6 +32,7 @@ ROOT = Path(__file__).resolve().parent.parent
 PKG = ROOT / "nangila"
 CSRC = ROOT / "csrc"
 OBJ = ROOT / "build"
+RECIPE = Path(__file__).resolve()  # a kernel's flags are part of what it is built from
 EXT_SUFFIX = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
 
 GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -97,6 +98,10 @@ def build_core(force: bool = False) -> Path:
     return out
 
 
+#: Kernels whose float32 results are documented as rounded like PyTorch's: no flushing of subnormal numbers (``--use_fast_math`` implies it).
+KEEP_SUBNORMALS = {"rms_norm", "rotary", "orthogonalize"}
+
+
 def kernel_sources() -> list[Path]:
     return sorted((CSRC / "kernels").glob("*.cu"))
 
@@ -107,11 +112,11 @@ def build_kernels(force: bool = False, verbose_ptxas: bool = False) -> Path:
     if not srcs:
         raise RuntimeError("no kernel sources found")
     hdrs = _headers(CSRC / "kernels", CSRC / "comm")
-    if not force and not _stale(out, srcs + hdrs):
+    if not force and not _stale(out, srcs + hdrs + [RECIPE]):
         return out
     nvcc = str(Path(_cuda_home()) / "bin" / "nvcc")
     OBJ.mkdir(exist_ok=True)
-    flags = [*GENCODE, "-O3", "-std=c++17", "-lineinfo", "--use_fast_math", "-Xcompiler", "-fPIC",
+    flags = [*GENCODE, "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
              "-Xcompiler", "-fvisibility=default", f"-I{CSRC / 'kernels'}", f"-I{CSRC / 'comm'}", f"-I{CSRC}"]
     if verbose_ptxas:
         flags += ["-Xptxas", "-v"]
@@ -120,8 +125,8 @@ def build_kernels(force: bool = False, verbose_ptxas: bool = False) -> Path:
     for s in srcs:
         o = OBJ / (s.stem + ".o")
         objs.append(o)
-        if force or _stale(o, [s] + hdrs):
-            jobs.append([nvcc, *flags, "-c", str(s), "-o", str(o)])
+        if force or _stale(o, [s, RECIPE] + hdrs):
+            jobs.append([nvcc, *flags, *([] if s.stem in KEEP_SUBNORMALS else ["--use_fast_math"]), "-c", str(s), "-o", str(o)])
     with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
         list(ex.map(_run, jobs))
     _run([nvcc, *GENCODE, "-shared", "-Xcompiler", "-fPIC", *map(str, objs), "-o", str(out), "-lcudart", "-lcuda"])
