@@ -43,7 +43,10 @@ def _check_eps(eps: float) -> None:
 def _plain(u: torch.Tensor, flat: List[float], eps: float) -> torch.Tensor:
     """The formula in float32."""
     x = u.float()
-    x = x / torch.linalg.vector_norm(x).clamp(min=eps)
+    # times a power of two that brings the largest value near one: squares of any update then fit into float32
+    by = torch.ldexp(torch.ones((), device=x.device), -torch.frexp(x.abs().amax()).exponent.clamp(-126, 126))
+    x = x * by
+    x = x / torch.maximum(torch.linalg.vector_norm(x), eps * by)
     tall = x.size(0) > x.size(1)
     x = x.mT if tall else x
     for i in range(0, len(flat), 3):
