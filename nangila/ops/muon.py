@@ -35,9 +35,13 @@ def _schedule(steps: int, coefficients: _Coefficients) -> List[float]:
     return flat
 
 
+#: An update of zeros is divided by eps and multiplied by up to 256, in float32.
+MIN_EPS = 1e-36
+
+
 def _check_eps(eps: float) -> None:
-    if not (math.isfinite(eps) and eps > 0):
-        raise ValueError(f"nangila: eps must be positive, got {eps}")
+    if not (math.isfinite(eps) and eps >= MIN_EPS):
+        raise ValueError(f"nangila: eps must be finite and at least {MIN_EPS}, got {eps}")
 
 
 def _plain(u: torch.Tensor, flat: List[float], eps: float) -> torch.Tensor:

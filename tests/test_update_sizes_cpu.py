@@ -4,6 +4,7 @@ import torch
 
 import _model_ops as plain
 from nangila import ops
+from nangila.optim import Muon
 
 COEF = (3.4445, -4.7750, 2.0315)
 # as for other sizes: the bf16 result's 2^-8, and fp32 products of 20 terms carried up by 485 at most
@@ -43,3 +44,20 @@ def test_ordinary_updates_are_what_they_were():
             gram = x @ x.mT
             x = COEF[0] * x + (COEF[1] * gram + COEF[2] * (gram @ gram)) @ x
         assert torch.equal(ops.orthogonalize(u), x.bfloat16())
+
+
+def test_an_eps_that_float32_cannot_divide_by_is_refused():
+    """Zeros over it would not be numbers, and with them the parameters."""
+    z = torch.zeros(6, 8)
+    p = torch.ones(6, 8)
+    for eps in (1e-300, 1e-46, 1e-37, 0.0, -1.0, float("inf"), float("nan")):
+        for call in (lambda: ops.orthogonalize(z, eps=eps), lambda: ops.muon_step([p], [z], [z.clone()], lr=0.1, eps=eps), lambda: Muon([torch.nn.Parameter(p)], eps=eps)):
+            with pytest.raises(ValueError, match="nangila: eps"):
+                call()
+    assert (ops.orthogonalize(z, eps=1e-36) == 0).all() and (p == 1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(6, 8), (200, 65536), (300, 200)])
+def test_zeros_over_the_smallest_eps_on_the_gpu(m, n):
+    assert (ops.orthogonalize(torch.zeros(m, n, device="cuda"), eps=1e-36) == 0).all()
