@@ -12,7 +12,7 @@ path up to the last rounding (the benchmark's step on one GPU: 126 -> 90 ms). It
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from typing import Optional, Union
 
 import torch
@@ -41,8 +41,21 @@ class LlamaConfig:
     rope_original_seq: Optional[int] = None
 
     def __post_init__(self):
-        if not self.fused and (self.rope_layout, self.rope_dim, self.rope_scaling) != ("interleaved", None, None):
-            raise ValueError("nangila: rope_layout, rope_dim and rope_scaling need fused=True")
+        self.check()
+
+    def check(self) -> None:
+        """Refuses options that would have no effect. Models and blocks check again what they are built from, for fields can be set in between."""
+        if not self.fused and (self.rope_layout, self.rope_dim, self.rope_scaling, self.rope_factor, self.rope_original_seq) != ("interleaved", None, None, 1.0, None):
+            raise ValueError("nangila: rope_layout, rope_dim, rope_scaling, rope_factor and rope_original_seq need fused=True")
+        if self.rope_scaling is None and self.rope_factor != 1.0:
+            raise ValueError("nangila: rope_factor needs a rope_scaling")
+        if self.rope_scaling != "yarn" and self.rope_original_seq is not None:
+            raise ValueError("nangila: rope_original_seq needs rope_scaling='yarn'")
+        if self.rope_layout not in ops.positions.LAYOUTS:
+            raise ValueError(f"nangila: rope_layout must be one of {ops.positions.LAYOUTS}, got {self.rope_layout!r}")
+        head_dim = self.d_model // self.n_head
+        if self.rope_dim is not None and not (2 <= self.rope_dim <= head_dim and self.rope_dim % 2 == 0):
+            raise ValueError(f"nangila: rope_dim must be even and 2 to {head_dim} (a head's columns), got {self.rope_dim}")
 
     @staticmethod
     def llama_1_3b() -> "LlamaConfig":
@@ -88,6 +101,7 @@ class Angles:
 class DecoderBlock(nn.Module):
     def __init__(self, cfg: LlamaConfig):
         super().__init__()
+        cfg.check()
         self.h, self.kv = cfg.n_head, cfg.n_kv_head
         self.hd = cfg.d_model // cfg.n_head
         self.fused, self.layout = cfg.fused, cfg.rope_layout
@@ -129,7 +143,7 @@ class DecoderBlock(nn.Module):
 class Llama(nn.Module):
     def __init__(self, cfg: LlamaConfig):
         super().__init__()
-        self.cfg = cfg
+        self.cfg = cfg = replace(cfg)  # checked; what is set in the caller's later does not change a model that is built
         self.embed = nn.Embedding(cfg.vocab_size, cfg.d_model)
         self.blocks = nn.ModuleList([DecoderBlock(cfg) for _ in range(cfg.n_layer)])
         self.norm = RMSNorm(cfg.d_model, cfg.eps)
@@ -159,7 +173,7 @@ class Llama(nn.Module):
         head_dim = cfg.d_model // cfg.n_head
         if not cfg.fused:
             return rope_table(seq, head_dim, cfg.rope_theta, device)
-        return ops.rotary_table(seq, cfg.rope_dim or head_dim, cfg.rope_theta, device, scaling=cfg.rope_scaling, factor=cfg.rope_factor,
+        return ops.rotary_table(seq, head_dim if cfg.rope_dim is None else cfg.rope_dim, cfg.rope_theta, device, scaling=cfg.rope_scaling, factor=cfg.rope_factor,
                                 original_seq=cfg.rope_original_seq)
 
     def num_params(self) -> int:
