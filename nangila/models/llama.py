@@ -156,7 +156,8 @@ class Llama(nn.Module):
     def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None):
         t = idx.size(1)
         if self._rope is None or self._rope.device != idx.device or self._rope.size(0) < t:
-            self._rope = self._table(max(t, self.cfg.max_seq), idx.device)
+            with torch.inference_mode(False):  # (a table made by an evaluation serves the training that follows)
+                self._rope = self._table(max(t, self.cfg.max_seq), idx.device)
         x = self.embed(idx)
         rope = Angles(self._rope) if self.cfg.fused else self._rope
         for blk in self.blocks:

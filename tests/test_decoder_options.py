@@ -51,3 +51,25 @@ def test_all_columns_can_be_named():
         m = Llama(LlamaConfig(**SMALL, fused=True, rope_dim=dim))
         m(torch.randint(0, 64, (1, 12)))
         assert m._rope.shape[1] == (dim or 16) // 2
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_training_after_an_evaluation_in_inference_mode(fused):
+    m = Llama(LlamaConfig(**SMALL, fused=fused))
+    idx = torch.randint(0, 64, (1, 12))
+    with torch.inference_mode():
+        want = m(idx)
+    out = m(idx)
+    out.sum().backward()
+    assert torch.equal(out, want) and all(p.grad is not None for p in m.parameters())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fused", [False, True])
+def test_training_after_an_evaluation_in_inference_mode_on_the_gpu(fused):
+    m = Llama(LlamaConfig(**SMALL, fused=fused)).cuda()
+    idx = torch.randint(0, 64, (1, 12), device="cuda")
+    with torch.inference_mode():
+        m(idx)
+    m(idx).sum().backward()
+    assert all(torch.isfinite(p.grad).all() for p in m.parameters())
