@@ -153,7 +153,7 @@ def build_llama(args, dev, world):
             "unit": "tokens/s", "items_per_step": b * t * world, "global_batch": b * world, "seq_len": t,
             "parallelism": f"fsdp{world} (fully_shard per block)",
             "compressor": "block-INT4 reduce-scatter + INT8 all-gather (fused kernels)" if colls else "stock FSDP2 (NCCL)",
-            "optimizer": "AdamW(fused)"}
+            "optimizer": "AdamW(fused)", "fused": args.fused}
     return model, opt, (_Hook() if colls else None), host, put, loss_fn, info
 
 
@@ -172,6 +172,8 @@ def main() -> int:
     ap.add_argument("--fused", action="store_true", help="Llama configuration: norms and rotary positions through nangila.ops (either arm)")
     ap.add_argument("--bucket-mb", type=int, default=25, help="DDP bucket size of the BERT configuration")
     args = ap.parse_args()
+    if args.fused and args.config != "llama-1.3b-fsdp":
+        ap.error("--fused is an option of llama-1.3b-fsdp")
     args.warmup = max(args.warmup, 3)
     rank, world, dev = init_distributed()
     if world != args.gpus:
