@@ -399,6 +399,8 @@ std::tuple<Tensor, c10::optional<Tensor>> rotary(const Tensor& q, const c10::opt
     return {oq, k.defined() ? c10::optional<Tensor>(ok) : c10::nullopt};
   }
   check_unseen({&q, &k, &table});
+  for (const Tensor* t : {&q, &k})
+    TORCH_CHECK_VALUE(!t->defined() || t->size(2) <= (int64_t(1) << 30), "nangila: the kernels take up to 2^30 heads, got ", t->sizes());
   if (wants_grad({&q, &k})) {
     variable_list o = Rotary::apply(q, k_in, table, positions_in, half);
     oq = o[0];
