@@ -46,6 +46,7 @@ void check_no_tracer() {
   using c10::impl::TorchDispatchModeKey;
   using c10::impl::TorchDispatchModeTLS;
   TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "nangila: the kernels cannot be traced (torch.jit.trace)");
+  if (!TorchDispatchModeTLS::any_modes_set()) return;
   for (const TorchDispatchModeKey key : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
     TORCH_CHECK_NOT_IMPLEMENTED(!TorchDispatchModeTLS::get_mode(key).has_value(), "nangila: the kernels cannot be traced (make_fx, export or fake tensors)");
 }
