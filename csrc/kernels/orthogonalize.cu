@@ -1359,7 +1359,9 @@ int product(const Matrix& a, const Matrix& b, const Matrix* in, const Matrix* lo
   ok = ok && make_map(&maps.out, out != nullptr ? *out : a, count, kChunk, 32) && make_map(&maps.mirror, out != nullptr ? *out : a, count, 32, kChunk, false);
   if (!ok) return int(cudaErrorNotSupported);
   // A tile of a pair takes hardly longer than a small one, which is bound by what L2 delivers to an SM (twice the bytes for each product); only its
-  // epilogue is longer. So it is the number of rounds that decides.
+  // epilogue is longer. So it is the number of rounds that decides. Measured, all products of five steps with small tiles, and with those of pairs: as many rounds of either, 768 x 768 157 us and
+  // 202, thirty of 384 x 300 195 and 237; two rounds or one, eight of 768 x 768 250 and 220; three and seven or two and four, twenty of 700 x 900 506 and 464; two and three or one and two,
+  // 2305 x 2177 651 and 481. Each product by its rounds, 2048 x 2048: 322, 316, and 288 so.
   const int sms = sm_count();
   const int64_t small = tiles_of(p, 128, count), large = tiles_of(p, 256, count);
   if constexpr (KIND == kGram) {

@@ -55,7 +55,8 @@ __device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
   b = y;
 }
 
-// A division of numbers below 2^31 by one that the host knows.
+// A division of numbers below 2^31 by one that the host knows: a multiplication by its reciprocal, rounded up to 33 bits, of which the leading one is added apart
+// (T. Granlund and P. Montgomery, Division by invariant integers using multiplication, 1994).
 struct Divisor {
   uint32_t by, magic, shift;
 };

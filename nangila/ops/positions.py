@@ -1,4 +1,8 @@
-"""Rotary positions (``csrc/kernels/rotary.cu``): pairs of columns of q and k turned by the angles of their positions."""
+"""Rotary positions (``csrc/kernels/rotary.cu``): pairs of columns of q and k turned by the angles of their positions (J. Su and others, 2021).
+
+The scalings for long contexts are published ones: positions divided (S. Chen and others, 2023), theta raised, and a blend of both by the pair's speed (B. Peng and
+others, 2023), with their constants as defaults.
+"""
 from __future__ import annotations
 
 import math
