@@ -166,6 +166,7 @@ std::string error_string(int code) { return cudaGetErrorString(static_cast<cudaE
 void register_more(py::module_& m);
 void register_ddp_hook(py::module_& m);  // ddp_hook.cpp
 void register_model(py::module_& m);     // glue_model.cpp
+void register_vocab(py::module_& m);     // glue_vocab.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "nangila torch glue over the sm_100a kernels";
@@ -187,4 +188,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_more(m);
   register_ddp_hook(m);
   register_model(m);
+  register_vocab(m);
 }

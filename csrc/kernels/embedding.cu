@@ -1,0 +1,439 @@
+// Token embeddings: out[i] = scale * weight[ids[i]], and the table's gradient dw[v] = scale * sum of dy[i] over ids[i] = v.
+//
+// The gradient goes by sorted tokens, so that every sum has a fixed order and no atomics decide it:
+//   1. a cluster of eight CTAs sorts the positions by id (radix sort, least significant digit first, stable), while all other CTAs fill the gradient with zeros, which is
+//      most of what is written: a batch has far fewer tokens than the table has rows;
+//   2. the sorted positions are cut into pieces of a few dozen, and each piece adds up its runs of equal ids, in fp32; a run that lies in one piece is
+//      a finished row, one that goes on in the next leaves partial sums;
+//   3. the partial sums of each run that crosses pieces are added up. A token that fills half the batch is spread over all SMs that way.
+// Ids outside the table and the padding id sort behind all others and are left out.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "follow.cuh"
+#include "launch_util.cuh"
+#include "nangila_kernels.h"
+#include "nangila_vocab_kernels.h"
+#include "ptx_sm100.cuh"
+#include "quant.cuh"
+#include "raw8.cuh"
+
+namespace nangila {
+namespace {
+
+__device__ __forceinline__ int64_t id_at(const void* ids, int ids_64, int64_t i) {
+  return ids_64 ? static_cast<const int64_t*>(ids)[i] : int64_t(static_cast<const int32_t*>(ids)[i]);
+}
+
+// ---- lookup ------------------------------------------------------------------------------------------------------
+constexpr int kLookupT = 256;
+constexpr int kLookupAtOnce = 4;  // vectors of a lane on their way together
+
+// A warp for each token.
+template <typename T, bool VECTOR>
+__global__ void __launch_bounds__(kLookupT) embedding_kernel(const __grid_constant__ NangilaEmbeddingParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = int64_t(gridDim.x) * (kLookupT / 32);
+  for (int64_t i = int64_t(blockIdx.x) * (kLookupT / 32) + (threadIdx.x >> 5); i < p.n; i += warps) {
+    const int64_t id = id_at(p.ids, p.ids_64, i);
+    const bool inside = id >= 0 && id < p.rows;
+    const T* from = static_cast<const T*>(p.weight) + (inside ? id : 0) * p.weight_stride;
+    T* to = static_cast<T*>(p.out) + i * p.d;
+    if (VECTOR) {
+      for (int c = lane * 8; c < p.d; c += 256 * kLookupAtOnce) {
+        dev::Raw8<T> raw[kLookupAtOnce];
+#pragma unroll
+        for (int k = 0; k < kLookupAtOnce; ++k)
+          if (c + 256 * k < p.d) dev::fetch(from + c + 256 * k, raw[k]);
+#pragma unroll
+        for (int k = 0; k < kLookupAtOnce; ++k) {
+          if (c + 256 * k >= p.d) continue;
+          float v[8];
+          dev::unpack(raw[k], v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = inside ? v[e] * p.scale : __uint_as_float(0x7fc00000u);
+          dev::pack(v, raw[k]);
+          dev::put(to + c + 256 * k, raw[k]);
+        }
+      }
+    } else {
+      for (int c = lane; c < p.d; c += 32) to[c] = dev::Vec16<T>::from_float(inside ? dev::Vec16<T>::to_float(from[c]) * p.scale : __uint_as_float(0x7fc00000u));
+    }
+  }
+}
+
+// ---- gradient ----------------------------------------------------------------------------------------------------
+constexpr int kSortT = 1024;
+constexpr int kSortCtas = 8;       // one cluster
+constexpr int kSortWarps = kSortCtas * kSortT / 32;
+constexpr int kMaxDigit = 10;      // bits
+constexpr int kSortSmem = ((kSortT / 32) + 1) * (4 << kMaxDigit) + 256;
+constexpr int kSumT = 256;
+constexpr int kSumAtOnce = 8;      // rows on their way together
+constexpr int kJoinT = 512;
+
+struct Sorted {
+  uint32_t *key[2], *at[2];        // ids and positions, there and back
+  uint32_t* crossing;              // [0]: how many; from [1] on: pieces in which a run begins that goes on behind them
+  float* partial;                  // [2 * pieces][pitch]
+  int passes, digit;               // bits of a digit
+  int last;                        // which of the two buffers the sorted ones are in
+  int per_warp;                    // positions of a warp of the sort, a multiple of 32
+  int piece, pieces, pitch;
+};
+
+__device__ __forceinline__ uint32_t load_cluster(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+
+__global__ void __launch_bounds__(kSortT, 1) embedding_sort_kernel(const __grid_constant__ NangilaEmbeddingGradParams p, const __grid_constant__ Sorted s) {
+  if (blockIdx.x >= kSortCtas) {  // zeros
+    uint4* to = static_cast<uint4*>(p.dw);
+    const int64_t bytes = p.rows * p.d * (p.dtype == NANGILA_F32 ? 4 : 2), words = bytes / 16;
+    const int64_t step = int64_t(gridDim.x - kSortCtas) * kSortT;
+    const int64_t first = int64_t(blockIdx.x - kSortCtas) * kSortT + threadIdx.x;
+    for (int64_t i = first; i < words; i += step) to[i] = make_uint4(0, 0, 0, 0);
+    if (first < (bytes & 15)) static_cast<uint8_t*>(p.dw)[words * 16 + first] = 0;
+    return;
+  }
+  extern __shared__ uint32_t smem[];
+  uint32_t* count = smem;                                       // [warp][digit]
+  uint32_t* total = count + (kSortT / 32) * (1 << kMaxDigit);   // of this CTA's positions, by digit
+  uint32_t* scan = total + (1 << kMaxDigit);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, digits = 1 << s.digit;
+  const uint32_t rank = blockIdx.x;
+  const int64_t from = int64_t(int(rank) * (kSortT / 32) + warp) * s.per_warp, to = min(p.n, from + s.per_warp);
+  if (rank == 0 && threadIdx.x == 0) s.crossing[0] = 0;
+  for (int pass = 0; pass < s.passes; ++pass) {
+    const uint32_t *src_key = s.key[(pass + 1) & 1], *src_at = s.at[(pass + 1) & 1];
+    uint32_t *dst_key = s.key[pass & 1], *dst_at = s.at[pass & 1];
+    const int shift = pass * s.digit;
+    auto key_of = [&](int64_t i) -> uint32_t {
+      if (pass > 0) return __ldcg(src_key + i);
+      const int64_t id = id_at(p.ids, p.ids_64, i);
+      return id >= 0 && id < p.rows && id != p.padding ? uint32_t(id) : uint32_t(p.rows);
+    };
+    for (int i = threadIdx.x; i < (kSortT / 32) * digits; i += kSortT) count[i] = 0;
+    __syncthreads();
+    uint32_t* mine = count + warp * digits;
+    for (int64_t i = from + lane; i < to; i += 32) atomicAdd(&mine[key_of(i) >> shift & uint32_t(digits - 1)], 1u);
+    __syncthreads();
+    // where each (digit, CTA, warp) begins: before it come all smaller digits, and this digit's positions of the CTAs and warps before
+    const int d = threadIdx.x;
+    if (d < digits) {
+      uint32_t run = 0;
+#pragma unroll 8
+      for (int w = 0; w < kSortT / 32; ++w) {
+        const uint32_t t = count[w * digits + d];
+        count[w * digits + d] = run;
+        run += t;
+      }
+      total[d] = run;
+    }
+    sm100::cluster_sync();
+    uint32_t before = 0, all = 0;
+    if (d < digits) {
+#pragma unroll
+      for (uint32_t q = 0; q < kSortCtas; ++q) {
+        const uint32_t v = load_cluster(sm100::cluster_address(total + d, q));
+        all += v;
+        before += q < rank ? v : 0u;
+      }
+    }
+    uint32_t sum = all;  // up to this digit, in the warp
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, sum, off);
+      if (lane >= off) sum += v;
+    }
+    if (lane == 31) scan[warp] = sum;
+    __syncthreads();
+    if (d < digits) {
+      for (int w = 0; w < warp; ++w) before += scan[w];
+      before += sum - all;
+#pragma unroll 8
+      for (int w = 0; w < kSortT / 32; ++w) count[w * digits + d] += before;
+    }
+    __syncthreads();
+    for (int64_t i0 = from; i0 < to; i0 += 32) {
+      const int64_t i = i0 + lane;
+      const bool here = i < to;
+      const uint32_t k = here ? key_of(i) : 0u, a = here ? (pass > 0 ? __ldcg(src_at + i) : uint32_t(i)) : 0u;
+      const uint32_t digit = here ? k >> shift & uint32_t(digits - 1) : uint32_t(digits);  // (those that are not here keep to themselves)
+      const uint32_t same = __match_any_sync(0xffffffffu, digit);
+      const uint32_t order = __popc(same & ((1u << lane) - 1u));
+      uint32_t pos = 0;
+      if (here) pos = mine[digit] + order;
+      __syncwarp();
+      if (here && order == 0) mine[digit] += __popc(same);
+      __syncwarp();
+      if (here) {
+        dst_key[pos] = k;
+        dst_at[pos] = a;
+      }
+    }
+    sm100::cluster_sync();  // what one CTA has written, all read in the next pass
+  }
+}
+
+// A thread takes VECTOR ? 8 : 1 adjacent columns of a piece; threadIdx.y: the piece of the CTA's.
+template <typename T, bool VECTOR>
+__global__ void __launch_bounds__(kSumT) embedding_sum_kernel(const __grid_constant__ NangilaEmbeddingGradParams p, const __grid_constant__ Sorted s) {
+  constexpr int W = VECTOR ? 8 : 1;
+  const int piece = blockIdx.x * blockDim.y + threadIdx.y, col = (blockIdx.y * blockDim.x + threadIdx.x) * W;
+  follow();
+  if (piece >= s.pieces || col >= p.d) return;
+  const uint32_t *key = s.key[s.last], *at = s.at[s.last];
+  const int64_t s0 = int64_t(piece) * s.piece, s1 = min(p.n, s0 + s.piece);
+  const T* dy = static_cast<const T*>(p.dy) + col;
+  uint32_t current = key[s0];
+  bool before = s0 > 0 && key[s0 - 1] == current;
+  float acc[W];
+#pragma unroll
+  for (int k = 0; k < W; ++k) acc[k] = 0.0f;
+  auto finish = [&](bool goes_on) {
+    if (current >= uint32_t(p.rows)) return;
+    if (!before && !goes_on) {
+      T* to = static_cast<T*>(p.dw) + int64_t(current) * p.d + col;
+      if constexpr (VECTOR) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = acc[k] * p.scale;
+        dev::Raw8<T> raw;
+        dev::pack(v, raw);
+        dev::put(to, raw);
+      } else {
+        *to = dev::Vec16<T>::from_float(acc[0] * p.scale);
+      }
+    } else {
+      float* to = s.partial + (int64_t(2) * piece + (before ? 0 : 1)) * s.pitch + col;
+      if constexpr (VECTOR) {
+        reinterpret_cast<float4*>(to)[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        reinterpret_cast<float4*>(to)[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      } else {
+        *to = acc[0];
+      }
+      if (!before && col == 0) s.crossing[1 + atomicAdd(s.crossing, 1u)] = uint32_t(piece);  // (in any order: each is summed by itself)
+    }
+  };
+  for (int64_t i0 = s0; i0 < s1; i0 += kSumAtOnce) {
+    uint32_t k[kSumAtOnce];
+    dev::Raw8<T> raw[VECTOR ? kSumAtOnce : 1];
+    T one[VECTOR ? 1 : kSumAtOnce];
+#pragma unroll
+    for (int j = 0; j < kSumAtOnce; ++j) {
+      k[j] = i0 + j < s1 ? key[i0 + j] : uint32_t(p.rows);
+      if (k[j] >= uint32_t(p.rows)) continue;
+      const T* row = dy + int64_t(at[i0 + j]) * p.dy_stride;
+      if constexpr (VECTOR) dev::fetch(row, raw[j]);
+      else one[j] = *row;
+    }
+#pragma unroll
+    for (int j = 0; j < kSumAtOnce; ++j) {
+      if (i0 + j >= s1) break;
+      if (k[j] != current) {
+        finish(false);
+        current = k[j];
+        before = false;
+#pragma unroll
+        for (int c = 0; c < W; ++c) acc[c] = 0.0f;
+      }
+      if (current >= uint32_t(p.rows)) return;  // nothing but what is left out from here on
+      if constexpr (VECTOR) {
+        float v[8];
+        dev::unpack(raw[j], v);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc[c] += v[c];
+      } else {
+        acc[0] += dev::Vec16<T>::to_float(one[j]);
+      }
+    }
+  }
+  finish(s1 < p.n && key[s1] == current);
+}
+
+// 128 columns of a run that crosses pieces: sixteen groups of warps' lanes take every sixteenth partial sum, and are added up in order.
+template <typename T>
+__global__ void __launch_bounds__(kJoinT) embedding_join_kernel(const __grid_constant__ NangilaEmbeddingGradParams p, const __grid_constant__ Sorted s) {
+  constexpr int kGroups = kJoinT / 32;
+  __shared__ float4 part[kGroups][32];
+  follow();
+  const uint32_t* key = s.key[s.last];
+  const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
+  const int blocks = (p.d + 127) / 128;
+  const int64_t tasks = int64_t(s.crossing[0]) * blocks;
+  for (int64_t task = blockIdx.x; task < tasks; task += gridDim.x) {
+    const int64_t first = s.crossing[1 + task / blocks];
+    const int col = int(task % blocks) * 128 + lane * 4;
+    const uint32_t id = key[(first + 1) * s.piece];
+    // the last position with this id
+    int64_t lo = (first + 1) * s.piece, hi = p.n;
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) / 2;
+      if (key[mid] == id) lo = mid;
+      else hi = mid;
+    }
+    const int64_t count = lo / s.piece - first;  // pieces behind the first
+    float4 sum = make_float4(0, 0, 0, 0);
+    if (col < p.d) {
+#pragma unroll 4
+      for (int64_t j = group; j <= count; j += kGroups) {
+        const float4 v = *reinterpret_cast<const float4*>(s.partial + (2 * (first + j) + (j == 0 ? 1 : 0)) * s.pitch + col);
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
+      }
+    }
+    part[group][lane] = sum;
+    __syncthreads();
+    if (group == 0) {
+      for (int g = 1; g < kGroups; ++g) {
+        const float4 v = part[g][lane];
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
+      }
+      const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+      T* to = static_cast<T*>(p.dw) + int64_t(id) * p.d + col;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (col + k < p.d) to[k] = dev::Vec16<T>::from_float(v[k] * p.scale);
+    }
+    __syncthreads();
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <typename T>
+int lookup(const NangilaEmbeddingParams& p, cudaStream_t stream) {
+  const bool vector = p.d % 8 == 0 && aligned16(p.weight) && aligned16(p.out) && p.weight_stride * int64_t(sizeof(T)) % 16 == 0;
+  auto* kernel = vector ? embedding_kernel<T, true> : embedding_kernel<T, false>;
+  int resident = 0;
+  if (const cudaError_t e = resident_ctas(reinterpret_cast<const void*>(kernel), kLookupT, 0, &resident)) return int(e);
+  const int64_t want = (p.n + kLookupT / 32 - 1) / (kLookupT / 32);
+  kernel<<<unsigned(std::min<int64_t>(want, resident)), kLookupT, 0, stream>>>(p);
+  return int(cudaGetLastError());
+}
+
+// How the work on n positions is cut up, and where it lies in the workspace.
+Sorted layout(int64_t n, int64_t rows, int32_t d, uint8_t* base, int64_t* bytes) {
+  Sorted s;
+  int64_t used = 0;
+  auto take = [&](int64_t size) {
+    uint8_t* at = base + used;
+    used += (size + 255) / 256 * 256;
+    return at;
+  };
+  for (int i = 0; i < 2; ++i) {
+    s.key[i] = reinterpret_cast<uint32_t*>(take(n * 4));
+    s.at[i] = reinterpret_cast<uint32_t*>(take(n * 4));
+  }
+  int bits = 1;
+  while (rows >> bits) ++bits;  // keys 0 .. rows
+  s.passes = (bits + kMaxDigit - 1) / kMaxDigit;
+  s.digit = (bits + s.passes - 1) / s.passes;
+  s.last = (s.passes - 1) & 1;
+  s.per_warp = int(((n + kSortWarps - 1) / kSortWarps + 31) / 32 * 32);
+  // pieces: some hundreds of them if there are positions enough, and no shorter than what a thread has on its way at a time
+  s.piece = 8;
+  while (s.piece < 64 && n > int64_t(s.piece) * 512) s.piece *= 2;
+  s.pieces = int((n + s.piece - 1) / s.piece);
+  s.pitch = (d + 7) / 8 * 8;
+  s.crossing = reinterpret_cast<uint32_t*>(take((int64_t(s.pieces) + 1) * 4));
+  s.partial = reinterpret_cast<float*>(take(int64_t(2) * s.pieces * s.pitch * 4));
+  *bytes = used;
+  return s;
+}
+
+template <typename T>
+int gradient(const NangilaEmbeddingGradParams& p, cudaStream_t stream) {
+  int64_t bytes = 0;
+  const Sorted s = layout(p.n, p.rows, p.d, static_cast<uint8_t*>(p.workspace), &bytes);
+  int resident = 0;
+  if (const cudaError_t e = resident_ctas(reinterpret_cast<const void*>(embedding_sort_kernel), kSortT, kSortSmem, &resident)) return int(e);
+  const int64_t words = p.rows * p.d * int64_t(sizeof(T)) / 16;
+  const int zero_clusters = int(std::max<int64_t>(1, std::min<int64_t>(resident / kSortCtas - 1, (words + kSortT * kSortCtas - 1) / (kSortT * kSortCtas))));
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kSortCtas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(kSortCtas * (1 + zero_clusters)));
+  cfg.blockDim = dim3(kSortT);
+  cfg.dynamicSmemBytes = kSortSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (const cudaError_t e = cudaLaunchKernelEx(&cfg, embedding_sort_kernel, p, s)) return int(e);
+  const bool vector = p.d % 8 == 0 && aligned16(p.dy) && aligned16(p.dw) && p.dy_stride * int64_t(sizeof(T)) % 16 == 0;
+  const int threads = vector ? p.d / 8 : p.d;
+  int x = 32;
+  while (x < kSumT && x < threads) x *= 2;
+  const int y = kSumT / x;
+  auto* sum = vector ? embedding_sum_kernel<T, true> : embedding_sum_kernel<T, false>;
+  cfg = {};
+  cudaLaunchAttribute next[1];
+  next[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  next[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(unsigned((s.pieces + y - 1) / y), unsigned((threads + x - 1) / x));
+  cfg.blockDim = dim3(unsigned(x), unsigned(y));
+  cfg.stream = stream;
+  cfg.attrs = next;
+  cfg.numAttrs = 1;
+  if (const cudaError_t e = cudaLaunchKernelEx(&cfg, sum, p, s)) return int(e);
+  if (s.pieces < 2) return 0;
+  const int64_t tasks = int64_t(s.pieces - 1) * ((p.d + 127) / 128);
+  return int(launch_following(embedding_join_kernel<T>, dim3(unsigned(std::min<int64_t>(tasks, 2 * 148))), kJoinT, 0, stream, p, s));
+}
+
+}  // namespace
+}  // namespace nangila
+
+extern "C" int nangila_embedding(const NangilaEmbeddingParams* p, cudaStream_t stream) {
+  using namespace nangila;
+  if (!p || !p->ids || !p->weight || !p->out || p->n < 0 || p->rows < 1 || p->d < 1) return int(cudaErrorInvalidValue);
+  if (p->n == 0) return 0;
+  try {
+    switch (p->dtype) {
+      case NANGILA_F32: return lookup<float>(*p, stream);
+      case NANGILA_F16: return lookup<__half>(*p, stream);
+      case NANGILA_BF16: return lookup<__nv_bfloat16>(*p, stream);
+      default: return int(cudaErrorInvalidValue);
+    }
+  } catch (...) {  // (the host's tables of kernels that were set up allocate)
+    return int(cudaErrorMemoryAllocation);
+  }
+}
+
+extern "C" int64_t nangila_embedding_workspace(int64_t n, int64_t rows, int32_t d) {
+  int64_t bytes = 0;
+  nangila::layout(n, rows, d, nullptr, &bytes);
+  return bytes;
+}
+
+extern "C" int nangila_embedding_backward(const NangilaEmbeddingGradParams* p, cudaStream_t stream) {
+  using namespace nangila;
+  if (!p || !p->ids || !p->dy || !p->dw || !p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255u) || p->n < 1 || p->n > NANGILA_EMBEDDING_MAX_TOKENS || p->rows < 1 ||
+      p->rows > NANGILA_EMBEDDING_MAX_ROWS || p->d < 1)
+    return int(cudaErrorInvalidValue);
+  try {
+    switch (p->dtype) {
+      case NANGILA_F32: return gradient<float>(*p, stream);
+      case NANGILA_F16: return gradient<__half>(*p, stream);
+      case NANGILA_BF16: return gradient<__nv_bfloat16>(*p, stream);
+      default: return int(cudaErrorInvalidValue);
+    }
+  } catch (...) {
+    return int(cudaErrorMemoryAllocation);
+  }
+}

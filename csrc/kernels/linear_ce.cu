@@ -1,0 +1,1095 @@
+// The loss of a language model's head without its logits: z = x w^T + b, loss_i = log sum_v exp(z_iv) - z_it, and the gradients of x, w, b (sm_100a).
+//
+// Losses alone: the tiles of z stay in tensor memory. Their epilogue takes each row's largest value and the sum of its exponentials over 128 classes, and those
+// are all that is written; a last kernel joins them to lse and loss. The target's own logit is a dot product in fp32 by itself and is left out of the sums:
+// loss = log(1 + sum over the others of exp(z_v - z_t)) keeps its digits where the model is sure.
+//
+// Gradients need G = exp(z - lse) - [v = t] twice: dx = G w and dw = G^T x. A group of tokens at a time (as many as fit into half a gigabyte of 16-bit values) the tiles' epilogue
+// writes exponentials E, and two products read them. The exponent's reference need not be lse, which is known only when the whole row is: in bf16, whose range is that of
+// fp32, E = exp(z - z_t) is as good. Its row sums give lse, and the factor f = exp(z_t - lse) of each row is applied to the rows of dx, and to those of x
+// on their way into dw. So the losses and the gradients take three products (6 n d V operations), where logits that are formed again for the gradients take four. A row in which some z is above z_t by more than
+// 60 (exp(60) = 1e26) is formed again with its largest value as the reference. fp16 has no such range, and gradients weighted row by row need their weights: there the
+// losses come first, and the gradients form z again with lse as the reference.
+//
+// Roundings: products of 16-bit operands, summed in fp32; E once to the type of x (with fp16 as 2^15 exp(z - lse), which keeps 11 bits down to 2^-29); f x once;
+// results once. The target's element of E is minus the sum of all others, in fp32, before its rounding: no 1 - p where p is near one.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <cstring>
+#include <mutex>
+#include <set>
+#include <utility>
+
+#include "follow.cuh"
+#include "launch_util.cuh"
+#include "nangila_kernels.h"
+#include "nangila_vocab_kernels.h"
+#include "ptx_sm100.cuh"
+#include "quant.cuh"
+#include "raw8.cuh"
+
+namespace nangila {
+namespace {
+
+using namespace sm100;
+
+constexpr int kTileM = 128;                      // rows of a CTA
+constexpr int kSlabK = 64;                       // one 128-byte swizzle row of 16-bit values
+constexpr int kOperandBytes = 128 * kSlabK * 2;  // what a CTA holds of an operand's slab
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kStages = 5;
+constexpr int kSlotBytes = 32 * 128;             // 32 rows of 64 values in 16 bits, or of 32 in fp32
+constexpr int kEpilogueWarps = 8;                // two for each quarter of tensor memory, each with one half of a tile's columns
+constexpr int kSlots = 2;                        // of each
+constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * kSlots * kSlotBytes + 1024 + 256;
+constexpr int kThreads = 64 + 32 * kEpilogueWarps;  // warp 0: TMA, warp 1: products, the others: epilogue
+constexpr uint64_t kTimeoutNs = 10ull * 1000 * 1000 * 1000;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kMostAbove = 60.0f * kLog2e;     // how far a logit may lie above a row's reference
+
+// kStats: the largest logit and the sum of exponentials of each row over half a tile's columns. kExp: E, and with `parts` the same sums. kScaled: alpha f_row D in 16 bits.
+// kSums, kAdded: D in fp32, written or added.
+enum Kind { kStats, kExp, kScaled, kSums, kAdded };
+
+// What is known of a group's rows when their tiles are made, and what comes out.
+struct Rows {
+  const int64_t* targets;
+  const float* ref;     // exponents' reference, times log2(e)
+  const float* mul;     // factors of E's rows; NULL: one
+  const float* value;   // with them, E's element at the target (else 0, to be filled in)
+  const float* bias;    // padded to whole tiles; NULL: none
+  float2* parts;        // [half tiles][stride]: largest z log2(e), sum of exp; NULL: not wanted
+  const int32_t* again; // for each 32 rows, whether they are to be formed again; NULL: all tiles are made
+  int64_t stride;
+  int n, classes;
+};
+struct Product {
+  int M, N, K;          // D is M x N
+  int tiles_m, tiles_n, total;
+  int n_inner;          // neighbouring tiles share rows (else columns)
+  const float* alpha;
+  const float* factor;  // of D's rows; NULL: one
+};
+struct Maps {
+  CUtensorMap a, b, out;
+};
+
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float (&f)[8]) {
+  dev::Raw8<T> r;
+  dev::pack(f, r);
+  return r.a;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Sixteen bytes `j` of a lane's row in a box of 32 rows of 128 bytes, as TMA swizzles them (the box starts on 1024 bytes).
+__device__ __forceinline__ uint4* box_at(uint8_t* box, int row, int j) { return reinterpret_cast<uint4*>(box + row * 128 + ((j ^ (row & 7)) << 4)); }
+
+struct TileAt {
+  int m0, n0;
+};
+template <int SIDE>
+__device__ __forceinline__ TileAt tile_at(const Product& p, int i) {
+  int rb, cb;
+  if (p.n_inner) {
+    rb = i / p.tiles_n;
+    cb = i - rb * p.tiles_n;
+  } else {
+    cb = i / p.tiles_m;
+    rb = i - cb * p.tiles_m;
+  }
+  return {rb * SIDE, cb * SIDE};
+}
+
+// What a CTA's roles share, in shared memory.
+struct Shared {
+  uint8_t *stages, *slots;
+  uint64_t *full, *empty;          // [kStages]
+  uint64_t *acc_full, *acc_empty;  // [2]
+  uint64_t* drained;
+  uint32_t* tmem_slot;
+  volatile uint32_t* failed;       // a wait has run out
+};
+__device__ __forceinline__ Shared shared_parts(uint8_t* raw) {
+  Shared s;
+  s.stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  s.slots = s.stages + kStages * kStageBytes;
+  s.full = reinterpret_cast<uint64_t*>(s.slots + kEpilogueWarps * kSlots * kSlotBytes);
+  s.empty = s.full + kStages;
+  s.acc_full = s.empty + kStages;
+  s.acc_empty = s.acc_full + 2;
+  s.drained = s.acc_empty + 2;
+  s.tmem_slot = reinterpret_cast<uint32_t*>(s.drained + 1);
+  s.failed = s.tmem_slot + 1;
+  return s;
+}
+template <bool PAIR>
+__device__ __forceinline__ void init_barriers(const Shared& s) {
+  for (int i = 0; i < kStages; ++i) {
+    mbar_init(&s.full[i], 1);
+    mbar_init(&s.empty[i], 1);
+  }
+  for (int i = 0; i < 2; ++i) {
+    mbar_init(&s.acc_full[i], 1);
+    mbar_init(&s.acc_empty[i], kEpilogueWarps * (PAIR ? 2 : 1));
+  }
+  mbar_init(s.drained, 1);
+  *s.failed = 0;
+  fence_barrier_init();
+}
+
+// TMA of a tile's slabs, `i` of which have gone before: both CTAs of a pair, each its own halves; the bytes are counted where the products are issued.
+// False when a wait has run out.
+template <bool PAIR, bool A_MN, bool B_MN>
+__device__ __forceinline__ bool load_tile(const Shared& s, const Maps& maps, const TileAt& at, uint32_t rank, int slabs, int& i) {
+  const int row = at.m0 + int(rank) * kTileM, col = at.n0 + int(rank) * 128;
+  for (int k = 0; k < slabs; ++k, ++i) {
+    const int st = i % kStages;
+    if (i >= kStages && !mbar_wait(&s.empty[st], uint32_t((i / kStages - 1) & 1), kTimeoutNs)) {
+      *s.failed = 1;
+      return false;
+    }
+    uint8_t* a = s.stages + st * kStageBytes;
+    uint8_t* b = a + kOperandBytes;
+    const int k0 = k * kSlabK;
+    if (rank == 0) mbar_arrive_expect_tx(&s.full[st], kStageBytes * (PAIR ? 2 : 1));
+    const uint32_t bar = PAIR ? rank0_address(&s.full[st]) : smem_u32(&s.full[st]);
+    if (A_MN) {
+      tma_operand<PAIR>(a, &maps.a, row, k0, 0, bar);
+      tma_operand<PAIR>(a + 8192, &maps.a, row + 64, k0, 0, bar);
+    } else {
+      tma_operand<PAIR>(a, &maps.a, k0, row, 0, bar);
+    }
+    if (B_MN) {
+      tma_operand<PAIR>(b, &maps.b, col, k0, 0, bar);
+      tma_operand<PAIR>(b + 8192, &maps.b, col + 64, k0, 0, bar);
+    } else {
+      tma_operand<PAIR>(b, &maps.b, k0, col, 0, bar);
+    }
+  }
+  return true;
+}
+// The copies that are still under way when the loads end: all have arrived when the products that read them are done; if somebody has given up, as
+// much as can be waited for (the bytes of a pair are counted by rank 0, the stages of rank 1 are given back by its products).
+__device__ __forceinline__ void drain_loads(const Shared& s, uint32_t rank, int i) {
+  for (int j = max(0, i - kStages); j < i; ++j) {
+    if (*s.failed == 0 || rank != 0) mbar_wait(&s.empty[j % kStages], uint32_t((j / kStages) & 1), kTimeoutNs);
+    else mbar_wait(&s.full[j % kStages], uint32_t((j / kStages) & 1), kTimeoutNs);
+  }
+}
+// The products of a tile, the n-th, into its accumulator. False when a wait has run out.
+template <bool PAIR, bool BF16, bool A_MN, bool B_MN>
+__device__ __forceinline__ bool multiply_tile(const Shared& s, uint32_t tmem, int slabs, int n, int& i) {
+  constexpr int kSide = PAIR ? 256 : 128;
+  constexpr uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(kSide >> 3) << 17) | (uint32_t(kSide >> 4) << 24);
+  const int acc = n & 1;
+  if (n >= 2 && !mbar_wait(&s.acc_empty[acc], uint32_t((n / 2 - 1) & 1), kTimeoutNs)) return false;
+  tc_fence_after_sync();
+  const uint32_t d = tmem + uint32_t(acc * kSide);
+  for (int k = 0; k < slabs; ++k, ++i) {
+    const int st = i % kStages;
+    if (!mbar_wait(&s.full[st], uint32_t((i / kStages) & 1), kTimeoutNs)) return false;
+    tc_fence_after_sync();
+    const uint32_t a = smem_u32(s.stages + st * kStageBytes), b = a + kOperandBytes;
+#pragma unroll
+    for (int kk = 0; kk < kSlabK / 16; ++kk) {
+      // K-major: 16 elements along K are 32 bytes of a swizzle row; MN-major: 16 K-rows are two groups of eight rows of 128 bytes
+      const uint64_t ad = A_MN ? make_smem_desc(a + kk * 2048, 8192, 1024) : make_smem_desc(a + kk * 32, 16, 1024);
+      const uint64_t bd = B_MN ? make_smem_desc(b + kk * 2048, 8192, 1024) : make_smem_desc(b + kk * 32, 16, 1024);
+      if (PAIR) umma_f16_pair(d, ad, bd, idesc, (k > 0 || kk > 0) ? 1u : 0u);
+      else umma_f16(d, ad, bd, idesc, (k > 0 || kk > 0) ? 1u : 0u);
+    }
+    if (PAIR) umma_commit_pair(&s.empty[st]);
+    else umma_commit(&s.empty[st]);
+  }
+  if (PAIR) umma_commit_pair(&s.acc_full[acc]);
+  else umma_commit(&s.acc_full[acc]);
+  return true;
+}
+template <bool PAIR>
+__device__ __forceinline__ void drain_products(const Shared& s) {
+  *s.failed = 1;
+  if (PAIR) umma_commit_pair(s.drained);
+  else umma_commit(s.drained);
+  mbar_wait(s.drained, 0, kTimeoutNs);
+}
+
+// The n-th tile's accumulator taken to where it belongs, by one of the epilogue's warps; `used`: how many slots it has filled so far.
+template <typename T, int KIND, bool PAIR>
+__device__ __forceinline__ void finish_tile(const Shared& s, uint32_t tmem, const Product& p, const Rows& rows, const Maps& maps, const TileAt& at, uint32_t rank, int n, uint32_t& used) {
+  constexpr int kSide = PAIR ? 256 : 128, kHalf = kSide / 2;
+  constexpr bool kStores = KIND != kStats;
+  constexpr int kChunk = KIND == kSums || KIND == kAdded ? 32 : 64;  // columns of a slot
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int quad = warp & 3, half = (warp - 2) >> 2;  // the lanes of tensor memory that this warp may read; its half of the columns
+  const int acc = n & 1;
+  const int row0 = at.m0 + int(rank) * kTileM + quad * 32, row = row0 + lane, col0 = at.n0 + half * kHalf;
+  const bool mine = row0 < p.M && col0 < p.N;
+  // of this lane's row
+  int target = -1;
+  bool dead = false;
+  float ref = 0.0f, mul = 1.0f, value = 0.0f;
+  if constexpr (KIND == kStats || KIND == kExp) {
+    if (mine && row < rows.n) {
+      const int64_t t = rows.targets[row];
+      dead = t < 0 || t >= rows.classes;
+      target = dead ? -1 : int(t);
+      if (KIND == kExp) {
+        ref = rows.ref[row];
+        if (rows.mul != nullptr) mul = rows.mul[row], value = rows.value[row];
+      }
+    } else {
+      dead = true;
+    }
+  }
+  float alpha = 1.0f;
+  if constexpr (KIND == kScaled) {
+    alpha = *p.alpha;
+    if (p.factor != nullptr && mine && row < p.M) {
+      const float f = p.factor[row];
+      dead = f == 0.0f;
+      alpha *= f;
+    }
+  }
+  bool ok = *s.failed == 0 && mbar_wait(&s.acc_full[acc], uint32_t((n / 2) & 1), kTimeoutNs);
+  ok = __all_sync(0xffffffffu, ok);
+  if (!ok) *s.failed = 1;
+  tc_fence_after_sync();
+  float most = -INFINITY, sum = 0.0f;
+  if (mine) {
+#pragma unroll 1
+    for (int c = 0; c < kHalf && col0 + c < p.N; c += kChunk) {
+      uint8_t* slot = s.slots + ((warp - 2) * kSlots + int(used % kSlots)) * kSlotBytes;
+      if (kStores) {
+        if (lane == 0) bulk_wait_read_but_one();  // the slot's last store
+        __syncwarp();
+      }
+#pragma unroll
+      for (int g = 0; g < kChunk / 16; ++g) {
+        float v[16];
+        const int first = col0 + c + g * 16;
+        tmem_ld_32x32b_x16(tmem + (uint32_t(quad * 32) << 16) + uint32_t(acc * kSide + half * kHalf + c + g * 16), v);
+        if (!ok) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(0x7fc00000u);
+        }
+        if constexpr (KIND == kStats || KIND == kExp) {
+          if (rows.bias != nullptr) {
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) {
+              const float4 b = *reinterpret_cast<const float4*>(rows.bias + first + k);
+              v[k] += b.x, v[k + 1] += b.y, v[k + 2] += b.z, v[k + 3] += b.w;
+            }
+          }
+          const bool edge = first + 16 > p.N, here = target >= first && target < first + 16;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) v[k] *= kLog2e;
+          if (edge || __any_sync(0xffffffffu, here)) {  // what is no class, and the target, stay out of the sums
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              if (first + k >= p.N || first + k == target) v[k] = -INFINITY;
+          }
+          float top = v[0];
+#pragma unroll
+          for (int k = 1; k < 16; ++k) top = fmaxf(top, v[k]);
+          if constexpr (KIND == kStats) {
+            const float now = fmaxf(most, top), base = now == -INFINITY ? 0.0f : now;
+            sum *= exp2_fast(most - base);
+            most = now;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) sum += exp2_fast(v[k] - base);
+          } else {
+            most = fmaxf(most, top);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              v[k] = exp2_fast(v[k] - ref);
+              sum += v[k];
+              v[k] *= mul;
+            }
+            if (__any_sync(0xffffffffu, here)) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k)
+                if (first + k == target) v[k] = value;
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) v[k] = dead ? 0.0f : v[k];
+          }
+        }
+        if constexpr (KIND == kScaled) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) v[k] = dead ? 0.0f : v[k] * alpha;
+        }
+        if constexpr (KIND == kExp || KIND == kScaled) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = v[8 * e + k];
+            *box_at(slot, lane, 2 * g + e) = pack16<T>(w);
+          }
+        }
+        if constexpr (KIND == kSums || KIND == kAdded) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *box_at(slot, lane, 4 * g + e) = make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3]));
+        }
+      }
+      if (kStores) {
+        fence_async_proxy();
+        __syncwarp();
+        if (lane == 0) {
+          if (KIND == kAdded) tma_add_3d(&maps.out, slot, col0 + c, row0, 0);
+          else tma_store_3d(&maps.out, slot, col0 + c, row0, 0);
+          bulk_commit();
+        }
+        ++used;
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncwarp();
+  if (lane == 0) mbar_arrive_at((PAIR ? rank0_address(&s.acc_empty[0]) : smem_u32(&s.acc_empty[0])) + uint32_t(acc) * 8);
+  if constexpr (KIND == kStats || KIND == kExp) {
+    if (mine && row < rows.n && rows.parts != nullptr) rows.parts[int64_t(col0 / kHalf) * rows.stride + row] = make_float2(most, sum);
+  }
+}
+
+// D = A B, walked over tile by tile by CTAs that stay (PAIR: pairs of CTAs that share the tensor cores' work on 256 x 256, each with its 128 rows of A, half of
+// B's columns, and 128 rows of the result; else one CTA and 128 x 128). A_MN / B_MN: the operand lies with its rows (columns of B) adjacent in memory, not its K. The accumulators of
+// two tiles share tensor memory: the epilogue of one runs under the products of the next.
+// A wait that runs out makes every result of this CTA from there on not a number.
+template <typename T, int KIND, bool A_MN, bool B_MN, bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1) ce_product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, const __grid_constant__ Rows rows) {
+  constexpr int kSide = PAIR ? 256 : 128;
+  extern __shared__ uint8_t smem_raw[];
+  const Shared s = shared_parts(smem_raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int slabs = (p.K + kSlabK - 1) / kSlabK;
+  const uint32_t rank = PAIR ? cluster_rank() : 0u;   // 0: the CTA that issues the pair's products
+  const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, step = PAIR ? gridDim.x / 2 : gridDim.x;
+  // rows to be formed again: their tiles alone (eight groups of 32 rows in a pair's tile, four in a CTA's)
+  const bool some = KIND == kExp && rows.again != nullptr;
+  if (some) {
+    follow();
+    bool any = false;
+    for (int i = threadIdx.x; i < (rows.n + 31) / 32; i += kThreads) any = any || rows.again[i] != 0;
+    if (__syncthreads_or(any) == 0) return;
+  }
+  auto skip = [&](const TileAt& at) {
+    if constexpr (KIND == kExp) {
+      if (!some) return false;
+      for (int i = at.m0 / 32; i < min((at.m0 + kSide) / 32, (rows.n + 31) / 32); ++i)
+        if (rows.again[i] != 0) return false;
+      return true;
+    } else {
+      return false;
+    }
+  };
+
+  if (threadIdx.x == 0) {
+    init_barriers<PAIR>(s);
+    prefetch_tensormap(&maps.a);
+    prefetch_tensormap(&maps.b);
+  }
+  if (KIND != kStats && threadIdx.x == 64) prefetch_tensormap(&maps.out);
+  if (warp == 1) {
+    if (PAIR) tmem_alloc_pair(s.tmem_slot, 2 * kSide);
+    else tmem_alloc(s.tmem_slot, 2 * kSide);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (PAIR) cluster_sync();  // the other CTA's barriers exist from here on
+  tc_fence_after_sync();
+  const uint32_t tmem = *s.tmem_slot;
+  may_follow();
+  follow();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int i = 0;
+      for (int tile = first; tile < p.total; tile += step) {
+        const TileAt at = tile_at<kSide>(p, tile);
+        if (skip(at)) continue;
+        if (!load_tile<PAIR, A_MN, B_MN>(s, maps, at, rank, slabs, i)) break;
+      }
+      drain_loads(s, rank, i);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      int i = 0, n = 0;
+      bool ok = true;
+      for (int tile = first; tile < p.total && ok; tile += step) {
+        if (skip(tile_at<kSide>(p, tile))) continue;
+        ok = multiply_tile<PAIR, std::is_same<T, __nv_bfloat16>::value, A_MN, B_MN>(s, tmem, slabs, n, i);
+        ++n;
+      }
+      if (!ok) drain_products<PAIR>(s);
+    }
+  } else {
+    int n = 0;
+    uint32_t used = 0;
+    for (int tile = first; tile < p.total; tile += step) {
+      const TileAt at = tile_at<kSide>(p, tile);
+      if (skip(at)) continue;
+      finish_tile<T, KIND, PAIR>(s, tmem, p, rows, maps, at, rank, n, used);
+      ++n;
+    }
+    if (lane == 0) bulk_wait_read();  // the stores have left shared memory; the end of the kernel is what others wait for
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (PAIR) cluster_sync();  // neither CTA's barriers and tensor memory go while the other may still use them
+  if (warp == 1) {
+    if (PAIR) tmem_dealloc_pair(tmem, 2 * kSide);
+    else tmem_dealloc(tmem, 2 * kSide);
+  }
+}
+
+// ---- what goes before, between and behind the products -----------------------------------------------------------------------
+
+constexpr int kBeginT = 256;
+constexpr int kRowsT = 256;
+constexpr int kRowsAtOnce = 32;   // rows of a CTA
+
+// Of the whole call. alpha: what G's rows are multiplied by in the end; unit: the largest weight of a row, by which the weights are divided.
+struct Scales {
+  float alpha, unit, count;
+};
+
+struct Begin {
+  NangilaLinearCeParams p;
+  int what;
+  float* zt;      // [n] the targets' logits
+  float* bias;    // padded to whole tiles
+  int bias_count;
+  Scales* scales;
+  float e_scale;  // power of two by which E is larger
+};
+template <typename T>
+__device__ __forceinline__ float bias_value(const void* b, int dtype, int i) {
+  return dtype == NANGILA_F32 ? static_cast<const float*>(b)[i] : dtype == NANGILA_F16 ? __half2float(static_cast<const __half*>(b)[i]) : __bfloat162float(static_cast<const __nv_bfloat16*>(b)[i]);
+}
+// CTA 0: how many targets are not ignored, the largest weight, and the factors that follow. The others: the targets' logits, a warp for each row; the bias in fp32.
+template <typename T>
+__global__ void __launch_bounds__(kBeginT) ce_begin_kernel(const __grid_constant__ Begin a) {
+  const NangilaLinearCeParams& p = a.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (blockIdx.x == 0) {
+    __shared__ int64_t counts[kBeginT / 32];
+    __shared__ float tops[kBeginT / 32];
+    int64_t count = 0;
+    float top = 0.0f;
+    bool bad = false;
+    for (int64_t i = threadIdx.x; i < p.n; i += kBeginT) {
+      const int64_t t = p.targets[i];
+      count += t != p.ignore ? 1 : 0;
+      if (p.upstream_rows && t >= 0 && t < p.classes && t != p.ignore) {
+        const float u = fabsf(p.upstream[i]);
+        bad = bad || !(u <= 3.0e38f);
+        top = fmaxf(top, u);
+      }
+    }
+    if (bad) top = __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+      count += __shfl_xor_sync(0xffffffffu, count, off);
+      const float other = __shfl_xor_sync(0xffffffffu, top, off);
+      top = !(top >= other) ? (isnan(top) ? top : other) : top;
+    }
+    if (lane == 0) counts[warp] = count, tops[warp] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < kBeginT / 32; ++w) {
+        count += counts[w];
+        top = !(top >= tops[w]) ? (isnan(top) ? top : tops[w]) : top;
+      }
+      float u = 1.0f;
+      if (a.what == NANGILA_CE_GRADIENTS) u = p.upstream_rows ? top : *p.upstream;
+      if (p.mean) u = count > 0 ? u / float(count) : 0.0f;
+      a.scales->alpha = u / a.e_scale;
+      a.scales->unit = p.upstream_rows ? top : 1.0f;
+      a.scales->count = float(count);
+    }
+    return;
+  }
+  const int64_t thread = int64_t(blockIdx.x - 1) * kBeginT + threadIdx.x, threads = int64_t(gridDim.x - 1) * kBeginT;
+  if (p.bias != nullptr)
+    for (int64_t i = thread; i < a.bias_count; i += threads) a.bias[i] = i < p.classes ? bias_value<T>(p.bias, p.bias_dtype, int(i)) : 0.0f;
+  if (a.what == NANGILA_CE_GRADIENTS) return;
+  for (int64_t i = thread / 32; i < p.n; i += threads / 32) {
+    const int64_t t = p.targets[i];
+    if (t < 0 || t >= p.classes || t == p.ignore) {
+      if (lane == 0) a.zt[i] = 0.0f;
+      continue;
+    }
+    const T* x = static_cast<const T*>(p.x) + i * p.x_stride;
+    const T* w = static_cast<const T*>(p.w) + t * p.w_stride;
+    float z = 0.0f;
+    for (int c = lane * 8; c < p.d; c += 256) {
+      dev::Raw8<T> rx, rw;
+      dev::fetch(x + c, rx);
+      dev::fetch(w + c, rw);
+      float u[8], v[8];
+      dev::unpack(rx, u);
+      dev::unpack(rw, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) z = __fmaf_rn(u[k], v[k], z);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) z += __shfl_xor_sync(0xffffffffu, z, off);
+    if (lane == 0) a.zt[i] = z + (p.bias != nullptr ? bias_value<T>(p.bias, p.bias_dtype, int(t)) : 0.0f);
+  }
+}
+
+// The rows of a group, before their tiles are made (gradients from lse) or behind them.
+struct Group {
+  NangilaLinearCeParams p;   // of the whole call
+  int64_t row0, stride;      // the group's first row; of `parts`
+  int n, parts_count;
+  const float* zt;           // [n] of the group, as are the following
+  const float2* parts;
+  float *ref, *mul, *value, *factor;
+  int32_t* again;            // [groups of 32 rows]; both passes of NANGILA_CE_BOTH
+  void* e;                   // [n][e_stride]
+  void* xs;                  // [n][d]: rows of x as dw's product takes them
+  int64_t e_stride;
+  const Scales* scales;
+  float e_scale;
+};
+// Losses and lse of the joined sums; with E: also the element at the target, the rows' factors and scaled rows of x. pass 0: NANGILA_CE_LOSSES; 1, 2: NANGILA_CE_BOTH, for all rows
+// and for those of tiles that were formed again.
+template <typename T>
+__global__ void __launch_bounds__(kRowsT) ce_rows_kernel(const __grid_constant__ Group a, int pass, int tile_rows) {
+  constexpr int kWarps = kRowsT / 32;
+  __shared__ float2 joined[kWarps][kRowsAtOnce];
+  __shared__ float factors[kRowsAtOnce];
+  follow();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row0 = blockIdx.x * kRowsAtOnce, row = row0 + lane;
+  if (pass == 2) {
+    const int all = (a.n + 31) / 32, per = tile_rows / 32;
+    const int from = int(blockIdx.x) / per * per;
+    bool any = false;
+    for (int i = from; i < min(from + per, all); ++i) any = any || a.again[i] != 0;
+    if (!any) return;
+  }
+  const bool here = row < a.n;
+  const float ref = pass != 0 && here ? a.ref[row] : 0.0f;
+  float most = -INFINITY, sum = 0.0f;
+  if (here) {
+    for (int i = warp; i < a.parts_count; i += kWarps) {
+      const float2 v = a.parts[int64_t(i) * a.stride + row];
+      if (pass == 0) {
+        const float now = fmaxf(most, v.x), base = now == -INFINITY ? 0.0f : now;
+        sum = sum * exp2_fast(most - base) + v.y * exp2_fast(v.x - base);
+        most = now;
+      } else {
+        most = fmaxf(most, v.x);
+        sum += v.y;
+      }
+    }
+  }
+  joined[warp][lane] = make_float2(most, sum);
+  __syncthreads();
+  if (warp == 0) {
+    for (int w = 1; w < kWarps; ++w) {
+      const float2 v = joined[w][lane];
+      if (pass == 0) {
+        const float now = fmaxf(most, v.x), base = now == -INFINITY ? 0.0f : now;
+        sum = sum * exp2_fast(most - base) + v.y * exp2_fast(v.x - base);
+        most = now;
+      } else {
+        most = fmaxf(most, v.x);
+        sum += v.y;
+      }
+    }
+    bool above = false;
+    float factor = 0.0f;
+    if (here) {
+      const int64_t i = a.row0 + row, t = a.p.targets[i];
+      const bool ignored = t == a.p.ignore, outside = !ignored && (t < 0 || t >= a.p.classes);
+      const float zt2 = a.zt[row] * kLog2e;
+      float loss, lse2;
+      if (pass == 0) {
+        // sum of exp2(z - most) over the others; the target's own on top
+        const float base = fmaxf(most, zt2);
+        const float rest = sum * exp2_fast(most - base), own = exp2_fast(zt2 - base);
+        lse2 = base + log2f(rest + own);
+        loss = zt2 >= most ? log1pf(sum * exp2_fast(most - zt2)) : (base - zt2) * kLn2 + logf(rest + own);
+      } else {
+        const float own = exp2_fast(zt2 - ref), whole = sum + own;
+        above = pass == 1 && !ignored && !outside && most - ref > kMostAbove;
+        factor = 1.0f / whole;
+        lse2 = ref + log2f(whole);
+        loss = ref == zt2 ? log1pf(sum) : (ref - zt2) * kLn2 + logf(whole);
+        if (above) a.ref[row] = most;  // (more than z_t: the largest of the row)
+        if (!ignored && !outside && a.e != nullptr) static_cast<T*>(a.e)[int64_t(row) * a.e_stride + t] = dev::Vec16<T>::from_float(-sum);
+      }
+      if (ignored || outside) {
+        loss = ignored ? 0.0f : __uint_as_float(0x7fc00000u);
+        factor = 0.0f;
+      }
+      a.p.losses[i] = loss;
+      if (a.p.lse != nullptr) a.p.lse[i] = lse2 * kLn2;
+      if (a.factor != nullptr) a.factor[row] = factor;
+    }
+    if (pass != 0) {
+      factors[lane] = factor;
+      const bool any = __any_sync(0xffffffffu, above);
+      if (pass == 1 && lane == 0) a.again[blockIdx.x] = any ? 1 : 0;
+    }
+  }
+  if (pass == 0 || a.xs == nullptr) return;
+  __syncthreads();
+  for (int r = warp; r < kRowsAtOnce && row0 + r < a.n; r += kWarps) {
+    const float f = factors[r];
+    const T* from = static_cast<const T*>(a.p.x) + (a.row0 + row0 + r) * a.p.x_stride;
+    T* to = static_cast<T*>(a.xs) + int64_t(row0 + r) * a.p.d;
+    for (int c = lane * 8; c < a.p.d; c += 256) {
+      dev::Raw8<T> raw;
+      dev::fetch(from + c, raw);
+      float v[8];
+      dev::unpack(raw, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = f == 0.0f ? 0.0f : v[k] * f;
+      dev::pack(v, raw);
+      dev::put(to + c, raw);
+    }
+  }
+}
+// NANGILA_CE_BOTH: the references before the tiles are made.
+__global__ void ce_refs_kernel(const float* zt, float* ref, int n) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < n) ref[i] = zt[i] * kLog2e;
+}
+// NANGILA_CE_GRADIENTS: what the tiles' epilogue takes of each row, and the rows of x without those that add nothing.
+template <typename T>
+__global__ void __launch_bounds__(kRowsT) ce_weights_kernel(const __grid_constant__ Group a) {
+  const int lane = threadIdx.x & 31;
+  const int row = (blockIdx.x * kRowsT + threadIdx.x) >> 5;
+  if (row >= a.n) return;
+  const int64_t i = a.row0 + row, t = a.p.targets[i];
+  const bool lives = t != a.p.ignore && t >= 0 && t < a.p.classes;
+  if (lane == 0) {
+    const float unit = a.scales->unit;
+    float weight = a.p.upstream_rows ? (unit > 0.0f ? a.p.upstream[i] / unit : unit) : 1.0f;
+    if (!lives) weight = 0.0f;
+    a.ref[row] = a.p.lse[i] * kLog2e;
+    a.mul[row] = weight * a.e_scale;
+    a.value[row] = expm1f(-a.p.losses[i]) * weight * a.e_scale;
+    a.factor[row] = lives ? 1.0f : 0.0f;
+  }
+  if (a.xs == nullptr) return;
+  const T* from = static_cast<const T*>(a.p.x) + i * a.p.x_stride;
+  T* to = static_cast<T*>(a.xs) + int64_t(row) * a.p.d;
+  for (int c = lane * 8; c < a.p.d; c += 256) {
+    dev::Raw8<T> raw;
+    dev::fetch(from + c, raw);
+    if (!lives) raw.a = make_uint4(0, 0, 0, 0);
+    dev::put(to + c, raw);
+  }
+}
+// The sum or mean of the losses, in a fixed order.
+__global__ void __launch_bounds__(1024) ce_total_kernel(const float* losses, int64_t n, const Scales* scales, int mean, float* out) {
+  __shared__ double part[32];
+  follow();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  double sum = 0.0;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) sum += double(losses[i]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  if (lane == 0) part[warp] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = 0.0;
+    for (int w = 0; w < 32; ++w) sum += part[w];
+    *out = float(mean ? sum / double(scales->count) : sum);
+  }
+}
+// Columns of E, each row times its factor, added up: 256 columns and a share of the rows a CTA, the shares' sums one behind the other.
+constexpr int kColumnT = 256;
+template <typename T>
+__global__ void __launch_bounds__(kColumnT) ce_columns_kernel(const T* e, int64_t e_stride, const float* factor, int n, int classes, int share, float* partial) {
+  __shared__ float part[8][256];
+  follow();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.x * 256 + lane * 8;
+  const int from = blockIdx.y * share, to = min(n, from + share);
+  float acc[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
+  if (col < classes) {
+#pragma unroll 4
+    for (int r = from + warp; r < to; r += 8) {
+      dev::Raw8<T> raw;
+      dev::fetch(e + int64_t(r) * e_stride + col, raw);
+      float v[8];
+      dev::unpack(raw, v);
+      const float f = factor[r];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) acc[k] = __fmaf_rn(v[k], f, acc[k]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) part[warp][lane * 8 + k] = acc[k];
+  __syncthreads();
+  float sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) sum += part[w][threadIdx.x];
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c < classes) partial[int64_t(blockIdx.y) * classes + c] = sum;
+}
+__global__ void ce_bias_grad_kernel(const float* partial, int shares, int classes, int rows, const Scales* scales, void* dbias, int dtype) {
+  follow();
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= rows) return;
+  float sum = 0.0f;
+  if (i < classes) {
+    for (int s = 0; s < shares; ++s) sum += partial[int64_t(s) * classes + i];
+    sum *= scales->alpha;
+  }
+  if (dtype == NANGILA_F32) static_cast<float*>(dbias)[i] = sum;
+  else if (dtype == NANGILA_F16) static_cast<__half*>(dbias)[i] = __float2half_rn(sum);
+  else static_cast<__nv_bfloat16*>(dbias)[i] = __float2bfloat16_rn(sum);
+}
+// dw = alpha sums, in 16 bits
+template <typename T>
+__global__ void __launch_bounds__(256) ce_round_kernel(const float* sums, const Scales* scales, T* out, int64_t n8) {
+  follow();
+  const float alpha = scales->alpha;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n8; i += int64_t(gridDim.x) * 256) {
+    dev::Raw8<float> in;
+    dev::fetch(sums + i * 8, in);
+    float v[8];
+    dev::unpack(in, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= alpha;
+    dev::Raw8<T> r;
+    dev::pack(v, r);
+    dev::put(out + i * 8, r);
+  }
+}
+template <typename T>
+__device__ void rescale(T* a, int64_t n, float f) {
+  const int64_t thread = int64_t(blockIdx.x) * blockDim.x + threadIdx.x, threads = int64_t(gridDim.x) * blockDim.x;
+  const int64_t whole = (reinterpret_cast<uintptr_t>(a) & 15u) == 0 ? n / 8 : 0;
+  for (int64_t i = thread; i < whole; i += threads) {
+    dev::Raw8<T> raw;
+    dev::fetch(a + i * 8, raw);
+    float v[8];
+    dev::unpack(raw, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= f;
+    dev::pack(v, raw);
+    dev::put(a + i * 8, raw);
+  }
+  for (int64_t i = whole * 8 + thread; i < n; i += threads) a[i] = dev::Vec16<T>::from_float(dev::Vec16<T>::to_float(a[i]) * f);
+}
+__global__ void __launch_bounds__(256) rescale_kernel(const __grid_constant__ NangilaRescaleParams p) {
+  const float f = *p.factor;
+  if (f == 1.0f) return;
+  for (int i = 0; i < 3; ++i) {
+    if (p.array[i] == nullptr) continue;
+    if (p.dtype[i] == NANGILA_F32) rescale(static_cast<float*>(p.array[i]), p.count[i], f);
+    else if (p.dtype[i] == NANGILA_F16) rescale(static_cast<__half*>(p.array[i]), p.count[i], f);
+    else rescale(static_cast<__nv_bfloat16*>(p.array[i]), p.count[i], f);
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------------
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                              CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  return fn;
+}
+struct Matrix {
+  const void* base;
+  int64_t rows, cols, ld;
+  CUtensorMapDataType type;
+};
+// copied in boxes of box_inner x box_outer; what lies outside reads as zero and is not written
+bool make_map(CUtensorMap* map, const Matrix& m, uint32_t box_inner, uint32_t box_outer) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const int size = m.type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2;
+  const cuuint64_t dims[3] = {cuuint64_t(m.cols), cuuint64_t(m.rows), 1};
+  const cuuint64_t strides[2] = {cuuint64_t(m.ld) * size, cuuint64_t(m.ld) * size * cuuint64_t(m.rows)};
+  const cuuint32_t box[3] = {box_inner, box_outer, 1}, step[3] = {1, 1, 1};
+  return fn(map, m.type, 3, const_cast<void*>(m.base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+int sm_count() {
+  static int sms[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (sms[dev] == 0) cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
+  return sms[dev];
+}
+// Shared memory above the default limit, asked for once for each kernel and device.
+int allow_smem(const void* kernel, int bytes) {
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> asked;
+  int dev = 0;
+  if (const cudaError_t e = cudaGetDevice(&dev)) return int(e);
+  std::lock_guard<std::mutex> lock(mu);
+  if (asked.count({kernel, dev})) return 0;
+  if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return int(e);
+  asked.insert({kernel, dev});
+  return 0;
+}
+
+// The product of a and b, `out` the result where there is one in memory.
+template <typename T, int KIND, bool A_MN, bool B_MN, bool PAIR>
+int launch_product(const Matrix& a, const Matrix& b, const Matrix* out, Product p, const Rows& rows, cudaStream_t stream) {
+  constexpr int kSide = PAIR ? 256 : 128;
+  Maps maps;
+  constexpr bool kWide = KIND == kSums || KIND == kAdded;
+  if (!make_map(&maps.a, a, 64, A_MN ? 64 : 128) || !make_map(&maps.b, b, 64, B_MN ? 64 : 128) || !make_map(&maps.out, out != nullptr ? *out : a, kWide ? 32 : 64, 32))
+    return int(cudaErrorNotSupported);
+  p.tiles_m = (p.M + kSide - 1) / kSide;
+  p.tiles_n = (p.N + kSide - 1) / kSide;
+  const int64_t total = int64_t(p.tiles_m) * p.tiles_n;
+  if (total > 0x3fffffff) return int(cudaErrorInvalidValue);
+  p.total = int(total);
+  auto* kernel = ce_product_kernel<T, KIND, A_MN, B_MN, PAIR>;
+  if (const int e = allow_smem(reinterpret_cast<const void*>(kernel), kSmem)) return e;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = PAIR ? 2 : 1;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  const int sms = sm_count();
+  cfg.gridDim = dim3(unsigned(PAIR ? 2 * std::min(p.total, sms / 2) : std::min(p.total, sms)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 2 : 1;
+  return int(cudaLaunchKernelEx(&cfg, kernel, maps, p, rows));
+}
+
+// How a call is cut up, and where its parts lie in the workspace.
+struct Plan {
+  int64_t group;      // tokens at a time
+  int64_t groups, e_stride, parts, shares, share;
+  bool pair;          // tiles of the logits
+  bool wide;          // dw is summed up over the groups
+  int64_t at_scales, at_zt, at_bias, at_ref, at_mul, at_value, at_factor, at_again, at_parts, at_e, at_xs, at_sums, at_columns, total;
+  int64_t bias_count;
+};
+constexpr int64_t kGroupBytes = int64_t(1) << 29;  // of E
+Plan plan(const NangilaLinearCeParams& p, int what) {
+  Plan l;
+  std::memset(&l, 0, sizeof l);
+  const int64_t classes = p.classes;
+  l.e_stride = (classes + 63) / 64 * 64;
+  // Tokens enough for the rows of one small tile take small tiles.
+  l.pair = p.n > 128;
+  const int64_t side = l.pair ? 256 : 128, half = side / 2;
+  l.parts = (classes + half - 1) / half;
+  const int64_t row_bytes = what == NANGILA_CE_LOSSES ? l.parts * 8 : l.e_stride * 2;
+  const int64_t most = std::max<int64_t>(256, (what == NANGILA_CE_LOSSES ? kGroupBytes / 8 : kGroupBytes) / row_bytes / 256 * 256);
+  l.groups = (p.n + most - 1) / most;
+  l.group = std::min(p.n, ((p.n + l.groups - 1) / l.groups + 255) / 256 * 256);
+  l.groups = (p.n + l.group - 1) / l.group;
+  l.wide = l.groups > 1 && p.dw != nullptr;
+  l.bias_count = (classes + side - 1) / side * side;
+  // rows of E that a CTA adds up for the bias's gradient: some hundreds of CTAs
+  const int64_t across = (classes + 255) / 256;
+  l.shares = std::max<int64_t>(1, std::min<int64_t>((l.group + 63) / 64, (4 * 148 + across - 1) / across));
+  l.share = (l.group + l.shares - 1) / l.shares;
+  auto take = [&](int64_t bytes) {
+    const int64_t at = l.total;
+    l.total += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  l.at_scales = take(sizeof(Scales));
+  l.at_zt = take(what == NANGILA_CE_GRADIENTS ? 0 : p.n * 4);
+  l.at_bias = take(p.bias != nullptr ? l.bias_count * 4 : 0);
+  l.at_parts = take(what == NANGILA_CE_GRADIENTS ? 0 : l.parts * l.group * 8);
+  if (what == NANGILA_CE_LOSSES) return l;
+  l.at_ref = take(l.group * 4);
+  l.at_mul = take(what == NANGILA_CE_GRADIENTS ? l.group * 4 : 0);
+  l.at_value = take(what == NANGILA_CE_GRADIENTS ? l.group * 4 : 0);
+  l.at_factor = take(l.group * 4);
+  l.at_again = take((l.group + 31) / 32 * 4);
+  l.at_e = take(l.group * l.e_stride * 2);
+  l.at_xs = take(p.dw != nullptr ? l.group * p.d * 2 : 0);
+  l.at_sums = take(l.wide ? int64_t(p.rows) * p.d * 4 : 0);
+  l.at_columns = take(p.dbias != nullptr ? l.groups * l.shares * classes * 4 : 0);
+  return l;
+}
+
+template <typename T, int KIND>
+int logits(bool pair, const Matrix& x, const Matrix& w, const Matrix* e, const Product& q, const Rows& rows, cudaStream_t stream) {
+  return pair ? launch_product<T, KIND, false, false, true>(x, w, e, q, rows, stream) : launch_product<T, KIND, false, false, false>(x, w, e, q, rows, stream);
+}
+
+template <typename T>
+int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
+  const CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const Plan l = plan(p, what);
+  auto* ws = static_cast<uint8_t*>(p.workspace);
+  auto* scales = reinterpret_cast<Scales*>(ws + l.at_scales);
+  auto* zt = reinterpret_cast<float*>(ws + l.at_zt);
+  auto* bias = p.bias != nullptr ? reinterpret_cast<float*>(ws + l.at_bias) : nullptr;
+  auto* sums = reinterpret_cast<float*>(ws + l.at_sums);
+  auto* columns = reinterpret_cast<float*>(ws + l.at_columns);
+
+  Begin begin;
+  std::memset(&begin, 0, sizeof begin);
+  begin.p = p;
+  begin.what = what;
+  begin.zt = zt;
+  begin.bias = bias;
+  begin.bias_count = int(l.bias_count);
+  begin.scales = scales;
+  begin.e_scale = what == NANGILA_CE_GRADIENTS && std::is_same<T, __half>::value ? 32768.0f : 1.0f;
+  ce_begin_kernel<T><<<unsigned(1 + std::min<int64_t>((p.n + kBeginT / 32 - 1) / (kBeginT / 32), 148 * 8)), kBeginT, 0, stream>>>(begin);
+  int e = int(cudaGetLastError());
+
+  for (int64_t g = 0; g < l.groups && e == 0; ++g) {
+    Group a;
+    std::memset(&a, 0, sizeof a);
+    a.p = p;
+    a.row0 = g * l.group;
+    a.n = int(std::min(l.group, p.n - a.row0));
+    a.stride = l.group;
+    a.parts_count = int(l.parts);
+    a.zt = zt + a.row0;
+    a.parts = reinterpret_cast<const float2*>(ws + l.at_parts);
+    a.scales = scales;
+    a.e_scale = begin.e_scale;
+    Rows rows;
+    std::memset(&rows, 0, sizeof rows);
+    rows.targets = p.targets + a.row0;
+    rows.bias = bias;
+    rows.parts = what == NANGILA_CE_GRADIENTS ? nullptr : reinterpret_cast<float2*>(ws + l.at_parts);
+    rows.stride = l.group;
+    rows.n = a.n;
+    rows.classes = p.classes;
+    Product q;
+    std::memset(&q, 0, sizeof q);
+    q.M = a.n;
+    q.N = p.classes;
+    q.K = p.d;
+    const Matrix x{static_cast<const T*>(p.x) + a.row0 * p.x_stride, a.n, p.d, p.x_stride, type}, w{p.w, p.classes, p.d, p.w_stride, type};
+    const unsigned row_ctas = unsigned((a.n + kRowsAtOnce - 1) / kRowsAtOnce);
+    const int tile_rows = l.pair ? 256 : 128;
+    if (what == NANGILA_CE_LOSSES) {
+      e = logits<T, kStats>(l.pair, x, w, nullptr, q, rows, stream);
+      if (e == 0) e = int(launch_following(ce_rows_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, 0, tile_rows));
+      continue;
+    }
+    a.ref = reinterpret_cast<float*>(ws + l.at_ref);
+    a.factor = reinterpret_cast<float*>(ws + l.at_factor);
+    a.e = ws + l.at_e;
+    a.e_stride = l.e_stride;
+    a.xs = p.dw != nullptr ? ws + l.at_xs : nullptr;
+    rows.ref = a.ref;
+    const Matrix ex{a.e, a.n, p.classes, l.e_stride, type};
+    if (what == NANGILA_CE_BOTH) {
+      a.again = reinterpret_cast<int32_t*>(ws + l.at_again);
+      ce_refs_kernel<<<unsigned((a.n + 255) / 256), 256, 0, stream>>>(a.zt, a.ref, a.n);
+      e = int(cudaGetLastError());
+      if (e == 0) e = logits<T, kExp>(l.pair, x, w, &ex, q, rows, stream);
+      if (e == 0) e = int(launch_following(ce_rows_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, 1, tile_rows));
+      rows.again = a.again;
+      if (e == 0) e = logits<T, kExp>(l.pair, x, w, &ex, q, rows, stream);
+      if (e == 0) e = int(launch_following(ce_rows_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, 2, tile_rows));
+    } else {
+      a.mul = reinterpret_cast<float*>(ws + l.at_mul);
+      a.value = reinterpret_cast<float*>(ws + l.at_value);
+      ce_weights_kernel<T><<<unsigned((int64_t(a.n) * 32 + kRowsT - 1) / kRowsT), kRowsT, 0, stream>>>(a);
+      e = int(cudaGetLastError());
+      rows.mul = a.mul;
+      rows.value = a.value;
+      if (e == 0) e = logits<T, kExp>(l.pair, x, w, &ex, q, rows, stream);
+    }
+    if (e == 0 && p.dbias != nullptr) {
+      e = int(launch_following(ce_columns_kernel<T>, dim3(unsigned((p.classes + 255) / 256), unsigned(l.shares)), kColumnT, 0, stream, static_cast<const T*>(a.e), l.e_stride,
+                               static_cast<const float*>(a.factor), a.n, int(p.classes), int(l.share), columns + g * l.shares * p.classes));
+    }
+    if (e == 0 && p.dx != nullptr) {
+      Product d = q;
+      d.N = p.d;
+      d.K = p.classes;
+      d.n_inner = 1;
+      d.alpha = &scales->alpha;
+      d.factor = a.factor;
+      const Matrix out{static_cast<T*>(p.dx) + a.row0 * p.d, a.n, p.d, p.d, type};
+      e = launch_product<T, kScaled, false, true, true>(ex, w, &out, d, rows, stream);
+    }
+    if (e == 0 && p.dw != nullptr) {
+      Product d = q;
+      d.M = p.rows;
+      d.N = p.d;
+      d.K = a.n;
+      d.n_inner = 1;
+      d.alpha = &scales->alpha;
+      const Matrix xs{a.xs, a.n, p.d, p.d, type}, out{p.dw, p.rows, p.d, p.d, type}, wide{sums, p.rows, p.d, p.d, CU_TENSOR_MAP_DATA_TYPE_FLOAT32};
+      if (!l.wide) e = launch_product<T, kScaled, true, true, true>(ex, xs, &out, d, rows, stream);
+      else if (g == 0) e = launch_product<T, kSums, true, true, true>(ex, xs, &wide, d, rows, stream);
+      else e = launch_product<T, kAdded, true, true, true>(ex, xs, &wide, d, rows, stream);
+    }
+  }
+  if (e == 0 && l.wide)
+    e = int(launch_following(ce_round_kernel<T>, dim3(unsigned(std::min<int64_t>((int64_t(p.rows) * p.d / 8 + 255) / 256, 148 * 8))), 256, 0, stream, static_cast<const float*>(sums),
+                             static_cast<const Scales*>(scales), static_cast<T*>(p.dw), int64_t(p.rows) * p.d / 8));
+  if (e == 0 && p.dbias != nullptr)
+    e = int(launch_following(ce_bias_grad_kernel, dim3(unsigned((p.rows + 255) / 256)), 256, 0, stream, static_cast<const float*>(columns), int(l.groups * l.shares), int(p.classes), int(p.rows),
+                             static_cast<const Scales*>(scales), p.dbias, int(p.bias_dtype)));
+  if (e == 0 && what != NANGILA_CE_GRADIENTS && p.loss != nullptr)
+    e = int(launch_following(ce_total_kernel, dim3(1), 1024, 0, stream, static_cast<const float*>(p.losses), p.n, static_cast<const Scales*>(scales), int(p.mean), p.loss));
+  return e;
+}
+
+bool aligned(const void* p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+bool sound(const NangilaLinearCeParams* p, int what) {
+  if (!p || what < 0 || what > 2 || p->n < 1 || p->n > (int64_t(1) << 40) || p->d < 8 || p->d % 8 != 0 || p->d > NANGILA_CE_MAX_WIDTH || p->classes < 1 || p->rows < p->classes ||
+      p->rows > NANGILA_CE_MAX_CLASSES)
+    return false;
+  if (p->dtype != NANGILA_BF16 && p->dtype != NANGILA_F16) return false;
+  return what != NANGILA_CE_BOTH || p->dtype == NANGILA_BF16;
+}
+
+}  // namespace
+}  // namespace nangila
+
+extern "C" int64_t nangila_linear_ce_workspace(const NangilaLinearCeParams* p, int what) { return nangila::sound(p, what) ? nangila::plan(*p, what).total : -1; }
+
+extern "C" int nangila_linear_ce(const NangilaLinearCeParams* p, int what, cudaStream_t stream) {
+  using namespace nangila;
+  if (!sound(p, what) || !p->x || !p->w || !p->targets || !p->losses || !p->workspace || !aligned(p->workspace, 256) || !aligned(p->x, 16) || !aligned(p->w, 16) || p->x_stride % 8 != 0 ||
+      p->w_stride % 8 != 0 || p->x_stride < p->d || p->w_stride < p->d || !aligned(p->dx, 16) || !aligned(p->dw, 16) || (p->dbias != nullptr && p->bias == nullptr) ||
+      (what == NANGILA_CE_GRADIENTS && (!p->lse || !p->upstream)) || (what == NANGILA_CE_LOSSES && !p->lse))
+    return int(cudaErrorInvalidValue);
+  try {
+    return p->dtype == NANGILA_BF16 ? run<__nv_bfloat16>(*p, what, stream) : run<__half>(*p, what, stream);
+  } catch (...) {  // (the host's tables of kernels that were set up allocate)
+    return int(cudaErrorMemoryAllocation);
+  }
+}
+
+extern "C" int nangila_rescale(const NangilaRescaleParams* p, cudaStream_t stream) {
+  using namespace nangila;
+  if (!p || !p->factor) return int(cudaErrorInvalidValue);
+  rescale_kernel<<<148 * 4, 256, 0, stream>>>(*p);
+  return int(cudaGetLastError());
+}

@@ -99,7 +99,7 @@ def build_core(force: bool = False) -> Path:
 
 
 #: Kernels whose float32 results are documented as rounded like PyTorch's: no flushing of subnormal numbers (``--use_fast_math`` implies it).
-KEEP_SUBNORMALS = {"rms_norm", "rotary", "orthogonalize"}
+KEEP_SUBNORMALS = {"rms_norm", "rotary", "orthogonalize", "dropout", "embedding", "linear_ce"}
 
 
 def kernel_sources() -> list[Path]:
