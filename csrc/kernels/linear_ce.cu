@@ -53,8 +53,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kMostAbove = 60.0f * kLog2e;     // how far a logit may lie above a row's reference
 
-// kStats: the largest logit and the sum of exponentials of each row over half a tile's columns. kExp: E, and with `parts` the same sums. kScaled: alpha f_row D in 16 bits.
-// kSums, kAdded: D in fp32, written or added.
+// What becomes of a tile. kStats: the largest logit and the sum of exponentials of each row over half a tile's columns. kExp: E, and with `parts` the same sums. kScaled: alpha f_row D in
+// 16 bits. kSums, kAdded: D in fp32, written or added.
 enum Kind { kStats, kExp, kScaled, kSums, kAdded };
 
 // What is known of a group's rows when their tiles are made, and what comes out.
@@ -69,15 +69,25 @@ struct Rows {
   int64_t stride;
   int n, classes;
 };
-struct Product {
-  int M, N, K;          // D is M x N
-  int tiles_m, tiles_n, total;
-  int n_inner;          // neighbouring tiles share rows (else columns)
-  const float* alpha;
-  const float* factor;  // of D's rows; NULL: one
-};
 struct Maps {
   CUtensorMap a, b, out;
+};
+// One result of the gradients' products, M x N, its K cut into `split` parts of `slabs` slabs (the last may have fewer).
+struct Result {
+  int M, N, K;
+  int tiles_n, total;   // tiles along N; of all parts
+  int split, slabs, per; // per: tiles of a part
+  int wide;             // 0: alpha f_row D in 16 bits; 1: D in fp32; 2: added to what is there
+  const float* factor;  // of D's rows; NULL: one
+};
+struct Gradients {
+  Result x, w;          // dx = E w, dw = E^T x'
+  const float* alpha;
+  int extra;            // tiles of dw that a pair takes on top of the others' where it has a tile of dx less
+};
+struct GradientMaps {
+  CUtensorMap e_rows, w, out_x;      // dx
+  CUtensorMap e_columns, xs, out_w;  // dw
 };
 
 template <typename T>
@@ -97,18 +107,6 @@ __device__ __forceinline__ uint4* box_at(uint8_t* box, int row, int j) { return 
 struct TileAt {
   int m0, n0;
 };
-template <int SIDE>
-__device__ __forceinline__ TileAt tile_at(const Product& p, int i) {
-  int rb, cb;
-  if (p.n_inner) {
-    rb = i / p.tiles_n;
-    cb = i - rb * p.tiles_n;
-  } else {
-    cb = i / p.tiles_m;
-    rb = i - cb * p.tiles_m;
-  }
-  return {rb * SIDE, cb * SIDE};
-}
 
 // What a CTA's roles share, in shared memory.
 struct Shared {
@@ -149,8 +147,8 @@ __device__ __forceinline__ void init_barriers(const Shared& s) {
 
 // TMA of a tile's slabs, `i` of which have gone before: both CTAs of a pair, each its own halves; the bytes are counted where the products are issued.
 // False when a wait has run out.
-template <bool PAIR, bool A_MN, bool B_MN>
-__device__ __forceinline__ bool load_tile(const Shared& s, const Maps& maps, const TileAt& at, uint32_t rank, int slabs, int& i) {
+template <bool PAIR>
+__device__ __forceinline__ bool load_tile(const Shared& s, const CUtensorMap* a_map, const CUtensorMap* b_map, bool a_mn, bool b_mn, const TileAt& at, uint32_t rank, int slab0, int slabs, int& i) {
   const int row = at.m0 + int(rank) * kTileM, col = at.n0 + int(rank) * 128;
   for (int k = 0; k < slabs; ++k, ++i) {
     const int st = i % kStages;
@@ -160,20 +158,20 @@ __device__ __forceinline__ bool load_tile(const Shared& s, const Maps& maps, con
     }
     uint8_t* a = s.stages + st * kStageBytes;
     uint8_t* b = a + kOperandBytes;
-    const int k0 = k * kSlabK;
+    const int k0 = (slab0 + k) * kSlabK;
     if (rank == 0) mbar_arrive_expect_tx(&s.full[st], kStageBytes * (PAIR ? 2 : 1));
     const uint32_t bar = PAIR ? rank0_address(&s.full[st]) : smem_u32(&s.full[st]);
-    if (A_MN) {
-      tma_operand<PAIR>(a, &maps.a, row, k0, 0, bar);
-      tma_operand<PAIR>(a + 8192, &maps.a, row + 64, k0, 0, bar);
+    if (a_mn) {
+      tma_operand<PAIR>(a, a_map, row, k0, 0, bar);
+      tma_operand<PAIR>(a + 8192, a_map, row + 64, k0, 0, bar);
     } else {
-      tma_operand<PAIR>(a, &maps.a, k0, row, 0, bar);
+      tma_operand<PAIR>(a, a_map, k0, row, 0, bar);
     }
-    if (B_MN) {
-      tma_operand<PAIR>(b, &maps.b, col, k0, 0, bar);
-      tma_operand<PAIR>(b + 8192, &maps.b, col + 64, k0, 0, bar);
+    if (b_mn) {
+      tma_operand<PAIR>(b, b_map, col, k0, 0, bar);
+      tma_operand<PAIR>(b + 8192, b_map, col + 64, k0, 0, bar);
     } else {
-      tma_operand<PAIR>(b, &maps.b, k0, col, 0, bar);
+      tma_operand<PAIR>(b, b_map, k0, col, 0, bar);
     }
   }
   return true;
@@ -187,10 +185,10 @@ __device__ __forceinline__ void drain_loads(const Shared& s, uint32_t rank, int 
   }
 }
 // The products of a tile, the n-th, into its accumulator. False when a wait has run out.
-template <bool PAIR, bool BF16, bool A_MN, bool B_MN>
-__device__ __forceinline__ bool multiply_tile(const Shared& s, uint32_t tmem, int slabs, int n, int& i) {
+template <bool PAIR, bool BF16>
+__device__ __forceinline__ bool multiply_tile(const Shared& s, uint32_t tmem, bool a_mn, bool b_mn, int slabs, int n, int& i) {
   constexpr int kSide = PAIR ? 256 : 128;
-  constexpr uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(kSide >> 3) << 17) | (uint32_t(kSide >> 4) << 24);
+  const uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | (uint32_t(kSide >> 3) << 17) | (uint32_t(kSide >> 4) << 24);
   const int acc = n & 1;
   if (n >= 2 && !mbar_wait(&s.acc_empty[acc], uint32_t((n / 2 - 1) & 1), kTimeoutNs)) return false;
   tc_fence_after_sync();
@@ -203,8 +201,8 @@ __device__ __forceinline__ bool multiply_tile(const Shared& s, uint32_t tmem, in
 #pragma unroll
     for (int kk = 0; kk < kSlabK / 16; ++kk) {
       // K-major: 16 elements along K are 32 bytes of a swizzle row; MN-major: 16 K-rows are two groups of eight rows of 128 bytes
-      const uint64_t ad = A_MN ? make_smem_desc(a + kk * 2048, 8192, 1024) : make_smem_desc(a + kk * 32, 16, 1024);
-      const uint64_t bd = B_MN ? make_smem_desc(b + kk * 2048, 8192, 1024) : make_smem_desc(b + kk * 32, 16, 1024);
+      const uint64_t ad = a_mn ? make_smem_desc(a + kk * 2048, 8192, 1024) : make_smem_desc(a + kk * 32, 16, 1024);
+      const uint64_t bd = b_mn ? make_smem_desc(b + kk * 2048, 8192, 1024) : make_smem_desc(b + kk * 32, 16, 1024);
       if (PAIR) umma_f16_pair(d, ad, bd, idesc, (k > 0 || kk > 0) ? 1u : 0u);
       else umma_f16(d, ad, bd, idesc, (k > 0 || kk > 0) ? 1u : 0u);
     }
@@ -223,160 +221,222 @@ __device__ __forceinline__ void drain_products(const Shared& s) {
   mbar_wait(s.drained, 0, kTimeoutNs);
 }
 
-// The n-th tile's accumulator taken to where it belongs, by one of the epilogue's warps; `used`: how many slots it has filled so far.
+__device__ __forceinline__ void nan16(float (&v)[16]) {
+#pragma unroll
+  for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(0x7fc00000u);
+}
+// The wait of an epilogue's warp for the n-th accumulator; false if it, or somebody's, has run out.
+__device__ __forceinline__ bool accumulator_here(const Shared& s, int n) {
+  const bool ok = *s.failed == 0 && mbar_wait(&s.acc_full[n & 1], uint32_t((n / 2) & 1), kTimeoutNs);
+  const bool all = __all_sync(0xffffffffu, ok);
+  if (!all) *s.failed = 1;
+  tc_fence_after_sync();
+  return all;
+}
+template <bool PAIR>
+__device__ __forceinline__ void accumulator_read(const Shared& s, int n) {
+  tc_fence_before_sync();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive_at((PAIR ? rank0_address(&s.acc_empty[0]) : smem_u32(&s.acc_empty[0])) + uint32_t(n & 1) * 8);
+}
+// A slot of this warp's that nothing goes out of any more, and its way out; `used`: how many have been filled.
+__device__ __forceinline__ uint8_t* free_slot(const Shared& s, uint32_t used) {
+  if ((threadIdx.x & 31) == 0) bulk_wait_read_but_one();
+  __syncwarp();
+  return s.slots + (((threadIdx.x >> 5) - 2) * kSlots + used % kSlots) * kSlotBytes;
+}
+__device__ __forceinline__ void send_slot(const uint8_t* slot, const CUtensorMap* map, int col, int row, int part, bool add) {
+  fence_async_proxy();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) {
+    if (add) tma_add_3d(map, slot, col, row, part);
+    else tma_store_3d(map, slot, col, row, part);
+    bulk_commit();
+  }
+}
+
+// A tile of logits, the n-th, by one of the epilogue's warps.
 template <typename T, int KIND, bool PAIR>
-__device__ __forceinline__ void finish_tile(const Shared& s, uint32_t tmem, const Product& p, const Rows& rows, const Maps& maps, const TileAt& at, uint32_t rank, int n, uint32_t& used) {
+__device__ __forceinline__ void finish_logits(const Shared& s, uint32_t tmem, const Rows& rows, const CUtensorMap* out, const TileAt& at, uint32_t rank, int n, uint32_t& used) {
   constexpr int kSide = PAIR ? 256 : 128, kHalf = kSide / 2;
-  constexpr bool kStores = KIND != kStats;
-  constexpr int kChunk = KIND == kSums || KIND == kAdded ? 32 : 64;  // columns of a slot
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quad = warp & 3, half = (warp - 2) >> 2;  // the lanes of tensor memory that this warp may read; its half of the columns
-  const int acc = n & 1;
   const int row0 = at.m0 + int(rank) * kTileM + quad * 32, row = row0 + lane, col0 = at.n0 + half * kHalf;
-  const bool mine = row0 < p.M && col0 < p.N;
+  const bool mine = row0 < rows.n && col0 < rows.classes;
   // of this lane's row
   int target = -1;
-  bool dead = false;
+  bool dead = true;
   float ref = 0.0f, mul = 1.0f, value = 0.0f;
-  if constexpr (KIND == kStats || KIND == kExp) {
-    if (mine && row < rows.n) {
-      const int64_t t = rows.targets[row];
-      dead = t < 0 || t >= rows.classes;
-      target = dead ? -1 : int(t);
-      if (KIND == kExp) {
-        ref = rows.ref[row];
-        if (rows.mul != nullptr) mul = rows.mul[row], value = rows.value[row];
-      }
-    } else {
-      dead = true;
+  if (mine && row < rows.n) {
+    const int64_t t = rows.targets[row];
+    dead = t < 0 || t >= rows.classes;
+    target = dead ? -1 : int(t);
+    if (KIND == kExp) {
+      ref = rows.ref[row];
+      if (rows.mul != nullptr) mul = rows.mul[row], value = rows.value[row];
     }
   }
-  float alpha = 1.0f;
-  if constexpr (KIND == kScaled) {
-    alpha = *p.alpha;
-    if (p.factor != nullptr && mine && row < p.M) {
-      const float f = p.factor[row];
-      dead = f == 0.0f;
-      alpha *= f;
-    }
-  }
-  bool ok = *s.failed == 0 && mbar_wait(&s.acc_full[acc], uint32_t((n / 2) & 1), kTimeoutNs);
-  ok = __all_sync(0xffffffffu, ok);
-  if (!ok) *s.failed = 1;
-  tc_fence_after_sync();
+  const bool ok = accumulator_here(s, n);
   float most = -INFINITY, sum = 0.0f;
   if (mine) {
 #pragma unroll 1
-    for (int c = 0; c < kHalf && col0 + c < p.N; c += kChunk) {
-      uint8_t* slot = s.slots + ((warp - 2) * kSlots + int(used % kSlots)) * kSlotBytes;
-      if (kStores) {
-        if (lane == 0) bulk_wait_read_but_one();  // the slot's last store
-        __syncwarp();
-      }
+    for (int c = 0; c < kHalf && col0 + c < rows.classes; c += 64) {
+      uint8_t* slot = KIND == kExp ? free_slot(s, used) : nullptr;
 #pragma unroll
-      for (int g = 0; g < kChunk / 16; ++g) {
+      for (int g = 0; g < 4; ++g) {
         float v[16];
         const int first = col0 + c + g * 16;
-        tmem_ld_32x32b_x16(tmem + (uint32_t(quad * 32) << 16) + uint32_t(acc * kSide + half * kHalf + c + g * 16), v);
-        if (!ok) {
+        tmem_ld_32x32b_x16(tmem + (uint32_t(quad * 32) << 16) + uint32_t((n & 1) * kSide + half * kHalf + c + g * 16), v);
+        if (!ok) nan16(v);
+        if (rows.bias != nullptr) {
 #pragma unroll
-          for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(0x7fc00000u);
-        }
-        if constexpr (KIND == kStats || KIND == kExp) {
-          if (rows.bias != nullptr) {
-#pragma unroll
-            for (int k = 0; k < 16; k += 4) {
-              const float4 b = *reinterpret_cast<const float4*>(rows.bias + first + k);
-              v[k] += b.x, v[k + 1] += b.y, v[k + 2] += b.z, v[k + 3] += b.w;
-            }
+          for (int k = 0; k < 16; k += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(rows.bias + first + k);
+            v[k] += b.x, v[k + 1] += b.y, v[k + 2] += b.z, v[k + 3] += b.w;
           }
-          const bool edge = first + 16 > p.N, here = target >= first && target < first + 16;
+        }
+        const bool edge = first + 16 > rows.classes, here = target >= first && target < first + 16;
 #pragma unroll
-          for (int k = 0; k < 16; ++k) v[k] *= kLog2e;
-          if (edge || __any_sync(0xffffffffu, here)) {  // what is no class, and the target, stay out of the sums
+        for (int k = 0; k < 16; ++k) v[k] *= kLog2e;
+        if (edge || __any_sync(0xffffffffu, here)) {  // what is no class, and the target, stay out of the sums
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            if (first + k >= rows.classes || first + k == target) v[k] = -INFINITY;
+        }
+        float top = v[0];
+#pragma unroll
+        for (int k = 1; k < 16; ++k) top = fmaxf(top, v[k]);
+        if constexpr (KIND == kStats) {
+          const float now = fmaxf(most, top), base = now == -INFINITY ? 0.0f : now;
+          sum *= exp2_fast(most - base);
+          most = now;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) sum += exp2_fast(v[k] - base);
+        } else {
+          most = fmaxf(most, top);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            v[k] = exp2_fast(v[k] - ref);
+            sum += v[k];
+            v[k] *= mul;
+          }
+          if (__any_sync(0xffffffffu, here)) {
 #pragma unroll
             for (int k = 0; k < 16; ++k)
-              if (first + k >= p.N || first + k == target) v[k] = -INFINITY;
+              if (first + k == target) v[k] = value;
           }
-          float top = v[0];
-#pragma unroll
-          for (int k = 1; k < 16; ++k) top = fmaxf(top, v[k]);
-          if constexpr (KIND == kStats) {
-            const float now = fmaxf(most, top), base = now == -INFINITY ? 0.0f : now;
-            sum *= exp2_fast(most - base);
-            most = now;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) sum += exp2_fast(v[k] - base);
-          } else {
-            most = fmaxf(most, top);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              v[k] = exp2_fast(v[k] - ref);
-              sum += v[k];
-              v[k] *= mul;
-            }
-            if (__any_sync(0xffffffffu, here)) {
-#pragma unroll
-              for (int k = 0; k < 16; ++k)
-                if (first + k == target) v[k] = value;
-            }
-#pragma unroll
-            for (int k = 0; k < 16; ++k) v[k] = dead ? 0.0f : v[k];
-          }
-        }
-        if constexpr (KIND == kScaled) {
-#pragma unroll
-          for (int k = 0; k < 16; ++k) v[k] = dead ? 0.0f : v[k] * alpha;
-        }
-        if constexpr (KIND == kExp || KIND == kScaled) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float w[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = v[8 * e + k];
+            for (int k = 0; k < 8; ++k) w[k] = dead ? 0.0f : v[8 * e + k];
             *box_at(slot, lane, 2 * g + e) = pack16<T>(w);
           }
         }
-        if constexpr (KIND == kSums || KIND == kAdded) {
+      }
+      if (KIND == kExp) {
+        send_slot(slot, out, col0 + c, row0, 0, false);
+        ++used;
+      }
+    }
+  }
+  accumulator_read<PAIR>(s, n);
+  if (mine && row < rows.n && rows.parts != nullptr) rows.parts[int64_t(col0 / kHalf) * rows.stride + row] = make_float2(most, sum);
+}
+
+// A tile of a gradient, the n-th, by one of the epilogue's warps: `wide` 0 in 16 bits, each row times `scale`; else in fp32, written (1) or added (2), as part `part`.
+template <typename T>
+__device__ __forceinline__ void finish_result(const Shared& s, uint32_t tmem, const Result& r, const float* alpha_at, const CUtensorMap* out, const TileAt& at, int part, uint32_t rank, int n,
+                                              uint32_t& used) {
+  constexpr int kSide = 256, kHalf = 128;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int quad = warp & 3, half = (warp - 2) >> 2;
+  const int row0 = at.m0 + int(rank) * kTileM + quad * 32, row = row0 + lane, col0 = at.n0 + half * kHalf;
+  const bool mine = row0 < r.M && col0 < r.N;
+  float scale = 1.0f;
+  bool dead = false;  // a row that adds nothing gets nothing either, whatever the rest holds
+  if (r.wide == 0) {
+    scale = *alpha_at;
+    if (r.factor != nullptr && mine && row < r.M) {
+      const float f = r.factor[row];
+      dead = f == 0.0f;
+      scale *= f;
+    }
+  }
+  const bool ok = accumulator_here(s, n);
+  if (mine) {
+    const int chunk = r.wide != 0 ? 32 : 64;  // columns of a slot
+#pragma unroll 1
+    for (int c = 0; c < kHalf && col0 + c < r.N; c += chunk) {
+      uint8_t* slot = free_slot(s, used);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        if (g * 16 >= chunk) break;
+        float v[16];
+        tmem_ld_32x32b_x16(tmem + (uint32_t(quad * 32) << 16) + uint32_t((n & 1) * kSide + half * kHalf + c + g * 16), v);
+        if (!ok) nan16(v);
+        if (r.wide == 0) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = dead ? 0.0f : v[8 * e + k] * scale;
+            *box_at(slot, lane, 2 * g + e) = pack16<T>(w);
+          }
+        } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             *box_at(slot, lane, 4 * g + e) = make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3]));
         }
       }
-      if (kStores) {
-        fence_async_proxy();
-        __syncwarp();
-        if (lane == 0) {
-          if (KIND == kAdded) tma_add_3d(&maps.out, slot, col0 + c, row0, 0);
-          else tma_store_3d(&maps.out, slot, col0 + c, row0, 0);
-          bulk_commit();
-        }
-        ++used;
-      }
+      send_slot(slot, out, col0 + c, row0, part, r.wide == 2);
+      ++used;
     }
   }
+  accumulator_read<true>(s, n);
+}
+
+// What all roles of a kernel of products begin and end with.
+template <bool PAIR>
+__device__ __forceinline__ uint32_t products_begin(const Shared& s) {
+  constexpr int kSide = PAIR ? 256 : 128;
+  if (threadIdx.x == 0) init_barriers<PAIR>(s);
+  if (threadIdx.x >> 5 == 1) {
+    if (PAIR) tmem_alloc_pair(s.tmem_slot, 2 * kSide);
+    else tmem_alloc(s.tmem_slot, 2 * kSide);
+  }
   tc_fence_before_sync();
-  __syncwarp();
-  if (lane == 0) mbar_arrive_at((PAIR ? rank0_address(&s.acc_empty[0]) : smem_u32(&s.acc_empty[0])) + uint32_t(acc) * 8);
-  if constexpr (KIND == kStats || KIND == kExp) {
-    if (mine && row < rows.n && rows.parts != nullptr) rows.parts[int64_t(col0 / kHalf) * rows.stride + row] = make_float2(most, sum);
+  __syncthreads();
+  if (PAIR) cluster_sync();  // the other CTA's barriers exist from here on
+  tc_fence_after_sync();
+  return *s.tmem_slot;
+}
+template <bool PAIR>
+__device__ __forceinline__ void products_end(uint32_t tmem) {
+  constexpr int kSide = PAIR ? 256 : 128;
+  tc_fence_before_sync();
+  __syncthreads();
+  if (PAIR) cluster_sync();  // neither CTA's barriers and tensor memory go while the other may still use them
+  if (threadIdx.x >> 5 == 1) {
+    if (PAIR) tmem_dealloc_pair(tmem, 2 * kSide);
+    else tmem_dealloc(tmem, 2 * kSide);
   }
 }
 
-// D = A B, walked over tile by tile by CTAs that stay (PAIR: pairs of CTAs that share the tensor cores' work on 256 x 256, each with its 128 rows of A, half of
-// B's columns, and 128 rows of the result; else one CTA and 128 x 128). A_MN / B_MN: the operand lies with its rows (columns of B) adjacent in memory, not its K. The accumulators of
-// two tiles share tensor memory: the epilogue of one runs under the products of the next.
+// z = x w^T, walked over tile by tile by CTAs that stay (PAIR: pairs of CTAs that share the tensor cores' work on 256 x 256, each with its 128 rows of x, half of
+// the classes, and 128 rows of the result; else one CTA and 128 x 128). The accumulators of two tiles share tensor memory: the epilogue of one runs under the products of the next.
+// Neighbouring tiles share classes: w is read once, x stays in L2.
 // A wait that runs out makes every result of this CTA from there on not a number.
-template <typename T, int KIND, bool A_MN, bool B_MN, bool PAIR>
-__global__ void __launch_bounds__(kThreads, 1) ce_product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, const __grid_constant__ Rows rows) {
+template <typename T, int KIND, bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1) ce_logits_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Rows rows, int tiles_m, int total, int slabs) {
   constexpr int kSide = PAIR ? 256 : 128;
   extern __shared__ uint8_t smem_raw[];
   const Shared s = shared_parts(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int slabs = (p.K + kSlabK - 1) / kSlabK;
   const uint32_t rank = PAIR ? cluster_rank() : 0u;   // 0: the CTA that issues the pair's products
   const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, step = PAIR ? gridDim.x / 2 : gridDim.x;
-  // rows to be formed again: their tiles alone (eight groups of 32 rows in a pair's tile, four in a CTA's)
+  auto tile_at = [&](int i) { return TileAt{i % tiles_m * kSide, i / tiles_m * kSide}; };
+  // rows to be formed again: their tiles alone
   const bool some = KIND == kExp && rows.again != nullptr;
   if (some) {
     follow();
@@ -394,32 +454,22 @@ __global__ void __launch_bounds__(kThreads, 1) ce_product_kernel(const __grid_co
       return false;
     }
   };
-
   if (threadIdx.x == 0) {
-    init_barriers<PAIR>(s);
     prefetch_tensormap(&maps.a);
     prefetch_tensormap(&maps.b);
+    if (KIND == kExp) prefetch_tensormap(&maps.out);
   }
-  if (KIND != kStats && threadIdx.x == 64) prefetch_tensormap(&maps.out);
-  if (warp == 1) {
-    if (PAIR) tmem_alloc_pair(s.tmem_slot, 2 * kSide);
-    else tmem_alloc(s.tmem_slot, 2 * kSide);
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  if (PAIR) cluster_sync();  // the other CTA's barriers exist from here on
-  tc_fence_after_sync();
-  const uint32_t tmem = *s.tmem_slot;
+  const uint32_t tmem = products_begin<PAIR>(s);
   may_follow();
   follow();
 
   if (warp == 0) {
     if (lane == 0) {
       int i = 0;
-      for (int tile = first; tile < p.total; tile += step) {
-        const TileAt at = tile_at<kSide>(p, tile);
+      for (int tile = first; tile < total; tile += step) {
+        const TileAt at = tile_at(tile);
         if (skip(at)) continue;
-        if (!load_tile<PAIR, A_MN, B_MN>(s, maps, at, rank, slabs, i)) break;
+        if (!load_tile<PAIR>(s, &maps.a, &maps.b, false, false, at, rank, 0, slabs, i)) break;
       }
       drain_loads(s, rank, i);
     }
@@ -427,9 +477,9 @@ __global__ void __launch_bounds__(kThreads, 1) ce_product_kernel(const __grid_co
     if (lane == 0 && rank == 0) {
       int i = 0, n = 0;
       bool ok = true;
-      for (int tile = first; tile < p.total && ok; tile += step) {
-        if (skip(tile_at<kSide>(p, tile))) continue;
-        ok = multiply_tile<PAIR, std::is_same<T, __nv_bfloat16>::value, A_MN, B_MN>(s, tmem, slabs, n, i);
+      for (int tile = first; tile < total && ok; tile += step) {
+        if (skip(tile_at(tile))) continue;
+        ok = multiply_tile<PAIR, std::is_same<T, __nv_bfloat16>::value>(s, tmem, false, false, slabs, n, i);
         ++n;
       }
       if (!ok) drain_products<PAIR>(s);
@@ -437,46 +487,142 @@ __global__ void __launch_bounds__(kThreads, 1) ce_product_kernel(const __grid_co
   } else {
     int n = 0;
     uint32_t used = 0;
-    for (int tile = first; tile < p.total; tile += step) {
-      const TileAt at = tile_at<kSide>(p, tile);
+    for (int tile = first; tile < total; tile += step) {
+      const TileAt at = tile_at(tile);
       if (skip(at)) continue;
-      finish_tile<T, KIND, PAIR>(s, tmem, p, rows, maps, at, rank, n, used);
+      finish_logits<T, KIND, PAIR>(s, tmem, rows, &maps.out, at, rank, n, used);
       ++n;
     }
     if (lane == 0) bulk_wait_read();  // the stores have left shared memory; the end of the kernel is what others wait for
   }
-  tc_fence_before_sync();
-  __syncthreads();
-  if (PAIR) cluster_sync();  // neither CTA's barriers and tensor memory go while the other may still use them
-  if (warp == 1) {
-    if (PAIR) tmem_dealloc_pair(tmem, 2 * kSide);
-    else tmem_dealloc(tmem, 2 * kSide);
+  products_end<PAIR>(tmem);
+}
+
+// dx = E w and dw = E^T x' in one launch of pairs of CTAs. A tile of dx has all classes as its K, one of dw all tokens of the group, and there may be fewer tiles of dx than pairs: each
+// pair takes its share of dx's tiles first, and where it has one less than others, tiles of dw for it. So both end together. dx's K is cut in parts where a
+// single tile would take longer than that.
+struct Task {
+  bool x;
+  TileAt at;
+  int part, slab0, slabs;
+};
+__device__ __forceinline__ bool task_of(const Gradients& g, int pair, int pairs, int k, Task& t) {
+  const int more = g.x.total % pairs;                      // pairs that have a tile of dx more than the others
+  const int mine = g.x.total / pairs + (pair < more ? 1 : 0);
+  int i;
+  t.x = k < mine;
+  if (t.x) {
+    i = k * pairs + pair;
+  } else {
+    const int j = k - mine, ahead = more > 0 ? g.extra : 0;  // tiles of dw of the pairs without
+    if (pair >= more && j < ahead) i = j * (pairs - more) + pair - more;
+    else i = ahead * (pairs - more) + (pair >= more ? j - ahead : j) * pairs + pair;
+    if (i >= g.w.total) return false;
   }
+  const Result& r = t.x ? g.x : g.w;
+  t.part = i / r.per;
+  i -= t.part * r.per;
+  t.slab0 = t.part * r.slabs;
+  t.slabs = min(r.slabs, (r.K + kSlabK - 1) / kSlabK - t.slab0);
+  t.at.m0 = i / r.tiles_n * 256;
+  t.at.n0 = i % r.tiles_n * 256;
+  return true;
+}
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) ce_gradients_kernel(const __grid_constant__ GradientMaps maps, const __grid_constant__ Gradients g) {
+  extern __shared__ uint8_t smem_raw[];
+  const Shared s = shared_parts(smem_raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&maps.e_rows);
+    prefetch_tensormap(&maps.w);
+    prefetch_tensormap(&maps.e_columns);
+    prefetch_tensormap(&maps.xs);
+  }
+  const uint32_t tmem = products_begin<true>(s);
+  may_follow();
+  follow();
+  Task t;
+  if (warp == 0) {
+    if (lane == 0) {
+      int i = 0;
+      for (int k = 0; task_of(g, pair, pairs, k, t); ++k)
+        if (!load_tile<true>(s, t.x ? &maps.e_rows : &maps.e_columns, t.x ? &maps.w : &maps.xs, !t.x, true, t.at, rank, t.slab0, t.slabs, i)) break;
+      drain_loads(s, rank, i);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      int i = 0;
+      bool ok = true;
+      for (int k = 0; ok && task_of(g, pair, pairs, k, t); ++k) ok = multiply_tile<true, std::is_same<T, __nv_bfloat16>::value>(s, tmem, !t.x, true, t.slabs, k, i);
+      if (!ok) drain_products<true>(s);
+    }
+  } else {
+    uint32_t used = 0;
+    for (int k = 0; task_of(g, pair, pairs, k, t); ++k)
+      finish_result<T>(s, tmem, t.x ? g.x : g.w, g.alpha, t.x ? &maps.out_x : &maps.out_w, t.at, t.part, rank, k, used);
+    if (lane == 0) bulk_wait_read();
+  }
+  products_end<true>(tmem);
 }
 
 // ---- what goes before, between and behind the products -----------------------------------------------------------------------
 
 constexpr int kBeginT = 256;
-constexpr int kRowsT = 256;
-constexpr int kRowsAtOnce = 32;   // rows of a CTA
+constexpr int kRowsT = 1024;
+constexpr int kRowsAtOnce = 32;   // rows of a CTA, one for each lane, and one for each warp
+constexpr int kWeightsT = 256;
 
 // Of the whole call. alpha: what G's rows are multiplied by in the end; unit: the largest weight of a row, by which the weights are divided.
 struct Scales {
-  float alpha, unit, count;
+  float alpha, unit;
 };
 
 struct Begin {
   NangilaLinearCeParams p;
   int what;
-  float* zt;      // [n] the targets' logits
+  float *zt, *ref; // [n] the targets' logits, and as references; NULL: not wanted
   float* bias;    // padded to whole tiles
   int bias_count;
   Scales* scales;
   float e_scale;  // power of two by which E is larger
 };
-template <typename T>
 __device__ __forceinline__ float bias_value(const void* b, int dtype, int i) {
   return dtype == NANGILA_F32 ? static_cast<const float*>(b)[i] : dtype == NANGILA_F16 ? __half2float(static_cast<const __half*>(b)[i]) : __bfloat162float(static_cast<const __nv_bfloat16*>(b)[i]);
+}
+// Row i's logit at its target, by a warp; 0 where that is no class or ignored.
+template <typename T>
+__device__ __forceinline__ float target_logit(const NangilaLinearCeParams& p, int64_t i) {
+  const int64_t t = p.targets[i];
+  if (t < 0 || t >= p.classes || t == p.ignore) return 0.0f;
+  const int lane = threadIdx.x & 31;
+  const T* x = static_cast<const T*>(p.x) + i * p.x_stride;
+  const T* w = static_cast<const T*>(p.w) + t * p.w_stride;
+  float z = 0.0f;
+  constexpr int kAtOnce = 4;
+  for (int c0 = lane * 8; c0 < p.d; c0 += 256 * kAtOnce) {
+    dev::Raw8<T> rx[kAtOnce], rw[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (c0 + 256 * j >= p.d) continue;
+      dev::fetch(x + c0 + 256 * j, rx[j]);
+      dev::fetch(w + c0 + 256 * j, rw[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (c0 + 256 * j >= p.d) continue;
+      float u[8], v[8];
+      dev::unpack(rx[j], u);
+      dev::unpack(rw[j], v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) z = __fmaf_rn(u[k], v[k], z);
+    }
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) z += __shfl_xor_sync(0xffffffffu, z, off);
+  return z + (p.bias != nullptr ? bias_value(p.bias, p.bias_dtype, int(t)) : 0.0f);
 }
 // CTA 0: how many targets are not ignored, the largest weight, and the factors that follow. The others: the targets' logits, a warp for each row; the bias in fp32.
 template <typename T>
@@ -517,36 +663,19 @@ __global__ void __launch_bounds__(kBeginT) ce_begin_kernel(const __grid_constant
       if (p.mean) u = count > 0 ? u / float(count) : 0.0f;
       a.scales->alpha = u / a.e_scale;
       a.scales->unit = p.upstream_rows ? top : 1.0f;
-      a.scales->count = float(count);
     }
     return;
   }
   const int64_t thread = int64_t(blockIdx.x - 1) * kBeginT + threadIdx.x, threads = int64_t(gridDim.x - 1) * kBeginT;
   if (p.bias != nullptr)
-    for (int64_t i = thread; i < a.bias_count; i += threads) a.bias[i] = i < p.classes ? bias_value<T>(p.bias, p.bias_dtype, int(i)) : 0.0f;
-  if (a.what == NANGILA_CE_GRADIENTS) return;
+    for (int64_t i = thread; i < a.bias_count; i += threads) a.bias[i] = i < p.classes ? bias_value(p.bias, p.bias_dtype, int(i)) : 0.0f;
+  if (a.zt == nullptr) return;
   for (int64_t i = thread / 32; i < p.n; i += threads / 32) {
-    const int64_t t = p.targets[i];
-    if (t < 0 || t >= p.classes || t == p.ignore) {
-      if (lane == 0) a.zt[i] = 0.0f;
-      continue;
+    const float z = target_logit<T>(p, i);
+    if (lane == 0) {
+      a.zt[i] = z;
+      a.ref[i] = z * kLog2e;
     }
-    const T* x = static_cast<const T*>(p.x) + i * p.x_stride;
-    const T* w = static_cast<const T*>(p.w) + t * p.w_stride;
-    float z = 0.0f;
-    for (int c = lane * 8; c < p.d; c += 256) {
-      dev::Raw8<T> rx, rw;
-      dev::fetch(x + c, rx);
-      dev::fetch(w + c, rw);
-      float u[8], v[8];
-      dev::unpack(rx, u);
-      dev::unpack(rw, v);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) z = __fmaf_rn(u[k], v[k], z);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) z += __shfl_xor_sync(0xffffffffu, z, off);
-    if (lane == 0) a.zt[i] = z + (p.bias != nullptr ? bias_value<T>(p.bias, p.bias_dtype, int(t)) : 0.0f);
   }
 }
 
@@ -565,13 +694,19 @@ struct Group {
   const Scales* scales;
   float e_scale;
 };
-// Losses and lse of the joined sums; with E: also the element at the target, the rows' factors and scaled rows of x. pass 0: NANGILA_CE_LOSSES; 1, 2: NANGILA_CE_BOTH, for all rows
+// The factor with which a row's element at the target, as it was rounded, comes out as `value`; where that is too small to tell, the factor it had. (The target's element is half
+// of a row's gradient, and often all that a class gets from it: its rounding goes into the factor, where it moves each of the others by as much as
+// their own roundings do. The encoder's loss: dx 1.4 -> 1.1 times the error that the results' rounding alone has, dw 1.7 -> 1.4.)
+__device__ __forceinline__ float folded(float value, float rounded, float factor) {
+  return fabsf(rounded) > 1e-4f && fabsf(rounded) < 1e30f ? value / rounded : factor;
+}
+// Losses and lse of the joined sums; with E: also the element at the target and the rows' factors. pass 0: NANGILA_CE_LOSSES; 1, 2: NANGILA_CE_BOTH, for all rows
 // and for those of tiles that were formed again.
 template <typename T>
 __global__ void __launch_bounds__(kRowsT) ce_rows_kernel(const __grid_constant__ Group a, int pass, int tile_rows) {
   constexpr int kWarps = kRowsT / 32;
   __shared__ float2 joined[kWarps][kRowsAtOnce];
-  __shared__ float factors[kRowsAtOnce];
+  __shared__ float logit[kRowsAtOnce];
   follow();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row0 = blockIdx.x * kRowsAtOnce, row = row0 + lane;
@@ -583,9 +718,14 @@ __global__ void __launch_bounds__(kRowsT) ce_rows_kernel(const __grid_constant__
     if (!any) return;
   }
   const bool here = row < a.n;
+  if (pass == 0 && row0 + warp < a.n) {
+    const float z = target_logit<T>(a.p, a.row0 + row0 + warp);
+    if (lane == 0) logit[warp] = z;
+  }
   const float ref = pass != 0 && here ? a.ref[row] : 0.0f;
   float most = -INFINITY, sum = 0.0f;
   if (here) {
+#pragma unroll 8
     for (int i = warp; i < a.parts_count; i += kWarps) {
       const float2 v = a.parts[int64_t(i) * a.stride + row];
       if (pass == 0) {
@@ -617,7 +757,7 @@ __global__ void __launch_bounds__(kRowsT) ce_rows_kernel(const __grid_constant__
     if (here) {
       const int64_t i = a.row0 + row, t = a.p.targets[i];
       const bool ignored = t == a.p.ignore, outside = !ignored && (t < 0 || t >= a.p.classes);
-      const float zt2 = a.zt[row] * kLog2e;
+      const float zt2 = (pass == 0 ? logit[lane] : a.zt[row]) * kLog2e;
       float loss, lse2;
       if (pass == 0) {
         // sum of exp2(z - most) over the others; the target's own on top
@@ -632,7 +772,11 @@ __global__ void __launch_bounds__(kRowsT) ce_rows_kernel(const __grid_constant__
         lse2 = ref + log2f(whole);
         loss = ref == zt2 ? log1pf(sum) : (ref - zt2) * kLn2 + logf(whole);
         if (above) a.ref[row] = most;  // (more than z_t: the largest of the row)
-        if (!ignored && !outside && a.e != nullptr) static_cast<T*>(a.e)[int64_t(row) * a.e_stride + t] = dev::Vec16<T>::from_float(-sum);
+        if (!ignored && !outside && a.e != nullptr) {
+          const T element = dev::Vec16<T>::from_float(-sum);
+          static_cast<T*>(a.e)[int64_t(row) * a.e_stride + t] = element;
+          factor = folded(sum / whole, -dev::Vec16<T>::to_float(element), factor);
+        }
       }
       if (ignored || outside) {
         loss = ignored ? 0.0f : __uint_as_float(0x7fc00000u);
@@ -642,40 +786,35 @@ __global__ void __launch_bounds__(kRowsT) ce_rows_kernel(const __grid_constant__
       if (a.p.lse != nullptr) a.p.lse[i] = lse2 * kLn2;
       if (a.factor != nullptr) a.factor[row] = factor;
     }
-    if (pass != 0) {
-      factors[lane] = factor;
+    if (pass == 1) {
       const bool any = __any_sync(0xffffffffu, above);
-      if (pass == 1 && lane == 0) a.again[blockIdx.x] = any ? 1 : 0;
-    }
-  }
-  if (pass == 0 || a.xs == nullptr) return;
-  __syncthreads();
-  for (int r = warp; r < kRowsAtOnce && row0 + r < a.n; r += kWarps) {
-    const float f = factors[r];
-    const T* from = static_cast<const T*>(a.p.x) + (a.row0 + row0 + r) * a.p.x_stride;
-    T* to = static_cast<T*>(a.xs) + int64_t(row0 + r) * a.p.d;
-    for (int c = lane * 8; c < a.p.d; c += 256) {
-      dev::Raw8<T> raw;
-      dev::fetch(from + c, raw);
-      float v[8];
-      dev::unpack(raw, v);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = f == 0.0f ? 0.0f : v[k] * f;
-      dev::pack(v, raw);
-      dev::put(to + c, raw);
+      if (lane == 0) a.again[blockIdx.x] = any ? 1 : 0;
     }
   }
 }
-// NANGILA_CE_BOTH: the references before the tiles are made.
-__global__ void ce_refs_kernel(const float* zt, float* ref, int n) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i < n) ref[i] = zt[i] * kLog2e;
+// NANGILA_CE_BOTH: the rows of x times their factors, as dw's product takes them.
+template <typename T>
+__global__ void __launch_bounds__(kWeightsT) ce_scale_kernel(const __grid_constant__ Group a) {
+  follow();
+  const int per = a.p.d / 8;
+  for (int64_t i = int64_t(blockIdx.x) * kWeightsT + threadIdx.x; i < int64_t(a.n) * per; i += int64_t(gridDim.x) * kWeightsT) {
+    const int row = int(i / per), c = int(i - int64_t(row) * per) * 8;
+    const float f = a.factor[row];
+    dev::Raw8<T> raw;
+    dev::fetch(static_cast<const T*>(a.p.x) + (a.row0 + row) * a.p.x_stride + c, raw);
+    float v[8];
+    dev::unpack(raw, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = f == 0.0f ? 0.0f : v[k] * f;
+    dev::pack(v, raw);
+    dev::put(static_cast<T*>(a.xs) + i * 8, raw);
+  }
 }
 // NANGILA_CE_GRADIENTS: what the tiles' epilogue takes of each row, and the rows of x without those that add nothing.
 template <typename T>
-__global__ void __launch_bounds__(kRowsT) ce_weights_kernel(const __grid_constant__ Group a) {
+__global__ void __launch_bounds__(kWeightsT) ce_weights_kernel(const __grid_constant__ Group a) {
   const int lane = threadIdx.x & 31;
-  const int row = (blockIdx.x * kRowsT + threadIdx.x) >> 5;
+  const int row = (blockIdx.x * kWeightsT + threadIdx.x) >> 5;
   if (row >= a.n) return;
   const int64_t i = a.row0 + row, t = a.p.targets[i];
   const bool lives = t != a.p.ignore && t >= 0 && t < a.p.classes;
@@ -685,8 +824,9 @@ __global__ void __launch_bounds__(kRowsT) ce_weights_kernel(const __grid_constan
     if (!lives) weight = 0.0f;
     a.ref[row] = a.p.lse[i] * kLog2e;
     a.mul[row] = weight * a.e_scale;
-    a.value[row] = expm1f(-a.p.losses[i]) * weight * a.e_scale;
-    a.factor[row] = lives ? 1.0f : 0.0f;
+    const float value = expm1f(-a.p.losses[i]) * weight * a.e_scale;
+    a.value[row] = value;
+    a.factor[row] = lives ? folded(value, dev::Vec16<T>::to_float(dev::Vec16<T>::from_float(value)), 1.0f) : 0.0f;
   }
   if (a.xs == nullptr) return;
   const T* from = static_cast<const T*>(a.p.x) + i * a.p.x_stride;
@@ -699,20 +839,31 @@ __global__ void __launch_bounds__(kRowsT) ce_weights_kernel(const __grid_constan
   }
 }
 // The sum or mean of the losses, in a fixed order.
-__global__ void __launch_bounds__(1024) ce_total_kernel(const float* losses, int64_t n, const Scales* scales, int mean, float* out) {
-  __shared__ double part[32];
+__global__ void __launch_bounds__(1024) ce_total_kernel(const float* losses, const int64_t* targets, int64_t n, int64_t ignore, int mean, float* out) {
+  __shared__ double part[32], counted[32];
   follow();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  double sum = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) sum += double(losses[i]);
+  double sum = 0.0, count = 0.0;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+    sum += double(losses[i]);
+    count += targets[i] != ignore ? 1.0 : 0.0;
+  }
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-  if (lane == 0) part[warp] = sum;
+  for (int off = 16; off > 0; off >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    count += __shfl_xor_sync(0xffffffffu, count, off);
+  }
+  if (lane == 0) part[warp] = sum, counted[warp] = count;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    sum = 0.0;
-    for (int w = 0; w < 32; ++w) sum += part[w];
-    *out = float(mean ? sum / double(scales->count) : sum);
+  if (warp == 0) {
+    sum = part[lane], count = counted[lane];
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      count += __shfl_xor_sync(0xffffffffu, count, off);
+    }
+    if (lane == 0) *out = float(mean ? sum / count : sum);
   }
 }
 // Columns of E, each row times its factor, added up: 256 columns and a share of the rows a CTA, the shares' sums one behind the other.
@@ -759,6 +910,31 @@ __global__ void ce_bias_grad_kernel(const float* partial, int shares, int classe
   if (dtype == NANGILA_F32) static_cast<float*>(dbias)[i] = sum;
   else if (dtype == NANGILA_F16) static_cast<__half*>(dbias)[i] = __float2half_rn(sum);
   else static_cast<__nv_bfloat16*>(dbias)[i] = __float2bfloat16_rn(sum);
+}
+// dx = alpha f_row times the sum of its parts, in 16 bits; parts are `part` elements apart
+template <typename T>
+__global__ void __launch_bounds__(256) ce_join_kernel(const float* sums, int64_t part, int parts, const float* factor, const Scales* scales, T* out, int64_t n8, int per) {
+  follow();
+  const float alpha = scales->alpha;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n8; i += int64_t(gridDim.x) * 256) {
+    const float f = factor[i / per];
+    float v[8], w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+#pragma unroll 4
+    for (int j = 0; j < parts; ++j) {
+      dev::Raw8<float> in;
+      dev::fetch(sums + j * part + i * 8, in);
+      dev::unpack(in, w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += w[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = f == 0.0f ? 0.0f : v[k] * (alpha * f);
+    dev::Raw8<T> r;
+    dev::pack(v, r);
+    dev::put(out + i * 8, r);
+  }
 }
 // dw = alpha sums, in 16 bits
 template <typename T>
@@ -820,13 +996,14 @@ struct Matrix {
   const void* base;
   int64_t rows, cols, ld;
   CUtensorMapDataType type;
+  int64_t parts = 1;  // one behind the other
 };
 // copied in boxes of box_inner x box_outer; what lies outside reads as zero and is not written
 bool make_map(CUtensorMap* map, const Matrix& m, uint32_t box_inner, uint32_t box_outer) {
   EncodeFn fn = encode_fn();
   if (!fn) return false;
   const int size = m.type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2;
-  const cuuint64_t dims[3] = {cuuint64_t(m.cols), cuuint64_t(m.rows), 1};
+  const cuuint64_t dims[3] = {cuuint64_t(m.cols), cuuint64_t(m.rows), cuuint64_t(m.parts)};
   const cuuint64_t strides[2] = {cuuint64_t(m.ld) * size, cuuint64_t(m.ld) * size * cuuint64_t(m.rows)};
   const cuuint32_t box[3] = {box_inner, box_outer, 1}, step[3] = {1, 1, 1};
   return fn(map, m.type, 3, const_cast<void*>(m.base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -852,36 +1029,72 @@ int allow_smem(const void* kernel, int bytes) {
   return 0;
 }
 
-// The product of a and b, `out` the result where there is one in memory.
-template <typename T, int KIND, bool A_MN, bool B_MN, bool PAIR>
-int launch_product(const Matrix& a, const Matrix& b, const Matrix* out, Product p, const Rows& rows, cudaStream_t stream) {
-  constexpr int kSide = PAIR ? 256 : 128;
-  Maps maps;
-  constexpr bool kWide = KIND == kSums || KIND == kAdded;
-  if (!make_map(&maps.a, a, 64, A_MN ? 64 : 128) || !make_map(&maps.b, b, 64, B_MN ? 64 : 128) || !make_map(&maps.out, out != nullptr ? *out : a, kWide ? 32 : 64, 32))
-    return int(cudaErrorNotSupported);
-  p.tiles_m = (p.M + kSide - 1) / kSide;
-  p.tiles_n = (p.N + kSide - 1) / kSide;
-  const int64_t total = int64_t(p.tiles_m) * p.tiles_n;
-  if (total > 0x3fffffff) return int(cudaErrorInvalidValue);
-  p.total = int(total);
-  auto* kernel = ce_product_kernel<T, KIND, A_MN, B_MN, PAIR>;
-  if (const int e = allow_smem(reinterpret_cast<const void*>(kernel), kSmem)) return e;
-  cudaLaunchAttribute attr[2];
+cudaLaunchConfig_t pairs_config(cudaLaunchAttribute (&attr)[2], int ctas, bool pair, cudaStream_t stream) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = PAIR ? 2 : 1;
+  attr[1].val.clusterDim.x = pair ? 2 : 1;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  const int sms = sm_count();
-  cfg.gridDim = dim3(unsigned(PAIR ? 2 * std::min(p.total, sms / 2) : std::min(p.total, sms)));
+  cfg.gridDim = dim3(unsigned(ctas));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = PAIR ? 2 : 1;
-  return int(cudaLaunchKernelEx(&cfg, kernel, maps, p, rows));
+  cfg.numAttrs = pair ? 2 : 1;
+  return cfg;
+}
+// The tiles of x w^T; e: where E goes.
+template <typename T, int KIND, bool PAIR>
+int launch_logits(const Matrix& x, const Matrix& w, const Matrix* e, const Rows& rows, cudaStream_t stream) {
+  constexpr int kSide = PAIR ? 256 : 128;
+  Maps maps;
+  if (!make_map(&maps.a, x, 64, 128) || !make_map(&maps.b, w, 64, 128) || !make_map(&maps.out, e != nullptr ? *e : x, 64, 32)) return int(cudaErrorNotSupported);
+  const int64_t tiles_m = (rows.n + kSide - 1) / kSide, total = tiles_m * ((rows.classes + kSide - 1) / kSide);
+  if (total > 0x3fffffff) return int(cudaErrorInvalidValue);
+  auto* kernel = ce_logits_kernel<T, KIND, PAIR>;
+  if (const int err = allow_smem(reinterpret_cast<const void*>(kernel), kSmem)) return err;
+  const int sms = sm_count();
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = pairs_config(attr, int(PAIR ? 2 * std::min<int64_t>(total, sms / 2) : std::min<int64_t>(total, sms)), PAIR, stream);
+  return int(cudaLaunchKernelEx(&cfg, kernel, maps, rows, int(tiles_m), int(total), int((x.cols + kSlabK - 1) / kSlabK)));
+}
+template <typename T, int KIND>
+int logits(bool pair, const Matrix& x, const Matrix& w, const Matrix* e, const Rows& rows, cudaStream_t stream) {
+  return pair ? launch_logits<T, KIND, true>(x, w, e, rows, stream) : launch_logits<T, KIND, false>(x, w, e, rows, stream);
+}
+
+Result result(int64_t M, int64_t N, int64_t K, int split) {
+  Result r;
+  std::memset(&r, 0, sizeof r);
+  r.M = int(M);
+  r.N = int(N);
+  r.K = int(K);
+  const int slabs = (r.K + kSlabK - 1) / kSlabK;
+  r.slabs = (slabs + split - 1) / split;
+  r.split = (slabs + r.slabs - 1) / r.slabs;
+  r.tiles_n = (r.N + 255) / 256;
+  r.per = (r.M + 255) / 256 * r.tiles_n;
+  r.total = r.per * r.split;
+  return r;
+}
+// Into how many parts dx's K is cut: as few as let a pair's tiles of dx end before its share of all work does. (With dw not wanted: before the tiles of the
+// busiest pair would take a tenth longer than its share.)
+int split_of(int64_t n, int64_t d, int64_t classes, int64_t rows, bool dw) {
+  const int pairs = sm_count() / 2;
+  const Result w = result(rows, d, n, 1);
+  int best = 1;
+  double least = 1e30;
+  for (int split = 1; split <= 16; ++split) {
+    const Result x = result(n, d, classes, split);
+    if (split > 1 && x.slabs < 8) break;
+    const double share = (double(x.per) * ((x.K + kSlabK - 1) / kSlabK) + (dw ? double(w.total) * w.slabs : 0.0)) / pairs;
+    const double busiest = double((x.total + pairs - 1) / pairs) * x.slabs;
+    // (sums of a part go through memory: some three slabs' time a tile)
+    const double cost = std::max(share, busiest) + (split > 1 ? 3.0 * x.total / pairs : 0.0);
+    if (cost < least * 0.97) least = cost, best = x.split;
+  }
+  return best;
 }
 
 // How a call is cut up, and where its parts lie in the workspace.
@@ -890,7 +1103,8 @@ struct Plan {
   int64_t groups, e_stride, parts, shares, share;
   bool pair;          // tiles of the logits
   bool wide;          // dw is summed up over the groups
-  int64_t at_scales, at_zt, at_bias, at_ref, at_mul, at_value, at_factor, at_again, at_parts, at_e, at_xs, at_sums, at_columns, total;
+  int split;          // parts of dx's K
+  int64_t at_scales, at_zt, at_bias, at_ref, at_mul, at_value, at_factor, at_again, at_parts, at_e, at_xs, at_sums, at_dx, at_columns, total;
   int64_t bias_count;
 };
 constexpr int64_t kGroupBytes = int64_t(1) << 29;  // of E
@@ -920,11 +1134,11 @@ Plan plan(const NangilaLinearCeParams& p, int what) {
     return at;
   };
   l.at_scales = take(sizeof(Scales));
-  l.at_zt = take(what == NANGILA_CE_GRADIENTS ? 0 : p.n * 4);
+  l.at_zt = take(what == NANGILA_CE_BOTH ? p.n * 4 : 0);
+  l.at_ref = take(what == NANGILA_CE_BOTH ? p.n * 4 : what == NANGILA_CE_GRADIENTS ? l.group * 4 : 0);
   l.at_bias = take(p.bias != nullptr ? l.bias_count * 4 : 0);
   l.at_parts = take(what == NANGILA_CE_GRADIENTS ? 0 : l.parts * l.group * 8);
   if (what == NANGILA_CE_LOSSES) return l;
-  l.at_ref = take(l.group * 4);
   l.at_mul = take(what == NANGILA_CE_GRADIENTS ? l.group * 4 : 0);
   l.at_value = take(what == NANGILA_CE_GRADIENTS ? l.group * 4 : 0);
   l.at_factor = take(l.group * 4);
@@ -932,13 +1146,10 @@ Plan plan(const NangilaLinearCeParams& p, int what) {
   l.at_e = take(l.group * l.e_stride * 2);
   l.at_xs = take(p.dw != nullptr ? l.group * p.d * 2 : 0);
   l.at_sums = take(l.wide ? int64_t(p.rows) * p.d * 4 : 0);
+  l.split = p.dx != nullptr ? split_of(l.group, p.d, classes, p.rows, p.dw != nullptr) : 1;
+  l.at_dx = take(l.split > 1 ? l.split * l.group * p.d * 4 : 0);
   l.at_columns = take(p.dbias != nullptr ? l.groups * l.shares * classes * 4 : 0);
   return l;
-}
-
-template <typename T, int KIND>
-int logits(bool pair, const Matrix& x, const Matrix& w, const Matrix* e, const Product& q, const Rows& rows, cudaStream_t stream) {
-  return pair ? launch_product<T, KIND, false, false, true>(x, w, e, q, rows, stream) : launch_product<T, KIND, false, false, false>(x, w, e, q, rows, stream);
 }
 
 template <typename T>
@@ -956,13 +1167,18 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
   std::memset(&begin, 0, sizeof begin);
   begin.p = p;
   begin.what = what;
-  begin.zt = zt;
+  begin.zt = what == NANGILA_CE_BOTH ? zt : nullptr;
+  begin.ref = reinterpret_cast<float*>(ws + l.at_ref);
   begin.bias = bias;
   begin.bias_count = int(l.bias_count);
   begin.scales = scales;
   begin.e_scale = what == NANGILA_CE_GRADIENTS && std::is_same<T, __half>::value ? 32768.0f : 1.0f;
-  ce_begin_kernel<T><<<unsigned(1 + std::min<int64_t>((p.n + kBeginT / 32 - 1) / (kBeginT / 32), 148 * 8)), kBeginT, 0, stream>>>(begin);
-  int e = int(cudaGetLastError());
+  int e = 0;
+  if (what != NANGILA_CE_LOSSES || p.bias != nullptr) {
+    const int64_t work = std::max<int64_t>(what == NANGILA_CE_BOTH ? (p.n + kBeginT / 32 - 1) / (kBeginT / 32) : 0, p.bias != nullptr ? (l.bias_count + kBeginT - 1) / kBeginT : 0);
+    ce_begin_kernel<T><<<unsigned(1 + std::min<int64_t>(work, 148 * 8)), kBeginT, 0, stream>>>(begin);
+    e = int(cudaGetLastError());
+  }
 
   for (int64_t g = 0; g < l.groups && e == 0; ++g) {
     Group a;
@@ -972,7 +1188,6 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
     a.n = int(std::min(l.group, p.n - a.row0));
     a.stride = l.group;
     a.parts_count = int(l.parts);
-    a.zt = zt + a.row0;
     a.parts = reinterpret_cast<const float2*>(ws + l.at_parts);
     a.scales = scales;
     a.e_scale = begin.e_scale;
@@ -984,20 +1199,15 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
     rows.stride = l.group;
     rows.n = a.n;
     rows.classes = p.classes;
-    Product q;
-    std::memset(&q, 0, sizeof q);
-    q.M = a.n;
-    q.N = p.classes;
-    q.K = p.d;
     const Matrix x{static_cast<const T*>(p.x) + a.row0 * p.x_stride, a.n, p.d, p.x_stride, type}, w{p.w, p.classes, p.d, p.w_stride, type};
     const unsigned row_ctas = unsigned((a.n + kRowsAtOnce - 1) / kRowsAtOnce);
     const int tile_rows = l.pair ? 256 : 128;
     if (what == NANGILA_CE_LOSSES) {
-      e = logits<T, kStats>(l.pair, x, w, nullptr, q, rows, stream);
+      e = logits<T, kStats>(l.pair, x, w, nullptr, rows, stream);
       if (e == 0) e = int(launch_following(ce_rows_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, 0, tile_rows));
       continue;
     }
-    a.ref = reinterpret_cast<float*>(ws + l.at_ref);
+    a.ref = reinterpret_cast<float*>(ws + l.at_ref) + (what == NANGILA_CE_BOTH ? a.row0 : 0);
     a.factor = reinterpret_cast<float*>(ws + l.at_factor);
     a.e = ws + l.at_e;
     a.e_stride = l.e_stride;
@@ -1005,48 +1215,59 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
     rows.ref = a.ref;
     const Matrix ex{a.e, a.n, p.classes, l.e_stride, type};
     if (what == NANGILA_CE_BOTH) {
+      a.zt = zt + a.row0;
       a.again = reinterpret_cast<int32_t*>(ws + l.at_again);
-      ce_refs_kernel<<<unsigned((a.n + 255) / 256), 256, 0, stream>>>(a.zt, a.ref, a.n);
-      e = int(cudaGetLastError());
-      if (e == 0) e = logits<T, kExp>(l.pair, x, w, &ex, q, rows, stream);
+      e = logits<T, kExp>(l.pair, x, w, &ex, rows, stream);
       if (e == 0) e = int(launch_following(ce_rows_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, 1, tile_rows));
       rows.again = a.again;
-      if (e == 0) e = logits<T, kExp>(l.pair, x, w, &ex, q, rows, stream);
+      if (e == 0) e = logits<T, kExp>(l.pair, x, w, &ex, rows, stream);
       if (e == 0) e = int(launch_following(ce_rows_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, 2, tile_rows));
+      if (e == 0 && a.xs != nullptr)
+        e = int(launch_following(ce_scale_kernel<T>, dim3(unsigned(std::min<int64_t>((int64_t(a.n) * p.d / 8 + kWeightsT - 1) / kWeightsT, 148 * 8))), kWeightsT, 0, stream, a));
     } else {
       a.mul = reinterpret_cast<float*>(ws + l.at_mul);
       a.value = reinterpret_cast<float*>(ws + l.at_value);
-      ce_weights_kernel<T><<<unsigned((int64_t(a.n) * 32 + kRowsT - 1) / kRowsT), kRowsT, 0, stream>>>(a);
+      ce_weights_kernel<T><<<unsigned((int64_t(a.n) * 32 + kWeightsT - 1) / kWeightsT), kWeightsT, 0, stream>>>(a);
       e = int(cudaGetLastError());
       rows.mul = a.mul;
       rows.value = a.value;
-      if (e == 0) e = logits<T, kExp>(l.pair, x, w, &ex, q, rows, stream);
+      if (e == 0) e = logits<T, kExp>(l.pair, x, w, &ex, rows, stream);
     }
     if (e == 0 && p.dbias != nullptr) {
       e = int(launch_following(ce_columns_kernel<T>, dim3(unsigned((p.classes + 255) / 256), unsigned(l.shares)), kColumnT, 0, stream, static_cast<const T*>(a.e), l.e_stride,
                                static_cast<const float*>(a.factor), a.n, int(p.classes), int(l.share), columns + g * l.shares * p.classes));
     }
-    if (e == 0 && p.dx != nullptr) {
-      Product d = q;
-      d.N = p.d;
-      d.K = p.classes;
-      d.n_inner = 1;
-      d.alpha = &scales->alpha;
-      d.factor = a.factor;
-      const Matrix out{static_cast<T*>(p.dx) + a.row0 * p.d, a.n, p.d, p.d, type};
-      e = launch_product<T, kScaled, false, true, true>(ex, w, &out, d, rows, stream);
-    }
-    if (e == 0 && p.dw != nullptr) {
-      Product d = q;
-      d.M = p.rows;
-      d.N = p.d;
-      d.K = a.n;
-      d.n_inner = 1;
-      d.alpha = &scales->alpha;
-      const Matrix xs{a.xs, a.n, p.d, p.d, type}, out{p.dw, p.rows, p.d, p.d, type}, wide{sums, p.rows, p.d, p.d, CU_TENSOR_MAP_DATA_TYPE_FLOAT32};
-      if (!l.wide) e = launch_product<T, kScaled, true, true, true>(ex, xs, &out, d, rows, stream);
-      else if (g == 0) e = launch_product<T, kSums, true, true, true>(ex, xs, &wide, d, rows, stream);
-      else e = launch_product<T, kAdded, true, true, true>(ex, xs, &wide, d, rows, stream);
+    if (e == 0 && (p.dx != nullptr || p.dw != nullptr)) {
+      Gradients q;
+      std::memset(&q, 0, sizeof q);
+      q.alpha = &scales->alpha;
+      GradientMaps maps;
+      bool ok = make_map(&maps.e_rows, ex, 64, 128) && make_map(&maps.e_columns, ex, 64, 64) && make_map(&maps.w, w, 64, 64) && make_map(&maps.xs, x, 64, 64) && make_map(&maps.out_x, x, 64, 32) &&
+                make_map(&maps.out_w, x, 64, 32);  // (those that are not wanted are not used)
+      if (p.dx != nullptr) {
+        q.x = result(a.n, p.d, p.classes, l.split);
+        q.x.factor = a.factor;
+        q.x.wide = q.x.split > 1 ? 1 : 0;
+        const Matrix out{static_cast<T*>(p.dx) + a.row0 * p.d, a.n, p.d, p.d, type}, parts{ws + l.at_dx, a.n, p.d, p.d, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, q.x.split};
+        ok = ok && (q.x.wide ? make_map(&maps.out_x, parts, 32, 32) : make_map(&maps.out_x, out, 64, 32));
+      }
+      if (p.dw != nullptr) {
+        q.w = result(p.rows, p.d, a.n, 1);
+        q.w.wide = !l.wide ? 0 : g == 0 ? 1 : 2;
+        const Matrix xs{a.xs, a.n, p.d, p.d, type}, out{p.dw, p.rows, p.d, p.d, type}, wide{sums, p.rows, p.d, p.d, CU_TENSOR_MAP_DATA_TYPE_FLOAT32};
+        ok = ok && make_map(&maps.xs, xs, 64, 64) && (l.wide ? make_map(&maps.out_w, wide, 32, 32) : make_map(&maps.out_w, out, 64, 32));
+      }
+      if (!ok) return int(cudaErrorNotSupported);
+      if (p.dx != nullptr && p.dw != nullptr) q.extra = (q.x.slabs + q.w.slabs / 2) / q.w.slabs;
+      auto* kernel = ce_gradients_kernel<T>;
+      if (const int err = allow_smem(reinterpret_cast<const void*>(kernel), kSmem)) return err;
+      cudaLaunchAttribute attr[2];
+      const cudaLaunchConfig_t cfg = pairs_config(attr, 2 * std::min(q.x.total + q.w.total, sm_count() / 2), true, stream);
+      e = int(cudaLaunchKernelEx(&cfg, kernel, maps, q));
+      if (e == 0 && q.x.wide)
+        e = int(launch_following(ce_join_kernel<T>, dim3(unsigned(std::min<int64_t>((int64_t(a.n) * p.d / 8 + 255) / 256, 148 * 8))), 256, 0, stream, reinterpret_cast<const float*>(ws + l.at_dx),
+                                 int64_t(a.n) * p.d, q.x.split, static_cast<const float*>(a.factor), static_cast<const Scales*>(scales), static_cast<T*>(p.dx) + a.row0 * p.d, int64_t(a.n) * p.d / 8,
+                                 int(p.d / 8)));
     }
   }
   if (e == 0 && l.wide)
@@ -1056,7 +1277,7 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
     e = int(launch_following(ce_bias_grad_kernel, dim3(unsigned((p.rows + 255) / 256)), 256, 0, stream, static_cast<const float*>(columns), int(l.groups * l.shares), int(p.classes), int(p.rows),
                              static_cast<const Scales*>(scales), p.dbias, int(p.bias_dtype)));
   if (e == 0 && what != NANGILA_CE_GRADIENTS && p.loss != nullptr)
-    e = int(launch_following(ce_total_kernel, dim3(1), 1024, 0, stream, static_cast<const float*>(p.losses), p.n, static_cast<const Scales*>(scales), int(p.mean), p.loss));
+    e = int(launch_following(ce_total_kernel, dim3(1), 1024, 0, stream, static_cast<const float*>(p.losses), p.targets, p.n, p.ignore, int(p.mean), p.loss));
   return e;
 }
 
