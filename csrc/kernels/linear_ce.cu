@@ -53,18 +53,18 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kMostAbove = 60.0f * kLog2e;     // how far a logit may lie above a row's reference
 
-// What becomes of a tile. kStats: the largest logit and the sum of exponentials of each row over half a tile's columns. kExp: E, and with `parts` the same sums. kScaled: alpha f_row D in
-// 16 bits. kSums, kAdded: D in fp32, written or added.
-enum Kind { kStats, kExp, kScaled, kSums, kAdded };
+// What becomes of a tile of logits. kStats: the largest one and the sum of exponentials of each row over half a tile's columns. kExp: the same, and E. kWeighted: E, its rows weighted
+// and with their elements at the target.
+enum Kind { kStats, kExp, kWeighted };
 
 // What is known of a group's rows when their tiles are made, and what comes out.
 struct Rows {
   const int64_t* targets;
   const float* ref;     // exponents' reference, times log2(e)
-  const float* mul;     // factors of E's rows; NULL: one
-  const float* value;   // with them, E's element at the target (else 0, to be filled in)
+  const float* mul;     // kWeighted: factors of E's rows
+  const float* value;   // and E's element at the target (kExp: 0, to be filled in)
   const float* bias;    // padded to whole tiles; NULL: none
-  float2* parts;        // [half tiles][stride]: largest z log2(e), sum of exp; NULL: not wanted
+  float2* parts;        // [half tiles][stride]: largest z log2(e), sum of exp
   const int32_t* again; // for each 32 rows, whether they are to be formed again; NULL: all tiles are made
   int64_t stride;
   int n, classes;
@@ -255,7 +255,99 @@ __device__ __forceinline__ void send_slot(const uint8_t* slot, const CUtensorMap
   }
 }
 
-// A tile of logits, the n-th, by one of the epilogue's warps.
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void halves_of(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+
+// What an epilogue's warp knows of the rows of a tile of logits, a lane each, and finds out about them.
+struct LogitRow {
+  int target;               // -1: none
+  bool dead;                // adds nothing
+  float ref, mul, value;
+  float most;               // raw logits
+  uint64_t sum[2];
+};
+// 32 columns from `first` on: their part of the row's sums, and with E its 64 bytes of the slot from sixteen bytes `at` on.
+template <typename T, int KIND>
+__device__ __forceinline__ void take_logits(const Rows& rows, LogitRow& r, uint32_t (&raw)[32], bool ok, int first, uint8_t* slot, int lane, int at) {
+  float v[32];
+#pragma unroll
+  for (int k = 0; k < 32; ++k) v[k] = ok ? __uint_as_float(raw[k]) : __uint_as_float(0x7fc00000u);
+  if (rows.bias != nullptr) {
+#pragma unroll
+    for (int k = 0; k < 32; k += 4) {
+      const float4 b = __ldg(reinterpret_cast<const float4*>(rows.bias + first + k));
+      v[k] += b.x, v[k + 1] += b.y, v[k + 2] += b.z, v[k + 3] += b.w;
+    }
+  }
+  const bool here = r.target >= first && r.target < first + 32, any = __any_sync(0xffffffffu, here);
+  if (any || first + 32 > rows.classes) {  // what is no class, and the target, stay out of the sums
+#pragma unroll
+    for (int k = 0; k < 32; ++k)
+      if (first + k >= rows.classes || first + k == r.target) v[k] = -INFINITY;
+  }
+  float base = r.ref;
+  if constexpr (KIND != kWeighted) {
+    float top[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top[k] = fmaxf(v[k], v[k + 4]);
+#pragma unroll
+    for (int k = 8; k < 32; ++k) top[k & 3] = fmaxf(top[k & 3], v[k]);
+    const float now = fmaxf(fmaxf(r.most, fmaxf(top[0], top[1])), fmaxf(top[2], top[3]));
+    if constexpr (KIND == kStats) {
+      // the sums so far, relative to the largest logit so far
+      const float to = now == -INFINITY ? 0.0f : now, by = exp2_fast((r.most - to) * kLog2e);
+      const uint64_t by2 = pair_of(by, by), none = pair_of(-0.0f, -0.0f);
+      r.sum[0] = fma_pair(r.sum[0], by2, none);
+      r.sum[1] = fma_pair(r.sum[1], by2, none);
+      base = to * kLog2e;
+    }
+    r.most = now;
+  }
+  const uint64_t scale = pair_of(kLog2e, kLog2e), from = pair_of(-base, -base);
+#pragma unroll
+  for (int k = 0; k < 32; k += 2) {
+    float a, b;
+    halves_of(fma_pair(pair_of(v[k], v[k + 1]), scale, from), a, b);
+    v[k] = exp2_fast(a), v[k + 1] = exp2_fast(b);
+    if constexpr (KIND != kWeighted) r.sum[(k / 2) & 1] = add_pair(r.sum[(k / 2) & 1], pair_of(v[k], v[k + 1]));
+  }
+  if constexpr (KIND == kStats) return;
+  if constexpr (KIND == kWeighted) {
+#pragma unroll
+    for (int k = 0; k < 32; ++k) v[k] *= r.mul;
+    if (any) {
+#pragma unroll
+      for (int k = 0; k < 32; ++k)
+        if (first + k == r.target) v[k] = r.value;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = v[8 * e + k];
+    uint4 packed = pack16<T>(w);
+    if (r.dead) packed = make_uint4(0, 0, 0, 0);
+    *box_at(slot, lane, at + e) = packed;
+  }
+}
+// A tile of logits, the n-th, by one of the epilogue's warps: 32 columns at a time, the next on their way out of tensor memory.
+// (Sixteen at a time, each waited for, the epilogue took longer than the products for K up to 1024: 1229 x 1024 x 30592 75 us.)
 template <typename T, int KIND, bool PAIR>
 __device__ __forceinline__ void finish_logits(const Shared& s, uint32_t tmem, const Rows& rows, const CUtensorMap* out, const TileAt& at, uint32_t rank, int n, uint32_t& used) {
   constexpr int kSide = PAIR ? 256 : 128, kHalf = kSide / 2;
@@ -263,85 +355,46 @@ __device__ __forceinline__ void finish_logits(const Shared& s, uint32_t tmem, co
   const int quad = warp & 3, half = (warp - 2) >> 2;  // the lanes of tensor memory that this warp may read; its half of the columns
   const int row0 = at.m0 + int(rank) * kTileM + quad * 32, row = row0 + lane, col0 = at.n0 + half * kHalf;
   const bool mine = row0 < rows.n && col0 < rows.classes;
-  // of this lane's row
-  int target = -1;
-  bool dead = true;
-  float ref = 0.0f, mul = 1.0f, value = 0.0f;
+  LogitRow r;
+  r.target = -1;
+  r.dead = true;
+  r.ref = 0.0f, r.mul = 1.0f, r.value = 0.0f;
+  r.most = -INFINITY;
+  r.sum[0] = r.sum[1] = 0;
   if (mine && row < rows.n) {
     const int64_t t = rows.targets[row];
-    dead = t < 0 || t >= rows.classes;
-    target = dead ? -1 : int(t);
-    if (KIND == kExp) {
-      ref = rows.ref[row];
-      if (rows.mul != nullptr) mul = rows.mul[row], value = rows.value[row];
-    }
+    r.dead = t < 0 || t >= rows.classes;
+    r.target = r.dead ? -1 : int(t);
+    if (KIND != kStats) r.ref = rows.ref[row];
+    if (KIND == kWeighted) r.mul = rows.mul[row], r.value = rows.value[row];
   }
   const bool ok = accumulator_here(s, n);
-  float most = -INFINITY, sum = 0.0f;
   if (mine) {
+    const uint32_t from = tmem + (uint32_t(quad * 32) << 16) + uint32_t((n & 1) * kSide + half * kHalf);
+    uint32_t left[32], right[32];
+    tmem_ld_32x32b_x32_start(from, left);
 #pragma unroll 1
     for (int c = 0; c < kHalf && col0 + c < rows.classes; c += 64) {
-      uint8_t* slot = KIND == kExp ? free_slot(s, used) : nullptr;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float v[16];
-        const int first = col0 + c + g * 16;
-        tmem_ld_32x32b_x16(tmem + (uint32_t(quad * 32) << 16) + uint32_t((n & 1) * kSide + half * kHalf + c + g * 16), v);
-        if (!ok) nan16(v);
-        if (rows.bias != nullptr) {
-#pragma unroll
-          for (int k = 0; k < 16; k += 4) {
-            const float4 b = *reinterpret_cast<const float4*>(rows.bias + first + k);
-            v[k] += b.x, v[k + 1] += b.y, v[k + 2] += b.z, v[k + 3] += b.w;
-          }
-        }
-        const bool edge = first + 16 > rows.classes, here = target >= first && target < first + 16;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] *= kLog2e;
-        if (edge || __any_sync(0xffffffffu, here)) {  // what is no class, and the target, stay out of the sums
-#pragma unroll
-          for (int k = 0; k < 16; ++k)
-            if (first + k >= rows.classes || first + k == target) v[k] = -INFINITY;
-        }
-        float top = v[0];
-#pragma unroll
-        for (int k = 1; k < 16; ++k) top = fmaxf(top, v[k]);
-        if constexpr (KIND == kStats) {
-          const float now = fmaxf(most, top), base = now == -INFINITY ? 0.0f : now;
-          sum *= exp2_fast(most - base);
-          most = now;
-#pragma unroll
-          for (int k = 0; k < 16; ++k) sum += exp2_fast(v[k] - base);
-        } else {
-          most = fmaxf(most, top);
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            v[k] = exp2_fast(v[k] - ref);
-            sum += v[k];
-            v[k] *= mul;
-          }
-          if (__any_sync(0xffffffffu, here)) {
-#pragma unroll
-            for (int k = 0; k < 16; ++k)
-              if (first + k == target) v[k] = value;
-          }
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float w[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = dead ? 0.0f : v[8 * e + k];
-            *box_at(slot, lane, 2 * g + e) = pack16<T>(w);
-          }
-        }
-      }
-      if (KIND == kExp) {
+      uint8_t* slot = KIND != kStats ? free_slot(s, used) : nullptr;
+      tmem_ld_wait(left);
+      tmem_ld_32x32b_x32_start(from + c + 32, right);
+      take_logits<T, KIND>(rows, r, left, ok, col0 + c, slot, lane, 0);
+      tmem_ld_wait(right);
+      if (c + 64 < kHalf) tmem_ld_32x32b_x32_start(from + c + 64, left);
+      take_logits<T, KIND>(rows, r, right, ok, col0 + c + 32, slot, lane, 4);
+      if (KIND != kStats) {
         send_slot(slot, out, col0 + c, row0, 0, false);
         ++used;
       }
     }
+    tmem_ld_wait(left);
   }
   accumulator_read<PAIR>(s, n);
-  if (mine && row < rows.n && rows.parts != nullptr) rows.parts[int64_t(col0 / kHalf) * rows.stride + row] = make_float2(most, sum);
+  if (KIND != kWeighted && mine && row < rows.n) {
+    float a, b;
+    halves_of(add_pair(r.sum[0], r.sum[1]), a, b);
+    rows.parts[int64_t(col0 / kHalf) * rows.stride + row] = make_float2(r.most * kLog2e, a + b);
+  }
 }
 
 // A tile of a gradient, the n-th, by one of the epilogue's warps: `wide` 0 in 16 bits, each row times `scale`; else in fp32, written (1) or added (2), as part `part`.
@@ -457,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_logits_kernel(const __grid_con
   if (threadIdx.x == 0) {
     prefetch_tensormap(&maps.a);
     prefetch_tensormap(&maps.b);
-    if (KIND == kExp) prefetch_tensormap(&maps.out);
+    if (KIND != kStats) prefetch_tensormap(&maps.out);
   }
   const uint32_t tmem = products_begin<PAIR>(s);
   may_follow();
@@ -1214,7 +1267,7 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
     a.xs = p.dw != nullptr ? ws + l.at_xs : nullptr;
     rows.ref = a.ref;
     const Matrix ex{a.e, a.n, p.classes, l.e_stride, type};
-    if (what == NANGILA_CE_BOTH) {
+    if constexpr (!std::is_same<T, __half>::value) if (what == NANGILA_CE_BOTH) {
       a.zt = zt + a.row0;
       a.again = reinterpret_cast<int32_t*>(ws + l.at_again);
       e = logits<T, kExp>(l.pair, x, w, &ex, rows, stream);
@@ -1224,14 +1277,15 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
       if (e == 0) e = int(launch_following(ce_rows_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, 2, tile_rows));
       if (e == 0 && a.xs != nullptr)
         e = int(launch_following(ce_scale_kernel<T>, dim3(unsigned(std::min<int64_t>((int64_t(a.n) * p.d / 8 + kWeightsT - 1) / kWeightsT, 148 * 8))), kWeightsT, 0, stream, a));
-    } else {
+    }
+    if (what == NANGILA_CE_GRADIENTS) {
       a.mul = reinterpret_cast<float*>(ws + l.at_mul);
       a.value = reinterpret_cast<float*>(ws + l.at_value);
       ce_weights_kernel<T><<<unsigned((int64_t(a.n) * 32 + kWeightsT - 1) / kWeightsT), kWeightsT, 0, stream>>>(a);
       e = int(cudaGetLastError());
       rows.mul = a.mul;
       rows.value = a.value;
-      if (e == 0) e = logits<T, kExp>(l.pair, x, w, &ex, rows, stream);
+      if (e == 0) e = logits<T, kWeighted>(l.pair, x, w, &ex, rows, stream);
     }
     if (e == 0 && p.dbias != nullptr) {
       e = int(launch_following(ce_columns_kernel<T>, dim3(unsigned((p.classes + 255) / 256), unsigned(l.shares)), kColumnT, 0, stream, static_cast<const T*>(a.e), l.e_stride,
