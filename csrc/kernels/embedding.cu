@@ -1,8 +1,8 @@
 // Token embeddings: out[i] = scale * weight[ids[i]], and the table's gradient dw[v] = scale * sum of dy[i] over ids[i] = v.
 //
 // The gradient goes by sorted tokens, so that every sum has a fixed order and no atomics decide it:
-//   1. a cluster of eight CTAs sorts the positions by id (radix sort, least significant digit first, stable), while all other CTAs fill the gradient with zeros, which is
-//      most of what is written: a batch has far fewer tokens than the table has rows;
+//   1. the gradient is filled with zeros, which is most of what is written: a batch has far fewer tokens than the table has rows. Meanwhile a cluster of eight CTAs sorts
+//      the positions by id (radix sort, least significant digit first, stable);
 //   2. the sorted positions are cut into pieces of a few dozen, and each piece adds up its runs of equal ids, in fp32; a run that lies in one piece is
 //      a finished row, one that goes on in the next leaves partial sums;
 //   3. the partial sums of each run that crosses pieces are added up. A token that fills half the batch is spread over all SMs that way.
@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <cstring>
 
 #include "follow.cuh"
 #include "launch_util.cuh"
@@ -29,12 +30,49 @@ __device__ __forceinline__ int64_t id_at(const void* ids, int ids_64, int64_t i)
   return ids_64 ? static_cast<const int64_t*>(ids)[i] : int64_t(static_cast<const int32_t*>(ids)[i]);
 }
 
+// Sixteen bytes from any address of a T, out of the two aligned sixteen that hold them. Those have to lie in the tensor, from `lo` to `hi`; near its ends
+// values are read one by one, and those behind its end are zero.
+template <typename T>
+__device__ __forceinline__ uint4 load16_any(const T* p, const char* lo, const char* hi) {
+  constexpr int N = 16 / sizeof(T);
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p) & ~uintptr_t(15);
+  const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(p) & 15u);
+  uint32_t w[8];
+  if (a >= reinterpret_cast<uintptr_t>(lo) && a + 32 <= reinterpret_cast<uintptr_t>(hi)) {
+    const uint4 x = dev::load_stream(reinterpret_cast<const void*>(a)), y = dev::load_stream(reinterpret_cast<const void*>(a + 16));
+    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w, w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
+    if (off & 8u) {
+#pragma unroll
+      for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (off & 4u) {
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    if (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2u) * 8u);
+    }
+  } else {
+    T v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const char*>(p + i + 1) <= hi ? p[i] : dev::Vec16<T>::from_float(0.0f);
+    memcpy(w, v, 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T>
+__device__ __forceinline__ void fetch_any(const T* p, const char* lo, const char* hi, dev::Raw8<T>& r) {
+  r.a = load16_any(p, lo, hi);
+  if constexpr (sizeof(T) == 4) r.b = load16_any(p + 4, lo, hi);
+}
+
 // ---- lookup ------------------------------------------------------------------------------------------------------
 constexpr int kLookupT = 256;
 constexpr int kLookupAtOnce = 4;  // vectors of a lane on their way together
 
-// A warp for each token.
-template <typename T, bool VECTOR>
+// A warp for each token, rows of whole vectors.
+template <typename T>
 __global__ void __launch_bounds__(kLookupT) embedding_kernel(const __grid_constant__ NangilaEmbeddingParams p) {
   const int lane = threadIdx.x & 31;
   const int64_t warps = int64_t(gridDim.x) * (kLookupT / 32);
@@ -43,25 +81,55 @@ __global__ void __launch_bounds__(kLookupT) embedding_kernel(const __grid_consta
     const bool inside = id >= 0 && id < p.rows;
     const T* from = static_cast<const T*>(p.weight) + (inside ? id : 0) * p.weight_stride;
     T* to = static_cast<T*>(p.out) + i * p.d;
-    if (VECTOR) {
-      for (int c = lane * 8; c < p.d; c += 256 * kLookupAtOnce) {
-        dev::Raw8<T> raw[kLookupAtOnce];
+    for (int c = lane * 8; c < p.d; c += 256 * kLookupAtOnce) {
+      dev::Raw8<T> raw[kLookupAtOnce];
 #pragma unroll
-        for (int k = 0; k < kLookupAtOnce; ++k)
-          if (c + 256 * k < p.d) dev::fetch(from + c + 256 * k, raw[k]);
+      for (int k = 0; k < kLookupAtOnce; ++k)
+        if (c + 256 * k < p.d) dev::fetch(from + c + 256 * k, raw[k]);
 #pragma unroll
-        for (int k = 0; k < kLookupAtOnce; ++k) {
-          if (c + 256 * k >= p.d) continue;
-          float v[8];
-          dev::unpack(raw[k], v);
+      for (int k = 0; k < kLookupAtOnce; ++k) {
+        if (c + 256 * k >= p.d) continue;
+        float v[8];
+        dev::unpack(raw[k], v);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = inside ? v[e] * p.scale : __uint_as_float(0x7fc00000u);
-          dev::pack(v, raw[k]);
-          dev::put(to + c + 256 * k, raw[k]);
-        }
+        for (int e = 0; e < 8; ++e) v[e] = inside ? v[e] * p.scale : __uint_as_float(0x7fc00000u);
+        dev::pack(v, raw[k]);
+        dev::put(to + c + 256 * k, raw[k]);
       }
+    }
+  }
+}
+// Rows that start anywhere: the packed output is cut into sixteen bytes each, and each of those is put together from its row, or value by value where two rows meet.
+// (A value at a time, a warp for each token, 16381 x 769 fp16 took 24 us.)
+template <typename T, typename Index>
+__global__ void __launch_bounds__(kLookupT) embedding_any_kernel(const __grid_constant__ NangilaEmbeddingParams p, Index values) {
+  constexpr int N = 16 / sizeof(T);
+  const char* lo = static_cast<const char*>(p.weight);
+  const char* hi = lo + ((p.rows - 1) * p.weight_stride + p.d) * int64_t(sizeof(T));
+  const float nan = __uint_as_float(0x7fc00000u);
+  const Index step = Index(gridDim.x) * kLookupT * N;
+  for (Index at = (Index(blockIdx.x) * kLookupT + threadIdx.x) * N; at < values; at += step) {
+    const Index i = at / Index(p.d);
+    const int col = int(at - i * Index(p.d));
+    T* to = static_cast<T*>(p.out) + at;
+    if (col + N <= p.d) {
+      const int64_t id = id_at(p.ids, p.ids_64, i);
+      const bool inside = id >= 0 && id < p.rows;
+      const uint4 raw = load16_any(static_cast<const T*>(p.weight) + (inside ? id : 0) * p.weight_stride + col, lo, hi);
+      T v[N];
+      memcpy(v, &raw, 16);
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] = dev::Vec16<T>::from_float(inside ? dev::Vec16<T>::to_float(v[k]) * p.scale : nan);
+      uint4 out;
+      memcpy(&out, v, 16);
+      *reinterpret_cast<uint4*>(to) = out;
     } else {
-      for (int c = lane; c < p.d; c += 32) to[c] = dev::Vec16<T>::from_float(inside ? dev::Vec16<T>::to_float(from[c]) * p.scale : __uint_as_float(0x7fc00000u));
+      for (int k = 0; k < N && at + Index(k) < values; ++k) {
+        const Index j = (at + Index(k)) / Index(p.d);
+        const int64_t id = id_at(p.ids, p.ids_64, j);
+        const bool inside = id >= 0 && id < p.rows;
+        to[k] = dev::Vec16<T>::from_float(inside ? dev::Vec16<T>::to_float(static_cast<const T*>(p.weight)[id * p.weight_stride + int64_t(at + Index(k) - j * Index(p.d))]) * p.scale : nan);
+      }
     }
   }
 }
@@ -75,10 +143,13 @@ constexpr int kSortSmem = ((kSortT / 32) + 1) * (4 << kMaxDigit) + 256;
 constexpr int kSumT = 256;
 constexpr int kSumAtOnce = 8;      // rows on their way together
 constexpr int kJoinT = 512;
+constexpr int kFew = 32;           // further pieces of a run that a warp adds up by itself
+constexpr int kFillT = 512;
 
 struct Sorted {
   uint32_t *key[2], *at[2];        // ids and positions, there and back
-  uint32_t* crossing;              // [0]: how many; from [1] on: pieces in which a run begins that goes on behind them
+  uint32_t* crossing;              // runs that begin in one piece and go on behind it. [0], [1]: how many of up to kFew pieces more, and of more than that
+  uint2* run;                      // [pieces] each the first piece and how many more: the short ones from the front, the long ones from the back
   float* partial;                  // [2 * pieces][pitch]
   int passes, digit;               // bits of a digit
   int last;                        // which of the two buffers the sorted ones are in
@@ -92,16 +163,16 @@ __device__ __forceinline__ uint32_t load_cluster(uint32_t a) {
   return v;
 }
 
+// Zeros in all of dw, two CTAs on each SM that stay. The sort is set up beside them. (In CTAs of the sort's own launch, whose clusters of eight do not all fit at a time, 131 MB took
+// 35 us, for 24.)
+__global__ void __launch_bounds__(kFillT) embedding_fill_kernel(uint8_t* dw, int64_t bytes) {
+  may_follow();
+  const int64_t step = int64_t(gridDim.x) * kFillT, first = int64_t(blockIdx.x) * kFillT + threadIdx.x, wide = bytes / 32;
+  for (int64_t i = first; i < wide; i += step) asm volatile("st.global.v8.b32 [%0], {%1, %1, %1, %1, %1, %1, %1, %1};" ::"l"(dw + i * 32), "r"(0) : "memory");
+  if (first < (bytes & 31)) dw[wide * 32 + first] = 0;
+}
+// Ends behind the kernel before it, which it does not wait for until then: what follows finds the work of both.
 __global__ void __launch_bounds__(kSortT, 1) embedding_sort_kernel(const __grid_constant__ NangilaEmbeddingGradParams p, const __grid_constant__ Sorted s) {
-  if (blockIdx.x >= kSortCtas) {  // zeros
-    uint4* to = static_cast<uint4*>(p.dw);
-    const int64_t bytes = p.rows * p.d * (p.dtype == NANGILA_F32 ? 4 : 2), words = bytes / 16;
-    const int64_t step = int64_t(gridDim.x - kSortCtas) * kSortT;
-    const int64_t first = int64_t(blockIdx.x - kSortCtas) * kSortT + threadIdx.x;
-    for (int64_t i = first; i < words; i += step) to[i] = make_uint4(0, 0, 0, 0);
-    if (first < (bytes & 15)) static_cast<uint8_t*>(p.dw)[words * 16 + first] = 0;
-    return;
-  }
   extern __shared__ uint32_t smem[];
   uint32_t* count = smem;                                       // [warp][digit]
   uint32_t* total = count + (kSortT / 32) * (1 << kMaxDigit);   // of this CTA's positions, by digit
@@ -109,7 +180,7 @@ __global__ void __launch_bounds__(kSortT, 1) embedding_sort_kernel(const __grid_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, digits = 1 << s.digit;
   const uint32_t rank = blockIdx.x;
   const int64_t from = int64_t(int(rank) * (kSortT / 32) + warp) * s.per_warp, to = min(p.n, from + s.per_warp);
-  if (rank == 0 && threadIdx.x == 0) s.crossing[0] = 0;
+  if (rank == 0 && threadIdx.x < 2) s.crossing[threadIdx.x] = 0;
   for (int pass = 0; pass < s.passes; ++pass) {
     const uint32_t *src_key = s.key[(pass + 1) & 1], *src_at = s.at[(pass + 1) & 1];
     uint32_t *dst_key = s.key[pass & 1], *dst_at = s.at[pass & 1];
@@ -180,59 +251,71 @@ __global__ void __launch_bounds__(kSortT, 1) embedding_sort_kernel(const __grid_
     }
     sm100::cluster_sync();  // what one CTA has written, all read in the next pass
   }
+  follow();
 }
 
-// A thread takes VECTOR ? 8 : 1 adjacent columns of a piece; threadIdx.y: the piece of the CTA's.
+// A thread takes eight adjacent columns of a piece; threadIdx.y: the piece of the CTA's. VECTOR: rows start on sixteen bytes and end with a whole eight.
 template <typename T, bool VECTOR>
 __global__ void __launch_bounds__(kSumT) embedding_sum_kernel(const __grid_constant__ NangilaEmbeddingGradParams p, const __grid_constant__ Sorted s) {
-  constexpr int W = VECTOR ? 8 : 1;
-  const int piece = blockIdx.x * blockDim.y + threadIdx.y, col = (blockIdx.y * blockDim.x + threadIdx.x) * W;
+  const int piece = blockIdx.x * blockDim.y + threadIdx.y, col = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
   follow();
   if (piece >= s.pieces || col >= p.d) return;
   const uint32_t *key = s.key[s.last], *at = s.at[s.last];
   const int64_t s0 = int64_t(piece) * s.piece, s1 = min(p.n, s0 + s.piece);
-  const T* dy = static_cast<const T*>(p.dy) + col;
+  const T* dy = static_cast<const T*>(p.dy);
+  const char* lo = reinterpret_cast<const char*>(dy);
+  const char* hi = lo + ((p.n - 1) * p.dy_stride + p.d) * int64_t(sizeof(T));
   uint32_t current = key[s0];
   bool before = s0 > 0 && key[s0 - 1] == current;
-  float acc[W];
+  float acc[8];
 #pragma unroll
-  for (int k = 0; k < W; ++k) acc[k] = 0.0f;
+  for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
   auto finish = [&](bool goes_on) {
     if (current >= uint32_t(p.rows)) return;
     if (!before && !goes_on) {
       T* to = static_cast<T*>(p.dw) + int64_t(current) * p.d + col;
-      if constexpr (VECTOR) {
-        float v[8];
+      float v[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = acc[k] * p.scale;
+      for (int k = 0; k < 8; ++k) v[k] = acc[k] * p.scale;
+      if constexpr (VECTOR) {
         dev::Raw8<T> raw;
         dev::pack(v, raw);
         dev::put(to, raw);
       } else {
-        *to = dev::Vec16<T>::from_float(acc[0] * p.scale);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (col + k < p.d) to[k] = dev::Vec16<T>::from_float(v[k]);
       }
     } else {
-      float* to = s.partial + (int64_t(2) * piece + (before ? 0 : 1)) * s.pitch + col;
-      if constexpr (VECTOR) {
-        reinterpret_cast<float4*>(to)[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        reinterpret_cast<float4*>(to)[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-      } else {
-        *to = acc[0];
+      float4* to = reinterpret_cast<float4*>(s.partial + (int64_t(2) * piece + (before ? 0 : 1)) * s.pitch + col);
+      to[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      to[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      if (!before && col == 0) {
+        // how many pieces more begin with this id: twice as far at a time, then halved
+        auto begins = [&](int64_t j) { return (piece + j) * s.piece < p.n && key[(piece + j) * s.piece] == current; };
+        int64_t in = 1, out = 2;  // the last that is known to, and one that may not
+        while (begins(out)) in = out, out *= 2;
+        while (out - in > 1) {
+          const int64_t mid = (in + out) / 2;
+          if (begins(mid)) in = mid;
+          else out = mid;
+        }
+        // (in any order: each is summed by itself)
+        if (in <= kFew) s.run[atomicAdd(s.crossing, 1u)] = make_uint2(uint32_t(piece), uint32_t(in));
+        else s.run[s.pieces - 1 - atomicAdd(s.crossing + 1, 1u)] = make_uint2(uint32_t(piece), uint32_t(in));
       }
-      if (!before && col == 0) s.crossing[1 + atomicAdd(s.crossing, 1u)] = uint32_t(piece);  // (in any order: each is summed by itself)
     }
   };
   for (int64_t i0 = s0; i0 < s1; i0 += kSumAtOnce) {
     uint32_t k[kSumAtOnce];
-    dev::Raw8<T> raw[VECTOR ? kSumAtOnce : 1];
-    T one[VECTOR ? 1 : kSumAtOnce];
+    dev::Raw8<T> raw[kSumAtOnce];
 #pragma unroll
     for (int j = 0; j < kSumAtOnce; ++j) {
       k[j] = i0 + j < s1 ? key[i0 + j] : uint32_t(p.rows);
       if (k[j] >= uint32_t(p.rows)) continue;
-      const T* row = dy + int64_t(at[i0 + j]) * p.dy_stride;
+      const T* row = dy + int64_t(at[i0 + j]) * p.dy_stride + col;
       if constexpr (VECTOR) dev::fetch(row, raw[j]);
-      else one[j] = *row;
+      else fetch_any(row, lo, hi, raw[j]);
     }
 #pragma unroll
     for (int j = 0; j < kSumAtOnce; ++j) {
@@ -242,23 +325,19 @@ __global__ void __launch_bounds__(kSumT) embedding_sum_kernel(const __grid_const
         current = k[j];
         before = false;
 #pragma unroll
-        for (int c = 0; c < W; ++c) acc[c] = 0.0f;
+        for (int c = 0; c < 8; ++c) acc[c] = 0.0f;
       }
       if (current >= uint32_t(p.rows)) return;  // nothing but what is left out from here on
-      if constexpr (VECTOR) {
-        float v[8];
-        dev::unpack(raw[j], v);
+      float v[8];
+      dev::unpack(raw[j], v);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) acc[c] += v[c];
-      } else {
-        acc[0] += dev::Vec16<T>::to_float(one[j]);
-      }
+      for (int c = 0; c < 8; ++c) acc[c] += v[c];
     }
   }
   finish(s1 < p.n && key[s1] == current);
 }
 
-// 128 columns of a run that crosses pieces: sixteen groups of warps' lanes take every sixteenth partial sum, and are added up in order.
+// The runs that cross pieces, 128 columns at a time: a long one by the sixteen warps of a CTA, each with every sixteenth partial sum, added up in order; a short one by a warp.
 template <typename T>
 __global__ void __launch_bounds__(kJoinT) embedding_join_kernel(const __grid_constant__ NangilaEmbeddingGradParams p, const __grid_constant__ Sorted s) {
   constexpr int kGroups = kJoinT / 32;
@@ -267,33 +346,34 @@ __global__ void __launch_bounds__(kJoinT) embedding_join_kernel(const __grid_con
   const uint32_t* key = s.key[s.last];
   const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
   const int blocks = (p.d + 127) / 128;
-  const int64_t tasks = int64_t(s.crossing[0]) * blocks;
-  for (int64_t task = blockIdx.x; task < tasks; task += gridDim.x) {
-    const int64_t first = s.crossing[1 + task / blocks];
-    const int col = int(task % blocks) * 128 + lane * 4;
-    const uint32_t id = key[(first + 1) * s.piece];
-    // the last position with this id
-    int64_t lo = (first + 1) * s.piece, hi = p.n;
-    while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) / 2;
-      if (key[mid] == id) lo = mid;
-      else hi = mid;
-    }
-    const int64_t count = lo / s.piece - first;  // pieces behind the first
+  auto sum_of = [&](const uint2 run, int col, int from, int step) {
     float4 sum = make_float4(0, 0, 0, 0);
-    if (col < p.d) {
 #pragma unroll 4
-      for (int64_t j = group; j <= count; j += kGroups) {
-        const float4 v = *reinterpret_cast<const float4*>(s.partial + (2 * (first + j) + (j == 0 ? 1 : 0)) * s.pitch + col);
-        sum.x += v.x;
-        sum.y += v.y;
-        sum.z += v.z;
-        sum.w += v.w;
-      }
+    for (int j = from; j <= int(run.y); j += step) {
+      const float4 v = *reinterpret_cast<const float4*>(s.partial + (int64_t(2) * (run.x + j) + (j == 0 ? 1 : 0)) * s.pitch + col);
+      sum.x += v.x;
+      sum.y += v.y;
+      sum.z += v.z;
+      sum.w += v.w;
     }
+    return sum;
+  };
+  auto put = [&](const uint2 run, int col, const float4& sum) {
+    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+    T* to = static_cast<T*>(p.dw) + int64_t(key[int64_t(run.x + 1) * s.piece]) * p.d + col;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (col + k < p.d) to[k] = dev::Vec16<T>::from_float(v[k] * p.scale);
+  };
+  const int64_t few = int64_t(s.crossing[0]) * blocks, many = int64_t(s.crossing[1]) * blocks;
+  for (int64_t task = blockIdx.x; task < many; task += gridDim.x) {
+    const uint2 run = s.run[s.pieces - 1 - task / blocks];
+    const int col = int(task % blocks) * 128 + lane * 4;
+    float4 sum = make_float4(0, 0, 0, 0);
+    if (col < p.d) sum = sum_of(run, col, group, kGroups);
     part[group][lane] = sum;
     __syncthreads();
-    if (group == 0) {
+    if (group == 0 && col < p.d) {
       for (int g = 1; g < kGroups; ++g) {
         const float4 v = part[g][lane];
         sum.x += v.x;
@@ -301,13 +381,14 @@ __global__ void __launch_bounds__(kJoinT) embedding_join_kernel(const __grid_con
         sum.z += v.z;
         sum.w += v.w;
       }
-      const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-      T* to = static_cast<T*>(p.dw) + int64_t(id) * p.d + col;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (col + k < p.d) to[k] = dev::Vec16<T>::from_float(v[k] * p.scale);
+      put(run, col, sum);
     }
     __syncthreads();
+  }
+  for (int64_t task = int64_t(blockIdx.x) * kGroups + group; task < few; task += int64_t(gridDim.x) * kGroups) {
+    const uint2 run = s.run[task / blocks];
+    const int col = int(task % blocks) * 128 + lane * 4;
+    if (col < p.d) put(run, col, sum_of(run, col, 0, 1));
   }
 }
 
@@ -317,11 +398,18 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 template <typename T>
 int lookup(const NangilaEmbeddingParams& p, cudaStream_t stream) {
   const bool vector = p.d % 8 == 0 && aligned16(p.weight) && aligned16(p.out) && p.weight_stride * int64_t(sizeof(T)) % 16 == 0;
-  auto* kernel = vector ? embedding_kernel<T, true> : embedding_kernel<T, false>;
   int resident = 0;
-  if (const cudaError_t e = resident_ctas(reinterpret_cast<const void*>(kernel), kLookupT, 0, &resident)) return int(e);
-  const int64_t want = (p.n + kLookupT / 32 - 1) / (kLookupT / 32);
-  kernel<<<unsigned(std::min<int64_t>(want, resident)), kLookupT, 0, stream>>>(p);
+  if (vector) {
+    if (const cudaError_t e = resident_ctas(reinterpret_cast<const void*>(embedding_kernel<T>), kLookupT, 0, &resident)) return int(e);
+    const int64_t want = (p.n + kLookupT / 32 - 1) / (kLookupT / 32);
+    embedding_kernel<T><<<unsigned(std::min<int64_t>(want, resident)), kLookupT, 0, stream>>>(p);
+    return int(cudaGetLastError());
+  }
+  const int64_t values = p.n * p.d, each = kLookupT * 16 / int64_t(sizeof(T));
+  const unsigned ctas = unsigned(std::min<int64_t>((values + each - 1) / each, 148 * 8));
+  // (where a position and the step behind the last fit into 32 bits, divisions are short)
+  if (values < (int64_t(1) << 31)) embedding_any_kernel<T, uint32_t><<<ctas, kLookupT, 0, stream>>>(p, uint32_t(values));
+  else embedding_any_kernel<T, uint64_t><<<ctas, kLookupT, 0, stream>>>(p, uint64_t(values));
   return int(cudaGetLastError());
 }
 
@@ -349,7 +437,8 @@ Sorted layout(int64_t n, int64_t rows, int32_t d, uint8_t* base, int64_t* bytes)
   while (s.piece < 64 && n > int64_t(s.piece) * 512) s.piece *= 2;
   s.pieces = int((n + s.piece - 1) / s.piece);
   s.pitch = (d + 7) / 8 * 8;
-  s.crossing = reinterpret_cast<uint32_t*>(take((int64_t(s.pieces) + 1) * 4));
+  s.crossing = reinterpret_cast<uint32_t*>(take(8));
+  s.run = reinterpret_cast<uint2*>(take(int64_t(s.pieces) * 8));
   s.partial = reinterpret_cast<float*>(take(int64_t(2) * s.pieces * s.pitch * 4));
   *bytes = used;
   return s;
@@ -361,34 +450,32 @@ int gradient(const NangilaEmbeddingGradParams& p, cudaStream_t stream) {
   const Sorted s = layout(p.n, p.rows, p.d, static_cast<uint8_t*>(p.workspace), &bytes);
   int resident = 0;
   if (const cudaError_t e = resident_ctas(reinterpret_cast<const void*>(embedding_sort_kernel), kSortT, kSortSmem, &resident)) return int(e);
-  const int64_t words = p.rows * p.d * int64_t(sizeof(T)) / 16;
-  const int zero_clusters = int(std::max<int64_t>(1, std::min<int64_t>(resident / kSortCtas - 1, (words + kSortT * kSortCtas - 1) / (kSortT * kSortCtas))));
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kSortCtas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  const int64_t size = p.rows * p.d * int64_t(sizeof(T));
+  embedding_fill_kernel<<<unsigned(std::min<int64_t>((size / 32 + kFillT) / kFillT, 2 * 148)), kFillT, 0, stream>>>(static_cast<uint8_t*>(p.dw), size);
+  if (const cudaError_t e = cudaGetLastError()) return int(e);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kSortCtas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(kSortCtas * (1 + zero_clusters)));
+  cfg.gridDim = dim3(kSortCtas);
   cfg.blockDim = dim3(kSortT);
   cfg.dynamicSmemBytes = kSortSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   if (const cudaError_t e = cudaLaunchKernelEx(&cfg, embedding_sort_kernel, p, s)) return int(e);
   const bool vector = p.d % 8 == 0 && aligned16(p.dy) && aligned16(p.dw) && p.dy_stride * int64_t(sizeof(T)) % 16 == 0;
-  const int threads = vector ? p.d / 8 : p.d;
+  const int threads = (p.d + 7) / 8;
   int x = 32;
   while (x < kSumT && x < threads) x *= 2;
   const int y = kSumT / x;
   auto* sum = vector ? embedding_sum_kernel<T, true> : embedding_sum_kernel<T, false>;
-  cfg = {};
-  cudaLaunchAttribute next[1];
-  next[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  next[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(unsigned((s.pieces + y - 1) / y), unsigned((threads + x - 1) / x));
   cfg.blockDim = dim3(unsigned(x), unsigned(y));
-  cfg.stream = stream;
-  cfg.attrs = next;
+  cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
   if (const cudaError_t e = cudaLaunchKernelEx(&cfg, sum, p, s)) return int(e);
   if (s.pieces < 2) return 0;
@@ -401,7 +488,7 @@ int gradient(const NangilaEmbeddingGradParams& p, cudaStream_t stream) {
 
 extern "C" int nangila_embedding(const NangilaEmbeddingParams* p, cudaStream_t stream) {
   using namespace nangila;
-  if (!p || !p->ids || !p->weight || !p->out || p->n < 0 || p->rows < 1 || p->d < 1) return int(cudaErrorInvalidValue);
+  if (!p || !p->ids || !p->weight || !p->out || !aligned16(p->out) || p->n < 0 || p->rows < 1 || p->d < 1) return int(cudaErrorInvalidValue);
   if (p->n == 0) return 0;
   try {
     switch (p->dtype) {
@@ -423,7 +510,7 @@ extern "C" int64_t nangila_embedding_workspace(int64_t n, int64_t rows, int32_t 
 
 extern "C" int nangila_embedding_backward(const NangilaEmbeddingGradParams* p, cudaStream_t stream) {
   using namespace nangila;
-  if (!p || !p->ids || !p->dy || !p->dw || !p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255u) || p->n < 1 || p->n > NANGILA_EMBEDDING_MAX_TOKENS || p->rows < 1 ||
+  if (!p || !p->ids || !p->dy || !p->dw || !p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255u) || (reinterpret_cast<uintptr_t>(p->dw) & 31u) || p->n < 1 || p->n > NANGILA_EMBEDDING_MAX_TOKENS || p->rows < 1 ||
       p->rows > NANGILA_EMBEDDING_MAX_ROWS || p->d < 1)
     return int(cudaErrorInvalidValue);
   try {

@@ -29,7 +29,7 @@ int nangila_dropout(const NangilaDropoutParams* p, cudaStream_t stream);
 typedef struct {
   const void* ids;         /* n adjacent int64 (ids_64) or int32 */
   const void* weight;      /* rows weight_stride elements apart */
-  void* out;               /* packed */
+  void* out;               /* packed, 16-byte aligned */
   int64_t n, rows, weight_stride;
   int32_t d, dtype, ids_64;
   float scale;
@@ -40,7 +40,7 @@ int nangila_embedding(const NangilaEmbeddingParams* p, cudaStream_t stream);
 typedef struct {
   const void* ids;
   const void* dy;          /* rows dy_stride elements apart */
-  void* dw;                /* packed */
+  void* dw;                /* packed, 32-byte aligned */
   void* workspace;         /* nangila_embedding_workspace() bytes, 256-byte aligned */
   int64_t n, rows, dy_stride, padding; /* padding: -1 for none */
   int32_t d, dtype, ids_64;
