@@ -24,111 +24,160 @@ namespace {
 
 constexpr int kT = 256;
 
-__device__ __forceinline__ uint4 philox(uint64_t block, uint32_t draw, uint32_t which, uint2 key) {
+// The keys of the ten rounds: in the kernel's parameters, where instructions take them from, or worked out by each thread from a seed in memory.
+struct Keys {
+  uint32_t x[10], y[10];
+};
+__host__ __device__ __forceinline__ void make_keys(uint64_t seed, Keys& k) {
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    k.x[r] = uint32_t(seed) + uint32_t(r) * 0x9E3779B9u;
+    k.y[r] = uint32_t(seed >> 32) + uint32_t(r) * 0xBB67AE85u;
+  }
+}
+struct Launch {
+  NangilaDropoutParams p;
+  Keys keys;
+  uint32_t upper, lower;  // of `least`, which is below 2^32
+};
+__device__ __forceinline__ uint4 philox(uint64_t block, uint32_t draw, uint32_t which, const Keys& k) {
   uint4 c = make_uint4(uint32_t(block), uint32_t(block >> 32), draw, which);
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t a = uint64_t(0xD2511F53u) * c.x, b = uint64_t(0xCD9E8D57u) * c.z;
-    c = make_uint4(uint32_t(b >> 32) ^ c.y ^ key.x, uint32_t(b), uint32_t(a >> 32) ^ c.w ^ key.y, uint32_t(a));
-    key.x += 0x9E3779B9u;
-    key.y += 0xBB67AE85u;
+    c = make_uint4(uint32_t(b >> 32) ^ c.y ^ k.x[r], uint32_t(b), uint32_t(a >> 32) ^ c.w ^ k.y[r], uint32_t(a));
   }
   return c;
 }
-// A block's eight values: v * scale where they are kept, 0 where not. An element's upper half is compared where it lies in its word.
-struct Limits {
-  uint32_t upper, lower;  // of `least`; upper up to 2^16 - 1
-  bool none;              // nothing is kept
-};
-__device__ __forceinline__ void drop8(float (&v)[8], float scale, uint64_t block, uint32_t draw, uint2 key, const Limits& limit) {
-  const uint4 c = philox(block, draw, 0, key);
+// A block's eight values, c its numbers' upper halves: v * scale where they reach `upper`, 0 where not. An upper half is compared where it lies in its word.
+__device__ __forceinline__ void drop8(float (&v)[8], float scale, const uint4& c, uint32_t upper) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w}, least = upper << 16;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = ((i & 1) ? w[i / 2] : w[i / 2] << 16) >= least ? v[i] * scale : 0.0f;
+}
+// Whether one of the upper halves may equal that of `least`: an equal one leaves a zero half of x, which borrows into its top bit (one above a zero half may too: looked at for nothing).
+__device__ __forceinline__ bool tied8(const uint4& c, uint32_t upper) {
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-  if (limit.lower != 0) {
-    // a half that is equal leaves a zero half of x, which borrows into its top bit (one above a zero half may too: looked at for nothing)
-    uint32_t tied = 0;
+  uint32_t tied = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t x = w[i] ^ (limit.upper * 0x10001u);
-      tied |= (x - 0x00010001u) & ~x;
-    }
-    if ((tied & 0x80008000u) != 0) {
-      const uint4 e = philox(block, draw, 1, key);
-      const uint32_t l[4] = {e.x, e.y, e.z, e.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t u = (i & 1) ? w[i / 2] >> 16 : w[i / 2] & 0xffffu, d = (i & 1) ? l[i / 2] >> 16 : l[i / 2] & 0xffffu;
-        if (u == limit.upper && d < limit.lower) v[i] = 0.0f;
-      }
-    }
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = w[i] ^ (upper * 0x10001u);
+    tied |= (x - 0x00010001u) & ~x;
   }
-  const uint32_t least = limit.upper << 16;
+  return (tied & 0x80008000u) != 0;
+}
+// Of the block's elements that tied, those whose lower half is below that of `least`: written once more, as dropped.
+template <typename T>
+__device__ __noinline__ void settle8(const Launch& a, int64_t block, uint4 c, const Keys& keys) {
+  const uint4 e = philox(uint64_t(block), a.p.draw, 1, keys);
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w}, l[4] = {e.x, e.y, e.z, e.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = ((i & 1) ? w[i / 2] : w[i / 2] << 16) >= least && !limit.none ? v[i] * scale : 0.0f;
+  for (int i = 0; i < 8; ++i) {
+    const int64_t at = block * 8 + i;
+    const uint32_t u = (i & 1) ? w[i / 2] >> 16 : w[i / 2] & 0xffffu, d = (i & 1) ? l[i / 2] >> 16 : l[i / 2] & 0xffffu;
+    if (at < a.p.n && u == a.upper && d < a.lower) static_cast<T*>(a.p.out)[at] = a.p.residual != nullptr ? static_cast<const T*>(a.p.residual)[at] : dev::Vec16<T>::from_float(0.0f);
+  }
 }
 
-// Blocks of a thread on their way together. (One at a time, the way to memory and the generator's ten rounds took turns: 8192 x 2048 bf16 with a residual 24 us, the gradient 23.)
-template <typename T>
-constexpr int kAtOnce = sizeof(T) == 4 ? 2 : 4;
+// Copies of a thread's own to its own place in shared memory: nobody else waits for them.
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <typename T, bool VECTOR>
-__global__ void __launch_bounds__(kT) dropout_kernel(const __grid_constant__ NangilaDropoutParams p) {
-  const uint64_t seed = p.seed_ptr != nullptr ? uint64_t(*p.seed_ptr) : p.seed;
-  const uint2 key = make_uint2(uint32_t(seed), uint32_t(seed >> 32));
-  const Limits limit{uint32_t(p.least >> 16) & 0xffffu, uint32_t(p.least) & 0xffffu, p.least >> 32 != 0};
+// A thread's blocks are on their way through shared memory, four of them (in fp32 two) at a time: with 32 warps an SM, 64 KB (and as much of the residual). In registers, one or two at a time, the
+// loads of all SMs did not cover the way to memory: 8192 x 2048 bf16 took 19 to 21 us, floor 10. The numbers themselves take 5 of it (twenty 32 x 32 bit products a block).
+template <typename T>
+constexpr int kAheadOf = sizeof(T) == 4 ? 2 : 4;
+
+template <typename T, bool VECTOR, bool SEED_IN_MEMORY>
+__global__ void __launch_bounds__(kT, 4) dropout_kernel(const __grid_constant__ Launch l) {
+  constexpr int kAhead = kAheadOf<T>, kParts = sizeof(T) / 2;  // sixteen bytes each, of a block
+  extern __shared__ uint4 ring[];        // [residual][kAhead][kParts][thread]
+  const NangilaDropoutParams& p = l.p;
+  Keys made;
+  if (SEED_IN_MEMORY) make_keys(uint64_t(*p.seed_ptr), made);
+  const Keys& keys = SEED_IN_MEMORY ? made : l.keys;
   const T* x = static_cast<const T*>(p.x);
   const T* r = static_cast<const T*>(p.residual);
   T* out = static_cast<T*>(p.out);
   const int64_t step = int64_t(gridDim.x) * kT, first = int64_t(blockIdx.x) * kT + threadIdx.x;
   const int64_t whole = VECTOR ? p.n / 8 : 0;
   if (VECTOR) {
-    for (int64_t b0 = first; b0 < whole; b0 += kAtOnce<T> * step) {
-      dev::Raw8<T> raw[kAtOnce<T>], add[kAtOnce<T>];
+    auto slot = [&](int which, int stage, int part) { return ring + ((which * kAhead + stage) * kParts + part) * kT + threadIdx.x; };
+    auto fetch = [&](int64_t b, int stage) {
+      if (b < whole) {
 #pragma unroll
-      for (int j = 0; j < kAtOnce<T>; ++j) {
-        const int64_t b = b0 + j * step;
-        if (b >= whole) break;
-        dev::fetch(x + b * 8, raw[j]);
-        if (r != nullptr) dev::fetch(r + b * 8, add[j]);
-      }
-#pragma unroll
-      for (int j = 0; j < kAtOnce<T>; ++j) {
-        const int64_t b = b0 + j * step;
-        if (b >= whole) break;
-        float v[8], a[8];
-        dev::unpack(raw[j], v);
-        drop8(v, p.scale, uint64_t(b), p.draw, key, limit);
-        if (r != nullptr) {
-          dev::unpack(add[j], a);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] += a[i];
+        for (int k = 0; k < kParts; ++k) {
+          copy16(slot(0, stage, k), reinterpret_cast<const uint4*>(x + b * 8) + k);
+          if (r != nullptr) copy16(slot(1, stage, k), reinterpret_cast<const uint4*>(r + b * 8) + k);
         }
-        dev::pack(v, raw[j]);
-        dev::put(out + b * 8, raw[j]);
       }
+      copies_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) fetch(first + k * step, k);
+    int stage = 0;
+    for (int64_t b = first; b < whole; b += step) {
+      const uint4 c = philox(uint64_t(b), p.draw, 0, keys);
+      copies_wait_but<kAhead - 1>();
+      dev::Raw8<T> raw;
+      float v[8], a[8];
+      raw.a = *slot(0, stage, 0);
+      if constexpr (kParts > 1) raw.b = *slot(0, stage, 1);
+      dev::unpack(raw, v);
+      drop8(v, p.scale, c, l.upper);
+      if (r != nullptr) {
+        raw.a = *slot(1, stage, 0);
+        if constexpr (kParts > 1) raw.b = *slot(1, stage, 1);
+        dev::unpack(raw, a);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += a[i];
+      }
+      fetch(b + kAhead * step, stage);
+      stage = stage + 1 == kAhead ? 0 : stage + 1;
+      dev::pack(v, raw);
+      dev::put(out + b * 8, raw);
+      if (tied8(c, l.upper) && l.lower != 0) settle8<T>(l, b, c, keys);
     }
+    copies_wait_but<0>();
   }
   for (int64_t b = whole + first; b < (p.n + 7) / 8; b += step) {  // the last elements, or all of them one by one
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = b * 8 + i < p.n ? dev::Vec16<T>::to_float(x[b * 8 + i]) : 0.0f;
-    drop8(v, p.scale, uint64_t(b), p.draw, key, limit);
+    const uint4 c = philox(uint64_t(b), p.draw, 0, keys);
+    drop8(v, p.scale, c, l.upper);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int64_t at = b * 8 + i;
       if (at < p.n) out[at] = dev::Vec16<T>::from_float(r != nullptr ? v[i] + dev::Vec16<T>::to_float(r[at]) : v[i]);
     }
+    if (tied8(c, l.upper) && l.lower != 0) settle8<T>(l, b, c, keys);
   }
 }
 
 template <typename T>
 int launch(const NangilaDropoutParams& p, cudaStream_t stream) {
+  if (p.least >> 32 != 0) {  // nothing is kept
+    const size_t bytes = size_t(p.n) * sizeof(T);
+    return int(p.residual != nullptr ? cudaMemcpyAsync(p.out, p.residual, bytes, cudaMemcpyDeviceToDevice, stream) : cudaMemsetAsync(p.out, 0, bytes, stream));
+  }
+  Launch l;
+  l.p = p;
+  make_keys(p.seed, l.keys);
+  l.upper = uint32_t(p.least >> 16);
+  l.lower = uint32_t(p.least) & 0xffffu;
   auto aligned = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
   const bool vector = aligned(p.x) && aligned(p.residual) && aligned(p.out);
-  auto* kernel = vector ? dropout_kernel<T, true> : dropout_kernel<T, false>;
+  auto* kernel = p.seed_ptr != nullptr ? (vector ? dropout_kernel<T, true, true> : dropout_kernel<T, false, true>) : (vector ? dropout_kernel<T, true, false> : dropout_kernel<T, false, false>);
+  constexpr size_t kRing = 2 * kAheadOf<T> * (sizeof(T) / 2) * kT * sizeof(uint4);  // with a residual
   int resident = 0;
-  if (const cudaError_t e = resident_ctas(reinterpret_cast<const void*>(kernel), kT, 0, &resident)) return int(e);
+  if (const cudaError_t e = resident_ctas(reinterpret_cast<const void*>(kernel), kT, kRing, &resident)) return int(e);
   const int64_t want = ((p.n + 7) / 8 + kT - 1) / kT;
-  kernel<<<unsigned(std::min<int64_t>(want, resident)), kT, 0, stream>>>(p);
+  kernel<<<unsigned(std::min<int64_t>(want, resident)), kT, vector ? (p.residual != nullptr ? kRing : kRing / 2) : 0, stream>>>(l);
   return int(cudaGetLastError());
 }
 

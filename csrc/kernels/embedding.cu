@@ -30,41 +30,32 @@ __device__ __forceinline__ int64_t id_at(const void* ids, int ids_64, int64_t i)
   return ids_64 ? static_cast<const int64_t*>(ids)[i] : int64_t(static_cast<const int32_t*>(ids)[i]);
 }
 
-// Sixteen bytes from any address of a T, out of the two aligned sixteen that hold them. Those have to lie in the tensor, from `lo` to `hi`; near its ends
-// values are read one by one, and those behind its end are zero.
-template <typename T>
-__device__ __forceinline__ uint4 load16_any(const T* p, const char* lo, const char* hi) {
-  constexpr int N = 16 / sizeof(T);
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p) & ~uintptr_t(15);
-  const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(p) & 15u);
-  uint32_t w[8];
-  if (a >= reinterpret_cast<uintptr_t>(lo) && a + 32 <= reinterpret_cast<uintptr_t>(hi)) {
-    const uint4 x = dev::load_stream(reinterpret_cast<const void*>(a)), y = dev::load_stream(reinterpret_cast<const void*>(a + 16));
-    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w, w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
-    if (off & 8u) {
-#pragma unroll
-      for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-    }
-    if (off & 4u) {
-#pragma unroll
-      for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-    }
-    if (sizeof(T) == 2) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2u) * 8u);
-    }
-  } else {
-    T v[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const char*>(p + i + 1) <= hi ? p[i] : dev::Vec16<T>::from_float(0.0f);
-    memcpy(w, v, 16);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+// Sixteen bytes from any address of a T, put together from the two aligned sixteen that hold them. An aligned sixteen that holds a byte of the tensor lies in the memory that
+// was allocated for it; one that holds none, from `lo` to `hi`, is not read, and is zero.
+struct Window {
+  uint4 x, y;
+};
+__device__ __forceinline__ Window window_at(const void* p, const char* lo, const char* hi) {
+  const char* a = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(15));
+  Window w;
+  w.x = w.y = make_uint4(0, 0, 0, 0);
+  if (a + 16 > lo && a < hi) w.x = __ldg(reinterpret_cast<const uint4*>(a));
+  if (a + 32 > lo && a + 16 < hi) w.y = __ldg(reinterpret_cast<const uint4*>(a + 16));
+  return w;
 }
 template <typename T>
-__device__ __forceinline__ void fetch_any(const T* p, const char* lo, const char* hi, dev::Raw8<T>& r) {
-  r.a = load16_any(p, lo, hi);
-  if constexpr (sizeof(T) == 4) r.b = load16_any(p + 4, lo, hi);
+__device__ __forceinline__ uint4 shifted(const Window& at, const void* p) {
+  const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(p));
+  uint32_t w[8] = {at.x.x, at.x.y, at.x.z, at.x.w, at.y.x, at.y.y, at.y.z, at.y.w};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) w[i] = (off & 8u) ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = (off & 4u) ? w[i + 1] : w[i];
+  if (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2u) * 8u);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // ---- lookup ------------------------------------------------------------------------------------------------------
@@ -99,36 +90,77 @@ __global__ void __launch_bounds__(kLookupT) embedding_kernel(const __grid_consta
     }
   }
 }
-// Rows that start anywhere: the packed output is cut into sixteen bytes each, and each of those is put together from its row, or value by value where two rows meet.
+// Rows that start anywhere: the packed output is cut into sixteen bytes each, and each of those is put together from its row, or from the two that meet in it.
 // (A value at a time, a warp for each token, 16381 x 769 fp16 took 24 us.)
 template <typename T, typename Index>
 __global__ void __launch_bounds__(kLookupT) embedding_any_kernel(const __grid_constant__ NangilaEmbeddingParams p, Index values) {
-  constexpr int N = 16 / sizeof(T);
+  constexpr int N = 16 / sizeof(T), kOnTheWay = 4;
   const char* lo = static_cast<const char*>(p.weight);
   const char* hi = lo + ((p.rows - 1) * p.weight_stride + p.d) * int64_t(sizeof(T));
   const float nan = __uint_as_float(0x7fc00000u);
+  auto row_of = [&](Index i, bool& inside) {
+    const int64_t id = id_at(p.ids, p.ids_64, i);
+    inside = id >= 0 && id < p.rows;
+    return static_cast<const T*>(p.weight) + (inside ? id : 0) * p.weight_stride;
+  };
+  auto scaled = [&](T v, bool inside) { return dev::Vec16<T>::from_float(inside ? dev::Vec16<T>::to_float(v) * p.scale : nan); };
   const Index step = Index(gridDim.x) * kLookupT * N;
-  for (Index at = (Index(blockIdx.x) * kLookupT + threadIdx.x) * N; at < values; at += step) {
-    const Index i = at / Index(p.d);
-    const int col = int(at - i * Index(p.d));
-    T* to = static_cast<T*>(p.out) + at;
-    if (col + N <= p.d) {
-      const int64_t id = id_at(p.ids, p.ids_64, i);
-      const bool inside = id >= 0 && id < p.rows;
-      const uint4 raw = load16_any(static_cast<const T*>(p.weight) + (inside ? id : 0) * p.weight_stride + col, lo, hi);
+  for (Index at0 = (Index(blockIdx.x) * kLookupT + threadIdx.x) * N; at0 < values; at0 += step * kOnTheWay) {
+    const T* from[kOnTheWay];
+    bool inside[kOnTheWay];
+    int col[kOnTheWay];
+    Window w[kOnTheWay];
+#pragma unroll
+    for (int j = 0; j < kOnTheWay; ++j) {
+      const Index at = at0 + step * j;
+      if (at >= values) break;
+      const Index i = at / Index(p.d);
+      col[j] = int(at - i * Index(p.d));
+      from[j] = row_of(i, inside[j]) + col[j];
+    }
+#pragma unroll
+    for (int j = 0; j < kOnTheWay; ++j)
+      if (at0 + step * j < values) w[j] = window_at(from[j], lo, hi);
+#pragma unroll
+    for (int j = 0; j < kOnTheWay; ++j) {
+      const Index at = at0 + step * j;
+      if (at >= values) break;
+      const uint4 raw = shifted<T>(w[j], from[j]);
       T v[N];
       memcpy(v, &raw, 16);
 #pragma unroll
-      for (int k = 0; k < N; ++k) v[k] = dev::Vec16<T>::from_float(inside ? dev::Vec16<T>::to_float(v[k]) * p.scale : nan);
-      uint4 out;
-      memcpy(&out, v, 16);
-      *reinterpret_cast<uint4*>(to) = out;
-    } else {
-      for (int k = 0; k < N && at + Index(k) < values; ++k) {
-        const Index j = (at + Index(k)) / Index(p.d);
-        const int64_t id = id_at(p.ids, p.ids_64, j);
-        const bool inside = id >= 0 && id < p.rows;
-        to[k] = dev::Vec16<T>::from_float(inside ? dev::Vec16<T>::to_float(static_cast<const T*>(p.weight)[id * p.weight_stride + int64_t(at + Index(k) - j * Index(p.d))]) * p.scale : nan);
+      for (int k = 0; k < N; ++k) v[k] = scaled(v[k], inside[j]);
+      T* to = static_cast<T*>(p.out) + at;
+      if (col[j] + N > p.d) {  // its end, and the next row's beginning
+        const int left = p.d - col[j];
+        bool in = false;
+        if (p.d >= N) {
+          const Index i = at / Index(p.d) + 1;
+          if (int64_t(i) < p.n) {
+            const T* row = row_of(i, in);
+            const uint4 next = shifted<T>(window_at(row - left, lo, hi), row - left);
+            T u[N];
+            memcpy(u, &next, 16);
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+              if (k >= left) v[k] = scaled(u[k], in);
+          }
+        } else {
+          for (int k = left; k < N && at + Index(k) < values; ++k) {
+            const Index i = (at + Index(k)) / Index(p.d);
+            const T* row = row_of(i, in);
+            v[k] = scaled(row[at + Index(k) - i * Index(p.d)], in);
+          }
+        }
+      }
+      if (at + N <= values) {
+        uint4 out;
+        memcpy(&out, v, 16);
+        *reinterpret_cast<uint4*>(to) = out;
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          if (at + Index(k) < values) to[k] = v[k];
       }
     }
   }
@@ -141,10 +173,10 @@ constexpr int kSortWarps = kSortCtas * kSortT / 32;
 constexpr int kMaxDigit = 10;      // bits
 constexpr int kSortSmem = ((kSortT / 32) + 1) * (4 << kMaxDigit) + 256;
 constexpr int kSumT = 256;
-constexpr int kSumAtOnce = 8;      // rows on their way together
 constexpr int kJoinT = 512;
 constexpr int kFew = 32;           // further pieces of a run that a warp adds up by itself
 constexpr int kFillT = 512;
+constexpr int kMaxPiece = 64;
 
 struct Sorted {
   uint32_t *key[2], *at[2];        // ids and positions, there and back
@@ -257,16 +289,27 @@ __global__ void __launch_bounds__(kSortT, 1) embedding_sort_kernel(const __grid_
 // A thread takes eight adjacent columns of a piece; threadIdx.y: the piece of the CTA's. VECTOR: rows start on sixteen bytes and end with a whole eight.
 template <typename T, bool VECTOR>
 __global__ void __launch_bounds__(kSumT) embedding_sum_kernel(const __grid_constant__ NangilaEmbeddingGradParams p, const __grid_constant__ Sorted s) {
+  constexpr int kAtOnce = VECTOR || sizeof(T) == 2 ? 8 : 4;  // rows on their way together
+  __shared__ uint32_t keys[kSumT / 32 * kMaxPiece], positions[kSumT / 32 * kMaxPiece];  // of the CTA's pieces
   const int piece = blockIdx.x * blockDim.y + threadIdx.y, col = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
   follow();
+  const uint32_t* key = s.key[s.last];
+  const int64_t all0 = int64_t(blockIdx.x) * blockDim.y * s.piece;
+  for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < int(blockDim.y) * s.piece && all0 + i < p.n; i += kSumT) {
+    keys[i] = key[all0 + i];
+    positions[i] = s.at[s.last][all0 + i];
+  }
+  __syncthreads();
   if (piece >= s.pieces || col >= p.d) return;
-  const uint32_t *key = s.key[s.last], *at = s.at[s.last];
-  const int64_t s0 = int64_t(piece) * s.piece, s1 = min(p.n, s0 + s.piece);
+  const int64_t s0 = int64_t(piece) * s.piece;
+  const int count = int(min(p.n, s0 + s.piece) - s0);
+  const uint32_t *mine = keys + threadIdx.y * s.piece, *at = positions + threadIdx.y * s.piece;
   const T* dy = static_cast<const T*>(p.dy);
   const char* lo = reinterpret_cast<const char*>(dy);
   const char* hi = lo + ((p.n - 1) * p.dy_stride + p.d) * int64_t(sizeof(T));
-  uint32_t current = key[s0];
+  uint32_t current = mine[0];
   bool before = s0 > 0 && key[s0 - 1] == current;
+  const uint32_t behind = s0 + count < p.n ? key[s0 + count] : uint32_t(p.rows);
   float acc[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
@@ -306,20 +349,27 @@ __global__ void __launch_bounds__(kSumT) embedding_sum_kernel(const __grid_const
       }
     }
   };
-  for (int64_t i0 = s0; i0 < s1; i0 += kSumAtOnce) {
-    uint32_t k[kSumAtOnce];
-    dev::Raw8<T> raw[kSumAtOnce];
+  for (int i0 = 0; i0 < count; i0 += kAtOnce) {
+    uint32_t k[kAtOnce];
+    dev::Raw8<T> raw[VECTOR ? kAtOnce : 1];
+    const T* row[VECTOR ? 1 : kAtOnce];
+    Window w[VECTOR ? 1 : kAtOnce][sizeof(T) / 2];
 #pragma unroll
-    for (int j = 0; j < kSumAtOnce; ++j) {
-      k[j] = i0 + j < s1 ? key[i0 + j] : uint32_t(p.rows);
+    for (int j = 0; j < kAtOnce; ++j) {
+      k[j] = i0 + j < count ? mine[i0 + j] : uint32_t(p.rows);
       if (k[j] >= uint32_t(p.rows)) continue;
-      const T* row = dy + int64_t(at[i0 + j]) * p.dy_stride + col;
-      if constexpr (VECTOR) dev::fetch(row, raw[j]);
-      else fetch_any(row, lo, hi, raw[j]);
+      const T* from = dy + int64_t(at[i0 + j]) * p.dy_stride + col;
+      if constexpr (VECTOR) {
+        dev::fetch(from, raw[j]);
+      } else {
+        row[j] = from;
+#pragma unroll
+        for (int h = 0; h < int(sizeof(T)) / 2; ++h) w[j][h] = window_at(from + 4 * h, lo, hi);
+      }
     }
 #pragma unroll
-    for (int j = 0; j < kSumAtOnce; ++j) {
-      if (i0 + j >= s1) break;
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (i0 + j >= count) break;
       if (k[j] != current) {
         finish(false);
         current = k[j];
@@ -329,12 +379,19 @@ __global__ void __launch_bounds__(kSumT) embedding_sum_kernel(const __grid_const
       }
       if (current >= uint32_t(p.rows)) return;  // nothing but what is left out from here on
       float v[8];
-      dev::unpack(raw[j], v);
+      if constexpr (VECTOR) {
+        dev::unpack(raw[j], v);
+      } else {
+        dev::Raw8<T> r;
+        r.a = shifted<T>(w[j][0], row[j]);
+        if constexpr (sizeof(T) == 4) r.b = shifted<T>(w[j][1], row[j]);
+        dev::unpack(r, v);
+      }
 #pragma unroll
       for (int c = 0; c < 8; ++c) acc[c] += v[c];
     }
   }
-  finish(s1 < p.n && key[s1] == current);
+  finish(behind == current);
 }
 
 // The runs that cross pieces, 128 columns at a time: a long one by the sixteen warps of a CTA, each with every sixteenth partial sum, added up in order; a short one by a warp.
@@ -434,7 +491,7 @@ Sorted layout(int64_t n, int64_t rows, int32_t d, uint8_t* base, int64_t* bytes)
   s.per_warp = int(((n + kSortWarps - 1) / kSortWarps + 31) / 32 * 32);
   // pieces: some hundreds of them if there are positions enough, and no shorter than what a thread has on its way at a time
   s.piece = 8;
-  while (s.piece < 64 && n > int64_t(s.piece) * 512) s.piece *= 2;
+  while (s.piece < kMaxPiece && n >= int64_t(s.piece) * 1024) s.piece *= 2;
   s.pieces = int((n + s.piece - 1) / s.piece);
   s.pitch = (d + 7) / 8 * 8;
   s.crossing = reinterpret_cast<uint32_t*>(take(8));
