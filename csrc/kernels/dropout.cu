@@ -79,7 +79,7 @@ __device__ __noinline__ void settle8(const Launch& a, int64_t block, uint4 c, co
   }
 }
 
-// Copies of a thread's own to its own place in shared memory: nobody else waits for them.
+// Copies of a thread's own, in groups.
 __device__ __forceinline__ void copy16(void* to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
 }
@@ -87,15 +87,15 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int N>
 __device__ __forceinline__ void copies_wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// A thread's blocks are on their way through shared memory, four of them (in fp32 two) at a time: with 32 warps an SM, 64 KB (and as much of the residual). In registers, one or two at a time, the
+// A thread's blocks are on their way through shared memory, four of them (in fp32 three) at a time: with 32 warps an SM, 64 KB (and as much of the residual). In registers, one or two at a time, the
 // loads of all SMs did not cover the way to memory: 8192 x 2048 bf16 took 19 to 21 us, floor 10. The numbers themselves take 5 of it (twenty 32 x 32 bit products a block).
 template <typename T>
-constexpr int kAheadOf = sizeof(T) == 4 ? 2 : 4;
+constexpr int kAheadOf = sizeof(T) == 4 ? 3 : 4;
 
 template <typename T, bool VECTOR, bool SEED_IN_MEMORY>
 __global__ void __launch_bounds__(kT, 4) dropout_kernel(const __grid_constant__ Launch l) {
   constexpr int kAhead = kAheadOf<T>, kParts = sizeof(T) / 2;  // sixteen bytes each, of a block
-  extern __shared__ uint4 ring[];        // [residual][kAhead][kParts][thread]
+  extern __shared__ uint4 ring[];        // [residual][kAhead][block of the thread][kParts]
   const NangilaDropoutParams& p = l.p;
   Keys made;
   if (SEED_IN_MEMORY) make_keys(uint64_t(*p.seed_ptr), made);
@@ -106,38 +106,48 @@ __global__ void __launch_bounds__(kT, 4) dropout_kernel(const __grid_constant__ 
   const int64_t step = int64_t(gridDim.x) * kT, first = int64_t(blockIdx.x) * kT + threadIdx.x;
   const int64_t whole = VECTOR ? p.n / 8 : 0;
   if (VECTOR) {
-    auto slot = [&](int which, int stage, int part) { return ring + ((which * kAhead + stage) * kParts + part) * kT + threadIdx.x; };
-    auto fetch = [&](int64_t b, int stage) {
-      if (b < whole) {
+    // a warp's 32 blocks lie side by side, and its lanes copy neighbouring sixteen bytes: with kParts > 1 not all of them their own
+    const int lane = threadIdx.x & 31;
+    auto slot = [&](int which, int stage) { return ring + (which * kAhead + stage) * kParts * kT + (threadIdx.x - lane) * kParts; };
+    auto fetch = [&](int64_t b0, int stage) {
 #pragma unroll
-        for (int k = 0; k < kParts; ++k) {
-          copy16(slot(0, stage, k), reinterpret_cast<const uint4*>(x + b * 8) + k);
-          if (r != nullptr) copy16(slot(1, stage, k), reinterpret_cast<const uint4*>(r + b * 8) + k);
-        }
+      for (int k = 0; k < kParts; ++k) {
+        const int64_t at = kParts > 1 ? b0 * kParts + k * 32 + lane : b0;
+        if (at >= whole * kParts) continue;
+        copy16(slot(0, stage) + k * 32 + lane, reinterpret_cast<const uint4*>(x) + at);
+        if (r != nullptr) copy16(slot(1, stage) + k * 32 + lane, reinterpret_cast<const uint4*>(r) + at);
       }
       copies_commit();
     };
+    auto read = [&](int which, int stage, float (&v)[8]) {
+      dev::Raw8<T> raw;
+      raw.a = slot(which, stage)[lane * kParts];
+      if constexpr (kParts > 1) raw.b = slot(which, stage)[lane * kParts + 1];
+      dev::unpack(raw, v);
+    };
+    // (each thread for itself where its copies are its own)
+    const int64_t first0 = kParts > 1 ? first - lane : first;
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) fetch(first + k * step, k);
+    for (int k = 0; k < kAhead; ++k) fetch(first0 + k * step, k);
     int stage = 0;
-    for (int64_t b = first; b < whole; b += step) {
+    for (int64_t b0 = first0; b0 < whole; b0 += step) {
+      const int64_t b = kParts > 1 ? b0 + lane : b0;
       const uint4 c = philox(uint64_t(b), p.draw, 0, keys);
       copies_wait_but<kAhead - 1>();
-      dev::Raw8<T> raw;
-      float v[8], a[8];
-      raw.a = *slot(0, stage, 0);
-      if constexpr (kParts > 1) raw.b = *slot(0, stage, 1);
-      dev::unpack(raw, v);
+      if (kParts > 1) __syncwarp();
+      float v[8], a[8];  // (of a block behind the last: never written)
+      read(0, stage, v);
       drop8(v, p.scale, c, l.upper);
       if (r != nullptr) {
-        raw.a = *slot(1, stage, 0);
-        if constexpr (kParts > 1) raw.b = *slot(1, stage, 1);
-        dev::unpack(raw, a);
+        read(1, stage, a);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += a[i];
       }
-      fetch(b + kAhead * step, stage);
+      if (kParts > 1) __syncwarp();
+      fetch(b0 + kAhead * step, stage);
       stage = stage + 1 == kAhead ? 0 : stage + 1;
+      if (kParts > 1 && b >= whole) continue;
+      dev::Raw8<T> raw;
       dev::pack(v, raw);
       dev::put(out + b * 8, raw);
       if (tied8(c, l.upper) && l.lower != 0) settle8<T>(l, b, c, keys);

@@ -90,77 +90,83 @@ __global__ void __launch_bounds__(kLookupT) embedding_kernel(const __grid_consta
     }
   }
 }
-// Rows that start anywhere: the packed output is cut into sixteen bytes each, and each of those is put together from its row, or from the two that meet in it.
-// (A value at a time, a warp for each token, 16381 x 769 fp16 took 24 us.)
+// Rows that start anywhere: the packed output is cut into sixteen bytes each, and each of those is put together from its row, or from the two that meet in it (value by value
+// where rows are shorter than that). (A value at a time, a warp for each token, 16381 x 769 fp16 took 24 us.)
 template <typename T, typename Index>
 __global__ void __launch_bounds__(kLookupT) embedding_any_kernel(const __grid_constant__ NangilaEmbeddingParams p, Index values) {
-  constexpr int N = 16 / sizeof(T), kOnTheWay = 4;
+  constexpr int N = 16 / sizeof(T), kOnTheWay = 2;
   const char* lo = static_cast<const char*>(p.weight);
   const char* hi = lo + ((p.rows - 1) * p.weight_stride + p.d) * int64_t(sizeof(T));
-  const float nan = __uint_as_float(0x7fc00000u);
   auto row_of = [&](Index i, bool& inside) {
     const int64_t id = id_at(p.ids, p.ids_64, i);
     inside = id >= 0 && id < p.rows;
     return static_cast<const T*>(p.weight) + (inside ? id : 0) * p.weight_stride;
   };
-  auto scaled = [&](T v, bool inside) { return dev::Vec16<T>::from_float(inside ? dev::Vec16<T>::to_float(v) * p.scale : nan); };
+  auto put_scaled = [&](const uint4& raw, bool inside, float (&v)[N], int from) {  // the values from `from` on
+    float u[8];
+    dev::Raw8<T> r;
+    r.a = raw;
+    if constexpr (sizeof(T) == 4) r.b = make_uint4(0, 0, 0, 0);
+    dev::unpack(r, u);
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (k >= from) v[k] = inside ? u[k] * p.scale : __uint_as_float(0x7fc00000u);
+  };
   const Index step = Index(gridDim.x) * kLookupT * N;
   for (Index at0 = (Index(blockIdx.x) * kLookupT + threadIdx.x) * N; at0 < values; at0 += step * kOnTheWay) {
-    const T* from[kOnTheWay];
-    bool inside[kOnTheWay];
-    int col[kOnTheWay];
-    Window w[kOnTheWay];
+    const T *row[kOnTheWay], *next[kOnTheWay];  // where the sixteen begin in their row, and would have begun in the one behind it
+    bool inside[kOnTheWay], next_inside[kOnTheWay];
+    int left[kOnTheWay];                        // values of the first row
+    Window w[kOnTheWay], next_w[kOnTheWay];
 #pragma unroll
     for (int j = 0; j < kOnTheWay; ++j) {
       const Index at = at0 + step * j;
-      if (at >= values) break;
+      left[j] = 0;
+      if (at >= values) continue;
       const Index i = at / Index(p.d);
-      col[j] = int(at - i * Index(p.d));
-      from[j] = row_of(i, inside[j]) + col[j];
+      const int col = int(at - i * Index(p.d));
+      left[j] = p.d - col;
+      row[j] = row_of(i, inside[j]) + col;
+      next[j] = row[j], next_inside[j] = false;
+      if (left[j] < N && int64_t(i) + 1 < p.n) next[j] = row_of(i + 1, next_inside[j]) - left[j];
     }
 #pragma unroll
-    for (int j = 0; j < kOnTheWay; ++j)
-      if (at0 + step * j < values) w[j] = window_at(from[j], lo, hi);
+    for (int j = 0; j < kOnTheWay; ++j) {
+      if (left[j] == 0) continue;
+      w[j] = window_at(row[j], lo, hi);
+      if (left[j] < N) next_w[j] = window_at(next[j], lo, hi);
+    }
 #pragma unroll
     for (int j = 0; j < kOnTheWay; ++j) {
+      if (left[j] == 0) continue;
       const Index at = at0 + step * j;
-      if (at >= values) break;
-      const uint4 raw = shifted<T>(w[j], from[j]);
-      T v[N];
-      memcpy(v, &raw, 16);
+      float v[N];
+      put_scaled(shifted<T>(w[j], row[j]), inside[j], v, 0);
+      if (left[j] < N) {
+        put_scaled(shifted<T>(next_w[j], next[j]), next_inside[j], v, left[j]);
+        if (p.d < N) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) v[k] = scaled(v[k], inside[j]);
-      T* to = static_cast<T*>(p.out) + at;
-      if (col[j] + N > p.d) {  // its end, and the next row's beginning
-        const int left = p.d - col[j];
-        bool in = false;
-        if (p.d >= N) {
-          const Index i = at / Index(p.d) + 1;
-          if (int64_t(i) < p.n) {
-            const T* row = row_of(i, in);
-            const uint4 next = shifted<T>(window_at(row - left, lo, hi), row - left);
-            T u[N];
-            memcpy(u, &next, 16);
-#pragma unroll
-            for (int k = 0; k < N; ++k)
-              if (k >= left) v[k] = scaled(u[k], in);
-          }
-        } else {
-          for (int k = left; k < N && at + Index(k) < values; ++k) {
+          for (int k = 0; k < N; ++k) {
+            if (k < left[j] || at + Index(k) >= values) continue;
             const Index i = (at + Index(k)) / Index(p.d);
-            const T* row = row_of(i, in);
-            v[k] = scaled(row[at + Index(k) - i * Index(p.d)], in);
+            bool in;
+            const T* from = row_of(i, in);
+            v[k] = in ? dev::Vec16<T>::to_float(from[at + Index(k) - i * Index(p.d)]) * p.scale : __uint_as_float(0x7fc00000u);
           }
         }
       }
+      T* to = static_cast<T*>(p.out) + at;
       if (at + N <= values) {
-        uint4 out;
-        memcpy(&out, v, 16);
-        *reinterpret_cast<uint4*>(to) = out;
+        float u[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) u[k] = v[k % N];
+        dev::Raw8<T> r;
+        dev::pack(u, r);
+        *reinterpret_cast<uint4*>(to) = r.a;
       } else {
 #pragma unroll
         for (int k = 0; k < N; ++k)
-          if (at + Index(k) < values) to[k] = v[k];
+          if (at + Index(k) < values) to[k] = dev::Vec16<T>::from_float(v[k]);
       }
     }
   }
