@@ -32,6 +32,7 @@
 #include "ptx_sm100.cuh"
 #include "quant.cuh"
 #include "raw8.cuh"
+#include "warp_sums.cuh"
 
 namespace nangila {
 namespace {
@@ -80,8 +81,17 @@ struct Result {
   int wide;             // 0: alpha f_row D in 16 bits; 1: D in fp32; 2: added to what is there
   const float* factor;  // of D's rows; NULL: one
 };
+// Columns of E, each row times its factor, added up: 256 columns and a share of the rows a warp, the shares' sums one behind the other.
+struct Columns {
+  const void* e;
+  const float* factor;
+  float* partial;       // [shares][e_stride]; NULL: not wanted
+  int64_t e_stride;
+  int n, blocks, shares, share;
+};
 struct Gradients {
   Result x, w;          // dx = E w, dw = E^T x'
+  Columns columns;
   const float* alpha;
   int extra;            // tiles of dw that a pair takes on top of the others' where it has a tile of dx less
 };
@@ -513,8 +523,8 @@ __global__ void __launch_bounds__(kThreads, 1) ce_logits_kernel(const __grid_con
     if (KIND != kStats) prefetch_tensormap(&maps.out);
   }
   const uint32_t tmem = products_begin<PAIR>(s);
-  may_follow();
   follow();
+  may_follow();  // (the next kernel reads x and w before it waits for this one: they are complete)
 
   if (warp == 0) {
     if (lane == 0) {
@@ -551,6 +561,162 @@ __global__ void __launch_bounds__(kThreads, 1) ce_logits_kernel(const __grid_con
   products_end<PAIR>(tmem);
 }
 
+// The same sums for few tokens, TOKENS at most: bound by reading w once, so w's rows are what fills the products' 128 rows, and as many of its slabs as fit into shared memory are on
+// their way. A tile's columns are tokens, its rows classes: each warp of the epilogue joins the 32 classes that its lanes hold, token by token, and keeps lane t's running pair for token t.
+// (With the tokens as rows, 16 of 128 of them there, 16 x 2048 x 32000 took 39 us.)
+template <int TOKENS>
+struct Few {
+  static constexpr int kStage = kOperandBytes + TOKENS * 128;
+  static constexpr int kCount = TOKENS <= 16 ? 12 : TOKENS <= 32 ? 10 : 9;
+  static constexpr int kBytes = kCount * kStage + 1024 + 256;
+};
+constexpr int kFewThreads = 64 + 128;
+template <typename T, int TOKENS>
+__global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Rows rows, int total, int slabs) {
+  using F = Few<TOKENS>;
+  constexpr int kColumns = TOKENS <= 16 ? 32 : 2 * TOKENS;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ int targets[TOKENS];
+  uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(stages + F::kCount * F::kStage);
+  uint64_t *empty = full + F::kCount, *acc_full = empty + F::kCount, *acc_empty = acc_full + 2, *drained = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  volatile uint32_t* failed = tmem_slot + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < F::kCount; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 4);
+    }
+    mbar_init(drained, 1);
+    *failed = 0;
+    fence_barrier_init();
+    prefetch_tensormap(&maps.a);
+    prefetch_tensormap(&maps.b);
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, kColumns);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  follow();
+  may_follow();  // (the next kernel reads x and w before it waits for this one: they are complete)
+  if (warp == 0) {
+    if (lane == 0) {
+      int i = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x)
+        for (int k = 0; k < slabs; ++k, ++i) {
+          const int st = i % F::kCount;
+          if (i >= F::kCount && !mbar_wait(&empty[st], uint32_t((i / F::kCount - 1) & 1), kTimeoutNs)) {
+            *failed = 1;
+            ok = false;
+            break;
+          }
+          uint8_t* a = stages + st * F::kStage;
+          mbar_arrive_expect_tx(&full[st], F::kStage);
+          tma_operand<false>(a, &maps.a, k * kSlabK, tile * kTileM, 0, smem_u32(&full[st]));
+          tma_operand<false>(a + kOperandBytes, &maps.b, k * kSlabK, 0, 0, smem_u32(&full[st]));
+        }
+      for (int j = max(0, i - F::kCount); j < i; ++j) mbar_wait(*failed == 0 ? &empty[j % F::kCount] : &full[j % F::kCount], uint32_t((j / F::kCount) & 1), kTimeoutNs);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = (1u << 4) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(TOKENS >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
+      int i = 0, n = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x, ++n) {
+        if (n >= 2 && !mbar_wait(&acc_empty[n & 1], uint32_t((n / 2 - 1) & 1), kTimeoutNs)) ok = false;
+        tc_fence_after_sync();
+        for (int k = 0; k < slabs && ok; ++k, ++i) {
+          const int st = i % F::kCount;
+          if (!mbar_wait(&full[st], uint32_t((i / F::kCount) & 1), kTimeoutNs)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t a = smem_u32(stages + st * F::kStage), b = a + kOperandBytes;
+#pragma unroll
+          for (int kk = 0; kk < kSlabK / 16; ++kk)
+            umma_f16(tmem + uint32_t((n & 1) * TOKENS), make_smem_desc(a + kk * 32, 16, 1024), make_smem_desc(b + kk * 32, 16, 1024), idesc, (k > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&empty[st]);
+        }
+        if (ok) umma_commit(&acc_full[n & 1]);
+      }
+      if (!ok) {
+        *failed = 1;
+        umma_commit(drained);
+        mbar_wait(drained, 0, kTimeoutNs);
+      }
+    }
+  } else {
+    const int quad = warp & 3;
+    for (int t = threadIdx.x - 64; t < TOKENS; t += 128) {
+      const int64_t v = t < rows.n ? rows.targets[t] : -1;
+      targets[t] = v >= 0 && v < rows.classes ? int(v) : -1;
+    }
+    asm volatile("" ::: "memory");
+    __syncwarp();
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    float most[(TOKENS + 31) / 32], sum[(TOKENS + 31) / 32];
+#pragma unroll
+    for (int j = 0; j < (TOKENS + 31) / 32; ++j) most[j] = -INFINITY, sum[j] = 0.0f;
+    int n = 0;
+    for (int tile = blockIdx.x; tile < total; tile += gridDim.x, ++n) {
+      const int row = tile * kTileM + quad * 32 + lane;  // the lane's class
+      const bool here = row < rows.classes;
+      const float bias = rows.bias != nullptr && here ? rows.bias[row] : 0.0f;
+      bool ok = *failed == 0 && mbar_wait(&acc_full[n & 1], uint32_t((n / 2) & 1), kTimeoutNs);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) *failed = 1;
+      tc_fence_after_sync();
+      float tops[(TOKENS + 31) / 32], sums[(TOKENS + 31) / 32];
+#pragma unroll
+      for (int g = 0; g < TOKENS / 16; ++g) {
+        float v[16];
+        tmem_ld_32x32b_x16(tmem + (uint32_t(quad * 32) << 16) + uint32_t((n & 1) * TOKENS + g * 16), v);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const int t = g * 16 + k;
+          float z = ok ? (v[k] + bias) * kLog2e : __uint_as_float(0x7fc00000u);
+          if (!here || row == targets[t]) z = -INFINITY;
+          float top = z;
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          const float e = exp2_fast(z - (top == -INFINITY ? 0.0f : top));
+          v[k] = e;
+          if (lane == (t & 31)) tops[t / 32] = top;
+        }
+        const float total16 = warp_sums_of_power<16>(v);  // of token g * 16 + lane / 2
+        const float mine = __shfl_sync(0xffffffffu, total16, (lane & 15) * 2);
+        if (lane / 16 == (g & 1) || TOKENS <= 16) sums[g / 2] = mine;
+      }
+#pragma unroll
+      for (int j = 0; j < (TOKENS + 31) / 32; ++j) {
+        if (TOKENS <= 16 && lane >= 16) continue;
+        const float now = fmaxf(most[j], tops[j]), base = now == -INFINITY ? 0.0f : now;
+        sum[j] = sum[j] * exp2_fast(most[j] - base) + sums[j] * exp2_fast(tops[j] - base);
+        most[j] = now;
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_at(smem_u32(&acc_empty[n & 1]));
+    }
+#pragma unroll
+    for (int j = 0; j < (TOKENS + 31) / 32; ++j) {
+      const int t = j * 32 + lane;
+      if (t < rows.n && t < TOKENS) rows.parts[int64_t(blockIdx.x * 4 + quad) * rows.stride + t] = make_float2(most[j], sum[j]);
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, kColumns);
+}
+
 // dx = E w and dw = E^T x' in one launch of pairs of CTAs. A tile of dx has all classes as its K, one of dw all tokens of the group, and there may be fewer tiles of dx than pairs: each
 // pair takes its share of dx's tiles first, and where it has one less than others, tiles of dw for it. So both end together. dx's K is cut in parts where a
 // single tile would take longer than that.
@@ -581,6 +747,33 @@ __device__ __forceinline__ bool task_of(const Gradients& g, int pair, int pairs,
   t.at.n0 = i % r.tiles_n * 256;
   return true;
 }
+template <typename T>
+__device__ __forceinline__ void add_columns(const Columns& c, int warp, int warps) {
+  const int lane = threadIdx.x & 31;
+  for (int task = warp; task < c.blocks * c.shares; task += warps) {
+    const int share = task / c.blocks, from = share * c.share, to = min(c.n, from + c.share);
+    const int64_t col = int64_t(task - share * c.blocks) * 256 + lane * 8;
+    if (col >= c.e_stride) continue;
+    const T* e = static_cast<const T*>(c.e) + col;
+    float acc[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
+#pragma unroll 8
+    for (int r = from; r < to; ++r) {
+      dev::Raw8<T> raw;
+      dev::fetch(e + r * c.e_stride, raw);
+      const float f = c.factor[r];
+      float v[8];
+      dev::unpack(raw, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) acc[k] = __fmaf_rn(v[k], f, acc[k]);
+    }
+    float4* out = reinterpret_cast<float4*>(c.partial + share * c.e_stride + col);
+    out[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    out[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+  }
+}
+// (The epilogue's warps have the bias's gradient to add up while the first tiles are made: 1229 x 30592 in a kernel of its own took 18 us.)
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) ce_gradients_kernel(const __grid_constant__ GradientMaps maps, const __grid_constant__ Gradients g) {
   extern __shared__ uint8_t smem_raw[];
@@ -614,6 +807,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gradients_kernel(const __grid_
     }
   } else {
     uint32_t used = 0;
+    if (g.columns.partial != nullptr) add_columns<T>(g.columns, int(blockIdx.x) * kEpilogueWarps + warp - 2, int(gridDim.x) * kEpilogueWarps);
     for (int k = 0; task_of(g, pair, pairs, k, t); ++k)
       finish_result<T>(s, tmem, t.x ? g.x : g.w, g.alpha, t.x ? &maps.out_x : &maps.out_w, t.at, t.part, rank, k, used);
     if (lane == 0) bulk_wait_read();
@@ -760,9 +954,13 @@ __global__ void __launch_bounds__(kRowsT) ce_rows_kernel(const __grid_constant__
   constexpr int kWarps = kRowsT / 32;
   __shared__ float2 joined[kWarps][kRowsAtOnce];
   __shared__ float logit[kRowsAtOnce];
-  follow();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row0 = blockIdx.x * kRowsAtOnce, row = row0 + lane;
+  if (pass == 0 && row0 + warp < a.n) {
+    const float z = target_logit<T>(a.p, a.row0 + row0 + warp);
+    if (lane == 0) logit[warp] = z;
+  }
+  follow();
   if (pass == 2) {
     const int all = (a.n + 31) / 32, per = tile_rows / 32;
     const int from = int(blockIdx.x) / per * per;
@@ -771,10 +969,6 @@ __global__ void __launch_bounds__(kRowsT) ce_rows_kernel(const __grid_constant__
     if (!any) return;
   }
   const bool here = row < a.n;
-  if (pass == 0 && row0 + warp < a.n) {
-    const float z = target_logit<T>(a.p, a.row0 + row0 + warp);
-    if (lane == 0) logit[warp] = z;
-  }
   const float ref = pass != 0 && here ? a.ref[row] : 0.0f;
   float most = -INFINITY, sum = 0.0f;
   if (here) {
@@ -866,29 +1060,32 @@ __global__ void __launch_bounds__(kWeightsT) ce_scale_kernel(const __grid_consta
 // NANGILA_CE_GRADIENTS: what the tiles' epilogue takes of each row, and the rows of x without those that add nothing.
 template <typename T>
 __global__ void __launch_bounds__(kWeightsT) ce_weights_kernel(const __grid_constant__ Group a) {
-  const int lane = threadIdx.x & 31;
-  const int row = (blockIdx.x * kWeightsT + threadIdx.x) >> 5;
-  if (row >= a.n) return;
-  const int64_t i = a.row0 + row, t = a.p.targets[i];
-  const bool lives = t != a.p.ignore && t >= 0 && t < a.p.classes;
-  if (lane == 0) {
+  follow();
+  const int64_t thread = int64_t(blockIdx.x) * kWeightsT + threadIdx.x, threads = int64_t(gridDim.x) * kWeightsT;
+  auto lives = [&](int64_t i) {
+    const int64_t t = a.p.targets[i];
+    return t != a.p.ignore && t >= 0 && t < a.p.classes;
+  };
+  for (int64_t row = thread; row < a.n; row += threads) {
+    const int64_t i = a.row0 + row;
     const float unit = a.scales->unit;
     float weight = a.p.upstream_rows ? (unit > 0.0f ? a.p.upstream[i] / unit : unit) : 1.0f;
-    if (!lives) weight = 0.0f;
+    if (!lives(i)) weight = 0.0f;
     a.ref[row] = a.p.lse[i] * kLog2e;
     a.mul[row] = weight * a.e_scale;
     const float value = expm1f(-a.p.losses[i]) * weight * a.e_scale;
     a.value[row] = value;
-    a.factor[row] = lives ? folded(value, dev::Vec16<T>::to_float(dev::Vec16<T>::from_float(value)), 1.0f) : 0.0f;
+    a.factor[row] = lives(i) ? folded(value, dev::Vec16<T>::to_float(dev::Vec16<T>::from_float(value)), 1.0f) : 0.0f;
   }
   if (a.xs == nullptr) return;
-  const T* from = static_cast<const T*>(a.p.x) + i * a.p.x_stride;
-  T* to = static_cast<T*>(a.xs) + int64_t(row) * a.p.d;
-  for (int c = lane * 8; c < a.p.d; c += 256) {
+  const int per = a.p.d / 8;
+#pragma unroll 4
+  for (int64_t i = thread; i < int64_t(a.n) * per; i += threads) {
+    const int64_t row = i / per;
     dev::Raw8<T> raw;
-    dev::fetch(from + c, raw);
-    if (!lives) raw.a = make_uint4(0, 0, 0, 0);
-    dev::put(to + c, raw);
+    dev::fetch(static_cast<const T*>(a.p.x) + (a.row0 + row) * a.p.x_stride + (i - row * per) * 8, raw);
+    if (!lives(a.row0 + row)) raw.a = make_uint4(0, 0, 0, 0);
+    dev::put(static_cast<T*>(a.xs) + i * 8, raw);
   }
 }
 // The sum or mean of the losses, in a fixed order.
@@ -919,45 +1116,15 @@ __global__ void __launch_bounds__(1024) ce_total_kernel(const float* losses, con
     if (lane == 0) *out = float(mean ? sum / count : sum);
   }
 }
-// Columns of E, each row times its factor, added up: 256 columns and a share of the rows a CTA, the shares' sums one behind the other.
-constexpr int kColumnT = 256;
-template <typename T>
-__global__ void __launch_bounds__(kColumnT) ce_columns_kernel(const T* e, int64_t e_stride, const float* factor, int n, int classes, int share, float* partial) {
-  __shared__ float part[8][256];
-  follow();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.x * 256 + lane * 8;
-  const int from = blockIdx.y * share, to = min(n, from + share);
-  float acc[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
-  if (col < classes) {
-#pragma unroll 4
-    for (int r = from + warp; r < to; r += 8) {
-      dev::Raw8<T> raw;
-      dev::fetch(e + int64_t(r) * e_stride + col, raw);
-      float v[8];
-      dev::unpack(raw, v);
-      const float f = factor[r];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) acc[k] = __fmaf_rn(v[k], f, acc[k]);
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < 8; ++k) part[warp][lane * 8 + k] = acc[k];
-  __syncthreads();
-  float sum = 0.0f;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) sum += part[w][threadIdx.x];
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c < classes) partial[int64_t(blockIdx.y) * classes + c] = sum;
-}
-__global__ void ce_bias_grad_kernel(const float* partial, int shares, int classes, int rows, const Scales* scales, void* dbias, int dtype) {
+// The bias's gradient out of the shares' sums of all groups.
+__global__ void ce_bias_grad_kernel(const float* partial, int64_t stride, int shares, int classes, int rows, const Scales* scales, void* dbias, int dtype) {
   follow();
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= rows) return;
   float sum = 0.0f;
   if (i < classes) {
-    for (int s = 0; s < shares; ++s) sum += partial[int64_t(s) * classes + i];
+#pragma unroll 8
+    for (int s = 0; s < shares; ++s) sum += partial[s * stride + i];
     sum *= scales->alpha;
   }
   if (dtype == NANGILA_F32) static_cast<float*>(dbias)[i] = sum;
@@ -1112,6 +1279,25 @@ int launch_logits(const Matrix& x, const Matrix& w, const Matrix* e, const Rows&
   const cudaLaunchConfig_t cfg = pairs_config(attr, int(PAIR ? 2 * std::min<int64_t>(total, sms / 2) : std::min<int64_t>(total, sms)), PAIR, stream);
   return int(cudaLaunchKernelEx(&cfg, kernel, maps, rows, int(tiles_m), int(total), int((x.cols + kSlabK - 1) / kSlabK)));
 }
+// The sums of few tokens; a part of them for each warp of the epilogue.
+constexpr int kFewTokens = 64;
+int few_ctas(int64_t classes) { return int(std::min<int64_t>((classes + kTileM - 1) / kTileM, sm_count())); }
+template <typename T, int TOKENS>
+int launch_few(const Matrix& x, const Matrix& w, const Rows& rows, cudaStream_t stream) {
+  Maps maps;
+  if (!make_map(&maps.a, w, 64, 128) || !make_map(&maps.b, x, 64, TOKENS) || !make_map(&maps.out, x, 64, TOKENS)) return int(cudaErrorNotSupported);
+  auto* kernel = ce_few_kernel<T, TOKENS>;
+  if (const int err = allow_smem(reinterpret_cast<const void*>(kernel), Few<TOKENS>::kBytes)) return err;
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = pairs_config(attr, few_ctas(rows.classes), false, stream);
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = Few<TOKENS>::kBytes;
+  return int(cudaLaunchKernelEx(&cfg, kernel, maps, rows, int((rows.classes + kTileM - 1) / kTileM), int((x.cols + kSlabK - 1) / kSlabK)));
+}
+template <typename T>
+int few(const Matrix& x, const Matrix& w, const Rows& rows, cudaStream_t stream) {
+  return rows.n <= 16 ? launch_few<T, 16>(x, w, rows, stream) : rows.n <= 32 ? launch_few<T, 32>(x, w, rows, stream) : launch_few<T, 64>(x, w, rows, stream);
+}
 template <typename T, int KIND>
 int logits(bool pair, const Matrix& x, const Matrix& w, const Matrix* e, const Rows& rows, cudaStream_t stream) {
   return pair ? launch_logits<T, KIND, true>(x, w, e, rows, stream) : launch_logits<T, KIND, false>(x, w, e, rows, stream);
@@ -1154,7 +1340,7 @@ int split_of(int64_t n, int64_t d, int64_t classes, int64_t rows, bool dw) {
 struct Plan {
   int64_t group;      // tokens at a time
   int64_t groups, e_stride, parts, shares, share;
-  bool pair;          // tiles of the logits
+  bool pair, few;     // tiles of the logits
   bool wide;          // dw is summed up over the groups
   int split;          // parts of dx's K
   int64_t at_scales, at_zt, at_bias, at_ref, at_mul, at_value, at_factor, at_again, at_parts, at_e, at_xs, at_sums, at_dx, at_columns, total;
@@ -1169,7 +1355,8 @@ Plan plan(const NangilaLinearCeParams& p, int what) {
   // Tokens enough for the rows of one small tile take small tiles.
   l.pair = p.n > 128;
   const int64_t side = l.pair ? 256 : 128, half = side / 2;
-  l.parts = (classes + half - 1) / half;
+  l.few = what == NANGILA_CE_LOSSES && p.n <= kFewTokens;
+  l.parts = l.few ? 4 * few_ctas(classes) : (classes + half - 1) / half;
   const int64_t row_bytes = what == NANGILA_CE_LOSSES ? l.parts * 8 : l.e_stride * 2;
   const int64_t most = std::max<int64_t>(256, (what == NANGILA_CE_LOSSES ? kGroupBytes / 8 : kGroupBytes) / row_bytes / 256 * 256);
   l.groups = (p.n + most - 1) / most;
@@ -1177,9 +1364,8 @@ Plan plan(const NangilaLinearCeParams& p, int what) {
   l.groups = (p.n + l.group - 1) / l.group;
   l.wide = l.groups > 1 && p.dw != nullptr;
   l.bias_count = (classes + side - 1) / side * side;
-  // rows of E that a CTA adds up for the bias's gradient: some hundreds of CTAs
-  const int64_t across = (classes + 255) / 256;
-  l.shares = std::max<int64_t>(1, std::min<int64_t>((l.group + 63) / 64, (4 * 148 + across - 1) / across));
+  // rows of E that a warp adds up for the bias's gradient: a task for each of the epilogue's warps
+  l.shares = std::max<int64_t>(1, std::min<int64_t>((l.group + 31) / 32, kEpilogueWarps * 148 / ((classes + 255) / 256)));
   l.share = (l.group + l.shares - 1) / l.shares;
   auto take = [&](int64_t bytes) {
     const int64_t at = l.total;
@@ -1201,7 +1387,7 @@ Plan plan(const NangilaLinearCeParams& p, int what) {
   l.at_sums = take(l.wide ? int64_t(p.rows) * p.d * 4 : 0);
   l.split = p.dx != nullptr ? split_of(l.group, p.d, classes, p.rows, p.dw != nullptr) : 1;
   l.at_dx = take(l.split > 1 ? l.split * l.group * p.d * 4 : 0);
-  l.at_columns = take(p.dbias != nullptr ? l.groups * l.shares * classes * 4 : 0);
+  l.at_columns = take(p.dbias != nullptr ? l.groups * l.shares * l.e_stride * 4 : 0);
   return l;
 }
 
@@ -1256,7 +1442,7 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
     const unsigned row_ctas = unsigned((a.n + kRowsAtOnce - 1) / kRowsAtOnce);
     const int tile_rows = l.pair ? 256 : 128;
     if (what == NANGILA_CE_LOSSES) {
-      e = logits<T, kStats>(l.pair, x, w, nullptr, rows, stream);
+      e = l.few ? few<T>(x, w, rows, stream) : logits<T, kStats>(l.pair, x, w, nullptr, rows, stream);
       if (e == 0) e = int(launch_following(ce_rows_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, 0, tile_rows));
       continue;
     }
@@ -1281,20 +1467,16 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
     if (what == NANGILA_CE_GRADIENTS) {
       a.mul = reinterpret_cast<float*>(ws + l.at_mul);
       a.value = reinterpret_cast<float*>(ws + l.at_value);
-      ce_weights_kernel<T><<<unsigned((int64_t(a.n) * 32 + kWeightsT - 1) / kWeightsT), kWeightsT, 0, stream>>>(a);
-      e = int(cudaGetLastError());
+      e = int(launch_following(ce_weights_kernel<T>, dim3(unsigned(std::min<int64_t>((int64_t(a.n) * p.d / 8 + kWeightsT - 1) / kWeightsT, 148 * 8))), kWeightsT, 0, stream, a));
       rows.mul = a.mul;
       rows.value = a.value;
       if (e == 0) e = logits<T, kWeighted>(l.pair, x, w, &ex, rows, stream);
     }
-    if (e == 0 && p.dbias != nullptr) {
-      e = int(launch_following(ce_columns_kernel<T>, dim3(unsigned((p.classes + 255) / 256), unsigned(l.shares)), kColumnT, 0, stream, static_cast<const T*>(a.e), l.e_stride,
-                               static_cast<const float*>(a.factor), a.n, int(p.classes), int(l.share), columns + g * l.shares * p.classes));
-    }
-    if (e == 0 && (p.dx != nullptr || p.dw != nullptr)) {
+    if (e == 0) {
       Gradients q;
       std::memset(&q, 0, sizeof q);
       q.alpha = &scales->alpha;
+      if (p.dbias != nullptr) q.columns = {a.e, a.factor, columns + g * l.shares * l.e_stride, l.e_stride, a.n, int((p.classes + 255) / 256), int(l.shares), int(l.share)};
       GradientMaps maps;
       bool ok = make_map(&maps.e_rows, ex, 64, 128) && make_map(&maps.e_columns, ex, 64, 64) && make_map(&maps.w, w, 64, 64) && make_map(&maps.xs, x, 64, 64) && make_map(&maps.out_x, x, 64, 32) &&
                 make_map(&maps.out_w, x, 64, 32);  // (those that are not wanted are not used)
@@ -1316,7 +1498,7 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
       auto* kernel = ce_gradients_kernel<T>;
       if (const int err = allow_smem(reinterpret_cast<const void*>(kernel), kSmem)) return err;
       cudaLaunchAttribute attr[2];
-      const cudaLaunchConfig_t cfg = pairs_config(attr, 2 * std::min(q.x.total + q.w.total, sm_count() / 2), true, stream);
+      const cudaLaunchConfig_t cfg = pairs_config(attr, 2 * (p.dbias != nullptr ? sm_count() / 2 : std::min(q.x.total + q.w.total, sm_count() / 2)), true, stream);
       e = int(cudaLaunchKernelEx(&cfg, kernel, maps, q));
       if (e == 0 && q.x.wide)
         e = int(launch_following(ce_join_kernel<T>, dim3(unsigned(std::min<int64_t>((int64_t(a.n) * p.d / 8 + 255) / 256, 148 * 8))), 256, 0, stream, reinterpret_cast<const float*>(ws + l.at_dx),
@@ -1328,7 +1510,7 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
     e = int(launch_following(ce_round_kernel<T>, dim3(unsigned(std::min<int64_t>((int64_t(p.rows) * p.d / 8 + 255) / 256, 148 * 8))), 256, 0, stream, static_cast<const float*>(sums),
                              static_cast<const Scales*>(scales), static_cast<T*>(p.dw), int64_t(p.rows) * p.d / 8));
   if (e == 0 && p.dbias != nullptr)
-    e = int(launch_following(ce_bias_grad_kernel, dim3(unsigned((p.rows + 255) / 256)), 256, 0, stream, static_cast<const float*>(columns), int(l.groups * l.shares), int(p.classes), int(p.rows),
+    e = int(launch_following(ce_bias_grad_kernel, dim3(unsigned((p.rows + 255) / 256)), 256, 0, stream, static_cast<const float*>(columns), l.e_stride, int(l.groups * l.shares), int(p.classes), int(p.rows),
                              static_cast<const Scales*>(scales), p.dbias, int(p.bias_dtype)));
   if (e == 0 && what != NANGILA_CE_GRADIENTS && p.loss != nullptr)
     e = int(launch_following(ce_total_kernel, dim3(1), 1024, 0, stream, static_cast<const float*>(p.losses), p.targets, p.n, p.ignore, int(p.mean), p.loss));
