@@ -155,80 +155,121 @@ __device__ __forceinline__ void init_barriers(const Shared& s) {
   fence_barrier_init();
 }
 
-// TMA of a tile's slabs, `i` of which have gone before: both CTAs of a pair, each its own halves; the bytes are counted where the products are issued.
-// False when a wait has run out.
+// The copies and the products are each issued by one lane of a warp, but all of its lanes go through the loops: what the instructions take is then the same for the warp, and stays in the
+// registers that they take it from. (With one lane in the loops, each of its instructions moved its operands there first: 640 cycles a slab, whose products take 512. 8192 x 768 x 50304's
+// logits, half of them at a time, 245 us.)
+__device__ __forceinline__ bool elected() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+// A wait of a whole warp, with one answer for all of it.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint64_t t0 = timer_ns();
+  uint32_t spins = 0;
+  while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+    if ((++spins & 255u) == 0u && __any_sync(0xffffffffu, timer_ns() - t0 > kTimeoutNs)) return false;
+  }
+  return true;
+}
+// Where a role is in the ring of stages.
+struct Ring {
+  int stage = 0;
+  uint32_t round = 0;  // how often the ring has been gone round
+  __device__ __forceinline__ void next(int stages) {
+    if (++stage == stages) stage = 0, ++round;
+  }
+};
+
+// TMA of a tile's slabs: both CTAs of a pair, each its own halves; the bytes are counted where the products are issued. By a whole warp. False when a wait has run out.
 template <bool PAIR>
-__device__ __forceinline__ bool load_tile(const Shared& s, const CUtensorMap* a_map, const CUtensorMap* b_map, bool a_mn, bool b_mn, const TileAt& at, uint32_t rank, int slab0, int slabs, int& i) {
+__device__ __forceinline__ bool load_tile(const Shared& s, const CUtensorMap* a_map, const CUtensorMap* b_map, bool a_mn, bool b_mn, const TileAt& at, uint32_t rank, int slab0, int slabs, Ring& ring) {
   const int row = at.m0 + int(rank) * kTileM, col = at.n0 + int(rank) * 128;
-  for (int k = 0; k < slabs; ++k, ++i) {
-    const int st = i % kStages;
-    if (i >= kStages && !mbar_wait(&s.empty[st], uint32_t((i / kStages - 1) & 1), kTimeoutNs)) {
+  for (int k = 0; k < slabs; ++k, ring.next(kStages)) {
+    const int st = ring.stage;
+    if (ring.round > 0 && !warp_wait(&s.empty[st], (ring.round - 1) & 1)) {
       *s.failed = 1;
       return false;
     }
-    uint8_t* a = s.stages + st * kStageBytes;
-    uint8_t* b = a + kOperandBytes;
-    const int k0 = (slab0 + k) * kSlabK;
-    if (rank == 0) mbar_arrive_expect_tx(&s.full[st], kStageBytes * (PAIR ? 2 : 1));
-    const uint32_t bar = PAIR ? rank0_address(&s.full[st]) : smem_u32(&s.full[st]);
-    if (a_mn) {
-      tma_operand<PAIR>(a, a_map, row, k0, 0, bar);
-      tma_operand<PAIR>(a + 8192, a_map, row + 64, k0, 0, bar);
-    } else {
-      tma_operand<PAIR>(a, a_map, k0, row, 0, bar);
+    if (elected()) {
+      uint8_t* a = s.stages + st * kStageBytes;
+      uint8_t* b = a + kOperandBytes;
+      const int k0 = (slab0 + k) * kSlabK;
+      if (rank == 0) mbar_arrive_expect_tx(&s.full[st], kStageBytes * (PAIR ? 2 : 1));
+      const uint32_t bar = PAIR ? rank0_address(&s.full[st]) : smem_u32(&s.full[st]);
+      if (a_mn) {
+        tma_operand<PAIR>(a, a_map, row, k0, 0, bar);
+        tma_operand<PAIR>(a + 8192, a_map, row + 64, k0, 0, bar);
+      } else {
+        tma_operand<PAIR>(a, a_map, k0, row, 0, bar);
+      }
+      if (b_mn) {
+        tma_operand<PAIR>(b, b_map, col, k0, 0, bar);
+        tma_operand<PAIR>(b + 8192, b_map, col + 64, k0, 0, bar);
+      } else {
+        tma_operand<PAIR>(b, b_map, k0, col, 0, bar);
+      }
     }
-    if (b_mn) {
-      tma_operand<PAIR>(b, b_map, col, k0, 0, bar);
-      tma_operand<PAIR>(b + 8192, b_map, col + 64, k0, 0, bar);
-    } else {
-      tma_operand<PAIR>(b, b_map, k0, col, 0, bar);
-    }
+    __syncwarp();
   }
   return true;
 }
 // The copies that are still under way when the loads end: all have arrived when the products that read them are done; if somebody has given up, as
 // much as can be waited for (the bytes of a pair are counted by rank 0, the stages of rank 1 are given back by its products).
-__device__ __forceinline__ void drain_loads(const Shared& s, uint32_t rank, int i) {
-  for (int j = max(0, i - kStages); j < i; ++j) {
-    if (*s.failed == 0 || rank != 0) mbar_wait(&s.empty[j % kStages], uint32_t((j / kStages) & 1), kTimeoutNs);
-    else mbar_wait(&s.full[j % kStages], uint32_t((j / kStages) & 1), kTimeoutNs);
+__device__ __forceinline__ void drain_loads(const Shared& s, uint32_t rank, Ring ring) {
+  const int under_way = ring.round > 0 ? kStages : ring.stage;
+  for (int j = 0; j < under_way; ++j) {
+    // backwards from the last one
+    if (ring.stage == 0) ring.stage = kStages, --ring.round;
+    --ring.stage;
+    if (*s.failed == 0 || rank != 0) warp_wait(&s.empty[ring.stage], ring.round & 1);
+    else warp_wait(&s.full[ring.stage], ring.round & 1);
   }
 }
-// The products of a tile, the n-th, into its accumulator. False when a wait has run out.
+// The products of a tile, the n-th, into its accumulator, by a whole warp. False when a wait has run out.
 template <bool PAIR, bool BF16>
-__device__ __forceinline__ bool multiply_tile(const Shared& s, uint32_t tmem, bool a_mn, bool b_mn, int slabs, int n, int& i) {
+__device__ __forceinline__ bool multiply_tile(const Shared& s, uint32_t tmem, bool a_mn, bool b_mn, int slabs, int n, Ring& ring) {
   constexpr int kSide = PAIR ? 256 : 128;
   const uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | (uint32_t(kSide >> 3) << 17) | (uint32_t(kSide >> 4) << 24);
   const int acc = n & 1;
-  if (n >= 2 && !mbar_wait(&s.acc_empty[acc], uint32_t((n / 2 - 1) & 1), kTimeoutNs)) return false;
+  if (n >= 2 && !warp_wait(&s.acc_empty[acc], uint32_t((n / 2 - 1) & 1))) return false;
   tc_fence_after_sync();
   const uint32_t d = tmem + uint32_t(acc * kSide);
-  for (int k = 0; k < slabs; ++k, ++i) {
-    const int st = i % kStages;
-    if (!mbar_wait(&s.full[st], uint32_t((i / kStages) & 1), kTimeoutNs)) return false;
+  // K-major: 16 elements along K are 32 bytes of a swizzle row; MN-major: 16 K-rows are two groups of eight rows of 128 bytes
+  const uint64_t a0 = make_smem_desc(smem_u32(s.stages), a_mn ? 8192 : 16, 1024), b0 = make_smem_desc(smem_u32(s.stages) + kOperandBytes, b_mn ? 8192 : 16, 1024);
+  const uint64_t a_step = (a_mn ? 2048 : 32) >> 4, b_step = (b_mn ? 2048 : 32) >> 4;
+  for (int k = 0; k < slabs; ++k, ring.next(kStages)) {
+    if (!warp_wait(&s.full[ring.stage], ring.round & 1)) return false;
     tc_fence_after_sync();
-    const uint32_t a = smem_u32(s.stages + st * kStageBytes), b = a + kOperandBytes;
+    if (elected()) {
+      const uint64_t from = uint64_t(uint32_t(ring.stage * (kStageBytes >> 4)));  // (addresses of 18 bits: nothing is carried out of their field)
 #pragma unroll
-    for (int kk = 0; kk < kSlabK / 16; ++kk) {
-      // K-major: 16 elements along K are 32 bytes of a swizzle row; MN-major: 16 K-rows are two groups of eight rows of 128 bytes
-      const uint64_t ad = a_mn ? make_smem_desc(a + kk * 2048, 8192, 1024) : make_smem_desc(a + kk * 32, 16, 1024);
-      const uint64_t bd = b_mn ? make_smem_desc(b + kk * 2048, 8192, 1024) : make_smem_desc(b + kk * 32, 16, 1024);
-      if (PAIR) umma_f16_pair(d, ad, bd, idesc, (k > 0 || kk > 0) ? 1u : 0u);
-      else umma_f16(d, ad, bd, idesc, (k > 0 || kk > 0) ? 1u : 0u);
+      for (int kk = 0; kk < kSlabK / 16; ++kk) {
+        if (PAIR) umma_f16_pair(d, a0 + from + kk * a_step, b0 + from + kk * b_step, idesc, (k > 0 || kk > 0) ? 1u : 0u);
+        else umma_f16(d, a0 + from + kk * a_step, b0 + from + kk * b_step, idesc, (k > 0 || kk > 0) ? 1u : 0u);
+      }
+      if (PAIR) umma_commit_pair(&s.empty[ring.stage]);
+      else umma_commit(&s.empty[ring.stage]);
+      if (k + 1 == slabs) {
+        if (PAIR) umma_commit_pair(&s.acc_full[acc]);
+        else umma_commit(&s.acc_full[acc]);
+      }
     }
-    if (PAIR) umma_commit_pair(&s.empty[st]);
-    else umma_commit(&s.empty[st]);
+    __syncwarp();
   }
-  if (PAIR) umma_commit_pair(&s.acc_full[acc]);
-  else umma_commit(&s.acc_full[acc]);
   return true;
 }
+// What has been issued ends, when a wait has run out.
 template <bool PAIR>
 __device__ __forceinline__ void drain_products(const Shared& s) {
   *s.failed = 1;
-  if (PAIR) umma_commit_pair(s.drained);
-  else umma_commit(s.drained);
-  mbar_wait(s.drained, 0, kTimeoutNs);
+  if (elected()) {
+    if (PAIR) umma_commit_pair(s.drained);
+    else umma_commit(s.drained);
+  }
+  __syncwarp();
+  warp_wait(s.drained, 0);
 }
 
 __device__ __forceinline__ void nan16(float (&v)[16]) {
@@ -527,22 +568,21 @@ __global__ void __launch_bounds__(kThreads, 1) ce_logits_kernel(const __grid_con
   may_follow();  // (the next kernel reads x and w before it waits for this one: they are complete)
 
   if (warp == 0) {
-    if (lane == 0) {
-      int i = 0;
-      for (int tile = first; tile < total; tile += step) {
-        const TileAt at = tile_at(tile);
-        if (skip(at)) continue;
-        if (!load_tile<PAIR>(s, &maps.a, &maps.b, false, false, at, rank, 0, slabs, i)) break;
-      }
-      drain_loads(s, rank, i);
+    Ring ring;
+    for (int tile = first; tile < total; tile += step) {
+      const TileAt at = tile_at(tile);
+      if (skip(at)) continue;
+      if (!load_tile<PAIR>(s, &maps.a, &maps.b, false, false, at, rank, 0, slabs, ring)) break;
     }
+    drain_loads(s, rank, ring);
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      int i = 0, n = 0;
+    if (rank == 0) {
+      Ring ring;
+      int n = 0;
       bool ok = true;
       for (int tile = first; tile < total && ok; tile += step) {
-        if (skip(tile_at(tile))) continue;
-        ok = multiply_tile<PAIR, std::is_same<T, __nv_bfloat16>::value>(s, tmem, false, false, slabs, n, i);
+        if (some && skip(tile_at(tile))) continue;
+        ok = multiply_tile<PAIR, std::is_same<T, __nv_bfloat16>::value>(s, tmem, false, false, slabs, n, ring);
         ++n;
       }
       if (!ok) drain_products<PAIR>(s);
@@ -606,52 +646,60 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const __grid_con
   follow();
   may_follow();  // (the next kernel reads x and w before it waits for this one: they are complete)
   if (warp == 0) {
-    if (lane == 0) {
-      int i = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x)
-        for (int k = 0; k < slabs; ++k, ++i) {
-          const int st = i % F::kCount;
-          if (i >= F::kCount && !mbar_wait(&empty[st], uint32_t((i / F::kCount - 1) & 1), kTimeoutNs)) {
-            *failed = 1;
-            ok = false;
-            break;
-          }
+    Ring ring;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x)
+      for (int k = 0; k < slabs; ++k, ring.next(F::kCount)) {
+        const int st = ring.stage;
+        if (ring.round > 0 && !warp_wait(&empty[st], (ring.round - 1) & 1)) {
+          *failed = 1;
+          ok = false;
+          break;
+        }
+        if (elected()) {
           uint8_t* a = stages + st * F::kStage;
           mbar_arrive_expect_tx(&full[st], F::kStage);
           tma_operand<false>(a, &maps.a, k * kSlabK, tile * kTileM, 0, smem_u32(&full[st]));
           tma_operand<false>(a + kOperandBytes, &maps.b, k * kSlabK, 0, 0, smem_u32(&full[st]));
         }
-      for (int j = max(0, i - F::kCount); j < i; ++j) mbar_wait(*failed == 0 ? &empty[j % F::kCount] : &full[j % F::kCount], uint32_t((j / F::kCount) & 1), kTimeoutNs);
+        __syncwarp();
+      }
+    const int under_way = ring.round > 0 ? F::kCount : ring.stage;
+    for (int j = 0; j < under_way; ++j) {
+      if (ring.stage == 0) ring.stage = F::kCount, --ring.round;
+      --ring.stage;
+      warp_wait(*failed == 0 ? &empty[ring.stage] : &full[ring.stage], ring.round & 1);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = (1u << 4) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(TOKENS >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
-      int i = 0, n = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x, ++n) {
-        if (n >= 2 && !mbar_wait(&acc_empty[n & 1], uint32_t((n / 2 - 1) & 1), kTimeoutNs)) ok = false;
-        tc_fence_after_sync();
-        for (int k = 0; k < slabs && ok; ++k, ++i) {
-          const int st = i % F::kCount;
-          if (!mbar_wait(&full[st], uint32_t((i / F::kCount) & 1), kTimeoutNs)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after_sync();
-          const uint32_t a = smem_u32(stages + st * F::kStage), b = a + kOperandBytes;
-#pragma unroll
-          for (int kk = 0; kk < kSlabK / 16; ++kk)
-            umma_f16(tmem + uint32_t((n & 1) * TOKENS), make_smem_desc(a + kk * 32, 16, 1024), make_smem_desc(b + kk * 32, 16, 1024), idesc, (k > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(&empty[st]);
+    constexpr uint32_t idesc = (1u << 4) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(TOKENS >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
+    const uint64_t a0 = make_smem_desc(smem_u32(stages), 16, 1024), b0 = make_smem_desc(smem_u32(stages) + kOperandBytes, 16, 1024);
+    Ring ring;
+    int n = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x, ++n) {
+      if (n >= 2 && !warp_wait(&acc_empty[n & 1], uint32_t((n / 2 - 1) & 1))) ok = false;
+      tc_fence_after_sync();
+      for (int k = 0; k < slabs && ok; ++k, ring.next(F::kCount)) {
+        if (!warp_wait(&full[ring.stage], ring.round & 1)) {
+          ok = false;
+          break;
         }
-        if (ok) umma_commit(&acc_full[n & 1]);
+        tc_fence_after_sync();
+        if (elected()) {
+          const uint64_t from = uint64_t(uint32_t(ring.stage * (F::kStage >> 4)));
+#pragma unroll
+          for (int kk = 0; kk < kSlabK / 16; ++kk) umma_f16(tmem + uint32_t((n & 1) * TOKENS), a0 + from + kk * 2, b0 + from + kk * 2, idesc, (k > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&empty[ring.stage]);
+          if (k + 1 == slabs) umma_commit(&acc_full[n & 1]);
+        }
+        __syncwarp();
       }
-      if (!ok) {
-        *failed = 1;
-        umma_commit(drained);
-        mbar_wait(drained, 0, kTimeoutNs);
-      }
+    }
+    if (!ok) {
+      *failed = 1;
+      if (elected()) umma_commit(drained);
+      __syncwarp();
+      warp_wait(drained, 0);
     }
   } else {
     const int quad = warp & 3;
@@ -792,17 +840,15 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gradients_kernel(const __grid_
   follow();
   Task t;
   if (warp == 0) {
-    if (lane == 0) {
-      int i = 0;
-      for (int k = 0; task_of(g, pair, pairs, k, t); ++k)
-        if (!load_tile<true>(s, t.x ? &maps.e_rows : &maps.e_columns, t.x ? &maps.w : &maps.xs, !t.x, true, t.at, rank, t.slab0, t.slabs, i)) break;
-      drain_loads(s, rank, i);
-    }
+    Ring ring;
+    for (int k = 0; task_of(g, pair, pairs, k, t); ++k)
+      if (!load_tile<true>(s, t.x ? &maps.e_rows : &maps.e_columns, t.x ? &maps.w : &maps.xs, !t.x, true, t.at, rank, t.slab0, t.slabs, ring)) break;
+    drain_loads(s, rank, ring);
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      int i = 0;
+    if (rank == 0) {
+      Ring ring;
       bool ok = true;
-      for (int k = 0; ok && task_of(g, pair, pairs, k, t); ++k) ok = multiply_tile<true, std::is_same<T, __nv_bfloat16>::value>(s, tmem, !t.x, true, t.slabs, k, i);
+      for (int k = 0; ok && task_of(g, pair, pairs, k, t); ++k) ok = multiply_tile<true, std::is_same<T, __nv_bfloat16>::value>(s, tmem, !t.x, true, t.slabs, k, ring);
       if (!ok) drain_products<true>(s);
     }
   } else {
