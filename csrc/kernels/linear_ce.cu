@@ -47,7 +47,9 @@ constexpr int kStages = 5;
 constexpr int kSlotBytes = 32 * 128;             // 32 rows of 64 values in 16 bits, or of 32 in fp32
 constexpr int kEpilogueWarps = 8;                // two for each quarter of tensor memory, each with one half of a tile's columns
 constexpr int kSlots = 2;                        // of each
-constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * kSlots * kSlotBytes + 1024 + 256;
+constexpr int kBiasBytes = 32 * 4;               // of 32 columns, for each of the epilogue's warps
+constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * (kSlots * kSlotBytes + kBiasBytes) + 1024 + 256;
+static_assert(kSmem <= 227 * 1024, "what a CTA can have");
 constexpr int kThreads = 64 + 32 * kEpilogueWarps;  // warp 0: TMA, warp 1: products, the others: epilogue
 constexpr uint64_t kTimeoutNs = 10ull * 1000 * 1000 * 1000;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -121,6 +123,7 @@ struct TileAt {
 // What a CTA's roles share, in shared memory.
 struct Shared {
   uint8_t *stages, *slots;
+  float* bias;                     // [kEpilogueWarps][32]
   uint64_t *full, *empty;          // [kStages]
   uint64_t *acc_full, *acc_empty;  // [2]
   uint64_t* drained;
@@ -131,7 +134,8 @@ __device__ __forceinline__ Shared shared_parts(uint8_t* raw) {
   Shared s;
   s.stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   s.slots = s.stages + kStages * kStageBytes;
-  s.full = reinterpret_cast<uint64_t*>(s.slots + kEpilogueWarps * kSlots * kSlotBytes);
+  s.bias = reinterpret_cast<float*>(s.slots + kEpilogueWarps * kSlots * kSlotBytes);
+  s.full = reinterpret_cast<uint64_t*>(s.bias + kEpilogueWarps * 32);
   s.empty = s.full + kStages;
   s.acc_full = s.empty + kStages;
   s.acc_empty = s.acc_full + 2;
@@ -334,14 +338,17 @@ struct LogitRow {
 };
 // 32 columns from `first` on: their part of the row's sums, and with E its 64 bytes of the slot from sixteen bytes `at` on.
 template <typename T, int KIND>
-__device__ __forceinline__ void take_logits(const Rows& rows, LogitRow& r, uint32_t (&raw)[32], bool ok, int first, uint8_t* slot, int lane, int at) {
+__device__ __forceinline__ void take_logits(const Rows& rows, LogitRow& r, uint32_t (&raw)[32], bool ok, int first, float bias, float* biases, uint8_t* slot, int lane, int at) {
   float v[32];
 #pragma unroll
   for (int k = 0; k < 32; ++k) v[k] = ok ? __uint_as_float(raw[k]) : __uint_as_float(0x7fc00000u);
-  if (rows.bias != nullptr) {
+  if (rows.bias != nullptr) {  // each lane's column to all lanes
+    __syncwarp();
+    biases[lane] = bias;
+    __syncwarp();
 #pragma unroll
     for (int k = 0; k < 32; k += 4) {
-      const float4 b = __ldg(reinterpret_cast<const float4*>(rows.bias + first + k));
+      const float4 b = *reinterpret_cast<const float4*>(biases + k);
       v[k] += b.x, v[k + 1] += b.y, v[k + 2] += b.z, v[k + 3] += b.w;
     }
   }
@@ -397,42 +404,70 @@ __device__ __forceinline__ void take_logits(const Rows& rows, LogitRow& r, uint3
     *box_at(slot, lane, at + e) = packed;
   }
 }
-// A tile of logits, the n-th, by one of the epilogue's warps: 32 columns at a time, the next on their way out of tensor memory.
-// (Sixteen at a time, each waited for, the epilogue took longer than the products for K up to 1024: 1229 x 1024 x 30592 75 us.)
+// What the epilogue's lanes read from memory for a tile: their row's, and one column's of each 32.
+template <int HALF>
+struct LogitInputs {
+  int64_t target;
+  float ref, mul, value, bias[HALF / 32];
+};
+// The warp's first row and column in a tile.
+template <bool PAIR>
+__device__ __forceinline__ TileAt warp_at(const TileAt& at, uint32_t rank) {
+  const int warp = threadIdx.x >> 5;  // (lanes 32 (warp & 3) and on of tensor memory are the ones that it may read; half of the columns)
+  return {at.m0 + int(rank) * kTileM + (warp & 3) * 32, at.n0 + ((warp - 2) >> 2) * (PAIR ? 128 : 64)};
+}
+template <int KIND, int HALF>
+__device__ __forceinline__ void fetch_inputs(const Rows& rows, const TileAt& at, LogitInputs<HALF>& in) {
+  const int lane = threadIdx.x & 31, row = at.m0 + lane;
+  in.target = -1;
+  in.ref = 0.0f, in.mul = 1.0f, in.value = 0.0f;
+  if (row < rows.n) {
+    in.target = rows.targets[row];
+    if (KIND != kStats) in.ref = rows.ref[row];
+    if (KIND == kWeighted) in.mul = rows.mul[row], in.value = rows.value[row];
+  }
+  if (rows.bias != nullptr) {
+#pragma unroll
+    for (int k = 0; k < HALF / 32; ++k) in.bias[k] = at.n0 + k * 32 < rows.classes ? rows.bias[at.n0 + k * 32 + lane] : 0.0f;
+  }
+}
+// A tile of logits, the n-th, by one of the epilogue's warps: 32 columns at a time, the next on their way out of tensor memory, what memory has to give for the tile after this one
+// on its way too. (Columns sixteen at a time and each waited for, rows and bias read when they were needed, which takes 2000 cycles while the operands' copies fill the way from L2, the epilogue
+// took longer than the products for K up to 1024: 1229 x 1024 x 30592 75 us.)
 template <typename T, int KIND, bool PAIR>
-__device__ __forceinline__ void finish_logits(const Shared& s, uint32_t tmem, const Rows& rows, const CUtensorMap* out, const TileAt& at, uint32_t rank, int n, uint32_t& used) {
+__device__ __forceinline__ void finish_logits(const Shared& s, uint32_t tmem, const Rows& rows, const CUtensorMap* out, const TileAt& at, const TileAt* next, uint32_t rank, int n,
+                                              LogitInputs<(PAIR ? 128 : 64)>& in, uint32_t& used) {
   constexpr int kSide = PAIR ? 256 : 128, kHalf = kSide / 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int quad = warp & 3, half = (warp - 2) >> 2;  // the lanes of tensor memory that this warp may read; its half of the columns
-  const int row0 = at.m0 + int(rank) * kTileM + quad * 32, row = row0 + lane, col0 = at.n0 + half * kHalf;
+  const TileAt mine_at = warp_at<PAIR>(at, rank);
+  const int row0 = mine_at.m0, row = row0 + lane, col0 = mine_at.n0;
   const bool mine = row0 < rows.n && col0 < rows.classes;
   LogitRow r;
-  r.target = -1;
-  r.dead = true;
-  r.ref = 0.0f, r.mul = 1.0f, r.value = 0.0f;
+  r.dead = in.target < 0 || in.target >= rows.classes;
+  r.target = r.dead ? -1 : int(in.target);
+  r.ref = in.ref, r.mul = in.mul, r.value = in.value;
   r.most = -INFINITY;
   r.sum[0] = r.sum[1] = 0;
-  if (mine && row < rows.n) {
-    const int64_t t = rows.targets[row];
-    r.dead = t < 0 || t >= rows.classes;
-    r.target = r.dead ? -1 : int(t);
-    if (KIND != kStats) r.ref = rows.ref[row];
-    if (KIND == kWeighted) r.mul = rows.mul[row], r.value = rows.value[row];
-  }
+  float bias[kHalf / 32];
+#pragma unroll
+  for (int k = 0; k < kHalf / 32; ++k) bias[k] = in.bias[k];
+  if (next != nullptr) fetch_inputs<KIND, kHalf>(rows, warp_at<PAIR>(*next, rank), in);
   const bool ok = accumulator_here(s, n);
   if (mine) {
-    const uint32_t from = tmem + (uint32_t(quad * 32) << 16) + uint32_t((n & 1) * kSide + half * kHalf);
+    const uint32_t from = tmem + (uint32_t((warp & 3) * 32) << 16) + uint32_t((n & 1) * kSide + ((warp - 2) >> 2) * kHalf);
+    float* biases = s.bias + (warp - 2) * 32;
     uint32_t left[32], right[32];
     tmem_ld_32x32b_x32_start(from, left);
-#pragma unroll 1
-    for (int c = 0; c < kHalf && col0 + c < rows.classes; c += 64) {
+#pragma unroll
+    for (int c = 0; c < kHalf; c += 64) {
+      if (col0 + c >= rows.classes) break;
       uint8_t* slot = KIND != kStats ? free_slot(s, used) : nullptr;
       tmem_ld_wait(left);
       tmem_ld_32x32b_x32_start(from + c + 32, right);
-      take_logits<T, KIND>(rows, r, left, ok, col0 + c, slot, lane, 0);
+      take_logits<T, KIND>(rows, r, left, ok, col0 + c, bias[c / 32], biases, slot, lane, 0);
       tmem_ld_wait(right);
       if (c + 64 < kHalf) tmem_ld_32x32b_x32_start(from + c + 64, left);
-      take_logits<T, KIND>(rows, r, right, ok, col0 + c + 32, slot, lane, 4);
+      take_logits<T, KIND>(rows, r, right, ok, col0 + c + 32, bias[c / 32 + 1], biases, slot, lane, 4);
       if (KIND != kStats) {
         send_slot(slot, out, col0 + c, row0, 0, false);
         ++used;
@@ -590,11 +625,20 @@ __global__ void __launch_bounds__(kThreads, 1) ce_logits_kernel(const __grid_con
   } else {
     int n = 0;
     uint32_t used = 0;
-    for (int tile = first; tile < total; tile += step) {
-      const TileAt at = tile_at(tile);
-      if (skip(at)) continue;
-      finish_logits<T, KIND, PAIR>(s, tmem, rows, &maps.out, at, rank, n, used);
-      ++n;
+    LogitInputs<(PAIR ? 128 : 64)> in;
+    auto from = [&](int tile) {  // the first one that is made
+      while (some && tile < total && skip(tile_at(tile))) tile += step;
+      return tile;
+    };
+    int tile = from(first);
+    TileAt at = tile_at(tile);
+    if (tile < total) fetch_inputs<KIND, (PAIR ? 128 : 64)>(rows, warp_at<PAIR>(at, rank), in);
+    for (; tile < total; ++n) {
+      const int then = from(tile + step);
+      const TileAt next = tile_at(then);
+      finish_logits<T, KIND, PAIR>(s, tmem, rows, &maps.out, at, then < total ? &next : nullptr, rank, n, in, used);
+      tile = then;
+      at = next;
     }
     if (lane == 0) bulk_wait_read();  // the stores have left shared memory; the end of the kernel is what others wait for
   }
