@@ -288,11 +288,12 @@ __device__ __forceinline__ bool accumulator_here(const Shared& s, int n) {
   tc_fence_after_sync();
   return all;
 }
+// (With an arrival that also waits for the warp's stores, 2400 cycles a tile.)
 template <bool PAIR>
 __device__ __forceinline__ void accumulator_read(const Shared& s, int n) {
   tc_fence_before_sync();
   __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive_at((PAIR ? rank0_address(&s.acc_empty[0]) : smem_u32(&s.acc_empty[0])) + uint32_t(n & 1) * 8);
+  if ((threadIdx.x & 31) == 0) mbar_arrive_only((PAIR ? rank0_address(&s.acc_empty[0]) : smem_u32(&s.acc_empty[0])) + uint32_t(n & 1) * 8);
 }
 // A slot of this warp's that nothing goes out of any more, and its way out; `used`: how many have been filled.
 __device__ __forceinline__ uint8_t* free_slot(const Shared& s, uint32_t used) {
@@ -796,7 +797,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const __grid_con
       }
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive_at(smem_u32(&acc_empty[n & 1]));
+      if (lane == 0) mbar_arrive_only(smem_u32(&acc_empty[n & 1]));
     }
 #pragma unroll
     for (int j = 0; j < (TOKENS + 31) / 32; ++j) {

@@ -131,6 +131,11 @@ __device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_address) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_address) : "memory");
 }
 
+// The same for a barrier that hands over no memory, only tensor memory that has been read (behind tc_fence_before_sync): it does not wait until this thread's stores are seen by the cluster.
+__device__ __forceinline__ void mbar_arrive_only(uint32_t cluster_address) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_address) : "memory");
+}
+
 // ---- untiled bulk copy global -> shared (both addresses 16-byte aligned, size a multiple of 16) ------
 // Never used with cluster multicast; the source is always this GPU's own memory.
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* gmem_src, uint32_t bytes, uint64_t* bar) {
