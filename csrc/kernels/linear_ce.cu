@@ -51,6 +51,8 @@ constexpr int kBiasBytes = 32 * 4;               // of 32 columns, for each of t
 constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * (kSlots * kSlotBytes + kBiasBytes) + 1024 + 256;
 static_assert(kSmem <= 227 * 1024, "what a CTA can have");
 constexpr int kThreads = 64 + 32 * kEpilogueWarps;  // warp 0: TMA, warp 1: products, the others: epilogue
+constexpr int kTasks = 4;                           // tiles that a pair of CTAs has taken and not all of its warps have read
+constexpr int kTaskReaders = 2 * (kEpilogueWarps + 1);  // the epilogues, the products of rank 0, the copies of rank 1
 constexpr uint64_t kTimeoutNs = 10ull * 1000 * 1000 * 1000;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -95,7 +97,7 @@ struct Gradients {
   Result x, w;          // dx = E w, dw = E^T x'
   Columns columns;
   const float* alpha;
-  int extra;            // tiles of dw that a pair takes on top of the others' where it has a tile of dx less
+  int* next;            // the next tile that nobody has taken
 };
 struct GradientMaps {
   CUtensorMap e_rows, w, out_x;      // dx
@@ -127,6 +129,8 @@ struct Shared {
   uint64_t *full, *empty;          // [kStages]
   uint64_t *acc_full, *acc_empty;  // [2]
   uint64_t* drained;
+  uint64_t *task_full, *task_empty;  // [kTasks]
+  volatile int* task;              // [kTasks]
   uint32_t* tmem_slot;
   volatile uint32_t* failed;       // a wait has run out
 };
@@ -140,7 +144,10 @@ __device__ __forceinline__ Shared shared_parts(uint8_t* raw) {
   s.acc_full = s.empty + kStages;
   s.acc_empty = s.acc_full + 2;
   s.drained = s.acc_empty + 2;
-  s.tmem_slot = reinterpret_cast<uint32_t*>(s.drained + 1);
+  s.task_full = s.drained + 1;
+  s.task_empty = s.task_full + kTasks;
+  s.task = reinterpret_cast<int*>(s.task_empty + kTasks);
+  s.tmem_slot = reinterpret_cast<uint32_t*>(s.task_empty + kTasks) + kTasks;
   s.failed = s.tmem_slot + 1;
   return s;
 }
@@ -155,6 +162,10 @@ __device__ __forceinline__ void init_barriers(const Shared& s) {
     mbar_init(&s.acc_empty[i], kEpilogueWarps * (PAIR ? 2 : 1));
   }
   mbar_init(s.drained, 1);
+  for (int i = 0; i < kTasks; ++i) {
+    mbar_init(&s.task_full[i], 1);
+    mbar_init(&s.task_empty[i], kTaskReaders);
+  }
   *s.failed = 0;
   fence_barrier_init();
 }
@@ -810,34 +821,59 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const __grid_con
   if (warp == 1) tmem_dealloc(tmem, kColumns);
 }
 
-// dx = E w and dw = E^T x' in one launch of pairs of CTAs. A tile of dx has all classes as its K, one of dw all tokens of the group, and there may be fewer tiles of dx than pairs: each
-// pair takes its share of dx's tiles first, and where it has one less than others, tiles of dw for it. So both end together. dx's K is cut in parts where a
-// single tile would take longer than that.
+// dx = E w and dw = E^T x' in one launch of pairs of CTAs. A tile of dx has all classes as its K, one of dw all tokens of the group, and there may be fewer tiles of dx than pairs: those
+// are taken first, by whoever comes for the next tile, and those of dw fill up what is left, so that all end together. dx's K is cut in parts where a
+// single tile would take longer than that. (Shared out beforehand by their slabs, the first pairs were done 90 us before the last of 440: 4096 x 768 x 50304.)
 struct Task {
   bool x;
   TileAt at;
   int part, slab0, slabs;
 };
-__device__ __forceinline__ bool task_of(const Gradients& g, int pair, int pairs, int k, Task& t) {
-  const int more = g.x.total % pairs;                      // pairs that have a tile of dx more than the others
-  const int mine = g.x.total / pairs + (pair < more ? 1 : 0);
-  int i;
-  t.x = k < mine;
-  if (t.x) {
-    i = k * pairs + pair;
-  } else {
-    const int j = k - mine, ahead = more > 0 ? g.extra : 0;  // tiles of dw of the pairs without
-    if (pair >= more && j < ahead) i = j * (pairs - more) + pair - more;
-    else i = ahead * (pairs - more) + (pair >= more ? j - ahead : j) * pairs + pair;
-    if (i >= g.w.total) return false;
-  }
+__device__ __forceinline__ bool task_of(const Gradients& g, int i, Task& t) {
+  t.x = i < g.x.total;
+  if (!t.x) i -= g.x.total;
   const Result& r = t.x ? g.x : g.w;
+  if (i >= r.total) return false;
   t.part = i / r.per;
   i -= t.part * r.per;
   t.slab0 = t.part * r.slabs;
   t.slabs = min(r.slabs, (r.K + kSlabK - 1) / kSlabK - t.slab0);
   t.at.m0 = i / r.tiles_n * 256;
   t.at.n0 = i % r.tiles_n * 256;
+  return true;
+}
+// Rank 0's copies take the pair's next tile, and tell all of its warps (both CTAs'); the one after it is asked for at the same time.
+struct Taker {
+  int ahead;  // in lane 0
+  Ring ring;
+};
+__device__ __forceinline__ bool take_task(const Shared& s, const Gradients& g, Taker& t, int& id) {
+  const int lane = threadIdx.x & 31;
+  if (t.ring.round > 0 && !warp_wait(&s.task_empty[t.ring.stage], (t.ring.round - 1) & 1)) return false;
+  id = __shfl_sync(0xffffffffu, t.ahead, 0);
+  if (lane < 2) {
+    store_cluster(cluster_address(const_cast<const int*>(&s.task[t.ring.stage]), uint32_t(lane)), id);
+    mbar_arrive_at(cluster_address(&s.task_full[t.ring.stage], uint32_t(lane)));
+  }
+  if (lane == 0) t.ahead = atomicAdd(g.next, 1);
+  __syncwarp();
+  t.ring.next(kTasks);
+  return true;
+}
+__device__ __forceinline__ bool read_task(const Shared& s, Ring& ring, int& id) {
+  uint64_t* bar = &s.task_full[ring.stage];
+  const uint32_t parity = ring.round & 1;
+  if (!__all_sync(0xffffffffu, mbar_try_wait_cluster(bar, parity))) {
+    const uint64_t t0 = timer_ns();
+    uint32_t spins = 0;
+    while (!__all_sync(0xffffffffu, mbar_try_wait_cluster(bar, parity))) {
+      if ((++spins & 255u) == 0u && __any_sync(0xffffffffu, timer_ns() - t0 > kTimeoutNs)) return false;
+    }
+  }
+  id = s.task[ring.stage];
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive_only(rank0_address(&s.task_empty[0]) + uint32_t(ring.stage) * 8);
+  ring.next(kTasks);
   return true;
 }
 template <typename T>
@@ -873,7 +909,6 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gradients_kernel(const __grid_
   const Shared s = shared_parts(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
-  const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
   if (threadIdx.x == 0) {
     prefetch_tensormap(&maps.e_rows);
     prefetch_tensormap(&maps.w);
@@ -884,23 +919,45 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gradients_kernel(const __grid_
   may_follow();
   follow();
   Task t;
+  int id = 0;
+  Ring tasks;
   if (warp == 0) {
     Ring ring;
-    for (int k = 0; task_of(g, pair, pairs, k, t); ++k)
+    Taker taker;
+    taker.ahead = rank == 0 && lane == 0 ? atomicAdd(g.next, 1) : 0;
+    for (;;) {
+      if (!(rank == 0 ? take_task(s, g, taker, id) : read_task(s, tasks, id))) {
+        *s.failed = 1;
+        break;
+      }
+      if (!task_of(g, id, t)) break;
       if (!load_tile<true>(s, t.x ? &maps.e_rows : &maps.e_columns, t.x ? &maps.w : &maps.xs, !t.x, true, t.at, rank, t.slab0, t.slabs, ring)) break;
+    }
     drain_loads(s, rank, ring);
   } else if (warp == 1) {
     if (rank == 0) {
       Ring ring;
       bool ok = true;
-      for (int k = 0; ok && task_of(g, pair, pairs, k, t); ++k) ok = multiply_tile<true, std::is_same<T, __nv_bfloat16>::value>(s, tmem, !t.x, true, t.slabs, k, ring);
+      for (int k = 0; ok; ++k) {
+        ok = read_task(s, tasks, id);
+        if (!ok || !task_of(g, id, t)) break;
+        ok = multiply_tile<true, std::is_same<T, __nv_bfloat16>::value>(s, tmem, !t.x, true, t.slabs, k, ring);
+      }
       if (!ok) drain_products<true>(s);
     }
   } else {
     uint32_t used = 0;
     if (g.columns.partial != nullptr) add_columns<T>(g.columns, int(blockIdx.x) * kEpilogueWarps + warp - 2, int(gridDim.x) * kEpilogueWarps);
-    for (int k = 0; task_of(g, pair, pairs, k, t); ++k)
-      finish_result<T>(s, tmem, t.x ? g.x : g.w, g.alpha, t.x ? &maps.out_x : &maps.out_w, t.at, t.part, rank, k, used);
+    for (int k = 0;; ++k) {
+      auto finish = [&](int n) { finish_result<T>(s, tmem, t.x ? g.x : g.w, g.alpha, t.x ? &maps.out_x : &maps.out_w, t.at, t.part, rank, n, used); };
+      if (!read_task(s, tasks, id)) {  // nobody knows what is missing: all of it is not a number
+        *s.failed = 1;
+        for (int i = 0; task_of(g, i, t); ++i) finish(i);
+        break;
+      }
+      if (!task_of(g, id, t)) break;
+      finish(k);
+    }
     if (lane == 0) bulk_wait_read();
   }
   products_end<true>(tmem);
@@ -925,6 +982,8 @@ struct Begin {
   float* bias;    // padded to whole tiles
   int bias_count;
   Scales* scales;
+  int* next;      // [groups] of the gradients' tiles; set to 0
+  int64_t groups;
   float e_scale;  // power of two by which E is larger
 };
 __device__ __forceinline__ float bias_value(const void* b, int dtype, int i) {
@@ -970,6 +1029,8 @@ __global__ void __launch_bounds__(kBeginT) ce_begin_kernel(const __grid_constant
   if (blockIdx.x == 0) {
     __shared__ int64_t counts[kBeginT / 32];
     __shared__ float tops[kBeginT / 32];
+    if (a.what != NANGILA_CE_LOSSES)
+      for (int64_t i = threadIdx.x; i < a.groups; i += kBeginT) a.next[i] = 0;
     int64_t count = 0;
     float top = 0.0f;
     bool bad = false;
@@ -1434,7 +1495,7 @@ struct Plan {
   bool pair, few;     // tiles of the logits
   bool wide;          // dw is summed up over the groups
   int split;          // parts of dx's K
-  int64_t at_scales, at_zt, at_bias, at_ref, at_mul, at_value, at_factor, at_again, at_parts, at_e, at_xs, at_sums, at_dx, at_columns, total;
+  int64_t at_scales, at_next, at_zt, at_bias, at_ref, at_mul, at_value, at_factor, at_again, at_parts, at_e, at_xs, at_sums, at_dx, at_columns, total;
   int64_t bias_count;
 };
 constexpr int64_t kGroupBytes = int64_t(1) << 29;  // of E
@@ -1464,6 +1525,7 @@ Plan plan(const NangilaLinearCeParams& p, int what) {
     return at;
   };
   l.at_scales = take(sizeof(Scales));
+  l.at_next = take(l.groups * 4);
   l.at_zt = take(what == NANGILA_CE_BOTH ? p.n * 4 : 0);
   l.at_ref = take(what == NANGILA_CE_BOTH ? p.n * 4 : what == NANGILA_CE_GRADIENTS ? l.group * 4 : 0);
   l.at_bias = take(p.bias != nullptr ? l.bias_count * 4 : 0);
@@ -1502,6 +1564,8 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
   begin.bias = bias;
   begin.bias_count = int(l.bias_count);
   begin.scales = scales;
+  begin.next = reinterpret_cast<int*>(ws + l.at_next);
+  begin.groups = l.groups;
   begin.e_scale = what == NANGILA_CE_GRADIENTS && std::is_same<T, __half>::value ? 32768.0f : 1.0f;
   int e = 0;
   if (what != NANGILA_CE_LOSSES || p.bias != nullptr) {
@@ -1585,7 +1649,7 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
         ok = ok && make_map(&maps.xs, xs, 64, 64) && (l.wide ? make_map(&maps.out_w, wide, 32, 32) : make_map(&maps.out_w, out, 64, 32));
       }
       if (!ok) return int(cudaErrorNotSupported);
-      if (p.dx != nullptr && p.dw != nullptr) q.extra = (q.x.slabs + q.w.slabs / 2) / q.w.slabs;
+      q.next = begin.next + g;
       auto* kernel = ce_gradients_kernel<T>;
       if (const int err = allow_smem(reinterpret_cast<const void*>(kernel), kSmem)) return err;
       cudaLaunchAttribute attr[2];
