@@ -72,6 +72,7 @@ def build_bert(args, dev, world):
     from nangila.models.bert import BertConfig, BertMLM, mask_tokens
 
     cfg = BertConfig.tiny() if args.small else BertConfig.large()
+    cfg.fused_vocab = args.fused_vocab
     model = BertMLM(cfg).to(dev)
     # the fused DGC kernel makes several grid-wide passes per bucket and the selection is taken per bucket, so
     # fewer, larger buckets amortise that and select more globally (--bucket-mb, same in both arms)
@@ -100,7 +101,7 @@ def build_bert(args, dev, world):
     info = {"model": "bert-tiny" if args.small else "bert-large 24L d1024 h16 mlp4096 vocab30522", "unit": "tokens/s",
             "items_per_step": b * t * world, "global_batch": b * world, "seq_len": t, "parallelism": f"dp{world}",
             "compressor": "DGC sparsity 0.999 with momentum correction" if hook else "stock DDP all-reduce",
-            "bucket_mb": args.bucket_mb, "optimizer": "AdamW(fused)"}
+            "bucket_mb": args.bucket_mb, "optimizer": "AdamW(fused)", "fused_vocab": args.fused_vocab}
     return ddp, opt, hook, host, put, loss_fn, info
 
 
@@ -111,7 +112,7 @@ def build_llama(args, dev, world):
     from nangila.models.llama import Llama, LlamaConfig
 
     cfg = LlamaConfig.tiny() if args.small else LlamaConfig.llama_1_3b()
-    cfg.fused = args.fused
+    cfg.fused, cfg.fused_vocab = args.fused, args.fused_vocab
     model = Llama(cfg).to(dev)
     mp = MixedPrecisionPolicy(param_dtype=torch.bfloat16, reduce_dtype=torch.bfloat16)
     for blk in model.blocks:
@@ -153,7 +154,7 @@ def build_llama(args, dev, world):
             "unit": "tokens/s", "items_per_step": b * t * world, "global_batch": b * world, "seq_len": t,
             "parallelism": f"fsdp{world} (fully_shard per block)",
             "compressor": "block-INT4 reduce-scatter + INT8 all-gather (fused kernels)" if colls else "stock FSDP2 (NCCL)",
-            "optimizer": "AdamW(fused)", "fused": args.fused}
+            "optimizer": "AdamW(fused)", "fused": args.fused, "fused_vocab": args.fused_vocab}
     return model, opt, (_Hook() if colls else None), host, put, loss_fn, info
 
 
@@ -171,7 +172,10 @@ def main() -> int:
     ap.add_argument("--no-e2e", action="store_true")
     ap.add_argument("--fused", action="store_true", help="Llama configuration: norms and rotary positions through nangila.ops (either arm)")
     ap.add_argument("--bucket-mb", type=int, default=25, help="DDP bucket size of the BERT configuration")
+    ap.add_argument("--fused-vocab", action="store_true", help="BERT and Llama configurations: embeddings and the head's loss through nangila.ops (either arm)")
     args = ap.parse_args()
+    if args.fused_vocab and args.config == "resnet50-powersgd":
+        ap.error("--fused-vocab is an option of bert-large-dgc and llama-1.3b-fsdp")
     if args.fused and args.config != "llama-1.3b-fsdp":
         ap.error("--fused is an option of llama-1.3b-fsdp")
     args.warmup = max(args.warmup, 3)

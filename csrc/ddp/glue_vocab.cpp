@@ -117,6 +117,8 @@ Tensor dropout(const Tensor& x, const c10::optional<Tensor>& residual_in, int64_
     TORCH_CHECK_TYPE(residual.scalar_type() == x.scalar_type(), "nangila: residual is ", residual.scalar_type(), ", x ", x.scalar_type());
     TORCH_CHECK_VALUE(residual.device() == x.device(), "nangila: residual is on ", residual.device(), ", x on ", x.device());
   }
+  check_no_tracer();  // (a mask would become a constant)
+  if (x.is_cuda()) check_unseen({&x, &residual});
   TORCH_CHECK_VALUE(least >= 0 && least <= int64_t(1) << 32 && draw >= 0 && draw < int64_t(1) << 32, "nangila: p or draw out of range");
   Mask mask{least, draw, seed_in.value_or(0), seed_tensor.value_or(Tensor())};
   if (mask.seed_tensor.defined()) {
@@ -139,7 +141,6 @@ Tensor dropout(const Tensor& x, const c10::optional<Tensor>& residual_in, int64_
     if (residual.defined()) y = y + residual.to(at::kFloat);
     return y.to(x.scalar_type());
   }
-  check_unseen({&x, &residual});
   if (!wants_grad({&x, &residual})) return dropout_launch(x, residual, mask);
   return Dropout::apply(x, residual_in, mask.seed_tensor.defined() ? c10::optional<Tensor>(mask.seed_tensor) : c10::nullopt, mask.least, mask.draw, mask.seed);
 }

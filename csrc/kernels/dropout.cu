@@ -53,7 +53,7 @@ __device__ __forceinline__ uint4 philox(uint64_t block, uint32_t draw, uint32_t 
 __device__ __forceinline__ void drop8(float (&v)[8], float scale, const uint4& c, uint32_t upper) {
   const uint32_t w[4] = {c.x, c.y, c.z, c.w}, least = upper << 16;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = ((i & 1) ? w[i / 2] : w[i / 2] << 16) >= least ? v[i] * scale : 0.0f;
+  for (int i = 0; i < 8; ++i) v[i] = ((i & 1) ? w[i / 2] : w[i / 2] << 16) >= least ? __fmul_rn(v[i], scale) : 0.0f;
 }
 // Whether one of the upper halves may equal that of `least`: an equal one leaves a zero half of x, which borrows into its top bit (one above a zero half may too: looked at for nothing).
 __device__ __forceinline__ bool tied8(const uint4& c, uint32_t upper) {

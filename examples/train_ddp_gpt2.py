@@ -36,6 +36,8 @@ def main() -> int:
     ap.add_argument("--micro-batch", type=int, default=8)
     ap.add_argument("--optimizer", default="adamw", choices=["adamw", "muon"],
                     help="muon: the blocks' matrices take Muon steps, everything else stays with AdamW")
+    ap.add_argument("--dropout", type=float, default=0.0, help="of the embeddings and the blocks' outputs")
+    ap.add_argument("--fused-vocab", action="store_true", help="embeddings and the head's loss through nangila.ops")
     ap.add_argument("--checkpoint", default="")
     ap.add_argument("--save-every", type=int, default=50)
     ap.add_argument("--liveness-timeout", type=float, default=0.0,
@@ -44,6 +46,7 @@ def main() -> int:
     rank, world, dev = init_distributed()
     seed_everything(0)
     cfg = GPT2Config.tiny() if args.tiny else GPT2Config.small()
+    cfg.dropout, cfg.fused_vocab = args.dropout, args.fused_vocab
     model = GPT2(cfg).to(dev)
     if dev.type == "cuda":
         model = model.to(torch.bfloat16)

@@ -28,11 +28,12 @@ def main() -> int:
     ap.add_argument("--parameter-bits", type=int, default=8, choices=[4, 8])
     ap.add_argument("--no-compress", action="store_true")
     ap.add_argument("--fused", action="store_true", help="norms and rotary positions through nangila.ops")
+    ap.add_argument("--fused-vocab", action="store_true", help="the embedding and the head's loss through nangila.ops")
     args = ap.parse_args()
     rank, world, dev = init_distributed()
     seed_everything(0)
     cfg = LlamaConfig.tiny() if args.tiny else LlamaConfig.llama_1_3b()
-    cfg.fused = args.fused
+    cfg.fused, cfg.fused_vocab = args.fused, args.fused_vocab
     model = Llama(cfg).to(dev)
     mp = MixedPrecisionPolicy(param_dtype=torch.bfloat16, reduce_dtype=torch.bfloat16)
     for blk in model.blocks:

@@ -4,6 +4,10 @@
 Post-LayerNorm encoder blocks, learned position and segment embeddings, GELU MLP, and the MLM head
 (dense + GELU + LayerNorm, decoder tied to the token embedding). The reference ships no model; its
 examples train Hugging Face models through DDP (examples/train_llm.py:230-332).
+
+``BertConfig(fused_vocab=True)`` takes the embeddings and the decoder with its loss through ``nangila.ops``: table gradients by sorted tokens, and no
+logits in memory. ``dropout`` drops, in training, from the embeddings and from each block's two outputs before they are added and normalised
+(``nangila.ops.dropout``; attention weights are not dropped).
 """
 from __future__ import annotations
 
@@ -12,6 +16,8 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from .. import ops
 
 
 @dataclass
@@ -26,6 +32,8 @@ class BertConfig:
     type_vocab: int = 2
     mask_token: int = 103
     mask_prob: float = 0.15
+    dropout: float = 0.0       # of the embeddings and the blocks' outputs, in training
+    fused_vocab: bool = False  # nangila.ops for the embeddings and the decoder's loss
 
     @staticmethod
     def large() -> "BertConfig":
@@ -44,7 +52,7 @@ class BertConfig:
 class EncoderBlock(nn.Module):
     def __init__(self, cfg: BertConfig):
         super().__init__()
-        self.n_head = cfg.n_head
+        self.n_head, self.dropout = cfg.n_head, cfg.dropout
         self.qkv = nn.Linear(cfg.d_model, 3 * cfg.d_model)
         self.proj = nn.Linear(cfg.d_model, cfg.d_model)
         self.ln1 = nn.LayerNorm(cfg.d_model, eps=1e-12)
@@ -56,8 +64,14 @@ class EncoderBlock(nn.Module):
         b, t, c = x.shape
         q, k, v = self.qkv(x).view(b, t, 3, self.n_head, c // self.n_head).unbind(dim=2)
         y = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), attn_mask=attn_mask)
-        x = self.ln1(x + self.proj(y.transpose(1, 2).reshape(b, t, c)))
-        return self.ln2(x + self.out(F.gelu(self.fc(x))))
+        x = self.ln1(self._add(x, self.proj(y.transpose(1, 2).reshape(b, t, c))))
+        return self.ln2(self._add(x, self.out(F.gelu(self.fc(x)))))
+
+    def _add(self, x: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
+        if not (self.training and self.dropout):
+            return x + y
+        # (under autocast the projection has another type than the normalised stream)
+        return ops.dropout(y.to(x.dtype), self.dropout, residual=x)
 
 
 class BertMLM(nn.Module):
@@ -84,9 +98,12 @@ class BertMLM(nn.Module):
     def encode(self, ids: torch.Tensor, segments: torch.Tensor | None = None,
                padding_mask: torch.Tensor | None = None) -> torch.Tensor:
         b, t = ids.shape
-        x = self.tok(ids) + self.pos(torch.arange(t, device=ids.device))
-        x = x + self.seg(segments if segments is not None else torch.zeros_like(ids))
+        look = (lambda i, table: ops.embedding(i, table.weight)) if self.cfg.fused_vocab else (lambda i, table: table(i))
+        x = look(ids, self.tok) + look(torch.arange(t, device=ids.device), self.pos)
+        x = x + look(segments if segments is not None else torch.zeros_like(ids), self.seg)
         x = self.ln_emb(x)
+        if self.training and self.cfg.dropout:
+            x = ops.dropout(x, self.cfg.dropout)
         mask = None if padding_mask is None else padding_mask[:, None, None, :].to(torch.bool)
         for blk in self.blocks:
             x = blk(x, mask)
@@ -103,6 +120,8 @@ class BertMLM(nn.Module):
             x = x.reshape(-1, x.size(-1))[sel]
             tgt = labels.reshape(-1)[sel]
         h = self.head_ln(F.gelu(self.head_dense(x)))
+        if self.cfg.fused_vocab and labels is not None:
+            return ops.linear_cross_entropy(h, self.tok.weight, tgt, bias=self.head_bias, num_classes=self.cfg.vocab_size)
         logits = F.linear(h, self.tok.weight, self.head_bias)
         if labels is None:
             return logits

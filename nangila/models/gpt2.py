@@ -8,6 +8,10 @@ The reference ships no model; its examples train Hugging Face causal LMs through
 GEMMs go to cuBLAS through ``torch.nn.functional.linear`` and attention to the fused
 ``scaled_dot_product_attention`` kernel; the loss over the padded vocabulary is this framework's fused
 cross-entropy kernel pair (``nangila/ops/fused_ce.py``); the gradient exchange is what this framework replaces.
+
+``GPT2Config(fused_vocab=True)`` takes the embeddings and the tied head with its loss through ``nangila.ops``: table gradients by sorted tokens, and no
+logits in memory. ``dropout`` drops, in training, from the embeddings and from what each block adds to the residual stream (``nangila.ops.dropout``;
+attention weights are not dropped).
 """
 from __future__ import annotations
 
@@ -18,6 +22,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .. import ops
 from ..ops import fused_grads as FG
 
 
@@ -30,6 +35,8 @@ class GPT2Config:
     vocab_size: int = 50257
     n_ctx: int = 1024
     padded_vocab: int = 50304  # multiple of 128: keeps the LM-head GEMM on aligned tiles
+    dropout: float = 0.0       # of the embeddings and the blocks' outputs, in training
+    fused_vocab: bool = False  # nangila.ops for the embeddings and the head's loss
 
     @staticmethod
     def small() -> "GPT2Config":
@@ -43,7 +50,7 @@ class GPT2Config:
 class Block(nn.Module):
     def __init__(self, cfg: GPT2Config):
         super().__init__()
-        self.n_head = cfg.n_head
+        self.n_head, self.dropout = cfg.n_head, cfg.dropout
         self.ln1 = nn.LayerNorm(cfg.d_model)
         self.qkv = nn.Linear(cfg.d_model, 3 * cfg.d_model)
         self.proj = nn.Linear(cfg.d_model, cfg.d_model)
@@ -58,9 +65,15 @@ class Block(nn.Module):
         qkv = FG.linear(FG.layer_norm(x, self.ln1), self.qkv).view(b, t, 3, self.n_head, c // self.n_head)
         q, k, v = qkv.unbind(dim=2)
         y = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True)
-        x = x + FG.linear(y.transpose(1, 2).reshape(b, t, c), self.proj)
-        x = x + FG.linear(F.gelu(FG.linear(FG.layer_norm(x, self.ln2), self.fc), approximate="tanh"), self.out)
+        x = self._add(x, FG.linear(y.transpose(1, 2).reshape(b, t, c), self.proj))
+        x = self._add(x, FG.linear(F.gelu(FG.linear(FG.layer_norm(x, self.ln2), self.fc), approximate="tanh"), self.out))
         return x
+
+    def _add(self, x: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
+        if not (self.training and self.dropout):
+            return x + y
+        # (under autocast the projection has another type than the residual stream)
+        return ops.dropout(y.to(x.dtype), self.dropout, residual=x)
 
 
 class GPT2(nn.Module):
@@ -88,10 +101,17 @@ class GPT2(nn.Module):
     def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None):
         b, t = idx.shape
         pos = torch.arange(t, device=idx.device)
-        x = self.wte(idx) + self.wpe(pos)
+        if self.cfg.fused_vocab:
+            x = ops.embedding(idx, self.wte.weight) + ops.embedding(pos, self.wpe.weight)
+        else:
+            x = self.wte(idx) + self.wpe(pos)
+        if self.training and self.cfg.dropout:
+            x = ops.dropout(x, self.cfg.dropout)
         for blk in self.blocks:
             x = blk(x)
         x = FG.layer_norm(x, self.ln_f)
+        if self.cfg.fused_vocab and targets is not None:
+            return ops.linear_cross_entropy(x, self.wte.weight, targets, num_classes=self.cfg.vocab_size)
         logits = F.linear(x, self.wte.weight)  # tied head over the padded vocabulary
         if targets is None:
             return logits

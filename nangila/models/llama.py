@@ -9,6 +9,8 @@ the architecture is defined directly and initialised randomly. Each :class:`Deco
 ``LlamaConfig(fused=True)`` takes the norms (with the residual's addition inside a block) and the rotary positions through
 ``nangila.ops``: one kernel each, forward and backward, where PyTorch's operations make several passes. Results agree with the other
 path up to the last rounding (the benchmark's step on one GPU: 126 -> 90 ms). It also opens the positions' options: the half layout, part of the head, scaling for long contexts.
+
+``LlamaConfig(fused_vocab=True)`` takes the embedding and the head with its loss through ``nangila.ops``: the table's gradient by sorted tokens, and no logits in memory.
 """
 from __future__ import annotations
 
@@ -39,6 +41,7 @@ class LlamaConfig:
     rope_scaling: Optional[str] = None       # "linear", "ntk" or "yarn" (nangila.ops.rotary_table)
     rope_factor: float = 1.0
     rope_original_seq: Optional[int] = None
+    fused_vocab: bool = False                # nangila.ops for the embedding and the head's loss
 
     def __post_init__(self):
         self.check()
@@ -158,11 +161,14 @@ class Llama(nn.Module):
         if self._rope is None or self._rope.device != idx.device or self._rope.size(0) < t:
             with torch.inference_mode(False):  # (a table made by an evaluation serves the training that follows)
                 self._rope = self._table(max(t, self.cfg.max_seq), idx.device)
-        x = self.embed(idx)
+        x = ops.embedding(idx, self.embed.weight) if self.cfg.fused_vocab else self.embed(idx)
         rope = Angles(self._rope) if self.cfg.fused else self._rope
         for blk in self.blocks:
             x = blk(x, rope)
-        logits = self.head(ops.rms_norm(x, self.norm.weight, eps=self.norm.eps) if self.cfg.fused else self.norm(x))
+        x = ops.rms_norm(x, self.norm.weight, eps=self.norm.eps) if self.cfg.fused else self.norm(x)
+        if self.cfg.fused_vocab and targets is not None:
+            return ops.linear_cross_entropy(x, self.head.weight, targets)
+        logits = self.head(x)
         if targets is None:
             return logits
         from ..ops.fused_ce import fused_cross_entropy  # fused kernels for bf16 logits on a GPU, PyTorch's path otherwise
