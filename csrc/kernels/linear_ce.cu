@@ -4,7 +4,7 @@
 // are all that is written; a last kernel joins them to lse and loss. The target's own logit is a dot product in fp32 by itself and is left out of the sums:
 // loss = log(1 + sum over the others of exp(z_v - z_t)) keeps its digits where the model is sure.
 //
-// Gradients need G = exp(z - lse) - [v = t] twice: dx = G w and dw = G^T x. A group of tokens at a time (as many as fit into half a gigabyte of 16-bit values) the tiles' epilogue
+// Gradients need G = exp(z - lse) - [v = t] twice: dx = G w and dw = G^T x. A group of tokens at a time (as many as fit into a gigabyte of 16-bit values) the tiles' epilogue
 // writes exponentials E, and two products read them. The exponent's reference need not be lse, which is known only when the whole row is: in bf16, whose range is that of
 // fp32, E = exp(z - z_t) is as good. Its row sums give lse, and the factor f = exp(z_t - lse) of each row is applied to the rows of dx, and to those of x
 // on their way into dw. So the losses and the gradients take three products (6 n d V operations), where logits that are formed again for the gradients take four. A row in which some z is above z_t by more than
@@ -396,7 +396,6 @@ __device__ __forceinline__ void take_logits(const Rows& rows, LogitRow& r, uint3
     v[k] = exp2_fast(a), v[k + 1] = exp2_fast(b);
     if constexpr (KIND != kWeighted) r.sum[(k / 2) & 1] = add_pair(r.sum[(k / 2) & 1], pair_of(v[k], v[k + 1]));
   }
-  if constexpr (KIND == kStats) return;
   if constexpr (KIND == kWeighted) {
 #pragma unroll
     for (int k = 0; k < 32; ++k) v[k] *= r.mul;
@@ -406,14 +405,16 @@ __device__ __forceinline__ void take_logits(const Rows& rows, LogitRow& r, uint3
         if (first + k == r.target) v[k] = r.value;
     }
   }
+  if constexpr (KIND != kStats) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float w[8];
+    for (int e = 0; e < 4; ++e) {
+      float w[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) w[k] = v[8 * e + k];
-    uint4 packed = pack16<T>(w);
-    if (r.dead) packed = make_uint4(0, 0, 0, 0);
-    *box_at(slot, lane, at + e) = packed;
+      for (int k = 0; k < 8; ++k) w[k] = v[8 * e + k];
+      uint4 packed = pack16<T>(w);
+      if (r.dead) packed = make_uint4(0, 0, 0, 0);
+      *box_at(slot, lane, at + e) = packed;
+    }
   }
 }
 // What the epilogue's lanes read from memory for a tile: their row's, and one column's of each 32.
@@ -1099,114 +1100,110 @@ struct Group {
 __device__ __forceinline__ float folded(float value, float rounded, float factor) {
   return fabsf(rounded) > 1e-4f && fabsf(rounded) < 1e30f ? value / rounded : factor;
 }
-// Losses and lse of the joined sums; with E: also the element at the target and the rows' factors. pass 0: NANGILA_CE_LOSSES; 1, 2: NANGILA_CE_BOTH, for all rows
-// and for those of tiles that were formed again.
+// A CTA's rows: losses and lse of the joined sums; with E also the element at the target and the rows' factors.
 template <typename T>
-__global__ void __launch_bounds__(kRowsT) ce_rows_kernel(const __grid_constant__ Group a, int pass, int tile_rows) {
+__device__ __forceinline__ void join_rows(const Group& a, int pass, const float* logit) {
   constexpr int kWarps = kRowsT / 32;
   __shared__ float2 joined[kWarps][kRowsAtOnce];
-  __shared__ float logit[kRowsAtOnce];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row0 = blockIdx.x * kRowsAtOnce, row = row0 + lane;
-  if (pass == 0 && row0 + warp < a.n) {
-    const float z = target_logit<T>(a.p, a.row0 + row0 + warp);
-    if (lane == 0) logit[warp] = z;
-  }
-  follow();
-  if (pass == 2) {
-    const int all = (a.n + 31) / 32, per = tile_rows / 32;
-    const int from = int(blockIdx.x) / per * per;
-    bool any = false;
-    for (int i = from; i < min(from + per, all); ++i) any = any || a.again[i] != 0;
-    if (!any) return;
-  }
+  const int row = blockIdx.x * kRowsAtOnce + lane;
   const bool here = row < a.n;
   const float ref = pass != 0 && here ? a.ref[row] : 0.0f;
   float most = -INFINITY, sum = 0.0f;
+  auto add = [&](const float2 v) {
+    if (pass == 0) {
+      const float now = fmaxf(most, v.x), base = now == -INFINITY ? 0.0f : now;
+      sum = sum * exp2_fast(most - base) + v.y * exp2_fast(v.x - base);
+      most = now;
+    } else {
+      most = fmaxf(most, v.x);
+      sum += v.y;
+    }
+  };
   if (here) {
 #pragma unroll 8
-    for (int i = warp; i < a.parts_count; i += kWarps) {
-      const float2 v = a.parts[int64_t(i) * a.stride + row];
-      if (pass == 0) {
-        const float now = fmaxf(most, v.x), base = now == -INFINITY ? 0.0f : now;
-        sum = sum * exp2_fast(most - base) + v.y * exp2_fast(v.x - base);
-        most = now;
-      } else {
-        most = fmaxf(most, v.x);
-        sum += v.y;
-      }
-    }
+    for (int i = warp; i < a.parts_count; i += kWarps) add(a.parts[int64_t(i) * a.stride + row]);
   }
   joined[warp][lane] = make_float2(most, sum);
   __syncthreads();
-  if (warp == 0) {
-    for (int w = 1; w < kWarps; ++w) {
-      const float2 v = joined[w][lane];
-      if (pass == 0) {
-        const float now = fmaxf(most, v.x), base = now == -INFINITY ? 0.0f : now;
-        sum = sum * exp2_fast(most - base) + v.y * exp2_fast(v.x - base);
-        most = now;
-      } else {
-        most = fmaxf(most, v.x);
-        sum += v.y;
+  if (warp != 0) return;
+  for (int w = 1; w < kWarps; ++w) add(joined[w][lane]);
+  bool above = false;
+  if (here) {
+    const int64_t i = a.row0 + row, t = a.p.targets[i];
+    const bool ignored = t == a.p.ignore, outside = !ignored && (t < 0 || t >= a.p.classes);
+    const float zt2 = (pass == 0 ? logit[lane] : a.zt[row]) * kLog2e;
+    float loss, lse2, factor = 0.0f;
+    if (pass == 0) {
+      // sum of exp2(z - most) over the others; the target's own on top
+      const float base = fmaxf(most, zt2);
+      const float rest = sum * exp2_fast(most - base), own = exp2_fast(zt2 - base);
+      lse2 = base + log2f(rest + own);
+      loss = zt2 >= most ? log1pf(sum * exp2_fast(most - zt2)) : (base - zt2) * kLn2 + logf(rest + own);
+    } else {
+      const float own = exp2_fast(zt2 - ref), whole = sum + own;
+      above = pass == 1 && !ignored && !outside && most - ref > kMostAbove;
+      factor = 1.0f / whole;
+      lse2 = ref + log2f(whole);
+      loss = ref == zt2 ? log1pf(sum) : (ref - zt2) * kLn2 + logf(whole);
+      if (above) a.ref[row] = most;  // (more than z_t: the largest of the row)
+      if (!ignored && !outside) {
+        const T element = dev::Vec16<T>::from_float(-sum);
+        static_cast<T*>(a.e)[int64_t(row) * a.e_stride + t] = element;
+        factor = folded(sum / whole, -dev::Vec16<T>::to_float(element), factor);
       }
     }
-    bool above = false;
-    float factor = 0.0f;
-    if (here) {
-      const int64_t i = a.row0 + row, t = a.p.targets[i];
-      const bool ignored = t == a.p.ignore, outside = !ignored && (t < 0 || t >= a.p.classes);
-      const float zt2 = (pass == 0 ? logit[lane] : a.zt[row]) * kLog2e;
-      float loss, lse2;
-      if (pass == 0) {
-        // sum of exp2(z - most) over the others; the target's own on top
-        const float base = fmaxf(most, zt2);
-        const float rest = sum * exp2_fast(most - base), own = exp2_fast(zt2 - base);
-        lse2 = base + log2f(rest + own);
-        loss = zt2 >= most ? log1pf(sum * exp2_fast(most - zt2)) : (base - zt2) * kLn2 + logf(rest + own);
-      } else {
-        const float own = exp2_fast(zt2 - ref), whole = sum + own;
-        above = pass == 1 && !ignored && !outside && most - ref > kMostAbove;
-        factor = 1.0f / whole;
-        lse2 = ref + log2f(whole);
-        loss = ref == zt2 ? log1pf(sum) : (ref - zt2) * kLn2 + logf(whole);
-        if (above) a.ref[row] = most;  // (more than z_t: the largest of the row)
-        if (!ignored && !outside && a.e != nullptr) {
-          const T element = dev::Vec16<T>::from_float(-sum);
-          static_cast<T*>(a.e)[int64_t(row) * a.e_stride + t] = element;
-          factor = folded(sum / whole, -dev::Vec16<T>::to_float(element), factor);
-        }
-      }
-      if (ignored || outside) {
-        loss = ignored ? 0.0f : __uint_as_float(0x7fc00000u);
-        factor = 0.0f;
-      }
-      a.p.losses[i] = loss;
-      if (a.p.lse != nullptr) a.p.lse[i] = lse2 * kLn2;
-      if (a.factor != nullptr) a.factor[row] = factor;
+    if (ignored || outside) {
+      loss = ignored ? 0.0f : __uint_as_float(0x7fc00000u);
+      factor = 0.0f;
     }
-    if (pass == 1) {
-      const bool any = __any_sync(0xffffffffu, above);
-      if (lane == 0) a.again[blockIdx.x] = any ? 1 : 0;
-    }
+    a.p.losses[i] = loss;
+    a.p.lse[i] = lse2 * kLn2;
+    if (pass != 0) a.factor[row] = factor;
+  }
+  if (pass == 1) {
+    const bool any = __any_sync(0xffffffffu, above);
+    if (lane == 0) a.again[blockIdx.x] = any ? 1 : 0;
   }
 }
-// NANGILA_CE_BOTH: the rows of x times their factors, as dw's product takes them.
+// NANGILA_CE_LOSSES (pass 0), and NANGILA_CE_BOTH's first pass over all rows (1).
 template <typename T>
-__global__ void __launch_bounds__(kWeightsT) ce_scale_kernel(const __grid_constant__ Group a) {
+__global__ void __launch_bounds__(kRowsT) ce_rows_kernel(const __grid_constant__ Group a, int pass) {
+  __shared__ float logit[kRowsAtOnce];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * kRowsAtOnce + warp;
+  if (pass == 0 && row < a.n) {
+    const float z = target_logit<T>(a.p, a.row0 + row);
+    if (lane == 0) logit[warp] = z;
+  }
   follow();
-  const int per = a.p.d / 8;
-  for (int64_t i = int64_t(blockIdx.x) * kWeightsT + threadIdx.x; i < int64_t(a.n) * per; i += int64_t(gridDim.x) * kWeightsT) {
-    const int row = int(i / per), c = int(i - int64_t(row) * per) * 8;
+  if (pass == 0) __syncthreads();
+  join_rows<T>(a, pass, logit);
+}
+// NANGILA_CE_BOTH: the rows of tiles that were formed again once more, and the rows of x times their factors, as dw's product takes them.
+template <typename T>
+__global__ void __launch_bounds__(kRowsT) ce_scale_kernel(const __grid_constant__ Group a, int tile_rows) {
+  follow();
+  const int all = (a.n + kRowsAtOnce - 1) / kRowsAtOnce, tile = tile_rows / kRowsAtOnce, first = int(blockIdx.x) / tile * tile;
+  bool any = false;
+  for (int i = first; i < min(first + tile, all); ++i) any = any || a.again[i] != 0;
+  if (any) {
+    join_rows<T>(a, 2, nullptr);
+    __syncthreads();
+  }
+  if (a.xs == nullptr) return;
+  const int per = a.p.d / 8, row0 = blockIdx.x * kRowsAtOnce, rows = min(kRowsAtOnce, a.n - row0);
+#pragma unroll 4
+  for (int i = threadIdx.x; i < rows * per; i += kRowsT) {
+    const int r = i / per, row = row0 + r;
     const float f = a.factor[row];
     dev::Raw8<T> raw;
-    dev::fetch(static_cast<const T*>(a.p.x) + (a.row0 + row) * a.p.x_stride + c, raw);
+    dev::fetch(static_cast<const T*>(a.p.x) + (a.row0 + row) * a.p.x_stride + (i - r * per) * 8, raw);
     float v[8];
     dev::unpack(raw, v);
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = f == 0.0f ? 0.0f : v[k] * f;
     dev::pack(v, raw);
-    dev::put(static_cast<T*>(a.xs) + i * 8, raw);
+    dev::put(static_cast<T*>(a.xs) + int64_t(row0) * a.p.d + int64_t(i) * 8, raw);
   }
 }
 // NANGILA_CE_GRADIENTS: what the tiles' epilogue takes of each row, and the rows of x without those that add nothing.
@@ -1240,90 +1237,117 @@ __global__ void __launch_bounds__(kWeightsT) ce_weights_kernel(const __grid_cons
     dev::put(static_cast<T*>(a.xs) + i * 8, raw);
   }
 }
-// The sum or mean of the losses, in a fixed order.
-__global__ void __launch_bounds__(1024) ce_total_kernel(const float* losses, const int64_t* targets, int64_t n, int64_t ignore, int mean, float* out) {
-  __shared__ double part[32], counted[32];
-  follow();
+// What is left behind the products, each by its own CTAs of one launch.
+struct Finish {
+  const Scales* scales;
+  // dx = alpha f_row times the sum of its parts
+  const float *dx_parts, *factor;
+  void* dx;
+  int64_t dx_part, dx_count;    // values of a part, eights of dx
+  int parts, per, dx_ctas;      // eights of a row
+  // dw = alpha sums
+  const float* dw_sums;
+  void* dw;
+  int64_t dw_count;             // eights
+  int dw_ctas;
+  // the bias's gradient out of the shares' sums of all groups
+  const float* columns;
+  void* dbias;
+  int64_t columns_stride;
+  int shares, classes, rows, bias_dtype, bias_ctas;
+  // the sum or mean of the losses
+  const float* losses;
+  const int64_t* targets;
+  float* loss;
+  int64_t n, ignore;
+  int mean;
+};
+constexpr int kFinishT = 256;
+// In a fixed order, in 64 bits.
+__device__ __forceinline__ void total_loss(const Finish& a) {
+  constexpr int kWarps = kFinishT / 32;
+  __shared__ double part[kWarps], counted[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  double sum = 0.0, count = 0.0;
-#pragma unroll 4
-  for (int64_t i = threadIdx.x; i < n; i += 1024) {
-    sum += double(losses[i]);
-    count += targets[i] != ignore ? 1.0 : 0.0;
+  double sum = 0.0;
+  int64_t count = 0;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < a.n; i += kFinishT) {
+    sum += double(a.losses[i]);
+    count += a.targets[i] != a.ignore ? 1 : 0;
   }
+  double counts = double(count);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
     sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    count += __shfl_xor_sync(0xffffffffu, count, off);
+    counts += __shfl_xor_sync(0xffffffffu, counts, off);
   }
-  if (lane == 0) part[warp] = sum, counted[warp] = count;
+  if (lane == 0) part[warp] = sum, counted[warp] = counts;
   __syncthreads();
-  if (warp == 0) {
-    sum = part[lane], count = counted[lane];
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      sum += __shfl_xor_sync(0xffffffffu, sum, off);
-      count += __shfl_xor_sync(0xffffffffu, count, off);
-    }
-    if (lane == 0) *out = float(mean ? sum / count : sum);
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kWarps; ++w) sum += part[w], counts += counted[w];
+    *a.loss = float(a.mean ? sum / counts : sum);
   }
 }
-// The bias's gradient out of the shares' sums of all groups.
-__global__ void ce_bias_grad_kernel(const float* partial, int64_t stride, int shares, int classes, int rows, const Scales* scales, void* dbias, int dtype) {
-  follow();
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= rows) return;
-  float sum = 0.0f;
-  if (i < classes) {
-#pragma unroll 8
-    for (int s = 0; s < shares; ++s) sum += partial[s * stride + i];
-    sum *= scales->alpha;
-  }
-  if (dtype == NANGILA_F32) static_cast<float*>(dbias)[i] = sum;
-  else if (dtype == NANGILA_F16) static_cast<__half*>(dbias)[i] = __float2half_rn(sum);
-  else static_cast<__nv_bfloat16*>(dbias)[i] = __float2bfloat16_rn(sum);
-}
-// dx = alpha f_row times the sum of its parts, in 16 bits; parts are `part` elements apart
 template <typename T>
-__global__ void __launch_bounds__(256) ce_join_kernel(const float* sums, int64_t part, int parts, const float* factor, const Scales* scales, T* out, int64_t n8, int per) {
+__global__ void __launch_bounds__(kFinishT) ce_finish_kernel(const __grid_constant__ Finish a) {
   follow();
-  const float alpha = scales->alpha;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n8; i += int64_t(gridDim.x) * 256) {
-    const float f = factor[i / per];
-    float v[8], w[8];
+  int cta = blockIdx.x;
+  if (cta < a.dx_ctas) {
+    const float alpha = a.scales->alpha;
+    for (int64_t i = int64_t(cta) * kFinishT + threadIdx.x; i < a.dx_count; i += int64_t(a.dx_ctas) * kFinishT) {
+      const float f = a.factor[i / a.per];
+      float v[8], w[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+      for (int k = 0; k < 8; ++k) v[k] = 0.0f;
 #pragma unroll 4
-    for (int j = 0; j < parts; ++j) {
-      dev::Raw8<float> in;
-      dev::fetch(sums + j * part + i * 8, in);
-      dev::unpack(in, w);
+      for (int j = 0; j < a.parts; ++j) {
+        dev::Raw8<float> in;
+        dev::fetch(a.dx_parts + j * a.dx_part + i * 8, in);
+        dev::unpack(in, w);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] += w[k];
+        for (int k = 0; k < 8; ++k) v[k] += w[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = f == 0.0f ? 0.0f : v[k] * (alpha * f);
+      dev::Raw8<T> r;
+      dev::pack(v, r);
+      dev::put(static_cast<T*>(a.dx) + i * 8, r);
     }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = f == 0.0f ? 0.0f : v[k] * (alpha * f);
-    dev::Raw8<T> r;
-    dev::pack(v, r);
-    dev::put(out + i * 8, r);
+    return;
   }
-}
-// dw = alpha sums, in 16 bits
-template <typename T>
-__global__ void __launch_bounds__(256) ce_round_kernel(const float* sums, const Scales* scales, T* out, int64_t n8) {
-  follow();
-  const float alpha = scales->alpha;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n8; i += int64_t(gridDim.x) * 256) {
-    dev::Raw8<float> in;
-    dev::fetch(sums + i * 8, in);
-    float v[8];
-    dev::unpack(in, v);
+  cta -= a.dx_ctas;
+  if (cta < a.dw_ctas) {
+    const float alpha = a.scales->alpha;
+#pragma unroll 4
+    for (int64_t i = int64_t(cta) * kFinishT + threadIdx.x; i < a.dw_count; i += int64_t(a.dw_ctas) * kFinishT) {
+      dev::Raw8<float> in;
+      dev::fetch(a.dw_sums + i * 8, in);
+      float v[8];
+      dev::unpack(in, v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] *= alpha;
-    dev::Raw8<T> r;
-    dev::pack(v, r);
-    dev::put(out + i * 8, r);
+      for (int k = 0; k < 8; ++k) v[k] *= alpha;
+      dev::Raw8<T> r;
+      dev::pack(v, r);
+      dev::put(static_cast<T*>(a.dw) + i * 8, r);
+    }
+    return;
   }
+  cta -= a.dw_ctas;
+  if (cta < a.bias_ctas) {
+    const int i = cta * kFinishT + threadIdx.x;
+    if (i >= a.rows) return;
+    float sum = 0.0f;
+    if (i < a.classes) {
+#pragma unroll 8
+      for (int s = 0; s < a.shares; ++s) sum += a.columns[s * a.columns_stride + i];
+      sum *= a.scales->alpha;
+    }
+    if (a.bias_dtype == NANGILA_F32) static_cast<float*>(a.dbias)[i] = sum;
+    else if (a.bias_dtype == NANGILA_F16) static_cast<__half*>(a.dbias)[i] = __float2half_rn(sum);
+    else static_cast<__nv_bfloat16*>(a.dbias)[i] = __float2bfloat16_rn(sum);
+    return;
+  }
+  total_loss(a);
 }
 template <typename T>
 __device__ void rescale(T* a, int64_t n, float f) {
@@ -1498,7 +1522,8 @@ struct Plan {
   int64_t at_scales, at_next, at_zt, at_bias, at_ref, at_mul, at_value, at_factor, at_again, at_parts, at_e, at_xs, at_sums, at_dx, at_columns, total;
   int64_t bias_count;
 };
-constexpr int64_t kGroupBytes = int64_t(1) << 29;  // of E
+// Of E. (Each group more adds to dw in fp32: 8192 x 768 x 50304 with a quarter, a half and one gigabyte, four, two and one groups, 1780, 1660 and 1535 us.)
+constexpr int64_t kGroupBytes = int64_t(1) << 30;
 Plan plan(const NangilaLinearCeParams& p, int what) {
   Plan l;
   std::memset(&l, 0, sizeof l);
@@ -1510,7 +1535,7 @@ Plan plan(const NangilaLinearCeParams& p, int what) {
   l.few = what == NANGILA_CE_LOSSES && p.n <= kFewTokens;
   l.parts = l.few ? 4 * few_ctas(classes) : (classes + half - 1) / half;
   const int64_t row_bytes = what == NANGILA_CE_LOSSES ? l.parts * 8 : l.e_stride * 2;
-  const int64_t most = std::max<int64_t>(256, (what == NANGILA_CE_LOSSES ? kGroupBytes / 8 : kGroupBytes) / row_bytes / 256 * 256);
+  const int64_t most = std::max<int64_t>(256, (what == NANGILA_CE_LOSSES ? kGroupBytes / 16 : kGroupBytes) / row_bytes / 256 * 256);
   l.groups = (p.n + most - 1) / most;
   l.group = std::min(p.n, ((p.n + l.groups - 1) / l.groups + 255) / 256 * 256);
   l.groups = (p.n + l.group - 1) / l.group;
@@ -1574,6 +1599,15 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
     e = int(cudaGetLastError());
   }
 
+  auto losses_into = [&](Finish& f) {
+    f.losses = p.losses;
+    f.targets = p.targets;
+    f.loss = p.loss;
+    f.n = p.n;
+    f.ignore = p.ignore;
+    f.mean = p.mean;
+  };
+
   for (int64_t g = 0; g < l.groups && e == 0; ++g) {
     Group a;
     std::memset(&a, 0, sizeof a);
@@ -1598,7 +1632,7 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
     const int tile_rows = l.pair ? 256 : 128;
     if (what == NANGILA_CE_LOSSES) {
       e = l.few ? few<T>(x, w, rows, stream) : logits<T, kStats>(l.pair, x, w, nullptr, rows, stream);
-      if (e == 0) e = int(launch_following(ce_rows_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, 0, tile_rows));
+      if (e == 0) e = int(launch_following(ce_rows_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, 0));
       continue;
     }
     a.ref = reinterpret_cast<float*>(ws + l.at_ref) + (what == NANGILA_CE_BOTH ? a.row0 : 0);
@@ -1612,12 +1646,10 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
       a.zt = zt + a.row0;
       a.again = reinterpret_cast<int32_t*>(ws + l.at_again);
       e = logits<T, kExp>(l.pair, x, w, &ex, rows, stream);
-      if (e == 0) e = int(launch_following(ce_rows_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, 1, tile_rows));
+      if (e == 0) e = int(launch_following(ce_rows_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, 1));
       rows.again = a.again;
       if (e == 0) e = logits<T, kExp>(l.pair, x, w, &ex, rows, stream);
-      if (e == 0) e = int(launch_following(ce_rows_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, 2, tile_rows));
-      if (e == 0 && a.xs != nullptr)
-        e = int(launch_following(ce_scale_kernel<T>, dim3(unsigned(std::min<int64_t>((int64_t(a.n) * p.d / 8 + kWeightsT - 1) / kWeightsT, 148 * 8))), kWeightsT, 0, stream, a));
+      if (e == 0) e = int(launch_following(ce_scale_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, tile_rows));
     }
     if (what == NANGILA_CE_GRADIENTS) {
       a.mul = reinterpret_cast<float*>(ws + l.at_mul);
@@ -1655,20 +1687,50 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
       cudaLaunchAttribute attr[2];
       const cudaLaunchConfig_t cfg = pairs_config(attr, 2 * (p.dbias != nullptr ? sm_count() / 2 : std::min(q.x.total + q.w.total, sm_count() / 2)), true, stream);
       e = int(cudaLaunchKernelEx(&cfg, kernel, maps, q));
-      if (e == 0 && q.x.wide)
-        e = int(launch_following(ce_join_kernel<T>, dim3(unsigned(std::min<int64_t>((int64_t(a.n) * p.d / 8 + 255) / 256, 148 * 8))), 256, 0, stream, reinterpret_cast<const float*>(ws + l.at_dx),
-                                 int64_t(a.n) * p.d, q.x.split, static_cast<const float*>(a.factor), static_cast<const Scales*>(scales), static_cast<T*>(p.dx) + a.row0 * p.d, int64_t(a.n) * p.d / 8,
-                                 int(p.d / 8)));
+      if (e == 0) {
+        auto ctas_of = [](int64_t work) { return int(std::min<int64_t>((work + kFinishT - 1) / kFinishT, 148 * 8)); };
+        const bool last = g + 1 == l.groups, total = last && what == NANGILA_CE_BOTH && p.loss != nullptr;
+        Finish f;
+        std::memset(&f, 0, sizeof f);
+        f.scales = scales;
+        if (q.x.wide) {
+          f.dx_parts = reinterpret_cast<const float*>(ws + l.at_dx);
+          f.factor = a.factor;
+          f.dx = static_cast<T*>(p.dx) + a.row0 * p.d;
+          f.dx_part = int64_t(a.n) * p.d;
+          f.dx_count = f.dx_part / 8;
+          f.parts = q.x.split;
+          f.per = int(p.d / 8);
+          f.dx_ctas = ctas_of(f.dx_count);
+        }
+        if (last && l.wide) {
+          f.dw_sums = sums;
+          f.dw = p.dw;
+          f.dw_count = int64_t(p.rows) * p.d / 8;
+          f.dw_ctas = ctas_of(f.dw_count);
+        }
+        if (last && p.dbias != nullptr) {
+          f.columns = columns;
+          f.dbias = p.dbias;
+          f.columns_stride = l.e_stride;
+          f.shares = int(l.groups * l.shares);
+          f.classes = p.classes;
+          f.rows = p.rows;
+          f.bias_dtype = p.bias_dtype;
+          f.bias_ctas = int((p.rows + kFinishT - 1) / kFinishT);
+        }
+        const int ctas = f.dx_ctas + f.dw_ctas + f.bias_ctas + (total ? 1 : 0);
+        if (total) losses_into(f);
+        if (ctas > 0) e = int(launch_following(ce_finish_kernel<T>, dim3(unsigned(ctas)), kFinishT, 0, stream, f));
+      }
     }
   }
-  if (e == 0 && l.wide)
-    e = int(launch_following(ce_round_kernel<T>, dim3(unsigned(std::min<int64_t>((int64_t(p.rows) * p.d / 8 + 255) / 256, 148 * 8))), 256, 0, stream, static_cast<const float*>(sums),
-                             static_cast<const Scales*>(scales), static_cast<T*>(p.dw), int64_t(p.rows) * p.d / 8));
-  if (e == 0 && p.dbias != nullptr)
-    e = int(launch_following(ce_bias_grad_kernel, dim3(unsigned((p.rows + 255) / 256)), 256, 0, stream, static_cast<const float*>(columns), l.e_stride, int(l.groups * l.shares), int(p.classes), int(p.rows),
-                             static_cast<const Scales*>(scales), p.dbias, int(p.bias_dtype)));
-  if (e == 0 && what != NANGILA_CE_GRADIENTS && p.loss != nullptr)
-    e = int(launch_following(ce_total_kernel, dim3(1), 1024, 0, stream, static_cast<const float*>(p.losses), p.targets, p.n, p.ignore, int(p.mean), p.loss));
+  if (e == 0 && what == NANGILA_CE_LOSSES && p.loss != nullptr) {
+    Finish f;
+    std::memset(&f, 0, sizeof f);
+    losses_into(f);
+    e = int(launch_following(ce_finish_kernel<T>, dim3(1), kFinishT, 0, stream, f));
+  }
   return e;
 }
 
@@ -1690,7 +1752,7 @@ extern "C" int nangila_linear_ce(const NangilaLinearCeParams* p, int what, cudaS
   using namespace nangila;
   if (!sound(p, what) || !p->x || !p->w || !p->targets || !p->losses || !p->workspace || !aligned(p->workspace, 256) || !aligned(p->x, 16) || !aligned(p->w, 16) || p->x_stride % 8 != 0 ||
       p->w_stride % 8 != 0 || p->x_stride < p->d || p->w_stride < p->d || !aligned(p->dx, 16) || !aligned(p->dw, 16) || (p->dbias != nullptr && p->bias == nullptr) ||
-      (what == NANGILA_CE_GRADIENTS && (!p->lse || !p->upstream)) || (what == NANGILA_CE_LOSSES && !p->lse))
+      !p->lse || (what == NANGILA_CE_GRADIENTS && !p->upstream))
     return int(cudaErrorInvalidValue);
   try {
     return p->dtype == NANGILA_BF16 ? run<__nv_bfloat16>(*p, what, stream) : run<__half>(*p, what, stream);

@@ -73,7 +73,7 @@ typedef struct {
   int32_t bias_dtype;      /* any of the three */
   int32_t mean;            /* u_i is divided by the count of targets that are not ignored */
   float* losses;           /* n */
-  float* lse;              /* n; NULL with NANGILA_CE_BOTH */
+  float* lse;              /* n */
   float* loss;             /* 1: the sum of the losses, or their mean; NULL: not wanted */
   void* dx;                /* packed, of the type of x; NULL: not wanted */
   void* dw;                /* rows x d, packed; NULL: not wanted */

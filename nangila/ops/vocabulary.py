@@ -30,7 +30,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     ``reduction``: ``"mean"`` over the targets that are not ``ignore_index`` (not a number if all are), ``"sum"``, or ``"none"``, losses of the shape of ``targets``. A row whose
     target is ``ignore_index`` has loss 0 and adds nothing to any gradient, whatever it holds; one whose target is no class has a loss that is not a number, and adds nothing either.
 
-    With gradients, a group of tokens at a time has its exponentials in 16 bits in a workspace of up to half a gigabyte (256 tokens at least). In bfloat16 the gradients of
+    With gradients, a group of tokens at a time has its exponentials in 16 bits in a workspace of up to a gigabyte (256 tokens at least). In bfloat16 the gradients of
     a mean or a sum are formed along with the loss and kept until the backward pass: evaluate under ``torch.no_grad()``. float16 and ``"none"`` form the logits again in the backward pass."""
     if reduction not in REDUCTIONS:
         raise ValueError(f"nangila: reduction must be one of {REDUCTIONS}, got {reduction!r}")
