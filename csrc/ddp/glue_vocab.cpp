@@ -129,6 +129,8 @@ Tensor dropout(const Tensor& x, const c10::optional<Tensor>& residual_in, int64_
     TORCH_CHECK_VALUE(t.device() == x.device(), "nangila: the seed is on ", t.device(), ", x on ", x.device());
     mask.seed_tensor = in_memory(t);
   } else if (!seed_in.has_value()) {
+    c10::cuda::OptionalCUDAGuard guard;
+    if (x.is_cuda()) guard.set_device(x.device());
     TORCH_CHECK(!x.is_cuda() || !capturing(), "nangila: a captured graph would repeat one mask for ever; give it a seed (a tensor, which can be changed between replays)");
     auto* gen = at::get_generator_or_default<at::CPUGeneratorImpl>(c10::nullopt, at::detail::getDefaultCPUGenerator());
     std::lock_guard<std::mutex> lock(gen->mutex_);

@@ -1206,34 +1206,53 @@ __global__ void __launch_bounds__(kRowsT) ce_scale_kernel(const __grid_constant_
     dev::put(static_cast<T*>(a.xs) + int64_t(row0) * a.p.d + int64_t(i) * 8, raw);
   }
 }
+// A row's weight, upstream over the largest one, as share * 2^power with a share of 1/2 to 1: the share goes into E, where it is rounded with the rest, the power into the row of x and the row's
+// factor, which it does not round. So a row of little weight keeps the digits of its own gradient in fp16 too. A single upstream gradient is alpha, and its rows' weight one.
+struct RowWeight {
+  float share;
+  int power;
+  bool lives;
+};
+__device__ __forceinline__ RowWeight row_weight(const Group& a, int64_t i) {
+  const int64_t t = a.p.targets[i];
+  RowWeight w{1.0f, 0, t != a.p.ignore && t >= 0 && t < a.p.classes};
+  if (a.p.upstream_rows) {
+    const float unit = a.scales->unit;
+    w.share = frexpf(unit > 0.0f ? a.p.upstream[i] / unit : unit, &w.power);
+  }
+  if (!w.lives) w.share = 0.0f;
+  return w;
+}
 // NANGILA_CE_GRADIENTS: what the tiles' epilogue takes of each row, and the rows of x without those that add nothing.
 template <typename T>
 __global__ void __launch_bounds__(kWeightsT) ce_weights_kernel(const __grid_constant__ Group a) {
   follow();
   const int64_t thread = int64_t(blockIdx.x) * kWeightsT + threadIdx.x, threads = int64_t(gridDim.x) * kWeightsT;
-  auto lives = [&](int64_t i) {
-    const int64_t t = a.p.targets[i];
-    return t != a.p.ignore && t >= 0 && t < a.p.classes;
-  };
   for (int64_t row = thread; row < a.n; row += threads) {
     const int64_t i = a.row0 + row;
-    const float unit = a.scales->unit;
-    float weight = a.p.upstream_rows ? (unit > 0.0f ? a.p.upstream[i] / unit : unit) : 1.0f;
-    if (!lives(i)) weight = 0.0f;
+    const RowWeight w = row_weight(a, i);
     a.ref[row] = a.p.lse[i] * kLog2e;
-    a.mul[row] = weight * a.e_scale;
-    const float value = expm1f(-a.p.losses[i]) * weight * a.e_scale;
+    a.mul[row] = w.share * a.e_scale;
+    const float value = expm1f(-a.p.losses[i]) * w.share * a.e_scale;
     a.value[row] = value;
-    a.factor[row] = lives(i) ? folded(value, dev::Vec16<T>::to_float(dev::Vec16<T>::from_float(value)), 1.0f) : 0.0f;
+    a.factor[row] = w.lives && w.share != 0.0f ? ldexpf(folded(value, dev::Vec16<T>::to_float(dev::Vec16<T>::from_float(value)), 1.0f), w.power) : 0.0f;
   }
   if (a.xs == nullptr) return;
   const int per = a.p.d / 8;
 #pragma unroll 4
   for (int64_t i = thread; i < int64_t(a.n) * per; i += threads) {
     const int64_t row = i / per;
+    const RowWeight w = row_weight(a, a.row0 + row);
     dev::Raw8<T> raw;
     dev::fetch(static_cast<const T*>(a.p.x) + (a.row0 + row) * a.p.x_stride + (i - row * per) * 8, raw);
-    if (!lives(a.row0 + row)) raw.a = make_uint4(0, 0, 0, 0);
+    if (w.power != 0) {
+      float v[8];
+      dev::unpack(raw, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = ldexpf(v[k], w.power);
+      dev::pack(v, raw);
+    }
+    if (!w.lives) raw.a = make_uint4(0, 0, 0, 0);
     dev::put(static_cast<T*>(a.xs) + i * 8, raw);
   }
 }

@@ -180,6 +180,35 @@ def test_targets_far_below_the_largest_logit(dtype, reduction):
     check_grads(grads, want, x, w, d, dtype)
 
 
+@pytest.mark.parametrize("n", [3, 100])
+def test_targets_far_below_the_largest_logit_of_few_rows(n):
+    x, w, t, _ = inputs(n, 64, 600)
+    away = w[(t + 1) % 600].float()
+    x[1::2] = (200 * away / away.square().sum(-1, keepdim=True))[1::2].to(torch.bfloat16)
+    want = head(x, w, t)
+    assert float(want["losses"].max()) > 100
+    loss, grads = run(x, w, t)
+    assert abs(float(loss) - float(want["loss"])) <= exp_error(want, 64, 600) + 8 * U * (float(want["losses"].abs().max()) + want["z_most"])
+    check_grads(grads, want, x, w, 64, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_weights_far_apart(dtype):
+    # each row's own gradient keeps its digits, whatever the others' weights are: row by row the same as alone, up to the roundings of E and of the result
+    n, d, rows = 300, 64, 500
+    x, w, t, _ = inputs(n, d, rows, dtype)
+    up = 4096.0 * 2.0 ** -torch.linspace(0, 14, n, device=DEV) * torch.where(torch.arange(n, device=DEV) % 3 == 0, -1.0, 1.0)
+    up[5] = 0.0
+    want = head(x, w, t, reduction="none", upstream=up)
+    _, grads = run(x, w, t, None, up, reduction="none")
+    hs, exp = half_step(dtype), exp_error(want, d, rows)
+    # (fp16's subnormal steps: of E, 2^-25 under 2^14 at least, of a row's weight; of the result)
+    small = 2.0 ** -39 * up.abs().double()[:, None] * w.double().abs().sum(0) if dtype == torch.float16 else 0.0
+    tol = want["dx_size"] * (hs * (1 + 2 * hs) + exp + (rows / 16 + 17) * 2.0 ** -22 + 8 * U) + small + rounding(want["dx"], dtype) * 1.01
+    assert bool(((grads[0].double() - want["dx"]).abs() <= tol).all()) and not grads[0][5].any()
+    check_grads(grads, want, x, w, d, dtype)
+
+
 def test_a_model_that_is_sure():
     # losses down to 1e-23: what is left of the gradient is the sum of the others, not 1 - p
     n, d, rows = 200, 64, 300
