@@ -307,22 +307,23 @@ HeadGrads head_gradients(Head& h, bool want_x, bool want_w, bool want_b) {
 }
 // the loss or losses, and what a backward pass needs: losses and lse, and with `both` the gradients for an upstream gradient of one
 struct HeadOut {
-  Tensor result, losses, lse;
+  Tensor result, losses, lse;  // (losses of their own, where the result may change under a caller's hands)
   HeadGrads grads;
 };
-HeadOut head_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& targets, int64_t classes, int64_t ignore, int64_t reduction, bool both) {
+HeadOut head_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& targets, int64_t classes, int64_t ignore, int64_t reduction, bool both, bool keep) {
   c10::cuda::CUDAGuard guard(x.device());
   const at::TensorOptions f32 = x.options().dtype(at::kFloat);
   HeadOut o;
   o.losses = at::empty(targets.sizes(), f32);
   o.lse = at::empty(targets.sizes(), f32);
   if (reduction != kNone) o.result = targets.numel() == 0 ? at::full({}, reduction == kMean ? NAN : 0.0, f32) : at::empty({}, f32);
-  else o.result = o.losses;
+  else o.result = keep ? at::empty(targets.sizes(), f32) : o.losses;
   if (targets.numel() == 0) return o;
   Head h = head_of(x, weight, bias, targets, classes, ignore, reduction == kMean);
   h.p.losses = o.losses.data_ptr<float>();
   h.p.lse = o.lse.data_ptr<float>();
   h.p.loss = reduction != kNone ? o.result.data_ptr<float>() : nullptr;
+  h.p.losses_too = reduction == kNone && keep ? o.result.data_ptr<float>() : nullptr;
   if (both) o.grads = head_gradients(h, x.requires_grad(), weight.requires_grad(), bias.defined() && bias.requires_grad());
   head_launch(h, both ? NANGILA_CE_BOTH : NANGILA_CE_LOSSES);
   return o;
@@ -334,7 +335,7 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
     const Tensor bias = bias_in.value_or(Tensor());
     // One upstream gradient for all rows: bf16 has the range to form the gradients along with the losses. (Half precision waits for the scale of its loss.)
     const bool both = reduction != kNone && x.scalar_type() == at::kBFloat16 && targets.numel() > 0;
-    HeadOut o = head_forward(x, weight, bias, targets, classes, ignore, reduction, both);
+    HeadOut o = head_forward(x, weight, bias, targets, classes, ignore, reduction, both, true);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({x, weight, bias, targets, o.losses, o.lse});
     ctx->saved_data["classes"] = classes;
@@ -346,7 +347,7 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
       if (o.grads.dw.defined()) ctx->saved_data["dw"] = o.grads.dw;
       if (o.grads.db.defined()) ctx->saved_data["db"] = o.grads.db;
     }
-    return reduction == kNone ? o.losses.clone() : o.result;
+    return o.result;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once_only();
@@ -441,7 +442,7 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
   }
   TORCH_CHECK_TYPE(x.scalar_type() != at::kFloat, "nangila: the kernels take float16 and bfloat16 on a CUDA device, not float32 (under torch.autocast it is cast)");
   check_unseen({&x, &weight, &bias});
-  if (!wants_grad({&x, &weight, &bias})) return head_forward(x, weight, bias, targets, classes, ignore, reduction, false).result;
+  if (!wants_grad({&x, &weight, &bias})) return head_forward(x, weight, bias, targets, classes, ignore, reduction, false, false).result;
   return LinearCrossEntropy::apply(x, weight, bias_in, targets, classes, ignore, reduction);
 }
 

@@ -674,6 +674,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const __grid_con
   constexpr int kColumns = TOKENS <= 16 ? 32 : 2 * TOKENS;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int targets[TOKENS];
+  __shared__ float2 joined[4][TOKENS];
   uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(stages + F::kCount * F::kStage);
   uint64_t *empty = full + F::kCount, *acc_full = empty + F::kCount, *acc_empty = acc_full + 2, *drained = acc_empty + 2;
@@ -811,10 +812,22 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const __grid_con
       __syncwarp();
       if (lane == 0) mbar_arrive_only(smem_u32(&acc_empty[n & 1]));
     }
+    // the four warps' pairs, for one part a CTA
 #pragma unroll
-    for (int j = 0; j < (TOKENS + 31) / 32; ++j) {
-      const int t = j * 32 + lane;
-      if (t < rows.n && t < TOKENS) rows.parts[int64_t(blockIdx.x * 4 + quad) * rows.stride + t] = make_float2(most[j], sum[j]);
+    for (int j = 0; j < (TOKENS + 31) / 32; ++j)
+      if (j * 32 + lane < TOKENS) joined[quad][j * 32 + lane] = make_float2(most[j], sum[j]);
+    __syncwarp();
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    const int t = threadIdx.x - 64;
+    if (t < TOKENS && t < rows.n) {
+      float2 all = joined[0][t];
+#pragma unroll
+      for (int q = 1; q < 4; ++q) {
+        const float2 v = joined[q][t];
+        const float now = fmaxf(all.x, v.x), base = now == -INFINITY ? 0.0f : now;
+        all = make_float2(now, all.y * exp2_fast(all.x - base) + v.y * exp2_fast(v.x - base));
+      }
+      rows.parts[int64_t(blockIdx.x) * rows.stride + t] = all;
     }
   }
   tc_fence_before_sync();
@@ -1158,6 +1171,7 @@ __device__ __forceinline__ void join_rows(const Group& a, int pass, const float*
       factor = 0.0f;
     }
     a.p.losses[i] = loss;
+    if (a.p.losses_too != nullptr) a.p.losses_too[i] = loss;
     a.p.lse[i] = lse2 * kLn2;
     if (pass != 0) a.factor[row] = factor;
   }
@@ -1474,7 +1488,7 @@ int launch_logits(const Matrix& x, const Matrix& w, const Matrix* e, const Rows&
   const cudaLaunchConfig_t cfg = pairs_config(attr, int(PAIR ? 2 * std::min<int64_t>(total, sms / 2) : std::min<int64_t>(total, sms)), PAIR, stream);
   return int(cudaLaunchKernelEx(&cfg, kernel, maps, rows, int(tiles_m), int(total), int((x.cols + kSlabK - 1) / kSlabK)));
 }
-// The sums of few tokens; a part of them for each warp of the epilogue.
+// The sums of few tokens; a part of them for each CTA.
 constexpr int kFewTokens = 64;
 int few_ctas(int64_t classes) { return int(std::min<int64_t>((classes + kTileM - 1) / kTileM, sm_count())); }
 template <typename T, int TOKENS>
@@ -1552,7 +1566,7 @@ Plan plan(const NangilaLinearCeParams& p, int what) {
   l.pair = p.n > 128;
   const int64_t side = l.pair ? 256 : 128, half = side / 2;
   l.few = what == NANGILA_CE_LOSSES && p.n <= kFewTokens;
-  l.parts = l.few ? 4 * few_ctas(classes) : (classes + half - 1) / half;
+  l.parts = l.few ? few_ctas(classes) : (classes + half - 1) / half;
   const int64_t row_bytes = what == NANGILA_CE_LOSSES ? l.parts * 8 : l.e_stride * 2;
   const int64_t most = std::max<int64_t>(256, (what == NANGILA_CE_LOSSES ? kGroupBytes / 16 : kGroupBytes) / row_bytes / 256 * 256);
   l.groups = (p.n + most - 1) / most;

@@ -73,6 +73,7 @@ typedef struct {
   int32_t bias_dtype;      /* any of the three */
   int32_t mean;            /* u_i is divided by the count of targets that are not ignored */
   float* losses;           /* n */
+  float* losses_too;       /* n: the same once more; NULL: not wanted */
   float* lse;              /* n */
   float* loss;             /* 1: the sum of the losses, or their mean; NULL: not wanted */
   void* dx;                /* packed, of the type of x; NULL: not wanted */

@@ -297,6 +297,17 @@ def test_the_upstream_gradient_and_a_second_pass():
         check_grads(grads, want, x, w, 64, torch.bfloat16)
 
 
+def test_losses_changed_in_place():
+    x, w, t, _ = inputs(100, 64, 200)
+    up = torch.rand(100, device=DEV)
+    leaves = [v.clone().requires_grad_() for v in (x, w)]
+    losses = ops.linear_cross_entropy(*leaves, t, reduction="none")
+    losses *= 2.0
+    got = torch.autograd.grad(losses, leaves, up)
+    for a, b in zip(got, run(x, w, t, None, 2.0 * up, reduction="none")[1]):
+        assert torch.equal(a, b)
+
+
 def test_captured_passes_replayed_on_other_inputs():
     x, w, t, _ = inputs(400, 128, 700)
     leaves = [v.clone().requires_grad_() for v in (x, w)]
