@@ -198,10 +198,16 @@ struct Ring {
 };
 
 // TMA of a tile's slabs: both CTAs of a pair, each its own halves; the bytes are counted where the products are issued. By a whole warp. False when a wait has run out.
-template <bool PAIR>
-__device__ __forceinline__ bool load_tile(const Shared& s, const CUtensorMap* a_map, const CUtensorMap* b_map, bool a_mn, bool b_mn, const TileAt& at, uint32_t rank, int slab0, int slabs, Ring& ring) {
+// before(k) comes before slab k's wait.
+template <bool PAIR, typename Before>
+__device__ __forceinline__ bool load_tile(const Shared& s, const CUtensorMap* a_map, const CUtensorMap* b_map, bool a_mn, bool b_mn, const TileAt& at, uint32_t rank, int slab0, int slabs, Ring& ring,
+                                          const Before& before) {
   const int row = at.m0 + int(rank) * kTileM, col = at.n0 + int(rank) * 128;
   for (int k = 0; k < slabs; ++k, ring.next(kStages)) {
+    if (!before(k)) {
+      *s.failed = 1;
+      return false;
+    }
     const int st = ring.stage;
     if (ring.round > 0 && !warp_wait(&s.empty[st], (ring.round - 1) & 1)) {
       *s.failed = 1;
@@ -243,8 +249,8 @@ __device__ __forceinline__ void drain_loads(const Shared& s, uint32_t rank, Ring
   }
 }
 // The products of a tile, the n-th, into its accumulator, by a whole warp. False when a wait has run out.
-template <bool PAIR, bool BF16>
-__device__ __forceinline__ bool multiply_tile(const Shared& s, uint32_t tmem, bool a_mn, bool b_mn, int slabs, int n, Ring& ring) {
+template <bool PAIR, bool BF16, typename Before>
+__device__ __forceinline__ bool multiply_tile(const Shared& s, uint32_t tmem, bool a_mn, bool b_mn, int slabs, int n, Ring& ring, const Before& before) {
   constexpr int kSide = PAIR ? 256 : 128;
   const uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | (uint32_t(kSide >> 3) << 17) | (uint32_t(kSide >> 4) << 24);
   const int acc = n & 1;
@@ -255,7 +261,7 @@ __device__ __forceinline__ bool multiply_tile(const Shared& s, uint32_t tmem, bo
   const uint64_t a0 = make_smem_desc(smem_u32(s.stages), a_mn ? 8192 : 16, 1024), b0 = make_smem_desc(smem_u32(s.stages) + kOperandBytes, b_mn ? 8192 : 16, 1024);
   const uint64_t a_step = (a_mn ? 2048 : 32) >> 4, b_step = (b_mn ? 2048 : 32) >> 4;
   for (int k = 0; k < slabs; ++k, ring.next(kStages)) {
-    if (!warp_wait(&s.full[ring.stage], ring.round & 1)) return false;
+    if (!before(k) || !warp_wait(&s.full[ring.stage], ring.round & 1)) return false;
     tc_fence_after_sync();
     if (elected()) {
       const uint64_t from = uint64_t(uint32_t(ring.stage * (kStageBytes >> 4)));  // (addresses of 18 bits: nothing is carried out of their field)
@@ -620,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_logits_kernel(const __grid_con
     for (int tile = first; tile < total; tile += step) {
       const TileAt at = tile_at(tile);
       if (skip(at)) continue;
-      if (!load_tile<PAIR>(s, &maps.a, &maps.b, false, false, at, rank, 0, slabs, ring)) break;
+      if (!load_tile<PAIR>(s, &maps.a, &maps.b, false, false, at, rank, 0, slabs, ring, [](int) { return true; })) break;
     }
     drain_loads(s, rank, ring);
   } else if (warp == 1) {
@@ -630,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_logits_kernel(const __grid_con
       bool ok = true;
       for (int tile = first; tile < total && ok; tile += step) {
         if (some && skip(tile_at(tile))) continue;
-        ok = multiply_tile<PAIR, std::is_same<T, __nv_bfloat16>::value>(s, tmem, false, false, slabs, n, ring);
+        ok = multiply_tile<PAIR, std::is_same<T, __nv_bfloat16>::value>(s, tmem, false, false, slabs, n, ring, [](int) { return true; });
         ++n;
       }
       if (!ok) drain_products<PAIR>(s);
@@ -856,22 +862,16 @@ __device__ __forceinline__ bool task_of(const Gradients& g, int i, Task& t) {
   t.at.n0 = i % r.tiles_n * 256;
   return true;
 }
-// Rank 0's copies take the pair's next tile, and tell all of its warps (both CTAs'); the one after it is asked for at the same time.
-struct Taker {
-  int ahead;  // in lane 0
-  Ring ring;
-};
-__device__ __forceinline__ bool take_task(const Shared& s, const Gradients& g, Taker& t, int& id) {
+// Rank 0's copies take the pair's next tile, and tell all of its warps (both CTAs').
+__device__ __forceinline__ bool tell_task(const Shared& s, Ring& ring, int id) {
   const int lane = threadIdx.x & 31;
-  if (t.ring.round > 0 && !warp_wait(&s.task_empty[t.ring.stage], (t.ring.round - 1) & 1)) return false;
-  id = __shfl_sync(0xffffffffu, t.ahead, 0);
+  if (ring.round > 0 && !warp_wait(&s.task_empty[ring.stage], (ring.round - 1) & 1)) return false;
   if (lane < 2) {
-    store_cluster(cluster_address(const_cast<const int*>(&s.task[t.ring.stage]), uint32_t(lane)), id);
-    mbar_arrive_at(cluster_address(&s.task_full[t.ring.stage], uint32_t(lane)));
+    store_cluster(cluster_address(const_cast<const int*>(&s.task[ring.stage]), uint32_t(lane)), id);
+    mbar_arrive_at(cluster_address(&s.task_full[ring.stage], uint32_t(lane)));
   }
-  if (lane == 0) t.ahead = atomicAdd(g.next, 1);
   __syncwarp();
-  t.ring.next(kTasks);
+  ring.next(kTasks);
   return true;
 }
 __device__ __forceinline__ bool read_task(const Shared& s, Ring& ring, int& id) {
@@ -935,27 +935,41 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gradients_kernel(const __grid_
   Task t;
   int id = 0;
   Ring tasks;
+  // The next tile is asked for, told and worked out while this one's last slabs are on their way. (Behind them, the copies began 1200 to 2500 cycles after the products could have, and those
+  // 500 later for theirs: 4096 x 768 x 50304 a tile of 64 slabs 37000 cycles, of them 33000 for products.)
   if (warp == 0) {
     Ring ring;
-    Taker taker;
-    taker.ahead = rank == 0 && lane == 0 ? atomicAdd(g.next, 1) : 0;
-    for (;;) {
-      if (!(rank == 0 ? take_task(s, g, taker, id) : read_task(s, tasks, id))) {
-        *s.failed = 1;
-        break;
-      }
-      if (!task_of(g, id, t)) break;
-      if (!load_tile<true>(s, t.x ? &maps.e_rows : &maps.e_columns, t.x ? &maps.w : &maps.xs, !t.x, true, t.at, rank, t.slab0, t.slabs, ring)) break;
+    int ahead = 0;  // in lane 0
+    bool ok = true;
+    if (rank == 0) {
+      if (lane == 0) ahead = atomicAdd(g.next, 1);
+      id = __shfl_sync(0xffffffffu, ahead, 0);
+      ok = tell_task(s, tasks, id);
+    } else {
+      ok = read_task(s, tasks, id);
     }
+    while (ok && task_of(g, id, t)) {
+      const Task now = t;
+      const int ask = max(0, now.slabs - 14), tell = rank == 0 ? max(0, now.slabs - 7) : max(0, now.slabs - 3);
+      ok = load_tile<true>(s, now.x ? &maps.e_rows : &maps.e_columns, now.x ? &maps.w : &maps.xs, !now.x, true, now.at, rank, now.slab0, now.slabs, ring, [&](int k) {
+        if (rank == 0) {
+          if (k == ask && lane == 0) ahead = atomicAdd(g.next, 1);
+          if (k != tell) return true;
+          id = __shfl_sync(0xffffffffu, ahead, 0);
+          return tell_task(s, tasks, id);
+        }
+        return k != tell || read_task(s, tasks, id);
+      });
+    }
+    if (!ok) *s.failed = 1;
     drain_loads(s, rank, ring);
   } else if (warp == 1) {
     if (rank == 0) {
       Ring ring;
-      bool ok = true;
-      for (int k = 0; ok; ++k) {
-        ok = read_task(s, tasks, id);
-        if (!ok || !task_of(g, id, t)) break;
-        ok = multiply_tile<true, std::is_same<T, __nv_bfloat16>::value>(s, tmem, !t.x, true, t.slabs, k, ring);
+      bool ok = read_task(s, tasks, id);
+      for (int k = 0; ok && task_of(g, id, t); ++k) {
+        const Task now = t;
+        ok = multiply_tile<true, std::is_same<T, __nv_bfloat16>::value>(s, tmem, !now.x, true, now.slabs, k, ring, [&](int slab) { return slab + 1 != now.slabs || read_task(s, tasks, id); });
       }
       if (!ok) drain_products<true>(s);
     }
