@@ -88,7 +88,8 @@ template <int N>
 __device__ __forceinline__ void copies_wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // A thread's blocks are on their way through shared memory, four of them (in fp32 three) at a time: with 32 warps an SM, 64 KB (and as much of the residual). In registers, one or two at a time, the
-// loads of all SMs did not cover the way to memory: 8192 x 2048 bf16 took 19 to 21 us, floor 10. The numbers themselves take 5 of it (twenty 32 x 32 bit products a block).
+// loads of all SMs did not cover the way to memory: 8192 x 2048 bf16 took 19 to 21 us, now 17 (4.0 TB/s; with a residual 19, 5.3 TB/s), floors 10 and 15. The numbers themselves
+// take 5 of it (twenty 32 x 32 bit products a block), comparisons and conversions keep the SMs' integer pipe 60 % busy. fp32 4099 x 1001: 8 us, floor 5.
 template <typename T>
 constexpr int kAheadOf = sizeof(T) == 4 ? 3 : 4;
 

@@ -178,9 +178,9 @@ constexpr int kSortCtas = 8;       // one cluster
 constexpr int kSortWarps = kSortCtas * kSortT / 32;
 constexpr int kMaxDigit = 10;      // bits
 constexpr int kSortSmem = ((kSortT / 32) + 1) * (4 << kMaxDigit) + 256;
-constexpr int kSumT = 256;
+constexpr int kSumT = 128;
 constexpr int kJoinT = 512;
-constexpr int kFew = 32;           // further pieces of a run that a warp adds up by itself
+constexpr int kFew = 4;            // further pieces of a run that a warp adds up by itself (65536 tokens x 1024, lookup and gradient: 119.5 us, with up to 32 122.2, with up to 256 126.3)
 constexpr int kFillT = 512;
 constexpr int kMaxPiece = 64;
 
@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(kFillT) embedding_fill_kernel(uint8_t* dw, int
   if (first < (bytes & 31)) dw[wide * 32 + first] = 0;
 }
 // Ends behind the kernel before it, which it does not wait for until then: what follows finds the work of both.
+template <int kBatch>  // of a lane's positions on their way together
 __global__ void __launch_bounds__(kSortT, 1) embedding_sort_kernel(const __grid_constant__ NangilaEmbeddingGradParams p, const __grid_constant__ Sorted s) {
   extern __shared__ uint32_t smem[];
   uint32_t* count = smem;                                       // [warp][digit]
@@ -231,7 +232,15 @@ __global__ void __launch_bounds__(kSortT, 1) embedding_sort_kernel(const __grid_
     for (int i = threadIdx.x; i < (kSortT / 32) * digits; i += kSortT) count[i] = 0;
     __syncthreads();
     uint32_t* mine = count + warp * digits;
-    for (int64_t i = from + lane; i < to; i += 32) atomicAdd(&mine[key_of(i) >> shift & uint32_t(digits - 1)], 1u);
+    for (int64_t i0 = from; i0 < to; i0 += 32 * kBatch) {
+      uint32_t k[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (i0 + 32 * j + lane < to) k[j] = key_of(i0 + 32 * j + lane);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (i0 + 32 * j + lane < to) atomicAdd(&mine[k[j] >> shift & uint32_t(digits - 1)], 1u);
+    }
     __syncthreads();
     // where each (digit, CTA, warp) begins: before it come all smaller digits, and this digit's positions of the CTAs and warps before
     const int d = threadIdx.x;
@@ -270,21 +279,31 @@ __global__ void __launch_bounds__(kSortT, 1) embedding_sort_kernel(const __grid_
       for (int w = 0; w < kSortT / 32; ++w) count[w * digits + d] += before;
     }
     __syncthreads();
-    for (int64_t i0 = from; i0 < to; i0 += 32) {
-      const int64_t i = i0 + lane;
-      const bool here = i < to;
-      const uint32_t k = here ? key_of(i) : 0u, a = here ? (pass > 0 ? __ldcg(src_at + i) : uint32_t(i)) : 0u;
-      const uint32_t digit = here ? k >> shift & uint32_t(digits - 1) : uint32_t(digits);  // (those that are not here keep to themselves)
-      const uint32_t same = __match_any_sync(0xffffffffu, digit);
-      const uint32_t order = __popc(same & ((1u << lane) - 1u));
-      uint32_t pos = 0;
-      if (here) pos = mine[digit] + order;
-      __syncwarp();
-      if (here && order == 0) mine[digit] += __popc(same);
-      __syncwarp();
-      if (here) {
-        dst_key[pos] = k;
-        dst_at[pos] = a;
+    for (int64_t i0 = from; i0 < to; i0 += 32 * kBatch) {
+      uint32_t k[kBatch], a[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int64_t i = i0 + 32 * j + lane;
+        if (i >= to) continue;
+        k[j] = key_of(i);
+        a[j] = pass > 0 ? __ldcg(src_at + i) : uint32_t(i);
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        if (i0 + 32 * j >= to) break;
+        const bool here = i0 + 32 * j + lane < to;
+        const uint32_t digit = here ? k[j] >> shift & uint32_t(digits - 1) : uint32_t(digits);  // (those that are not here keep to themselves)
+        const uint32_t same = __match_any_sync(0xffffffffu, digit);
+        const uint32_t order = __popc(same & ((1u << lane) - 1u));
+        uint32_t pos = 0;
+        if (here) pos = mine[digit] + order;
+        __syncwarp();
+        if (here && order == 0) mine[digit] += __popc(same);
+        __syncwarp();
+        if (here) {
+          dst_key[pos] = k[j];
+          dst_at[pos] = a[j];
+        }
       }
     }
     sm100::cluster_sync();  // what one CTA has written, all read in the next pass
@@ -294,8 +313,9 @@ __global__ void __launch_bounds__(kSortT, 1) embedding_sort_kernel(const __grid_
 
 // A thread takes eight adjacent columns of a piece; threadIdx.y: the piece of the CTA's. VECTOR: rows start on sixteen bytes and end with a whole eight.
 template <typename T, bool VECTOR>
-__global__ void __launch_bounds__(kSumT) embedding_sum_kernel(const __grid_constant__ NangilaEmbeddingGradParams p, const __grid_constant__ Sorted s) {
-  constexpr int kAtOnce = VECTOR || sizeof(T) == 2 ? 8 : 4;  // rows on their way together
+__global__ void __launch_bounds__(kSumT, (!VECTOR ? 512 : sizeof(T) == 4 ? 768 : 1024) / kSumT) embedding_sum_kernel(const __grid_constant__ NangilaEmbeddingGradParams p, const __grid_constant__ Sorted s) {
+  // Rows on their way together. (Eight, with half as many threads an SM: 65536 tokens x 1024, lookup and gradient, 120 us, for 114.)
+  constexpr int kAtOnce = !VECTOR && sizeof(T) == 2 ? 8 : 4;
   __shared__ uint32_t keys[kSumT / 32 * kMaxPiece], positions[kSumT / 32 * kMaxPiece];  // of the CTA's pieces
   const int piece = blockIdx.x * blockDim.y + threadIdx.y, col = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
   follow();
@@ -495,7 +515,8 @@ Sorted layout(int64_t n, int64_t rows, int32_t d, uint8_t* base, int64_t* bytes)
   s.digit = (bits + s.passes - 1) / s.passes;
   s.last = (s.passes - 1) & 1;
   s.per_warp = int(((n + kSortWarps - 1) / kSortWarps + 31) / 32 * 32);
-  // pieces: some hundreds of them if there are positions enough, and no shorter than what a thread has on its way at a time
+  // Pieces: no shorter than what a thread has on its way at a time, and longer where there are positions enough for a thousand of them. (Lookup and gradient, in pieces of 8, so, of 64:
+  // 512 tokens x 1024 26.7, 26.7, 34.9 us; 8192 x 2048 63.7, 59.4, 61.5; 65536 x 1024 142.6, 122.2, 122.2.)
   s.piece = 8;
   while (s.piece < kMaxPiece && n >= int64_t(s.piece) * 1024) s.piece *= 2;
   s.pieces = int((n + s.piece - 1) / s.piece);
@@ -511,8 +532,10 @@ template <typename T>
 int gradient(const NangilaEmbeddingGradParams& p, cudaStream_t stream) {
   int64_t bytes = 0;
   const Sorted s = layout(p.n, p.rows, p.d, static_cast<uint8_t*>(p.workspace), &bytes);
+  // (One position of a lane at a time is less to fetch of the kernel itself: 8192 tokens 13 us, in batches of eight 15.7; 65536 x 1024, lookup and gradient, 114 and 112.8.)
+  auto* sort = s.per_warp <= 64 ? embedding_sort_kernel<1> : embedding_sort_kernel<8>;
   int resident = 0;
-  if (const cudaError_t e = resident_ctas(reinterpret_cast<const void*>(embedding_sort_kernel), kSortT, kSortSmem, &resident)) return int(e);
+  if (const cudaError_t e = resident_ctas(reinterpret_cast<const void*>(sort), kSortT, kSortSmem, &resident)) return int(e);
   const int64_t size = p.rows * p.d * int64_t(sizeof(T));
   embedding_fill_kernel<<<unsigned(std::min<int64_t>((size / 32 + kFillT) / kFillT, 2 * 148)), kFillT, 0, stream>>>(static_cast<uint8_t*>(p.dw), size);
   if (const cudaError_t e = cudaGetLastError()) return int(e);
@@ -529,7 +552,7 @@ int gradient(const NangilaEmbeddingGradParams& p, cudaStream_t stream) {
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  if (const cudaError_t e = cudaLaunchKernelEx(&cfg, embedding_sort_kernel, p, s)) return int(e);
+  if (const cudaError_t e = cudaLaunchKernelEx(&cfg, sort, p, s)) return int(e);
   const bool vector = p.d % 8 == 0 && aligned16(p.dy) && aligned16(p.dw) && p.dy_stride * int64_t(sizeof(T)) % 16 == 0;
   const int threads = (p.d + 7) / 8;
   int x = 32;

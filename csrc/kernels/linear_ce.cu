@@ -843,7 +843,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few_kernel(const __grid_con
 
 // dx = E w and dw = E^T x' in one launch of pairs of CTAs. A tile of dx has all classes as its K, one of dw all tokens of the group, and there may be fewer tiles of dx than pairs: those
 // are taken first, by whoever comes for the next tile, and those of dw fill up what is left, so that all end together. dx's K is cut in parts where a
-// single tile would take longer than that. (Shared out beforehand by their slabs, the first pairs were done 90 us before the last of 440: 4096 x 768 x 50304.)
+// single tile would take longer than that. (Shared out beforehand by their slabs, 4096 x 768 x 50304 took 417 to 428 us, for 407 to 414.)
 struct Task {
   bool x;
   TileAt at;
@@ -1502,7 +1502,8 @@ int launch_logits(const Matrix& x, const Matrix& w, const Matrix* e, const Rows&
   const cudaLaunchConfig_t cfg = pairs_config(attr, int(PAIR ? 2 * std::min<int64_t>(total, sms / 2) : std::min<int64_t>(total, sms)), PAIR, stream);
   return int(cudaLaunchKernelEx(&cfg, kernel, maps, rows, int(tiles_m), int(total), int((x.cols + kSlabK - 1) / kSlabK)));
 }
-// The sums of few tokens; a part of them for each CTA.
+// The sums of few tokens; a part of them for each CTA. (2048 x 32000, losses alone in a captured graph: 16 tokens 30.7 us and 43.0 with tokens as rows, 64 tokens 30.8 and 32.8; above that
+// the accumulators' columns are as many as tokens' rows would be, 128 tokens 33.3.)
 constexpr int kFewTokens = 64;
 int few_ctas(int64_t classes) { return int(std::min<int64_t>((classes + kTileM - 1) / kTileM, sm_count())); }
 template <typename T, int TOKENS>
@@ -1540,8 +1541,8 @@ Result result(int64_t M, int64_t N, int64_t K, int split) {
   r.total = r.per * r.split;
   return r;
 }
-// Into how many parts dx's K is cut: as few as let a pair's tiles of dx end before its share of all work does. (With dw not wanted: before the tiles of the
-// busiest pair would take a tenth longer than its share.)
+// Into how many parts dx's K is cut: as few as let a pair's tiles of dx end before its share of all work does. (Loss and gradients of n tokens at 2048 x 32000: n = 128 in one part 258 us,
+// in four 166, in more 175; n = 1229 in one 410, in two 406, in four 430.)
 int split_of(int64_t n, int64_t d, int64_t classes, int64_t rows, bool dw) {
   const int pairs = sm_count() / 2;
   const Result w = result(rows, d, n, 1);
@@ -1550,11 +1551,11 @@ int split_of(int64_t n, int64_t d, int64_t classes, int64_t rows, bool dw) {
   for (int split = 1; split <= 16; ++split) {
     const Result x = result(n, d, classes, split);
     if (split > 1 && x.slabs < 8) break;
-    const double share = (double(x.per) * ((x.K + kSlabK - 1) / kSlabK) + (dw ? double(w.total) * w.slabs : 0.0)) / pairs;
+    // (a tile of dw takes as long as eight slabs at least, what its results take; sums of a part go through memory: some three slabs' time a tile)
+    const double share = (double(x.per) * ((x.K + kSlabK - 1) / kSlabK) + (dw ? double(w.total) * std::max(w.slabs, 8) : 0.0)) / pairs;
     const double busiest = double((x.total + pairs - 1) / pairs) * x.slabs;
-    // (sums of a part go through memory: some three slabs' time a tile)
     const double cost = std::max(share, busiest) + (split > 1 ? 3.0 * x.total / pairs : 0.0);
-    if (cost < least * 0.97) least = cost, best = x.split;
+    if (cost < least * 0.99) least = cost, best = x.split;
   }
   return best;
 }
@@ -1576,7 +1577,7 @@ Plan plan(const NangilaLinearCeParams& p, int what) {
   std::memset(&l, 0, sizeof l);
   const int64_t classes = p.classes;
   l.e_stride = (classes + 63) / 64 * 64;
-  // Tokens enough for the rows of one small tile take small tiles.
+  // Tokens that one small tile has rows for take small tiles. (Loss and gradients at 2048 x 32000: 128 tokens 175 us, in pairs' tiles 179; 200 tokens 197, and 187.)
   l.pair = p.n > 128;
   const int64_t side = l.pair ? 256 : 128, half = side / 2;
   l.few = what == NANGILA_CE_LOSSES && p.n <= kFewTokens;
