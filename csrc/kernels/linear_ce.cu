@@ -998,7 +998,7 @@ constexpr int kRowsT = 1024;
 constexpr int kRowsAtOnce = 32;   // rows of a CTA, one for each lane, and one for each warp
 constexpr int kWeightsT = 256;
 
-// Of the whole call. alpha: what G's rows are multiplied by in the end; unit: the largest weight of a row, by which the weights are divided.
+// Of the whole call. alpha: what G's rows are multiplied by in the end; unit: the largest finite weight of a row, by which the weights are divided (1 where all are 0).
 struct Scales {
   float alpha, unit;
 };
@@ -1061,30 +1061,27 @@ __global__ void __launch_bounds__(kBeginT) ce_begin_kernel(const __grid_constant
       for (int64_t i = threadIdx.x; i < a.groups; i += kBeginT) a.next[i] = 0;
     int64_t count = 0;
     float top = 0.0f;
-    bool bad = false;
     for (int64_t i = threadIdx.x; i < p.n; i += kBeginT) {
       const int64_t t = p.targets[i];
       count += t != p.ignore ? 1 : 0;
       if (p.upstream_rows && t >= 0 && t < p.classes && t != p.ignore) {
         const float u = fabsf(p.upstream[i]);
-        bad = bad || !(u <= 3.0e38f);
-        top = fmaxf(top, u);
+        if (u < INFINITY) top = fmaxf(top, u);  // (the others' rows alone are not finite: row_weight)
       }
     }
-    if (bad) top = __uint_as_float(0x7fc00000u);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
       count += __shfl_xor_sync(0xffffffffu, count, off);
-      const float other = __shfl_xor_sync(0xffffffffu, top, off);
-      top = !(top >= other) ? (isnan(top) ? top : other) : top;
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
     }
     if (lane == 0) counts[warp] = count, tops[warp] = top;
     __syncthreads();
     if (threadIdx.x == 0) {
       for (int w = 1; w < kBeginT / 32; ++w) {
         count += counts[w];
-        top = !(top >= tops[w]) ? (isnan(top) ? top : tops[w]) : top;
+        top = fmaxf(top, tops[w]);
       }
+      if (top == 0.0f) top = 1.0f;
       float u = 1.0f;
       if (a.what == NANGILA_CE_GRADIENTS) u = p.upstream_rows ? top : *p.upstream;
       if (p.mean) u = count > 0 ? u / float(count) : 0.0f;
@@ -1245,8 +1242,9 @@ __device__ __forceinline__ RowWeight row_weight(const Group& a, int64_t i) {
   const int64_t t = a.p.targets[i];
   RowWeight w{1.0f, 0, t != a.p.ignore && t >= 0 && t < a.p.classes};
   if (a.p.upstream_rows) {
-    const float unit = a.scales->unit;
-    w.share = frexpf(unit > 0.0f ? a.p.upstream[i] / unit : unit, &w.power);
+    const float ratio = a.p.upstream[i] / a.scales->unit;
+    // one that is not finite makes its row's share that, and touches no other row of dx
+    w.share = isfinite(ratio) ? frexpf(ratio, &w.power) : __uint_as_float(0x7fc00000u);
   }
   if (!w.lives) w.share = 0.0f;
   return w;

@@ -244,6 +244,27 @@ def test_values_that_are_not_finite_are_told():
     assert bool(loss.isnan()) and bool(grads[0][17].isnan().all()) and int(grads[0].isnan().any(1).sum()) == 1 and bool(grads[1].isnan().any())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_an_upstream_gradient_that_is_not_finite_stays_in_its_row(dtype, bad):
+    x, w, t, b = inputs(300, 64, 500, dtype, bias=torch.float32)
+    t[::3] = -100
+    up = torch.rand(300, device=DEV) + 0.5
+    _, clean = run(x, w, t, b, up, reduction="none")
+    up[::3] = bad
+    _, grads = run(x, w, t, b, up, reduction="none")
+    assert all(torch.equal(got, want) for got, want in zip(grads, clean))
+    up[100] = bad
+    _, grads = run(x, w, t, b, up, reduction="none")
+    assert int((~grads[0].isfinite()).any(1).sum()) == 1 and not grads[0][100].isfinite().any()
+    others, hs = torch.arange(300, device=DEV) != 100, half_step(dtype)
+    want = head(x, w, t, b, reduction="none", upstream=torch.where(others & (t != -100), up, 0.0))
+    small = 2.0 ** -39 * want["u_size"] * w.double().abs().sum(0) if dtype == torch.float16 else 0.0
+    tol = want["dx_size"] * (hs * (1 + 2 * hs) + exp_error(want, 64, 500) + (500 / 16 + 17) * 2.0 ** -22 + 8 * U) + small + rounding(want["dx"], dtype) * 1.01
+    assert bool(((grads[0].double() - want["dx"]).abs() <= tol)[others].all())
+    assert not grads[1].isfinite().any() and not grads[2].isfinite().any()
+
+
 def test_shapes_strides_and_types():
     x, w, t, _ = inputs(120, 64, 90)
     want, grads = run(x, w, t)
