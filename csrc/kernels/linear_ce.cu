@@ -1394,6 +1394,8 @@ __global__ void __launch_bounds__(kFinishT) ce_finish_kernel(const __grid_consta
   }
   total_loss(a);
 }
+// (What is zero stays so: rows that add nothing get nothing from a factor that is not finite either.)
+__device__ __forceinline__ float rescaled(float v, float f) { return v == 0.0f ? v : v * f; }
 template <typename T>
 __device__ void rescale(T* a, int64_t n, float f) {
   const int64_t thread = int64_t(blockIdx.x) * blockDim.x + threadIdx.x, threads = int64_t(gridDim.x) * blockDim.x;
@@ -1404,11 +1406,11 @@ __device__ void rescale(T* a, int64_t n, float f) {
     float v[8];
     dev::unpack(raw, v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] *= f;
+    for (int k = 0; k < 8; ++k) v[k] = rescaled(v[k], f);
     dev::pack(v, raw);
     dev::put(a + i * 8, raw);
   }
-  for (int64_t i = whole * 8 + thread; i < n; i += threads) a[i] = dev::Vec16<T>::from_float(dev::Vec16<T>::to_float(a[i]) * f);
+  for (int64_t i = whole * 8 + thread; i < n; i += threads) a[i] = dev::Vec16<T>::from_float(rescaled(dev::Vec16<T>::to_float(a[i]), f));
 }
 __global__ void __launch_bounds__(256) rescale_kernel(const __grid_constant__ NangilaRescaleParams p) {
   const float f = *p.factor;

@@ -265,6 +265,17 @@ def test_an_upstream_gradient_that_is_not_finite_stays_in_its_row(dtype, bad):
     assert not grads[1].isfinite().any() and not grads[2].isfinite().any()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_ignored_rows_get_nothing_from_an_upstream_gradient_that_is_not_finite(dtype, bad):
+    x, w, t, _ = inputs(300, 64, 500, dtype)
+    t[::3] = -100
+    for reduction in ("mean", "sum"):
+        _, (dx, dw) = run(x, w, t, None, torch.tensor(bad, device=DEV), reduction=reduction)
+        live = t != -100
+        assert not dx[~live].any() and not dx[live].isfinite().any(1).any() and not dw.isfinite().any(1).all()
+
+
 def test_shapes_strides_and_types():
     x, w, t, _ = inputs(120, 64, 90)
     want, grads = run(x, w, t)
