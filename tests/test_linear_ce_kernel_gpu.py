@@ -276,6 +276,29 @@ def test_ignored_rows_get_nothing_from_an_upstream_gradient_that_is_not_finite(d
         assert not dx[~live].any() and not dx[live].isfinite().any(1).any() and not dw.isfinite().any(1).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+@pytest.mark.parametrize("n", [5, 150])
+def test_targets_closed_by_a_bias_of_minus_infinity(dtype, reduction, n):
+    # an infinite loss; its gradient is the softmax of the open classes, minus one at the target
+    x, w, t, b = inputs(n, 64, 300, dtype, bias=torch.float32)
+    t = t % 100
+    t[::4] = 200
+    b[100:] = -float("inf")
+    losses = ops.linear_cross_entropy(x, w, t, bias=b, reduction="none")
+    closed = torch.arange(n, device=DEV) % 4 == 0
+    assert bool((losses[closed] == float("inf")).all())
+    leaves = [v.double().requires_grad_() for v in (x, w, b)]
+    probabilities = torch.softmax(leaves[0].detach() @ leaves[1].detach().T + leaves[2].detach(), 1)
+    g = probabilities - torch.nn.functional.one_hot(t, 300)
+    want = dict(head(x, w, t % 100, torch.where(b.isinf(), 0.0, b), reduction="sum"))
+    want["dx"], want["dw"], want["db"] = g @ w.double(), g.T @ x.double(), g.sum(0)
+    want["dx_size"], want["dw_size"], want["db_size"] = g.abs() @ w.double().abs(), g.abs().T @ x.double().abs(), g.abs().sum(0)
+    loss, grads = run(x, w, t, b, torch.ones(n, device=DEV) if reduction == "none" else None, reduction=reduction)
+    assert torch.equal(loss.isinf(), closed) if reduction == "none" else bool(loss.isinf())
+    check_grads(grads, want, x, w, 64, dtype)
+
+
 def test_shapes_strides_and_types():
     x, w, t, _ = inputs(120, 64, 90)
     want, grads = run(x, w, t)
