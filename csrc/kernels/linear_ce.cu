@@ -84,6 +84,7 @@ struct Result {
   int split, slabs, per; // per: tiles of a part
   int wide;             // 0: alpha f_row D in 16 bits; 1: D in fp32; 2: added to what is there
   const float* factor;  // of D's rows; NULL: one
+  int live;             // rows from here on get zeros (`wide` 0)
 };
 // Columns of E, each row times its factor, added up: 256 columns and a share of the rows a warp, the shares' sums one behind the other.
 struct Columns {
@@ -515,9 +516,10 @@ __device__ __forceinline__ void finish_result(const Shared& s, uint32_t tmem, co
   bool dead = false;  // a row that adds nothing gets nothing either, whatever the rest holds
   if (r.wide == 0) {
     scale = *alpha_at;
+    dead = row >= r.live;
     if (r.factor != nullptr && mine && row < r.M) {
       const float f = r.factor[row];
-      dead = f == 0.0f;
+      dead = dead || f == 0.0f;
       scale *= f;
     }
   }
@@ -1290,10 +1292,10 @@ struct Finish {
   void* dx;
   int64_t dx_part, dx_count;    // values of a part, eights of dx
   int parts, per, dx_ctas;      // eights of a row
-  // dw = alpha sums
+  // dw = alpha sums, zero behind the classes
   const float* dw_sums;
   void* dw;
-  int64_t dw_count;             // eights
+  int64_t dw_count, dw_live;    // eights; of them the classes'
   int dw_ctas;
   // the bias's gradient out of the shares' sums of all groups
   const float* columns;
@@ -1370,7 +1372,7 @@ __global__ void __launch_bounds__(kFinishT) ce_finish_kernel(const __grid_consta
       float v[8];
       dev::unpack(in, v);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= alpha;
+      for (int k = 0; k < 8; ++k) v[k] = i < a.dw_live ? v[k] * alpha : 0.0f;
       dev::Raw8<T> r;
       dev::pack(v, r);
       dev::put(static_cast<T*>(a.dw) + i * 8, r);
@@ -1717,6 +1719,7 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
                 make_map(&maps.out_w, x, 64, 32);  // (those that are not wanted are not used)
       if (p.dx != nullptr) {
         q.x = result(a.n, p.d, p.classes, l.split);
+        q.x.live = a.n;
         q.x.factor = a.factor;
         q.x.wide = q.x.split > 1 ? 1 : 0;
         const Matrix out{static_cast<T*>(p.dx) + a.row0 * p.d, a.n, p.d, p.d, type}, parts{ws + l.at_dx, a.n, p.d, p.d, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, q.x.split};
@@ -1724,6 +1727,7 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
       }
       if (p.dw != nullptr) {
         q.w = result(p.rows, p.d, a.n, 1);
+        q.w.live = p.classes;  // (zeros of E times what is not finite would not be zero)
         q.w.wide = !l.wide ? 0 : g == 0 ? 1 : 2;
         const Matrix xs{a.xs, a.n, p.d, p.d, type}, out{p.dw, p.rows, p.d, p.d, type}, wide{sums, p.rows, p.d, p.d, CU_TENSOR_MAP_DATA_TYPE_FLOAT32};
         ok = ok && make_map(&maps.xs, xs, 64, 64) && (l.wide ? make_map(&maps.out_w, wide, 32, 32) : make_map(&maps.out_w, out, 64, 32));
@@ -1755,6 +1759,7 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
           f.dw_sums = sums;
           f.dw = p.dw;
           f.dw_count = int64_t(p.rows) * p.d / 8;
+          f.dw_live = int64_t(p.classes) * p.d / 8;
           f.dw_ctas = ctas_of(f.dw_count);
         }
         if (last && p.dbias != nullptr) {

@@ -299,6 +299,22 @@ def test_targets_closed_by_a_bias_of_minus_infinity(dtype, reduction, n):
     check_grads(grads, want, x, w, 64, dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+@pytest.mark.parametrize("n,rows", [(300, 500), (300, 33000), (40000, 16100)])
+def test_padding_gets_zeros_whatever_the_rest_holds(dtype, reduction, n, rows):
+    # (the last in more than one group of tokens, whose sums are joined)
+    x, w, t, b = inputs(n, 16, rows, dtype, classes=rows - 100, bias=torch.float32)
+    x[17, 3] = float("nan")
+    w[rows - 50] = float("nan")
+    up = torch.full((n,) if reduction == "none" else (), float("inf"), device=DEV)
+    _, (dx, dw, db) = run(x, w, t, b, up, reduction=reduction, num_classes=rows - 100)
+    assert not dw[rows - 100:].any() and not db[rows - 100:].any() and not dw[:rows - 100].isfinite().any(1).any()
+    x[17, 3] = 0.0
+    _, (dx, dw, db) = run(x, w, t, b, torch.ones_like(up), reduction=reduction, num_classes=rows - 100)
+    assert bool(dx.isfinite().all() and dw.isfinite().all()) and not dw[rows - 100:].any() and not db[rows - 100:].any()
+
+
 def test_shapes_strides_and_types():
     x, w, t, _ = inputs(120, 64, 90)
     want, grads = run(x, w, t)
