@@ -432,8 +432,10 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
   TORCH_CHECK_VALUE(classes >= 1 && classes <= weight.size(0), "nangila: num_classes must be 1 to ", weight.size(0), " (the rows of weight), got ", classes);
   TORCH_CHECK_VALUE(reduction >= kNone && reduction <= kSum, "nangila: unknown reduction");
   if (x.is_cpu()) {
-    const Tensor z = at::linear(x.to(at::kFloat), weight.to(at::kFloat), bias.defined() ? bias.to(at::kFloat) : bias).narrow(-1, 0, classes);
+    // (rows that add nothing and the padding stay out of the products: what they hold would come back as 0 times that)
     const Tensor t = targets.to(at::kLong), ignored = t == ignore, outside = (t < 0).logical_or(t >= classes).logical_and(ignored.logical_not());
+    const Tensor rows = x.to(at::kFloat).masked_fill(ignored.logical_or(outside).unsqueeze(-1), 0.0);
+    const Tensor z = at::linear(rows, weight.narrow(0, 0, classes).to(at::kFloat), bias.defined() ? bias.narrow(0, 0, classes).to(at::kFloat) : bias);
     const Tensor zt = z.gather(-1, t.clamp(0, classes - 1).unsqueeze(-1)).squeeze(-1);
     Tensor losses = at::where(ignored, at::zeros({}, z.options()), z.logsumexp(-1) - zt);
     losses = at::where(outside, at::full({}, NAN, z.options()), losses);

@@ -66,6 +66,26 @@ def test_linear_cross_entropy(reduction):
     assert bool(ops.linear_cross_entropy(x, w, torch.full_like(t, 30), reduction="none").isnan().all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_rows_that_add_nothing_hold_anything(reduction, dtype):
+    g = torch.Generator().manual_seed(1)
+    x, w = torch.randn(9, 8, generator=g).to(dtype), torch.randn(12, 8, generator=g).to(dtype)
+    t = torch.randint(0, 10, (9,), generator=g)
+    t[::3] = -100
+    t[1] = 10  # no class
+    results = []
+    for row, other, padding in ((0.0, 0.0, 0.0), (float("nan"), float("inf"), float("nan"))):
+        x[::3], x[1], w[10:] = row, other, padding
+        leaves = [v.clone().requires_grad_() for v in (x, w)]
+        loss = ops.linear_cross_entropy(*leaves, t, num_classes=10, reduction=reduction)
+        results.append((loss, *torch.autograd.grad(loss, leaves, torch.ones_like(loss))))
+    for clean, dirty in zip(*results):
+        assert torch.equal(clean.nan_to_num(7.0), dirty.nan_to_num(7.0))
+    _, dx, dw = results[1]
+    assert bool(dx.isfinite().all() and dw.isfinite().all()) and not dx[::3].any() and not dx[1].any() and not dw[10:].any()
+
+
 def test_refusals():
     x, w, t = torch.randn(3, 8), torch.randn(5, 8), torch.tensor([0, 1, 2])
     ids = torch.tensor([1, 2])
