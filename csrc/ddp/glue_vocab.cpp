@@ -432,6 +432,7 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
   TORCH_CHECK_VALUE(classes >= 1 && classes <= weight.size(0), "nangila: num_classes must be 1 to ", weight.size(0), " (the rows of weight), got ", classes);
   TORCH_CHECK_VALUE(reduction >= kNone && reduction <= kSum, "nangila: unknown reduction");
   if (x.is_cpu()) {
+    c10::impl::ExcludeDispatchKeyGuard in_float(c10::autocast_dispatch_keyset);  // (autocast would form the logits in 16 bits)
     // (rows that add nothing and the padding stay out of the products: what they hold would come back as 0 times that)
     const Tensor t = targets.to(at::kLong), ignored = t == ignore, outside = (t < 0).logical_or(t >= classes).logical_and(ignored.logical_not());
     const Tensor rows = x.to(at::kFloat).masked_fill(ignored.logical_or(outside).unsqueeze(-1), 0.0);

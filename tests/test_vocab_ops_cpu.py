@@ -86,6 +86,20 @@ def test_rows_that_add_nothing_hold_anything(reduction, dtype):
     assert bool(dx.isfinite().all() and dw.isfinite().all()) and not dx[::3].any() and not dx[1].any() and not dw[10:].any()
 
 
+def test_autocast_on_the_cpu_leaves_float32():
+    g = torch.Generator().manual_seed(2)
+    x, w, t = torch.randn(9, 8, generator=g), torch.randn(12, 8, generator=g), torch.randint(0, 12, (9,), generator=g)
+    results = []
+    for on in (False, True):
+        leaves = [v.clone().requires_grad_() for v in (x, w)]
+        with torch.autocast("cpu", dtype=torch.bfloat16, enabled=on):
+            losses = ops.linear_cross_entropy(*leaves, t, reduction="none")
+            y = ops.embedding(t, leaves[1])
+        results.append((losses, y, *torch.autograd.grad(losses.sum() + y.sum(), leaves)))
+    for plain, cast in zip(*results):
+        assert cast.dtype == torch.float32 and torch.equal(plain, cast)
+
+
 def test_refusals():
     x, w, t = torch.randn(3, 8), torch.randn(5, 8), torch.tensor([0, 1, 2])
     ids = torch.tensor([1, 2])
