@@ -239,7 +239,7 @@ Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, const c1
   if (weight.is_cpu()) {
     const Tensor outside = (ids < 0).logical_or(ids >= weight.size(0));
     const Tensor y = at::embedding(weight.to(at::kFloat), ids.to(at::kLong).clamp(0, weight.size(0) - 1), padding) * scale;
-    return at::where(outside.unsqueeze(-1), at::full({}, NAN, y.options()), y).to(weight.scalar_type());
+    return at::where(outside.unsqueeze(-1), at::full({}, NAN, y.options()), y).to(weight.scalar_type()).contiguous();
   }
   check_unseen({&weight});
   if (!wants_grad({&weight})) return embedding_launch(ids, weight, scale);

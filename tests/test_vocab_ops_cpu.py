@@ -100,6 +100,17 @@ def test_autocast_on_the_cpu_leaves_float32():
         assert cast.dtype == torch.float32 and torch.equal(plain, cast)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_results_are_packed(dtype):
+    ids, w = torch.tensor([[0, 1, 2], [3, 3, 0]]).T, torch.arange(20.0).to(dtype).view(5, 4).T
+    for i in (ids, ids.contiguous()):
+        for table in (w, w.contiguous()):
+            y = ops.embedding(i, table)
+            assert y.is_contiguous() and torch.equal(y, w[ids])
+    for x in (w, w[:, :1].expand(4, 5)):
+        assert ops.dropout(x, 0.5, seed=3).is_contiguous() and ops.dropout(x, 0.5, seed=3, residual=w).is_contiguous()
+
+
 def test_refusals():
     x, w, t = torch.randn(3, 8), torch.randn(5, 8), torch.tensor([0, 1, 2])
     ids = torch.tensor([1, 2])
