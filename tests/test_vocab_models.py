@@ -2,6 +2,7 @@
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -180,3 +181,51 @@ def test_a_captured_training_step():
         graph.replay()
         want, dtable = run(s)
         assert torch.equal(loss, want) and torch.equal(grad, dtable)
+
+
+def _all_three(ids, table, targets, seed):
+    x = ops.dropout(ops.embedding(ids, table, scale=50.0), 0.1, seed=seed)
+    loss = ops.linear_cross_entropy(x, table, targets, num_classes=1000)
+    return loss.detach(), torch.autograd.grad(loss, table)[0]
+
+
+@pytest.mark.gpu
+def test_two_threads_at_once():
+    torch.manual_seed(0)
+    work = []
+    for i in range(2):
+        table = torch.randn(1024, 128, device="cuda").mul(0.02).to(torch.float16 if i else torch.bfloat16).requires_grad_()
+        work.append((torch.randint(0, 1000, (3, 70 + 30 * i), device="cuda"), table, torch.randint(0, 1000, (3, 70 + 30 * i), device="cuda"), 5 + i))
+    want = [_all_three(*w) for w in work]
+    torch.cuda.synchronize()
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            out = [_all_three(*work[i]) for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+        return all(torch.equal(loss, want[i][0]) and torch.equal(grad, want[i][1]) for loss, grad in out)
+
+    with ThreadPoolExecutor(2) as pool:
+        assert all(pool.map(run, range(2)))
+
+
+@pytest.mark.gpu
+def test_two_captured_graphs_replayed_at_once():
+    torch.manual_seed(0)
+    graphs, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    for i, stream in enumerate(streams):
+        table = torch.randn(1024, 128, device="cuda").mul(0.02).to(torch.bfloat16).requires_grad_()
+        inputs = (torch.randint(0, 1000, (2, 300), device="cuda"), table, torch.randint(0, 1000, (2, 300), device="cuda"), torch.tensor(7 + i, device="cuda"))
+        want = [t.clone() for t in _all_three(*inputs)]
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got = _all_three(*inputs)
+        graphs.append((graph, got, want, inputs))  # (a graph does not hold what it reads)
+    for _ in range(20):
+        for stream, (graph, *_) in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, got, want, _ in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
