@@ -1233,7 +1233,7 @@ __global__ void __launch_bounds__(kRowsT) ce_scale_kernel(const __grid_constant_
     dev::put(static_cast<T*>(a.xs) + int64_t(row0) * a.p.d + int64_t(i) * 8, raw);
   }
 }
-// A row's weight, upstream over the largest one, as share * 2^power with a share of 1/2 to 1: the share goes into E, where it is rounded with the rest, the power into the row of x and the row's
+// A row's weight, upstream over the largest one, as share * 2^power with a share above 1/2, up to 1: the share goes into E, where it is rounded with the rest, the power into the row of x and the row's
 // factor, which it does not round. So a row of little weight keeps the digits of its own gradient in fp16 too. A single upstream gradient is alpha, and its rows' weight one.
 struct RowWeight {
   float share;
@@ -1247,6 +1247,7 @@ __device__ __forceinline__ RowWeight row_weight(const Group& a, int64_t i) {
     const float ratio = a.p.upstream[i] / a.scales->unit;
     // one that is not finite makes its row's share that, and touches no other row of dx
     w.share = isfinite(ratio) ? frexpf(ratio, &w.power) : __uint_as_float(0x7fc00000u);
+    if (fabsf(w.share) == 0.5f) w.share *= 2.0f, --w.power;  // (the largest weight's row of x is not doubled: it may be near the type's largest value)
   }
   if (!w.lives) w.share = 0.0f;
   return w;

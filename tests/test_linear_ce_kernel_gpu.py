@@ -209,6 +209,19 @@ def test_weights_far_apart(dtype):
     check_grads(grads, want, x, w, d, dtype)
 
 
+def test_rows_near_half_precisions_largest_value():
+    # the row of the largest weight as it is: nothing is doubled on the way
+    n, d, rows = 40, 8, 50
+    x, w, t, _ = inputs(n, d, rows, torch.float16)
+    x, w = (60000.0 * x.float() / x.float().abs().amax(1, keepdim=True)).half(), (w.float() * 1e-4).half()
+    up = torch.full((n,), 2.0 ** -8, device=DEV)
+    want = head(x, w, t, reduction="none", upstream=up)
+    _, grads = run(x, w, t, None, up, reduction="none")
+    check_grads(grads, want, x, w, d, torch.float16)
+    _, grads = run(x, w, t, None, torch.tensor(2.0 ** -8, device=DEV), reduction="sum")
+    check_grads(grads, want, x, w, d, torch.float16)
+
+
 def test_a_model_that_is_sure():
     # losses down to 1e-23: what is left of the gradient is the sum of the others, not 1 - p
     n, d, rows = 200, 64, 300
