@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <cstdint>
 #include <cstring>
@@ -99,6 +100,7 @@ struct Gradients {
   Columns columns;
   const float* alpha;
   int* next;            // the next tile that nobody has taken
+  int w_again;          // where along dw's K the rows of E begin once more, for the rests of x'
 };
 struct GradientMaps {
   CUtensorMap e_rows, w, out_x;      // dx
@@ -199,10 +201,10 @@ struct Ring {
 };
 
 // TMA of a tile's slabs: both CTAs of a pair, each its own halves; the bytes are counted where the products are issued. By a whole warp. False when a wait has run out.
-// before(k) comes before slab k's wait.
+// before(k) comes before slab k's wait. `again`: where along K operand A begins once more.
 template <bool PAIR, typename Before>
-__device__ __forceinline__ bool load_tile(const Shared& s, const CUtensorMap* a_map, const CUtensorMap* b_map, bool a_mn, bool b_mn, const TileAt& at, uint32_t rank, int slab0, int slabs, Ring& ring,
-                                          const Before& before) {
+__device__ __forceinline__ bool load_tile(const Shared& s, const CUtensorMap* a_map, const CUtensorMap* b_map, bool a_mn, bool b_mn, const TileAt& at, uint32_t rank, int slab0, int slabs, int again,
+                                          Ring& ring, const Before& before) {
   const int row = at.m0 + int(rank) * kTileM, col = at.n0 + int(rank) * 128;
   for (int k = 0; k < slabs; ++k, ring.next(kStages)) {
     if (!before(k)) {
@@ -217,14 +219,14 @@ __device__ __forceinline__ bool load_tile(const Shared& s, const CUtensorMap* a_
     if (elected()) {
       uint8_t* a = s.stages + st * kStageBytes;
       uint8_t* b = a + kOperandBytes;
-      const int k0 = (slab0 + k) * kSlabK;
+      const int k0 = (slab0 + k) * kSlabK, a_k0 = k0 < again ? k0 : k0 - again;
       if (rank == 0) mbar_arrive_expect_tx(&s.full[st], kStageBytes * (PAIR ? 2 : 1));
       const uint32_t bar = PAIR ? rank0_address(&s.full[st]) : smem_u32(&s.full[st]);
       if (a_mn) {
-        tma_operand<PAIR>(a, a_map, row, k0, 0, bar);
-        tma_operand<PAIR>(a + 8192, a_map, row + 64, k0, 0, bar);
+        tma_operand<PAIR>(a, a_map, row, a_k0, 0, bar);
+        tma_operand<PAIR>(a + 8192, a_map, row + 64, a_k0, 0, bar);
       } else {
-        tma_operand<PAIR>(a, a_map, k0, row, 0, bar);
+        tma_operand<PAIR>(a, a_map, a_k0, row, 0, bar);
       }
       if (b_mn) {
         tma_operand<PAIR>(b, b_map, col, k0, 0, bar);
@@ -628,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_logits_kernel(const __grid_con
     for (int tile = first; tile < total; tile += step) {
       const TileAt at = tile_at(tile);
       if (skip(at)) continue;
-      if (!load_tile<PAIR>(s, &maps.a, &maps.b, false, false, at, rank, 0, slabs, ring, [](int) { return true; })) break;
+      if (!load_tile<PAIR>(s, &maps.a, &maps.b, false, false, at, rank, 0, slabs, INT_MAX, ring, [](int) { return true; })) break;
     }
     drain_loads(s, rank, ring);
   } else if (warp == 1) {
@@ -953,7 +955,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gradients_kernel(const __grid_
     while (ok && task_of(g, id, t)) {
       const Task now = t;
       const int ask = max(0, now.slabs - 14), tell = rank == 0 ? max(0, now.slabs - 7) : max(0, now.slabs - 3);
-      ok = load_tile<true>(s, now.x ? &maps.e_rows : &maps.e_columns, now.x ? &maps.w : &maps.xs, !now.x, true, now.at, rank, now.slab0, now.slabs, ring, [&](int k) {
+      ok = load_tile<true>(s, now.x ? &maps.e_rows : &maps.e_columns, now.x ? &maps.w : &maps.xs, !now.x, true, now.at, rank, now.slab0, now.slabs, now.x ? INT_MAX : g.w_again, ring, [&](int k) {
         if (rank == 0) {
           if (k == ask && lane == 0) ahead = atomicAdd(g.next, 1);
           if (k != tell) return true;
@@ -1116,10 +1118,34 @@ struct Group {
   int32_t* again;            // [groups of 32 rows]; both passes of NANGILA_CE_BOTH
   void* e;                   // [n][e_stride]
   void* xs;                  // [n][d]: rows of x as dw's product takes them
+  int rests;                 // not 0: xs has so many rows, zeros behind n, and as many again of what their rounding left over
   int64_t e_stride;
   const Scales* scales;
   float e_scale;
 };
+// Eight values of a row of x', and with rests what their rounding left over. What would round to an infinity is rounded to the largest value: the rest has the difference.
+template <typename T>
+__device__ __forceinline__ void put_scaled(const Group& a, int64_t at, float (&v)[8]) {
+  dev::Raw8<T> raw;
+  if (a.rests != 0) {
+    float left[8];
+    if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) left[k] = v[k], v[k] = isfinite(v[k]) ? fminf(fmaxf(v[k], -65504.0f), 65504.0f) : v[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) left[k] = v[k];
+    }
+    dev::pack(v, raw);
+    dev::put(static_cast<T*>(a.xs) + at, raw);
+    dev::unpack(raw, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = isfinite(v[k]) ? left[k] - v[k] : 0.0f;
+    at += int64_t(a.rests) * a.p.d;
+  }
+  dev::pack(v, raw);
+  dev::put(static_cast<T*>(a.xs) + at, raw);
+}
 // The factor with which a row's element at the target, as it was rounded, comes out as `value`; where that is too small to tell, the factor it had. (The target's element is half
 // of a row's gradient, and often all that a class gets from it: its rounding goes into the factor, where it moves each of the others by as much as
 // their own roundings do. The encoder's loss: dx 1.4 -> 1.1 times the error that the results' rounding alone has, dw 1.7 -> 1.4.)
@@ -1218,19 +1244,22 @@ __global__ void __launch_bounds__(kRowsT) ce_scale_kernel(const __grid_constant_
     __syncthreads();
   }
   if (a.xs == nullptr) return;
-  const int per = a.p.d / 8, row0 = blockIdx.x * kRowsAtOnce, rows = min(kRowsAtOnce, a.n - row0);
+  const int per = a.p.d / 8, row0 = blockIdx.x * kRowsAtOnce, last = blockIdx.x + 1 == gridDim.x, rows = last ? max(a.n, a.rests) - row0 : kRowsAtOnce;
 #pragma unroll 4
   for (int i = threadIdx.x; i < rows * per; i += kRowsT) {
     const int r = i / per, row = row0 + r;
-    const float f = a.factor[row];
-    dev::Raw8<T> raw;
-    dev::fetch(static_cast<const T*>(a.p.x) + (a.row0 + row) * a.p.x_stride + (i - r * per) * 8, raw);
+    const float f = row < a.n ? a.factor[row] : 0.0f;
     float v[8];
-    dev::unpack(raw, v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = f == 0.0f ? 0.0f : v[k] * f;
-    dev::pack(v, raw);
-    dev::put(static_cast<T*>(a.xs) + int64_t(row0) * a.p.d + int64_t(i) * 8, raw);
+    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+    if (f != 0.0f) {
+      dev::Raw8<T> raw;
+      dev::fetch(static_cast<const T*>(a.p.x) + (a.row0 + row) * a.p.x_stride + (i - r * per) * 8, raw);
+      dev::unpack(raw, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] *= f;
+    }
+    put_scaled<T>(a, int64_t(row0) * a.p.d + int64_t(i) * 8, v);
   }
 }
 // A row's weight, upstream over the largest one, as share * 2^power with a share above 1/2, up to 1: the share goes into E, where it is rounded with the rest, the power into the row of x and the row's
@@ -1257,17 +1286,40 @@ template <typename T>
 __global__ void __launch_bounds__(kWeightsT) ce_weights_kernel(const __grid_constant__ Group a) {
   follow();
   const int64_t thread = int64_t(blockIdx.x) * kWeightsT + threadIdx.x, threads = int64_t(gridDim.x) * kWeightsT;
+  auto value_of = [&](const RowWeight& w, int64_t i) { return expm1f(-a.p.losses[i]) * w.share * a.e_scale; };
+  auto factor_of = [&](const RowWeight& w, float value) {
+    return w.lives && w.share != 0.0f ? ldexpf(folded(value, dev::Vec16<T>::to_float(dev::Vec16<T>::from_float(value)), 1.0f), w.power) : 0.0f;
+  };
   for (int64_t row = thread; row < a.n; row += threads) {
     const int64_t i = a.row0 + row;
     const RowWeight w = row_weight(a, i);
     a.ref[row] = a.p.lse[i] * kLog2e;
     a.mul[row] = w.share * a.e_scale;
-    const float value = expm1f(-a.p.losses[i]) * w.share * a.e_scale;
+    const float value = value_of(w, i);
     a.value[row] = value;
-    a.factor[row] = w.lives && w.share != 0.0f ? ldexpf(folded(value, dev::Vec16<T>::to_float(dev::Vec16<T>::from_float(value)), 1.0f), w.power) : 0.0f;
+    a.factor[row] = factor_of(w, value);
   }
   if (a.xs == nullptr) return;
   const int per = a.p.d / 8;
+  if (a.rests != 0) {
+    for (int64_t i = thread; i < int64_t(a.rests) * per; i += threads) {
+      const int64_t row = i / per;
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+      const RowWeight w = row < a.n ? row_weight(a, a.row0 + row) : RowWeight{0.0f, 0, false};
+      if (w.lives) {
+        const float f = factor_of(w, value_of(w, a.row0 + row));
+        dev::Raw8<T> raw;
+        dev::fetch(static_cast<const T*>(a.p.x) + (a.row0 + row) * a.p.x_stride + (i - row * per) * 8, raw);
+        dev::unpack(raw, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= f;
+      }
+      put_scaled<T>(a, i * 8, v);
+    }
+    return;
+  }
 #pragma unroll 4
   for (int64_t i = thread; i < int64_t(a.n) * per; i += threads) {
     const int64_t row = i / per;
@@ -1569,12 +1621,17 @@ struct Plan {
   int64_t groups, e_stride, parts, shares, share;
   bool pair, few;     // tiles of the logits
   bool wide;          // dw is summed up over the groups
+  int rests;          // rows of xs with their roundings' rests behind them; 0: without
   int split;          // parts of dx's K
   int64_t at_scales, at_next, at_zt, at_bias, at_ref, at_mul, at_value, at_factor, at_again, at_parts, at_e, at_xs, at_sums, at_dx, at_columns, total;
   int64_t bias_count;
 };
 // Of E. (Each group more adds to dw in fp32: 8192 x 768 x 50304 with a quarter, a half and one gigabyte, four, two and one groups, 1780, 1660 and 1535 us.)
 constexpr int64_t kGroupBytes = int64_t(1) << 30;
+// Up to so many tokens dw's product has the rests of x' roundings too. A class's gradient is then often one token's, x times what is nearly -1: without them the rounding of x times the row's factor
+// is its largest error, 1.4 times the one that the result's rounding alone makes and up to 28 times where that one is exact, with them 1.0 to 1.3. What it costs, bf16 x 2048 x 32000 with loss and dx:
+// 16 tokens 170 -> 182 us, 128 tokens 166 -> 182, 256 tokens 185 -> 205; 512, where rounding shows less as classes have several tokens, would be 260 -> 313.
+constexpr int kRestsTokens = 256;
 Plan plan(const NangilaLinearCeParams& p, int what) {
   Plan l;
   std::memset(&l, 0, sizeof l);
@@ -1612,7 +1669,8 @@ Plan plan(const NangilaLinearCeParams& p, int what) {
   l.at_factor = take(l.group * 4);
   l.at_again = take((l.group + 31) / 32 * 4);
   l.at_e = take(l.group * l.e_stride * 2);
-  l.at_xs = take(p.dw != nullptr ? l.group * p.d * 2 : 0);
+  l.rests = p.dw != nullptr && p.n <= kRestsTokens ? int((p.n + kSlabK - 1) / kSlabK * kSlabK) : 0;
+  l.at_xs = take(p.dw != nullptr ? std::max<int64_t>(l.group, 2 * l.rests) * p.d * 2 : 0);
   l.at_sums = take(l.wide ? int64_t(p.rows) * p.d * 4 : 0);
   l.split = p.dx != nullptr ? split_of(l.group, p.d, classes, p.rows, p.dw != nullptr) : 1;
   l.at_dx = take(l.split > 1 ? l.split * l.group * p.d * 4 : 0);
@@ -1691,6 +1749,7 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
     a.e = ws + l.at_e;
     a.e_stride = l.e_stride;
     a.xs = p.dw != nullptr ? ws + l.at_xs : nullptr;
+    a.rests = l.rests;
     rows.ref = a.ref;
     const Matrix ex{a.e, a.n, p.classes, l.e_stride, type};
     if constexpr (!std::is_same<T, __half>::value) if (what == NANGILA_CE_BOTH) {
@@ -1727,10 +1786,11 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
         ok = ok && (q.x.wide ? make_map(&maps.out_x, parts, 32, 32) : make_map(&maps.out_x, out, 64, 32));
       }
       if (p.dw != nullptr) {
-        q.w = result(p.rows, p.d, a.n, 1);
+        q.w = result(p.rows, p.d, l.rests != 0 ? 2 * l.rests : a.n, 1);
+        q.w_again = l.rests != 0 ? l.rests : INT_MAX;
         q.w.live = p.classes;  // (zeros of E times what is not finite would not be zero)
         q.w.wide = !l.wide ? 0 : g == 0 ? 1 : 2;
-        const Matrix xs{a.xs, a.n, p.d, p.d, type}, out{p.dw, p.rows, p.d, p.d, type}, wide{sums, p.rows, p.d, p.d, CU_TENSOR_MAP_DATA_TYPE_FLOAT32};
+        const Matrix xs{a.xs, l.rests != 0 ? 2 * l.rests : a.n, p.d, p.d, type}, out{p.dw, p.rows, p.d, p.d, type}, wide{sums, p.rows, p.d, p.d, CU_TENSOR_MAP_DATA_TYPE_FLOAT32};
         ok = ok && make_map(&maps.xs, xs, 64, 64) && (l.wide ? make_map(&maps.out_w, wide, 32, 32) : make_map(&maps.out_w, out, 64, 32));
       }
       if (!ok) return int(cudaErrorNotSupported);

@@ -222,6 +222,29 @@ def test_rows_near_half_precisions_largest_value():
     check_grads(grads, want, x, w, d, torch.float16)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+@pytest.mark.parametrize("n,d,rows", [(1, 64, 3000), (7, 72, 2000), (64, 256, 9000), (65, 1, 300), (130, 33, 5000), (256, 512, 3001)])
+def test_classes_of_single_tokens_keep_their_digits(dtype, reduction, n, d, rows):
+    # what few tokens give to their own classes is rounded once, in the result
+    x, w, t, _ = inputs(n, d, rows, dtype, ignored=0.3)
+    t[0] = 1
+    up = torch.rand(n, device=DEV) + 0.5 if reduction == "none" else None
+    want = head(x, w, t, reduction="sum" if up is None else "none", upstream=up)
+    live = t != -100
+    u = torch.ones(n, device=DEV).double() if up is None else up.double()
+    g = torch.softmax(x.double() @ w.double().T, 1) * u[:, None]
+    own = torch.nn.functional.one_hot(t.clamp(min=0), rows).bool() & live[:, None]
+    to_others = torch.where(live[:, None] & ~own, g, 0.0)
+    to_own = torch.where(own, to_others.sum(1, keepdim=True), 0.0)
+    hs, exp, sums = half_step(dtype), exp_error(want, d, rows), (2 * n / 16 + 25) * 2.0 ** -22
+    # the others' roundings and the target's, which is folded into the row; two roundings one behind the other of x times its factor
+    tol = (to_others.T @ x.double().abs()) * (2 * hs * (1 + 2 * hs) + exp + sums) + (to_own.T @ x.double().abs()) * (2 * hs * hs + exp + sums) + rounding(want["dw"], dtype) * 1.01
+    tol = tol + (2.0 ** -39 if dtype == torch.float16 else 2.0 ** -100) * want["x_size"] + (2.0 ** -24 * want["u_size"] if dtype == torch.float16 else 0.0)
+    _, (_, dw) = run(x, w, t, None, up, reduction=reduction)
+    assert bool(((dw.double() - want["dw"]).abs() <= tol).all()), ((dw.double() - want["dw"]).abs() - tol).max()
+
+
 def test_a_model_that_is_sure():
     # losses down to 1e-23: what is left of the gradient is the sum of the others, not 1 - p
     n, d, rows = 200, 64, 300
