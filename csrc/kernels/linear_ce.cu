@@ -1249,16 +1249,12 @@ __global__ void __launch_bounds__(kRowsT) ce_scale_kernel(const __grid_constant_
   for (int i = threadIdx.x; i < rows * per; i += kRowsT) {
     const int r = i / per, row = row0 + r;
     const float f = row < a.n ? a.factor[row] : 0.0f;
+    dev::Raw8<T> raw;
+    dev::fetch(static_cast<const T*>(a.p.x) + (a.row0 + min(row, a.n - 1)) * a.p.x_stride + (i - r * per) * 8, raw);
     float v[8];
+    dev::unpack(raw, v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-    if (f != 0.0f) {
-      dev::Raw8<T> raw;
-      dev::fetch(static_cast<const T*>(a.p.x) + (a.row0 + row) * a.p.x_stride + (i - r * per) * 8, raw);
-      dev::unpack(raw, v);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= f;
-    }
+    for (int k = 0; k < 8; ++k) v[k] = f == 0.0f ? 0.0f : v[k] * f;
     put_scaled<T>(a, int64_t(row0) * a.p.d + int64_t(i) * 8, v);
   }
 }
