@@ -1592,8 +1592,8 @@ Result result(int64_t M, int64_t N, int64_t K, int split) {
   r.total = r.per * r.split;
   return r;
 }
-// Into how many parts dx's K is cut: as few as let a pair's tiles of dx end before its share of all work does. (Loss and gradients of n tokens at 2048 x 32000: n = 128 in one part 258 us,
-// in four 166, in more 175; n = 1229 in one 410, in two 406, in four 430.)
+// Into how many parts dx's K is cut: as few as let a pair's tiles of dx end before its share of all work does. (Loss and gradients of n tokens at 2048 x 32000: n = 128 in one part 257 us,
+// in two 192, in four 179, in eight 187; n = 1229 in one 440, in two 450, in four 462.)
 int split_of(int64_t n, int64_t d, int64_t classes, int64_t rows, bool dw) {
   const int pairs = sm_count() / 2;
   const Result w = result(rows, d, n, 1);
@@ -1633,7 +1633,7 @@ Plan plan(const NangilaLinearCeParams& p, int what) {
   std::memset(&l, 0, sizeof l);
   const int64_t classes = p.classes;
   l.e_stride = (classes + 63) / 64 * 64;
-  // Tokens that one small tile has rows for take small tiles. (Loss and gradients at 2048 x 32000: 128 tokens 175 us, in pairs' tiles 179; 200 tokens 197, and 187.)
+  // Tokens that one small tile has rows for take small tiles. (Loss and gradients at 2048 x 32000: 128 tokens 179 us, in pairs' tiles 178; 200 tokens 216, and 207.)
   l.pair = p.n > 128;
   const int64_t side = l.pair ? 256 : 128, half = side / 2;
   l.few = what == NANGILA_CE_LOSSES && p.n <= kFewTokens;
