@@ -1232,7 +1232,8 @@ __global__ void __launch_bounds__(kRowsT) ce_rows_kernel(const __grid_constant__
   if (pass == 0) __syncthreads();
   join_rows<T>(a, pass, logit);
 }
-// NANGILA_CE_BOTH: the rows of tiles that were formed again once more, and the rows of x times their factors, as dw's product takes them.
+// NANGILA_CE_BOTH: the rows of tiles that were formed again once more, and the rows of x times their factors, as dw's product takes them; blockIdx.y: a share of those. (Each share
+// joins the rows for itself, and writes the same.)
 template <typename T>
 __global__ void __launch_bounds__(kRowsT) ce_scale_kernel(const __grid_constant__ Group a, int tile_rows) {
   follow();
@@ -1246,7 +1247,7 @@ __global__ void __launch_bounds__(kRowsT) ce_scale_kernel(const __grid_constant_
   if (a.xs == nullptr) return;
   const int per = a.p.d / 8, row0 = blockIdx.x * kRowsAtOnce, last = blockIdx.x + 1 == gridDim.x, rows = last ? max(a.n, a.rests) - row0 : kRowsAtOnce;
 #pragma unroll 4
-  for (int i = threadIdx.x; i < rows * per; i += kRowsT) {
+  for (int i = blockIdx.y * kRowsT + threadIdx.x; i < rows * per; i += kRowsT * gridDim.y) {
     const int r = i / per, row = row0 + r;
     const float f = row < a.n ? a.factor[row] : 0.0f;
     dev::Raw8<T> raw;
@@ -1592,8 +1593,8 @@ Result result(int64_t M, int64_t N, int64_t K, int split) {
   r.total = r.per * r.split;
   return r;
 }
-// Into how many parts dx's K is cut: as few as let a pair's tiles of dx end before its share of all work does. (Loss and gradients of n tokens at 2048 x 32000: n = 128 in one part 257 us,
-// in two 192, in four 179, in eight 187; n = 1229 in one 440, in two 450, in four 462.)
+// Into how many parts dx's K is cut: as few as let a pair's tiles of dx end before its share of all work does. (Loss and gradients of n tokens at 2048 x 32000: n = 128 in one part 252 us,
+// in two 187, in four 174, in eight 182; n = 1229 in one 440, in two 452, in four 463.)
 int split_of(int64_t n, int64_t d, int64_t classes, int64_t rows, bool dw) {
   const int pairs = sm_count() / 2;
   const Result w = result(rows, d, n, 1);
@@ -1626,14 +1627,14 @@ struct Plan {
 constexpr int64_t kGroupBytes = int64_t(1) << 30;
 // Up to so many tokens dw's product has the rests of x' roundings too. A class's gradient is then often one token's, x times what is nearly -1: without them the rounding of x times the row's factor
 // is its largest error, 1.4 times the one that the result's rounding alone makes and up to 28 times where that one is exact, with them 1.0 to 1.3. What it costs, bf16 x 2048 x 32000 with loss and dx:
-// 16 tokens 170 -> 182 us, 128 tokens 166 -> 182, 256 tokens 185 -> 205; 512, where rounding shows less as classes have several tokens, would be 260 -> 313.
+// 16 tokens 166 -> 169 us, 128 tokens 165 -> 176, 256 tokens 182 -> 199; 512, where rounding shows less as classes have several tokens, would be 242 -> 286.
 constexpr int kRestsTokens = 256;
 Plan plan(const NangilaLinearCeParams& p, int what) {
   Plan l;
   std::memset(&l, 0, sizeof l);
   const int64_t classes = p.classes;
   l.e_stride = (classes + 63) / 64 * 64;
-  // Tokens that one small tile has rows for take small tiles. (Loss and gradients at 2048 x 32000: 128 tokens 179 us, in pairs' tiles 178; 200 tokens 216, and 207.)
+  // Tokens that one small tile has rows for take small tiles. (Loss and gradients at 2048 x 32000: 128 tokens 173.6 us, in pairs' tiles 174.2, losses alone 35 and 37; 200 tokens 209, and 198.)
   l.pair = p.n > 128;
   const int64_t side = l.pair ? 256 : 128, half = side / 2;
   l.few = what == NANGILA_CE_LOSSES && p.n <= kFewTokens;
@@ -1755,7 +1756,9 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
       if (e == 0) e = int(launch_following(ce_rows_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, 1));
       rows.again = a.again;
       if (e == 0) e = logits<T, kExp>(l.pair, x, w, &ex, rows, stream);
-      if (e == 0) e = int(launch_following(ce_scale_kernel<T>, dim3(row_ctas), kRowsT, 0, stream, a, tile_rows));
+      // So many shares that there are CTAs for all SMs, if rows are long enough. (16 x 2048 x 32000 4.7 us, in one share 14.)
+      const unsigned row_shares = a.xs == nullptr ? 1u : unsigned(std::max<int64_t>(1, std::min<int64_t>(2 * 148 / row_ctas, (int64_t(kRowsAtOnce) * p.d / 8 + kRowsT - 1) / kRowsT)));
+      if (e == 0) e = int(launch_following(ce_scale_kernel<T>, dim3(row_ctas, row_shares), kRowsT, 0, stream, a, tile_rows));
     }
     if (what == NANGILA_CE_GRADIENTS) {
       a.mul = reinterpret_cast<float*>(ws + l.at_mul);

@@ -192,6 +192,20 @@ def test_targets_far_below_the_largest_logit_of_few_rows(n):
     check_grads(grads, want, x, w, 64, torch.bfloat16)
 
 
+@pytest.mark.parametrize("n,d,rows", [(3, 2048, 600), (100, 1000, 5000), (300, 2056, 700)])
+def test_targets_far_below_the_largest_logit_of_wide_rows(n, d, rows):
+    x, w, t, _ = inputs(n, d, rows)
+    away = w[(t + 1) % rows].float()
+    x[1::2] = (200 * away / away.square().sum(-1, keepdim=True))[1::2].to(torch.bfloat16)
+    want = head(x, w, t)
+    assert float(want["losses"].max()) > 100
+    loss, grads = run(x, w, t)
+    assert abs(float(loss) - float(want["loss"])) <= exp_error(want, d, rows) + 8 * U * (float(want["losses"].abs().max()) + want["z_most"])
+    check_grads(grads, want, x, w, d, torch.bfloat16)
+    again, twice = run(x, w, t)
+    assert torch.equal(loss, again) and all(torch.equal(a, b) for a, b in zip(grads, twice))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_weights_far_apart(dtype):
     # each row's own gradient keeps its digits, whatever the others' weights are: row by row the same as alone, up to the roundings of E and of the result
