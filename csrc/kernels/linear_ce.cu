@@ -181,12 +181,14 @@ __device__ __forceinline__ bool elected() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
   return one != 0;
 }
-// A wait of a whole warp, with one answer for all of it.
+// A wait of a whole warp, with one answer for all of it. CLUSTER: for what the other CTA did before it arrived, too.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  auto done = [&] { return __all_sync(0xffffffffu, CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) != 0; };
+  if (done()) return true;
   const uint64_t t0 = timer_ns();
   uint32_t spins = 0;
-  while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+  while (!done()) {
     if ((++spins & 255u) == 0u && __any_sync(0xffffffffu, timer_ns() - t0 > kTimeoutNs)) return false;
   }
   return true;
@@ -866,10 +868,11 @@ __device__ __forceinline__ bool task_of(const Gradients& g, int i, Task& t) {
   t.at.n0 = i % r.tiles_n * 256;
   return true;
 }
-// Rank 0's copies take the pair's next tile, and tell all of its warps (both CTAs').
+// Rank 0's copies take the pair's next tile, and tell all of its warps (both CTAs'). A slot is written again when all have read it: they give it back with what orders their reads before
+// that, in the cluster, as the slot of the other CTA is among what is written.
 __device__ __forceinline__ bool tell_task(const Shared& s, Ring& ring, int id) {
   const int lane = threadIdx.x & 31;
-  if (ring.round > 0 && !warp_wait(&s.task_empty[ring.stage], (ring.round - 1) & 1)) return false;
+  if (ring.round > 0 && !warp_wait<true>(&s.task_empty[ring.stage], (ring.round - 1) & 1)) return false;
   if (lane < 2) {
     store_cluster(cluster_address(const_cast<const int*>(&s.task[ring.stage]), uint32_t(lane)), id);
     mbar_arrive_at(cluster_address(&s.task_full[ring.stage], uint32_t(lane)));
@@ -879,18 +882,10 @@ __device__ __forceinline__ bool tell_task(const Shared& s, Ring& ring, int id) {
   return true;
 }
 __device__ __forceinline__ bool read_task(const Shared& s, Ring& ring, int& id) {
-  uint64_t* bar = &s.task_full[ring.stage];
-  const uint32_t parity = ring.round & 1;
-  if (!__all_sync(0xffffffffu, mbar_try_wait_cluster(bar, parity))) {
-    const uint64_t t0 = timer_ns();
-    uint32_t spins = 0;
-    while (!__all_sync(0xffffffffu, mbar_try_wait_cluster(bar, parity))) {
-      if ((++spins & 255u) == 0u && __any_sync(0xffffffffu, timer_ns() - t0 > kTimeoutNs)) return false;
-    }
-  }
+  if (!warp_wait<true>(&s.task_full[ring.stage], ring.round & 1)) return false;
   id = s.task[ring.stage];
   __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive_only(rank0_address(&s.task_empty[0]) + uint32_t(ring.stage) * 8);
+  if ((threadIdx.x & 31) == 0) mbar_arrive_at(rank0_address(&s.task_empty[0]) + uint32_t(ring.stage) * 8);
   ring.next(kTasks);
   return true;
 }
