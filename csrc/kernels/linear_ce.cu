@@ -72,7 +72,7 @@ struct Rows {
   const float* bias;    // padded to whole tiles; NULL: none
   float2* parts;        // [half tiles][stride]: largest z log2(e), sum of exp
   const int32_t* again; // for each 32 rows, whether they are to be formed again; NULL: all tiles are made
-  int64_t stride;
+  int64_t stride, ignore;
   int n, classes;
 };
 struct Maps {
@@ -467,7 +467,7 @@ __device__ __forceinline__ void finish_logits(const Shared& s, uint32_t tmem, co
   const int row0 = mine_at.m0, row = row0 + lane, col0 = mine_at.n0;
   const bool mine = row0 < rows.n && col0 < rows.classes;
   LogitRow r;
-  r.dead = in.target < 0 || in.target >= rows.classes;
+  r.dead = in.target < 0 || in.target >= rows.classes || in.target == rows.ignore;  // (what is ignored may be a class)
   r.target = r.dead ? -1 : int(in.target);
   r.ref = in.ref, r.mul = in.mul, r.value = in.value;
   r.most = -INFINITY;
@@ -1726,6 +1726,7 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
     rows.bias = bias;
     rows.parts = what == NANGILA_CE_GRADIENTS ? nullptr : reinterpret_cast<float2*>(ws + l.at_parts);
     rows.stride = l.group;
+    rows.ignore = p.ignore;
     rows.n = a.n;
     rows.classes = p.classes;
     const Matrix x{static_cast<const T*>(p.x) + a.row0 * p.x_stride, a.n, p.d, p.x_stride, type}, w{p.w, p.classes, p.d, p.w_stride, type};
