@@ -295,11 +295,11 @@ void head_launch(Head& h, int what) {
 struct HeadGrads {
   Tensor dx, dw, db;  // dx and dw with padded columns
 };
-HeadGrads head_gradients(Head& h, bool want_x, bool want_w, bool want_b) {
+HeadGrads head_gradients(Head& h, bool want_x, bool want_w, bool want_b, at::ScalarType db_type) {
   HeadGrads g;
   if (want_x) g.dx = at::empty({h.n, h.d}, h.x.options());
   if (want_w) g.dw = at::empty({h.p.rows, h.d}, h.weight.options());
-  if (want_b) g.db = at::empty({h.p.rows}, h.bias.options());
+  if (want_b) g.db = at::empty({h.p.rows}, h.bias.options().dtype(db_type));
   h.p.dx = want_x ? g.dx.data_ptr() : nullptr;
   h.p.dw = want_w ? g.dw.data_ptr() : nullptr;
   h.p.dbias = want_b ? g.db.data_ptr() : nullptr;
@@ -324,7 +324,7 @@ HeadOut head_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, 
   h.p.lse = o.lse.data_ptr<float>();
   h.p.loss = reduction != kNone ? o.result.data_ptr<float>() : nullptr;
   h.p.losses_too = reduction == kNone && keep ? o.result.data_ptr<float>() : nullptr;
-  if (both) o.grads = head_gradients(h, x.requires_grad(), weight.requires_grad(), bias.defined() && bias.requires_grad());
+  if (both) o.grads = head_gradients(h, x.requires_grad(), weight.requires_grad(), bias.defined() && bias.requires_grad(), at::kFloat);
   head_launch(h, both ? NANGILA_CE_BOTH : NANGILA_CE_LOSSES);
   return o;
 }
@@ -387,7 +387,14 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
       };
       g.dx = scaled("dx", want_x);
       g.dw = scaled("dw", want_w);
-      g.db = scaled("db", want_b);
+      if (want_b) {  // (held in float32 until now: the rounding is that of the bias's type, which may have no place for what comes before the upstream gradient)
+        const Tensor wide = ctx->saved_data["db"].toTensor();
+        g.db = at::empty(wide.sizes(), bias.options());
+        r.wide = wide.data_ptr<float>();
+        r.narrow = g.db.data_ptr();
+        r.narrow_count = wide.numel();
+        r.narrow_dtype = dtype_code(g.db);
+      }
       r.factor = upstream.data_ptr<float>();
       check_launch(nangila_rescale(&r, at::cuda::getCurrentCUDAStream()), "linear_cross_entropy gradient");
       if (!keep) {
@@ -400,7 +407,7 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
       h.p.lse = lse.data_ptr<float>();
       h.p.upstream = upstream.data_ptr<float>();
       h.p.upstream_rows = reduction == kNone ? 1 : 0;
-      g = head_gradients(h, want_x, want_w, want_b);
+      g = head_gradients(h, want_x, want_w, want_b, want_b ? bias.scalar_type() : at::kFloat);
       head_launch(h, NANGILA_CE_GRADIENTS);
     }
     auto unpadded = [&](const Tensor& t) { return t.size(1) == width ? t : t.narrow(1, 0, width).contiguous(); };

@@ -1016,6 +1016,11 @@ struct Begin {
 __device__ __forceinline__ float bias_value(const void* b, int dtype, int i) {
   return dtype == NANGILA_F32 ? static_cast<const float*>(b)[i] : dtype == NANGILA_F16 ? __half2float(static_cast<const __half*>(b)[i]) : __bfloat162float(static_cast<const __nv_bfloat16*>(b)[i]);
 }
+__device__ __forceinline__ void put_bias_value(void* b, int dtype, int64_t i, float v) {
+  if (dtype == NANGILA_F32) static_cast<float*>(b)[i] = v;
+  else if (dtype == NANGILA_F16) static_cast<__half*>(b)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(b)[i] = __float2bfloat16_rn(v);
+}
 // Row i's logit at its target, by a warp; 0 where that is no class or ignored.
 template <typename T>
 __device__ __forceinline__ float target_logit(const NangilaLinearCeParams& p, int64_t i) {
@@ -1346,7 +1351,7 @@ struct Finish {
   const float* columns;
   void* dbias;
   int64_t columns_stride;
-  int shares, classes, rows, bias_dtype, bias_ctas;
+  int shares, classes, rows, dbias_dtype, bias_ctas;
   // the sum or mean of the losses
   const float* losses;
   const int64_t* targets;
@@ -1434,9 +1439,7 @@ __global__ void __launch_bounds__(kFinishT) ce_finish_kernel(const __grid_consta
       for (int s = 0; s < a.shares; ++s) sum += a.columns[s * a.columns_stride + i];
       sum *= a.scales->alpha;
     }
-    if (a.bias_dtype == NANGILA_F32) static_cast<float*>(a.dbias)[i] = sum;
-    else if (a.bias_dtype == NANGILA_F16) static_cast<__half*>(a.dbias)[i] = __float2half_rn(sum);
-    else static_cast<__nv_bfloat16*>(a.dbias)[i] = __float2bfloat16_rn(sum);
+    put_bias_value(a.dbias, a.dbias_dtype, i, sum);
     return;
   }
   total_loss(a);
@@ -1461,8 +1464,10 @@ __device__ void rescale(T* a, int64_t n, float f) {
 }
 __global__ void __launch_bounds__(256) rescale_kernel(const __grid_constant__ NangilaRescaleParams p) {
   const float f = *p.factor;
+  if (p.wide != nullptr)
+    for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < p.narrow_count; i += int64_t(gridDim.x) * blockDim.x) put_bias_value(p.narrow, p.narrow_dtype, i, rescaled(p.wide[i], f));
   if (f == 1.0f) return;
-  for (int i = 0; i < 3; ++i) {
+  for (int i = 0; i < 2; ++i) {
     if (p.array[i] == nullptr) continue;
     if (p.dtype[i] == NANGILA_F32) rescale(static_cast<float*>(p.array[i]), p.count[i], f);
     else if (p.dtype[i] == NANGILA_F16) rescale(static_cast<__half*>(p.array[i]), p.count[i], f);
@@ -1825,7 +1830,7 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
           f.shares = int(l.groups * l.shares);
           f.classes = p.classes;
           f.rows = p.rows;
-          f.bias_dtype = p.bias_dtype;
+          f.dbias_dtype = what == NANGILA_CE_BOTH ? NANGILA_F32 : p.bias_dtype;  // (rounded when the upstream gradient is known: nangila_rescale)
           f.bias_ctas = int((p.rows + kFinishT - 1) / kFinishT);
         }
         const int ctas = f.dx_ctas + f.dw_ctas + f.bias_ctas + (total ? 1 : 0);
@@ -1872,7 +1877,7 @@ extern "C" int nangila_linear_ce(const NangilaLinearCeParams* p, int what, cudaS
 
 extern "C" int nangila_rescale(const NangilaRescaleParams* p, cudaStream_t stream) {
   using namespace nangila;
-  if (!p || !p->factor) return int(cudaErrorInvalidValue);
+  if (!p || !p->factor || (p->wide && !p->narrow)) return int(cudaErrorInvalidValue);
   rescale_kernel<<<148 * 4, 256, 0, stream>>>(*p);
   return int(cudaGetLastError());
 }

@@ -78,7 +78,7 @@ typedef struct {
   float* loss;             /* 1: the sum of the losses, or their mean; NULL: not wanted */
   void* dx;                /* packed, of the type of x; NULL: not wanted */
   void* dw;                /* rows x d, packed; NULL: not wanted */
-  void* dbias;             /* rows, of the bias's type; NULL: not wanted */
+  void* dbias;             /* rows, of the bias's type, NANGILA_CE_BOTH: float32; NULL: not wanted */
   const float* upstream;   /* NANGILA_CE_GRADIENTS: 1 value, or n */
   int32_t upstream_rows;   /* whether there are n */
   void* workspace;         /* nangila_linear_ce_workspace() bytes, 256-byte aligned */
@@ -86,11 +86,16 @@ typedef struct {
 int64_t nangila_linear_ce_workspace(const NangilaLinearCeParams* p, int what);
 int nangila_linear_ce(const NangilaLinearCeParams* p, int what, cudaStream_t stream);
 
-/* The arrays (NULL: none) multiplied by *factor, rounded to their types; nothing is read or written where it is one. */
+/* The arrays (NULL: none) multiplied by *factor, rounded to their types; nothing of them is read or written where it is one. And `narrow`, the values of `wide` times
+ * *factor. */
 typedef struct {
-  void* array[3];
-  int64_t count[3];
-  int32_t dtype[3];
+  void* array[2];
+  int64_t count[2];
+  int32_t dtype[2];
+  const float* wide;       /* NULL: none */
+  void* narrow;
+  int64_t narrow_count;
+  int32_t narrow_dtype;
   const float* factor;
 } NangilaRescaleParams;
 int nangila_rescale(const NangilaRescaleParams* p, cudaStream_t stream);
