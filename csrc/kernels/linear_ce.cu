@@ -869,7 +869,8 @@ __device__ __forceinline__ bool task_of(const Gradients& g, int i, Task& t) {
   return true;
 }
 // Rank 0's copies take the pair's next tile, and tell all of its warps (both CTAs'). A slot is written again when all have read it: they give it back with what orders their reads before
-// that, in the cluster, as the slot of the other CTA is among what is written.
+// that, rank 0's warps in their CTA, rank 1's in the cluster. (The latter takes much longer: by rank 0's products and epilogue too, loss and gradients of 1229 x 1024 x 30592 took 244 us, for
+// 236. Rank 1's slots given back by a warp that does nothing else: the same.)
 __device__ __forceinline__ bool tell_task(const Shared& s, Ring& ring, int id) {
   const int lane = threadIdx.x & 31;
   if (ring.round > 0 && !warp_wait<true>(&s.task_empty[ring.stage], (ring.round - 1) & 1)) return false;
@@ -881,11 +882,14 @@ __device__ __forceinline__ bool tell_task(const Shared& s, Ring& ring, int id) {
   ring.next(kTasks);
   return true;
 }
-__device__ __forceinline__ bool read_task(const Shared& s, Ring& ring, int& id) {
+__device__ __forceinline__ bool read_task(const Shared& s, uint32_t rank, Ring& ring, int& id) {
   if (!warp_wait<true>(&s.task_full[ring.stage], ring.round & 1)) return false;
   id = s.task[ring.stage];
   __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive_at(rank0_address(&s.task_empty[0]) + uint32_t(ring.stage) * 8);
+  if ((threadIdx.x & 31) == 0) {
+    if (rank == 0) mbar_arrive(&s.task_empty[ring.stage]);
+    else mbar_arrive_at(rank0_address(&s.task_empty[ring.stage]));
+  }
   ring.next(kTasks);
   return true;
 }
@@ -945,7 +949,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gradients_kernel(const __grid_
       id = __shfl_sync(0xffffffffu, ahead, 0);
       ok = tell_task(s, tasks, id);
     } else {
-      ok = read_task(s, tasks, id);
+      ok = read_task(s, rank, tasks, id);
     }
     while (ok && task_of(g, id, t)) {
       const Task now = t;
@@ -957,7 +961,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gradients_kernel(const __grid_
           id = __shfl_sync(0xffffffffu, ahead, 0);
           return tell_task(s, tasks, id);
         }
-        return k != tell || read_task(s, tasks, id);
+        return k != tell || read_task(s, rank, tasks, id);
       });
     }
     if (!ok) *s.failed = 1;
@@ -965,10 +969,10 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gradients_kernel(const __grid_
   } else if (warp == 1) {
     if (rank == 0) {
       Ring ring;
-      bool ok = read_task(s, tasks, id);
+      bool ok = read_task(s, rank, tasks, id);
       for (int k = 0; ok && task_of(g, id, t); ++k) {
         const Task now = t;
-        ok = multiply_tile<true, std::is_same<T, __nv_bfloat16>::value>(s, tmem, !now.x, true, now.slabs, k, ring, [&](int slab) { return slab + 1 != now.slabs || read_task(s, tasks, id); });
+        ok = multiply_tile<true, std::is_same<T, __nv_bfloat16>::value>(s, tmem, !now.x, true, now.slabs, k, ring, [&](int slab) { return slab + 1 != now.slabs || read_task(s, rank, tasks, id); });
       }
       if (!ok) drain_products<true>(s);
     }
@@ -977,7 +981,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gradients_kernel(const __grid_
     if (g.columns.partial != nullptr) add_columns<T>(g.columns, int(blockIdx.x) * kEpilogueWarps + warp - 2, int(gridDim.x) * kEpilogueWarps);
     for (int k = 0;; ++k) {
       auto finish = [&](int n) { finish_result<T>(s, tmem, t.x ? g.x : g.w, g.alpha, t.x ? &maps.out_x : &maps.out_w, t.at, t.part, rank, n, used); };
-      if (!read_task(s, tasks, id)) {  // nobody knows what is missing: all of it is not a number
+      if (!read_task(s, rank, tasks, id)) {  // nobody knows what is missing: all of it is not a number
         *s.failed = 1;
         for (int i = 0; task_of(g, i, t); ++i) finish(i);
         break;
