@@ -1000,10 +1000,12 @@ constexpr int kBeginT = 256;
 constexpr int kRowsT = 1024;
 constexpr int kRowsAtOnce = 32;   // rows of a CTA, one for each lane, and one for each warp
 constexpr int kWeightsT = 256;
+constexpr int kTops = kWeightsT;  // CTAs that look at x (Begin), one for each thread of who joins them
 
-// Of the whole call. alpha: what G's rows are multiplied by in the end; unit: the largest finite weight of a row, by which the weights are divided (1 where all are 0).
+// Of the whole call. alpha: what G's rows are multiplied by in the end; unit: the largest finite weight of a row, by which the weights are divided (1 where all are 0); plain: alpha for rows of
+// x as they are.
 struct Scales {
-  float alpha, unit;
+  float alpha, unit, plain;
 };
 
 struct Begin {
@@ -1016,6 +1018,8 @@ struct Begin {
   int* next;      // [groups] of the gradients' tiles; set to 0
   int64_t groups;
   float e_scale;  // power of two by which E is larger
+  float* tops;    // [top_ctas] the largest |upstream x| of the rows that a CTA has looked at; NULL: not wanted
+  int top_ctas;
 };
 __device__ __forceinline__ float bias_value(const void* b, int dtype, int i) {
   return dtype == NANGILA_F32 ? static_cast<const float*>(b)[i] : dtype == NANGILA_F16 ? __half2float(static_cast<const __half*>(b)[i]) : __bfloat162float(static_cast<const __nv_bfloat16*>(b)[i]);
@@ -1057,7 +1061,28 @@ __device__ __forceinline__ float target_logit(const NangilaLinearCeParams& p, in
   for (int off = 16; off > 0; off >>= 1) z += __shfl_xor_sync(0xffffffffu, z, off);
   return z + (p.bias != nullptr ? bias_value(p.bias, p.bias_dtype, int(t)) : 0.0f);
 }
-// CTA 0: how many targets are not ignored, the largest weight, and the factors that follow. The others: the targets' logits, a warp for each row; the bias in fp32.
+// The largest |upstream x| of row i, by a warp; 0 where the row adds nothing or either is not finite.
+template <typename T>
+__device__ __forceinline__ float weighted_top(const NangilaLinearCeParams& p, int64_t i) {
+  const int64_t t = p.targets[i];
+  const float u = fabsf(p.upstream[i]);
+  if (t < 0 || t >= p.classes || t == p.ignore || !(u < INFINITY)) return 0.0f;
+  const T* x = static_cast<const T*>(p.x) + i * p.x_stride;
+  float top = 0.0f;
+#pragma unroll 4
+  for (int c = (threadIdx.x & 31) * 8; c < p.d; c += 256) {
+    dev::Raw8<T> raw;
+    dev::fetch(x + c, raw);
+    float v[8];
+    dev::unpack(raw, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  return top < INFINITY ? fminf(top * u, 3e38f) : 0.0f;
+}
+// CTA 0: how many targets are not ignored, the largest weight, and the factors that follow. The others: the targets' logits, a warp for each row; the bias in fp32; the largest |upstream x|.
 template <typename T>
 __global__ void __launch_bounds__(kBeginT) ce_begin_kernel(const __grid_constant__ Begin a) {
   const NangilaLinearCeParams& p = a.p;
@@ -1093,7 +1118,7 @@ __global__ void __launch_bounds__(kBeginT) ce_begin_kernel(const __grid_constant
       float u = 1.0f;
       if (a.what == NANGILA_CE_GRADIENTS) u = p.upstream_rows ? top : *p.upstream;
       if (p.mean) u = count > 0 ? u / float(count) : 0.0f;
-      a.scales->alpha = u / a.e_scale;
+      a.scales->alpha = a.scales->plain = u / a.e_scale;
       a.scales->unit = p.upstream_rows ? top : 1.0f;
     }
     return;
@@ -1101,6 +1126,17 @@ __global__ void __launch_bounds__(kBeginT) ce_begin_kernel(const __grid_constant
   const int64_t thread = int64_t(blockIdx.x - 1) * kBeginT + threadIdx.x, threads = int64_t(gridDim.x - 1) * kBeginT;
   if (p.bias != nullptr)
     for (int64_t i = thread; i < a.bias_count; i += threads) a.bias[i] = i < p.classes ? bias_value(p.bias, p.bias_dtype, int(i)) : 0.0f;
+  if (a.tops != nullptr && int(blockIdx.x) <= a.top_ctas) {
+    __shared__ float largest[kBeginT / 32];
+    float top = 0.0f;
+    for (int64_t i = thread / 32; i < p.n; i += int64_t(a.top_ctas) * (kBeginT / 32)) top = fmaxf(top, weighted_top<T>(p, i));
+    if (lane == 0) largest[warp] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < kBeginT / 32; ++w) top = fmaxf(top, largest[w]);
+      a.tops[blockIdx.x - 1] = top;
+    }
+  }
   if (a.zt == nullptr) return;
   for (int64_t i = thread / 32; i < p.n; i += threads / 32) {
     const float z = target_logit<T>(p, i);
@@ -1124,8 +1160,10 @@ struct Group {
   void* xs;                  // [n][d]: rows of x as dw's product takes them
   int rests;                 // not 0: xs has so many rows, zeros behind n, and as many again of what their rounding left over
   int64_t e_stride;
-  const Scales* scales;
+  Scales* scales;
   float e_scale;
+  const float* tops;         // as in Begin
+  int top_ctas;
 };
 // Eight values of a row of x', and with rests what their rounding left over. What would round to an infinity is rounded to the largest value: the rest has the difference.
 template <typename T>
@@ -1264,13 +1302,16 @@ __global__ void __launch_bounds__(kRowsT) ce_scale_kernel(const __grid_constant_
   }
 }
 // A row's weight, upstream over the largest one, as share * 2^power with a share above 1/2, up to 1: the share goes into E, where it is rounded with the rest, the power into the row of x and the row's
-// factor, which it does not round. So a row of little weight keeps the digits of its own gradient in fp16 too. A single upstream gradient is alpha, and its rows' weight one.
+// factor, which it does not round. A single upstream gradient is alpha, and its rows' weight one.
+// In fp16 all rows of x' are as much larger, by a power of two that alpha takes back (`lift`), as the largest |upstream x| of the call lets them be: what x' loses below 2^-24 is then at most 2^-38 of
+// that in dw, for each token and probability, and as much as the results' own subnormal steps where dw does not overflow. (As they were, a row of 2^-20 of the largest weight had four bits.) So a
+// row of little weight keeps the digits of its own gradients in fp16 too. Looking at x costs 0.7 us at 1023 x 1000 (119.9 -> 120.6, loss and gradients).
 struct RowWeight {
   float share;
   int power;
   bool lives;
 };
-__device__ __forceinline__ RowWeight row_weight(const Group& a, int64_t i) {
+__device__ __forceinline__ RowWeight row_weight(const Group& a, int64_t i, int lift) {
   const int64_t t = a.p.targets[i];
   RowWeight w{1.0f, 0, t != a.p.ignore && t >= 0 && t < a.p.classes};
   if (a.p.upstream_rows) {
@@ -1278,22 +1319,40 @@ __device__ __forceinline__ RowWeight row_weight(const Group& a, int64_t i) {
     // one that is not finite makes its row's share that, and touches no other row of dx
     w.share = isfinite(ratio) ? frexpf(ratio, &w.power) : __uint_as_float(0x7fc00000u);
     if (fabsf(w.share) == 0.5f) w.share *= 2.0f, --w.power;  // (the largest weight's row of x is not doubled: it may be near the type's largest value)
+    w.power += lift;
   }
   if (!w.lives) w.share = 0.0f;
   return w;
+}
+// |x'| stays below 2^15: |x| 2^power is below twice the largest |upstream x| over the unit. By all threads of a CTA.
+__device__ __forceinline__ int lift_of(const Group& a) {
+  if (a.tops == nullptr) return 0;
+  __shared__ float largest[kWeightsT / 32];
+  const int lane = threadIdx.x & 31;
+  float top = int(threadIdx.x) < a.top_ctas ? a.tops[threadIdx.x] : 0.0f;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  if (lane == 0) largest[threadIdx.x >> 5] = top;
+  __syncthreads();
+  for (int w = 0; w < kWeightsT / 32; ++w) top = fmaxf(top, largest[w]);
+  int power = 14;  // (all zeros, or weights so small that alpha would lose digits, where dw is zero in fp16 whatever x: as they are)
+  if (top > 0.0f && a.scales->plain > 1e-28f) frexpf(top / a.scales->unit, &power);
+  return max(0, min(30, 14 - power));
 }
 // NANGILA_CE_GRADIENTS: what the tiles' epilogue takes of each row, and the rows of x without those that add nothing.
 template <typename T>
 __global__ void __launch_bounds__(kWeightsT) ce_weights_kernel(const __grid_constant__ Group a) {
   follow();
   const int64_t thread = int64_t(blockIdx.x) * kWeightsT + threadIdx.x, threads = int64_t(gridDim.x) * kWeightsT;
+  const int lift = lift_of(a);
+  if (thread == 0 && a.tops != nullptr) a.scales->alpha = ldexpf(a.scales->plain, -lift);  // (by each group the same)
   auto value_of = [&](const RowWeight& w, int64_t i) { return expm1f(-a.p.losses[i]) * w.share * a.e_scale; };
   auto factor_of = [&](const RowWeight& w, float value) {
     return w.lives && w.share != 0.0f ? ldexpf(folded(value, dev::Vec16<T>::to_float(dev::Vec16<T>::from_float(value)), 1.0f), w.power) : 0.0f;
   };
   for (int64_t row = thread; row < a.n; row += threads) {
     const int64_t i = a.row0 + row;
-    const RowWeight w = row_weight(a, i);
+    const RowWeight w = row_weight(a, i, lift);
     a.ref[row] = a.p.lse[i] * kLog2e;
     a.mul[row] = w.share * a.e_scale;
     const float value = value_of(w, i);
@@ -1308,7 +1367,7 @@ __global__ void __launch_bounds__(kWeightsT) ce_weights_kernel(const __grid_cons
       float v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-      const RowWeight w = row < a.n ? row_weight(a, a.row0 + row) : RowWeight{0.0f, 0, false};
+      const RowWeight w = row < a.n ? row_weight(a, a.row0 + row, lift) : RowWeight{0.0f, 0, false};
       if (w.lives) {
         const float f = factor_of(w, value_of(w, a.row0 + row));
         dev::Raw8<T> raw;
@@ -1324,7 +1383,7 @@ __global__ void __launch_bounds__(kWeightsT) ce_weights_kernel(const __grid_cons
 #pragma unroll 4
   for (int64_t i = thread; i < int64_t(a.n) * per; i += threads) {
     const int64_t row = i / per;
-    const RowWeight w = row_weight(a, a.row0 + row);
+    const RowWeight w = row_weight(a, a.row0 + row, lift);
     dev::Raw8<T> raw;
     dev::fetch(static_cast<const T*>(a.p.x) + (a.row0 + row) * a.p.x_stride + (i - row * per) * 8, raw);
     if (w.power != 0) {
@@ -1624,8 +1683,9 @@ struct Plan {
   bool wide;          // dw is summed up over the groups
   int rests;          // rows of xs with their roundings' rests behind them; 0: without
   int split;          // parts of dx's K
-  int64_t at_scales, at_next, at_zt, at_bias, at_ref, at_mul, at_value, at_factor, at_again, at_parts, at_e, at_xs, at_sums, at_dx, at_columns, total;
+  int64_t at_scales, at_next, at_tops, at_zt, at_bias, at_ref, at_mul, at_value, at_factor, at_again, at_parts, at_e, at_xs, at_sums, at_dx, at_columns, total;
   int64_t bias_count;
+  int top_ctas;       // that look at x; 0: none
 };
 // Of E. (Each group more adds to dw in fp32: 8192 x 768 x 50304 with a quarter, a half and one gigabyte, four, two and one groups, 1780, 1660 and 1535 us.)
 constexpr int64_t kGroupBytes = int64_t(1) << 30;
@@ -1660,6 +1720,8 @@ Plan plan(const NangilaLinearCeParams& p, int what) {
   };
   l.at_scales = take(sizeof(Scales));
   l.at_next = take(l.groups * 4);
+  l.top_ctas = what == NANGILA_CE_GRADIENTS && p.dtype == NANGILA_F16 && p.upstream_rows && p.dw != nullptr ? int(std::min<int64_t>((p.n + kBeginT / 32 - 1) / (kBeginT / 32), kTops)) : 0;
+  l.at_tops = take(l.top_ctas * 4);
   l.at_zt = take(what == NANGILA_CE_BOTH ? p.n * 4 : 0);
   l.at_ref = take(what == NANGILA_CE_BOTH ? p.n * 4 : what == NANGILA_CE_GRADIENTS ? l.group * 4 : 0);
   l.at_bias = take(p.bias != nullptr ? l.bias_count * 4 : 0);
@@ -1701,11 +1763,13 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
   begin.scales = scales;
   begin.next = reinterpret_cast<int*>(ws + l.at_next);
   begin.groups = l.groups;
+  begin.tops = l.top_ctas != 0 ? reinterpret_cast<float*>(ws + l.at_tops) : nullptr;
+  begin.top_ctas = l.top_ctas;
   begin.e_scale = what == NANGILA_CE_GRADIENTS && std::is_same<T, __half>::value ? 32768.0f : 1.0f;
   int e = 0;
   if (what != NANGILA_CE_LOSSES || p.bias != nullptr) {
     const int64_t work = std::max<int64_t>(what == NANGILA_CE_BOTH ? (p.n + kBeginT / 32 - 1) / (kBeginT / 32) : 0, p.bias != nullptr ? (l.bias_count + kBeginT - 1) / kBeginT : 0);
-    ce_begin_kernel<T><<<unsigned(1 + std::min<int64_t>(work, 148 * 8)), kBeginT, 0, stream>>>(begin);
+    ce_begin_kernel<T><<<unsigned(1 + std::max<int64_t>(std::min<int64_t>(work, 148 * 8), l.top_ctas)), kBeginT, 0, stream>>>(begin);
     e = int(cudaGetLastError());
   }
 
@@ -1728,6 +1792,8 @@ int run(const NangilaLinearCeParams& p, int what, cudaStream_t stream) {
     a.parts_count = int(l.parts);
     a.parts = reinterpret_cast<const float2*>(ws + l.at_parts);
     a.scales = scales;
+    a.tops = begin.tops;
+    a.top_ctas = begin.top_ctas;
     a.e_scale = begin.e_scale;
     Rows rows;
     std::memset(&rows, 0, sizeof rows);
