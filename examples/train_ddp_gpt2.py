@@ -69,6 +69,7 @@ def main() -> int:
             muon.load_state_dict(ck["muon"])
         hook.load_state_dict(ck["hook"])
         start = ck["step"]
+    torch.manual_seed(4321 + rank)  # the weights are made: each rank drops other elements from here on
     gen = torch.Generator().manual_seed(1234 + rank)
     seq = min(cfg.n_ctx, 1024)
     for step in range(start, args.steps):
