@@ -5,6 +5,7 @@
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/engine.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -337,16 +338,12 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
     const bool both = reduction != kNone && x.scalar_type() == at::kBFloat16 && targets.numel() > 0;
     HeadOut o = head_forward(x, weight, bias, targets, classes, ignore, reduction, both, true);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({x, weight, bias, targets, o.losses, o.lse});
+    // (what has been formed among them: hooks on saved tensors, and checkpoints, have it in their hands)
+    ctx->save_for_backward({x, weight, bias, targets, o.losses, o.lse, o.grads.dx, o.grads.dw, o.grads.db});
     ctx->saved_data["classes"] = classes;
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["reduction"] = reduction;
     ctx->saved_data["both"] = both;
-    if (both) {
-      if (o.grads.dx.defined()) ctx->saved_data["dx"] = o.grads.dx;
-      if (o.grads.dw.defined()) ctx->saved_data["dw"] = o.grads.dw;
-      if (o.grads.db.defined()) ctx->saved_data["db"] = o.grads.db;
-    }
     return o.result;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -369,38 +366,31 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
     const Tensor upstream = in_memory(upstream_in).to(at::kFloat).contiguous();
     HeadGrads g;
     if (ctx->saved_data["both"].toBool()) {
-      // What the forward pass has formed is multiplied in place and given away; a second pass over the same graph forms it again. (A captured pass can be replayed
-      // apart from its forward pass: it leaves them as they are.)
-      const bool keep = capturing();
+      // What the forward pass has formed is multiplied in place and given away, unless it is wanted again: by another pass over the same graph, or when a captured pass is replayed.
+      const bool keep = capturing() || torch::autograd::get_current_graph_task_keep_graph();
       NangilaRescaleParams r;
       std::memset(&r, 0, sizeof r);
       int i = 0;
-      auto scaled = [&](const char* name, bool want) {
+      auto scaled = [&](const Tensor& formed, bool want) {
         if (!want) return Tensor();
-        Tensor t = ctx->saved_data[name].toTensor();
-        if (keep) t = t.clone();
+        const Tensor t = keep ? formed.clone() : formed;
         r.array[i] = t.data_ptr();
         r.count[i] = t.numel();
         r.dtype[i] = dtype_code(t);
         ++i;
         return t;
       };
-      g.dx = scaled("dx", want_x);
-      g.dw = scaled("dw", want_w);
+      g.dx = scaled(saved[6], want_x);
+      g.dw = scaled(saved[7], want_w);
       if (want_b) {  // (held in float32 until now: the rounding is that of the bias's type, which may have no place for what comes before the upstream gradient)
-        const Tensor wide = ctx->saved_data["db"].toTensor();
-        g.db = at::empty(wide.sizes(), bias.options());
-        r.wide = wide.data_ptr<float>();
+        g.db = at::empty(saved[8].sizes(), bias.options());
+        r.wide = saved[8].data_ptr<float>();
         r.narrow = g.db.data_ptr();
-        r.narrow_count = wide.numel();
+        r.narrow_count = g.db.numel();
         r.narrow_dtype = dtype_code(g.db);
       }
       r.factor = upstream.data_ptr<float>();
       check_launch(nangila_rescale(&r, at::cuda::getCurrentCUDAStream()), "linear_cross_entropy gradient");
-      if (!keep) {
-        ctx->saved_data["both"] = false;
-        for (const char* name : {"dx", "dw", "db"}) ctx->saved_data.erase(name);
-      }
     } else {
       Head h = head_of(x, weight, bias, targets, ctx->saved_data["classes"].toInt(), ctx->saved_data["ignore"].toInt(), reduction == kMean);
       h.p.losses = losses.data_ptr<float>();
