@@ -54,6 +54,12 @@ inline void once_only() {
   TORCH_CHECK(!at::GradMode::is_enabled(), "nangila: this gradient cannot be differentiated again (create_graph=True)");
 }
 
+// What comes back of a saved tensor goes through a user's hooks, if there are some, and the kernels take its memory as it is.
+inline void check_saved(bool as_it_was) { TORCH_CHECK_VALUE(as_it_was, "nangila: a hook on saved tensors gave back a tensor of another shape, type or device than it was given"); }
+inline bool saved_as(const Tensor& t, at::ScalarType type, int64_t numel, const at::Device& device) {
+  return t.defined() && t.layout() == at::kStrided && t.scalar_type() == type && t.numel() == numel && t.device() == device;
+}
+
 // The tensor with its values in memory: a view that is negated only when it is read has others there, zeros that nobody has read yet have none.
 inline Tensor in_memory(const Tensor& t) {
   if (t._is_zerotensor()) return at::zeros(t.sizes(), t.options());

@@ -110,7 +110,7 @@ class RmsNorm : public torch::autograd::Function<RmsNorm> {
     once_only();
     const variable_list saved = ctx->get_saved_variables();
     Tensor h = saved[0], weight = in_memory(saved[1]).contiguous();
-    const Tensor& rstd = saved[2];
+    const Tensor rstd = saved[2].contiguous();
     Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
     variable_list out(4);
     if (!dy.defined() && !dh.defined()) return out;
@@ -119,8 +119,11 @@ class RmsNorm : public torch::autograd::Function<RmsNorm> {
     const bool two = ctx->saved_data["residual"].toBool(), for_x = ctx->needs_input_grad(0), for_residual = two && ctx->needs_input_grad(1);
     const bool want_x = for_x || for_residual, want_w = ctx->needs_input_grad(two ? 2 : 1) && dy.defined();
     if (!want_x && !want_w) return out;
-    c10::cuda::CUDAGuard guard(h.device());
-    const int64_t d = h.size(-1), rows = h.numel() / d;
+    const int64_t d = weight.numel(), rows = rstd.numel();
+    const at::Device device = dy.defined() ? dy.device() : dh.device();
+    check_saved(known(h.scalar_type()) && saved_as(h, h.scalar_type(), rows * d, device) && known(weight.scalar_type()) && saved_as(weight, weight.scalar_type(), d, device) &&
+                saved_as(rstd, at::kFloat, rows, device) && (!dy.defined() || dy.numel() == rows * d) && (!dh.defined() || dh.numel() == rows * d) && h.dim() > 0 && h.size(-1) == d);
+    c10::cuda::CUDAGuard guard(device);
     Tensor dx, dw, partial;
     if (want_x) dx = at::empty(h.sizes(), h.options());
     if (rows == 0) {
@@ -297,6 +300,7 @@ class Rotary : public torch::autograd::Function<Rotary> {
     Tensor gq = ctx->needs_input_grad(0) ? grads[0] : Tensor(), gk = grads.size() > 1 && ctx->needs_input_grad(1) ? grads[1] : Tensor();
     if (!gq.defined() && !gk.defined()) return out;
     check_unseen({&gq, &gk});
+    check_rotary(gq.defined() ? gq : gk, gq.defined() ? gk : Tensor(), saved[0], saved[1]);  // (what a hook on saved tensors gave back)
     std::tie(out[0], out[1]) = rotary_launch(gq, gk, saved[0], saved[1], ctx->saved_data["half"].toBool(), true);
     return out;
   }

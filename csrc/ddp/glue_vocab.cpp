@@ -104,6 +104,7 @@ class Dropout : public torch::autograd::Function<Dropout> {
     check_unseen({&dy});
     const bool residual = ctx->saved_data["residual"].toBool();
     const Mask mask{ctx->saved_data["least"].toInt(), ctx->saved_data["draw"].toInt(), ctx->saved_data["seed"].toInt(), ctx->get_saved_variables()[0]};
+    check_saved(!mask.seed_tensor.defined() || saved_as(mask.seed_tensor, at::kLong, 1, dy.device()));
     if (ctx->needs_input_grad(0)) out[0] = dropout_launch(dy, Tensor(), mask);
     if (residual && ctx->needs_input_grad(1)) out[1] = dy;
     return out;
@@ -198,12 +199,14 @@ class Embedding : public torch::autograd::Function<Embedding> {
     if (!dy_in.defined() || !ctx->needs_input_grad(0)) return out;
     check_unseen({&dy_in});
     c10::cuda::CUDAGuard guard(dy_in.device());
-    const Tensor ids = in_memory(ctx->get_saved_variables()[0]).contiguous();
+    const Tensor saved = ctx->get_saved_variables()[0];
     NangilaEmbeddingGradParams p;
     std::memset(&p, 0, sizeof p);
-    p.n = ids.numel();
     p.rows = ctx->saved_data["rows"].toInt();
     p.d = int32_t(ctx->saved_data["d"].toInt());
+    p.n = dy_in.numel() / p.d;
+    check_saved(saved_as(saved, at::kLong, p.n, dy_in.device()) || saved_as(saved, at::kInt, p.n, dy_in.device()));
+    const Tensor ids = in_memory(saved).contiguous();
     if (p.n == 0) {
       out[0] = at::zeros({p.rows, p.d}, dy_in.options());
       return out;
@@ -340,6 +343,7 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
     ctx->set_materialize_grads(false);
     // (what has been formed among them: hooks on saved tensors, and checkpoints, have it in their hands)
     ctx->save_for_backward({x, weight, bias, targets, o.losses, o.lse, o.grads.dx, o.grads.dw, o.grads.db});
+    ctx->saved_data["rows"] = weight.size(0);
     ctx->saved_data["classes"] = classes;
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["reduction"] = reduction;
@@ -353,10 +357,17 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
     if (!upstream_in.defined()) return out;
     check_unseen({&upstream_in});
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &targets = saved[3], &losses = saved[4], &lse = saved[5];
+    const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &targets = saved[3];
     const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = bias.defined() && ctx->needs_input_grad(2);
     const int64_t reduction = ctx->saved_data["reduction"].toInt(), width = x.size(-1);
-    if (targets.numel() == 0) {
+    const int64_t n = targets.numel(), rows = weight.size(0), padded = (width + 7) / 8 * 8;
+    const at::ScalarType type = x.scalar_type();
+    const at::Device device = upstream_in.device();
+    check_saved((type == at::kHalf || type == at::kBFloat16) && saved_as(x, type, n * width, device) && saved_as(weight, type, rows * width, device) && weight.dim() == 2 &&
+                rows == ctx->saved_data["rows"].toInt() && (saved_as(targets, at::kLong, n, device) || saved_as(targets, at::kInt, n, device)) && saved_as(saved[4], at::kFloat, n, device) &&
+                saved_as(saved[5], at::kFloat, n, device) && upstream_in.numel() == (reduction == kNone ? n : 1) &&
+                (!bias.defined() || (known(bias.scalar_type()) && saved_as(bias, bias.scalar_type(), rows, device))));
+    if (n == 0) {
       if (want_x) out[0] = at::zeros_like(x);
       if (want_w) out[1] = at::zeros_like(weight);
       if (want_b) out[2] = at::zeros_like(bias);
@@ -371,20 +382,24 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
       NangilaRescaleParams r;
       std::memset(&r, 0, sizeof r);
       int i = 0;
+      Tensor formed_db;
       auto scaled = [&](const Tensor& formed, bool want) {
         if (!want) return Tensor();
-        const Tensor t = keep ? formed.clone() : formed;
+        const Tensor t = keep ? formed.clone(at::MemoryFormat::Contiguous) : formed.contiguous();
         r.array[i] = t.data_ptr();
         r.count[i] = t.numel();
         r.dtype[i] = dtype_code(t);
         ++i;
         return t;
       };
+      check_saved((!want_x || saved_as(saved[6], type, n * padded, device)) && (!want_w || saved_as(saved[7], type, rows * padded, device)) &&
+                  (!want_b || saved_as(saved[8], at::kFloat, rows, device)));
       g.dx = scaled(saved[6], want_x);
       g.dw = scaled(saved[7], want_w);
       if (want_b) {  // (held in float32 until now: the rounding is that of the bias's type, which may have no place for what comes before the upstream gradient)
-        g.db = at::empty(saved[8].sizes(), bias.options());
-        r.wide = saved[8].data_ptr<float>();
+        formed_db = saved[8].contiguous();
+        g.db = at::empty({rows}, bias.options());
+        r.wide = formed_db.data_ptr<float>();
         r.narrow = g.db.data_ptr();
         r.narrow_count = g.db.numel();
         r.narrow_dtype = dtype_code(g.db);
@@ -393,6 +408,7 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
       check_launch(nangila_rescale(&r, at::cuda::getCurrentCUDAStream()), "linear_cross_entropy gradient");
     } else {
       Head h = head_of(x, weight, bias, targets, ctx->saved_data["classes"].toInt(), ctx->saved_data["ignore"].toInt(), reduction == kMean);
+      const Tensor losses = saved[4].contiguous(), lse = saved[5].contiguous();
       h.p.losses = losses.data_ptr<float>();
       h.p.lse = lse.data_ptr<float>();
       h.p.upstream = upstream.data_ptr<float>();
