@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kLookupT) embedding_any_kernel(const __grid_co
 
 // ---- gradient ----------------------------------------------------------------------------------------------------
 constexpr int kSortT = 1024;
-constexpr int kSortCtas = 8;       // one cluster
+constexpr int kSortCtas = 8;       // one cluster: 13 us for 8192 positions, hidden by the zeros; of long lists of narrow rows it is the most (262144 x 64 of 32000 103 us, of 180 with the lookup)
 constexpr int kSortWarps = kSortCtas * kSortT / 32;
 constexpr int kMaxDigit = 10;      // bits
 constexpr int kSortSmem = ((kSortT / 32) + 1) * (4 << kMaxDigit) + 256;

@@ -7,7 +7,7 @@ examples train Hugging Face models through DDP (examples/train_llm.py:230-332).
 
 ``BertConfig(fused_vocab=True)`` takes the embeddings and the decoder with its loss through ``nangila.ops``: table gradients by sorted tokens, and no
 logits in memory. ``dropout`` drops, in training, from the embeddings and from each block's two outputs before they are added and normalised
-(``nangila.ops.dropout``; attention weights are not dropped).
+(``nangila.ops.dropout``; attention weights are not dropped). The masks' seeds come from PyTorch's generator: such a step cannot be captured in a graph.
 """
 from __future__ import annotations
 

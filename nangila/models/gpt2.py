@@ -11,7 +11,7 @@ cross-entropy kernel pair (``nangila/ops/fused_ce.py``); the gradient exchange i
 
 ``GPT2Config(fused_vocab=True)`` takes the embeddings and the tied head with its loss through ``nangila.ops``: table gradients by sorted tokens, and no
 logits in memory. ``dropout`` drops, in training, from the embeddings and from what each block adds to the residual stream (``nangila.ops.dropout``;
-attention weights are not dropped).
+attention weights are not dropped). The masks' seeds come from PyTorch's generator: such a step cannot be captured in a graph.
 """
 from __future__ import annotations
 

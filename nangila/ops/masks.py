@@ -19,8 +19,8 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: Union[int, torch.Tensor, None
 
     ``seed``: a number below 2^64, or one int64 on the device of ``x``, which is read when the kernel runs, forward and backward: a captured graph draws other masks
     when it is changed between replays. None: taken from PyTorch's default CPU generator (``torch.manual_seed``), not while a graph is captured.
-    ``draw``, below 2^32, tells apart masks of one seed. Data-parallel ranks need seeds of their own, or they drop the same elements. ``p`` is held in 2^-32, and the factor goes by what is held. What is dropped may be
-    infinite or not a number. Differentiable once in ``x`` and ``residual``."""
+    ``draw``, below 2^32, tells apart masks of one seed. Data-parallel ranks need seeds of their own, or they drop the same elements. ``p`` is held
+    in 2^-32, and the factor goes by what is held. What is dropped may be infinite or not a number. Differentiable once in ``x`` and ``residual``."""
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"nangila: p must be 0 to 1, got {p}")
     if not 0 <= draw < 2 ** 32:
