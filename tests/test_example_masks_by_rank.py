@@ -1,6 +1,7 @@
 """Ranks that train the same weights drop different elements: else the noise of dropout is not averaged over them."""
 import json
 import os
+import socket
 import subprocess
 import sys
 
@@ -43,8 +44,11 @@ json.dump({{"masks": made, "weights": weights}}, open(os.path.join({out!r}, "ran
 def test_masks_differ_between_ranks(tmp_path, compressor):
     path = tmp_path / "wrapped.py"
     path.write_text(WRAPPER.format(root=ROOT, out=str(tmp_path), args=["--tiny", "--steps", "4", "--warmup-steps", "2", "--micro-batch", "2", "--dropout", "0.2", "--compressor", compressor]))
+    with socket.socket() as free:
+        free.bind(("127.0.0.1", 0))
+        port = str(free.getsockname()[1])
     env = dict(os.environ, CUDA_VISIBLE_DEVICES="", OMP_NUM_THREADS="1", PYTHONHASHSEED="0")
-    r = subprocess.run([sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node", "2", "--master-addr", "127.0.0.1", "--master-port", "29596", str(path)],
+    r = subprocess.run([sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node", "2", "--master-addr", "127.0.0.1", "--master-port", port, str(path)],
                        cwd=ROOT, env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-3000:]
     a, b = (json.load(open(tmp_path / f"rank{rank}")) for rank in (0, 1))
